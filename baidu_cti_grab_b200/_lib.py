@@ -20,6 +20,7 @@ LIB_PATH = os.path.join(HERE, "librep_b200.so")
 
 RB_F32, RB_BF16, RB_F16, RB_I32, RB_I8, RB_I64 = 0, 1, 2, 3, 4, 5
 RB_ACT_DYNAMIC, RB_ACT_STATIC, RB_ACT_NONE = 0, 1, 2
+RB_SCORE_SOFTMAX, RB_SCORE_SIGMOID = 0, 1
 RB_OK, RB_ERR_VALUE, RB_ERR_UNSUPPORTED, RB_ERR_CUDA, RB_ERR_DEVICE = 0, 1, 2, 3, 4
 RB_MAX_SLOTS = 32
 RB_MAX_DEST = 8
@@ -57,6 +58,10 @@ SIGNATURES = {
     "rb_smoe_workspace_size": [_i64, _i32, _i32, _i32, _i32, _i32],
     "rb_smoe_experts": [_vp, _i32, _i64, _i64, _i32, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp,
                         _i64, _vp, _i64, _vp],
+    "rb_route_topk": [_vp, _i32, _i64, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _i32, _vp, _i32,
+                      _vp, _vp, _vp],
+    "rb_route_topk_backward": [_vp, _i32, _i64, _i64, _i32, _vp, _i32, _i32, _vp, _i32, _vp, _i32, _i32, _i32, _f32,
+                               _vp, _i32, _vp],
     "rb_rep_gather_pool_scatter": [_vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _i32, _i64,
                                    _i64, _vp],
     "rb_ipc_export": [_vp, _vp, _vp],

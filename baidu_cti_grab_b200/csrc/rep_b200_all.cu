@@ -5,4 +5,5 @@
 #include "quant.cu"
 #include "gemm_tc.cu"
 #include "moe.cu"
+#include "route.cu"
 #include "peer.cu"

@@ -493,6 +493,97 @@ def smoe_experts(x: torch.Tensor, topk_idx: torch.Tensor, topk_score: torch.Tens
     return out
 
 
+# ------------------------------------------------------- routing to experts
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_SCORES = {"softmax": L.RB_SCORE_SOFTMAX, "sigmoid": L.RB_SCORE_SIGMOID}
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """L.call on `dev`'s current stream, which becomes the last argument."""
+    if torch.cuda.current_device() == dev.index:
+        L.call(name, *args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            L.call(name, *args, _stream(dev))
+
+
+def _score_kind(score: str) -> int:
+    try:
+        return _SCORES[score]
+    except KeyError:
+        raise ValueError(f"score must be one of {sorted(_SCORES)}, not {score!r}") from None
+
+
+def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
+               groups: int = 1, topk_groups: int = 1, group_top: int = 2, renormalize: bool = False,
+               scale: float = 1.0, idx_dtype: torch.dtype = torch.int64, score_dtype: Optional[torch.dtype] = None,
+               want_probs: bool = False, want_counts: bool = False):
+    """The choice of k experts per token that smoe_experts takes (rb_route_topk).
+
+    logits [T, E] fp32/bf16/f16 (rows may be strided), E <= 512, k <= 32; a logit of -inf or of
+    the type's lowest value masks its expert.  bias fp32 [E] counts for the choice only.  Of `groups`
+    equal runs of experts the topk_groups with the highest sums of their group_top best stay.
+    Returns (idx [T, k] by falling choice value, ties to the lowest index; score [T, k] in score_dtype
+    (default: the logits'), probs [T, E] in score_dtype or None, counts int32 [E] or None)."""
+    dev = require_cuda("route_topk", logits, bias)
+    if logits.dim() != 2 or logits.dtype not in _FLOATS:
+        raise ValueError("route_topk expects logits [T, E] in fp32, bf16 or f16")
+    T, E = logits.shape
+    kind = _score_kind(score)
+    if bias is not None:
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (E,):
+            raise ValueError(f"bias must be fp32 [{E}]")
+        bias = bias.contiguous()
+    if idx_dtype not in (torch.int64, torch.int32):
+        raise ValueError("idx_dtype must be int64 or int32")
+    score_dtype = logits.dtype if score_dtype is None else score_dtype
+    if score_dtype not in _FLOATS:
+        raise ValueError("score_dtype must be fp32, bf16 or f16")
+    if not 1 <= k <= max(E, 1):
+        raise ValueError(f"k must be in [1, {E}]")
+    if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
+        logits = logits.contiguous()
+    idx = torch.empty((T, k), dtype=idx_dtype, device=dev)
+    chosen = torch.empty((T, k), dtype=score_dtype, device=dev)
+    probs = torch.empty((T, E), dtype=score_dtype, device=dev) if want_probs else None
+    counts = torch.empty((E,), dtype=torch.int32, device=dev) if want_counts else None
+    _call_on(dev, "rb_route_topk", logits.data_ptr(), rb_dtype(logits), max(logits.stride(0), E), T, E, _ptr(bias), k,
+             kind, groups, topk_groups, group_top, int(renormalize), float(scale), idx.data_ptr(),
+             L.RB_I64 if idx_dtype == torch.int64 else L.RB_I32, chosen.data_ptr(), rb_dtype(chosen), _ptr(probs),
+             _ptr(counts))
+    return idx, chosen, probs, counts
+
+
+def route_topk_backward(logits: torch.Tensor, idx: torch.Tensor, grad_score: Optional[torch.Tensor],
+                        grad_probs: Optional[torch.Tensor] = None, *, score: str = "softmax",
+                        renormalize: bool = False, scale: float = 1.0) -> torch.Tensor:
+    """Gradient [T, E] of route_topk's logits, in their dtype (rb_route_topk_backward), from the
+    gradients of its scores [T, k] and probs [T, E] (either may be None) and its idx."""
+    dev = require_cuda("route_topk_backward", logits, idx, grad_score, grad_probs)
+    if logits.dim() != 2 or logits.dtype not in _FLOATS:
+        raise ValueError("route_topk_backward expects logits [T, E] in fp32, bf16 or f16")
+    T, E = logits.shape
+    kind = _score_kind(score)
+    if idx.dim() != 2 or idx.shape[0] != T or idx.dtype not in (torch.int64, torch.int32):
+        raise ValueError("idx must be int64 or int32 [T, k]")
+    if grad_score is not None and (grad_score.shape != idx.shape or grad_score.dtype not in _FLOATS):
+        raise ValueError("grad_score must be a float tensor of idx's shape")
+    if grad_probs is not None and (grad_probs.shape != logits.shape or grad_probs.dtype not in _FLOATS):
+        raise ValueError("grad_probs must be a float tensor of the logits' shape")
+    if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
+        logits = logits.contiguous()
+    idx = idx.contiguous()
+    grad_score = None if grad_score is None else grad_score.contiguous()
+    grad_probs = None if grad_probs is None else grad_probs.contiguous()
+    out = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    _call_on(dev, "rb_route_topk_backward", logits.data_ptr(), rb_dtype(logits), max(logits.stride(0), E), T, E,
+             idx.data_ptr(), L.RB_I64 if idx.dtype == torch.int64 else L.RB_I32, idx.shape[1], _ptr(grad_score),
+             rb_dtype(grad_score) if grad_score is not None else 0, _ptr(grad_probs),
+             rb_dtype(grad_probs) if grad_probs is not None else 0, kind, int(renormalize), float(scale),
+             out.data_ptr(), rb_dtype(out))
+    return out
+
+
 def device_error(reset: bool = False) -> int:
     return L.device_error(reset)
 

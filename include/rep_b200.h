@@ -314,6 +314,40 @@ int rb_smoe_experts(const void* x, int x_dtype, int64_t ldx, int64_t T, int D, c
                     const void* w2, const void* b2, int F, void* workspace, int64_t workspace_bytes,
                     void* out, int64_t ldo, void* stream);
 
+/*
+ * Routing to experts: the idx and score that rb_smoe_experts takes, from logits.
+ *   logits     [T, ld] fp32, bf16 or fp16, E <= 512 experts; a logit of -inf or of
+ *              the type's lowest finite value masks its expert for the token
+ *   scores     s = softmax over the token's unmasked logits (RB_SCORE_SOFTMAX) or
+ *              sigmoid (RB_SCORE_SIGMOID); 0 where masked
+ *   bias       [E] fp32 or NULL: added for the choice only, c = s + bias; a masked
+ *              expert's c is -inf, a NaN is above every number
+ *   groups     the experts as `groups` runs of E / groups; a group's value is the sum
+ *              of its group_top (1 or 2) highest c, and the topk_groups groups of the
+ *              highest values stay
+ *   idx        [T, k] RB_I64 or RB_I32, k <= 32: the experts of the k highest c among
+ *              the groups that stay, c falling; ties (groups too) to the lowest
+ *              index, decided on the exact values, whatever the fp32 scores round to.
+ *              Where fewer than k are unmasked, masked ones follow with score 0.
+ *   score      [T, k]: s of the chosen, divided by their sum when `renormalize` (0
+ *              when the sum is 0), times `scale`
+ *   probs      [T, E] contiguous, score_dtype, or NULL: every expert's s
+ *   counts     [E] int32 or NULL: how often each expert was chosen
+ * The backward call gives grad_logits [T, E] (contiguous, out_dtype) from
+ * grad_score [T, k] and grad_probs [T, E] (contiguous, each may be NULL) with the
+ * same logits and the idx of the forward call (distinct in a row; one outside
+ * [0, E) is passed over); bias and groups take no part.
+ */
+enum rb_score_kind { RB_SCORE_SOFTMAX = 0, RB_SCORE_SIGMOID = 1 };
+int rb_route_topk(const void* logits, int dtype, int64_t ld, int64_t T, int E, const void* bias, int k,
+                  int score_kind, int groups, int topk_groups, int group_top, int renormalize, float scale,
+                  void* idx, int idx_dtype, void* score, int score_dtype, void* probs, void* counts,
+                  void* stream);
+int rb_route_topk_backward(const void* logits, int dtype, int64_t ld, int64_t T, int E, const void* idx,
+                           int idx_dtype, int k, const void* grad_score, int grad_dtype,
+                           const void* grad_probs, int probs_dtype, int score_kind, int renormalize,
+                           float scale, void* grad_logits, int out_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
