@@ -21,6 +21,9 @@ LIB_PATH = os.path.join(HERE, "librep_b200.so")
 RB_F32, RB_BF16, RB_F16, RB_I32, RB_I8, RB_I64 = 0, 1, 2, 3, 4, 5
 RB_ACT_DYNAMIC, RB_ACT_STATIC, RB_ACT_NONE = 0, 1, 2
 RB_SCORE_SOFTMAX, RB_SCORE_SIGMOID = 0, 1
+RB_NORM_NONE, RB_NORM_LAYER, RB_NORM_RMS = 0, 1, 2
+RB_GATE_NONE, RB_GATE_CHANNEL, RB_GATE_ROW, RB_GATE_FULL = 0, 1, 2, 3
+RB_GATE_ACT_NONE, RB_GATE_ACT_SIGMOID = 0, 1
 RB_OK, RB_ERR_VALUE, RB_ERR_UNSUPPORTED, RB_ERR_CUDA, RB_ERR_DEVICE = 0, 1, 2, 3, 4
 RB_MAX_SLOTS = 32
 RB_MAX_DEST = 8
@@ -62,6 +65,12 @@ SIGNATURES = {
                       _vp, _vp, _vp],
     "rb_route_topk_backward": [_vp, _i32, _i64, _i64, _i32, _vp, _i32, _i32, _vp, _i32, _vp, _i32, _i32, _i32, _f32,
                                _vp, _i32, _vp],
+    "rb_sandwich_norm": [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _i32, _f32, _i32, _vp, _i32, _i64, _i32,
+                         _f32, _i32, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _vp],
+    "rb_sandwich_norm_workspace_size": [_i64, _i32, _i32],
+    "rb_sandwich_norm_backward": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _i32,
+                                  _i32, _vp, _i32, _i64, _i32, _f32, _i32, _vp, _vp, _i32, _vp, _i64, _vp, _vp, _vp, _vp,
+                                  _vp, _vp, _vp, _vp],
     "rb_rep_gather_pool_scatter": [_vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _i32, _i64,
                                    _i64, _vp],
     "rb_ipc_export": [_vp, _vp, _vp],
@@ -73,7 +82,7 @@ SIGNATURES = {
     "rb_version": [],
 }
 
-RETURNS_I64 = {"rb_w8a8_gemm_workspace_size", "rb_smoe_workspace_size"}
+RETURNS_I64 = {"rb_w8a8_gemm_workspace_size", "rb_smoe_workspace_size", "rb_sandwich_norm_workspace_size"}
 
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None

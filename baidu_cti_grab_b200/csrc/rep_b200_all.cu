@@ -6,4 +6,5 @@
 #include "gemm_tc.cu"
 #include "moe.cu"
 #include "route.cu"
+#include "block_norm.cu"
 #include "peer.cu"

@@ -589,6 +589,123 @@ def route_topk_backward(logits: torch.Tensor, idx: torch.Tensor, grad_score: Opt
     return out
 
 
+# -------------------------------------- norms, gate and residual between blocks
+_NORMS = {None: L.RB_NORM_NONE, "layer": L.RB_NORM_LAYER, "rms": L.RB_NORM_RMS}
+_GATE_ACTS = {"none": L.RB_GATE_ACT_NONE, "sigmoid": L.RB_GATE_ACT_SIGMOID}
+
+
+def _norm_args(name, x, h, post, post_weight, post_bias, gate, gate_act, pre, pre_weight, pre_bias):
+    """What both directions check: (device, rows, width, x2, h2, gate2, gate kind, gate pitch, post, pre, act codes)."""
+    dev = require_cuda(name, x, h, post_weight, post_bias, gate, pre_weight, pre_bias)
+    if x.dtype not in _FLOATS or x.dim() < 1 or x.shape != h.shape or h.dtype != x.dtype:
+        raise ValueError(f"{name} expects x and h [..., D] of one shape and one type (fp32, bf16 or f16)")
+    try:
+        kinds = _NORMS[post], _NORMS[pre]
+    except KeyError:
+        raise ValueError("post and pre are 'layer', 'rms' or None") from None
+    if gate_act not in _GATE_ACTS:
+        raise ValueError(f"gate_act must be one of {sorted(_GATE_ACTS)}")
+    D = x.shape[-1]
+    for kind, w, b in ((post, post_weight, post_bias), (pre, pre_weight, pre_bias)):
+        for t in (w, b):
+            if t is not None and (tuple(t.shape) != (D,) or t.dtype not in _FLOATS or not t.is_contiguous()):
+                raise ValueError(f"norm weights and biases must be contiguous fp32, bf16 or f16 [{D}]")
+            if t is not None and kind is None:
+                raise ValueError("a weight or bias was given without its norm")
+        if w is not None and b is not None and w.dtype != b.dtype:
+            raise ValueError("a norm's weight and bias must share a type")
+    x2, h2 = _rows2d(x, D), _rows2d(h, D)
+    N = x2.shape[0]
+    kind, ldg, gate2 = L.RB_GATE_NONE, 0, gate
+    if gate is not None:
+        if gate.dtype not in _FLOATS:
+            raise ValueError("the gate must be fp32, bf16 or f16")
+        if gate.dim() == 1 and gate.shape[0] == D and (x.dim() > 1 or D != 1):
+            kind, gate2 = L.RB_GATE_CHANNEL, gate.contiguous()
+        elif tuple(gate.shape) == (*x.shape[:-1], 1):
+            kind, gate2, ldg = L.RB_GATE_ROW, gate.reshape(-1).contiguous(), 1
+        elif gate.shape == x.shape:
+            if gate.dtype != x.dtype:
+                raise ValueError("a gate of every element must have x's type")
+            kind, gate2 = L.RB_GATE_FULL, _rows2d(gate, D)
+            ldg = max(gate2.stride(0), D)
+        else:
+            raise ValueError(f"the gate must be [{D}], [..., 1] or of x's shape")
+    return dev, N, D, x2, h2, gate2, kind, ldg, kinds[0], kinds[1], _GATE_ACTS[gate_act]
+
+
+def _rows2d(t: torch.Tensor, D: int) -> torch.Tensor:
+    """t [..., D] as rows [N, D] with contiguous values (a copy only where no view has them)."""
+    t2 = t if t.dim() == 2 else t.reshape(-1, D) if D else t.reshape(0, 0)
+    if t2.stride(1) != 1 or (t2.shape[0] > 1 and t2.stride(0) < D):
+        t2 = t2.contiguous()
+    return t2
+
+
+def _norm_dtype(w: Optional[torch.Tensor], b: Optional[torch.Tensor]) -> int:
+    return rb_dtype(w) if w is not None else rb_dtype(b) if b is not None else 0
+
+
+def sandwich_norm(x: torch.Tensor, h: torch.Tensor, *, post: Optional[str] = None,
+                  post_weight: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None,
+                  post_eps: float = 1e-5, gate: Optional[torch.Tensor] = None, gate_act: str = "none", scale: float = 1.0,
+                  pre: Optional[str] = None, pre_weight: Optional[torch.Tensor] = None,
+                  pre_bias: Optional[torch.Tensor] = None, pre_eps: float = 1e-5, want_stats: bool = False):
+    """The seam between two blocks as one kernel (rb_sandwich_norm): y = x + scale * act(gate) * post(h), z = pre(y).
+
+    x (the residual stream) and h (a block's output) [..., D], D <= 8192; post and pre 'layer', 'rms' or
+    None with optional weights and biases [D]; gate None, [D], [..., 1] or x's shape, as it is or its
+    sigmoid.  Returns (y, z or None, stats fp32 [N, 4] or None: what sandwich_norm_backward takes)."""
+    dev, N, D, x2, h2, g2, gk, ldg, k1, k2, act = _norm_args("sandwich_norm", x, h, post, post_weight, post_bias, gate,
+                                                             gate_act, pre, pre_weight, pre_bias)
+    y = x.new_empty(x.shape)
+    z = x.new_empty(x.shape) if k2 != L.RB_NORM_NONE else None
+    stats = x.new_empty((N, 4), dtype=torch.float32) if want_stats else None
+    _call_on(dev, "rb_sandwich_norm", x2.data_ptr(), max(x2.stride(0), D), h2.data_ptr(), max(h2.stride(0), D),
+             rb_dtype(x2), N, D, k1, _ptr(post_weight), _ptr(post_bias), _norm_dtype(post_weight, post_bias),
+             float(post_eps), gk, _ptr(g2), 0 if g2 is None else rb_dtype(g2), ldg, act, float(scale), k2,
+             _ptr(pre_weight), _ptr(pre_bias), _norm_dtype(pre_weight, pre_bias), float(pre_eps), y.data_ptr(), _ptr(z),
+             _ptr(stats))
+    return y, z, stats
+
+
+def sandwich_norm_backward(grad_y: Optional[torch.Tensor], grad_z: Optional[torch.Tensor], x: torch.Tensor,
+                           h: torch.Tensor, stats: torch.Tensor, *, post: Optional[str] = None,
+                           post_weight: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None,
+                           gate: Optional[torch.Tensor] = None, gate_act: str = "none", scale: float = 1.0,
+                           pre: Optional[str] = None, pre_weight: Optional[torch.Tensor] = None,
+                           pre_bias: Optional[torch.Tensor] = None):
+    """Gradients (x, h, gate, post_weight, post_bias, pre_weight, pre_bias) of sandwich_norm, None where
+    there is no such input (rb_sandwich_norm_backward), from those of y and z (either may be None) and the
+    forward call's inputs and stats.  The same bits every time."""
+    dev, N, D, x2, h2, g2, gk, ldg, k1, k2, act = _norm_args("sandwich_norm_backward", x, h, post, post_weight, post_bias,
+                                                             gate, gate_act, pre, pre_weight, pre_bias)
+    require_cuda("sandwich_norm_backward", x, grad_y, grad_z, stats)
+    grads = []
+    for t in (grad_y, grad_z):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError("grad_y and grad_z must have x's shape and type")
+        grads.append(None if t is None else _rows2d(t, D))
+    dy, dz = grads
+    if dz is not None and pre is None:
+        raise ValueError("grad_z was given without pre")
+    if tuple(stats.shape) != (N, 4) or stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise ValueError(f"stats must be the forward call's fp32 [{N}, 4]")
+    dx, dh = x.new_empty(x.shape), x.new_empty(x.shape)
+    outs = [None if t is None else t.new_empty(t.shape) for t in (gate, post_weight, post_bias, pre_weight, pre_bias)]
+    ws_bytes = int(L.load().rb_sandwich_norm_workspace_size(N, D, rb_dtype(x2)))
+    if ws_bytes < 0:
+        raise ValueError(f"rows of {D} values are not supported")
+    ws = x.new_empty((ws_bytes,), dtype=torch.uint8)
+    _call_on(dev, "rb_sandwich_norm_backward", _ptr(dy), D if dy is None else max(dy.stride(0), D), _ptr(dz),
+             D if dz is None else max(dz.stride(0), D), x2.data_ptr(), max(x2.stride(0), D), h2.data_ptr(),
+             max(h2.stride(0), D), stats.data_ptr(), rb_dtype(x2), N, D, k1, _ptr(post_weight), _ptr(post_bias),
+             _norm_dtype(post_weight, post_bias), gk, _ptr(g2), 0 if g2 is None else rb_dtype(g2), ldg, act, float(scale), k2,
+             _ptr(pre_weight), _ptr(pre_bias), _norm_dtype(pre_weight, pre_bias), ws.data_ptr(), ws_bytes, dx.data_ptr(),
+             dh.data_ptr(), _ptr(outs[0]), _ptr(outs[1]), _ptr(outs[2]), _ptr(outs[3]), _ptr(outs[4]))
+    return (dx, dh, *outs)
+
+
 def device_error(reset: bool = False) -> int:
     return L.device_error(reset)
 

@@ -348,6 +348,45 @@ int rb_route_topk_backward(const void* logits, int dtype, int64_t ld, int64_t T,
                            const void* grad_probs, int probs_dtype, int score_kind, int renormalize,
                            float scale, void* grad_logits, int out_dtype, void* stream);
 
+/*
+ * The norm after a block, its gate and residual scale, and the norm before the
+ * next block, on rows of D <= 8192 values:
+ *   n = post(h);  y = x + scale * act(gate) * n;  z = pre(y)
+ *   x, h       [N, ldx], [N, ldh] of one type (fp32, bf16, fp16); y and z [N, D]
+ *              contiguous, of that type; each rounded once from fp32
+ *   post, pre  RB_NORM_NONE, RB_NORM_LAYER ((v - mean) / sqrt(var + eps)) or
+ *              RB_NORM_RMS (v / sqrt(mean v^2 + eps)), times w plus b ([D], any
+ *              float type, or NULL); without pre, z is not written
+ *   gate       none; RB_GATE_CHANNEL [D]; RB_GATE_ROW [N], ldg elements apart;
+ *              RB_GATE_FULL [N, ldg] in the rows' type; as it is or its sigmoid
+ *   stats      [N, 4] fp32, 16-byte aligned, or NULL: mean and 1/deviation of post
+ *              and pre, for the backward call
+ * pre takes the unrounded y.  Rows on 16-byte boundaries with D a multiple of 8
+ * come by bulk copies; others value by value.
+ * The backward call takes dL/dy and dL/dz (either may be NULL: zeros), the same
+ * x, h, gate and weights and the stats, and writes dx, dh [N, D] contiguous, dgate
+ * (gate's shape and type, contiguous) and the weights' gradients in their types
+ * (each may be NULL).  Sums over rows are taken in a fixed order (the same bits
+ * every time).  workspace: rb_sandwich_norm_workspace_size bytes (-1: bad shape).
+ */
+enum rb_norm_kind { RB_NORM_NONE = 0, RB_NORM_LAYER = 1, RB_NORM_RMS = 2 };
+enum rb_gate_kind { RB_GATE_NONE = 0, RB_GATE_CHANNEL = 1, RB_GATE_ROW = 2, RB_GATE_FULL = 3 };
+enum rb_gate_act { RB_GATE_ACT_NONE = 0, RB_GATE_ACT_SIGMOID = 1 };
+int rb_sandwich_norm(const void* x, int64_t ldx, const void* h, int64_t ldh, int dtype, int64_t N, int D,
+                     int post, const void* post_w, const void* post_b, int post_dtype, float post_eps,
+                     int gate_kind, const void* gate, int gate_dtype, int64_t ldg, int gate_act, float scale,
+                     int pre, const void* pre_w, const void* pre_b, int pre_dtype, float pre_eps,
+                     void* y, void* z, float* stats, void* stream);
+int64_t rb_sandwich_norm_workspace_size(int64_t N, int D, int dtype);
+int rb_sandwich_norm_backward(const void* dy, int64_t ldy, const void* dz, int64_t ldz, const void* x,
+                              int64_t ldx, const void* h, int64_t ldh, const float* stats, int dtype,
+                              int64_t N, int D, int post, const void* post_w, const void* post_b,
+                              int post_dtype, int gate_kind, const void* gate, int gate_dtype, int64_t ldg,
+                              int gate_act, float scale, int pre, const void* pre_w, const void* pre_b,
+                              int pre_dtype, void* workspace, int64_t workspace_bytes, void* dx, void* dh,
+                              void* dgate, void* dpost_w, void* dpost_b, void* dpre_w, void* dpre_b,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif
