@@ -35,18 +35,22 @@ constexpr int kMaxStages = 4;
 enum Kind : int { kNone = RB_NORM_NONE, kLayer = RB_NORM_LAYER, kRms = RB_NORM_RMS };
 enum Gate : int { kGateNone = RB_GATE_NONE, kGateChannel = RB_GATE_CHANNEL, kGateRow = RB_GATE_ROW, kGateFull = RB_GATE_FULL };
 enum Act : int { kActNone = RB_GATE_ACT_NONE, kActSigmoid = RB_GATE_ACT_SIGMOID };
-constexpr int kSums = 5;  // column sums of backward: dw_post, db_post, dw_pre, db_pre, dgate
+// column sums of backward, t' = act(g) t with the gates of rows and elements: P = sum t' v^ and Q = sum t' of the
+// post norm (from which its weight's, bias's and a channel gate's gradients follow), dw and db of the pre norm
+constexpr int kSums = 4;
 
 struct Params {
-  const void *x, *h, *gate, *dy, *dz;     // rows (dy, dz: backward only; each may be null)
+  const void* src[5];                     // rows read: x, h, then a gate of every element | dy, dz and that gate; null: absent
+  int64_t pitch[5];                       // their bytes from row to row
+  const void* gate;
   const void *w1, *b1, *w2, *b2;          // post and pre affine, or null
   void *out0, *out1, *out2;               // y, z | dx, dh, dgate (rows or elements)
   float* stats;                           // [N, 4]: post mean, 1/deviation, pre mean, 1/deviation
   float* partial;                         // backward: [CTAs][kSums][D]
-  int64_t N, ldx, ldh, ldg, ldy, ldz;
+  int64_t N, ldg;
   float eps1, eps2, scale;
   int D, post, pre, gate_kind, act, w1_dtype, w2_dtype, gate_dtype;
-  int bulk, stages, row_bytes, need_sums;
+  int bulk, stages, row_bytes, need_sums, table_at, arrays;  // arrays: of src, those that are there
 };
 
 // eight values as they lie in memory
@@ -122,27 +126,131 @@ __device__ __forceinline__ void param8(const void* p, int dtype, int c, int D, f
   for (int i = 0; i < 8; ++i) v[i] = c + i < D ? load_as_f32(p, dtype, c + i) : 0.0f;
 }
 
+template <typename T>
+__device__ __forceinline__ void widen2(const Eight<T>& e, F2* v) {
+  float f[8];
+  widen(e, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
+}
+template <typename T>
+__device__ __forceinline__ void narrow2(const F2* v, Eight<T>& e) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 q = un(v[i]);
+    f[2 * i] = q.x;
+    f[2 * i + 1] = q.y;
+  }
+  narrow(f, e);
+}
+__device__ __forceinline__ float total(F2 v) {
+  const float2 f = un(v);
+  return f.x + f.y;
+}
+
+// What a column's constants come to: out of the post norm, y = x + a (A v^ + B) with A = scale a_c w, B = scale a_c b,
+// a_c the channel's gate (1 without one) and a the row's or element's; the pre norm's w and b.  A thread's columns
+// stay its own for all rows, so the constants are made once: registers hold them where HOLD, shared memory as fp32
+// where a thread would need too many registers and they fit (`table`), else they are made again for each row.
+struct Columns {
+  const Params* p;
+  const float* table;  // [4][pitch] A, B, w, b of the pre norm, or null
+  int pitch;
+};
+__device__ __forceinline__ float gate_act(float g, int act);
+template <int WHICH>
+__device__ __forceinline__ void make_column8(const Params& p, int c, float* v) {
+  if constexpr (WHICH < 2) {
+    param8(WHICH == 0 ? p.w1 : p.b1, p.w1_dtype, c, p.D, WHICH == 0 ? 1.0f : 0.0f, v);
+    float g[8];
+    if (p.gate_kind == kGateChannel) param8(p.gate, p.gate_dtype, c, p.D, 1.0f, g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= p.gate_kind == kGateChannel ? p.scale * gate_act(g[i], p.act) : p.scale;
+  } else {
+    param8(WHICH == 2 ? p.w2 : p.b2, p.w2_dtype, c, p.D, WHICH == 2 ? 1.0f : 0.0f, v);
+  }
+}
+template <int WHICH>
+__device__ __forceinline__ void column8(const Columns& t, int c, F2* v) {
+  float f[8];
+  if (t.table != nullptr) {
+    if (c >= t.pitch) {  // a thread whose columns lie beyond the row
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = f2(0.0f, 0.0f);
+      return;
+    }
+    const float4* at = reinterpret_cast<const float4*>(t.table + WHICH * t.pitch + c);
+    const float4 a = at[0], b = at[1];
+    v[0] = f2(a.x, a.y);
+    v[1] = f2(a.z, a.w);
+    v[2] = f2(b.x, b.y);
+    v[3] = f2(b.z, b.w);
+    return;
+  }
+  make_column8<WHICH>(*t.p, c, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
+}
+// the table's first `n` rows, by all threads of the CTA
+template <int N>
+__device__ __forceinline__ void fill_table(const Params& p, float* table, int pitch) {
+  for (int c = threadIdx.x * 8; c < pitch; c += blockDim.x * 8) {
+    float f[8];
+    auto put = [&](int which) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) table[which * pitch + c + i] = f[i];
+    };
+    make_column8<0>(p, c, f);
+    put(0);
+    make_column8<1>(p, c, f);
+    put(1);
+    make_column8<2>(p, c, f);
+    put(2);
+    if constexpr (N > 3) {
+      make_column8<3>(p, c, f);
+      put(3);
+    }
+  }
+}
+
+// the sigmoid is off by a few units of 2^-24 (and |g| of them where it is small itself)
 __device__ __forceinline__ float gate_act(float g, int act) {
-  return act == kActSigmoid ? __fdividef(1.0f, 1.0f + expf(-g)) : g;
+  return act == kActSigmoid ? __fdividef(1.0f, 1.0f + __expf(-g)) : g;
 }
 
 // A team of G threads on a row of up to 8 V G values; thread r of the team holds the eights r, r + G, ...
+// Teams of one or two warps share a CTA of 256 threads, wider ones are a CTA.
 template <int G>
 struct Team {
-  static constexpr int kTeams = G == 32 ? 8 : 1;  // teams of a CTA
+  static constexpr int kTeams = G <= 64 ? 256 / G : 1;  // of a CTA
   static constexpr int kThreads = G * kTeams;
-  static constexpr int kWarps = kThreads / 32;
-  __device__ static int index() { return G == 32 ? (int)(threadIdx.x >> 5) : 0; }
-  __device__ static int rank() { return G == 32 ? (int)(threadIdx.x & 31) : (int)threadIdx.x; }
+  static constexpr int kWarps = G / 32;  // of a team
+  static constexpr int kRoom = 2 * kTeams * kWarps * 4;
+  __device__ static int index() { return kTeams == 1 ? 0 : (int)threadIdx.x / G; }
+  __device__ static int rank() { return kTeams == 1 ? (int)threadIdx.x : (int)threadIdx.x % G; }
   __device__ static void sync() {
     if constexpr (G == 32) __syncwarp();
-    else __syncthreads();
+    else if constexpr (kTeams == 1) __syncthreads();
+    else asm volatile("barrier.cta.sync %0, %1;" ::"r"(1 + index()), "n"(G) : "memory");
   }
   __device__ static bool all(bool ok) {
     if constexpr (G == 32) return __all_sync(kAll, ok);
-    else return __syncthreads_and(ok) != 0;
+    else if constexpr (kTeams == 1) return __syncthreads_and(ok) != 0;
+    else {
+      uint32_t every;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\t"
+          "setp.ne.u32 p, %1, 0;\n\t"
+          "barrier.cta.red.and.pred q, %2, %3, p;\n\t"
+          "selp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(every)
+          : "r"((uint32_t)ok), "r"(1 + index()), "n"(G)
+          : "memory");
+      return every != 0;
+    }
   }
-  // sums of M values over the team; `room` holds 2 * kWarps * 4 floats, used in turns
+  // sums of M values over the team; `room` holds kRoom floats, its halves used in turns
   template <int M>
   __device__ static void sum(float (&v)[M], float* room, int& turn) {
 #pragma unroll
@@ -150,21 +258,31 @@ struct Team {
 #pragma unroll
       for (int m = 0; m < M; ++m) v[m] += __shfl_xor_sync(kAll, v[m], o);
     if constexpr (G > 32) {
-      float* at = room + turn * kWarps * 4;
+      float* at = room + (turn * kTeams + index()) * kWarps * 4;
       turn ^= 1;  // the next sum writes the other half, so one barrier per sum is enough
-      if ((threadIdx.x & 31) == 0)
-#pragma unroll
-        for (int m = 0; m < M; ++m) at[(threadIdx.x >> 5) * 4 + m] = v[m];
-      __syncthreads();
       const int lane = threadIdx.x & 31;
+      if (lane == 0)
 #pragma unroll
-      for (int m = 0; m < M; ++m) v[m] = lane < kWarps ? at[lane * 4 + m] : 0.0f;
+        for (int m = 0; m < M; ++m) at[(rank() >> 5) * 4 + m] = v[m];
+      sync();
+      if constexpr (kWarps <= 4) {
 #pragma unroll
-      for (int o = kWarps / 2; o > 0; o >>= 1)
+        for (int m = 0; m < M; ++m) {
+          v[m] = at[m];
 #pragma unroll
-        for (int m = 0; m < M; ++m) v[m] += __shfl_xor_sync(kAll, v[m], o);
+          for (int w = 1; w < kWarps; ++w) v[m] += at[w * 4 + m];
+        }
+      } else {
 #pragma unroll
-      for (int m = 0; m < M; ++m) v[m] = __shfl_sync(kAll, v[m], 0);
+        for (int m = 0; m < M; ++m) v[m] = lane < kWarps ? at[lane * 4 + m] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+            if (o < kWarps) v[m] += __shfl_xor_sync(kAll, v[m], o);
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m] = __shfl_sync(kAll, v[m], 0);
+      }
     }
   }
 };
@@ -175,46 +293,54 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// The rows of a team's turn it: row = first + it * step.  `src` are the arrays that a row is read from.
+// A team's rows: first, first + step, ...  A arrays each.
 template <typename T, int G, int V, int A>
 struct Rows {
-  const char* src[A];
-  int64_t pitch[A];  // bytes
-  uint8_t* ring;     // this team's stages
-  uint64_t* full;    // this team's barriers
+  const Params& p;
+  uint8_t* ring;   // this team's stages
+  uint64_t* full;  // this team's barriers
   volatile int* abort_flag;
-  int64_t first, step, N;
-  int D, stages, row_bytes, bulk;
+  int64_t first, step;
+  int D, stages;
 
-  __device__ uint8_t* slot(int stage, int a) const { return ring + ((int64_t)stage * A + a) * row_bytes; }
-  __device__ void request(int stage, int64_t row) const {  // one thread
+  const char* next;     // thread a < A of the team asks for array a: its next row, or null
+  int64_t next_step;    // bytes from one of the team's rows to the next
+
+  __device__ uint8_t* slot(int stage, int a) const { return ring + (stage * A + a) * p.row_bytes; }
+  __device__ void request(int stage) {  // the team's first warp
+    const int lane = threadIdx.x & 31;
     const uint32_t bytes = (uint32_t)(D * (int)sizeof(T));
-    uint32_t n = 0;
-#pragma unroll
-    for (int a = 0; a < A; ++a) n += src[a] != nullptr ? bytes : 0u;
     const uint32_t bar = smem_u32(full + stage);
-    mbar_arrive_expect_tx(bar, n);
-#pragma unroll
-    for (int a = 0; a < A; ++a)
-      if (src[a] != nullptr) bulk_load(smem_u32(slot(stage, a)), src[a] + row * pitch[a], bytes, bar);
+    if (lane == 0) mbar_arrive_expect_tx(bar, p.arrays * bytes);
+    __syncwarp();
+    if (next != nullptr) {
+      bulk_load(smem_u32(slot(stage, lane)), next, bytes, bar);
+      next += next_step;
+    }
   }
-  __device__ void start() const {
-    if (bulk && Team<G>::rank() == 0)
-      for (int s = 0; s < stages; ++s)
-        if (first + s * step < N) request(s, first + s * step);
+  __device__ void start() {
+    const int r = Team<G>::rank();
+    next = nullptr;
+    if (!p.bulk || r >= 32) return;
+    if (r < A && p.src[r] != nullptr) {
+      next = static_cast<const char*>(p.src[r]) + first * p.pitch[r];
+      next_step = step * p.pitch[r];
+    }
+    for (int s = 0; s < stages; ++s)
+      if (first + s * step < p.N) request(s);
   }
   // Row `row`'s eights (zeros beyond D and for absent arrays) into registers; asks for the row `stages` turns on.
-  __device__ bool take(int64_t row, int stage, uint32_t phase, Eight<T> (&e)[A][V]) const {
+  __device__ bool take(int64_t row, int stage, uint32_t phase, Eight<T> (&e)[A][V]) {
     const int r = Team<G>::rank();
     bool ok = true;
-    if (bulk) {
+    if (p.bulk) {
       ok = mbar_wait_bounded(smem_u32(full + stage), phase, kWaitTimeoutProducer, abort_flag);
     } else {
       // rows that no 16-byte copy can fetch: value by value, neighbours by neighbouring threads
 #pragma unroll
       for (int a = 0; a < A; ++a) {
-        if (src[a] == nullptr) continue;
-        const T* from = reinterpret_cast<const T*>(src[a] + row * pitch[a]);
+        if (p.src[a] == nullptr) continue;
+        const T* from = reinterpret_cast<const T*>(static_cast<const char*>(p.src[a]) + row * p.pitch[a]);
         T* to = reinterpret_cast<T*>(slot(stage, a));
         for (int c = r; c < D; c += G) to[c] = from[c];
       }
@@ -228,7 +354,7 @@ struct Rows {
 #pragma unroll
         for (int q = 0; q < (int)(sizeof(T) / 2); ++q) {
           e[a][v].q[q] = make_uint4(0u, 0u, 0u, 0u);
-          if (ok && src[a] != nullptr && c < D)
+          if (ok && p.src[a] != nullptr && c < D)
             e[a][v].q[q] = reinterpret_cast<const uint4*>(slot(stage, a) + (int64_t)c * sizeof(T))[q];
         }
         if (c < D && c + 8 > D) {  // a row's last eight may be short
@@ -239,18 +365,17 @@ struct Rows {
         }
       }
     ok = Team<G>::all(ok);
-    const int64_t next = row + stages * step;
-    if (bulk && ok && next < N && r == 0) {
+    if (p.bulk && ok && r < 32 && row + stages * step < p.N) {
       // the slot was read through the generic proxy: order those reads before the copy's writes
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      request(stage, next);
+      request(stage);
     }
     return ok;
   }
   // After a wait that gave up at (row, stage, phase): the copies still in flight land before this CTA leaves.
   __device__ void drain(int64_t row, int stage, uint32_t phase) const {
-    if (!bulk || Team<G>::rank() != 0) return;
-    for (int s = 0; s < stages && row < N; ++s, row += step) {
+    if (!p.bulk || Team<G>::rank() != 0) return;
+    for (int s = 0; s < stages && row < p.N; ++s, row += step) {
       mbar_wait_bounded(smem_u32(full + stage), phase, kWaitTimeoutProducer, nullptr);
       if (++stage == stages) {
         stage = 0;
@@ -259,16 +384,16 @@ struct Rows {
     }
   }
   // A row out: straight from registers, or (rows that 16-byte stores do not fit) through this stage's slot a
-  __device__ void put(void* out, int64_t row, int stage, int a, const float (&v)[V * 8]) const {
+  __device__ void put(void* out, int64_t row, int stage, int a, const F2 (&v)[V * 4]) const {
     const int r = Team<G>::rank();
     T* to = static_cast<T*>(out) + row * D;
-    if (bulk) {
+    if (p.bulk) {
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const int c = (k * G + r) * 8;
         if (c >= D) continue;
         Eight<T> e;
-        narrow(v + 8 * k, e);
+        narrow2(v + 4 * k, e);
 #pragma unroll
         for (int q = 0; q < (int)(sizeof(T) / 2); ++q) reinterpret_cast<uint4*>(to + c)[q] = e.q[q];
       }
@@ -280,7 +405,7 @@ struct Rows {
       const int c = (k * G + r) * 8;
       if (c >= D) continue;
       Eight<T> e;
-      narrow(v + 8 * k, e);
+      narrow2(v + 4 * k, e);
 #pragma unroll
       for (int q = 0; q < (int)(sizeof(T) / 2); ++q) reinterpret_cast<uint4*>(via + c)[q] = e.q[q];
     }
@@ -290,33 +415,50 @@ struct Rows {
   }
 };
 
+// zeros beyond a row's D: the columns of eight k of this thread begin at (k G + r) 8
+template <int G, int V>
+__device__ __forceinline__ void zero_tail(F2 (&v)[V * 4], int D) {
+  const int r = Team<G>::rank();
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * G + r) * 8;
+    if (c + 8 > D) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = un(v[4 * k + i]);
+        v[4 * k + i] = f2(c + 2 * i < D ? f.x : 0.0f, c + 2 * i + 1 < D ? f.y : 0.0f);
+      }
+    }
+  }
+}
+
 // v centred and normalised in place over the team's row; mean and 1 / deviation
 template <int G, int V>
-__device__ __forceinline__ void normalise(float (&v)[V * 8], int kind, float eps, int D, float* room, int& turn,
-                                          float& mean, float& rstd) {
-  const int r = Team<G>::rank();
+__device__ __forceinline__ void normalise(F2 (&v)[V * 4], int kind, float eps, int D, float* room, int& turn,
+                                    float& mean, float& rstd) {
   const float inv = 1.0f / (float)D;
   mean = 0.0f;
   if (kind == kLayer) {
-    float s[1] = {0.0f};
+    F2 a = v[0];
 #pragma unroll
-    for (int i = 0; i < V * 8; ++i) s[0] += v[i];
+    for (int i = 1; i < V * 4; ++i) a = add2(a, v[i]);
+    float s[1] = {total(a)};
     Team<G>::sum(s, room, turn);
     mean = s[0] * inv;
+    const F2 m = f2(-mean, -mean);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = (k * G + r) * 8;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[8 * k + i] = c + i < D ? v[8 * k + i] - mean : 0.0f;
-    }
+    for (int i = 0; i < V * 4; ++i) v[i] = add2(v[i], m);
+    zero_tail<G, V>(v, D);
   }
-  float s[1] = {0.0f};
+  F2 a = mul2(v[0], v[0]);
 #pragma unroll
-  for (int i = 0; i < V * 8; ++i) s[0] = fmaf(v[i], v[i], s[0]);
+  for (int i = 1; i < V * 4; ++i) a = fma2(v[i], v[i], a);
+  float s[1] = {total(a)};
   Team<G>::sum(s, room, turn);
   rstd = rsqrtf(fmaf(s[0], inv, eps));
+  const F2 q = f2(rstd, rstd);
 #pragma unroll
-  for (int i = 0; i < V * 8; ++i) v[i] *= rstd;
+  for (int i = 0; i < V * 4; ++i) v[i] = mul2(v[i], q);
 }
 
 template <int G>
@@ -330,34 +472,46 @@ __device__ __forceinline__ void init_ring(uint64_t* full, int stages, volatile i
   __syncthreads();
 }
 
-template <typename T, int G, int V>
-__global__ void __launch_bounds__(Team<G>::kThreads) sandwich_kernel(const __grid_constant__ Params p) {
+template <typename T, int G, int V, bool HOLD>
+__global__ void __launch_bounds__(Team<G>::kThreads, 512 / Team<G>::kThreads)
+    sandwich_kernel(const __grid_constant__ Params p) {
   using Tm = Team<G>;
   constexpr int kArrays = 3;  // x, h, a gate of every element
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ __align__(8) uint64_t full[kMaxStages * Tm::kTeams];
-  __shared__ float room[2 * Tm::kWarps * 4];
+  __shared__ float room[Tm::kRoom];
   __shared__ int abort_flag;
   init_ring<G>(full, p.stages, &abort_flag);
   const int r = Tm::rank();
-  Rows<T, G, V, kArrays> rows;
-  rows.src[0] = static_cast<const char*>(p.x);
-  rows.src[1] = static_cast<const char*>(p.h);
-  rows.src[2] = p.gate_kind == kGateFull ? static_cast<const char*>(p.gate) : nullptr;
-  rows.pitch[0] = p.ldx * (int64_t)sizeof(T);
-  rows.pitch[1] = p.ldh * (int64_t)sizeof(T);
-  rows.pitch[2] = p.ldg * (int64_t)sizeof(T);
-  rows.ring = ring + (int64_t)Tm::index() * p.stages * kArrays * p.row_bytes;
-  rows.full = full + Tm::index() * p.stages;
-  rows.abort_flag = &abort_flag;
-  rows.first = (int64_t)blockIdx.x * Tm::kTeams + Tm::index();
-  rows.step = (int64_t)gridDim.x * Tm::kTeams;
-  rows.N = p.N;
-  rows.D = p.D;
-  rows.stages = p.stages;
-  rows.row_bytes = p.row_bytes;
-  rows.bulk = p.bulk;
+  Rows<T, G, V, kArrays> rows{p,
+                              ring + Tm::index() * p.stages * kArrays * p.row_bytes,
+                              full + Tm::index() * p.stages,
+                              &abort_flag,
+                              (int64_t)blockIdx.x * Tm::kTeams + Tm::index(),
+                              (int64_t)gridDim.x * Tm::kTeams,
+                              p.D,
+                              p.stages,
+                              nullptr,
+                              0};
   rows.start();
+
+  Columns cols{&p, nullptr, (p.D + 7) / 8 * 8};
+  F2 held[HOLD ? 4 : 1][HOLD ? V * 4 : 1];
+  if constexpr (HOLD) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int c = (k * G + r) * 8;
+      column8<0>(cols, c, held[0] + 4 * k);
+      column8<1>(cols, c, held[1] + 4 * k);
+      column8<2>(cols, c, held[2] + 4 * k);
+      column8<3>(cols, c, held[3] + 4 * k);
+    }
+  } else if (p.table_at >= 0) {
+    float* table = reinterpret_cast<float*>(ring + p.table_at);
+    fill_table<4>(p, table, cols.pitch);
+    __syncthreads();
+    cols.table = table;
+  }
 
   int stage = 0, turn = 0;
   uint32_t phase = 0;
@@ -373,46 +527,53 @@ __global__ void __launch_bounds__(Team<G>::kThreads) sandwich_kernel(const __gri
       rows.drain(row, stage, phase);
       break;
     }
-    const float row_gate = next_gate;
+    const F2 row_gate = f2(next_gate, next_gate);
     ahead(row + rows.step);
-    float n[V * 8], y[V * 8];
+    F2 n[V * 4], y[V * 4];
     float mean1 = 0.0f, rstd1 = 1.0f, mean2 = 0.0f, rstd2 = 1.0f;
 #pragma unroll
-    for (int k = 0; k < V; ++k) widen(e[1][k], n + 8 * k);
+    for (int k = 0; k < V; ++k) widen2(e[1][k], n + 4 * k);
     if (p.post != kNone) normalise<G, V>(n, p.post, p.eps1, p.D, room, turn, mean1, rstd1);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const int c = (k * G + r) * 8;
-      float* nk = n + 8 * k;
-      if (p.post != kNone) {
-        float w[8], b[8];
-        param8(p.w1, p.w1_dtype, c, p.D, 1.0f, w);
-        param8(p.b1, p.w1_dtype, c, p.D, 0.0f, b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) nk[i] = fmaf(nk[i], w[i], b[i]);
+      F2 A[4], B[4];
+      if constexpr (!HOLD) {
+        column8<0>(cols, c, A);
+        column8<1>(cols, c, B);
       }
-      if (p.gate_kind == kGateChannel || p.gate_kind == kGateFull) {
+      F2 x[4];
+      widen2(e[0][k], x);
+      F2 a[4] = {row_gate, row_gate, row_gate, row_gate};
+      if (p.gate_kind == kGateFull) {
         float g[8];
-        if (p.gate_kind == kGateFull) widen(e[2][k], g);
-        else param8(p.gate, p.gate_dtype, c, p.D, 1.0f, g);
+        widen(e[2][k], g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) nk[i] *= gate_act(g[i], p.act);
+        for (int i = 0; i < 4; ++i) a[i] = f2(gate_act(g[2 * i], p.act), gate_act(g[2 * i + 1], p.act));
       }
-      widen(e[0][k], y + 8 * k);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[8 * k + i] = c + i < p.D ? fmaf(p.scale * row_gate, nk[i], y[8 * k + i]) : 0.0f;
+      for (int i = 0; i < 4; ++i) {
+        const F2 q = HOLD ? fma2(n[4 * k + i], held[0][HOLD ? 4 * k + i : 0], held[1][HOLD ? 4 * k + i : 0])
+                          : fma2(n[4 * k + i], A[i], B[i]);
+        y[4 * k + i] = fma2(a[i], q, x[i]);
+      }
     }
+    zero_tail<G, V>(y, p.D);
     rows.put(p.out0, row, stage, 0, y);
     if (p.pre != kNone) {
       normalise<G, V>(y, p.pre, p.eps2, p.D, room, turn, mean2, rstd2);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const int c = (k * G + r) * 8;
-        float w[8], b[8];
-        param8(p.w2, p.w2_dtype, c, p.D, 1.0f, w);
-        param8(p.b2, p.w2_dtype, c, p.D, 0.0f, b);
+        F2 w[4], b[4];
+        if constexpr (!HOLD) {
+          column8<2>(cols, c, w);
+          column8<3>(cols, c, b);
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[8 * k + i] = fmaf(y[8 * k + i], w[i], b[i]);
+        for (int i = 0; i < 4; ++i)
+          y[4 * k + i] = HOLD ? fma2(y[4 * k + i], held[2][HOLD ? 4 * k + i : 0], held[3][HOLD ? 4 * k + i : 0])
+                              : fma2(y[4 * k + i], w[i], b[i]);
       }
       rows.put(p.out1, row, stage, 0, y);
     }
@@ -425,49 +586,57 @@ __global__ void __launch_bounds__(Team<G>::kThreads) sandwich_kernel(const __gri
   }
 }
 
-// LEAN: no biases and no gate per channel, so two of the five column sums.
-template <typename T, int G, int V, bool LEAN>
-__global__ void __launch_bounds__(Team<G>::kThreads) sandwich_backward_kernel(const __grid_constant__ Params p) {
+// LEAN: no biases and no gate per channel: the column sums P and dw alone.
+template <typename T, int G, int V, bool HOLD, bool LEAN>
+__global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 512 / Team<G>::kThreads : 1)
+    sandwich_backward_kernel(const __grid_constant__ Params p) {
   using Tm = Team<G>;
   constexpr int kArrays = 5;  // x, h, dy, dz, a gate of every element
   constexpr int NV = V * 8;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ __align__(8) uint64_t full[kMaxStages * Tm::kTeams];
-  __shared__ float room[2 * Tm::kWarps * 4];
+  __shared__ float room[Tm::kRoom];
   __shared__ int abort_flag;
   init_ring<G>(full, p.stages, &abort_flag);
   const int r = Tm::rank();
-  Rows<T, G, V, kArrays> rows;
-  rows.src[0] = static_cast<const char*>(p.x);
-  rows.src[1] = static_cast<const char*>(p.h);
-  rows.src[2] = static_cast<const char*>(p.dy);
-  rows.src[3] = static_cast<const char*>(p.dz);
-  rows.src[4] = p.gate_kind == kGateFull ? static_cast<const char*>(p.gate) : nullptr;
-  rows.pitch[0] = p.ldx * (int64_t)sizeof(T);
-  rows.pitch[1] = p.ldh * (int64_t)sizeof(T);
-  rows.pitch[2] = p.ldy * (int64_t)sizeof(T);
-  rows.pitch[3] = p.ldz * (int64_t)sizeof(T);
-  rows.pitch[4] = p.ldg * (int64_t)sizeof(T);
-  rows.ring = ring + (int64_t)Tm::index() * p.stages * kArrays * p.row_bytes;
-  rows.full = full + Tm::index() * p.stages;
-  rows.abort_flag = &abort_flag;
-  rows.first = (int64_t)blockIdx.x * Tm::kTeams + Tm::index();
-  rows.step = (int64_t)gridDim.x * Tm::kTeams;
-  rows.N = p.N;
-  rows.D = p.D;
-  rows.stages = p.stages;
-  rows.row_bytes = p.row_bytes;
-  rows.bulk = p.bulk;
+  Rows<T, G, V, kArrays> rows{p,
+                              ring + Tm::index() * p.stages * kArrays * p.row_bytes,
+                              full + Tm::index() * p.stages,
+                              &abort_flag,
+                              (int64_t)blockIdx.x * Tm::kTeams + Tm::index(),
+                              (int64_t)gridDim.x * Tm::kTeams,
+                              p.D,
+                              p.stages,
+                              nullptr,
+                              0};
   rows.start();
 
+  Columns cols{&p, nullptr, (p.D + 7) / 8 * 8};
+  F2 held[HOLD ? 3 : 1][HOLD ? V * 4 : 1];  // A, B, the pre norm's w
+  if constexpr (HOLD) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int c = (k * G + r) * 8;
+      column8<0>(cols, c, held[0] + 4 * k);
+      column8<1>(cols, c, held[1] + 4 * k);
+      column8<2>(cols, c, held[2] + 4 * k);
+    }
+  } else if (p.table_at >= 0) {
+    float* table = reinterpret_cast<float*>(ring + p.table_at);
+    fill_table<3>(p, table, cols.pitch);
+    __syncthreads();
+    cols.table = table;
+  }
+
   constexpr int kHeld = LEAN ? 2 : kSums;
-  float acc[kHeld][NV];  // dw_post, dw_pre, then db_post, db_pre, dgate
+  F2 acc[kHeld][NV / 2];  // P, dw, then Q, db
 #pragma unroll
   for (int a = 0; a < kHeld; ++a)
 #pragma unroll
-    for (int i = 0; i < NV; ++i) acc[a][i] = 0.0f;
+    for (int i = 0; i < NV / 2; ++i) acc[a][i] = f2(0.0f, 0.0f);
 
   const float inv = 1.0f / (float)p.D;
+  const bool mean1 = p.post == kLayer, mean2 = p.pre == kLayer;
   int stage = 0, turn = 0;
   uint32_t phase = 0;
   float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
@@ -475,114 +644,147 @@ __global__ void __launch_bounds__(Team<G>::kThreads) sandwich_backward_kernel(co
   auto ahead = [&](int64_t row) {  // the next row's scalars
     if (row < p.N) {
       st = __ldg(reinterpret_cast<const float4*>(p.stats) + row);
-      if (p.gate_kind == kGateRow) g_row = load_as_f32(p.gate, p.gate_dtype, row * p.ldg);
+      if (p.gate_kind == kGateRow) g_row = gate_act(load_as_f32(p.gate, p.gate_dtype, row * p.ldg), p.act);
     }
   };
   ahead(rows.first);
   for (int64_t row = rows.first; row < p.N; row += rows.step) {
     const float4 s = st;
-    const float gr = g_row;
+    const F2 a_row = f2(g_row, g_row);
     Eight<T> e[kArrays][V];
     if (!rows.take(row, stage, phase, e)) {
       rows.drain(row, stage, phase);
       break;
     }
     ahead(row + rows.step);
-    const float a_row = gate_act(gr, p.gate_kind == kGateRow ? p.act : (int)kActNone);
-    float hh[NV], yh[NV], t[NV];
-    float s12[2] = {0.0f, 0.0f};
-    // n and y again; the pre norm's two sums
+    F2 hh[NV / 2], yh[NV / 2], t[NV / 2], a[NV / 2];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = (k * G + r) * 8;
-      float w[8], b[8], g[8], x[8], dz[8], w2[8];
-      widen(e[1][k], hh + 8 * k);
-      widen(e[0][k], x);
-      widen(e[3][k], dz);
-      if (p.pre != kNone) {
-        param8(p.w1, p.w1_dtype, c, p.D, 1.0f, w);
-        param8(p.b1, p.w1_dtype, c, p.D, 0.0f, b);
-        param8(p.w2, p.w2_dtype, c, p.D, 1.0f, w2);
-        if (p.gate_kind == kGateFull) widen(e[4][k], g);
-        else if (p.gate_kind == kGateChannel) param8(p.gate, p.gate_dtype, c, p.D, 1.0f, g);
-      }
+    for (int i = 0; i < NV / 2; ++i) a[i] = a_row;
+    if (p.gate_kind == kGateFull) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool in = c + i < p.D;
-        const float q = in ? (hh[8 * k + i] - s.x) * s.y : 0.0f;
-        hh[8 * k + i] = q;
-        t[8 * k + i] = 0.0f;
-        if (p.pre != kNone) {
-          float a = a_row;
-          if (p.gate_kind == kGateFull || p.gate_kind == kGateChannel) a = gate_act(g[i], p.act);
-          const float y = fmaf(p.scale * a, fmaf(q, w[i], b[i]), x[i]);
-          const float f = in ? (y - s.z) * s.w : 0.0f;
-          yh[8 * k + i] = f;
-          const float u = dz[i] * w2[i];
-          t[8 * k + i] = u;
-          s12[0] += u;
-          s12[1] = fmaf(u, f, s12[1]);
-          acc[1][8 * k + i] = fmaf(dz[i], f, acc[1][8 * k + i]);
-          if constexpr (!LEAN) acc[3][8 * k + i] += dz[i];
-        }
+      for (int k = 0; k < V; ++k) {
+        float g[8];
+        widen(e[4][k], g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[4 * k + i] = f2(gate_act(g[2 * i], p.act), gate_act(g[2 * i + 1], p.act));
       }
+    }
+    // v^ of the post norm, and with n and y made again the pre norm's two sums
+    {
+      const F2 m = f2(-s.x, -s.x), q = f2(s.y, s.y);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        widen2(e[1][k], hh + 4 * k);
+#pragma unroll
+        for (int i = 4 * k; i < 4 * k + 4; ++i) hh[i] = mul2(add2(hh[i], m), q);
+      }
+      zero_tail<G, V>(hh, p.D);
     }
     if (p.pre != kNone) {
-      Tm::sum(s12, room, turn);
-      if (p.pre == kRms) s12[0] = 0.0f;
+      const F2 m = f2(-s.z, -s.z), q = f2(s.w, s.w);
+      F2 s1 = f2(0.0f, 0.0f), s2 = s1;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) t[i] = s.w * (t[i] - s12[0] * inv - yh[i] * (s12[1] * inv));
+      for (int k = 0; k < V; ++k) {
+        const int c = (k * G + r) * 8;
+        F2 A[4], B[4], x[4];
+        if constexpr (!HOLD) {
+          column8<0>(cols, c, A);
+          column8<1>(cols, c, B);
+        }
+        widen2(e[0][k], x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = 4 * k + i;
+          const F2 n = HOLD ? fma2(hh[j], held[0][HOLD ? j : 0], held[1][HOLD ? j : 0]) : fma2(hh[j], A[i], B[i]);
+          yh[j] = mul2(add2(fma2(a[j], n, x[i]), m), q);
+        }
+      }
+      zero_tail<G, V>(yh, p.D);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const int c = (k * G + r) * 8;
+        F2 w[4], dz[4];
+        if constexpr (!HOLD) column8<2>(cols, c, w);
+        widen2(e[3][k], dz);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = 4 * k + i;
+          const F2 u = HOLD ? mul2(dz[i], held[2][HOLD ? j : 0]) : mul2(dz[i], w[i]);
+          t[j] = u;
+          s1 = add2(s1, u);
+          s2 = fma2(u, yh[j], s2);
+          acc[1][j] = fma2(dz[i], yh[j], acc[1][j]);
+          if constexpr (!LEAN) acc[3][j] = add2(acc[3][j], dz[i]);
+        }
+      }
+      float s12[2] = {total(s1), total(s2)};
+      Tm::sum(s12, room, turn);
+      const F2 c1 = mean2 ? f2(-s12[0] * inv, -s12[0] * inv) : f2(0.0f, 0.0f), c2 = f2(-s12[1] * inv, -s12[1] * inv);
+#pragma unroll
+      for (int i = 0; i < NV / 2; ++i) t[i] = mul2(fma2(yh[i], c2, add2(t[i], c1)), q);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV / 2; ++i) t[i] = f2(0.0f, 0.0f);
     }
     // t reaches y; its way into h, the gate and the post norm's weights
-    float s34[3] = {0.0f, 0.0f, 0.0f};
-    float out[NV];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      F2 dy[4];
+      widen2(e[2][k], dy);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[4 * k + i] = add2(t[4 * k + i], dy[i]);
+    }
+    zero_tail<G, V>(t, p.D);
+    rows.put(p.out0, row, stage, 0, t);
+    F2 s3 = f2(0.0f, 0.0f), s4 = s3, s5 = s3;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const int c = (k * G + r) * 8;
-      float w[8], b[8], g[8], dy[8];
-      widen(e[2][k], dy);
-      param8(p.w1, p.w1_dtype, c, p.D, 1.0f, w);
-      param8(p.b1, p.w1_dtype, c, p.D, 0.0f, b);
-      if (p.gate_kind == kGateFull) widen(e[4][k], g);
-      else if (p.gate_kind == kGateChannel) param8(p.gate, p.gate_dtype, c, p.D, 1.0f, g);
+      F2 A[4], B[4];
+      if constexpr (!HOLD) {
+        column8<0>(cols, c, A);
+        column8<1>(cols, c, B);
+      }
+      if (p.gate_kind == kGateFull || p.gate_kind == kGateRow) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = 8 * k + i;
-        const bool in = c + i < p.D;
-        const float tt = in ? t[j] + dy[i] : 0.0f;
-        t[j] = tt;
-        float a = a_row;
-        if (p.gate_kind == kGateFull || p.gate_kind == kGateChannel) a = gate_act(g[i], p.act);
-        const float dn = p.scale * a * tt;
-        float da = p.scale * fmaf(hh[j], w[i], b[i]) * tt;
-        if (p.act == kActSigmoid) da *= a * (1.0f - a);
-        yh[j] = da;  // a gate of every element: its gradient
-        s34[2] += da;
-        if constexpr (!LEAN) {
-          acc[2][j] += dn;
-          acc[4][j] += da;
+        for (int i = 0; i < 4; ++i) {
+          const int j = 4 * k + i;
+          F2 da = mul2(HOLD ? fma2(hh[j], held[0][HOLD ? j : 0], held[1][HOLD ? j : 0]) : fma2(hh[j], A[i], B[i]), t[j]);
+          if (p.act == kActSigmoid) da = mul2(da, mul2(a[j], sub2(f2(1.0f, 1.0f), a[j])));
+          yh[j] = da;  // of every element: its gradient
+          s5 = add2(s5, da);
         }
-        acc[0][j] = fmaf(dn, hh[j], acc[0][j]);
-        const float v = dn * w[i];
-        out[j] = v;
-        s34[0] += v;
-        s34[1] = fmaf(v, hh[j], s34[1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = 4 * k + i;
+        const F2 Aj = HOLD ? held[0][HOLD ? j : 0] : A[i];
+        const F2 tp = mul2(a[j], t[j]);
+        acc[0][j] = fma2(tp, hh[j], acc[0][j]);
+        if constexpr (!LEAN) acc[2][j] = add2(acc[2][j], tp);
+        const F2 v = mul2(tp, Aj);
+        t[j] = v;
+        s3 = add2(s3, v);
+        s4 = fma2(v, hh[j], s4);
       }
     }
-    rows.put(p.out0, row, stage, 0, t);
     if (p.gate_kind == kGateFull) rows.put(p.out2, row, stage, 0, yh);
-    if (p.post != kNone || p.gate_kind == kGateRow) Tm::sum(s34, room, turn);
-    if (p.gate_kind == kGateRow && r == 0) {
-      if (p.gate_dtype == RB_F32) static_cast<float*>(p.out2)[row] = s34[2];
-      else if (p.gate_dtype == RB_BF16) static_cast<__nv_bfloat16*>(p.out2)[row] = __float2bfloat16_rn(s34[2]);
-      else static_cast<__half*>(p.out2)[row] = __float2half_rn(s34[2]);
-    }
-    if (p.post != kNone) {
-      if (p.post == kRms) s34[0] = 0.0f;
+    if (p.post != kNone || p.gate_kind == kGateRow) {
+      float s345[3] = {total(s3), total(s4), total(s5)};
+      Tm::sum(s345, room, turn);
+      if (p.gate_kind == kGateRow && r == 0) {
+        if (p.gate_dtype == RB_F32) static_cast<float*>(p.out2)[row] = s345[2];
+        else if (p.gate_dtype == RB_BF16) static_cast<__nv_bfloat16*>(p.out2)[row] = __float2bfloat16_rn(s345[2]);
+        else static_cast<__half*>(p.out2)[row] = __float2half_rn(s345[2]);
+      }
+      if (p.post != kNone) {
+        const F2 c3 = mean1 ? f2(-s345[0] * inv, -s345[0] * inv) : f2(0.0f, 0.0f), c4 = f2(-s345[1] * inv, -s345[1] * inv);
+        const F2 q = f2(s.y, s.y);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) out[i] = s.y * (out[i] - s34[0] * inv - hh[i] * (s34[1] * inv));
+        for (int i = 0; i < NV / 2; ++i) t[i] = mul2(fma2(hh[i], c4, add2(t[i], c3)), q);
+      }
     }
-    rows.put(p.out1, row, stage, 0, out);
+    rows.put(p.out1, row, stage, 0, t);
     if (++stage == p.stages) {
       stage = 0;
       phase ^= 1;
@@ -591,7 +793,10 @@ __global__ void __launch_bounds__(Team<G>::kThreads) sandwich_backward_kernel(co
 
   if (!p.need_sums) return;
   // the CTA's sums: its teams one after another through shared memory, then this CTA's row of `partial`
-  constexpr int kPlace[kSums] = {0, 2, 1, 3, 4};  // acc index -> dw_post, db_post, dw_pre, db_pre, dgate
+  auto held_sum = [&](int a, int j) {
+    const float2 f = un(acc[a][j >> 1]);
+    return (j & 1) ? f.y : f.x;
+  };
   if constexpr (Tm::kTeams == 1) {
 #pragma unroll
     for (int a = 0; a < kHeld; ++a)
@@ -600,7 +805,7 @@ __global__ void __launch_bounds__(Team<G>::kThreads) sandwich_backward_kernel(co
         const int c = (k * G + r) * 8;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (c + i < p.D) p.partial[((int64_t)blockIdx.x * kSums + kPlace[a]) * p.D + c + i] = acc[a][8 * k + i];
+          if (c + i < p.D) p.partial[((int64_t)blockIdx.x * kSums + a) * p.D + c + i] = held_sum(a, 8 * k + i);
       }
   } else {
     __syncthreads();  // every team is done with the ring
@@ -616,7 +821,7 @@ __global__ void __launch_bounds__(Team<G>::kThreads) sandwich_backward_kernel(co
             for (int i = 0; i < 8; ++i)
               if (c + i < p.D) {
                 float* at = sums + a * p.D + c + i;
-                *at = (w == 0 ? 0.0f : *at) + acc[a][8 * k + i];
+                *at = (w == 0 ? 0.0f : *at) + held_sum(a, 8 * k + i);
               }
           }
       }
@@ -624,69 +829,111 @@ __global__ void __launch_bounds__(Team<G>::kThreads) sandwich_backward_kernel(co
     }
     for (int c = threadIdx.x; c < kHeld * p.D; c += Tm::kThreads) {
       const int a = c / p.D;
-      p.partial[((int64_t)blockIdx.x * kSums + kPlace[a]) * p.D + (c - a * p.D)] = sums[c];
+      p.partial[((int64_t)blockIdx.x * kSums + a) * p.D + (c - a * p.D)] = sums[c];
     }
   }
 }
 
 struct SumOut {
-  void* out[kSums];
-  int dtype[kSums];
+  void *dw1, *db1, *dw2, *db2, *dgate;
 };
 
-// out[s][c] = the sum of partial[cta][s][c] over the CTAs, in a fixed order: 32 columns a block, the CTAs in
-// eight runs
-__global__ void __launch_bounds__(256) column_sums_kernel(const float* __restrict__ partial, int ctas, int D,
-                                                          const __grid_constant__ SumOut o) {
-  __shared__ float part[8][32];
-  const int s = blockIdx.y;
-  if (o.out[s] == nullptr) return;
-  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-  float v = 0.0f;
-  if (c < D) {
-#pragma unroll 8
-    for (int b = run; b < ctas; b += 8) v += partial[((int64_t)b * kSums + s) * D + c];
-  }
-  part[run][lane] = v;
-  __syncthreads();
-  if (run == 0 && c < D) {
+__device__ __forceinline__ void store_param(void* p, int dtype, int c, float v) {
+  if (p == nullptr) return;
+  if (dtype == RB_F32) static_cast<float*>(p)[c] = v;
+  else if (dtype == RB_BF16) static_cast<__nv_bfloat16*>(p)[c] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(p)[c] = __float2half_rn(v);
+}
+
+// The CTAs' sums of eight columns, in a fixed order (32 runs of CTAs, then a tree), and what follows from them:
+// dw = scale a_c P, db = scale a_c Q, dgate = scale act'(g) (w P + b Q).
+constexpr int kSumRuns = 32;
+__global__ void __launch_bounds__(8 * kSumRuns) column_sums_kernel(const __grid_constant__ Params p, int ctas, int held,
+                                                             const __grid_constant__ SumOut o) {
+  __shared__ float part[kSums][kSumRuns][8];
+  const int at = threadIdx.x & 7, run = threadIdx.x >> 3, c = blockIdx.x * 8 + at;
+  float v[kSums] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < p.D) {
+#pragma unroll 4
+    for (int b = run; b < ctas; b += kSumRuns)
 #pragma unroll
-    for (int k = 1; k < 8; ++k) v += part[k][lane];
-    if (o.dtype[s] == RB_F32) static_cast<float*>(o.out[s])[c] = v;
-    else if (o.dtype[s] == RB_BF16) static_cast<__nv_bfloat16*>(o.out[s])[c] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(o.out[s])[c] = __float2half_rn(v);
+      for (int s = 0; s < kSums; ++s)
+        if (s < held) v[s] += p.partial[((int64_t)b * kSums + s) * p.D + c];
   }
+#pragma unroll
+  for (int s = 0; s < kSums; ++s) part[s][run][at] = v[s];
+  for (int n = kSumRuns / 2; n > 0; n >>= 1) {
+    __syncthreads();
+    if (run < n)
+#pragma unroll
+      for (int s = 0; s < kSums; ++s) part[s][run][at] += part[s][run + n][at];
+  }
+  if (run != 0 || c >= p.D) return;
+  const float P = part[0][0][at], dw = part[1][0][at], Q = part[2][0][at], db = part[3][0][at];
+  float k = p.scale;
+  if (p.gate_kind == kGateChannel) {
+    const float g = load_as_f32(p.gate, p.gate_dtype, c), a = gate_act(g, p.act);
+    const float w = p.w1 != nullptr ? load_as_f32(p.w1, p.w1_dtype, c) : 1.0f;
+    const float b = p.b1 != nullptr ? load_as_f32(p.b1, p.w1_dtype, c) : 0.0f;
+    const float d = p.act == kActSigmoid ? a * (1.0f - a) : 1.0f;
+    store_param(o.dgate, p.gate_dtype, c, p.scale * d * fmaf(w, P, b * Q));
+    k *= a;
+  }
+  store_param(o.dw1, p.w1_dtype, c, k * P);
+  store_param(o.db1, p.w1_dtype, c, k * Q);
+  store_param(o.dw2, p.w2_dtype, c, dw);
+  store_param(o.db2, p.w2_dtype, c, db);
 }
 
 // ------------------------------------------------------------------- host
+constexpr int kMaxSmem = 225 * 1024;
 struct Shape {
-  int threads, teams, stages, row_bytes, smem, per_sm;
+  int threads, teams, stages, row_bytes, smem, table_at;
 };
 
-// team and ring of a width: as many stages (up to kMaxStages) as fit `budget` bytes of a CTA's shared memory
-static Shape shape_of(int team, int arrays, int D, int elt, int budget, int per_sm) {
+// A width's team and ring: as many stages (up to kMaxStages) as fit `budget` bytes of a CTA's shared memory, beside
+// `table` rows of fp32 column constants where asked for and where they fit.
+static Shape shape_of(int team, int arrays, int D, int elt, int64_t budget, int table) {
   Shape s{};
-  s.teams = team == 32 ? 8 : 1;
+  s.teams = team <= 64 ? 256 / team : 1;
   s.threads = team * s.teams;
-  s.row_bytes = (D * elt + 15) / 16 * 16;
-  const int64_t stage = (int64_t)s.teams * arrays * s.row_bytes;
+  s.row_bytes = (D + 7) / 8 * 8 * elt;  // whole eights: a thread reads and writes them as such
+  const int64_t stage = (int64_t)s.teams * arrays * s.row_bytes, columns = (int64_t)table * ((D + 7) / 8 * 8) * 4;
+  const bool room = table > 0 && stage + columns <= kMaxSmem;
+  if (room) budget -= columns;
   s.stages = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxStages, budget / stage));
-  s.smem = (int)(stage * s.stages);
-  s.per_sm = per_sm;
+  s.table_at = room ? (int)(stage * s.stages) : -1;
+  s.smem = (int)(stage * s.stages + (room ? columns : 0));
   return s;
 }
 
-static int forward_team(int D) { return D <= 1024 ? 32 : D <= 2048 ? 128 : D <= 4096 ? 256 : 512; }
-static int backward_team(int D) { return D <= 512 ? 32 : D <= 2048 ? 128 : D <= 4096 ? 256 : 512; }
-
-constexpr int kBackwardBudget = 110 * 1024;
+// eight values a thread
+static int team_of(int D) {
+  for (int team : {32, 64, 128, 256, 512, 640})
+    if (D <= 8 * team) return team;
+  return 1024;
+}
+static int ctas_per_sm(const Shape& s, int threads_per_sm) {
+  const int by_smem = 226 * 1024 / (s.smem + 2048);
+  return std::max(1, std::min(by_smem, threads_per_sm / s.threads));
+}
+// bytes of a CTA's ring, where an SM is to hold `threads` threads and 200 KB of rings
+static int64_t ring_budget(int team, int threads) {
+  const int cta = team <= 64 ? 256 : team;
+  return (int64_t)200 * 1024 / std::max(1, threads / cta);
+}
+constexpr int kForwardThreads = 512, kBackwardThreads = 512;  // an SM's, by the kernels' registers
+static Shape backward_shape(int D, int elt) {
+  const int team = team_of(D);
+  Shape s = shape_of(team, 5, D, elt, ring_budget(team, kBackwardThreads), team >= 640 ? 3 : 0);
+  if (s.teams > 1) s.smem = std::max(s.smem, kSums * D * 4);
+  return s;
+}
 static int backward_ctas(int D, int elt, int64_t N) {
-  const Shape s = shape_of(backward_team(D), 5, D, elt, kBackwardBudget, 1);
-  const int per_sm = s.threads >= 256 ? 1 : 2;
-  return (int)std::min<int64_t>((N + s.teams - 1) / s.teams, (int64_t)sm_count() * per_sm);
+  const Shape s = backward_shape(D, elt);
+  return (int)std::min<int64_t>((N + s.teams - 1) / s.teams, (int64_t)sm_count() * ctas_per_sm(s, kBackwardThreads));
 }
 
-constexpr int kMaxSmem = 225 * 1024;
 template <auto Kernel>
 static int launch(const Params& p, const Shape& s, int ctas, cudaStream_t st, const char* name) {
   static std::once_flag once[64];
@@ -701,36 +948,56 @@ static int launch(const Params& p, const Shape& s, int ctas, cudaStream_t st, co
 
 template <typename T>
 static int forward(Params& p, cudaStream_t st) {
-  const int team = forward_team(p.D);
-  const Shape s = shape_of(team, 3, p.D, (int)sizeof(T), 72 * 1024, 2);
+  // Sixteen values a thread: a row's fixed instructions (copies, waits, sums) fall to half the warps, and two rows
+  // fit an SM where eight values leave room for one (50 M bf16 values on a B200, layer norms, sixteen against
+  // eight a thread: 512 wide 94 / 146 us, 1024 119 / 151, 2048 119 / 174, 4096 133 / 185, 8192 145 / 195).  Just
+  // above 4096 the 512 threads of such a team would be used to two thirds, and eight values are ahead (5000
+  // wide: 229 / 180).
+  const bool two = p.D > 256 && (p.D <= 4096 || p.D > 5120);
+  const int team = two ? team_of((p.D + 1) / 2) : team_of(p.D);
+  const Shape s = shape_of(team, 3, p.D, (int)sizeof(T), ring_budget(team, kForwardThreads), 0);
   p.stages = s.stages;
   p.row_bytes = s.row_bytes;
-  const int64_t ctas = std::min<int64_t>((p.N + s.teams - 1) / s.teams, (int64_t)sm_count() * (s.smem > 110 * 1024 ? 1 : 3));
+  p.table_at = s.table_at;
+  const int ctas = (int)std::min<int64_t>((p.N + s.teams - 1) / s.teams, (int64_t)sm_count() * ctas_per_sm(s, kForwardThreads));
   const char* name = "sandwich_kernel launch";
-  if (team == 32) {
-    if (p.D <= 256) return launch<sandwich_kernel<T, 32, 1>>(p, s, (int)ctas, st, name);
-    if (p.D <= 512) return launch<sandwich_kernel<T, 32, 2>>(p, s, (int)ctas, st, name);
-    return launch<sandwich_kernel<T, 32, 4>>(p, s, (int)ctas, st, name);
+  if (two) {
+    switch (team) {
+      case 32: return launch<sandwich_kernel<T, 32, 2, true>>(p, s, ctas, st, name);
+      case 64: return launch<sandwich_kernel<T, 64, 2, true>>(p, s, ctas, st, name);
+      case 128: return launch<sandwich_kernel<T, 128, 2, true>>(p, s, ctas, st, name);
+      case 256: return launch<sandwich_kernel<T, 256, 2, true>>(p, s, ctas, st, name);
+      default: return launch<sandwich_kernel<T, 512, 2, true>>(p, s, ctas, st, name);
+    }
   }
-  if (team == 128) return launch<sandwich_kernel<T, 128, 2>>(p, s, (int)ctas, st, name);
-  if (team == 256) return launch<sandwich_kernel<T, 256, 2>>(p, s, (int)ctas, st, name);
-  return launch<sandwich_kernel<T, 512, 2>>(p, s, (int)ctas, st, name);
+  switch (team) {
+    case 32: return launch<sandwich_kernel<T, 32, 1, true>>(p, s, ctas, st, name);
+    case 64: return launch<sandwich_kernel<T, 64, 1, true>>(p, s, ctas, st, name);
+    case 128: return launch<sandwich_kernel<T, 128, 1, true>>(p, s, ctas, st, name);
+    case 256: return launch<sandwich_kernel<T, 256, 1, true>>(p, s, ctas, st, name);
+    case 512: return launch<sandwich_kernel<T, 512, 1, true>>(p, s, ctas, st, name);
+    case 640: return launch<sandwich_kernel<T, 640, 1, true>>(p, s, ctas, st, name);
+    default: return launch<sandwich_kernel<T, 1024, 1, true>>(p, s, ctas, st, name);
+  }
 }
 
 template <typename T, bool LEAN>
 static int backward(Params& p, cudaStream_t st) {
-  const int team = backward_team(p.D);
-  Shape s = shape_of(team, 5, p.D, (int)sizeof(T), kBackwardBudget, 1);
+  const Shape s = backward_shape(p.D, (int)sizeof(T));
   p.stages = s.stages;
   p.row_bytes = s.row_bytes;
-  if (s.teams > 1) s.smem = std::max(s.smem, kSums * p.D * 4);
+  p.table_at = s.table_at;
   const int ctas = backward_ctas(p.D, (int)sizeof(T), p.N);
   const char* name = "sandwich_backward_kernel launch";
-  if (team == 32) return launch<sandwich_backward_kernel<T, 32, 2, LEAN>>(p, s, ctas, st, name);
-  if (p.D <= 1024) return launch<sandwich_backward_kernel<T, 128, 1, LEAN>>(p, s, ctas, st, name);
-  if (team == 128) return launch<sandwich_backward_kernel<T, 128, 2, LEAN>>(p, s, ctas, st, name);
-  if (team == 256) return launch<sandwich_backward_kernel<T, 256, 2, LEAN>>(p, s, ctas, st, name);
-  return launch<sandwich_backward_kernel<T, 512, 2, LEAN>>(p, s, ctas, st, name);
+  switch (team_of(p.D)) {
+    case 32: return launch<sandwich_backward_kernel<T, 32, 1, true, LEAN>>(p, s, ctas, st, name);
+    case 64: return launch<sandwich_backward_kernel<T, 64, 1, true, LEAN>>(p, s, ctas, st, name);
+    case 128: return launch<sandwich_backward_kernel<T, 128, 1, true, LEAN>>(p, s, ctas, st, name);
+    case 256: return launch<sandwich_backward_kernel<T, 256, 1, true, LEAN>>(p, s, ctas, st, name);
+    case 512: return launch<sandwich_backward_kernel<T, 512, 1, true, LEAN>>(p, s, ctas, st, name);
+    case 640: return launch<sandwich_backward_kernel<T, 640, 1, false, LEAN>>(p, s, ctas, st, name);
+    default: return launch<sandwich_backward_kernel<T, 1024, 1, false, LEAN>>(p, s, ctas, st, name);
+  }
 }
 
 static bool is_float(int dt) { return dt == RB_F32 || dt == RB_BF16 || dt == RB_F16; }
@@ -778,8 +1045,14 @@ extern "C" int rb_sandwich_norm(const void* x, int64_t ldx, const void* h, int64
   if (N == 0) return RB_OK;
   const int elt = dtype_size(dtype);
   Params p{};
-  p.x = x;
-  p.h = h;
+  const void* gates = gate_kind == kGateFull ? gate : nullptr;
+  const void* src[3] = {x, h, gates};
+  const int64_t ld[3] = {ldx, ldh, ldg};
+  for (int a = 0; a < 3; ++a) {
+    p.src[a] = src[a];
+    p.pitch[a] = ld[a] * elt;
+    p.arrays += src[a] != nullptr;
+  }
   p.gate = gate;
   p.w1 = w1;
   p.b1 = b1;
@@ -789,8 +1062,6 @@ extern "C" int rb_sandwich_norm(const void* x, int64_t ldx, const void* h, int64
   p.out1 = z;
   p.stats = stats;
   p.N = N;
-  p.ldx = ldx;
-  p.ldh = ldh;
   p.ldg = ldg;
   p.eps1 = eps1;
   p.eps2 = eps2;
@@ -816,12 +1087,12 @@ extern "C" int64_t rb_sandwich_norm_workspace_size(int64_t N, int D, int dtype) 
 }
 
 extern "C" int rb_sandwich_norm_backward(const void* dy, int64_t ldy, const void* dz, int64_t ldz, const void* x, int64_t ldx,
-                                         const void* h, int64_t ldh, const float* stats, int dtype, int64_t N, int D,
-                                         int post, const void* w1, const void* b1, int w1_dtype, int gate_kind,
-                                         const void* gate, int gate_dtype, int64_t ldg, int gate_act, float scale, int pre,
-                                         const void* w2, const void* b2, int w2_dtype, void* workspace,
-                                         int64_t workspace_bytes, void* dx, void* dh, void* dgate, void* dw1, void* db1,
-                                         void* dw2, void* db2, void* stream) {
+                                   const void* h, int64_t ldh, const float* stats, int dtype, int64_t N, int D,
+                                   int post, const void* w1, const void* b1, int w1_dtype, int gate_kind,
+                                   const void* gate, int gate_dtype, int64_t ldg, int gate_act, float scale, int pre,
+                                   const void* w2, const void* b2, int w2_dtype, void* workspace,
+                                   int64_t workspace_bytes, void* dx, void* dh, void* dgate, void* dw1, void* db1,
+                                   void* dw2, void* db2, void* stream) {
   using namespace rb::bnorm;
   int rc = check(dtype, N, D, post, pre, gate_kind, gate_act, w1, b1, w1_dtype, w2, b2, w2_dtype, gate, gate_dtype);
   if (rc) return rc;
@@ -839,11 +1110,15 @@ extern "C" int rb_sandwich_norm_backward(const void* dy, int64_t ldy, const void
   if (!device_is_sm100()) return fail(RB_ERR_DEVICE, "rb_sandwich_norm_backward needs an sm_100 (B200) device");
   const int elt = dtype_size(dtype);
   Params p{};
-  p.x = x;
-  p.h = h;
+  const void* gates = gate_kind == kGateFull ? gate : nullptr;
+  const void* src[5] = {x, h, dy, dz, gates};
+  const int64_t ld[5] = {ldx, ldh, ldy, ldz, ldg};
+  for (int a = 0; a < 5; ++a) {
+    p.src[a] = src[a];
+    p.pitch[a] = ld[a] * elt;
+    p.arrays += src[a] != nullptr;
+  }
   p.gate = gate;
-  p.dy = dy;
-  p.dz = dz;
   p.w1 = w1;
   p.b1 = b1;
   p.w2 = w2;
@@ -854,11 +1129,7 @@ extern "C" int rb_sandwich_norm_backward(const void* dy, int64_t ldy, const void
   p.stats = const_cast<float*>(stats);
   p.partial = static_cast<float*>(workspace);
   p.N = N;
-  p.ldx = ldx;
-  p.ldh = ldh;
   p.ldg = ldg;
-  p.ldy = ldy;
-  p.ldz = ldz;
   p.scale = scale;
   p.D = D;
   p.post = post;
@@ -871,18 +1142,11 @@ extern "C" int rb_sandwich_norm_backward(const void* dy, int64_t ldy, const void
   p.bulk = rows_fit(x, ldx, D, elt) && rows_fit(h, ldh, D, elt) && rows_fit(dy, ldy, D, elt) && rows_fit(dz, ldz, D, elt) &&
            rows_fit(dx, D, D, elt) && rows_fit(dh, D, D, elt) &&
            (gate_kind != kGateFull || (rows_fit(gate, ldg, D, elt) && rows_fit(dgate, D, D, elt)));
-  SumOut o{};
-  const int gdt = gate_dtype;
-  void* outs[kSums] = {dw1, db1, dw2, db2, gate_kind == kGateChannel ? dgate : nullptr};
-  const int dts[kSums] = {w1_dtype, w1_dtype, w2_dtype, w2_dtype, gdt};
-  for (int s = 0; s < kSums; ++s) {
-    o.out[s] = outs[s];
-    o.dtype[s] = dts[s];
-    p.need_sums |= outs[s] != nullptr;
-  }
+  SumOut o{dw1, db1, dw2, db2, gate_kind == kGateChannel ? dgate : nullptr};
+  p.need_sums = o.dw1 != nullptr || o.db1 != nullptr || o.dw2 != nullptr || o.db2 != nullptr || o.dgate != nullptr;
   cudaStream_t st = (cudaStream_t)stream;
+  const bool lean = o.db1 == nullptr && o.db2 == nullptr && o.dgate == nullptr;
   if (N > 0) {
-    const bool lean = outs[1] == nullptr && outs[3] == nullptr && outs[4] == nullptr;
     if (dtype == RB_BF16) rc = lean ? backward<__nv_bfloat16, true>(p, st) : backward<__nv_bfloat16, false>(p, st);
     else if (dtype == RB_F16) rc = lean ? backward<__half, true>(p, st) : backward<__half, false>(p, st);
     else rc = lean ? backward<float, true>(p, st) : backward<float, false>(p, st);
@@ -890,6 +1154,6 @@ extern "C" int rb_sandwich_norm_backward(const void* dy, int64_t ldy, const void
   }
   if (!p.need_sums) return RB_OK;
   const int ctas = N > 0 ? backward_ctas(D, elt, N) : 0;  // no rows: sums of nothing
-  column_sums_kernel<<<dim3((unsigned)((D + 31) / 32), kSums), 256, 0, st>>>(p.partial, ctas, D, o);
+  column_sums_kernel<<<(unsigned)((D + 7) / 8), 8 * kSumRuns, 0, st>>>(p, ctas, lean ? 2 : kSums, o);
   return check_cuda(cudaGetLastError(), "column_sums_kernel launch");
 }
