@@ -71,6 +71,9 @@ SIGNATURES = {
     "rb_sandwich_norm_backward": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _i32,
                                   _i32, _vp, _i32, _i64, _i32, _f32, _i32, _vp, _vp, _i32, _vp, _i64, _vp, _vp, _vp, _vp,
                                   _vp, _vp, _vp, _vp],
+    "rb_low_rank_workspace_size": [_i64, _i32, _i32, _i32],
+    "rb_low_rank_add": [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp, _i64,
+                        _vp, _i64, _vp],
     "rb_rep_gather_pool_scatter": [_vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _i32, _i64,
                                    _i64, _vp],
     "rb_ipc_export": [_vp, _vp, _vp],
@@ -82,7 +85,8 @@ SIGNATURES = {
     "rb_version": [],
 }
 
-RETURNS_I64 = {"rb_w8a8_gemm_workspace_size", "rb_smoe_workspace_size", "rb_sandwich_norm_workspace_size"}
+RETURNS_I64 = {"rb_w8a8_gemm_workspace_size", "rb_smoe_workspace_size", "rb_sandwich_norm_workspace_size",
+               "rb_low_rank_workspace_size"}
 
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None

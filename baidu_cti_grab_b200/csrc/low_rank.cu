@@ -1,0 +1,712 @@
+// low_rank.cu -- low-rank adapters of many requests beside a projection that they
+// share: out[t] = y[t] + scale[i] * B_i (A_i x[t]) for token t's adapter i = idx[t]
+// (y is the shared projection's output; a token without an adapter keeps y).
+//
+// Three kernels, by the sizes:
+//
+// * token kernel: a cluster of CTAs per token, CUDA cores.  Few tokens are bound by
+//   the latency of reading their adapters: the CTAs of a cluster split A's columns,
+//   share the partial h = A x through distributed shared memory and split B's rows.
+//   Also takes every shape that the tensor maps cannot.
+// * tile kernel: 128 tokens a CTA on tcgen05.  The tile's distinct adapters are
+//   listed, and taken in groups whose padded ranks fill 64 columns:
+//     H [128, 64] = X [128, K] . [A_i ; A_j ; ...]^T   all of the group in one MMA per K step
+//     each row keeps its own adapter's columns, the others become zeros
+//     out tile = H . [B_i | B_j | ...]^T               the zeros select the adapter
+//   so tokens need no sorting and a tile of mixed requests costs MMA work (of which
+//   there is plenty), not bytes.  A row is written in the group that has its adapter.
+// * the same split in two, H then out, when 128-token tiles are too few to fill the
+//   GPU: H is split along K (fp32 partials in the workspace, summed in a fixed
+//   order), out along N.
+//
+// What bounds it: HBM from about 20k tokens (x and y read, out written once), the
+// two GEMMs being 2 r (K + N) operations a token.  h is rounded to the model type
+// before the second product (its operand on the tensor cores), as it is where the
+// two products are separate operations; sums are fp32, out is rounded once.
+#include "common.cuh"
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
+namespace rb {
+namespace lowrank {
+
+constexpr unsigned kAll = 0xffffffffu;
+constexpr int kMaxRank = 128;
+
+struct Params {
+  const void *y, *x, *a, *b, *idx;
+  const float* scale;  // [R] or null
+  void* out;
+  float* part;         // [splits][T][rank] partial h, or null
+  int64_t ldy, ldx, ldo, T;
+  int K, N, R, rank, idx64;
+  int rp, group;       // rank padded to 16, 32 or 64; adapters of a group
+  int splits;          // of K (H alone) -- partials to sum (out alone)
+  int chunks;          // 64-column chunks of a CTA (out alone)
+  int vec_y, vec_out;  // bytes of the loads and stores that rows allow: 32, 16 or 2
+};
+
+__device__ __forceinline__ int adapter_of(const Params& p, int64_t t) {
+  if (t >= p.T) return -1;
+  const int64_t i = p.idx64 ? __ldg(static_cast<const int64_t*>(p.idx) + t)
+                            : (int64_t)__ldg(static_cast<const int32_t*>(p.idx) + t);
+  return i >= 0 && i < p.R ? (int)i : -1;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) { return (float)v; }
+
+// eight 16-bit values times eight others, added up
+template <typename T>
+__device__ __forceinline__ float dot8(uint4 a, uint4 b, float s) {
+  const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      s = fmaf(bf16_lo(aw[i]), bf16_lo(bw[i]), s);
+      s = fmaf(bf16_hi(aw[i]), bf16_hi(bw[i]), s);
+    } else {
+      const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&aw[i]));
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&bw[i]));
+      s = fmaf(u.x, v.x, s);
+      s = fmaf(u.y, v.y, s);
+    }
+  }
+  return s;
+}
+
+// ------------------------------------------------------------ token kernel
+constexpr int kTokenThreads = 256;
+
+// VEC: 16-byte loads of x, A and B (K and rank multiples of 8, aligned bases and rows).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kTokenThreads) token_kernel(const __grid_constant__ Params p) {
+  __shared__ float s_part[kMaxRank], s_h[kMaxRank];
+  const uint32_t rank = tc::pair::cluster_rank();
+  uint32_t size;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+  const int64_t t = blockIdx.x / size;
+  const int i = adapter_of(p, t);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T* x = static_cast<const T*>(p.x) + t * p.ldx;
+  const T* y = static_cast<const T*>(p.y) + t * p.ldy;
+  T* out = static_cast<T*>(p.out) + t * p.ldo;
+  const int n0 = (int)((int64_t)p.N * rank / size), n1 = (int)((int64_t)p.N * (rank + 1) / size);
+  if (i < 0) {  // the whole cluster alike
+    if (out != y)
+      for (int n = n0 + threadIdx.x; n < n1; n += kTokenThreads) out[n] = y[n];
+    return;
+  }
+  // this CTA's part of h: eights of K from k0 to k1, a warp for each rank in turn
+  const T* a = static_cast<const T*>(p.a) + (int64_t)i * p.rank * p.K;
+  const int eights = (p.K + 7) / 8;
+  const int k0 = (int)((int64_t)eights * rank / size) * 8;
+  const int k1 = min(p.K, (int)((int64_t)eights * (rank + 1) / size) * 8);
+  for (int j = warp; j < p.rank; j += kTokenThreads / 32) {
+    const T* row = a + (int64_t)j * p.K;
+    float s = 0.0f;
+    if constexpr (VEC) {
+#pragma unroll 4
+      for (int k = k0 + lane * 8; k < k1; k += 256)
+        s = dot8<T>(__ldg(reinterpret_cast<const uint4*>(row + k)), __ldg(reinterpret_cast<const uint4*>(x + k)), s);
+    } else {
+      for (int k = k0 + lane; k < k1; k += 32) s = fmaf(to_f32(row[k]), to_f32(x[k]), s);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
+    if (lane == 0) s_part[j] = s;
+  }
+  if (size > 1) {
+    tc::pair::cluster_sync_all();
+    for (int j = threadIdx.x; j < p.rank; j += kTokenThreads) {
+      float s = 0.0f;
+      for (uint32_t c = 0; c < size; ++c) {
+        float v;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(tc::pair::map_rank(smem_u32(&s_part[j]), c)) : "memory");
+        s += v;
+      }
+      s_h[j] = s;
+    }
+    tc::pair::cluster_sync_all();  // no CTA leaves while another may read its part
+  } else {
+    __syncthreads();
+    for (int j = threadIdx.x; j < p.rank; j += kTokenThreads) s_h[j] = s_part[j];
+    __syncthreads();
+  }
+  const float w = p.scale != nullptr ? __ldg(p.scale + i) : 1.0f;
+  const T* b = static_cast<const T*>(p.b) + (int64_t)i * p.N * p.rank;
+  for (int n = n0 + threadIdx.x; n < n1; n += kTokenThreads) {
+    const T* row = b + (int64_t)n * p.rank;
+    const float base = to_f32(y[n]);
+    float s = 0.0f;
+    if constexpr (VEC) {
+      for (int j = 0; j < p.rank; j += 8) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + j));
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s = fmaf(to_f32(e[q]), s_h[j + q], s);
+      }
+    } else {
+      for (int j = 0; j < p.rank; ++j) s = fmaf(to_f32(row[j]), s_h[j], s);
+    }
+    out[n] = T(fmaf(w, s, base));
+  }
+}
+
+// ------------------------------------------------------------- tile kernel
+constexpr int kRows = 128;        // tokens of a tile
+constexpr int kCols = 64;         // columns of H: a group's padded ranks
+constexpr int kChunk = 64;        // columns of an out chunk
+constexpr int kStages = 3;        // ring of X and A blocks of 64 columns of K
+constexpr int kXBytes = kRows * 128, kABytes = kCols * 128, kStageBytes = kXBytes + kABytes;
+constexpr int kHBytes = kRows * 128;
+constexpr int kBBytes = kChunk * kCols * 2;
+constexpr int kTileSmem = 1024 + kStages * kStageBytes + kHBytes + 2 * kBBytes;
+constexpr int kTmemCols = 256;    // H at column 0, two out chunks at 64 and 128
+constexpr int kTileThreads = 192; // TMA warp, MMA warp, four warps of rows
+
+enum Mode : int { kFused = 0, kHOnly = 1, kOutOnly = 2 };
+
+// K-major operand rows of 32, 64 or 128 bytes under the swizzle of that width, in groups of eight rows
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, int row_bytes) {
+  const uint64_t layout = row_bytes == 128 ? 2 : row_bytes == 64 ? 4 : 6;
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(8 * row_bytes >> 4) << 32) |
+         ((uint64_t)1 << 46) | (layout << 61);
+}
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return pack_bf16x2(lo, hi);
+  else return pack_f16x2(lo, hi);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(bf16_lo(w), bf16_hi(w));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// sixteen values of a row from column c on (0 beyond N) as they lie in memory, and back
+template <typename T>
+__device__ __forceinline__ void load16(const T* row, int c, int N, int vec, uint32_t* w) {
+  if (c + 16 <= N && vec >= 16) {
+    if (vec == 32) {
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "l"(row + c));
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(row + c), b = *reinterpret_cast<const uint4*>(row + c + 8);
+      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+      w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    }
+    return;
+  }
+  const uint16_t* u = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t lo = c + 2 * i < N ? u[c + 2 * i] : 0u, hi = c + 2 * i + 1 < N ? u[c + 2 * i + 1] : 0u;
+    w[i] = lo | (hi << 16);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store16(T* row, int c, int N, int vec, const uint32_t* w) {
+  if (c + 16 <= N && vec >= 16) {
+    if (vec == 32) {
+      stg_v8(row + c, w);
+    } else {
+      *reinterpret_cast<uint4*>(row + c) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(row + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+    return;
+  }
+  uint16_t* u = reinterpret_cast<uint16_t*>(row);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (c + 2 * i < N) u[c + 2 * i] = (uint16_t)w[i];
+    if (c + 2 * i + 1 < N) u[c + 2 * i + 1] = (uint16_t)(w[i] >> 16);
+  }
+}
+
+// grid: x = tiles of 128 tokens; y = splits of K (H alone) or of N (out alone)
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kTileThreads, 2)
+    tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA,
+                const __grid_constant__ CUtensorMap tmB, const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sX = smem;
+  uint8_t* sA = sX + kStages * kXBytes;
+  uint8_t* sH = sA + kStages * kABytes;
+  uint8_t* sB = sH + kHBytes;
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], hfull, hready, bfull[2], bempty[2], dfull[2], dempty[2], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word, s_count;
+  __shared__ int s_list[kRows], s_slot[kRows];
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row0 = (int64_t)blockIdx.x * kRows;
+  constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+  constexpr uint32_t kIdesc = (1u << 4) | kType | ((uint32_t)(kRows >> 4) << 24);  // N is added where it is known
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(&hfull), 1);
+    mbar_init(smem_u32(&hready), 128);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(smem_u32(&bfull[s]), 1);
+      mbar_init(smem_u32(&bempty[s]), 1);
+      mbar_init(smem_u32(&dfull[s]), 1);
+      mbar_init(smem_u32(&dempty[s]), 128);
+    }
+    mbar_init(smem_u32(&done), 1);
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmA)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmB)) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == 2) {
+    // the tile's distinct adapters in the order of their first row, and each row's place among them
+    int count = 0;
+    for (int c = 0; c < kRows / 32; ++c) {
+      const int i = adapter_of(p, row0 + c * 32 + lane);
+      const unsigned peers = __match_any_sync(kAll, i);
+      const int leader = __ffs(peers) - 1;
+      int at = -1;
+      if (i >= 0 && lane == leader)
+        for (int q = 0; q < count && at < 0; ++q)
+          if (s_list[q] == i) at = q;
+      const unsigned fresh = __ballot_sync(kAll, i >= 0 && lane == leader && at < 0);
+      if (fresh >> lane & 1) {
+        at = count + __popc(fresh & ((1u << lane) - 1u));
+        s_list[at] = i;
+      }
+      count += __popc(fresh);
+      s_slot[c * 32 + lane] = __shfl_sync(kAll, at, leader);  // -1 for rows without an adapter
+      __syncwarp();
+    }
+    if (lane == 0) s_count = count;
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int count = s_count;
+  const int groups = (count + p.group - 1) / p.group;
+  const int kblocks = (p.K + 63) / 64;
+  const int split = MODE == kFused ? 0 : (int)blockIdx.y;
+  const int kb0 = MODE == kHOnly ? (int)((int64_t)kblocks * split / p.splits) : 0;
+  const int kb1 = MODE == kHOnly ? (int)((int64_t)kblocks * (split + 1) / p.splits) : kblocks;
+  const int all_chunks = (p.N + kChunk - 1) / kChunk;
+  const int ch0 = MODE == kOutOnly ? split * p.chunks : 0;
+  const int ch1 = MODE == kOutOnly ? min(all_chunks, ch0 + p.chunks) : all_chunks;
+  const int row_bytes = p.rp * 2;          // of a B operand row
+  const int b_slot = kChunk * row_bytes;   // of an adapter's B chunk
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------------------------------------------------- producer
+      const uint64_t once = tc::policy_evict_first(), keep = tc::policy_evict_last();
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, bphase = 0;
+      uint32_t issued = 0, issued_phase = 0;  // bits: ring stages, then the two B buffers
+      bool ok = true;
+      for (int g = 0; g < groups && ok; ++g) {
+        const int first = g * p.group, n = min(p.group, count - first);
+        if constexpr (MODE != kOutOnly) {
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait_bounded(smem_u32(&empty[stage]), phase ^ 1, kWaitTimeoutProducer, abort_flag)) {
+              ok = false;
+              break;
+            }
+            const uint32_t fb = smem_u32(&full[stage]);
+            mbar_arrive_expect_tx(fb, kXBytes + n * p.rp * 128);
+            tc::tma_load_2d(smem_u32(sX + stage * kXBytes), &tmX, kb * 64, (int)row0, fb, groups > 1 ? keep : once);
+            for (int j = 0; j < n; ++j)
+              tc::tma_load_2d(smem_u32(sA + stage * kABytes + j * p.rp * 128), &tmA, kb * 64, s_list[first + j] * p.rank, fb, keep);
+            issued |= 1u << stage;
+            issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+        }
+        if constexpr (MODE != kHOnly) {
+          for (int ch = ch0; ch < ch1 && ok; ++ch) {
+            if (!mbar_wait_bounded(smem_u32(&bempty[buf]), bphase ^ 1, kWaitTimeoutProducer, abort_flag)) {
+              ok = false;
+              break;
+            }
+            const uint32_t fb = smem_u32(&bfull[buf]);
+            mbar_arrive_expect_tx(fb, n * b_slot);
+            for (int j = 0; j < n; ++j)
+              tc::tma_load_2d(smem_u32(sB + buf * kBBytes + j * b_slot), &tmB, 0, s_list[first + j] * p.N + ch * kChunk, fb, keep);
+            issued |= 1u << (kStages + buf);
+            issued_phase = (issued_phase & ~(1u << (kStages + buf))) | (bphase << (kStages + buf));
+            buf ^= 1;
+            if (buf == 0) bphase ^= 1;
+          }
+        }
+      }
+      // never leave a copy in flight behind an exiting CTA
+      for (int s = 0; s < kStages + 2; ++s)
+        if (issued >> s & 1)
+          mbar_wait_bounded(smem_u32(s < kStages ? &full[s] : &bfull[s - kStages]), (issued_phase >> s) & 1u,
+                            kWaitTimeoutProducer, nullptr);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // --------------------------------------------------------------- MMA
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, bphase = 0;
+      bool ok = true;
+      for (int g = 0; g < groups && ok; ++g) {
+        const int n = min(p.group, count - g * p.group);
+        if constexpr (MODE != kOutOnly) {
+          const uint32_t idesc = kIdesc | ((uint32_t)(n * p.rp >> 3) << 17);
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait_bounded(smem_u32(&full[stage]), phase, kWaitTimeoutMma, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc::tc_fence_after();
+            const uint64_t xd = operand_desc(smem_u32(sX + stage * kXBytes), 128);
+            const uint64_t ad = operand_desc(smem_u32(sA + stage * kABytes), 128);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) umma_f16(tmem, xd + 2 * s, ad + 2 * s, idesc, (kb > kb0 || s > 0) ? 1u : 0u);
+            tc::umma_commit(smem_u32(&empty[stage]));
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+          if (!ok) break;
+          tc::umma_commit(smem_u32(&hfull));
+        }
+        // the rows' warps have H in shared memory (and are done with its TMEM columns)
+        if (!mbar_wait_bounded(smem_u32(&hready), g & 1, kWaitTimeoutMma, abort_flag)) break;
+        if constexpr (MODE != kHOnly) {
+          tc::tc_fence_after();
+          const uint32_t idesc = kIdesc | ((uint32_t)(kChunk >> 3) << 17);
+          const uint64_t hd = operand_desc(smem_u32(sH), 128);
+          for (int ch = ch0; ch < ch1; ++ch) {
+            if (!mbar_wait_bounded(smem_u32(&bfull[buf]), bphase, kWaitTimeoutMma, abort_flag) ||
+                !mbar_wait_bounded(smem_u32(&dempty[buf]), bphase ^ 1, kWaitTimeoutMma, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc::tc_fence_after();
+            for (int j = 0; j < n; ++j) {
+              const uint64_t bd = operand_desc(smem_u32(sB + buf * kBBytes + j * b_slot), row_bytes);
+              for (int s = 0; s < p.rp / 16; ++s)
+                umma_f16(tmem + kCols + buf * kChunk, hd + 2 * (j * (p.rp / 16) + s), bd + 2 * s, idesc, (j > 0 || s > 0) ? 1u : 0u);
+            }
+            tc::umma_commit(smem_u32(&bempty[buf]));
+            tc::umma_commit(smem_u32(&dfull[buf]));
+            buf ^= 1;
+            if (buf == 0) bphase ^= 1;
+          }
+        }
+      }
+      tc::umma_commit(smem_u32(&done));
+      mbar_wait_bounded(smem_u32(&done), 0, kWaitTimeoutMma, nullptr);
+    }
+  } else {
+    // ----------------------------------------------------------- the rows
+    const int quarter = warp & 3;  // the TMEM lanes that this warp can read
+    const int r = quarter * 32 + lane;
+    const int64_t row = row0 + r;
+    const bool live = row < p.T;
+    const int slot = s_slot[r];
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const float w = MODE != kHOnly && slot >= 0 && p.scale != nullptr ? __ldg(p.scale + s_list[slot]) : 1.0f;
+    const T* y = static_cast<const T*>(p.y) + row * p.ldy;
+    T* out = static_cast<T*>(p.out) + row * p.ldo;
+    int buf = 0;
+    uint32_t bphase = 0;
+    bool ok = true;
+    if (MODE != kHOnly && live && slot < 0 && out != y) {
+      for (int c = ch0 * kChunk; c < min(p.N, ch1 * kChunk); c += 16) {
+        uint32_t v[8];
+        load16(y, c, p.N, p.vec_y, v);
+        store16(out, c, p.N, p.vec_out, v);
+      }
+    }
+    for (int g = 0; g < groups && ok; ++g) {
+      const int first = g * p.group, n = min(p.group, count - first);
+      const int mine = slot >= first && slot < first + n ? slot - first : -1;
+      if constexpr (MODE != kOutOnly) {
+        if (!mbar_wait_bounded(smem_u32(&hfull), g & 1, kWaitTimeoutEpilogue, abort_flag)) break;
+        tc::tc_fence_after();
+      }
+      // own adapter's h into this row of the H tile, zeros into the others' columns (and the rank's padding)
+      for (int j = 0; j < n; ++j) {
+        for (int c = 0; c < p.rp; c += 16) {
+          uint32_t v[16];
+          if constexpr (MODE == kOutOnly) {
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+              float s = 0.0f;
+              if (mine == j && c + q < p.rank)
+                for (int k = 0; k < p.splits; ++k) s += p.part[((int64_t)k * p.T + row) * p.rank + c + q];
+              v[q] = __float_as_uint(s);
+            }
+          } else {
+            __syncwarp();
+            tc::swp::tmem_ld16(tmem + lanes + (uint32_t)(j * p.rp + c), v);
+          }
+          if constexpr (MODE == kHOnly) {
+            if (mine == j) {
+              float* to = p.part + ((int64_t)split * p.T + row) * p.rank + c;
+#pragma unroll
+              for (int q = 0; q < 16; q += 4)
+                if (c + q < p.rank)
+                  *reinterpret_cast<float4*>(to + q) = make_float4(__uint_as_float(v[q]), __uint_as_float(v[q + 1]),
+                                                                   __uint_as_float(v[q + 2]), __uint_as_float(v[q + 3]));
+            }
+          } else {
+            uint32_t h[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const bool in = mine == j && c + 2 * q < p.rank;  // the rank is even
+              h[q] = in ? pack2<T>(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])) : 0u;
+            }
+            const int piece = (j * p.rp + c) / 8;  // 16-byte pieces of the row, swizzled by the row's place in its eight
+            *reinterpret_cast<uint4*>(sH + r * 128 + ((piece ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(sH + r * 128 + (((piece + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+          }
+        }
+      }
+      tc::tc_fence_before();
+      if constexpr (MODE != kHOnly) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(smem_u32(&hready));
+      if constexpr (MODE != kHOnly) {
+        for (int ch = ch0; ch < ch1; ++ch) {
+          const int c0 = ch * kChunk;
+          uint32_t base[kChunk / 2];
+          if (mine >= 0) {  // requested before the wait for the product
+#pragma unroll
+            for (int c = 0; c < kChunk; c += 16)
+              if (c0 + c < p.N) load16(y, c0 + c, p.N, p.vec_y, base + c / 2);
+          }
+          if (!mbar_wait_bounded(smem_u32(&dfull[buf]), bphase, kWaitTimeoutEpilogue, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < kChunk / 32; ++h) {
+            uint32_t v[32];
+            __syncwarp();
+            tc::tmem_ld32(tmem + lanes + (uint32_t)(kCols + buf * kChunk + h * 32), v);
+            if (h == kChunk / 32 - 1) {
+              tc::tc_fence_before();
+              mbar_arrive(smem_u32(&dempty[buf]));
+            }
+            if (mine < 0) continue;
+            uint32_t o[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+              const float2 f = unpack2<T>(base[h * 16 + q]);
+              o[q] = pack2<T>(fmaf(w, __uint_as_float(v[2 * q]), f.x), fmaf(w, __uint_as_float(v[2 * q + 1]), f.y));
+            }
+#pragma unroll
+            for (int c = 0; c < 32; c += 16)
+              if (c0 + h * 32 + c < p.N) store16(out, c0 + h * 32 + c, p.N, p.vec_out, o + c / 2);
+          }
+          buf ^= 1;
+          if (buf == 0) bphase ^= 1;
+        }
+      }
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------- host
+// how a call runs: tokens (no tile), one fused kernel, or H and out apart
+struct Plan {
+  int tiles;   // 0: the token kernel
+  int splits;  // 1: fused
+  int chunks;  // 64-column chunks of a CTA of the out kernel
+};
+constexpr int kTokenMax = 96;
+
+static Plan plan_of(int64_t T, int K, int N, int rank) {
+  Plan q{};
+  if (T <= kTokenMax || rank % 8 != 0 || rank > 64 || K % 8 != 0) return q;
+  const int64_t tiles = (T + kRows - 1) / kRows;
+  const int sms = sm_count();
+  q.tiles = (int)tiles;
+  q.splits = 1;
+  const int kblocks = (K + 63) / 64, chunks = (N + kChunk - 1) / kChunk;
+  q.chunks = chunks;
+  if (tiles * 2 <= sms) {  // two CTAs an SM are resident; below half of the SMs the two phases are spread
+    const int64_t want = (2 * sms + tiles - 1) / tiles;
+    q.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, (int64_t)(kblocks + 3) / 4, 16}));
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(want, chunks));
+    q.chunks = (int)((chunks + parts - 1) / parts);
+    if (q.splits == 1 && q.chunks == chunks) return q;
+    if (q.splits == 1) q.splits = -1;  // apart, without a split of K
+  }
+  return q;
+}
+
+static int make_map(CUtensorMap* tm, const void* base, int64_t inner, int64_t outer, int64_t ld_bytes, uint32_t box_inner,
+                    uint32_t box_outer, CUtensorMapDataType dt) {
+  auto enc = tc::encode_fn();
+  if (enc == nullptr) return fail(RB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+  cuuint64_t strides[1] = {(cuuint64_t)ld_bytes};
+  cuuint32_t box[2] = {box_inner, box_outer};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapSwizzle sw = box_inner == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : box_inner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                                                               : CU_TENSOR_MAP_SWIZZLE_32B;
+  CUresult r = enc(tm, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(RB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return RB_OK;
+}
+
+static int vec_bytes(const void* p, int64_t ld) {
+  for (int v : {32, 16})
+    if (aligned(p, v) && (ld * 2) % v == 0) return v;
+  return 2;
+}
+
+template <typename T>
+static int run_tokens(const Params& p, bool vec, cudaStream_t st) {
+  // CTAs of a token: enough for two an SM, and no more than its adapter's bytes are worth (16 KB each)
+  const int64_t bytes = (int64_t)p.rank * (p.K + p.N) * 2;
+  int c = 1;
+  while (c < 8 && p.T * c < 2 * sm_count() && bytes / (2 * c) >= 16 * 1024) c *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.T * c));
+  cfg.blockDim = dim3(kTokenThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)c;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = vec ? cudaLaunchKernelEx(&cfg, token_kernel<T, true>, p) : cudaLaunchKernelEx(&cfg, token_kernel<T, false>, p);
+  return check_cuda(e, "low-rank token_kernel launch");
+}
+
+template <typename T>
+static int run_tiles(Params& p, const Plan& q, CUtensorMapDataType dt, cudaStream_t st) {
+  static std::once_flag once[64];
+  int dev = 0, rc;
+  cudaGetDevice(&dev);
+  cudaError_t e = cudaSuccess;
+  std::call_once(once[dev & 63], [&] {
+    const void* fns[3] = {(const void*)tile_kernel<T, kFused>, (const void*)tile_kernel<T, kHOnly>, (const void*)tile_kernel<T, kOutOnly>};
+    for (const void* f : fns)
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem);
+  });
+  if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(low-rank tile_kernel)");
+  CUtensorMap tmX, tmA, tmB;
+  if ((rc = make_map(&tmX, p.x, p.K, p.T, p.ldx * 2, 64, kRows, dt))) return rc;
+  if ((rc = make_map(&tmA, p.a, p.K, (int64_t)p.R * p.rank, (int64_t)p.K * 2, 64, (uint32_t)p.rp, dt))) return rc;
+  if ((rc = make_map(&tmB, p.b, p.rank, (int64_t)p.R * p.N, (int64_t)p.rank * 2, (uint32_t)p.rp, kChunk, dt))) return rc;
+  if (q.splits == 1) {
+    tile_kernel<T, kFused><<<q.tiles, kTileThreads, kTileSmem, st>>>(tmX, tmA, tmB, p);
+    return check_cuda(cudaGetLastError(), "low-rank tile_kernel launch");
+  }
+  p.splits = std::max(1, q.splits);
+  p.chunks = q.chunks;
+  tile_kernel<T, kHOnly><<<dim3(q.tiles, p.splits), kTileThreads, kTileSmem, st>>>(tmX, tmA, tmB, p);
+  if ((rc = check_cuda(cudaGetLastError(), "low-rank tile_kernel launch (H)"))) return rc;
+  const int parts = ((p.N + kChunk - 1) / kChunk + p.chunks - 1) / p.chunks;
+  tile_kernel<T, kOutOnly><<<dim3(q.tiles, parts), kTileThreads, kTileSmem, st>>>(tmX, tmA, tmB, p);
+  return check_cuda(cudaGetLastError(), "low-rank tile_kernel launch (out)");
+}
+
+}  // namespace lowrank
+}  // namespace rb
+
+using namespace rb;
+
+extern "C" int64_t rb_low_rank_workspace_size(int64_t T, int K, int N, int rank) {
+  if (T < 0 || K <= 0 || N <= 0 || rank <= 0 || rank > lowrank::kMaxRank || T > 0x7fffffffLL) return -1;
+  const lowrank::Plan q = lowrank::plan_of(T, K, N, rank);
+  return q.tiles == 0 || q.splits == 1 ? 0 : (int64_t)std::max(1, q.splits) * T * rank * 4;
+}
+
+extern "C" int rb_low_rank_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int dtype, int64_t T, int K, int N,
+                               const void* a, const void* b, int R, int rank, const void* idx, int idx_dtype,
+                               const float* scale, void* workspace, int64_t workspace_bytes, void* out, int64_t ldo,
+                               void* stream) {
+  using namespace rb::lowrank;
+  if (T < 0 || K <= 0 || N <= 0 || R <= 0 || rank <= 0) return fail(RB_ERR_VALUE, "negative or empty adapter shape");
+  if (dtype != RB_BF16 && dtype != RB_F16) return fail(RB_ERR_UNSUPPORTED, "rb_low_rank_add takes bf16 or f16");
+  if (rank > kMaxRank) return fail(RB_ERR_UNSUPPORTED, "ranks above %d", kMaxRank);
+  if (idx_dtype != RB_I64 && idx_dtype != RB_I32) return fail(RB_ERR_VALUE, "adapter ids must be int64 or int32");
+  if (T > 0x7fffffffLL / 8 || (int64_t)R * N > 0x7fffffffLL || (int64_t)R * rank > 0x7fffffffLL)
+    return fail(RB_ERR_UNSUPPORTED, "more than 2^28 tokens, or than 2^31 rows of all adapters");
+  if (ldy < N || ldo < N || ldx < K) return fail(RB_ERR_VALUE, "leading dimension smaller than the row");
+  if (T > 0 && (y == nullptr || x == nullptr || a == nullptr || b == nullptr || idx == nullptr || out == nullptr))
+    return fail(RB_ERR_VALUE, "null operand");
+  Plan q = plan_of(T, K, N, rank);
+  const bool fit = aligned(x, 16) && (ldx * 2) % 16 == 0 && aligned(a, 16) && aligned(b, 16) && K % 8 == 0 && rank % 8 == 0;
+  if (!fit) q.tiles = 0;
+  const int64_t need = q.tiles == 0 ? 0 : rb_low_rank_workspace_size(T, K, N, rank);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(RB_ERR_VALUE, "workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need,
+                (long long)workspace_bytes);
+  if (!device_is_sm100()) return fail(RB_ERR_DEVICE, "rb_low_rank_add needs an sm_100 (B200) device");
+  if (T == 0) return RB_OK;
+  Params p{};
+  p.y = y;
+  p.x = x;
+  p.a = a;
+  p.b = b;
+  p.idx = idx;
+  p.scale = scale;
+  p.out = out;
+  p.part = static_cast<float*>(workspace);
+  p.ldy = ldy;
+  p.ldx = ldx;
+  p.ldo = ldo;
+  p.T = T;
+  p.K = K;
+  p.N = N;
+  p.R = R;
+  p.rank = rank;
+  p.idx64 = idx_dtype == RB_I64;
+  p.rp = rank <= 16 ? 16 : rank <= 32 ? 32 : 64;
+  p.group = kCols / p.rp;
+  p.splits = 1;
+  p.vec_y = vec_bytes(y, ldy);
+  p.vec_out = vec_bytes(out, ldo);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (q.tiles == 0)
+    return dtype == RB_BF16 ? run_tokens<__nv_bfloat16>(p, fit, st) : run_tokens<__half>(p, fit, st);
+  return dtype == RB_BF16 ? run_tiles<__nv_bfloat16>(p, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, st)
+                          : run_tiles<__half>(p, q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, st);
+}

@@ -7,4 +7,5 @@
 #include "moe.cu"
 #include "route.cu"
 #include "block_norm.cu"
+#include "low_rank.cu"
 #include "peer.cu"

@@ -706,6 +706,52 @@ def sandwich_norm_backward(grad_y: Optional[torch.Tensor], grad_z: Optional[torc
     return (dx, dh, *outs)
 
 
+# -------------------------------------------------------- low-rank adapters
+def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.Tensor,
+                 scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[t] + scale[i] * b[i] @ (a[i] @ x[t]) with i = adapter[t] (rb_low_rank_add): the adapters of many
+    requests beside the projection that gave y.
+
+    y [T, N] and x [T, K] bf16/f16; a [R, rank, K] and b [R, N, rank] contiguous in the same type, rank <= 128;
+    adapter int32/int64 [T], -1 (or anything outside [0, R)) for a token without one; scale fp32 [R].
+    ``out`` may be y.  Forward only: an input that asks for a gradient is refused."""
+    dev = require_cuda("low_rank_add", y, x, a, b, adapter, scale, out)
+    if y.dim() != 2 or x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
+        raise ValueError("low_rank_add expects y [T, N], x [T, K], a [R, rank, K] and b [R, N, rank]")
+    (T, N), (R, rank, K) = y.shape, a.shape
+    if tuple(x.shape) != (T, K) or tuple(b.shape) != (R, N, rank):
+        raise ValueError(f"x must be [{T}, {K}] and b [{R}, {N}, {rank}]")
+    if x.dtype not in (torch.bfloat16, torch.float16) or any(t.dtype != x.dtype for t in (y, a, b)):
+        raise ValueError("y, x, a and b must all be bf16 or all f16")
+    if tuple(adapter.shape) != (T,) or adapter.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"adapter must be int32 or int64 [{T}]")
+    if scale is not None and (tuple(scale.shape) != (R,) or scale.dtype != torch.float32):
+        raise ValueError(f"scale must be fp32 [{R}]")
+    if not a.is_contiguous() or not b.is_contiguous():
+        raise ValueError("a and b must be contiguous")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, x, a, b, scale)):
+        raise RuntimeError("low_rank_add has no backward: call it under torch.no_grad() or on detached tensors")
+    if out is None:
+        out = y.new_empty((T, N))
+    elif tuple(out.shape) != (T, N) or out.dtype != y.dtype or (N > 0 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N):
+        raise ValueError(f"out must be a row-major [{T}, {N}] {y.dtype} tensor")
+    if y.stride(1) != 1 or (T > 1 and y.stride(0) < N):
+        y = y.contiguous()
+    if x.stride(1) != 1 or (T > 1 and x.stride(0) < K):
+        x = x.contiguous()
+    adapter = adapter.contiguous()
+    scale = None if scale is None else scale.contiguous()
+    ws_bytes = int(L.load().rb_low_rank_workspace_size(T, K, N, rank))
+    if ws_bytes < 0:
+        raise ValueError("rb_low_rank_workspace_size rejected the shape")
+    ws = x.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+    _call_on(dev, "rb_low_rank_add", y.data_ptr(), max(y.stride(0), N), x.data_ptr(), max(x.stride(0), K), rb_dtype(x), T, K,
+             N, a.data_ptr(), b.data_ptr(), R, rank, adapter.data_ptr(),
+             L.RB_I64 if adapter.dtype == torch.int64 else L.RB_I32, _ptr(scale), _ptr(ws), ws_bytes, out.data_ptr(),
+             max(out.stride(0), N))
+    return out
+
+
 def device_error(reset: bool = False) -> int:
     return L.device_error(reset)
 

@@ -387,6 +387,29 @@ int rb_sandwich_norm_backward(const void* dy, int64_t ldy, const void* dz, int64
                               void* dgate, void* dpost_w, void* dpost_b, void* dpre_w, void* dpre_b,
                               void* stream);
 
+/*
+ * Low-rank adapters of many requests beside a projection that they share:
+ *   out[t] = y[t] + scale[i] * B_i (A_i x[t]),  i = idx[t]
+ *   y, out     [T, ldy], [T, ldo] RB_BF16 or RB_F16: the shared projection's output
+ *              and the sum; out may be y itself (same pointer and pitch)
+ *   x          [T, ldx], K values a row, the same type
+ *   a, b       [R, rank, K] and [R, N, rank] contiguous, the same type; rank <= 128
+ *   idx        [T] RB_I64 or RB_I32: each token's adapter, in any order; one outside
+ *              [0, R) (-1 by custom) means none: out[t] = y[t]
+ *   scale      [R] fp32 or NULL (1)
+ *   workspace  rb_low_rank_workspace_size(T, K, N, rank) bytes (may be 0; -1: bad
+ *              shape), 16-byte aligned
+ * Sums are fp32; from 97 tokens on, where rank and K are multiples of 8, rank <= 64
+ * and x, a and b are on 16-byte rows, the products run on the tensor cores and
+ * A_i x is rounded to the model type between them; else it stays fp32.  out is
+ * rounded once.  Forward only.
+ */
+int64_t rb_low_rank_workspace_size(int64_t T, int K, int N, int rank);
+int rb_low_rank_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int dtype, int64_t T, int K,
+                    int N, const void* a, const void* b, int R, int rank, const void* idx, int idx_dtype,
+                    const float* scale, void* workspace, int64_t workspace_bytes, void* out, int64_t ldo,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,175 @@
+"""Low-rank adapters beside a shared projection (rb_low_rank_add, adapters.py) on the GPU against the
+definition in float64.
+
+Tolerance: h = A x is a sum of K products in fp32, off by at most K u of sum |a| |x| (u = 2^-24); on the
+tensor-core path it is rounded to the model type (half a step of |h|, or of its smallest subnormal).  B h adds rank u of
+sum |B| |h|.  So out is within  sum_j |B_j| |s| (eps / 2 |h_j| + tiny + (K + rank) u sum |a| |x|)  and, rounded once, half a
+step of itself (the fp32 sum with y adds u of the terms, inside the same bound's factor 1.01).
+"""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _inputs(T, K, N, rank, R, dtype, run, seed):
+    gen = torch.Generator().manual_seed(seed)
+    x, y = torch.randn(T, K, generator=gen).to(dtype), torch.randn(T, N, generator=gen).to(dtype)
+    a = (torch.randn(R, rank, K, generator=gen) * K ** -0.5).to(dtype)
+    b = (torch.randn(R, N, rank, generator=gen) * rank ** -0.5).to(dtype)
+    scale = torch.rand(R, generator=gen) + 0.5
+    starts = torch.rand(T, generator=gen) < 1.0 / run
+    chosen = torch.randint(-1, R, (T + 1,), generator=gen)
+    return y, x, a, b, chosen[starts.long().cumsum(0)], scale
+
+
+def _check(got, y, x, a, b, adapter, scale):
+    dev = got.device
+    y, x, a, b, adapter = (t.to(dev) for t in (y, x, a, b, adapter))
+    scale = torch.ones(a.shape[0], device=dev) if scale is None else scale.to(dev)
+    rank, K = a.shape[1:]
+    fi = torch.finfo(y.dtype)
+    want, bound = y.double(), torch.zeros_like(y, dtype=torch.float64)
+    tiny = fi.smallest_normal * fi.eps / 2
+    for i in range(a.shape[0]):
+        t = (adapter == i).nonzero()[:, 0]
+        if not len(t):
+            continue
+        xi, ai, bi, s = x[t].double(), a[i].double(), b[i].double(), scale[i].double()
+        h = xi @ ai.t()
+        want[t] += s * (h @ bi.t())
+        off = fi.eps / 2 * h.abs() + tiny + (K + rank) * 2.0 ** -24 * (xi.abs() @ ai.abs().t())
+        bound[t] = 1.01 * s.abs() * (off @ bi.abs().t()) + 2.0 ** -23 * y[t].double().abs()
+    off = (got.double() - want).abs()
+    limit = fi.eps / 2 * want.abs() + bound + tiny
+    assert bool((off <= limit).all()), (float((off - limit).max()), int((off > limit).sum()))
+    none = (adapter < 0) | (adapter >= a.shape[0])
+    assert torch.equal(got[none], y[none])
+
+
+SHAPES = [
+    # T, K, N, rank, R, dtype, run
+    (1, 512, 1536, 16, 4, BF, 1),
+    (1, 14336, 512, 32, 2, BF, 1),
+    (7, 40, 24, 8, 3, HF, 2),
+    (64, 512, 1536, 16, 32, BF, 1),
+    (96, 512, 513, 16, 5, BF, 4),
+    (97, 512, 512, 16, 5, BF, 30),
+    (128, 64, 64, 16, 1, BF, 10),
+    (129, 8, 16, 8, 2, HF, 10),
+    (300, 72, 200, 8, 7, BF, 9),
+    (300, 512, 512, 32, 3, HF, 25),
+    (700, 200, 100, 64, 3, BF, 50),
+    (700, 200, 101, 24, 5, HF, 20),
+    (515, 1000, 1544, 8, 24, HF, 7),
+    (513, 512, 640, 40, 9, BF, 3),
+    (1000, 4096, 512, 48, 4, BF, 80),
+    (2049, 14336, 512, 32, 6, BF, 100),
+    (256, 512, 512, 16, 300, BF, 1),        # every row of a tile its own adapter
+    (19000, 128, 192, 16, 11, BF, 60),      # enough tiles for one fused kernel
+    (19001, 256, 72, 8, 130, HF, 2),
+    (200, 100, 64, 16, 3, BF, 9),           # K not a multiple of 8: token kernel
+    (200, 96, 64, 12, 3, HF, 9),            # rank not a multiple of 8
+    (130, 96, 64, 128, 3, BF, 9),           # rank above the tensor path's
+]
+
+
+@pytest.mark.parametrize("T,K,N,rank,R,dtype,run", SHAPES)
+def test_against_float64(cuda_device, T, K, N, rank, R, dtype, run):
+    from baidu_cti_grab_b200 import device_ops
+
+    args = _inputs(T, K, N, rank, R, dtype, run, T + K)
+    y, x, a, b, adapter, scale = (t.to(cuda_device) for t in args)
+    got = device_ops.low_rank_add(y, x, a, b, adapter, scale)
+    _check(got, *args)
+    assert torch.equal(device_ops.low_rank_add(y, x, a, b, adapter.int(), scale), got)  # and the same bits again
+    _check(device_ops.low_rank_add(y, x, a, b, adapter), *args[:5], None)
+    place = y.clone()
+    assert device_ops.low_rank_add(place, x, a, b, adapter, scale, out=place) is place
+    assert torch.equal(place, got)
+    torch.cuda.synchronize()
+    assert device_ops.device_error() == 0
+
+
+@pytest.mark.parametrize("T", [50, 600, 19500])
+def test_strides_odd_offsets_and_rows_left_alone(cuda_device, T):
+    from baidu_cti_grab_b200 import device_ops
+
+    K, N = 128, 96
+    args = _inputs(T, K, N, 16, 6, BF, 12, 5)
+    y, x, a, b, adapter, scale = (t.to(cuda_device) for t in args)
+    want = device_ops.low_rank_add(y, x, a, b, adapter, scale)
+    for ldx, offx, ld, off in ((K + 8, 0, N + 16, 0), (K + 8, 8, N + 8, 8), (K, 1, N + 3, 1)):
+        rx = torch.zeros(T * ldx + offx, dtype=BF, device=cuda_device)
+        xv = rx[offx:].view(T, ldx)[:, :K]
+        xv.copy_(x)
+        ry, ro = (torch.full((T * ld + off,), 7.0, dtype=BF, device=cuda_device) for _ in range(2))
+        yv, ov = ry[off:].view(T, ld)[:, :N], ro[off:].view(T, ld)
+        yv.copy_(y)
+        got = device_ops.low_rank_add(yv, xv, a, b, adapter, scale, out=ov[:, :N])
+        if offx % 8 == 0:
+            assert torch.equal(got, want)
+        else:
+            _check(got, *args)  # unaligned rows: the token kernel, which does not round h
+        assert bool((ov[:, N:] == 7.0).all()) and bool((ro[:off] == 7.0).all())
+
+
+def test_no_adapter_none_of_a_tile_and_nan(cuda_device):
+    from baidu_cti_grab_b200 import device_ops
+
+    for T in (40, 400, 20000):
+        y, x, a, b, adapter, scale = (t.to(cuda_device) for t in _inputs(T, 64, 80, 16, 5, HF, 10, 2))
+        none = torch.full_like(adapter, -1)
+        assert torch.equal(device_ops.low_rank_add(y, x, a, b, none, scale), y)
+        none[::2] = 5  # past the bank
+        assert torch.equal(device_ops.low_rank_add(y, x, a, b, none, scale), y)
+        clean = device_ops.low_rank_add(y, x, a, b, adapter, scale)
+        bad = x.clone()
+        bad[3] = float("nan")
+        a2 = a.clone()
+        a2[4] = float("inf")  # an adapter that is not sound reaches its own tokens only
+        adapter[3] = 0
+        got = device_ops.low_rank_add(y, bad, a2, b, adapter, scale)
+        rows = adapter != 4
+        rows[3] = False
+        assert torch.equal(got[rows], clean[rows])
+        assert bool(got[3].isnan().all())
+    y0 = device_ops.low_rank_add(y[:0], x[:0], a, b, adapter[:0], scale)
+    assert y0.shape == (0, 80)
+
+
+def test_bank_streams_and_graphs(cuda_device):
+    from baidu_cti_grab_b200 import adapters, device_ops
+
+    gen = torch.Generator().manual_seed(3)
+    parts = [((torch.randn(r, 256, generator=gen) / 16).to(BF), (torch.randn(320, r, generator=gen) / 4).to(BF), 0.5 + i)
+             for i, r in enumerate((8, 16, 4))]
+    bank = adapters.AdapterBank.stack(parts).to(cuda_device)
+    assert bank.a.shape == (3, 16, 256) and bank.to(torch.bfloat16).scale.dtype == torch.float32
+    offsets = torch.tensor([0, 100, 100, 350, 700], device=cuda_device)
+    who = adapters.AdapterBank.per_token(torch.tensor([2, 0, -1, 1], device=cuda_device), offsets, 700)
+    y, x = (torch.randn(700, n, generator=gen).to(BF).to(cuda_device) for n in (320, 256))
+    got = bank(y, x, who)
+    _check(got, y, x, bank.a, bank.b, who, bank.scale)
+    assert torch.equal(bank(y.view(7, 100, 320), x.view(7, 100, 256), who.view(7, 100)).view(700, 320), got)
+    with pytest.raises(RuntimeError):
+        device_ops.low_rank_add(y, x.clone().requires_grad_(), bank.a, bank.b, who)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = bank(y, x, who)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, got)
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    held = []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            held.append(bank(y, x, who))
+    for g in graphs * 2:
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(h, got) for h in held)

@@ -1,0 +1,56 @@
+"""What rb_low_rank_add and its Python wrappers refuse, before any device work (no GPU)."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+FAKE = 1 << 20  # an address that no call reaches: every one below fails a host check
+
+
+def _call(y=FAKE, ldy=512, x=FAKE, ldx=256, dtype=1, T=4, K=256, N=512, a=FAKE, b=FAKE, R=3, rank=16, idx=FAKE, it=5, ws=None,
+          size=0, out=FAKE, ldo=512):
+    from baidu_cti_grab_b200 import _lib
+
+    lib = _lib.load()
+    rc = lib.rb_low_rank_add(y, ldy, x, ldx, dtype, T, K, N, a, b, R, rank, idx, it, None, ws, size, out, ldo, None)
+    return rc, _lib.last_error()
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(T=-1), "negative"), (dict(K=0), "empty"), (dict(N=0), "empty"), (dict(R=0), "empty"), (dict(rank=0), "empty"),
+    (dict(rank=129), "ranks"), (dict(dtype=0), "bf16"), (dict(it=1), "adapter ids"), (dict(T=1 << 29), "tokens"),
+    (dict(R=1 << 24), "rows of all"), (dict(ldy=511), "leading"), (dict(ldo=1), "leading"), (dict(ldx=255), "leading"),
+    (dict(y=None), "null"), (dict(x=None), "null"), (dict(a=None), "null"), (dict(b=None), "null"), (dict(idx=None), "null"),
+    (dict(out=None), "null"), (dict(T=1000), "workspace"), (dict(T=1000, ws=FAKE, size=16), "workspace"),
+    (dict(T=1000, ws=FAKE + 4, size=1 << 30), "workspace")])
+def test_refuses_on_the_host(bad, word):
+    from baidu_cti_grab_b200 import _lib
+
+    rc, msg = _call(**bad)
+    assert rc in (_lib.RB_ERR_VALUE, _lib.RB_ERR_UNSUPPORTED) and word in msg, (rc, msg)
+
+
+def test_workspace_sizes():
+    """Few tokens and many tiles need none; tiles that are too few for the SMs hold partial h, fp32."""
+    from baidu_cti_grab_b200 import _lib
+
+    size = _lib.load().rb_low_rank_workspace_size
+    assert size(96, 512, 512, 16) == 0 and size(100000, 512, 512, 16) == 0 and size(0, 512, 512, 16) == 0
+    assert size(4099, 14336, 512, 32) % (4099 * 32 * 4) == 0 and size(4099, 14336, 512, 32) > 0
+    assert size(1000, 100, 512, 16) == 0 and size(1000, 512, 512, 12) == 0 and size(1000, 512, 512, 72) == 0
+    assert size(-1, 512, 512, 16) == -1 and size(10, 0, 512, 16) == -1 and size(10, 512, 512, 129) == -1
+
+
+def test_wrappers_refuse():
+    from baidu_cti_grab_b200 import adapters, device_ops
+
+    t = torch.zeros(4, 8, dtype=torch.bfloat16)
+    a, b = torch.zeros(2, 8, 8, dtype=torch.bfloat16), torch.zeros(2, 8, 8, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError):
+        device_ops.low_rank_add(t, t, a, b, torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(RuntimeError):
+        adapters.AdapterBank(a, b)(t, t, torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        adapters.AdapterBank(a, b[:1])
+    with pytest.raises(ValueError):
+        adapters.AdapterBank.stack([])
