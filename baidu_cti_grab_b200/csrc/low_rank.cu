@@ -9,7 +9,7 @@
 //   share the partial h = A x through distributed shared memory and split B's rows.
 //   Also takes every shape that the tensor maps cannot.
 // * tile kernel: 128 tokens a CTA on tcgen05.  The tile's distinct adapters are
-//   listed, and taken in groups whose padded ranks fill 64 columns:
+//   listed, and taken in groups whose padded ranks fill 64 (or 128) columns:
 //     H [128, 64] = X [128, K] . [A_i ; A_j ; ...]^T   all of the group in one MMA per K step
 //     each row keeps its own adapter's columns, the others become zeros
 //     out tile = H . [B_i | B_j | ...]^T               the zeros select the adapter
@@ -42,7 +42,8 @@ struct Params {
   float* part;         // [splits][T][rank] partial h, or null
   int64_t ldy, ldx, ldo, T;
   int K, N, R, rank, idx64;
-  int rp, group;       // rank padded to 16, 32 or 64; adapters of a group
+  int rp;              // rank padded to 16, 32 or 64
+  int chunk_io;        // y and out can be moved by whole chunks
   int splits;          // of K (H alone) -- partials to sum (out alone)
   int chunks;          // 64-column chunks of a CTA (out alone)
   int vec_y, vec_out;  // bytes of the loads and stores that rows allow: 32, 16 or 2
@@ -156,18 +157,25 @@ __global__ void __launch_bounds__(kTokenThreads) token_kernel(const __grid_const
 }
 
 // ------------------------------------------------------------- tile kernel
-constexpr int kRows = 128;        // tokens of a tile
-constexpr int kCols = 64;         // columns of H: a group's padded ranks
-constexpr int kChunk = 64;        // columns of an out chunk
-constexpr int kStages = 3;        // ring of X and A blocks of 64 columns of K
-constexpr int kXBytes = kRows * 128, kABytes = kCols * 128, kStageBytes = kXBytes + kABytes;
-constexpr int kHBytes = kRows * 128;
-constexpr int kBBytes = kChunk * kCols * 2;
-constexpr int kTileSmem = 1024 + kStages * kStageBytes + kHBytes + 2 * kBBytes;
-constexpr int kTmemCols = 256;    // H at column 0, two out chunks at 64 and 128
-constexpr int kTileThreads = 192; // TMA warp, MMA warp, four warps of rows
+constexpr int kRows = 128;         // tokens of a tile
+constexpr int kChunk = 64;         // columns of an out chunk
+constexpr int kTileThreads = 192;  // TMA warp, MMA warp, four warps of rows
+constexpr int kXBytes = kRows * 128;  // 64 columns of X (of K), or of y
 
 enum Mode : int { kFused = 0, kHOnly = 1, kOutOnly = 2 };
+
+// Two CTAs fit an SM in each form (the fused one 104 KB, H alone 96 KB, out alone 96 KB).
+template <int MODE>
+struct Tile {
+  static constexpr int kCols = MODE == kFused ? 64 : 128;  // of H: the padded ranks of a group of adapters
+  static constexpr int kStages = MODE == kOutOnly ? 2 : 3;  // ring of X (and A) blocks of 64 columns of K, then of y
+  static constexpr int kABytes = MODE == kOutOnly ? 0 : kCols * 128;
+  static constexpr int kHBytes = MODE == kHOnly ? 0 : kRows * kCols * 2;  // 64-column tiles of 16 KB
+  static constexpr int kBBytes = MODE == kHOnly ? 0 : kChunk * kCols * 2;
+  static constexpr int kSmem = 1024 + kStages * (kXBytes + kABytes) + kHBytes + 2 * kBBytes;
+  static constexpr int kHCols = MODE == kOutOnly ? 0 : kCols;  // TMEM: H, then two out chunks
+  static constexpr int kTmemCols = MODE == kFused ? 256 : 128;
+};
 
 // K-major operand rows of 32, 64 or 128 bytes under the swizzle of that width, in groups of eight rows
 __device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, int row_bytes) {
@@ -181,6 +189,20 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
+}
+
+// whether all 128 threads of the rows' warps say so; they meet here
+__device__ __forceinline__ bool rows_all(bool ok) {
+  uint32_t every;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(every)
+      : "r"((uint32_t)ok)
+      : "memory");
+  return every != 0;
 }
 
 template <typename T>
@@ -239,13 +261,16 @@ __device__ __forceinline__ void store16(T* row, int c, int N, int vec, const uin
 template <typename T, int MODE>
 __global__ void __launch_bounds__(kTileThreads, 2)
     tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA,
-                const __grid_constant__ CUtensorMap tmB, const __grid_constant__ Params p) {
+                const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY,
+                const __grid_constant__ CUtensorMap tmO, const __grid_constant__ Params p) {
+  using C = Tile<MODE>;
+  constexpr int kStages = C::kStages, kABytes = C::kABytes, kBBytes = C::kBBytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* sX = smem;
   uint8_t* sA = sX + kStages * kXBytes;
   uint8_t* sH = sA + kStages * kABytes;
-  uint8_t* sB = sH + kHBytes;
+  uint8_t* sB = sH + C::kHBytes;
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], hfull, hready, bfull[2], bempty[2], dfull[2], dempty[2], done;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word, s_count;
@@ -278,7 +303,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmB)) : "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemCols)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -309,7 +334,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const int count = s_count;
-  const int groups = (count + p.group - 1) / p.group;
+  const int group = C::kCols / p.rp;  // adapters of a group
+  const int groups = (count + group - 1) / group;
+  // one group (as a rule): y comes and out goes by whole 64-column chunks through the ring
+  const bool whole = MODE != kHOnly && groups == 1 && p.chunk_io != 0;
   const int kblocks = (p.K + 63) / 64;
   const int split = MODE == kFused ? 0 : (int)blockIdx.y;
   const int kb0 = MODE == kHOnly ? (int)((int64_t)kblocks * split / p.splits) : 0;
@@ -329,7 +357,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       uint32_t issued = 0, issued_phase = 0;  // bits: ring stages, then the two B buffers
       bool ok = true;
       for (int g = 0; g < groups && ok; ++g) {
-        const int first = g * p.group, n = min(p.group, count - first);
+        const int first = g * group, n = min(group, count - first);
         if constexpr (MODE != kOutOnly) {
           for (int kb = kb0; kb < kb1; ++kb) {
             if (!mbar_wait_bounded(smem_u32(&empty[stage]), phase ^ 1, kWaitTimeoutProducer, abort_flag)) {
@@ -363,6 +391,20 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             issued_phase = (issued_phase & ~(1u << (kStages + buf))) | (bphase << (kStages + buf));
             buf ^= 1;
             if (buf == 0) bphase ^= 1;
+            if (!whole) continue;
+            if (!mbar_wait_bounded(smem_u32(&empty[stage]), phase ^ 1, kWaitTimeoutProducer, abort_flag)) {
+              ok = false;
+              break;
+            }
+            const uint32_t fy = smem_u32(&full[stage]);
+            mbar_arrive_expect_tx(fy, kXBytes);
+            tc::tma_load_2d(smem_u32(sX + stage * kXBytes), &tmY, ch * kChunk, (int)row0, fy, once);
+            issued |= 1u << stage;
+            issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
         }
       }
@@ -379,7 +421,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       uint32_t phase = 0, bphase = 0;
       bool ok = true;
       for (int g = 0; g < groups && ok; ++g) {
-        const int n = min(p.group, count - g * p.group);
+        const int n = min(group, count - g * group);
         if constexpr (MODE != kOutOnly) {
           const uint32_t idesc = kIdesc | ((uint32_t)(n * p.rp >> 3) << 17);
           for (int kb = kb0; kb < kb1; ++kb) {
@@ -416,8 +458,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             tc::tc_fence_after();
             for (int j = 0; j < n; ++j) {
               const uint64_t bd = operand_desc(smem_u32(sB + buf * kBBytes + j * b_slot), row_bytes);
-              for (int s = 0; s < p.rp / 16; ++s)
-                umma_f16(tmem + kCols + buf * kChunk, hd + 2 * (j * (p.rp / 16) + s), bd + 2 * s, idesc, (j > 0 || s > 0) ? 1u : 0u);
+              for (int s = 0; s < p.rp / 16; ++s) {
+                const int at = j * (p.rp / 16) + s;  // sixteen columns of H: four to a 16 KB tile
+                umma_f16(tmem + C::kHCols + buf * kChunk, hd + (uint64_t)((at >> 2) * (kXBytes >> 4) + 2 * (at & 3)), bd + 2 * s,
+                         idesc, at > 0 ? 1u : 0u);
+              }
             }
             tc::umma_commit(smem_u32(&bempty[buf]));
             tc::umma_commit(smem_u32(&dfull[buf]));
@@ -443,7 +488,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     int buf = 0;
     uint32_t bphase = 0;
     bool ok = true;
-    if (MODE != kHOnly && live && slot < 0 && out != y) {
+    if (MODE != kHOnly && !whole && live && slot < 0 && out != y) {
       for (int c = ch0 * kChunk; c < min(p.N, ch1 * kChunk); c += 16) {
         uint32_t v[8];
         load16(y, c, p.N, p.vec_y, v);
@@ -451,10 +496,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       }
     }
     for (int g = 0; g < groups && ok; ++g) {
-      const int first = g * p.group, n = min(p.group, count - first);
+      const int first = g * group, n = min(group, count - first);
       const int mine = slot >= first && slot < first + n ? slot - first : -1;
       if constexpr (MODE != kOutOnly) {
-        if (!mbar_wait_bounded(smem_u32(&hfull), g & 1, kWaitTimeoutEpilogue, abort_flag)) break;
+        // a thread that gave up still meets the others at the chunks' barrier
+        ok = mbar_wait_bounded(smem_u32(&hfull), g & 1, kWaitTimeoutEpilogue, abort_flag);
         tc::tc_fence_after();
       }
       // own adapter's h into this row of the H tile, zeros into the others' columns (and the rank's padding)
@@ -462,13 +508,26 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         for (int c = 0; c < p.rp; c += 16) {
           uint32_t v[16];
           if constexpr (MODE == kOutOnly) {
+            float s[16];
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-              float s = 0.0f;
-              if (mine == j && c + q < p.rank)
-                for (int k = 0; k < p.splits; ++k) s += p.part[((int64_t)k * p.T + row) * p.rank + c + q];
-              v[q] = __float_as_uint(s);
+            for (int q = 0; q < 16; ++q) s[q] = 0.0f;
+            if (mine == j) {
+              const float* from = p.part + row * p.rank + c;
+#pragma unroll 4
+              for (int k = 0; k < p.splits; ++k, from += p.T * p.rank) {
+#pragma unroll
+                for (int q = 0; q < 16; q += 4) {
+                  if (c + q >= p.rank) continue;
+                  const float4 f = __ldg(reinterpret_cast<const float4*>(from + q));
+                  s[q] += f.x;
+                  s[q + 1] += f.y;
+                  s[q + 2] += f.z;
+                  s[q + 3] += f.w;
+                }
+              }
             }
+#pragma unroll
+            for (int q = 0; q < 16; ++q) v[q] = __float_as_uint(s[q]);
           } else {
             __syncwarp();
             tc::swp::tmem_ld16(tmem + lanes + (uint32_t)(j * p.rp + c), v);
@@ -489,16 +548,75 @@ __global__ void __launch_bounds__(kTileThreads, 2)
               const bool in = mine == j && c + 2 * q < p.rank;  // the rank is even
               h[q] = in ? pack2<T>(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])) : 0u;
             }
-            const int piece = (j * p.rp + c) / 8;  // 16-byte pieces of the row, swizzled by the row's place in its eight
-            *reinterpret_cast<uint4*>(sH + r * 128 + ((piece ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(sH + r * 128 + (((piece + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+            // 16-byte pieces of the row, swizzled by the row's place in its eight; eight pieces to a tile
+            const int at = (j * p.rp + c) / 8, piece = at & 7;
+            uint8_t* to = sH + (at >> 3) * kXBytes + r * 128;
+            *reinterpret_cast<uint4*>(to + ((piece ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(to + (((piece + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
           }
         }
       }
       tc::tc_fence_before();
       if constexpr (MODE != kHOnly) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(smem_u32(&hready));
-      if constexpr (MODE != kHOnly) {
+      if (whole) {
+        const int before = MODE == kFused ? kb1 - kb0 : 0;  // X blocks that the ring carried
+        int stage = before % kStages;
+        uint32_t phase = (uint32_t)(before / kStages) & 1u;
+        int last = -1;  // the stage whose store may still be reading
+        for (int ch = ch0; ch < ch1; ++ch) {
+          ok = ok && mbar_wait_bounded(smem_u32(&full[stage]), phase, kWaitTimeoutEpilogue, abort_flag) &&
+               mbar_wait_bounded(smem_u32(&dfull[buf]), bphase, kWaitTimeoutEpilogue, abort_flag);
+          tc::tc_fence_after();
+          uint8_t* mem = sX + stage * kXBytes + r * 128;
+#pragma unroll
+          for (int h = 0; h < kChunk / 32; ++h) {
+            uint32_t v[32];
+            __syncwarp();
+            tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + buf * kChunk + h * 32), v);
+            if (h == kChunk / 32 - 1) {
+              tc::tc_fence_before();
+              mbar_arrive(smem_u32(&dempty[buf]));
+            }
+            if (mine < 0 || !ok) continue;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint4* at = reinterpret_cast<uint4*>(mem + (((4 * h + q) ^ (r & 7)) << 4));
+              const uint4 f = *at;
+              const uint32_t fw[4] = {f.x, f.y, f.z, f.w};
+              uint32_t o[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 u = unpack2<T>(fw[i]);
+                o[i] = pack2<T>(fmaf(w, __uint_as_float(v[8 * q + 2 * i]), u.x), fmaf(w, __uint_as_float(v[8 * q + 2 * i + 1]), u.y));
+              }
+              *at = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          ok = rows_all(ok);
+          if (!ok) break;
+          if (threadIdx.x == 64) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                             reinterpret_cast<uint64_t>(&tmO)),
+                         "r"(smem_u32(sX + stage * kXBytes)), "r"(ch * kChunk), "r"((int)row0)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            if (last >= 0) {
+              asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+              mbar_arrive(smem_u32(&empty[last]));
+            }
+            last = stage;
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+          buf ^= 1;
+          if (buf == 0) bphase ^= 1;
+        }
+        if (threadIdx.x == 64) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      } else if constexpr (MODE != kHOnly) {
         for (int ch = ch0; ch < ch1; ++ch) {
           const int c0 = ch * kChunk;
           uint32_t base[kChunk / 2];
@@ -516,7 +634,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
           for (int h = 0; h < kChunk / 32; ++h) {
             uint32_t v[32];
             __syncwarp();
-            tc::tmem_ld32(tmem + lanes + (uint32_t)(kCols + buf * kChunk + h * 32), v);
+            tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + buf * kChunk + h * 32), v);
             if (h == kChunk / 32 - 1) {
               tc::tc_fence_before();
               mbar_arrive(smem_u32(&dempty[buf]));
@@ -542,7 +660,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   __syncthreads();
   if (warp == 1) {
     tc::tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
   }
 }
 
@@ -565,7 +683,7 @@ static Plan plan_of(int64_t T, int K, int N, int rank) {
   const int kblocks = (K + 63) / 64, chunks = (N + kChunk - 1) / kChunk;
   q.chunks = chunks;
   if (tiles * 2 <= sms) {  // two CTAs an SM are resident; below half of the SMs the two phases are spread
-    const int64_t want = (2 * sms + tiles - 1) / tiles;
+    const int64_t want = 2 * sms / tiles;
     q.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, (int64_t)(kblocks + 3) / 4, 16}));
     const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(want, chunks));
     q.chunks = (int)((chunks + parts - 1) / parts);
@@ -625,25 +743,32 @@ static int run_tiles(Params& p, const Plan& q, CUtensorMapDataType dt, cudaStrea
   cudaGetDevice(&dev);
   cudaError_t e = cudaSuccess;
   std::call_once(once[dev & 63], [&] {
-    const void* fns[3] = {(const void*)tile_kernel<T, kFused>, (const void*)tile_kernel<T, kHOnly>, (const void*)tile_kernel<T, kOutOnly>};
-    for (const void* f : fns)
-      if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem);
+    e = cudaFuncSetAttribute(tile_kernel<T, kFused>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<kFused>::kSmem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(tile_kernel<T, kHOnly>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<kHOnly>::kSmem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(tile_kernel<T, kOutOnly>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<kOutOnly>::kSmem);
   });
   if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(low-rank tile_kernel)");
-  CUtensorMap tmX, tmA, tmB;
+  CUtensorMap tmX, tmA, tmB, tmY, tmO;
   if ((rc = make_map(&tmX, p.x, p.K, p.T, p.ldx * 2, 64, kRows, dt))) return rc;
   if ((rc = make_map(&tmA, p.a, p.K, (int64_t)p.R * p.rank, (int64_t)p.K * 2, 64, (uint32_t)p.rp, dt))) return rc;
   if ((rc = make_map(&tmB, p.b, p.rank, (int64_t)p.R * p.N, (int64_t)p.rank * 2, (uint32_t)p.rp, kChunk, dt))) return rc;
+  tmY = tmO = tmX;  // not used where rows do not allow whole chunks
+  if (p.chunk_io) {
+    if ((rc = make_map(&tmY, p.y, p.N, p.T, p.ldy * 2, kChunk, kRows, dt))) return rc;
+    if ((rc = make_map(&tmO, p.out, p.N, p.T, p.ldo * 2, kChunk, kRows, dt))) return rc;
+  }
   if (q.splits == 1) {
-    tile_kernel<T, kFused><<<q.tiles, kTileThreads, kTileSmem, st>>>(tmX, tmA, tmB, p);
+    tile_kernel<T, kFused><<<q.tiles, kTileThreads, Tile<kFused>::kSmem, st>>>(tmX, tmA, tmB, tmY, tmO, p);
     return check_cuda(cudaGetLastError(), "low-rank tile_kernel launch");
   }
   p.splits = std::max(1, q.splits);
   p.chunks = q.chunks;
-  tile_kernel<T, kHOnly><<<dim3(q.tiles, p.splits), kTileThreads, kTileSmem, st>>>(tmX, tmA, tmB, p);
+  tile_kernel<T, kHOnly><<<dim3(q.tiles, p.splits), kTileThreads, Tile<kHOnly>::kSmem, st>>>(tmX, tmA, tmB, tmY, tmO, p);
   if ((rc = check_cuda(cudaGetLastError(), "low-rank tile_kernel launch (H)"))) return rc;
   const int parts = ((p.N + kChunk - 1) / kChunk + p.chunks - 1) / p.chunks;
-  tile_kernel<T, kOutOnly><<<dim3(q.tiles, parts), kTileThreads, kTileSmem, st>>>(tmX, tmA, tmB, p);
+  tile_kernel<T, kOutOnly><<<dim3(q.tiles, parts), kTileThreads, Tile<kOutOnly>::kSmem, st>>>(tmX, tmA, tmB, tmY, tmO, p);
   return check_cuda(cudaGetLastError(), "low-rank tile_kernel launch (out)");
 }
 
@@ -700,10 +825,10 @@ extern "C" int rb_low_rank_add(const void* y, int64_t ldy, const void* x, int64_
   p.rank = rank;
   p.idx64 = idx_dtype == RB_I64;
   p.rp = rank <= 16 ? 16 : rank <= 32 ? 32 : 64;
-  p.group = kCols / p.rp;
   p.splits = 1;
   p.vec_y = vec_bytes(y, ldy);
   p.vec_out = vec_bytes(out, ldo);
+  p.chunk_io = p.vec_y >= 16 && p.vec_out >= 16;
   cudaStream_t st = (cudaStream_t)stream;
   if (q.tiles == 0)
     return dtype == RB_BF16 ? run_tokens<__nv_bfloat16>(p, fit, st) : run_tokens<__half>(p, fit, st);
