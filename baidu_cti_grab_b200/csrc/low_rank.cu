@@ -9,7 +9,7 @@
 //   share the partial h = A x through distributed shared memory and split B's rows.
 //   Also takes every shape that the tensor maps cannot.
 // * tile kernel: 128 tokens a CTA on tcgen05.  The tile's distinct adapters are
-//   listed, and taken in groups whose padded ranks fill 64 (or 128) columns:
+//   listed, and taken in groups whose ranks fill 64 (or 128) columns:
 //     H [128, 64] = X [128, K] . [A_i ; A_j ; ...]^T   all of the group in one MMA per K step
 //     each row keeps its own adapter's columns, the others become zeros
 //     out tile = H . [B_i | B_j | ...]^T               the zeros select the adapter
@@ -42,7 +42,6 @@ struct Params {
   float* part;         // [splits][T][rank] partial h, or null
   int64_t ldy, ldx, ldo, T;
   int K, N, R, rank, idx64;
-  int rp;              // rank padded to 16, 32 or 64
   int chunk_io;        // y and out can be moved by whole chunks
   int splits;          // of K (H alone) -- partials to sum (out alone)
   int chunks;          // 64-column chunks of a CTA (out alone)
@@ -159,29 +158,39 @@ __global__ void __launch_bounds__(kTokenThreads) token_kernel(const __grid_const
 // ------------------------------------------------------------- tile kernel
 constexpr int kRows = 128;         // tokens of a tile
 constexpr int kChunk = 64;         // columns of an out chunk
-constexpr int kTileThreads = 192;  // TMA warp, MMA warp, four warps of rows
+constexpr int kRowThreads = 256;   // two warps for each 32 rows (TMEM lanes): the halves of a chunk
+constexpr int kTileThreads = 64 + kRowThreads;  // TMA warp, MMA warp, the rows' warps
 constexpr int kXBytes = kRows * 128;  // 64 columns of X (of K), or of y
+constexpr int kPiece = kChunk * 16;   // eight columns of B for a chunk
+constexpr int kZeroBytes = kPiece;    // what an odd piece of eight columns is paired with
 
 enum Mode : int { kFused = 0, kHOnly = 1, kOutOnly = 2 };
 
 // Two CTAs fit an SM in each form (the fused one 104 KB, H alone 96 KB, out alone 96 KB).
 template <int MODE>
 struct Tile {
-  static constexpr int kCols = MODE == kFused ? 64 : 128;  // of H: the padded ranks of a group of adapters
+  static constexpr int kCols = MODE == kFused ? 64 : 128;  // of H: the ranks of a group of adapters
   static constexpr int kStages = MODE == kOutOnly ? 2 : 3;  // ring of X (and A) blocks of 64 columns of K, then of y
   static constexpr int kABytes = MODE == kOutOnly ? 0 : kCols * 128;
   static constexpr int kHBytes = MODE == kHOnly ? 0 : kRows * kCols * 2;  // 64-column tiles of 16 KB
   static constexpr int kBBytes = MODE == kHOnly ? 0 : kChunk * kCols * 2;
-  static constexpr int kSmem = 1024 + kStages * (kXBytes + kABytes) + kHBytes + 2 * kBBytes;
+  static constexpr int kSmem = 1024 + kStages * (kXBytes + kABytes) + kHBytes + 2 * kBBytes + kZeroBytes;
   static constexpr int kHCols = MODE == kOutOnly ? 0 : kCols;  // TMEM: H, then two out chunks
   static constexpr int kTmemCols = MODE == kFused ? 256 : 128;
 };
 
-// K-major operand rows of 32, 64 or 128 bytes under the swizzle of that width, in groups of eight rows
-__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, int row_bytes) {
-  const uint64_t layout = row_bytes == 128 ? 2 : row_bytes == 64 ? 4 : 6;
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(8 * row_bytes >> 4) << 32) |
-         ((uint64_t)1 << 46) | (layout << 61);
+// K-major operand without swizzle: eight rows of 16 bytes are 128 bytes in a row, groups of eight rows follow each
+// other, and the second eight columns of K lie `next` bytes on
+__device__ __forceinline__ uint64_t plain_desc(uint32_t saddr, uint32_t next) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, uint32_t bar,
+                                            uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+      : "memory");
 }
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -191,16 +200,16 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
 }
 
-// whether all 128 threads of the rows' warps say so; they meet here
+// whether all threads of the rows' warps say so; they meet here
 __device__ __forceinline__ bool rows_all(bool ok) {
   uint32_t every;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 1, 128, p;\n\t"
+      "barrier.cta.red.and.pred q, 1, %2, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(every)
-      : "r"((uint32_t)ok)
+            : "r"((uint32_t)ok), "n"(kRowThreads)
       : "memory");
   return every != 0;
 }
@@ -287,12 +296,12 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       mbar_init(smem_u32(&empty[s]), 1);
     }
     mbar_init(smem_u32(&hfull), 1);
-    mbar_init(smem_u32(&hready), 128);
+    mbar_init(smem_u32(&hready), kRowThreads);
     for (int s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&bfull[s]), 1);
       mbar_init(smem_u32(&bempty[s]), 1);
       mbar_init(smem_u32(&dfull[s]), 1);
-      mbar_init(smem_u32(&dempty[s]), 128);
+      mbar_init(smem_u32(&dempty[s]), kRowThreads);
     }
     mbar_init(smem_u32(&done), 1);
     abort_word = 0;
@@ -306,6 +315,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == 3) {
+    for (int i = lane; i < kZeroBytes / 16; i += 32)
+      reinterpret_cast<uint4*>(sB + 2 * kBBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 2) {
     // the tile's distinct adapters in the order of their first row, and each row's place among them
@@ -334,7 +348,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const int count = s_count;
-  const int group = C::kCols / p.rp;  // adapters of a group
+  uint8_t* const s_zero = sB + 2 * kBBytes;
+  const int group = C::kCols / p.rank;  // adapters of a group
   const int groups = (count + group - 1) / group;
   // one group (as a rule): y comes and out goes by whole 64-column chunks through the ring
   const bool whole = MODE != kHOnly && groups == 1 && p.chunk_io != 0;
@@ -345,8 +360,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   const int all_chunks = (p.N + kChunk - 1) / kChunk;
   const int ch0 = MODE == kOutOnly ? split * p.chunks : 0;
   const int ch1 = MODE == kOutOnly ? min(all_chunks, ch0 + p.chunks) : all_chunks;
-  const int row_bytes = p.rp * 2;          // of a B operand row
-  const int b_slot = kChunk * row_bytes;   // of an adapter's B chunk
+  const int eights = p.rank / 8;           // pieces of eight columns of an adapter
 
   if (warp == 0) {
     if (lane == 0) {
@@ -365,10 +379,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
               break;
             }
             const uint32_t fb = smem_u32(&full[stage]);
-            mbar_arrive_expect_tx(fb, kXBytes + n * p.rp * 128);
+            mbar_arrive_expect_tx(fb, kXBytes + n * p.rank * 128);
             tc::tma_load_2d(smem_u32(sX + stage * kXBytes), &tmX, kb * 64, (int)row0, fb, groups > 1 ? keep : once);
             for (int j = 0; j < n; ++j)
-              tc::tma_load_2d(smem_u32(sA + stage * kABytes + j * p.rp * 128), &tmA, kb * 64, s_list[first + j] * p.rank, fb, keep);
+              tc::tma_load_2d(smem_u32(sA + stage * kABytes + j * p.rank * 128), &tmA, kb * 64, s_list[first + j] * p.rank, fb, keep);
             issued |= 1u << stage;
             issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
             if (++stage == kStages) {
@@ -384,9 +398,9 @@ __global__ void __launch_bounds__(kTileThreads, 2)
               break;
             }
             const uint32_t fb = smem_u32(&bfull[buf]);
-            mbar_arrive_expect_tx(fb, n * b_slot);
+            mbar_arrive_expect_tx(fb, n * eights * kPiece);
             for (int j = 0; j < n; ++j)
-              tc::tma_load_2d(smem_u32(sB + buf * kBBytes + j * b_slot), &tmB, 0, s_list[first + j] * p.N + ch * kChunk, fb, keep);
+              tma_load_3d(smem_u32(sB + buf * kBBytes + j * eights * kPiece), &tmB, 0, s_list[first + j] * p.N + ch * kChunk, 0, fb, keep);
             issued |= 1u << (kStages + buf);
             issued_phase = (issued_phase & ~(1u << (kStages + buf))) | (bphase << (kStages + buf));
             buf ^= 1;
@@ -423,15 +437,15 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       for (int g = 0; g < groups && ok; ++g) {
         const int n = min(group, count - g * group);
         if constexpr (MODE != kOutOnly) {
-          const uint32_t idesc = kIdesc | ((uint32_t)(n * p.rp >> 3) << 17);
+          const uint32_t idesc = kIdesc | ((uint32_t)((n * eights + 1) & ~1) << 17);  // N in eights, an even number
           for (int kb = kb0; kb < kb1; ++kb) {
             if (!mbar_wait_bounded(smem_u32(&full[stage]), phase, kWaitTimeoutMma, abort_flag)) {
               ok = false;
               break;
             }
             tc::tc_fence_after();
-            const uint64_t xd = operand_desc(smem_u32(sX + stage * kXBytes), 128);
-            const uint64_t ad = operand_desc(smem_u32(sA + stage * kABytes), 128);
+            const uint64_t xd = tc::sw128_desc(smem_u32(sX + stage * kXBytes));
+            const uint64_t ad = tc::sw128_desc(smem_u32(sA + stage * kABytes));
 #pragma unroll
             for (int s = 0; s < 4; ++s) umma_f16(tmem, xd + 2 * s, ad + 2 * s, idesc, (kb > kb0 || s > 0) ? 1u : 0u);
             tc::umma_commit(smem_u32(&empty[stage]));
@@ -448,7 +462,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         if constexpr (MODE != kHOnly) {
           tc::tc_fence_after();
           const uint32_t idesc = kIdesc | ((uint32_t)(kChunk >> 3) << 17);
-          const uint64_t hd = operand_desc(smem_u32(sH), 128);
+          const uint64_t hd = tc::sw128_desc(smem_u32(sH));
           for (int ch = ch0; ch < ch1; ++ch) {
             if (!mbar_wait_bounded(smem_u32(&bfull[buf]), bphase, kWaitTimeoutMma, abort_flag) ||
                 !mbar_wait_bounded(smem_u32(&dempty[buf]), bphase ^ 1, kWaitTimeoutMma, abort_flag)) {
@@ -456,13 +470,13 @@ __global__ void __launch_bounds__(kTileThreads, 2)
               break;
             }
             tc::tc_fence_after();
-            for (int j = 0; j < n; ++j) {
-              const uint64_t bd = operand_desc(smem_u32(sB + buf * kBBytes + j * b_slot), row_bytes);
-              for (int s = 0; s < p.rp / 16; ++s) {
-                const int at = j * (p.rp / 16) + s;  // sixteen columns of H: four to a 16 KB tile
-                umma_f16(tmem + C::kHCols + buf * kChunk, hd + (uint64_t)((at >> 2) * (kXBytes >> 4) + 2 * (at & 3)), bd + 2 * s,
-                         idesc, at > 0 ? 1u : 0u);
-              }
+            const uint32_t bt = smem_u32(sB + buf * kBBytes);
+            for (int e = 0; e < n * eights; e += 2) {
+              const int at = e >> 1;  // sixteen columns of H: four to a 16 KB tile
+              const uint32_t from = bt + (uint32_t)(e * kPiece);
+              const uint64_t bd = plain_desc(from, e + 1 < n * eights ? (uint32_t)kPiece : smem_u32(s_zero) - from);
+              umma_f16(tmem + C::kHCols + buf * kChunk, hd + (uint64_t)((at >> 2) * (kXBytes >> 4) + 2 * (at & 3)), bd, idesc,
+                       e > 0 ? 1u : 0u);
             }
             tc::umma_commit(smem_u32(&bempty[buf]));
             tc::umma_commit(smem_u32(&dfull[buf]));
@@ -477,6 +491,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   } else {
     // ----------------------------------------------------------- the rows
     const int quarter = warp & 3;  // the TMEM lanes that this warp can read
+    const int half = (warp - 2) >> 2;  // its 32 columns of a chunk, and every other sixteen of H
     const int r = quarter * 32 + lane;
     const int64_t row = row0 + r;
     const bool live = row < p.T;
@@ -489,7 +504,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     uint32_t bphase = 0;
     bool ok = true;
     if (MODE != kHOnly && !whole && live && slot < 0 && out != y) {
-      for (int c = ch0 * kChunk; c < min(p.N, ch1 * kChunk); c += 16) {
+      for (int c = ch0 * kChunk + half * 16; c < min(p.N, ch1 * kChunk); c += 32) {
         uint32_t v[8];
         load16(y, c, p.N, p.vec_y, v);
         store16(out, c, p.N, p.vec_out, v);
@@ -503,56 +518,60 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         ok = mbar_wait_bounded(smem_u32(&hfull), g & 1, kWaitTimeoutEpilogue, abort_flag);
         tc::tc_fence_after();
       }
-      // own adapter's h into this row of the H tile, zeros into the others' columns (and the rank's padding)
-      for (int j = 0; j < n; ++j) {
-        for (int c = 0; c < p.rp; c += 16) {
-          uint32_t v[16];
-          if constexpr (MODE == kOutOnly) {
-            float s[16];
+      // own adapter's h into this row of the H tile, zeros into the others' columns: sixteen columns at a time, whose
+      // eights may be of two adapters
+      for (int c = half * 16; c < n * p.rank; c += 32) {
+        const int e = c / 8;
+        const bool in[2] = {mine >= 0 && e / eights == mine, mine >= 0 && (e + 1) / eights == mine};
+        uint32_t v[16];
+        if constexpr (MODE == kOutOnly) {
+          float s[16];
 #pragma unroll
-            for (int q = 0; q < 16; ++q) s[q] = 0.0f;
-            if (mine == j) {
-              const float* from = p.part + row * p.rank + c;
+          for (int q = 0; q < 16; ++q) s[q] = 0.0f;
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            if (!in[d]) continue;
+            const float* from = p.part + row * p.rank + (c + 8 * d - mine * p.rank);
 #pragma unroll 4
-              for (int k = 0; k < p.splits; ++k, from += p.T * p.rank) {
-#pragma unroll
-                for (int q = 0; q < 16; q += 4) {
-                  if (c + q >= p.rank) continue;
-                  const float4 f = __ldg(reinterpret_cast<const float4*>(from + q));
-                  s[q] += f.x;
-                  s[q + 1] += f.y;
-                  s[q + 2] += f.z;
-                  s[q + 3] += f.w;
-                }
-              }
+            for (int k = 0; k < p.splits; ++k, from += p.T * p.rank) {
+              const float4 f = __ldg(reinterpret_cast<const float4*>(from)), h = __ldg(reinterpret_cast<const float4*>(from) + 1);
+              s[8 * d] += f.x;
+              s[8 * d + 1] += f.y;
+              s[8 * d + 2] += f.z;
+              s[8 * d + 3] += f.w;
+              s[8 * d + 4] += h.x;
+              s[8 * d + 5] += h.y;
+              s[8 * d + 6] += h.z;
+              s[8 * d + 7] += h.w;
             }
-#pragma unroll
-            for (int q = 0; q < 16; ++q) v[q] = __float_as_uint(s[q]);
-          } else {
-            __syncwarp();
-            tc::swp::tmem_ld16(tmem + lanes + (uint32_t)(j * p.rp + c), v);
           }
-          if constexpr (MODE == kHOnly) {
-            if (mine == j) {
-              float* to = p.part + ((int64_t)split * p.T + row) * p.rank + c;
 #pragma unroll
-              for (int q = 0; q < 16; q += 4)
-                if (c + q < p.rank)
-                  *reinterpret_cast<float4*>(to + q) = make_float4(__uint_as_float(v[q]), __uint_as_float(v[q + 1]),
-                                                                   __uint_as_float(v[q + 2]), __uint_as_float(v[q + 3]));
-            }
-          } else {
-            uint32_t h[8];
+          for (int q = 0; q < 16; ++q) v[q] = __float_as_uint(s[q]);
+        } else {
+          __syncwarp();
+          tc::swp::tmem_ld16(tmem + lanes + (uint32_t)c, v);
+        }
+        if constexpr (MODE == kHOnly) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const bool in = mine == j && c + 2 * q < p.rank;  // the rank is even
-              h[q] = in ? pack2<T>(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])) : 0u;
-            }
-            // 16-byte pieces of the row, swizzled by the row's place in its eight; eight pieces to a tile
-            const int at = (j * p.rp + c) / 8, piece = at & 7;
-            uint8_t* to = sH + (at >> 3) * kXBytes + r * 128;
-            *reinterpret_cast<uint4*>(to + ((piece ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(to + (((piece + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+          for (int d = 0; d < 2; ++d) {
+            if (!in[d]) continue;
+            float* to = p.part + ((int64_t)split * p.T + row) * p.rank + (c + 8 * d - mine * p.rank);
+#pragma unroll
+            for (int q = 0; q < 8; q += 4)
+              *reinterpret_cast<float4*>(to + q) =
+                  make_float4(__uint_as_float(v[8 * d + q]), __uint_as_float(v[8 * d + q + 1]), __uint_as_float(v[8 * d + q + 2]),
+                              __uint_as_float(v[8 * d + q + 3]));
+          }
+        } else {
+          // 16-byte pieces of the row, swizzled by the row's place in its eight; eight pieces to a tile
+          uint8_t* to = sH + (e >> 3) * kXBytes + r * 128;
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            uint32_t h[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              h[q] = in[d] ? pack2<T>(__uint_as_float(v[8 * d + 2 * q]), __uint_as_float(v[8 * d + 2 * q + 1])) : 0u;
+            *reinterpret_cast<uint4*>(to + ((((e + d) & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
           }
         }
       }
@@ -569,19 +588,15 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                mbar_wait_bounded(smem_u32(&dfull[buf]), bphase, kWaitTimeoutEpilogue, abort_flag);
           tc::tc_fence_after();
           uint8_t* mem = sX + stage * kXBytes + r * 128;
-#pragma unroll
-          for (int h = 0; h < kChunk / 32; ++h) {
-            uint32_t v[32];
-            __syncwarp();
-            tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + buf * kChunk + h * 32), v);
-            if (h == kChunk / 32 - 1) {
-              tc::tc_fence_before();
-              mbar_arrive(smem_u32(&dempty[buf]));
-            }
-            if (mine < 0 || !ok) continue;
+          uint32_t v[32];
+          __syncwarp();
+          tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + buf * kChunk + half * 32), v);
+          tc::tc_fence_before();
+          mbar_arrive(smem_u32(&dempty[buf]));
+          if (mine >= 0 && ok) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              uint4* at = reinterpret_cast<uint4*>(mem + (((4 * h + q) ^ (r & 7)) << 4));
+              uint4* at = reinterpret_cast<uint4*>(mem + (((4 * half + q) ^ (r & 7)) << 4));
               const uint4 f = *at;
               const uint32_t fw[4] = {f.x, f.y, f.z, f.w};
               uint32_t o[4];
@@ -618,11 +633,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         if (threadIdx.x == 64) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       } else if constexpr (MODE != kHOnly) {
         for (int ch = ch0; ch < ch1; ++ch) {
-          const int c0 = ch * kChunk;
-          uint32_t base[kChunk / 2];
+          const int c0 = ch * kChunk + half * 32;
+          uint32_t base[16];
           if (mine >= 0) {  // requested before the wait for the product
 #pragma unroll
-            for (int c = 0; c < kChunk; c += 16)
+            for (int c = 0; c < 32; c += 16)
               if (c0 + c < p.N) load16(y, c0 + c, p.N, p.vec_y, base + c / 2);
           }
           if (!mbar_wait_bounded(smem_u32(&dfull[buf]), bphase, kWaitTimeoutEpilogue, abort_flag)) {
@@ -630,25 +645,21 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             break;
           }
           tc::tc_fence_after();
-#pragma unroll
-          for (int h = 0; h < kChunk / 32; ++h) {
-            uint32_t v[32];
-            __syncwarp();
-            tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + buf * kChunk + h * 32), v);
-            if (h == kChunk / 32 - 1) {
-              tc::tc_fence_before();
-              mbar_arrive(smem_u32(&dempty[buf]));
-            }
-            if (mine < 0) continue;
+          uint32_t v[32];
+          __syncwarp();
+          tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + buf * kChunk + half * 32), v);
+          tc::tc_fence_before();
+          mbar_arrive(smem_u32(&dempty[buf]));
+          if (mine >= 0) {
             uint32_t o[16];
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
-              const float2 f = unpack2<T>(base[h * 16 + q]);
+              const float2 f = unpack2<T>(base[q]);
               o[q] = pack2<T>(fmaf(w, __uint_as_float(v[2 * q]), f.x), fmaf(w, __uint_as_float(v[2 * q + 1]), f.y));
             }
 #pragma unroll
             for (int c = 0; c < 32; c += 16)
-              if (c0 + h * 32 + c < p.N) store16(out, c0 + h * 32 + c, p.N, p.vec_out, o + c / 2);
+              if (c0 + c < p.N) store16(out, c0 + c, p.N, p.vec_out, o + c / 2);
           }
           buf ^= 1;
           if (buf == 0) bphase ^= 1;
@@ -693,18 +704,16 @@ static Plan plan_of(int64_t T, int K, int N, int rank) {
   return q;
 }
 
-static int make_map(CUtensorMap* tm, const void* base, int64_t inner, int64_t outer, int64_t ld_bytes, uint32_t box_inner,
-                    uint32_t box_outer, CUtensorMapDataType dt) {
+// b [R * N, rank] as pieces of eight columns: a box holds an adapter's 64 rows, piece after piece
+static int make_piece_map(CUtensorMap* tm, const void* b, int64_t rows, int rank, CUtensorMapDataType dt) {
   auto enc = tc::encode_fn();
   if (enc == nullptr) return fail(RB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
-  cuuint64_t strides[1] = {(cuuint64_t)ld_bytes};
-  cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
-  const CUtensorMapSwizzle sw = box_inner == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : box_inner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                                                               : CU_TENSOR_MAP_SWIZZLE_32B;
-  CUresult r = enc(tm, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  cuuint64_t dims[3] = {8, (cuuint64_t)rows, (cuuint64_t)(rank / 8)};
+  cuuint64_t strides[2] = {(cuuint64_t)rank * 2, 16};
+  cuuint32_t box[3] = {8, kChunk, (cuuint32_t)(rank / 8)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(tm, dt, 3, const_cast<void*>(b), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(RB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return RB_OK;
 }
@@ -751,13 +760,13 @@ static int run_tiles(Params& p, const Plan& q, CUtensorMapDataType dt, cudaStrea
   });
   if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(low-rank tile_kernel)");
   CUtensorMap tmX, tmA, tmB, tmY, tmO;
-  if ((rc = make_map(&tmX, p.x, p.K, p.T, p.ldx * 2, 64, kRows, dt))) return rc;
-  if ((rc = make_map(&tmA, p.a, p.K, (int64_t)p.R * p.rank, (int64_t)p.K * 2, 64, (uint32_t)p.rp, dt))) return rc;
-  if ((rc = make_map(&tmB, p.b, p.rank, (int64_t)p.R * p.N, (int64_t)p.rank * 2, (uint32_t)p.rp, kChunk, dt))) return rc;
+  if ((rc = tc::make_tmap(&tmX, p.x, p.K, p.T, p.ldx * 2, 64, kRows, dt))) return rc;
+  if ((rc = tc::make_tmap(&tmA, p.a, p.K, (int64_t)p.R * p.rank, (int64_t)p.K * 2, 64, (uint32_t)p.rank, dt))) return rc;
+  if ((rc = make_piece_map(&tmB, p.b, (int64_t)p.R * p.N, p.rank, dt))) return rc;
   tmY = tmO = tmX;  // not used where rows do not allow whole chunks
   if (p.chunk_io) {
-    if ((rc = make_map(&tmY, p.y, p.N, p.T, p.ldy * 2, kChunk, kRows, dt))) return rc;
-    if ((rc = make_map(&tmO, p.out, p.N, p.T, p.ldo * 2, kChunk, kRows, dt))) return rc;
+    if ((rc = tc::make_tmap(&tmY, p.y, p.N, p.T, p.ldy * 2, kChunk, kRows, dt))) return rc;
+    if ((rc = tc::make_tmap(&tmO, p.out, p.N, p.T, p.ldo * 2, kChunk, kRows, dt))) return rc;
   }
   if (q.splits == 1) {
     tile_kernel<T, kFused><<<q.tiles, kTileThreads, Tile<kFused>::kSmem, st>>>(tmX, tmA, tmB, tmY, tmO, p);
@@ -824,7 +833,6 @@ extern "C" int rb_low_rank_add(const void* y, int64_t ldy, const void* x, int64_
   p.R = R;
   p.rank = rank;
   p.idx64 = idx_dtype == RB_I64;
-  p.rp = rank <= 16 ? 16 : rank <= 32 ? 32 : 64;
   p.splits = 1;
   p.vec_y = vec_bytes(y, ldy);
   p.vec_out = vec_bytes(out, ldo);
