@@ -293,79 +293,88 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// A team's rows: first, first + step, ...  A arrays each.
-template <typename T, int G, int V, int A>
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+// A team's rows: first, first + step, ...  A arrays each.  BULK: by bulk copies (D a multiple of 8, rows on 16-byte
+// boundaries); else value by value through the same shared memory.
+template <typename T, int G, int V, int A, bool BULK>
 struct Rows {
   const Params& p;
   uint8_t* ring;   // this team's stages
   uint64_t* full;  // this team's barriers
   volatile int* abort_flag;
   int64_t first, step;
-  int D, stages;
+  const char* next;   // thread a < A of the team asks for array a: its next row, or null
+  int64_t next_step;  // bytes from one of the team's rows to the next
 
-  const char* next;     // thread a < A of the team asks for array a: its next row, or null
-  int64_t next_step;    // bytes from one of the team's rows to the next
-
-  __device__ uint8_t* slot(int stage, int a) const { return ring + (stage * A + a) * p.row_bytes; }
+  __device__ uint32_t slot(int stage, int a) const { return smem_u32(ring) + (uint32_t)((stage * A + a) * p.row_bytes); }
   __device__ void request(int stage) {  // the team's first warp
     const int lane = threadIdx.x & 31;
-    const uint32_t bytes = (uint32_t)(D * (int)sizeof(T));
+    const uint32_t bytes = (uint32_t)(p.D * (int)sizeof(T));
     const uint32_t bar = smem_u32(full + stage);
     if (lane == 0) mbar_arrive_expect_tx(bar, p.arrays * bytes);
     __syncwarp();
     if (next != nullptr) {
-      bulk_load(smem_u32(slot(stage, lane)), next, bytes, bar);
+      bulk_load(slot(stage, lane), next, bytes, bar);
       next += next_step;
     }
   }
   __device__ void start() {
-    const int r = Team<G>::rank();
     next = nullptr;
-    if (!p.bulk || r >= 32) return;
-    if (r < A && p.src[r] != nullptr) {
-      next = static_cast<const char*>(p.src[r]) + first * p.pitch[r];
-      next_step = step * p.pitch[r];
+    if constexpr (BULK) {
+      const int r = Team<G>::rank();
+      if (r >= 32) return;
+      if (r < A && p.src[r] != nullptr) {
+        next = static_cast<const char*>(p.src[r]) + first * p.pitch[r];
+        next_step = step * p.pitch[r];
+      }
+      for (int s = 0; s < p.stages; ++s)
+        if (first + s * step < p.N) request(s);
     }
-    for (int s = 0; s < stages; ++s)
-      if (first + s * step < p.N) request(s);
   }
   // Row `row`'s eights (zeros beyond D and for absent arrays) into registers; asks for the row `stages` turns on.
   __device__ bool take(int64_t row, int stage, uint32_t phase, Eight<T> (&e)[A][V]) {
     const int r = Team<G>::rank();
     bool ok = true;
-    if (p.bulk) {
+    if constexpr (BULK) {
       ok = mbar_wait_bounded(smem_u32(full + stage), phase, kWaitTimeoutProducer, abort_flag);
     } else {
-      // rows that no 16-byte copy can fetch: value by value, neighbours by neighbouring threads
+      // neighbours by neighbouring threads
 #pragma unroll
       for (int a = 0; a < A; ++a) {
         if (p.src[a] == nullptr) continue;
         const T* from = reinterpret_cast<const T*>(static_cast<const char*>(p.src[a]) + row * p.pitch[a]);
-        T* to = reinterpret_cast<T*>(slot(stage, a));
-        for (int c = r; c < D; c += G) to[c] = from[c];
+        T* to = reinterpret_cast<T*>(ring + (stage * A + a) * p.row_bytes);
+        for (int c = r; c < p.D; c += G) to[c] = from[c];
       }
       Team<G>::sync();
     }
+    const uint32_t base = slot(stage, 0);
 #pragma unroll
-    for (int a = 0; a < A; ++a)
+    for (int v = 0; v < V; ++v) {
+      const int c = (v * G + r) * 8;
+      const bool in = ok && c < p.D;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int c = (v * G + r) * 8;
+      for (int a = 0; a < A; ++a) {
 #pragma unroll
         for (int q = 0; q < (int)(sizeof(T) / 2); ++q) {
           e[a][v].q[q] = make_uint4(0u, 0u, 0u, 0u);
-          if (ok && p.src[a] != nullptr && c < D)
-            e[a][v].q[q] = reinterpret_cast<const uint4*>(slot(stage, a) + (int64_t)c * sizeof(T))[q];
+          if (in && p.src[a] != nullptr) e[a][v].q[q] = ld_shared(base + (uint32_t)(a * p.row_bytes + c * (int)sizeof(T) + 16 * q));
         }
-        if (c < D && c + 8 > D) {  // a row's last eight may be short
+        if (!BULK && c < p.D && c + 8 > p.D) {  // a row's last eight may be short
           T* t = reinterpret_cast<T*>(&e[a][v]);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (c + i >= D) t[i] = T(0.0f);
+            if (c + i >= p.D) t[i] = T(0.0f);
         }
       }
+    }
     ok = Team<G>::all(ok);
-    if (p.bulk && ok && r < 32 && row + stages * step < p.N) {
+    if (BULK && ok && r < 32 && row + p.stages * step < p.N) {
       // the slot was read through the generic proxy: order those reads before the copy's writes
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       request(stage);
@@ -374,68 +383,42 @@ struct Rows {
   }
   // After a wait that gave up at (row, stage, phase): the copies still in flight land before this CTA leaves.
   __device__ void drain(int64_t row, int stage, uint32_t phase) const {
-    if (!p.bulk || Team<G>::rank() != 0) return;
-    for (int s = 0; s < stages && row < p.N; ++s, row += step) {
+    if (!BULK || Team<G>::rank() != 0) return;
+    for (int s = 0; s < p.stages && row < p.N; ++s, row += step) {
       mbar_wait_bounded(smem_u32(full + stage), phase, kWaitTimeoutProducer, nullptr);
-      if (++stage == stages) {
+      if (++stage == p.stages) {
         stage = 0;
         phase ^= 1;
       }
     }
   }
-  // A row out: straight from registers, or (rows that 16-byte stores do not fit) through this stage's slot a
-  __device__ void put(void* out, int64_t row, int stage, int a, const F2 (&v)[V * 4]) const {
+  // A row out: straight from registers, or (rows that 16-byte stores do not fit) through this stage's first slot
+  __device__ void put(void* out, int64_t row, int stage, const F2 (&v)[V * 4]) const {
     const int r = Team<G>::rank();
-    T* to = static_cast<T*>(out) + row * D;
-    if (p.bulk) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int c = (k * G + r) * 8;
-        if (c >= D) continue;
-        Eight<T> e;
-        narrow2(v + 4 * k, e);
-#pragma unroll
-        for (int q = 0; q < (int)(sizeof(T) / 2); ++q) reinterpret_cast<uint4*>(to + c)[q] = e.q[q];
-      }
-      return;
-    }
-    T* via = reinterpret_cast<T*>(slot(stage, a));
+    T* to = static_cast<T*>(out) + row * p.D;
+    T* via = BULK ? to : reinterpret_cast<T*>(ring + stage * A * p.row_bytes);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const int c = (k * G + r) * 8;
-      if (c >= D) continue;
+      if (c >= p.D) continue;
       Eight<T> e;
       narrow2(v + 4 * k, e);
 #pragma unroll
       for (int q = 0; q < (int)(sizeof(T) / 2); ++q) reinterpret_cast<uint4*>(via + c)[q] = e.q[q];
     }
-    Team<G>::sync();
-    for (int c = r; c < D; c += G) to[c] = via[c];
-    Team<G>::sync();
+    if constexpr (!BULK) {
+      Team<G>::sync();
+      for (int c = r; c < p.D; c += G) to[c] = via[c];
+      Team<G>::sync();
+    }
   }
 };
 
-// zeros beyond a row's D: the columns of eight k of this thread begin at (k G + r) 8
-template <int G, int V>
-__device__ __forceinline__ void zero_tail(F2 (&v)[V * 4], int D) {
-  const int r = Team<G>::rank();
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const int c = (k * G + r) * 8;
-    if (c + 8 > D) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = un(v[4 * k + i]);
-        v[4 * k + i] = f2(c + 2 * i < D ? f.x : 0.0f, c + 2 * i + 1 < D ? f.y : 0.0f);
-      }
-    }
-  }
-}
-
-// v centred and normalised in place over the team's row; mean and 1 / deviation
-template <int G, int V>
+// v centred and normalised in place over the team's row (zeros beyond D stay zeros); mean and 1 / deviation
+template <int G, int V, bool BULK>
 __device__ __forceinline__ void normalise(F2 (&v)[V * 4], int kind, float eps, int D, float* room, int& turn,
-                                    float& mean, float& rstd) {
+                                          float& mean, float& rstd) {
+  const int r = Team<G>::rank();
   const float inv = 1.0f / (float)D;
   mean = 0.0f;
   if (kind == kLayer) {
@@ -445,10 +428,19 @@ __device__ __forceinline__ void normalise(F2 (&v)[V * 4], int kind, float eps, i
     float s[1] = {total(a)};
     Team<G>::sum(s, room, turn);
     mean = s[0] * inv;
-    const F2 m = f2(-mean, -mean);
 #pragma unroll
-    for (int i = 0; i < V * 4; ++i) v[i] = add2(v[i], m);
-    zero_tail<G, V>(v, D);
+    for (int k = 0; k < V; ++k) {
+      const int c = (k * G + r) * 8;
+      const F2 m = c < D ? f2(-mean, -mean) : f2(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[4 * k + i] = add2(v[4 * k + i], m);
+        if constexpr (!BULK) {
+          const float2 f = un(v[4 * k + i]);
+          v[4 * k + i] = f2(c + 2 * i < D ? f.x : 0.0f, c + 2 * i + 1 < D ? f.y : 0.0f);
+        }
+      }
+    }
   }
   F2 a = mul2(v[0], v[0]);
 #pragma unroll
@@ -472,7 +464,7 @@ __device__ __forceinline__ void init_ring(uint64_t* full, int stages, volatile i
   __syncthreads();
 }
 
-template <typename T, int G, int V, bool HOLD>
+template <typename T, int G, int V, bool BULK>
 __global__ void __launch_bounds__(Team<G>::kThreads, 512 / Team<G>::kThreads)
     sandwich_kernel(const __grid_constant__ Params p) {
   using Tm = Team<G>;
@@ -483,34 +475,25 @@ __global__ void __launch_bounds__(Team<G>::kThreads, 512 / Team<G>::kThreads)
   __shared__ int abort_flag;
   init_ring<G>(full, p.stages, &abort_flag);
   const int r = Tm::rank();
-  Rows<T, G, V, kArrays> rows{p,
-                              ring + Tm::index() * p.stages * kArrays * p.row_bytes,
-                              full + Tm::index() * p.stages,
-                              &abort_flag,
-                              (int64_t)blockIdx.x * Tm::kTeams + Tm::index(),
-                              (int64_t)gridDim.x * Tm::kTeams,
-                              p.D,
-                              p.stages,
-                              nullptr,
-                              0};
+  Rows<T, G, V, kArrays, BULK> rows{p,
+                                    ring + Tm::index() * p.stages * kArrays * p.row_bytes,
+                                    full + Tm::index() * p.stages,
+                                    &abort_flag,
+                                    (int64_t)blockIdx.x * Tm::kTeams + Tm::index(),
+                                    (int64_t)gridDim.x * Tm::kTeams,
+                                    nullptr,
+                                    0};
   rows.start();
 
-  Columns cols{&p, nullptr, (p.D + 7) / 8 * 8};
-  F2 held[HOLD ? 4 : 1][HOLD ? V * 4 : 1];
-  if constexpr (HOLD) {
+  const Columns cols{&p, nullptr, 0};
+  F2 A[V * 4], B[V * 4], w2[V * 4], b2[V * 4];  // zeros beyond D
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = (k * G + r) * 8;
-      column8<0>(cols, c, held[0] + 4 * k);
-      column8<1>(cols, c, held[1] + 4 * k);
-      column8<2>(cols, c, held[2] + 4 * k);
-      column8<3>(cols, c, held[3] + 4 * k);
-    }
-  } else if (p.table_at >= 0) {
-    float* table = reinterpret_cast<float*>(ring + p.table_at);
-    fill_table<4>(p, table, cols.pitch);
-    __syncthreads();
-    cols.table = table;
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * G + r) * 8;
+    column8<0>(cols, c, A + 4 * k);
+    column8<1>(cols, c, B + 4 * k);
+    column8<2>(cols, c, w2 + 4 * k);
+    column8<3>(cols, c, b2 + 4 * k);
   }
 
   int stage = 0, turn = 0;
@@ -533,18 +516,11 @@ __global__ void __launch_bounds__(Team<G>::kThreads, 512 / Team<G>::kThreads)
     float mean1 = 0.0f, rstd1 = 1.0f, mean2 = 0.0f, rstd2 = 1.0f;
 #pragma unroll
     for (int k = 0; k < V; ++k) widen2(e[1][k], n + 4 * k);
-    if (p.post != kNone) normalise<G, V>(n, p.post, p.eps1, p.D, room, turn, mean1, rstd1);
+    if (p.post != kNone) normalise<G, V, BULK>(n, p.post, p.eps1, p.D, room, turn, mean1, rstd1);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int c = (k * G + r) * 8;
-      F2 A[4], B[4];
-      if constexpr (!HOLD) {
-        column8<0>(cols, c, A);
-        column8<1>(cols, c, B);
-      }
-      F2 x[4];
+      F2 x[4], a[4] = {row_gate, row_gate, row_gate, row_gate};
       widen2(e[0][k], x);
-      F2 a[4] = {row_gate, row_gate, row_gate, row_gate};
       if (p.gate_kind == kGateFull) {
         float g[8];
         widen(e[2][k], g);
@@ -552,30 +528,14 @@ __global__ void __launch_bounds__(Team<G>::kThreads, 512 / Team<G>::kThreads)
         for (int i = 0; i < 4; ++i) a[i] = f2(gate_act(g[2 * i], p.act), gate_act(g[2 * i + 1], p.act));
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const F2 q = HOLD ? fma2(n[4 * k + i], held[0][HOLD ? 4 * k + i : 0], held[1][HOLD ? 4 * k + i : 0])
-                          : fma2(n[4 * k + i], A[i], B[i]);
-        y[4 * k + i] = fma2(a[i], q, x[i]);
-      }
+      for (int i = 4 * k; i < 4 * k + 4; ++i) y[i] = fma2(a[i & 3], fma2(n[i], A[i], B[i]), x[i & 3]);
     }
-    zero_tail<G, V>(y, p.D);
-    rows.put(p.out0, row, stage, 0, y);
+    rows.put(p.out0, row, stage, y);
     if (p.pre != kNone) {
-      normalise<G, V>(y, p.pre, p.eps2, p.D, room, turn, mean2, rstd2);
+      normalise<G, V, BULK>(y, p.pre, p.eps2, p.D, room, turn, mean2, rstd2);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int c = (k * G + r) * 8;
-        F2 w[4], b[4];
-        if constexpr (!HOLD) {
-          column8<2>(cols, c, w);
-          column8<3>(cols, c, b);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          y[4 * k + i] = HOLD ? fma2(y[4 * k + i], held[2][HOLD ? 4 * k + i : 0], held[3][HOLD ? 4 * k + i : 0])
-                              : fma2(y[4 * k + i], w[i], b[i]);
-      }
-      rows.put(p.out1, row, stage, 0, y);
+      for (int i = 0; i < V * 4; ++i) y[i] = fma2(y[i], w2[i], b2[i]);
+      rows.put(p.out1, row, stage, y);
     }
     if (p.stats != nullptr && r == 0)
       reinterpret_cast<float4*>(p.stats)[row] = make_float4(mean1, rstd1, mean2, rstd2);
@@ -586,41 +546,36 @@ __global__ void __launch_bounds__(Team<G>::kThreads, 512 / Team<G>::kThreads)
   }
 }
 
-// LEAN: no biases and no gate per channel: the column sums P and dw alone.
-template <typename T, int G, int V, bool HOLD, bool LEAN>
+// LEAN: no biases and no gate per channel: the column sums P and dw alone.  FULL: a gate of every element.  HOLD:
+// the column constants are in registers.  Eight values a thread.
+template <typename T, int G, bool BULK, bool HOLD, bool LEAN, bool FULL>
 __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 512 / Team<G>::kThreads : 1)
     sandwich_backward_kernel(const __grid_constant__ Params p) {
   using Tm = Team<G>;
-  constexpr int kArrays = 5;  // x, h, dy, dz, a gate of every element
-  constexpr int NV = V * 8;
+  constexpr int kArrays = FULL ? 5 : 4;  // x, h, dy, dz, a gate of every element
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ __align__(8) uint64_t full[kMaxStages * Tm::kTeams];
   __shared__ float room[Tm::kRoom];
   __shared__ int abort_flag;
   init_ring<G>(full, p.stages, &abort_flag);
-  const int r = Tm::rank();
-  Rows<T, G, V, kArrays> rows{p,
-                              ring + Tm::index() * p.stages * kArrays * p.row_bytes,
-                              full + Tm::index() * p.stages,
-                              &abort_flag,
-                              (int64_t)blockIdx.x * Tm::kTeams + Tm::index(),
-                              (int64_t)gridDim.x * Tm::kTeams,
-                              p.D,
-                              p.stages,
-                              nullptr,
-                              0};
+  const int r = Tm::rank(), c = 8 * r;
+  Rows<T, G, 1, kArrays, BULK> rows{p,
+                                    ring + Tm::index() * p.stages * kArrays * p.row_bytes,
+                                    full + Tm::index() * p.stages,
+                                    &abort_flag,
+                                    (int64_t)blockIdx.x * Tm::kTeams + Tm::index(),
+                                    (int64_t)gridDim.x * Tm::kTeams,
+                                    nullptr,
+                                    0};
   rows.start();
 
+  // A, B and the pre norm's w are zeros beyond D, as x, h, dy and dz are: what a thread computes there reaches no sum
   Columns cols{&p, nullptr, (p.D + 7) / 8 * 8};
-  F2 held[HOLD ? 3 : 1][HOLD ? V * 4 : 1];  // A, B, the pre norm's w
+  F2 A[4], B[4], w2[4];
   if constexpr (HOLD) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = (k * G + r) * 8;
-      column8<0>(cols, c, held[0] + 4 * k);
-      column8<1>(cols, c, held[1] + 4 * k);
-      column8<2>(cols, c, held[2] + 4 * k);
-    }
+    column8<0>(cols, c, A);
+    column8<1>(cols, c, B);
+    column8<2>(cols, c, w2);
   } else if (p.table_at >= 0) {
     float* table = reinterpret_cast<float*>(ring + p.table_at);
     fill_table<3>(p, table, cols.pitch);
@@ -629,14 +584,14 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
   }
 
   constexpr int kHeld = LEAN ? 2 : kSums;
-  F2 acc[kHeld][NV / 2];  // P, dw, then Q, db
+  F2 acc[kHeld][4];  // P, dw, then Q, db
 #pragma unroll
   for (int a = 0; a < kHeld; ++a)
 #pragma unroll
-    for (int i = 0; i < NV / 2; ++i) acc[a][i] = f2(0.0f, 0.0f);
+    for (int i = 0; i < 4; ++i) acc[a][i] = f2(0.0f, 0.0f);
 
-  const float inv = 1.0f / (float)p.D;
-  const bool mean1 = p.post == kLayer, mean2 = p.pre == kLayer;
+  const float inv1 = p.post == kLayer ? -1.0f / (float)p.D : 0.0f, inv2 = p.pre == kLayer ? -1.0f / (float)p.D : 0.0f;
+  const float inv = -1.0f / (float)p.D;
   int stage = 0, turn = 0;
   uint32_t phase = 0;
   float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
@@ -644,147 +599,114 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
   auto ahead = [&](int64_t row) {  // the next row's scalars
     if (row < p.N) {
       st = __ldg(reinterpret_cast<const float4*>(p.stats) + row);
-      if (p.gate_kind == kGateRow) g_row = gate_act(load_as_f32(p.gate, p.gate_dtype, row * p.ldg), p.act);
+      if (!FULL && p.gate_kind == kGateRow) g_row = gate_act(load_as_f32(p.gate, p.gate_dtype, row * p.ldg), p.act);
     }
   };
   ahead(rows.first);
   for (int64_t row = rows.first; row < p.N; row += rows.step) {
     const float4 s = st;
-    const F2 a_row = f2(g_row, g_row);
-    Eight<T> e[kArrays][V];
+    const float ar = g_row;
+    Eight<T> e[kArrays][1];
     if (!rows.take(row, stage, phase, e)) {
       rows.drain(row, stage, phase);
       break;
     }
     ahead(row + rows.step);
-    F2 hh[NV / 2], yh[NV / 2], t[NV / 2], a[NV / 2];
+    // the gates of this row; without gates of every element one value, in every a[i]
+    F2 a[FULL ? 4 : 1];
+    if constexpr (FULL) {
+      float g[8];
+      widen(e[4][0], g);
 #pragma unroll
-    for (int i = 0; i < NV / 2; ++i) a[i] = a_row;
-    if (p.gate_kind == kGateFull) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        float g[8];
-        widen(e[4][k], g);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[4 * k + i] = f2(gate_act(g[2 * i], p.act), gate_act(g[2 * i + 1], p.act));
-      }
+      for (int i = 0; i < 4; ++i) a[i] = f2(gate_act(g[2 * i], p.act), gate_act(g[2 * i + 1], p.act));
+    } else {
+      a[0] = f2(ar, ar);
     }
-    // v^ of the post norm, and with n and y made again the pre norm's two sums
+    F2 hh[4], yh[4], t[4];
+    widen2(e[1][0], hh);
     {
-      const F2 m = f2(-s.x, -s.x), q = f2(s.y, s.y);
+      const F2 q = f2(s.y, s.y), m = f2(-s.x * s.y, -s.x * s.y);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        widen2(e[1][k], hh + 4 * k);
-#pragma unroll
-        for (int i = 4 * k; i < 4 * k + 4; ++i) hh[i] = mul2(add2(hh[i], m), q);
-      }
-      zero_tail<G, V>(hh, p.D);
+      for (int i = 0; i < 4; ++i) hh[i] = fma2(hh[i], q, m);
     }
     if (p.pre != kNone) {
-      const F2 m = f2(-s.z, -s.z), q = f2(s.w, s.w);
-      F2 s1 = f2(0.0f, 0.0f), s2 = s1;
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int c = (k * G + r) * 8;
-        F2 A[4], B[4], x[4];
-        if constexpr (!HOLD) {
-          column8<0>(cols, c, A);
-          column8<1>(cols, c, B);
-        }
-        widen2(e[0][k], x);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = 4 * k + i;
-          const F2 n = HOLD ? fma2(hh[j], held[0][HOLD ? j : 0], held[1][HOLD ? j : 0]) : fma2(hh[j], A[i], B[i]);
-          yh[j] = mul2(add2(fma2(a[j], n, x[i]), m), q);
-        }
-      }
-      zero_tail<G, V>(yh, p.D);
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int c = (k * G + r) * 8;
-        F2 w[4], dz[4];
-        if constexpr (!HOLD) column8<2>(cols, c, w);
-        widen2(e[3][k], dz);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = 4 * k + i;
-          const F2 u = HOLD ? mul2(dz[i], held[2][HOLD ? j : 0]) : mul2(dz[i], w[i]);
-          t[j] = u;
-          s1 = add2(s1, u);
-          s2 = fma2(u, yh[j], s2);
-          acc[1][j] = fma2(dz[i], yh[j], acc[1][j]);
-          if constexpr (!LEAN) acc[3][j] = add2(acc[3][j], dz[i]);
-        }
-      }
-      float s12[2] = {total(s1), total(s2)};
-      Tm::sum(s12, room, turn);
-      const F2 c1 = mean2 ? f2(-s12[0] * inv, -s12[0] * inv) : f2(0.0f, 0.0f), c2 = f2(-s12[1] * inv, -s12[1] * inv);
-#pragma unroll
-      for (int i = 0; i < NV / 2; ++i) t[i] = mul2(fma2(yh[i], c2, add2(t[i], c1)), q);
-    } else {
-#pragma unroll
-      for (int i = 0; i < NV / 2; ++i) t[i] = f2(0.0f, 0.0f);
-    }
-    // t reaches y; its way into h, the gate and the post norm's weights
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      F2 dy[4];
-      widen2(e[2][k], dy);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) t[4 * k + i] = add2(t[4 * k + i], dy[i]);
-    }
-    zero_tail<G, V>(t, p.D);
-    rows.put(p.out0, row, stage, 0, t);
-    F2 s3 = f2(0.0f, 0.0f), s4 = s3, s5 = s3;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = (k * G + r) * 8;
-      F2 A[4], B[4];
+      // n and y again, and the pre norm's two sums
+      const F2 q = f2(s.w, s.w), m = f2(-s.z * s.w, -s.z * s.w);
+      F2 s1 = f2(0.0f, 0.0f), s2 = s1, x[4], dz[4];
       if constexpr (!HOLD) {
         column8<0>(cols, c, A);
         column8<1>(cols, c, B);
+        column8<2>(cols, c, w2);
       }
-      if (p.gate_kind == kGateFull || p.gate_kind == kGateRow) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = 4 * k + i;
-          F2 da = mul2(HOLD ? fma2(hh[j], held[0][HOLD ? j : 0], held[1][HOLD ? j : 0]) : fma2(hh[j], A[i], B[i]), t[j]);
-          if (p.act == kActSigmoid) da = mul2(da, mul2(a[j], sub2(f2(1.0f, 1.0f), a[j])));
-          yh[j] = da;  // of every element: its gradient
-          s5 = add2(s5, da);
-        }
-      }
+      widen2(e[0][0], x);
+      widen2(e[3][0], dz);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int j = 4 * k + i;
-        const F2 Aj = HOLD ? held[0][HOLD ? j : 0] : A[i];
-        const F2 tp = mul2(a[j], t[j]);
-        acc[0][j] = fma2(tp, hh[j], acc[0][j]);
-        if constexpr (!LEAN) acc[2][j] = add2(acc[2][j], tp);
-        const F2 v = mul2(tp, Aj);
-        t[j] = v;
-        s3 = add2(s3, v);
-        s4 = fma2(v, hh[j], s4);
+        yh[i] = fma2(fma2(a[FULL ? i : 0], fma2(hh[i], A[i], B[i]), x[i]), q, m);
+        t[i] = mul2(dz[i], w2[i]);
+        s1 = add2(s1, t[i]);
+        s2 = fma2(t[i], yh[i], s2);
+        acc[1][i] = fma2(dz[i], yh[i], acc[1][i]);
+        if constexpr (!LEAN) acc[3][i] = add2(acc[3][i], dz[i]);
+      }
+      float s12[2] = {total(s1), total(s2)};
+      Tm::sum(s12, room, turn);
+      const float c1 = s12[0] * inv2 * s.w, c2 = s12[1] * inv * s.w;
+      const F2 k1 = f2(c1, c1), k2 = f2(c2, c2);
+      F2 dy[4];
+      widen2(e[2][0], dy);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = add2(fma2(yh[i], k2, fma2(t[i], q, k1)), dy[i]);
+    } else {
+      widen2(e[2][0], t);
+    }
+    // t reaches y; its way into h, the gate and the post norm's weights
+    rows.put(p.out0, row, stage, t);
+    if constexpr (!HOLD) {
+      column8<0>(cols, c, A);
+      column8<1>(cols, c, B);
+    }
+    F2 s3 = f2(0.0f, 0.0f), s4 = s3, s5 = s3;
+    if (FULL || p.gate_kind == kGateRow) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const F2 ai = a[FULL ? i : 0];
+        F2 da = mul2(fma2(hh[i], A[i], B[i]), t[i]);
+        if (p.act == kActSigmoid) da = mul2(da, fma2(mul2(ai, f2(-1.0f, -1.0f)), ai, ai));
+        yh[i] = da;  // of every element: its gradient
+        s5 = add2(s5, da);
       }
     }
-    if (p.gate_kind == kGateFull) rows.put(p.out2, row, stage, 0, yh);
-    if (p.post != kNone || p.gate_kind == kGateRow) {
-      float s345[3] = {total(s3), total(s4), total(s5)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const F2 tp = mul2(a[FULL ? i : 0], t[i]);
+      acc[0][i] = fma2(tp, hh[i], acc[0][i]);
+      if constexpr (!LEAN) acc[2][i] = add2(acc[2][i], tp);
+      t[i] = mul2(tp, A[i]);
+      s3 = add2(s3, t[i]);
+      s4 = fma2(t[i], hh[i], s4);
+    }
+    if constexpr (FULL) rows.put(p.out2, row, stage, yh);
+    if (p.post != kNone || (!FULL && p.gate_kind == kGateRow)) {
+      float s345[FULL ? 2 : 3];
+      s345[0] = total(s3);
+      s345[1] = total(s4);
+      if constexpr (!FULL) s345[2] = total(s5);
       Tm::sum(s345, room, turn);
-      if (p.gate_kind == kGateRow && r == 0) {
-        if (p.gate_dtype == RB_F32) static_cast<float*>(p.out2)[row] = s345[2];
-        else if (p.gate_dtype == RB_BF16) static_cast<__nv_bfloat16*>(p.out2)[row] = __float2bfloat16_rn(s345[2]);
-        else static_cast<__half*>(p.out2)[row] = __float2half_rn(s345[2]);
+      if (!FULL && p.gate_kind == kGateRow && r == 0) {
+        const float d = s345[FULL ? 0 : 2];
+        if (p.gate_dtype == RB_F32) static_cast<float*>(p.out2)[row] = d;
+        else if (p.gate_dtype == RB_BF16) static_cast<__nv_bfloat16*>(p.out2)[row] = __float2bfloat16_rn(d);
+        else static_cast<__half*>(p.out2)[row] = __float2half_rn(d);
       }
       if (p.post != kNone) {
-        const F2 c3 = mean1 ? f2(-s345[0] * inv, -s345[0] * inv) : f2(0.0f, 0.0f), c4 = f2(-s345[1] * inv, -s345[1] * inv);
-        const F2 q = f2(s.y, s.y);
+        const float c3 = s345[0] * inv1 * s.y, c4 = s345[1] * inv * s.y;
+        const F2 k3 = f2(c3, c3), k4 = f2(c4, c4), q = f2(s.y, s.y);
 #pragma unroll
-        for (int i = 0; i < NV / 2; ++i) t[i] = mul2(fma2(hh[i], c4, add2(t[i], c3)), q);
+        for (int i = 0; i < 4; ++i) t[i] = fma2(hh[i], k4, fma2(t[i], q, k3));
       }
     }
-    rows.put(p.out1, row, stage, 0, t);
+    rows.put(p.out1, row, stage, t);
     if (++stage == p.stages) {
       stage = 0;
       phase ^= 1;
@@ -801,12 +723,8 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
 #pragma unroll
     for (int a = 0; a < kHeld; ++a)
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int c = (k * G + r) * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c + i < p.D) p.partial[((int64_t)blockIdx.x * kSums + a) * p.D + c + i] = held_sum(a, 8 * k + i);
-      }
+      for (int i = 0; i < 8; ++i)
+        if (c + i < p.D) p.partial[((int64_t)blockIdx.x * kSums + a) * p.D + c + i] = held_sum(a, i);
   } else {
     __syncthreads();  // every team is done with the ring
     float* sums = reinterpret_cast<float*>(ring);
@@ -815,21 +733,17 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
 #pragma unroll
         for (int a = 0; a < kHeld; ++a)
 #pragma unroll
-          for (int k = 0; k < V; ++k) {
-            const int c = (k * G + r) * 8;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (c + i < p.D) {
-                float* at = sums + a * p.D + c + i;
-                *at = (w == 0 ? 0.0f : *at) + held_sum(a, 8 * k + i);
-              }
-          }
+          for (int i = 0; i < 8; ++i)
+            if (c + i < p.D) {
+              float* at = sums + a * p.D + c + i;
+              *at = (w == 0 ? 0.0f : *at) + held_sum(a, i);
+            }
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < kHeld * p.D; c += Tm::kThreads) {
-      const int a = c / p.D;
-      p.partial[((int64_t)blockIdx.x * kSums + a) * p.D + (c - a * p.D)] = sums[c];
+    for (int j = threadIdx.x; j < kHeld * p.D; j += Tm::kThreads) {
+      const int a = j / p.D;
+      p.partial[((int64_t)blockIdx.x * kSums + a) * p.D + (j - a * p.D)] = sums[j];
     }
   }
 }
@@ -923,14 +837,14 @@ static int64_t ring_budget(int team, int threads) {
   return (int64_t)200 * 1024 / std::max(1, threads / cta);
 }
 constexpr int kForwardThreads = 512, kBackwardThreads = 512;  // an SM's, by the kernels' registers
-static Shape backward_shape(int D, int elt) {
+static Shape backward_shape(int D, int elt, bool full) {
   const int team = team_of(D);
-  Shape s = shape_of(team, 5, D, elt, ring_budget(team, kBackwardThreads), team >= 640 ? 3 : 0);
+  Shape s = shape_of(team, full ? 5 : 4, D, elt, ring_budget(team, kBackwardThreads), team >= 640 ? 3 : 0);
   if (s.teams > 1) s.smem = std::max(s.smem, kSums * D * 4);
   return s;
 }
-static int backward_ctas(int D, int elt, int64_t N) {
-  const Shape s = backward_shape(D, elt);
+static int backward_ctas(int D, int elt, int64_t N) {  // the same with and without gates of every element
+  const Shape s = backward_shape(D, elt, true);
   return (int)std::min<int64_t>((N + s.teams - 1) / s.teams, (int64_t)sm_count() * ctas_per_sm(s, kBackwardThreads));
 }
 
@@ -961,42 +875,50 @@ static int forward(Params& p, cudaStream_t st) {
   p.table_at = s.table_at;
   const int ctas = (int)std::min<int64_t>((p.N + s.teams - 1) / s.teams, (int64_t)sm_count() * ctas_per_sm(s, kForwardThreads));
   const char* name = "sandwich_kernel launch";
+#define RB_FORWARD(G, V)                                                      \
+  return p.bulk ? launch<sandwich_kernel<T, G, V, true>>(p, s, ctas, st, name) \
+                : launch<sandwich_kernel<T, G, V, false>>(p, s, ctas, st, name)
   if (two) {
     switch (team) {
-      case 32: return launch<sandwich_kernel<T, 32, 2, true>>(p, s, ctas, st, name);
-      case 64: return launch<sandwich_kernel<T, 64, 2, true>>(p, s, ctas, st, name);
-      case 128: return launch<sandwich_kernel<T, 128, 2, true>>(p, s, ctas, st, name);
-      case 256: return launch<sandwich_kernel<T, 256, 2, true>>(p, s, ctas, st, name);
-      default: return launch<sandwich_kernel<T, 512, 2, true>>(p, s, ctas, st, name);
+      case 32: RB_FORWARD(32, 2);
+      case 64: RB_FORWARD(64, 2);
+      case 128: RB_FORWARD(128, 2);
+      case 256: RB_FORWARD(256, 2);
+      default: RB_FORWARD(512, 2);
     }
   }
-  switch (team) {
-    case 32: return launch<sandwich_kernel<T, 32, 1, true>>(p, s, ctas, st, name);
-    case 64: return launch<sandwich_kernel<T, 64, 1, true>>(p, s, ctas, st, name);
-    case 128: return launch<sandwich_kernel<T, 128, 1, true>>(p, s, ctas, st, name);
-    case 256: return launch<sandwich_kernel<T, 256, 1, true>>(p, s, ctas, st, name);
-    case 512: return launch<sandwich_kernel<T, 512, 1, true>>(p, s, ctas, st, name);
-    case 640: return launch<sandwich_kernel<T, 640, 1, true>>(p, s, ctas, st, name);
-    default: return launch<sandwich_kernel<T, 1024, 1, true>>(p, s, ctas, st, name);
-  }
+  if (team == 32) RB_FORWARD(32, 1);
+  RB_FORWARD(640, 1);
+#undef RB_FORWARD
 }
 
-template <typename T, bool LEAN>
-static int backward(Params& p, cudaStream_t st) {
-  const Shape s = backward_shape(p.D, (int)sizeof(T));
+template <typename T, int G, bool HOLD, bool LEAN>
+static int backward_of(const Params& p, const Shape& s, int ctas, cudaStream_t st) {
+  const char* name = "sandwich_backward_kernel launch";
+  const bool full = p.gate_kind == kGateFull;
+  if (!p.bulk)
+    return full ? launch<sandwich_backward_kernel<T, G, false, HOLD, false, true>>(p, s, ctas, st, name)
+                : launch<sandwich_backward_kernel<T, G, false, HOLD, false, false>>(p, s, ctas, st, name);
+  return full ? launch<sandwich_backward_kernel<T, G, true, HOLD, LEAN, true>>(p, s, ctas, st, name)
+              : launch<sandwich_backward_kernel<T, G, true, HOLD, LEAN, false>>(p, s, ctas, st, name);
+}
+
+template <typename T>
+static int backward(Params& p, bool lean, cudaStream_t st) {
+  const Shape s = backward_shape(p.D, (int)sizeof(T), p.gate_kind == kGateFull);
   p.stages = s.stages;
   p.row_bytes = s.row_bytes;
   p.table_at = s.table_at;
   const int ctas = backward_ctas(p.D, (int)sizeof(T), p.N);
-  const char* name = "sandwich_backward_kernel launch";
   switch (team_of(p.D)) {
-    case 32: return launch<sandwich_backward_kernel<T, 32, 1, true, LEAN>>(p, s, ctas, st, name);
-    case 64: return launch<sandwich_backward_kernel<T, 64, 1, true, LEAN>>(p, s, ctas, st, name);
-    case 128: return launch<sandwich_backward_kernel<T, 128, 1, true, LEAN>>(p, s, ctas, st, name);
-    case 256: return launch<sandwich_backward_kernel<T, 256, 1, true, LEAN>>(p, s, ctas, st, name);
-    case 512: return launch<sandwich_backward_kernel<T, 512, 1, true, LEAN>>(p, s, ctas, st, name);
-    case 640: return launch<sandwich_backward_kernel<T, 640, 1, false, LEAN>>(p, s, ctas, st, name);
-    default: return launch<sandwich_backward_kernel<T, 1024, 1, false, LEAN>>(p, s, ctas, st, name);
+    case 32: return backward_of<T, 32, true, false>(p, s, ctas, st);
+    case 64: return backward_of<T, 64, true, false>(p, s, ctas, st);
+    case 128: return backward_of<T, 128, true, false>(p, s, ctas, st);
+    case 256: return backward_of<T, 256, true, false>(p, s, ctas, st);
+    case 512: return backward_of<T, 512, true, false>(p, s, ctas, st);
+    // wider teams have fewer registers a thread: without biases and channel gates two sums are left out
+    case 640: return lean ? backward_of<T, 640, false, true>(p, s, ctas, st) : backward_of<T, 640, false, false>(p, s, ctas, st);
+    default: return lean ? backward_of<T, 1024, false, true>(p, s, ctas, st) : backward_of<T, 1024, false, false>(p, s, ctas, st);
   }
 }
 
@@ -1145,11 +1067,12 @@ extern "C" int rb_sandwich_norm_backward(const void* dy, int64_t ldy, const void
   SumOut o{dw1, db1, dw2, db2, gate_kind == kGateChannel ? dgate : nullptr};
   p.need_sums = o.dw1 != nullptr || o.db1 != nullptr || o.dw2 != nullptr || o.db2 != nullptr || o.dgate != nullptr;
   cudaStream_t st = (cudaStream_t)stream;
+  // (the narrow teams and rows that no bulk copy fetches keep all sums)
   const bool lean = o.db1 == nullptr && o.db2 == nullptr && o.dgate == nullptr;
   if (N > 0) {
-    if (dtype == RB_BF16) rc = lean ? backward<__nv_bfloat16, true>(p, st) : backward<__nv_bfloat16, false>(p, st);
-    else if (dtype == RB_F16) rc = lean ? backward<__half, true>(p, st) : backward<__half, false>(p, st);
-    else rc = lean ? backward<float, true>(p, st) : backward<float, false>(p, st);
+    rc = dtype == RB_BF16 ? backward<__nv_bfloat16>(p, lean, st)
+         : dtype == RB_F16 ? backward<__half>(p, lean, st)
+                           : backward<float>(p, lean, st);
     if (rc) return rc;
   }
   if (!p.need_sums) return RB_OK;
