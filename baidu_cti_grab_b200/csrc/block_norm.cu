@@ -150,14 +150,10 @@ __device__ __forceinline__ float total(F2 v) {
 }
 
 // What a column's constants come to: out of the post norm, y = x + a (A v^ + B) with A = scale a_c w, B = scale a_c b,
-// a_c the channel's gate (1 without one) and a the row's or element's; the pre norm's w and b.  A thread's columns
-// stay its own for all rows, so the constants are made once: registers hold them where HOLD, shared memory as fp32
-// where a thread would need too many registers and they fit (`table`), else they are made again for each row.
-struct Columns {
-  const Params* p;
-  const float* table;  // [4][pitch] A, B, w, b of the pre norm, or null
-  int pitch;
-};
+// a_c the channel's gate (1 without one) and a the row's or element's; the pre norm's w and b; zeros beyond D.  A
+// thread's columns stay its own for all rows, so they are made once and held in registers; where a thread has too few
+// of those (backward, wider than 5120) in shared memory as fp32, and where that is full too they are made for each row.
+enum Where : int { kRegisters = 0, kTable = 1, kAgain = 2 };
 __device__ __forceinline__ float gate_act(float g, int act);
 template <int WHICH>
 __device__ __forceinline__ void make_column8(const Params& p, int c, float* v) {
@@ -172,45 +168,31 @@ __device__ __forceinline__ void make_column8(const Params& p, int c, float* v) {
   }
 }
 template <int WHICH>
-__device__ __forceinline__ void column8(const Columns& t, int c, F2* v) {
+__device__ __forceinline__ void column8(const Params& p, int c, F2* v) {
   float f[8];
-  if (t.table != nullptr) {
-    if (c >= t.pitch) {  // a thread whose columns lie beyond the row
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = f2(0.0f, 0.0f);
-      return;
-    }
-    const float4* at = reinterpret_cast<const float4*>(t.table + WHICH * t.pitch + c);
-    const float4 a = at[0], b = at[1];
-    v[0] = f2(a.x, a.y);
-    v[1] = f2(a.z, a.w);
-    v[2] = f2(b.x, b.y);
-    v[3] = f2(b.z, b.w);
-    return;
-  }
-  make_column8<WHICH>(*t.p, c, f);
+  make_column8<WHICH>(p, c, f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
 }
-// the table's first `n` rows, by all threads of the CTA
-template <int N>
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+// eight of a row of the table, from a shared address
+__device__ __forceinline__ void table8(uint32_t at, F2* v) {
+  const uint4 a = ld_shared(at), b = ld_shared(at + 16);
+  v[0] = f2(__uint_as_float(a.x), __uint_as_float(a.y));
+  v[1] = f2(__uint_as_float(a.z), __uint_as_float(a.w));
+  v[2] = f2(__uint_as_float(b.x), __uint_as_float(b.y));
+  v[3] = f2(__uint_as_float(b.z), __uint_as_float(b.w));
+}
+// the table [3][pitch] of A, B and the pre norm's w, by all threads of the CTA
 __device__ __forceinline__ void fill_table(const Params& p, float* table, int pitch) {
   for (int c = threadIdx.x * 8; c < pitch; c += blockDim.x * 8) {
-    float f[8];
-    auto put = [&](int which) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) table[which * pitch + c + i] = f[i];
-    };
-    make_column8<0>(p, c, f);
-    put(0);
-    make_column8<1>(p, c, f);
-    put(1);
-    make_column8<2>(p, c, f);
-    put(2);
-    if constexpr (N > 3) {
-      make_column8<3>(p, c, f);
-      put(3);
-    }
+    make_column8<0>(p, c, table + c);
+    make_column8<1>(p, c, table + pitch + c);
+    make_column8<2>(p, c, table + 2 * pitch + c);
   }
 }
 
@@ -291,12 +273,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
-}
-
-__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-  return v;
 }
 
 // A team's rows: first, first + step, ...  A arrays each.  BULK: by bulk copies (D a multiple of 8, rows on 16-byte
@@ -383,12 +359,14 @@ struct Rows {
   }
   // After a wait that gave up at (row, stage, phase): the copies still in flight land before this CTA leaves.
   __device__ void drain(int64_t row, int stage, uint32_t phase) const {
-    if (!BULK || Team<G>::rank() != 0) return;
-    for (int s = 0; s < p.stages && row < p.N; ++s, row += step) {
-      mbar_wait_bounded(smem_u32(full + stage), phase, kWaitTimeoutProducer, nullptr);
-      if (++stage == p.stages) {
-        stage = 0;
-        phase ^= 1;
+    if constexpr (BULK) {
+      if (Team<G>::rank() != 0) return;
+      for (int s = 0; s < p.stages && row < p.N; ++s, row += step) {
+        mbar_wait_bounded(smem_u32(full + stage), phase, kWaitTimeoutProducer, nullptr);
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
     }
   }
@@ -465,7 +443,7 @@ __device__ __forceinline__ void init_ring(uint64_t* full, int stages, volatile i
 }
 
 template <typename T, int G, int V, bool BULK>
-__global__ void __launch_bounds__(Team<G>::kThreads, 512 / Team<G>::kThreads)
+__global__ void __launch_bounds__(Team<G>::kThreads, G == 320 ? 2 : 512 / Team<G>::kThreads)
     sandwich_kernel(const __grid_constant__ Params p) {
   using Tm = Team<G>;
   constexpr int kArrays = 3;  // x, h, a gate of every element
@@ -485,15 +463,14 @@ __global__ void __launch_bounds__(Team<G>::kThreads, 512 / Team<G>::kThreads)
                                     0};
   rows.start();
 
-  const Columns cols{&p, nullptr, 0};
   F2 A[V * 4], B[V * 4], w2[V * 4], b2[V * 4];  // zeros beyond D
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     const int c = (k * G + r) * 8;
-    column8<0>(cols, c, A + 4 * k);
-    column8<1>(cols, c, B + 4 * k);
-    column8<2>(cols, c, w2 + 4 * k);
-    column8<3>(cols, c, b2 + 4 * k);
+    column8<0>(p, c, A + 4 * k);
+    column8<1>(p, c, B + 4 * k);
+    column8<2>(p, c, w2 + 4 * k);
+    column8<3>(p, c, b2 + 4 * k);
   }
 
   int stage = 0, turn = 0;
@@ -546,9 +523,9 @@ __global__ void __launch_bounds__(Team<G>::kThreads, 512 / Team<G>::kThreads)
   }
 }
 
-// LEAN: no biases and no gate per channel: the column sums P and dw alone.  FULL: a gate of every element.  HOLD:
-// the column constants are in registers.  Eight values a thread.
-template <typename T, int G, bool BULK, bool HOLD, bool LEAN, bool FULL>
+// LEAN: no biases and no gate per channel: the column sums P and dw alone.  FULL: a gate of every element.  WHERE:
+// the column constants.  Eight values a thread.
+template <typename T, int G, bool BULK, int WHERE, bool LEAN, bool FULL>
 __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 512 / Team<G>::kThreads : 1)
     sandwich_backward_kernel(const __grid_constant__ Params p) {
   using Tm = Team<G>;
@@ -570,18 +547,30 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
   rows.start();
 
   // A, B and the pre norm's w are zeros beyond D, as x, h, dy and dz are: what a thread computes there reaches no sum
-  Columns cols{&p, nullptr, (p.D + 7) / 8 * 8};
+  const int pitch = (p.D + 7) / 8 * 8;
   F2 A[4], B[4], w2[4];
-  if constexpr (HOLD) {
-    column8<0>(cols, c, A);
-    column8<1>(cols, c, B);
-    column8<2>(cols, c, w2);
-  } else if (p.table_at >= 0) {
-    float* table = reinterpret_cast<float*>(ring + p.table_at);
-    fill_table<3>(p, table, cols.pitch);
+  uint32_t table = 0;
+  if constexpr (WHERE == kTable) {
+    fill_table(p, reinterpret_cast<float*>(ring + p.table_at), pitch);
     __syncthreads();
-    cols.table = table;
+    table = smem_u32(ring + p.table_at) + (c < p.D ? 4 * c : 0);  // a thread beyond D: any columns, its x, h, dy and dz are 0
   }
+  auto columns = [&](bool pre) {
+    if constexpr (WHERE == kTable) {
+      table8(table, A);
+      table8(table + 4 * pitch, B);
+      if (pre) table8(table + 8 * pitch, w2);
+      if (c >= p.D) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) A[i] = B[i] = w2[i] = f2(0.0f, 0.0f);
+      }
+    } else {
+      column8<0>(p, c, A);
+      column8<1>(p, c, B);
+      if (pre) column8<2>(p, c, w2);
+    }
+  };
+  if constexpr (WHERE == kRegisters) columns(true);
 
   constexpr int kHeld = LEAN ? 2 : kSums;
   F2 acc[kHeld][4];  // P, dw, then Q, db
@@ -633,11 +622,7 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
       // n and y again, and the pre norm's two sums
       const F2 q = f2(s.w, s.w), m = f2(-s.z * s.w, -s.z * s.w);
       F2 s1 = f2(0.0f, 0.0f), s2 = s1, x[4], dz[4];
-      if constexpr (!HOLD) {
-        column8<0>(cols, c, A);
-        column8<1>(cols, c, B);
-        column8<2>(cols, c, w2);
-      }
+      if constexpr (WHERE != kRegisters) columns(true);
       widen2(e[0][0], x);
       widen2(e[3][0], dz);
 #pragma unroll
@@ -662,10 +647,7 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
     }
     // t reaches y; its way into h, the gate and the post norm's weights
     rows.put(p.out0, row, stage, t);
-    if constexpr (!HOLD) {
-      column8<0>(cols, c, A);
-      column8<1>(cols, c, B);
-    }
+    if constexpr (WHERE != kRegisters) columns(false);
     F2 s3 = f2(0.0f, 0.0f), s4 = s3, s5 = s3;
     if (FULL || p.gate_kind == kGateRow) {
 #pragma unroll
@@ -839,7 +821,7 @@ static int64_t ring_budget(int team, int threads) {
 constexpr int kForwardThreads = 512, kBackwardThreads = 512;  // an SM's, by the kernels' registers
 static Shape backward_shape(int D, int elt, bool full) {
   const int team = team_of(D);
-  Shape s = shape_of(team, full ? 5 : 4, D, elt, ring_budget(team, kBackwardThreads), team >= 640 ? 3 : 0);
+  Shape s = shape_of(team, full ? 5 : 4, D, elt, ring_budget(team, kBackwardThreads), team == 1024 ? 3 : 0);
   if (s.teams > 1) s.smem = std::max(s.smem, kSums * D * 4);
   return s;
 }
@@ -863,17 +845,17 @@ static int launch(const Params& p, const Shape& s, int ctas, cudaStream_t st, co
 template <typename T>
 static int forward(Params& p, cudaStream_t st) {
   // Sixteen values a thread: a row's fixed instructions (copies, waits, sums) fall to half the warps, and two rows
-  // fit an SM where eight values leave room for one (50 M bf16 values on a B200, layer norms, sixteen against
-  // eight a thread: 512 wide 94 / 146 us, 1024 119 / 151, 2048 119 / 174, 4096 133 / 185, 8192 145 / 195).  Just
-  // above 4096 the 512 threads of such a team would be used to two thirds, and eight values are ahead (5000
-  // wide: 229 / 180).
-  const bool two = p.D > 256 && (p.D <= 4096 || p.D > 5120);
-  const int team = two ? team_of((p.D + 1) / 2) : team_of(p.D);
-  const Shape s = shape_of(team, 3, p.D, (int)sizeof(T), ring_budget(team, kForwardThreads), 0);
+  // fit an SM where eight values leave room for one (50 M bf16 values on a B200, layer norms, sixteen against eight a
+  // thread when it was chosen: 512 wide 94 / 146 us, 1024 119 / 151, 2048 119 / 174, 4096 133 / 185, 8192 145 / 195).
+  // Teams of 320 just above 4096: two rows an SM, where 512 threads would be used to two thirds (5000 wide: 146 us,
+  // 186 with 640 threads of eight, 229 with 512 of sixteen).
+  const bool two = p.D > 256;
+  const int team = !two ? 32 : p.D <= 4096 ? team_of((p.D + 1) / 2) : p.D <= 5120 ? 320 : 512;
+  const Shape s = shape_of(team, 3, p.D, (int)sizeof(T), ring_budget(team, team == 320 ? 640 : kForwardThreads), 0);
   p.stages = s.stages;
   p.row_bytes = s.row_bytes;
   p.table_at = s.table_at;
-  const int ctas = (int)std::min<int64_t>((p.N + s.teams - 1) / s.teams, (int64_t)sm_count() * ctas_per_sm(s, kForwardThreads));
+  const int ctas = (int)std::min<int64_t>((p.N + s.teams - 1) / s.teams, (int64_t)sm_count() * ctas_per_sm(s, team == 320 ? 640 : kForwardThreads));
   const char* name = "sandwich_kernel launch";
 #define RB_FORWARD(G, V)                                                      \
   return p.bulk ? launch<sandwich_kernel<T, G, V, true>>(p, s, ctas, st, name) \
@@ -884,23 +866,23 @@ static int forward(Params& p, cudaStream_t st) {
       case 64: RB_FORWARD(64, 2);
       case 128: RB_FORWARD(128, 2);
       case 256: RB_FORWARD(256, 2);
+      case 320: RB_FORWARD(320, 2);
       default: RB_FORWARD(512, 2);
     }
   }
-  if (team == 32) RB_FORWARD(32, 1);
-  RB_FORWARD(640, 1);
+  RB_FORWARD(32, 1);
 #undef RB_FORWARD
 }
 
-template <typename T, int G, bool HOLD, bool LEAN>
+template <typename T, int G, int WHERE, bool LEAN>
 static int backward_of(const Params& p, const Shape& s, int ctas, cudaStream_t st) {
   const char* name = "sandwich_backward_kernel launch";
   const bool full = p.gate_kind == kGateFull;
   if (!p.bulk)
-    return full ? launch<sandwich_backward_kernel<T, G, false, HOLD, false, true>>(p, s, ctas, st, name)
-                : launch<sandwich_backward_kernel<T, G, false, HOLD, false, false>>(p, s, ctas, st, name);
-  return full ? launch<sandwich_backward_kernel<T, G, true, HOLD, LEAN, true>>(p, s, ctas, st, name)
-              : launch<sandwich_backward_kernel<T, G, true, HOLD, LEAN, false>>(p, s, ctas, st, name);
+    return full ? launch<sandwich_backward_kernel<T, G, false, WHERE, false, true>>(p, s, ctas, st, name)
+                : launch<sandwich_backward_kernel<T, G, false, WHERE, false, false>>(p, s, ctas, st, name);
+  return full ? launch<sandwich_backward_kernel<T, G, true, WHERE, LEAN, true>>(p, s, ctas, st, name)
+              : launch<sandwich_backward_kernel<T, G, true, WHERE, LEAN, false>>(p, s, ctas, st, name);
 }
 
 template <typename T>
@@ -911,15 +893,21 @@ static int backward(Params& p, bool lean, cudaStream_t st) {
   p.table_at = s.table_at;
   const int ctas = backward_ctas(p.D, (int)sizeof(T), p.N);
   switch (team_of(p.D)) {
-    case 32: return backward_of<T, 32, true, false>(p, s, ctas, st);
-    case 64: return backward_of<T, 64, true, false>(p, s, ctas, st);
-    case 128: return backward_of<T, 128, true, false>(p, s, ctas, st);
-    case 256: return backward_of<T, 256, true, false>(p, s, ctas, st);
-    case 512: return backward_of<T, 512, true, false>(p, s, ctas, st);
+    case 32: return backward_of<T, 32, kRegisters, false>(p, s, ctas, st);
+    case 64: return backward_of<T, 64, kRegisters, false>(p, s, ctas, st);
+    case 128: return backward_of<T, 128, kRegisters, false>(p, s, ctas, st);
+    case 256: return backward_of<T, 256, kRegisters, false>(p, s, ctas, st);
+    case 512: return backward_of<T, 512, kRegisters, false>(p, s, ctas, st);
     // wider teams have fewer registers a thread: without biases and channel gates two sums are left out
-    case 640: return lean ? backward_of<T, 640, false, true>(p, s, ctas, st) : backward_of<T, 640, false, false>(p, s, ctas, st);
-    default: return lean ? backward_of<T, 1024, false, true>(p, s, ctas, st) : backward_of<T, 1024, false, false>(p, s, ctas, st);
+    case 640:
+      return lean ? backward_of<T, 640, kRegisters, true>(p, s, ctas, st) : backward_of<T, 640, kRegisters, false>(p, s, ctas, st);
+    default: break;
   }
+  if (s.table_at < 0) {  // fp32 rows and gates of every element from 7201 columns on
+    if constexpr (sizeof(T) == 4) return backward_of<T, 1024, kAgain, false>(p, s, ctas, st);
+    else return fail(RB_ERR_UNSUPPORTED, "no shared memory for the column constants");  // not reached: 16-bit rows leave room
+  }
+  return lean ? backward_of<T, 1024, kTable, true>(p, s, ctas, st) : backward_of<T, 1024, kTable, false>(p, s, ctas, st);
 }
 
 static bool is_float(int dt) { return dt == RB_F32 || dt == RB_BF16 || dt == RB_F16; }
