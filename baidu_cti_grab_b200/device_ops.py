@@ -505,18 +505,50 @@ _SCORES = {"softmax": L.RB_SCORE_SOFTMAX, "sigmoid": L.RB_SCORE_SIGMOID}
 
 def _call_on(dev: torch.device, name: str, *args) -> None:
     """L.call on `dev`'s current stream, which becomes the last argument."""
-    if torch.cuda.current_device() == dev.index:
-        L.call(name, *args, _raw_stream(dev.index))
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        L.call(name, *args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            L.call(name, *args, _raw_stream(dev.index))
+            L.call(name, *args, _raw_stream(index))
 
 
-def _score_kind(score: str) -> int:
-    try:
-        return _SCORES[score]
-    except KeyError:
-        raise ValueError(f"score must be one of {sorted(_SCORES)}, not {score!r}") from None
+_PLAN_BYTES: Dict[tuple, int] = {}  # workspace bytes of the shapes seen last
+
+
+def _plan_bytes(dev: torch.device, name: str, *shape: int) -> int:
+    """What a workspace-size entry point says of a shape on `dev` (it goes by the device's SMs)."""
+    key = (dev.index, name, *shape)
+    n = _PLAN_BYTES.get(key)
+    if n is None:
+        with torch.cuda.device(dev):
+            n = int(getattr(L.load(), name)(*shape))
+        if n < 0:
+            raise ValueError(f"{name} rejected the shape {shape}")
+        if len(_PLAN_BYTES) >= 4096:
+            _PLAN_BYTES.clear()
+        _PLAN_BYTES[key] = n
+    return n
+
+
+def _device_of(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
+    """require_cuda for a call whose first tensor is always there (a microsecond less)."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise RuntimeError(f"{name} expects CUDA tensors")
+    for t in others:
+        if t is not None and t.device != dev:
+            require_cuda(name, first, t)
+    return dev
+
+
+def _rows_of(t: torch.Tensor, rows: int, width: int) -> Tuple[torch.Tensor, int]:
+    """A matrix with contiguous rows (a copy only where t has none) and its row pitch in elements."""
+    s0, s1 = t.stride()
+    if (s1 != 1 and width > 1) or (rows > 1 and s0 < width):
+        t = t.contiguous()
+        s0 = width
+    return t, max(s0, width)
 
 
 def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
@@ -530,32 +562,41 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: Op
     equal runs of experts the topk_groups with the highest sums of their group_top best stay.
     Returns (idx [T, k] by falling choice value, ties to the lowest index; score [T, k] in score_dtype
     (default: the logits'), probs [T, E] in score_dtype or None, counts int32 [E] or None)."""
-    dev = require_cuda("route_topk", logits, bias)
-    if logits.dim() != 2 or logits.dtype not in _FLOATS:
+    dev = _device_of("route_topk", logits, bias)
+    dtype = logits.dtype
+    if logits.dim() != 2 or dtype not in _FLOATS:
         raise ValueError("route_topk expects logits [T, E] in fp32, bf16 or f16")
     T, E = logits.shape
-    kind = _score_kind(score)
+    kind = _SCORES.get(score)
+    if kind is None:
+        raise ValueError(f"score must be one of {sorted(_SCORES)}, not {score!r}")
+    bias_ptr = None
     if bias is not None:
-        if bias.dtype != torch.float32 or tuple(bias.shape) != (E,):
+        if bias.dtype != torch.float32 or bias.shape != (E,):
             raise ValueError(f"bias must be fp32 [{E}]")
         bias = bias.contiguous()
-    if idx_dtype not in (torch.int64, torch.int32):
+        bias_ptr = bias.data_ptr()
+    if idx_dtype is not torch.int64 and idx_dtype is not torch.int32:
         raise ValueError("idx_dtype must be int64 or int32")
-    score_dtype = logits.dtype if score_dtype is None else score_dtype
-    if score_dtype not in _FLOATS:
+    if score_dtype is None:
+        score_dtype = dtype
+    elif score_dtype not in _FLOATS:
         raise ValueError("score_dtype must be fp32, bf16 or f16")
     if not 1 <= k <= max(E, 1):
         raise ValueError(f"k must be in [1, {E}]")
-    if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
-        logits = logits.contiguous()
-    idx = logits.new_empty((T, k), dtype=idx_dtype)
-    chosen = logits.new_empty((T, k), dtype=score_dtype)
-    probs = logits.new_empty((T, E), dtype=score_dtype) if want_probs else None
-    counts = logits.new_empty((E,), dtype=torch.int32) if want_counts else None
-    _call_on(dev, "rb_route_topk", logits.data_ptr(), rb_dtype(logits), max(logits.stride(0), E), T, E, _ptr(bias), k,
-             kind, groups, topk_groups, group_top, int(renormalize), float(scale), idx.data_ptr(),
-             L.RB_I64 if idx_dtype == torch.int64 else L.RB_I32, chosen.data_ptr(), rb_dtype(chosen), _ptr(probs),
-             _ptr(counts))
+    logits, ld = _rows_of(logits, T, E)
+    idx = torch.empty((T, k), dtype=idx_dtype, device=dev)
+    chosen = torch.empty((T, k), dtype=score_dtype, device=dev)
+    probs = counts = probs_ptr = counts_ptr = None
+    if want_probs:
+        probs = torch.empty((T, E), dtype=score_dtype, device=dev)
+        probs_ptr = probs.data_ptr()
+    if want_counts:
+        counts = torch.empty((E,), dtype=torch.int32, device=dev)
+        counts_ptr = counts.data_ptr()
+    _call_on(dev, "rb_route_topk", logits.data_ptr(), _DT[dtype], ld, T, E, bias_ptr, k, kind, groups, topk_groups,
+             group_top, renormalize, scale, idx.data_ptr(), L.RB_I64 if idx_dtype is torch.int64 else L.RB_I32,
+             chosen.data_ptr(), _DT[score_dtype], probs_ptr, counts_ptr)
     return idx, chosen, probs, counts
 
 
@@ -564,28 +605,34 @@ def route_topk_backward(logits: torch.Tensor, idx: torch.Tensor, grad_score: Opt
                         renormalize: bool = False, scale: float = 1.0) -> torch.Tensor:
     """Gradient [T, E] of route_topk's logits, in their dtype (rb_route_topk_backward), from the
     gradients of its scores [T, k] and probs [T, E] (either may be None) and its idx."""
-    dev = require_cuda("route_topk_backward", logits, idx, grad_score, grad_probs)
-    if logits.dim() != 2 or logits.dtype not in _FLOATS:
+    dev = _device_of("route_topk_backward", logits, idx, grad_score, grad_probs)
+    dtype = logits.dtype
+    if logits.dim() != 2 or dtype not in _FLOATS:
         raise ValueError("route_topk_backward expects logits [T, E] in fp32, bf16 or f16")
     T, E = logits.shape
-    kind = _score_kind(score)
+    kind = _SCORES.get(score)
+    if kind is None:
+        raise ValueError(f"score must be one of {sorted(_SCORES)}, not {score!r}")
     if idx.dim() != 2 or idx.shape[0] != T or idx.dtype not in (torch.int64, torch.int32):
         raise ValueError("idx must be int64 or int32 [T, k]")
-    if grad_score is not None and (grad_score.shape != idx.shape or grad_score.dtype not in _FLOATS):
-        raise ValueError("grad_score must be a float tensor of idx's shape")
-    if grad_probs is not None and (grad_probs.shape != logits.shape or grad_probs.dtype not in _FLOATS):
-        raise ValueError("grad_probs must be a float tensor of the logits' shape")
-    if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
-        logits = logits.contiguous()
+    gs_ptr = gp_ptr = None
+    gs_type = gp_type = 0
+    if grad_score is not None:
+        if grad_score.shape != idx.shape or grad_score.dtype not in _FLOATS:
+            raise ValueError("grad_score must be a float tensor of idx's shape")
+        grad_score = grad_score.contiguous()
+        gs_ptr, gs_type = grad_score.data_ptr(), _DT[grad_score.dtype]
+    if grad_probs is not None:
+        if grad_probs.shape != logits.shape or grad_probs.dtype not in _FLOATS:
+            raise ValueError("grad_probs must be a float tensor of the logits' shape")
+        grad_probs = grad_probs.contiguous()
+        gp_ptr, gp_type = grad_probs.data_ptr(), _DT[grad_probs.dtype]
+    logits, ld = _rows_of(logits, T, E)
     idx = idx.contiguous()
-    grad_score = None if grad_score is None else grad_score.contiguous()
-    grad_probs = None if grad_probs is None else grad_probs.contiguous()
-    out = logits.new_empty((T, E))
-    _call_on(dev, "rb_route_topk_backward", logits.data_ptr(), rb_dtype(logits), max(logits.stride(0), E), T, E,
-             idx.data_ptr(), L.RB_I64 if idx.dtype == torch.int64 else L.RB_I32, idx.shape[1], _ptr(grad_score),
-             rb_dtype(grad_score) if grad_score is not None else 0, _ptr(grad_probs),
-             rb_dtype(grad_probs) if grad_probs is not None else 0, kind, int(renormalize), float(scale),
-             out.data_ptr(), rb_dtype(out))
+    out = torch.empty((T, E), dtype=dtype, device=dev)
+    _call_on(dev, "rb_route_topk_backward", logits.data_ptr(), _DT[dtype], ld, T, E, idx.data_ptr(),
+             L.RB_I64 if idx.dtype is torch.int64 else L.RB_I32, idx.shape[1], gs_ptr, gs_type, gp_ptr, gp_type, kind,
+             renormalize, scale, out.data_ptr(), _DT[dtype])
     return out
 
 
@@ -594,56 +641,61 @@ _NORMS = {None: L.RB_NORM_NONE, "layer": L.RB_NORM_LAYER, "rms": L.RB_NORM_RMS}
 _GATE_ACTS = {"none": L.RB_GATE_ACT_NONE, "sigmoid": L.RB_GATE_ACT_SIGMOID}
 
 
-def _norm_args(name, x, h, post, post_weight, post_bias, gate, gate_act, pre, pre_weight, pre_bias):
-    """What both directions check: (device, rows, width, x2, h2, gate2, gate kind, gate pitch, post, pre, act codes)."""
-    dev = require_cuda(name, x, h, post_weight, post_bias, gate, pre_weight, pre_bias)
-    if x.dtype not in _FLOATS or x.dim() < 1 or x.shape != h.shape or h.dtype != x.dtype:
-        raise ValueError(f"{name} expects x and h [..., D] of one shape and one type (fp32, bf16 or f16)")
-    try:
-        kinds = _NORMS[post], _NORMS[pre]
-    except KeyError:
-        raise ValueError("post and pre are 'layer', 'rms' or None") from None
-    if gate_act not in _GATE_ACTS:
-        raise ValueError(f"gate_act must be one of {sorted(_GATE_ACTS)}")
-    D = x.shape[-1]
-    for kind, w, b in ((post, post_weight, post_bias), (pre, pre_weight, pre_bias)):
-        for t in (w, b):
-            if t is not None and (tuple(t.shape) != (D,) or t.dtype not in _FLOATS or not t.is_contiguous()):
-                raise ValueError(f"norm weights and biases must be contiguous fp32, bf16 or f16 [{D}]")
-            if t is not None and kind is None:
-                raise ValueError("a weight or bias was given without its norm")
-        if w is not None and b is not None and w.dtype != b.dtype:
+def _affine(weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], kind: Optional[str], D: int):
+    """(weight pointer, bias pointer, type) of a norm's parameters."""
+    dtype = None
+    for t in (weight, bias):
+        if t is None:
+            continue
+        if kind is None:
+            raise ValueError("a weight or bias was given without its norm")
+        if t.shape != (D,) or t.dtype not in _FLOATS or not t.is_contiguous():
+            raise ValueError(f"norm weights and biases must be contiguous fp32, bf16 or f16 [{D}]")
+        if dtype is not None and t.dtype != dtype:
             raise ValueError("a norm's weight and bias must share a type")
-    x2, h2 = _rows2d(x, D), _rows2d(h, D)
-    N = x2.shape[0]
-    kind, ldg, gate2 = L.RB_GATE_NONE, 0, gate
+        dtype = t.dtype
+    return _ptr(weight), _ptr(bias), 0 if dtype is None else _DT[dtype]
+
+
+def _norm_args(name, x, h, post, post_weight, post_bias, gate, gate_act, pre, pre_weight, pre_bias):
+    """What both directions check: (device, rows, width, x rows, their pitch, h rows, their pitch, gate (kind, tensor, type,
+    pitch), post (kind, weight, bias, type), pre likewise, act code)."""
+    dev = _device_of(name, x, h, post_weight, post_bias, gate, pre_weight, pre_bias)
+    dtype, shape = x.dtype, x.shape
+    if dtype not in _FLOATS or len(shape) < 1 or shape != h.shape or h.dtype != dtype:
+        raise ValueError(f"{name} expects x and h [..., D] of one shape and one type (fp32, bf16 or f16)")
+    k1, k2, act = _NORMS.get(post), _NORMS.get(pre), _GATE_ACTS.get(gate_act)
+    if k1 is None or k2 is None:
+        raise ValueError("post and pre are 'layer', 'rms' or None")
+    if act is None:
+        raise ValueError(f"gate_act must be one of {sorted(_GATE_ACTS)}")
+    D = shape[-1]
+    first, second = (k1, *_affine(post_weight, post_bias, post, D)), (k2, *_affine(pre_weight, pre_bias, pre, D))
+    x2, ldx = _rows2d(x, D)
+    h2, ldh = _rows2d(h, D)
+    g = (L.RB_GATE_NONE, None, 0, 0)
     if gate is not None:
         if gate.dtype not in _FLOATS:
             raise ValueError("the gate must be fp32, bf16 or f16")
-        if gate.dim() == 1 and gate.shape[0] == D and (x.dim() > 1 or D != 1):
-            kind, gate2 = L.RB_GATE_CHANNEL, gate.contiguous()
-        elif tuple(gate.shape) == (*x.shape[:-1], 1):
-            kind, gate2, ldg = L.RB_GATE_ROW, gate.reshape(-1).contiguous(), 1
-        elif gate.shape == x.shape:
-            if gate.dtype != x.dtype:
+        if gate.shape == (D,) and (len(shape) > 1 or D != 1):
+            g = (L.RB_GATE_CHANNEL, gate.contiguous(), _DT[gate.dtype], 0)
+        elif gate.shape == (*shape[:-1], 1):
+            g = (L.RB_GATE_ROW, gate.reshape(-1).contiguous(), _DT[gate.dtype], 1)
+        elif gate.shape == shape:
+            if gate.dtype != dtype:
                 raise ValueError("a gate of every element must have x's type")
-            kind, gate2 = L.RB_GATE_FULL, _rows2d(gate, D)
-            ldg = max(gate2.stride(0), D)
+            g2, ldg = _rows2d(gate, D)
+            g = (L.RB_GATE_FULL, g2, _DT[dtype], ldg)
         else:
             raise ValueError(f"the gate must be [{D}], [..., 1] or of x's shape")
-    return dev, N, D, x2, h2, gate2, kind, ldg, kinds[0], kinds[1], _GATE_ACTS[gate_act]
+    return dev, x2.shape[0], D, x2, ldx, h2, ldh, g, first, second, act
 
 
-def _rows2d(t: torch.Tensor, D: int) -> torch.Tensor:
-    """t [..., D] as rows [N, D] with contiguous values (a copy only where no view has them)."""
-    t2 = t if t.dim() == 2 else t.reshape(-1, D) if D else t.reshape(0, 0)
-    if t2.stride(1) != 1 or (t2.shape[0] > 1 and t2.stride(0) < D):
-        t2 = t2.contiguous()
-    return t2
-
-
-def _norm_dtype(w: Optional[torch.Tensor], b: Optional[torch.Tensor]) -> int:
-    return rb_dtype(w) if w is not None else rb_dtype(b) if b is not None else 0
+def _rows2d(t: torch.Tensor, D: int) -> Tuple[torch.Tensor, int]:
+    """t [..., D] as rows [N, D] with contiguous values (a copy only where no view has them), and their pitch."""
+    if t.dim() != 2:
+        t = t.reshape(-1, D) if D else t.reshape(0, 0)
+    return _rows_of(t, t.shape[0], D)
 
 
 def sandwich_norm(x: torch.Tensor, h: torch.Tensor, *, post: Optional[str] = None,
@@ -656,16 +708,14 @@ def sandwich_norm(x: torch.Tensor, h: torch.Tensor, *, post: Optional[str] = Non
     x (the residual stream) and h (a block's output) [..., D], D <= 8192; post and pre 'layer', 'rms' or
     None with optional weights and biases [D]; gate None, [D], [..., 1] or x's shape, as it is or its
     sigmoid.  Returns (y, z or None, stats fp32 [N, 4] or None: what sandwich_norm_backward takes)."""
-    dev, N, D, x2, h2, g2, gk, ldg, k1, k2, act = _norm_args("sandwich_norm", x, h, post, post_weight, post_bias, gate,
-                                                             gate_act, pre, pre_weight, pre_bias)
-    y = x.new_empty(x.shape)
-    z = x.new_empty(x.shape) if k2 != L.RB_NORM_NONE else None
-    stats = x.new_empty((N, 4), dtype=torch.float32) if want_stats else None
-    _call_on(dev, "rb_sandwich_norm", x2.data_ptr(), max(x2.stride(0), D), h2.data_ptr(), max(h2.stride(0), D),
-             rb_dtype(x2), N, D, k1, _ptr(post_weight), _ptr(post_bias), _norm_dtype(post_weight, post_bias),
-             float(post_eps), gk, _ptr(g2), 0 if g2 is None else rb_dtype(g2), ldg, act, float(scale), k2,
-             _ptr(pre_weight), _ptr(pre_bias), _norm_dtype(pre_weight, pre_bias), float(pre_eps), y.data_ptr(), _ptr(z),
-             _ptr(stats))
+    dev, N, D, x2, ldx, h2, ldh, g, first, second, act = _norm_args("sandwich_norm", x, h, post, post_weight, post_bias,
+                                                                    gate, gate_act, pre, pre_weight, pre_bias)
+    gk, g2, gt, ldg = g
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    z = torch.empty_like(y) if second[0] != L.RB_NORM_NONE else None
+    stats = torch.empty((N, 4), dtype=torch.float32, device=dev) if want_stats else None
+    _call_on(dev, "rb_sandwich_norm", x2.data_ptr(), ldx, h2.data_ptr(), ldh, _DT[x.dtype], N, D, *first, post_eps, gk,
+             _ptr(g2), gt, ldg, act, scale, *second, pre_eps, y.data_ptr(), _ptr(z), _ptr(stats))
     return y, z, stats
 
 
@@ -678,31 +728,33 @@ def sandwich_norm_backward(grad_y: Optional[torch.Tensor], grad_z: Optional[torc
     """Gradients (x, h, gate, post_weight, post_bias, pre_weight, pre_bias) of sandwich_norm, None where
     there is no such input (rb_sandwich_norm_backward), from those of y and z (either may be None) and the
     forward call's inputs and stats.  The same bits every time."""
-    dev, N, D, x2, h2, g2, gk, ldg, k1, k2, act = _norm_args("sandwich_norm_backward", x, h, post, post_weight, post_bias,
-                                                             gate, gate_act, pre, pre_weight, pre_bias)
-    require_cuda("sandwich_norm_backward", x, grad_y, grad_z, stats)
+    dev, N, D, x2, ldx, h2, ldh, g, first, second, act = _norm_args("sandwich_norm_backward", x, h, post, post_weight,
+                                                                    post_bias, gate, gate_act, pre, pre_weight, pre_bias)
+    _device_of("sandwich_norm_backward", x, grad_y, grad_z, stats)
+    gk, g2, gt, ldg = g
     grads = []
     for t in (grad_y, grad_z):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+        if t is None:
+            grads += (None, D)
+            continue
+        if t.shape != x.shape or t.dtype != x.dtype:
             raise ValueError("grad_y and grad_z must have x's shape and type")
-        grads.append(None if t is None else _rows2d(t, D))
-    dy, dz = grads
+        t, ld = _rows2d(t, D)
+        grads += (t, ld)
+    dy, ldy, dz, ldz = grads
     if dz is not None and pre is None:
         raise ValueError("grad_z was given without pre")
-    if tuple(stats.shape) != (N, 4) or stats.dtype != torch.float32 or not stats.is_contiguous():
+    if stats.shape != (N, 4) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise ValueError(f"stats must be the forward call's fp32 [{N}, 4]")
-    dx, dh = x.new_empty(x.shape), x.new_empty(x.shape)
-    outs = [None if t is None else t.new_empty(t.shape) for t in (gate, post_weight, post_bias, pre_weight, pre_bias)]
-    ws_bytes = int(L.load().rb_sandwich_norm_workspace_size(N, D, rb_dtype(x2)))
-    if ws_bytes < 0:
-        raise ValueError(f"rows of {D} values are not supported")
-    ws = x.new_empty((ws_bytes,), dtype=torch.uint8)
-    _call_on(dev, "rb_sandwich_norm_backward", _ptr(dy), D if dy is None else max(dy.stride(0), D), _ptr(dz),
-             D if dz is None else max(dz.stride(0), D), x2.data_ptr(), max(x2.stride(0), D), h2.data_ptr(),
-             max(h2.stride(0), D), stats.data_ptr(), rb_dtype(x2), N, D, k1, _ptr(post_weight), _ptr(post_bias),
-             _norm_dtype(post_weight, post_bias), gk, _ptr(g2), 0 if g2 is None else rb_dtype(g2), ldg, act, float(scale), k2,
-             _ptr(pre_weight), _ptr(pre_bias), _norm_dtype(pre_weight, pre_bias), ws.data_ptr(), ws_bytes, dx.data_ptr(),
-             dh.data_ptr(), _ptr(outs[0]), _ptr(outs[1]), _ptr(outs[2]), _ptr(outs[3]), _ptr(outs[4]))
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dh = torch.empty_like(dx)
+    outs = [None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
+            for t in (gate, post_weight, post_bias, pre_weight, pre_bias)]
+    ws_bytes = _plan_bytes(dev, "rb_sandwich_norm_workspace_size", N, D, _DT[x.dtype])
+    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+    _call_on(dev, "rb_sandwich_norm_backward", _ptr(dy), ldy, _ptr(dz), ldz, x2.data_ptr(), ldx, h2.data_ptr(), ldh,
+             stats.data_ptr(), _DT[x.dtype], N, D, *first, gk, _ptr(g2), gt, ldg, act, scale, *second, ws.data_ptr(),
+             ws_bytes, dx.data_ptr(), dh.data_ptr(), *(_ptr(t) for t in outs))
     return (dx, dh, *outs)
 
 
@@ -715,40 +767,39 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     y [T, N] and x [T, K] bf16/f16; a [R, rank, K] and b [R, N, rank] contiguous in the same type, rank <= 128;
     adapter int32/int64 [T], -1 (or anything outside [0, R)) for a token without one; scale fp32 [R].
     ``out`` may be y.  Forward only: an input that asks for a gradient is refused."""
-    dev = require_cuda("low_rank_add", y, x, a, b, adapter, scale, out)
+    dev = _device_of("low_rank_add", y, x, a, b, adapter, scale, out)
     if y.dim() != 2 or x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
         raise ValueError("low_rank_add expects y [T, N], x [T, K], a [R, rank, K] and b [R, N, rank]")
     (T, N), (R, rank, K) = y.shape, a.shape
-    if tuple(x.shape) != (T, K) or tuple(b.shape) != (R, N, rank):
+    if x.shape != (T, K) or b.shape != (R, N, rank):
         raise ValueError(f"x must be [{T}, {K}] and b [{R}, {N}, {rank}]")
-    if x.dtype not in (torch.bfloat16, torch.float16) or any(t.dtype != x.dtype for t in (y, a, b)):
+    dtype = x.dtype
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or y.dtype is not dtype or a.dtype is not dtype \
+            or b.dtype is not dtype:
         raise ValueError("y, x, a and b must all be bf16 or all f16")
-    if tuple(adapter.shape) != (T,) or adapter.dtype not in (torch.int64, torch.int32):
+    if adapter.shape != (T,) or adapter.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"adapter must be int32 or int64 [{T}]")
-    if scale is not None and (tuple(scale.shape) != (R,) or scale.dtype != torch.float32):
-        raise ValueError(f"scale must be fp32 [{R}]")
+    if scale is not None:
+        if scale.shape != (R,) or scale.dtype is not torch.float32:
+            raise ValueError(f"scale must be fp32 [{R}]")
+        scale = scale.contiguous()
     if not a.is_contiguous() or not b.is_contiguous():
         raise ValueError("a and b must be contiguous")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, x, a, b, scale)):
+    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad
+                                    or (scale is not None and scale.requires_grad)):
         raise RuntimeError("low_rank_add has no backward: call it under torch.no_grad() or on detached tensors")
     if out is None:
-        out = y.new_empty((T, N))
-    elif tuple(out.shape) != (T, N) or out.dtype != y.dtype or (N > 0 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N):
-        raise ValueError(f"out must be a row-major [{T}, {N}] {y.dtype} tensor")
-    if y.stride(1) != 1 or (T > 1 and y.stride(0) < N):
-        y = y.contiguous()
-    if x.stride(1) != 1 or (T > 1 and x.stride(0) < K):
-        x = x.contiguous()
+        out = torch.empty((T, N), dtype=dtype, device=dev)
+    elif out.shape != (T, N) or out.dtype is not dtype or (N > 1 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N):
+        raise ValueError(f"out must be a row-major [{T}, {N}] {dtype} tensor")
+    y, ldy = _rows_of(y, T, N)
+    x, ldx = _rows_of(x, T, K)
     adapter = adapter.contiguous()
-    scale = None if scale is None else scale.contiguous()
-    ws_bytes = int(L.load().rb_low_rank_workspace_size(T, K, N, rank))
-    if ws_bytes < 0:
-        raise ValueError("rb_low_rank_workspace_size rejected the shape")
-    ws = x.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
-    _call_on(dev, "rb_low_rank_add", y.data_ptr(), max(y.stride(0), N), x.data_ptr(), max(x.stride(0), K), rb_dtype(x), T, K,
-             N, a.data_ptr(), b.data_ptr(), R, rank, adapter.data_ptr(),
-             L.RB_I64 if adapter.dtype == torch.int64 else L.RB_I32, _ptr(scale), _ptr(ws), ws_bytes, out.data_ptr(),
-             max(out.stride(0), N))
+    ws_bytes = _plan_bytes(dev, "rb_low_rank_workspace_size", T, K, N, rank)
+    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev) if ws_bytes else None
+    _call_on(dev, "rb_low_rank_add", y.data_ptr(), ldy, x.data_ptr(), ldx, _DT[dtype], T, K, N, a.data_ptr(), b.data_ptr(), R,
+             rank, adapter.data_ptr(), L.RB_I64 if adapter.dtype is torch.int64 else L.RB_I32, _ptr(scale), _ptr(ws), ws_bytes,
+             out.data_ptr(), max(out.stride(0), N))
     return out
 
 
