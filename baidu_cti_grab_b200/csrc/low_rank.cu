@@ -42,6 +42,7 @@ struct Params {
   float* part;         // [splits][T][rank] partial h, or null
   int64_t ldy, ldx, ldo, T;
   int K, N, R, rank, idx64;
+  int unit;            // columns of B that a copy brings side by side: 64, 32 or 16 (swizzled), 8
   int chunk_io;        // y and out can be moved by whole chunks
   int splits;          // of K (H alone) -- partials to sum (out alone)
   int chunks;          // 64-column chunks of a CTA (out alone)
@@ -159,20 +160,21 @@ __global__ void __launch_bounds__(kTokenThreads) token_kernel(const __grid_const
 constexpr int kRows = 128;         // tokens of a tile
 constexpr int kChunk = 64;         // columns of an out chunk
 constexpr int kRowThreads = 256;   // two warps for each 32 rows (TMEM lanes): the halves of a chunk
-constexpr int kTileThreads = 64 + kRowThreads;  // TMA warp, MMA warp, the rows' warps
+constexpr int kTileThreads = 96 + kRowThreads;  // a warp for the copies, one for the MMAs, the rows' warps, the lists' warp
+constexpr int kListWarp = 2 + kRowThreads / 32;
 constexpr int kXBytes = kRows * 128;  // 64 columns of X (of K), or of y
 constexpr int kPiece = kChunk * 16;   // eight columns of B for a chunk
 constexpr int kZeroBytes = kPiece;    // what an odd piece of eight columns is paired with
 
 enum Mode : int { kFused = 0, kHOnly = 1, kOutOnly = 2 };
 
-// Two CTAs fit an SM in each form (the fused one 104 KB, H alone 96 KB, out alone 96 KB).
+// Two CTAs fit an SM in each form (the fused one 106 KB, H alone 98 KB, out alone 106 KB).
 template <int MODE>
 struct Tile {
-  static constexpr int kCols = MODE == kFused ? 64 : 128;  // of H: the ranks of a group of adapters
-  static constexpr int kStages = MODE == kOutOnly ? 2 : 3;  // ring of X (and A) blocks of 64 columns of K, then of y
+  static constexpr int kCols = MODE == kFused ? 64 : MODE == kHOnly ? 128 : 96;  // of H: the ranks of a group of adapters
+  static constexpr int kStages = 3;  // ring of X (and A) blocks of 64 columns of K, then of y
   static constexpr int kABytes = MODE == kOutOnly ? 0 : kCols * 128;
-  static constexpr int kHBytes = MODE == kHOnly ? 0 : kRows * kCols * 2;  // 64-column tiles of 16 KB
+  static constexpr int kHBytes = MODE == kHOnly ? 0 : (kCols + 63) / 64 * kXBytes;  // 64-column tiles of 16 KB
   static constexpr int kBBytes = MODE == kHOnly ? 0 : kChunk * kCols * 2;
   static constexpr int kSmem = 1024 + kStages * (kXBytes + kABytes) + kHBytes + 2 * kBBytes + kZeroBytes;
   static constexpr int kHCols = MODE == kOutOnly ? 0 : kCols;  // TMEM: H, then two out chunks
@@ -183,6 +185,17 @@ struct Tile {
 // other, and the second eight columns of K lie `next` bytes on
 __device__ __forceinline__ uint64_t plain_desc(uint32_t saddr, uint32_t next) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// the same with rows of 32, 64 or 128 bytes under the swizzle of that width
+__device__ __forceinline__ uint64_t swizzled_desc(uint32_t saddr, int row_bytes) {
+  const uint64_t layout = row_bytes == 128 ? 2 : row_bytes == 64 ? 4 : 6;
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(8 * row_bytes >> 4) << 32) |
+         ((uint64_t)1 << 46) | (layout << 61);
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, uint32_t bar,
                                             uint64_t policy) {
@@ -266,7 +279,52 @@ __device__ __forceinline__ void store16(T* row, int c, int N, int vec, const uin
   }
 }
 
-// grid: x = tiles of 128 tokens; y = splits of K (H alone) or of N (out alone)
+// A position in a ring of S slots: the slot, and the parity of its use.
+template <int S>
+struct Turn {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ void next() {
+    if (++slot == S) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+  __device__ void skip(int n) {
+    slot += n;
+    parity ^= (uint32_t)(slot / S) & 1u;
+    slot %= S;
+  }
+};
+
+// Asks the hardware for the tile of a CTA that has not started yet (cluster launch control); the 16-byte answer
+// lands at `to` and completes 16 bytes on `bar`.
+__device__ __forceinline__ void ask_tile(uint32_t to, uint32_t bar) {
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(to), "r"(bar)
+               : "memory");
+}
+// The answer: blockIdx.x of the CTA whose work was taken over, or -1.
+__device__ __forceinline__ int told_tile(uint32_t from) {
+  uint32_t taken, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(taken), "=r"(x)
+      : "r"(from)
+      : "memory");
+  return taken ? (int)x : -1;
+}
+
+// One CTA a tile of 128 tokens (blockIdx.x); blockIdx.y: split of K (H alone) or of N (out alone).  A fused CTA goes on
+// with the tiles of CTAs that have not started: while the rows' warps finish a tile, the next one's adapters are listed
+// and the ring is filled with its X, and a tile of many adapters (several groups, each with X again) leaves its other
+// tiles to the rest.  103725 x 512 took 84 us with a CTA a tile (a quarter of it before its first X block had come) and
+// with tiles dealt out beforehand (half of the CTAs ended at 64 us, the last at 91).
 template <typename T, int MODE>
 __global__ void __launch_bounds__(kTileThreads, 2)
     tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA,
@@ -280,13 +338,16 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   uint8_t* sA = sX + kStages * kXBytes;
   uint8_t* sH = sA + kStages * kABytes;
   uint8_t* sB = sH + C::kHBytes;
+  uint8_t* const s_zero = sB + 2 * kBBytes;
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], hfull, hready, bfull[2], bempty[2], dfull[2], dempty[2], done;
+  __shared__ __align__(8) uint64_t lfull[2], lempty[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word, s_count;
-  __shared__ int s_list[kRows], s_slot[kRows];
+  __shared__ int abort_word;
+  __shared__ int s_tile[2], s_count[2], s_list[2][kRows], s_slot[2][kRows];  // of this tile and the next; tile -1: no more
+  __shared__ __align__(16) uint4 s_told;
+  __shared__ __align__(8) uint64_t told;
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row0 = (int64_t)blockIdx.x * kRows;
   constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
   constexpr uint32_t kIdesc = (1u << 4) | kType | ((uint32_t)(kRows >> 4) << 24);  // N is added where it is known
 
@@ -302,14 +363,19 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       mbar_init(smem_u32(&bempty[s]), 1);
       mbar_init(smem_u32(&dfull[s]), 1);
       mbar_init(smem_u32(&dempty[s]), kRowThreads);
+      mbar_init(smem_u32(&lfull[s]), 1);
+      mbar_init(smem_u32(&lempty[s]), kRowThreads + 2);  // the rows' threads, the copies' and the MMAs'
     }
     mbar_init(smem_u32(&done), 1);
+    mbar_init(smem_u32(&told), 1);
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmA)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmB)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmY)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmO)) : "memory");
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::kTmemCols)
@@ -317,42 +383,14 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (warp == 3) {
-    for (int i = lane; i < kZeroBytes / 16; i += 32)
-      reinterpret_cast<uint4*>(sB + 2 * kBBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = lane; i < kZeroBytes / 16; i += 32) reinterpret_cast<uint4*>(s_zero)[i] = make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
-  if (warp == 2) {
-    // the tile's distinct adapters in the order of their first row, and each row's place among them
-    int count = 0;
-    for (int c = 0; c < kRows / 32; ++c) {
-      const int i = adapter_of(p, row0 + c * 32 + lane);
-      const unsigned peers = __match_any_sync(kAll, i);
-      const int leader = __ffs(peers) - 1;
-      int at = -1;
-      if (i >= 0 && lane == leader)
-        for (int q = 0; q < count && at < 0; ++q)
-          if (s_list[q] == i) at = q;
-      const unsigned fresh = __ballot_sync(kAll, i >= 0 && lane == leader && at < 0);
-      if (fresh >> lane & 1) {
-        at = count + __popc(fresh & ((1u << lane) - 1u));
-        s_list[at] = i;
-      }
-      count += __popc(fresh);
-      s_slot[c * 32 + lane] = __shfl_sync(kAll, at, leader);  // -1 for rows without an adapter
-      __syncwarp();
-    }
-    if (lane == 0) s_count = count;
   }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int count = s_count;
-  uint8_t* const s_zero = sB + 2 * kBBytes;
   const int group = C::kCols / p.rank;  // adapters of a group
-  const int groups = (count + group - 1) / group;
-  // one group (as a rule): y comes and out goes by whole 64-column chunks through the ring
-  const bool whole = MODE != kHOnly && groups == 1 && p.chunk_io != 0;
   const int kblocks = (p.K + 63) / 64;
   const int split = MODE == kFused ? 0 : (int)blockIdx.y;
   const int kb0 = MODE == kHOnly ? (int)((int64_t)kblocks * split / p.splits) : 0;
@@ -360,67 +398,83 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   const int all_chunks = (p.N + kChunk - 1) / kChunk;
   const int ch0 = MODE == kOutOnly ? split * p.chunks : 0;
   const int ch1 = MODE == kOutOnly ? min(all_chunks, ch0 + p.chunks) : all_chunks;
-  const int eights = p.rank / 8;           // pieces of eight columns of an adapter
+  const int eights = p.rank / 8;  // pieces of eight columns of an adapter
+  // one group (as a rule): y comes and out goes by whole 64-column chunks through the ring
+  auto is_whole = [&](int groups) { return MODE != kHOnly && groups == 1 && p.chunk_io != 0; };
 
   if (warp == 0) {
     if (lane == 0) {
-      // ---------------------------------------------------------- producer
+      // ---------------------------------------------------------- copies
       const uint64_t once = tc::policy_evict_first(), keep = tc::policy_evict_last();
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, bphase = 0;
+      Turn<kStages> ring;
+      Turn<2> bt, lt;
       uint32_t issued = 0, issued_phase = 0;  // bits: ring stages, then the two B buffers
       bool ok = true;
-      for (int g = 0; g < groups && ok; ++g) {
-        const int first = g * group, n = min(group, count - first);
-        if constexpr (MODE != kOutOnly) {
-          for (int kb = kb0; kb < kb1; ++kb) {
-            if (!mbar_wait_bounded(smem_u32(&empty[stage]), phase ^ 1, kWaitTimeoutProducer, abort_flag)) {
-              ok = false;
-              break;
+      auto note = [&](int bit, uint32_t parity) {
+        issued |= 1u << bit;
+        issued_phase = (issued_phase & ~(1u << bit)) | (parity << bit);
+      };
+      while (ok) {
+        if (!mbar_wait_bounded(smem_u32(&lfull[lt.slot]), lt.parity, kWaitTimeoutProducer, abort_flag)) break;
+        const int tile = s_tile[lt.slot], row0 = tile * kRows;
+        if (tile < 0) break;
+        const int* list = s_list[lt.slot];
+        const int count = s_count[lt.slot], groups = (count + group - 1) / group;
+        const bool whole = is_whole(groups);
+        for (int g = 0; g < groups && ok; ++g) {
+          const int first = g * group, n = min(group, count - first);
+          if constexpr (MODE != kOutOnly) {
+            for (int kb = kb0; kb < kb1; ++kb) {
+              if (!mbar_wait_bounded(smem_u32(&empty[ring.slot]), ring.parity ^ 1, kWaitTimeoutProducer, abort_flag)) {
+                ok = false;
+                break;
+              }
+              const uint32_t fb = smem_u32(&full[ring.slot]);
+              mbar_arrive_expect_tx(fb, kXBytes + n * p.rank * 128);
+              tc::tma_load_2d(smem_u32(sX + ring.slot * kXBytes), &tmX, kb * 64, row0, fb, groups > 1 ? keep : once);
+              for (int j = 0; j < n; ++j)
+                tc::tma_load_2d(smem_u32(sA + ring.slot * kABytes + j * p.rank * 128), &tmA, kb * 64, list[first + j] * p.rank, fb, keep);
+              note(ring.slot, ring.parity);
+              ring.next();
             }
-            const uint32_t fb = smem_u32(&full[stage]);
-            mbar_arrive_expect_tx(fb, kXBytes + n * p.rank * 128);
-            tc::tma_load_2d(smem_u32(sX + stage * kXBytes), &tmX, kb * 64, (int)row0, fb, groups > 1 ? keep : once);
-            for (int j = 0; j < n; ++j)
-              tc::tma_load_2d(smem_u32(sA + stage * kABytes + j * p.rank * 128), &tmA, kb * 64, s_list[first + j] * p.rank, fb, keep);
-            issued |= 1u << stage;
-            issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1;
+          }
+          if constexpr (MODE != kHOnly) {
+            for (int ch = ch0; ch < ch1 && ok; ++ch) {
+              if (!mbar_wait_bounded(smem_u32(&bempty[bt.slot]), bt.parity ^ 1, kWaitTimeoutProducer, abort_flag)) {
+                ok = false;
+                break;
+              }
+              const uint32_t fb = smem_u32(&bfull[bt.slot]);
+              const int left = min(kChunk, p.N - ch * kChunk);  // rows of B that the chunk has
+              mbar_arrive_expect_tx(fb, p.rank == 8 ? n * left * 16 : n * eights * kPiece);
+              for (int j = 0; j < n; ++j) {
+                const int row = list[first + j] * p.N + ch * kChunk;
+                const uint32_t to = smem_u32(sB + bt.slot * kBBytes + j * eights * kPiece);
+                if (p.rank == 8) {  // 16 bytes a row: the chunk's rows lie as the operand wants them
+                  bulk_copy(to, static_cast<const T*>(p.b) + (int64_t)row * 8, left * 16, fb);
+                } else if (p.unit == 8) {
+                  tma_load_3d(to, &tmB, 0, row, 0, fb, keep);
+                } else {
+                  for (int u = 0; u < p.rank; u += p.unit) tc::tma_load_2d(to + u * kChunk * 2, &tmB, u, row, fb, keep);
+                }
+              }
+              note(kStages + bt.slot, bt.parity);
+              bt.next();
+              if (!whole) continue;
+              if (!mbar_wait_bounded(smem_u32(&empty[ring.slot]), ring.parity ^ 1, kWaitTimeoutProducer, abort_flag)) {
+                ok = false;
+                break;
+              }
+              const uint32_t fy = smem_u32(&full[ring.slot]);
+              mbar_arrive_expect_tx(fy, kXBytes);
+              tc::tma_load_2d(smem_u32(sX + ring.slot * kXBytes), &tmY, ch * kChunk, row0, fy, once);
+              note(ring.slot, ring.parity);
+              ring.next();
             }
           }
         }
-        if constexpr (MODE != kHOnly) {
-          for (int ch = ch0; ch < ch1 && ok; ++ch) {
-            if (!mbar_wait_bounded(smem_u32(&bempty[buf]), bphase ^ 1, kWaitTimeoutProducer, abort_flag)) {
-              ok = false;
-              break;
-            }
-            const uint32_t fb = smem_u32(&bfull[buf]);
-            mbar_arrive_expect_tx(fb, n * eights * kPiece);
-            for (int j = 0; j < n; ++j)
-              tma_load_3d(smem_u32(sB + buf * kBBytes + j * eights * kPiece), &tmB, 0, s_list[first + j] * p.N + ch * kChunk, 0, fb, keep);
-            issued |= 1u << (kStages + buf);
-            issued_phase = (issued_phase & ~(1u << (kStages + buf))) | (bphase << (kStages + buf));
-            buf ^= 1;
-            if (buf == 0) bphase ^= 1;
-            if (!whole) continue;
-            if (!mbar_wait_bounded(smem_u32(&empty[stage]), phase ^ 1, kWaitTimeoutProducer, abort_flag)) {
-              ok = false;
-              break;
-            }
-            const uint32_t fy = smem_u32(&full[stage]);
-            mbar_arrive_expect_tx(fy, kXBytes);
-            tc::tma_load_2d(smem_u32(sX + stage * kXBytes), &tmY, ch * kChunk, (int)row0, fy, once);
-            issued |= 1u << stage;
-            issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1;
-            }
-          }
-        }
+        mbar_arrive(smem_u32(&lempty[lt.slot]));
+        lt.next();
       }
       // never leave a copy in flight behind an exiting CTA
       for (int s = 0; s < kStages + 2; ++s)
@@ -431,241 +485,327 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   } else if (warp == 1) {
     if (lane == 0) {
       // --------------------------------------------------------------- MMA
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, bphase = 0;
+      Turn<kStages> ring;
+      Turn<2> bt, lt;
+      uint32_t hparity = 0;
       bool ok = true;
-      for (int g = 0; g < groups && ok; ++g) {
-        const int n = min(group, count - g * group);
-        if constexpr (MODE != kOutOnly) {
-          const uint32_t idesc = kIdesc | ((uint32_t)((n * eights + 1) & ~1) << 17);  // N in eights, an even number
-          for (int kb = kb0; kb < kb1; ++kb) {
-            if (!mbar_wait_bounded(smem_u32(&full[stage]), phase, kWaitTimeoutMma, abort_flag)) {
-              ok = false;
-              break;
-            }
-            tc::tc_fence_after();
-            const uint64_t xd = tc::sw128_desc(smem_u32(sX + stage * kXBytes));
-            const uint64_t ad = tc::sw128_desc(smem_u32(sA + stage * kABytes));
+      while (ok) {
+        if (!mbar_wait_bounded(smem_u32(&lfull[lt.slot]), lt.parity, kWaitTimeoutMma, abort_flag)) break;
+        if (s_tile[lt.slot] < 0) break;
+        const int count = s_count[lt.slot], groups = (count + group - 1) / group;
+        mbar_arrive(smem_u32(&lempty[lt.slot]));
+        lt.next();
+        for (int g = 0; g < groups && ok; ++g) {
+          const int n = min(group, count - g * group);
+          if constexpr (MODE != kOutOnly) {
+            const uint32_t idesc = kIdesc | ((uint32_t)((n * eights + 1) & ~1) << 17);  // N in eights, an even number
+            for (int kb = kb0; kb < kb1; ++kb) {
+              if (!mbar_wait_bounded(smem_u32(&full[ring.slot]), ring.parity, kWaitTimeoutMma, abort_flag)) {
+                ok = false;
+                break;
+              }
+              tc::tc_fence_after();
+              const uint64_t xd = tc::sw128_desc(smem_u32(sX + ring.slot * kXBytes));
+              const uint64_t ad = tc::sw128_desc(smem_u32(sA + ring.slot * kABytes));
 #pragma unroll
-            for (int s = 0; s < 4; ++s) umma_f16(tmem, xd + 2 * s, ad + 2 * s, idesc, (kb > kb0 || s > 0) ? 1u : 0u);
-            tc::umma_commit(smem_u32(&empty[stage]));
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1;
+              for (int s = 0; s < 4; ++s) umma_f16(tmem, xd + 2 * s, ad + 2 * s, idesc, (kb > kb0 || s > 0) ? 1u : 0u);
+              tc::umma_commit(smem_u32(&empty[ring.slot]));
+              ring.next();
             }
+            if (!ok) break;
+            tc::umma_commit(smem_u32(&hfull));
           }
-          if (!ok) break;
-          tc::umma_commit(smem_u32(&hfull));
-        }
-        // the rows' warps have H in shared memory (and are done with its TMEM columns)
-        if (!mbar_wait_bounded(smem_u32(&hready), g & 1, kWaitTimeoutMma, abort_flag)) break;
-        if constexpr (MODE != kHOnly) {
-          tc::tc_fence_after();
-          const uint32_t idesc = kIdesc | ((uint32_t)(kChunk >> 3) << 17);
-          const uint64_t hd = tc::sw128_desc(smem_u32(sH));
-          for (int ch = ch0; ch < ch1; ++ch) {
-            if (!mbar_wait_bounded(smem_u32(&bfull[buf]), bphase, kWaitTimeoutMma, abort_flag) ||
-                !mbar_wait_bounded(smem_u32(&dempty[buf]), bphase ^ 1, kWaitTimeoutMma, abort_flag)) {
-              ok = false;
-              break;
-            }
+          // the rows' warps have H in shared memory (and are done with its TMEM columns)
+          if (!mbar_wait_bounded(smem_u32(&hready), hparity, kWaitTimeoutMma, abort_flag)) {
+            ok = false;
+            break;
+          }
+          hparity ^= 1;
+          if constexpr (MODE != kHOnly) {
             tc::tc_fence_after();
-            const uint32_t bt = smem_u32(sB + buf * kBBytes);
-            for (int e = 0; e < n * eights; e += 2) {
-              const int at = e >> 1;  // sixteen columns of H: four to a 16 KB tile
-              const uint32_t from = bt + (uint32_t)(e * kPiece);
-              const uint64_t bd = plain_desc(from, e + 1 < n * eights ? (uint32_t)kPiece : smem_u32(s_zero) - from);
-              umma_f16(tmem + C::kHCols + buf * kChunk, hd + (uint64_t)((at >> 2) * (kXBytes >> 4) + 2 * (at & 3)), bd, idesc,
-                       e > 0 ? 1u : 0u);
+            const uint32_t idesc = kIdesc | ((uint32_t)(kChunk >> 3) << 17);
+            const uint64_t hd = tc::sw128_desc(smem_u32(sH));
+            for (int ch = ch0; ch < ch1; ++ch) {
+              if (!mbar_wait_bounded(smem_u32(&bfull[bt.slot]), bt.parity, kWaitTimeoutMma, abort_flag) ||
+                  !mbar_wait_bounded(smem_u32(&dempty[bt.slot]), bt.parity ^ 1, kWaitTimeoutMma, abort_flag)) {
+                ok = false;
+                break;
+              }
+              tc::tc_fence_after();
+              const uint32_t at_b = smem_u32(sB + bt.slot * kBBytes);
+              for (int e = 0; e < n * eights; e += 2) {
+                const int at = e >> 1;  // sixteen columns of H: four to a 16 KB tile
+                uint64_t bd;
+                if (p.unit == 8) {
+                  const uint32_t from = at_b + (uint32_t)(e * kPiece);
+                  bd = plain_desc(from, e + 1 < n * eights ? (uint32_t)kPiece : smem_u32(s_zero) - from);
+                } else {  // a box holds `unit` columns
+                  const int in_box = (e * 8) & (p.unit - 1);
+                  bd = swizzled_desc(at_b + (uint32_t)((e * 8 - in_box) * kChunk * 2), p.unit * 2) + (uint64_t)(in_box >> 3);
+                }
+                umma_f16(tmem + C::kHCols + bt.slot * kChunk, hd + (uint64_t)((at >> 2) * (kXBytes >> 4) + 2 * (at & 3)), bd, idesc,
+                         e > 0 ? 1u : 0u);
+              }
+              tc::umma_commit(smem_u32(&bempty[bt.slot]));
+              tc::umma_commit(smem_u32(&dfull[bt.slot]));
+              bt.next();
             }
-            tc::umma_commit(smem_u32(&bempty[buf]));
-            tc::umma_commit(smem_u32(&dfull[buf]));
-            buf ^= 1;
-            if (buf == 0) bphase ^= 1;
           }
+        }
+        if (MODE == kFused && ok && is_whole(groups)) {
+          // y's chunks passed through the ring without this thread.  The rows release the last product only after
+          // they have seen the last chunk, so from there on every slot's next use is one of X again; to wait for
+          // that earlier could take a use two turns back for it (a barrier tells uses by parity alone).
+          const int back = bt.slot ^ 1;
+          const uint32_t parity = back == 1 ? bt.parity ^ 1 : bt.parity;
+          if (!mbar_wait_bounded(smem_u32(&dempty[back]), parity, kWaitTimeoutMma, abort_flag)) break;
+          ring.skip(ch1 - ch0);
         }
       }
       tc::umma_commit(smem_u32(&done));
       mbar_wait_bounded(smem_u32(&done), 0, kWaitTimeoutMma, nullptr);
     }
+  } else if (warp == kListWarp) {
+    // ------------------------------------------------------- the tiles' adapters
+    Turn<2> lt;
+    uint32_t answers = 0;
+    bool asked = false;
+    for (int tile = blockIdx.x;;) {
+      if (!__all_sync(kAll, mbar_wait_bounded(smem_u32(&lempty[lt.slot]), lt.parity ^ 1, kWaitTimeoutProducer, abort_flag))) break;
+      if (tile < 0) {
+        if (lane == 0) {
+          s_tile[lt.slot] = -1;
+          mbar_arrive(smem_u32(&lfull[lt.slot]));
+        }
+        break;
+      }
+      if (MODE == kFused) {
+        if (lane == 0) ask_tile(smem_u32(&s_told), smem_u32(&told));
+        asked = true;
+      }
+      // distinct adapters in the order of their first row, and each row's place among them
+      int* list = s_list[lt.slot];
+      int id[kRows / 32], count = 0;
+#pragma unroll
+      for (int c = 0; c < kRows / 32; ++c) id[c] = adapter_of(p, (int64_t)tile * kRows + c * 32 + lane);
+#pragma unroll
+      for (int c = 0; c < kRows / 32; ++c) {
+        const int i = id[c];
+        const unsigned peers = __match_any_sync(kAll, i);
+        const int leader = __ffs(peers) - 1;
+        int at = -1;
+        if (i >= 0 && lane == leader)
+          for (int q = 0; q < count && at < 0; ++q)
+            if (list[q] == i) at = q;
+        const unsigned fresh = __ballot_sync(kAll, i >= 0 && lane == leader && at < 0);
+        if (fresh >> lane & 1) {
+          at = count + __popc(fresh & ((1u << lane) - 1u));
+          list[at] = i;
+        }
+        count += __popc(fresh);
+        s_slot[lt.slot][c * 32 + lane] = __shfl_sync(kAll, at, leader);  // -1 for rows without an adapter
+        __syncwarp();
+      }
+      if (lane == 0) {
+        s_tile[lt.slot] = tile;
+        s_count[lt.slot] = count;
+        mbar_arrive(smem_u32(&lfull[lt.slot]));
+      }
+      lt.next();
+      tile = -1;
+      if (MODE == kFused) {
+        if (!__all_sync(kAll, mbar_wait_bounded(smem_u32(&told), answers & 1u, kWaitTimeoutProducer, abort_flag))) break;
+        asked = false;
+        ++answers;
+        tile = told_tile(smem_u32(&s_told));
+        __syncwarp();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the answer was read before the next one may land
+      }
+    }
+    // never leave an answer in flight behind an exiting CTA
+    if (asked) mbar_wait_bounded(smem_u32(&told), answers & 1u, kWaitTimeoutProducer, nullptr);
   } else {
     // ----------------------------------------------------------- the rows
     const int quarter = warp & 3;  // the TMEM lanes that this warp can read
     const int half = (warp - 2) >> 2;  // its 32 columns of a chunk, and every other sixteen of H
     const int r = quarter * 32 + lane;
-    const int64_t row = row0 + r;
-    const bool live = row < p.T;
-    const int slot = s_slot[r];
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const float w = MODE != kHOnly && slot >= 0 && p.scale != nullptr ? __ldg(p.scale + s_list[slot]) : 1.0f;
-    const T* y = static_cast<const T*>(p.y) + row * p.ldy;
-    T* out = static_cast<T*>(p.out) + row * p.ldo;
-    int buf = 0;
-    uint32_t bphase = 0;
+    Turn<kStages> ring;
+    Turn<2> bt, lt;
+    uint32_t hparity = 0;
     bool ok = true;
-    if (MODE != kHOnly && !whole && live && slot < 0 && out != y) {
-      for (int c = ch0 * kChunk + half * 16; c < min(p.N, ch1 * kChunk); c += 32) {
-        uint32_t v[8];
-        load16(y, c, p.N, p.vec_y, v);
-        store16(out, c, p.N, p.vec_out, v);
+    // 16-byte pieces of a row of the H tile are swizzled by the row's place in its eight; eight pieces to 16 KB
+    auto piece_at = [&](int e) { return reinterpret_cast<uint4*>(sH + (e >> 3) * kXBytes + r * 128 + (((e & 7) ^ (r & 7)) << 4)); };
+    while (true) {
+      // the rows' threads leave together, since they count on one another at their barrier
+      ok = rows_all(ok && mbar_wait_bounded(smem_u32(&lfull[lt.slot]), lt.parity, kWaitTimeoutEpilogue, abort_flag));
+      if (!ok) break;
+      const int tile = s_tile[lt.slot];
+      if (tile < 0) break;
+      const int64_t row = (int64_t)tile * kRows + r;
+      const bool live = row < p.T;
+      const int count = s_count[lt.slot], groups = (count + group - 1) / group, slot = s_slot[lt.slot][r];
+      const float w = MODE != kHOnly && slot >= 0 && p.scale != nullptr ? __ldg(p.scale + s_list[lt.slot][slot]) : 1.0f;
+      mbar_arrive(smem_u32(&lempty[lt.slot]));
+      lt.next();
+      const bool whole = is_whole(groups);
+      const T* y = static_cast<const T*>(p.y) + row * p.ldy;
+      T* out = static_cast<T*>(p.out) + row * p.ldo;
+      if (MODE != kHOnly && !whole && live && slot < 0 && out != y) {
+        for (int c = ch0 * kChunk + half * 16; c < min(p.N, ch1 * kChunk); c += 32) {
+          uint32_t v[8];
+          load16(y, c, p.N, p.vec_y, v);
+          store16(out, c, p.N, p.vec_out, v);
+        }
       }
-    }
-    for (int g = 0; g < groups && ok; ++g) {
-      const int first = g * group, n = min(group, count - first);
-      const int mine = slot >= first && slot < first + n ? slot - first : -1;
-      if constexpr (MODE != kOutOnly) {
-        // a thread that gave up still meets the others at the chunks' barrier
-        ok = mbar_wait_bounded(smem_u32(&hfull), g & 1, kWaitTimeoutEpilogue, abort_flag);
-        tc::tc_fence_after();
-      }
-      // own adapter's h into this row of the H tile, zeros into the others' columns: sixteen columns at a time, whose
-      // eights may be of two adapters
-      for (int c = half * 16; c < n * p.rank; c += 32) {
-        const int e = c / 8;
-        const bool in[2] = {mine >= 0 && e / eights == mine, mine >= 0 && (e + 1) / eights == mine};
-        uint32_t v[16];
+      // a thread that gave up on a wait still meets the others at a whole chunk's barrier
+      for (int g = 0; g < groups && (ok || whole); ++g) {
+        const int first = g * group, n = min(group, count - first);
+        const int mine = slot >= first && slot < first + n ? slot - first : -1;
+        if constexpr (MODE != kOutOnly) {
+          ok = ok && mbar_wait_bounded(smem_u32(&hfull), hparity, kWaitTimeoutEpilogue, abort_flag);
+          tc::tc_fence_after();
+          ring.skip(kb1 - kb0);
+        }
+        hparity ^= 1;
+        // own adapter's h into this row of the H tile, zeros into the others' columns: sixteen columns at a time, whose
+        // eights may be of two adapters
         if constexpr (MODE == kOutOnly) {
-          float s[16];
-#pragma unroll
-          for (int q = 0; q < 16; ++q) s[q] = 0.0f;
-#pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            if (!in[d]) continue;
-            const float* from = p.part + row * p.rank + (c + 8 * d - mine * p.rank);
-#pragma unroll 4
-            for (int k = 0; k < p.splits; ++k, from += p.T * p.rank) {
-              const float4 f = __ldg(reinterpret_cast<const float4*>(from)), h = __ldg(reinterpret_cast<const float4*>(from) + 1);
-              s[8 * d] += f.x;
-              s[8 * d + 1] += f.y;
-              s[8 * d + 2] += f.z;
-              s[8 * d + 3] += f.w;
-              s[8 * d + 4] += h.x;
-              s[8 * d + 5] += h.y;
-              s[8 * d + 6] += h.z;
-              s[8 * d + 7] += h.w;
+          for (int c = half * 16; c < n * p.rank; c += 32) *piece_at(c / 8) = *piece_at(c / 8 + 1) = make_uint4(0u, 0u, 0u, 0u);
+          for (int q = 0; mine >= 0 && q < eights; ++q) {
+            const int e = mine * eights + q;
+            if (((e >> 1) & 1) != half) continue;  // the other warp's sixteen columns
+            const float4* from = reinterpret_cast<const float4*>(p.part + row * p.rank + 8 * q);
+            float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+            for (int k = 0; k < p.splits; ++k) {
+              const float4 f = __ldg(from + k * (p.T * p.rank / 4)), h = __ldg(from + k * (p.T * p.rank / 4) + 1);
+              s[0] += f.x;
+              s[1] += f.y;
+              s[2] += f.z;
+              s[3] += f.w;
+              s[4] += h.x;
+              s[5] += h.y;
+              s[6] += h.z;
+              s[7] += h.w;
             }
-          }
-#pragma unroll
-          for (int q = 0; q < 16; ++q) v[q] = __float_as_uint(s[q]);
-        } else {
-          __syncwarp();
-          tc::swp::tmem_ld16(tmem + lanes + (uint32_t)c, v);
-        }
-        if constexpr (MODE == kHOnly) {
-#pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            if (!in[d]) continue;
-            float* to = p.part + ((int64_t)split * p.T + row) * p.rank + (c + 8 * d - mine * p.rank);
-#pragma unroll
-            for (int q = 0; q < 8; q += 4)
-              *reinterpret_cast<float4*>(to + q) =
-                  make_float4(__uint_as_float(v[8 * d + q]), __uint_as_float(v[8 * d + q + 1]), __uint_as_float(v[8 * d + q + 2]),
-                              __uint_as_float(v[8 * d + q + 3]));
+            *piece_at(e) = make_uint4(pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3]), pack2<T>(s[4], s[5]), pack2<T>(s[6], s[7]));
           }
         } else {
-          // 16-byte pieces of the row, swizzled by the row's place in its eight; eight pieces to a tile
-          uint8_t* to = sH + (e >> 3) * kXBytes + r * 128;
+          for (int c = half * 16; c < n * p.rank; c += 32) {
+            const int e = c / 8;
+            const bool in[2] = {mine >= 0 && e / eights == mine, mine >= 0 && (e + 1) / eights == mine};
+            uint32_t v[16];
+            __syncwarp();
+            tc::swp::tmem_ld16(tmem + lanes + (uint32_t)c, v);
 #pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            uint32_t h[4];
+            for (int d = 0; d < 2; ++d) {
+              if constexpr (MODE == kHOnly) {
+                if (!in[d]) continue;
+                float* to = p.part + ((int64_t)split * p.T + row) * p.rank + (c + 8 * d - mine * p.rank);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              h[q] = in[d] ? pack2<T>(__uint_as_float(v[8 * d + 2 * q]), __uint_as_float(v[8 * d + 2 * q + 1])) : 0u;
-            *reinterpret_cast<uint4*>(to + ((((e + d) & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-          }
-        }
-      }
-      tc::tc_fence_before();
-      if constexpr (MODE != kHOnly) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(smem_u32(&hready));
-      if (whole) {
-        const int before = MODE == kFused ? kb1 - kb0 : 0;  // X blocks that the ring carried
-        int stage = before % kStages;
-        uint32_t phase = (uint32_t)(before / kStages) & 1u;
-        int last = -1;  // the stage whose store may still be reading
-        for (int ch = ch0; ch < ch1; ++ch) {
-          ok = ok && mbar_wait_bounded(smem_u32(&full[stage]), phase, kWaitTimeoutEpilogue, abort_flag) &&
-               mbar_wait_bounded(smem_u32(&dfull[buf]), bphase, kWaitTimeoutEpilogue, abort_flag);
-          tc::tc_fence_after();
-          uint8_t* mem = sX + stage * kXBytes + r * 128;
-          uint32_t v[32];
-          __syncwarp();
-          tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + buf * kChunk + half * 32), v);
-          tc::tc_fence_before();
-          mbar_arrive(smem_u32(&dempty[buf]));
-          if (mine >= 0 && ok) {
+                for (int q = 0; q < 8; q += 4)
+                  *reinterpret_cast<float4*>(to + q) =
+                      make_float4(__uint_as_float(v[8 * d + q]), __uint_as_float(v[8 * d + q + 1]),
+                                  __uint_as_float(v[8 * d + q + 2]), __uint_as_float(v[8 * d + q + 3]));
+              } else {
+                uint32_t h[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint4* at = reinterpret_cast<uint4*>(mem + (((4 * half + q) ^ (r & 7)) << 4));
-              const uint4 f = *at;
-              const uint32_t fw[4] = {f.x, f.y, f.z, f.w};
-              uint32_t o[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float2 u = unpack2<T>(fw[i]);
-                o[i] = pack2<T>(fmaf(w, __uint_as_float(v[8 * q + 2 * i]), u.x), fmaf(w, __uint_as_float(v[8 * q + 2 * i + 1]), u.y));
+                for (int q = 0; q < 4; ++q)
+                  h[q] = in[d] ? pack2<T>(__uint_as_float(v[8 * d + 2 * q]), __uint_as_float(v[8 * d + 2 * q + 1])) : 0u;
+                *piece_at(e + d) = make_uint4(h[0], h[1], h[2], h[3]);
               }
-              *at = make_uint4(o[0], o[1], o[2], o[3]);
             }
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          ok = rows_all(ok);
-          if (!ok) break;
-          if (threadIdx.x == 64) {
-            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
-                             reinterpret_cast<uint64_t>(&tmO)),
-                         "r"(smem_u32(sX + stage * kXBytes)), "r"(ch * kChunk), "r"((int)row0)
-                         : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            if (last >= 0) {
-              asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-              mbar_arrive(smem_u32(&empty[last]));
-            }
-            last = stage;
-          }
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
-          buf ^= 1;
-          if (buf == 0) bphase ^= 1;
         }
-        if (threadIdx.x == 64) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-      } else if constexpr (MODE != kHOnly) {
-        for (int ch = ch0; ch < ch1; ++ch) {
-          const int c0 = ch * kChunk + half * 32;
-          uint32_t base[16];
-          if (mine >= 0) {  // requested before the wait for the product
+        tc::tc_fence_before();
+        if constexpr (MODE != kHOnly) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(smem_u32(&hready));
+        if (whole) {
+          int last = -1;  // the stage whose store may still be reading
+          for (int ch = ch0; ch < ch1; ++ch) {
+            ok = ok && mbar_wait_bounded(smem_u32(&full[ring.slot]), ring.parity, kWaitTimeoutEpilogue, abort_flag) &&
+                 mbar_wait_bounded(smem_u32(&dfull[bt.slot]), bt.parity, kWaitTimeoutEpilogue, abort_flag);
+            tc::tc_fence_after();
+            uint8_t* mem = sX + ring.slot * kXBytes + r * 128;
+            uint32_t v[32];
+            __syncwarp();
+            tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + bt.slot * kChunk + half * 32), v);
+            tc::tc_fence_before();
+            mbar_arrive(smem_u32(&dempty[bt.slot]));
+            if (mine >= 0 && ok) {
 #pragma unroll
-            for (int c = 0; c < 32; c += 16)
-              if (c0 + c < p.N) load16(y, c0 + c, p.N, p.vec_y, base + c / 2);
-          }
-          if (!mbar_wait_bounded(smem_u32(&dfull[buf]), bphase, kWaitTimeoutEpilogue, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc::tc_fence_after();
-          uint32_t v[32];
-          __syncwarp();
-          tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + buf * kChunk + half * 32), v);
-          tc::tc_fence_before();
-          mbar_arrive(smem_u32(&dempty[buf]));
-          if (mine >= 0) {
-            uint32_t o[16];
+              for (int q = 0; q < 4; ++q) {
+                uint4* at = reinterpret_cast<uint4*>(mem + (((4 * half + q) ^ (r & 7)) << 4));
+                const uint4 f = *at;
+                const uint32_t fw[4] = {f.x, f.y, f.z, f.w};
+                uint32_t o[4];
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-              const float2 f = unpack2<T>(base[q]);
-              o[q] = pack2<T>(fmaf(w, __uint_as_float(v[2 * q]), f.x), fmaf(w, __uint_as_float(v[2 * q + 1]), f.y));
+                for (int i = 0; i < 4; ++i) {
+                  const float2 u = unpack2<T>(fw[i]);
+                  o[i] = pack2<T>(fmaf(w, __uint_as_float(v[8 * q + 2 * i]), u.x), fmaf(w, __uint_as_float(v[8 * q + 2 * i + 1]), u.y));
+                }
+                *at = make_uint4(o[0], o[1], o[2], o[3]);
+              }
             }
-#pragma unroll
-            for (int c = 0; c < 32; c += 16)
-              if (c0 + c < p.N) store16(out, c0 + c, p.N, p.vec_out, o + c / 2);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            ok = rows_all(ok);
+            if (!ok) break;
+            if (threadIdx.x == 64) {
+              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                               reinterpret_cast<uint64_t>(&tmO)),
+                           "r"(smem_u32(sX + ring.slot * kXBytes)), "r"(ch * kChunk), "r"(tile * kRows)
+                           : "memory");
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+              if (last >= 0) {
+                asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                mbar_arrive(smem_u32(&empty[last]));
+              }
+              last = ring.slot;
+            }
+            ring.next();
+            bt.next();
           }
-          buf ^= 1;
-          if (buf == 0) bphase ^= 1;
+          if (threadIdx.x == 64) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            if (last >= 0) mbar_arrive(smem_u32(&empty[last]));
+          }
+        } else if constexpr (MODE != kHOnly) {
+          for (int ch = ch0; ch < ch1; ++ch) {
+            const int c0 = ch * kChunk + half * 32;
+            uint32_t base[16];
+            if (mine >= 0) {  // requested before the wait for the product
+#pragma unroll
+              for (int c = 0; c < 32; c += 16)
+                if (c0 + c < p.N) load16(y, c0 + c, p.N, p.vec_y, base + c / 2);
+            }
+            if (!mbar_wait_bounded(smem_u32(&dfull[bt.slot]), bt.parity, kWaitTimeoutEpilogue, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc::tc_fence_after();
+            uint32_t v[32];
+            __syncwarp();
+            tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + bt.slot * kChunk + half * 32), v);
+            tc::tc_fence_before();
+            mbar_arrive(smem_u32(&dempty[bt.slot]));
+            if (mine >= 0) {
+              uint32_t o[16];
+#pragma unroll
+              for (int q = 0; q < 16; ++q) {
+                const float2 f = unpack2<T>(base[q]);
+                o[q] = pack2<T>(fmaf(w, __uint_as_float(v[2 * q]), f.x), fmaf(w, __uint_as_float(v[2 * q + 1]), f.y));
+              }
+#pragma unroll
+              for (int c = 0; c < 32; c += 16)
+                if (c0 + c < p.N) store16(out, c0 + c, p.N, p.vec_out, o + c / 2);
+            }
+            bt.next();
+          }
         }
       }
     }
+    if (threadIdx.x == 64) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -704,16 +844,22 @@ static Plan plan_of(int64_t T, int K, int N, int rank) {
   return q;
 }
 
-// b [R * N, rank] as pieces of eight columns: a box holds an adapter's 64 rows, piece after piece
-static int make_piece_map(CUtensorMap* tm, const void* b, int64_t rows, int rank, CUtensorMapDataType dt) {
+// b [R * N, rank].  unit 8: pieces of eight columns, a box holds an adapter's 64 rows piece after piece; else boxes of
+// 64 rows and `unit` columns under the swizzle of their width (fewer and wider requests).
+static int make_b_map(CUtensorMap* tm, const void* b, int64_t rows, int rank, int unit, CUtensorMapDataType dt) {
   auto enc = tc::encode_fn();
   if (enc == nullptr) return fail(RB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[3] = {8, (cuuint64_t)rows, (cuuint64_t)(rank / 8)};
+  const bool pieces = unit == 8;
+  cuuint64_t dims[3] = {pieces ? 8 : (cuuint64_t)rank, (cuuint64_t)rows, (cuuint64_t)(rank / 8)};
   cuuint64_t strides[2] = {(cuuint64_t)rank * 2, 16};
-  cuuint32_t box[3] = {8, kChunk, (cuuint32_t)(rank / 8)};
+  cuuint32_t box[3] = {(cuuint32_t)unit, kChunk, (cuuint32_t)(rank / 8)};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(tm, dt, 3, const_cast<void*>(b), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUtensorMapSwizzle sw = unit == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                : unit == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                : unit == 16 ? CU_TENSOR_MAP_SWIZZLE_32B
+                                             : CU_TENSOR_MAP_SWIZZLE_NONE;
+  CUresult r = enc(tm, dt, pieces ? 3 : 2, const_cast<void*>(b), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(RB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return RB_OK;
 }
@@ -762,7 +908,7 @@ static int run_tiles(Params& p, const Plan& q, CUtensorMapDataType dt, cudaStrea
   CUtensorMap tmX, tmA, tmB, tmY, tmO;
   if ((rc = tc::make_tmap(&tmX, p.x, p.K, p.T, p.ldx * 2, 64, kRows, dt))) return rc;
   if ((rc = tc::make_tmap(&tmA, p.a, p.K, (int64_t)p.R * p.rank, (int64_t)p.K * 2, 64, (uint32_t)p.rank, dt))) return rc;
-  if ((rc = make_piece_map(&tmB, p.b, (int64_t)p.R * p.N, p.rank, dt))) return rc;
+  if ((rc = make_b_map(&tmB, p.b, (int64_t)p.R * p.N, p.rank, p.unit, dt))) return rc;
   tmY = tmO = tmX;  // not used where rows do not allow whole chunks
   if (p.chunk_io) {
     if ((rc = tc::make_tmap(&tmY, p.y, p.N, p.T, p.ldy * 2, kChunk, kRows, dt))) return rc;
@@ -834,6 +980,7 @@ extern "C" int rb_low_rank_add(const void* y, int64_t ldy, const void* x, int64_
   p.rank = rank;
   p.idx64 = idx_dtype == RB_I64;
   p.splits = 1;
+  p.unit = rank % 64 == 0 ? 64 : rank % 32 == 0 ? 32 : rank % 16 == 0 ? 16 : 8;
   p.vec_y = vec_bytes(y, ldy);
   p.vec_out = vec_bytes(out, ldo);
   p.chunk_io = p.vec_y >= 16 && p.vec_out >= 16;

@@ -72,6 +72,8 @@ SHAPES = [
     (256, 512, 512, 16, 300, BF, 1),        # every row of a tile its own adapter
     (19000, 128, 192, 16, 11, BF, 60),      # enough tiles for one fused kernel
     (19001, 256, 72, 8, 130, HF, 2),
+    (60000, 72, 136, 16, 9, BF, 40),        # several tiles a CTA, of one group and of more
+    (60001, 64, 72, 64, 5, HF, 30),
     (200, 100, 64, 16, 3, BF, 9),           # K not a multiple of 8: token kernel
     (200, 96, 64, 12, 3, HF, 9),            # rank not a multiple of 8
     (130, 96, 64, 128, 3, BF, 9),           # rank above the tensor path's
