@@ -168,11 +168,11 @@ constexpr int kZeroBytes = kPiece;    // what an odd piece of eight columns is p
 
 enum Mode : int { kFused = 0, kHOnly = 1, kOutOnly = 2 };
 
-// Two CTAs fit an SM in each form (the fused one 106 KB, H alone 98 KB, out alone 106 KB).
+// Two CTAs fit an SM in each form (the fused one 106 KB, H alone 98 KB, out alone 98 KB).
 template <int MODE>
 struct Tile {
-  static constexpr int kCols = MODE == kFused ? 64 : MODE == kHOnly ? 128 : 96;  // of H: the ranks of a group of adapters
-  static constexpr int kStages = 3;  // ring of X (and A) blocks of 64 columns of K, then of y
+  static constexpr int kCols = MODE == kFused ? 64 : 128;  // of H: the ranks of a group of adapters
+  static constexpr int kStages = MODE == kOutOnly ? 2 : 3;  // ring of X (and A) blocks of 64 columns of K, then of y
   static constexpr int kABytes = MODE == kOutOnly ? 0 : kCols * 128;
   static constexpr int kHBytes = MODE == kHOnly ? 0 : (kCols + 63) / 64 * kXBytes;  // 64-column tiles of 16 KB
   static constexpr int kBBytes = MODE == kHOnly ? 0 : kChunk * kCols * 2;
@@ -351,6 +351,9 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
   constexpr uint32_t kIdesc = (1u << 4) | kType | ((uint32_t)(kRows >> 4) << 24);  // N is added where it is known
 
+  // The out kernel may start while this one's last CTAs run: it lists its tiles and asks for B and y meanwhile, none
+  // of which this kernel writes.
+  if constexpr (MODE == kHOnly) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
@@ -579,10 +582,6 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         }
         break;
       }
-      if (MODE == kFused) {
-        if (lane == 0) ask_tile(smem_u32(&s_told), smem_u32(&told));
-        asked = true;
-      }
       // distinct adapters in the order of their first row, and each row's place among them
       int* list = s_list[lt.slot];
       int id[kRows / 32], count = 0;
@@ -611,9 +610,15 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         s_count[lt.slot] = count;
         mbar_arrive(smem_u32(&lfull[lt.slot]));
       }
+      const Turn<2> mine = lt;
       lt.next();
       tile = -1;
       if (MODE == kFused) {
+        // a tile of several groups takes long: its CTA takes over another one only when it is through
+        if (count > group && !__all_sync(kAll, mbar_wait_bounded(smem_u32(&lempty[mine.slot]), mine.parity, kWaitTimeoutProducer, abort_flag)))
+          break;
+        if (lane == 0) ask_tile(smem_u32(&s_told), smem_u32(&told));
+        asked = true;
         if (!__all_sync(kAll, mbar_wait_bounded(smem_u32(&told), answers & 1u, kWaitTimeoutProducer, abort_flag))) break;
         asked = false;
         ++answers;
@@ -634,6 +639,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     Turn<2> bt, lt;
     uint32_t hparity = 0;
     bool ok = true;
+    // all of H's partials are written, and x (which out may overlay) is read, before anything is read or written here
+    if constexpr (MODE == kOutOnly) asm volatile("griddepcontrol.wait;" ::: "memory");
     // 16-byte pieces of a row of the H tile are swizzled by the row's place in its eight; eight pieces to 16 KB
     auto piece_at = [&](int e) { return reinterpret_cast<uint4*>(sH + (e >> 3) * kXBytes + r * 128 + (((e & 7) ^ (r & 7)) << 4)); };
     while (true) {
@@ -646,7 +653,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       const bool live = row < p.T;
       const int count = s_count[lt.slot], groups = (count + group - 1) / group, slot = s_slot[lt.slot][r];
       const float w = MODE != kHOnly && slot >= 0 && p.scale != nullptr ? __ldg(p.scale + s_list[lt.slot][slot]) : 1.0f;
-      mbar_arrive(smem_u32(&lempty[lt.slot]));
+      if (groups <= 1) mbar_arrive(smem_u32(&lempty[lt.slot]));
+      const Turn<2> held = lt;
       lt.next();
       const bool whole = is_whole(groups);
       const T* y = static_cast<const T*>(p.y) + row * p.ldy;
@@ -679,7 +687,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
             for (int k = 0; k < p.splits; ++k) {
-              const float4 f = __ldg(from + k * (p.T * p.rank / 4)), h = __ldg(from + k * (p.T * p.rank / 4) + 1);
+              const float4 f = __ldcg(from + k * (p.T * p.rank / 4)), h = __ldcg(from + k * (p.T * p.rank / 4) + 1);
               s[0] += f.x;
               s[1] += f.y;
               s[2] += f.z;
@@ -722,7 +730,6 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         if constexpr (MODE != kHOnly) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(smem_u32(&hready));
         if (whole) {
-          int last = -1;  // the stage whose store may still be reading
           for (int ch = ch0; ch < ch1; ++ch) {
             ok = ok && mbar_wait_bounded(smem_u32(&full[ring.slot]), ring.parity, kWaitTimeoutEpilogue, abort_flag) &&
                  mbar_wait_bounded(smem_u32(&dfull[bt.slot]), bt.parity, kWaitTimeoutEpilogue, abort_flag);
@@ -757,18 +764,13 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                            "r"(smem_u32(sX + ring.slot * kXBytes)), "r"(ch * kChunk), "r"(tile * kRows)
                            : "memory");
               asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-              if (last >= 0) {
-                asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                mbar_arrive(smem_u32(&empty[last]));
-              }
-              last = ring.slot;
+              // free as soon as it is read: at the ring's two or three stages, leaving that to the next chunk held y's
+              // requests back by one (9001 x 1000 to 1544: out alone 35 us)
+              asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+              mbar_arrive(smem_u32(&empty[ring.slot]));
             }
             ring.next();
             bt.next();
-          }
-          if (threadIdx.x == 64) {
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            if (last >= 0) mbar_arrive(smem_u32(&empty[last]));
           }
         } else if constexpr (MODE != kHOnly) {
           for (int ch = ch0; ch < ch1; ++ch) {
@@ -804,6 +806,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
           }
         }
       }
+      if (groups > 1) mbar_arrive(smem_u32(&lempty[held.slot]));
     }
     if (threadIdx.x == 64) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
@@ -836,7 +839,8 @@ static Plan plan_of(int64_t T, int K, int N, int rank) {
   if (tiles * 2 <= sms) {  // two CTAs an SM are resident; below half of the SMs the two phases are spread
     const int64_t want = 2 * sms / tiles;
     q.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, (int64_t)(kblocks + 3) / 4, 16}));
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(want, chunks));
+    // every part sums H's partials again: two chunks at least for each
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(want, chunks / 2));
     q.chunks = (int)((chunks + parts - 1) / parts);
     if (q.splits == 1 && q.chunks == chunks) return q;
     if (q.splits == 1) q.splits = -1;  // apart, without a split of K
@@ -923,8 +927,18 @@ static int run_tiles(Params& p, const Plan& q, CUtensorMapDataType dt, cudaStrea
   tile_kernel<T, kHOnly><<<dim3(q.tiles, p.splits), kTileThreads, Tile<kHOnly>::kSmem, st>>>(tmX, tmA, tmB, tmY, tmO, p);
   if ((rc = check_cuda(cudaGetLastError(), "low-rank tile_kernel launch (H)"))) return rc;
   const int parts = ((p.N + kChunk - 1) / kChunk + p.chunks - 1) / p.chunks;
-  tile_kernel<T, kOutOnly><<<dim3(q.tiles, parts), kTileThreads, Tile<kOutOnly>::kSmem, st>>>(tmX, tmA, tmB, tmY, tmO, p);
-  return check_cuda(cudaGetLastError(), "low-rank tile_kernel launch (out)");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(q.tiles, parts);
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = Tile<kOutOnly>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, tile_kernel<T, kOutOnly>, tmX, tmA, tmB, tmY, tmO, p),
+                    "low-rank tile_kernel launch (out)");
 }
 
 }  // namespace lowrank
