@@ -21,9 +21,14 @@
 // Each lane sorts its V words once (a network of minima and maxima), so a round
 // is one maximum over the lanes' heads and a shift in the lane that had it.
 //
-// What bounds it: instructions, not bytes (16411 x 256 fp32 logits are 17 MB, 2.8
-// us).  Rounds over unsorted lanes and 64-bit words took 25.6 M warp instructions
-// and 40 us there.
+// What bounds it: the launch for small calls (one token 2.5 us, 103725 x 8 4.2 us),
+// instructions for many experts (integer minima, maxima and selects run at half
+// rate), never bytes.  16411 x 256 fp32 in groups with a bias (17 MB, 2.8 us of HBM):
+// 18.8 M warp instructions, 29 us, of which about 11 are one or two tokens whose
+// groups are decided again in fp64, late in the grid; rounds over unsorted lanes and
+// 64-bit words took 25.6 M and 40 us.  24490 x 64: 7.3 us forward, 6.2 backward.
+// Eight values a lane: with sixteen (half the lanes a token) 16411 x 256 took 22 us
+// for 14 (bf16, no bias), and a persistent grid that asked a token ahead 20.
 #include "common.cuh"
 
 namespace rb {
@@ -237,7 +242,10 @@ template <int L, int V>
 __device__ __forceinline__ float scores(const float* l, int kind, float* s) {
   if (kind == kSigmoid) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = __fdividef(1.0f, 1.0f + expf(-l[i]));
+    for (int i = 0; i < V; ++i) {
+      const float e = expf(-fabsf(l[i]));  // at most 1: no overflow, and small scores keep their precision
+      s[i] = __fdividef(l[i] < 0.0f ? e : 1.0f, 1.0f + e);
+    }
     return 1.0f;
   }
   float m = l[0];
@@ -434,12 +442,12 @@ __global__ void __launch_bounds__(kThreads) route_topk_kernel(const __grid_const
   // fp32 errors of a choice value, in units u = 2^-24 of the token's largest |score| + |bias|.  Softmax: l -
   // max and its exp x + 2 where the score is e^-x of the largest, the sum 21 additions and its terms' own
   // errors (at most 8), reciprocal and product 2, the bias added 1: at most 34.  Sigmoid: exp 2, 1 + that 1,
-  // the quotient 2, the bias 1: 6.  A word's dropped bits: 2 V.  Values are in doubt within twice the sum; a
+  // the quotient 4, the bias 1: 8.  A word's dropped bits: 2 V.  Values are in doubt within twice the sum; a
   // group's value is two of them added.
   bool doubt = false;
   float eps = 0.0f, eps_group = 0.0f;
   if constexpr (GUARD) {
-    const float base = p.by_logit ? 0.0f : p.kind == kSoftmax ? 34.0f : 6.0f;
+    const float base = p.by_logit ? 0.0f : p.kind == kSoftmax ? 34.0f : 8.0f;
     mag = sub_max<L>(mag) * 0x1p-24f;
     eps = 2.0f * (base + 2.0f * V) * mag;
     eps_group = 2.0f * (2.0f * base + 1.0f) * mag;

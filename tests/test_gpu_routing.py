@@ -176,6 +176,21 @@ def test_nan_infinity_and_masks_stay_in_their_rows(cuda_device):
     assert int(idx.min()) >= 0 and int(idx.max()) < 40
 
 
+def test_sigmoids_of_very_negative_logits_keep_their_ratios(cuda_device):
+    """Scores near fp32's smallest numbers: e^-85 is normal (1.2e-37), e^-95 subnormal (5.5e-42, in steps of 2^-149);
+    renormalised weights of the former are as exact as any."""
+    from baidu_cti_grab_b200 import device_ops
+
+    logits = (-85.0 - torch.rand(64, 24, generator=torch.Generator().manual_seed(1))).float()
+    idx, w, _, _ = device_ops.route_topk(logits.to(cuda_device), 4, score="sigmoid", renormalize=True)
+    want_idx, want_w, _ = _reference(logits, 4, "sigmoid", None, 1, 1, 2, True, 1.0)
+    assert torch.equal(idx.cpu(), want_idx)
+    _close(w, want_w, FP, 2.0 ** -18)
+    low = (logits - 10.0).to(cuda_device)
+    _, _, probs, _ = device_ops.route_topk(low, 4, score="sigmoid", want_probs=True)
+    assert bool(((probs.cpu().double() - torch.sigmoid(logits.double() - 10.0)).abs() <= 2.0 ** -148).all())
+
+
 def test_strides_types_and_no_tokens(cuda_device):
     from baidu_cti_grab_b200 import device_ops
 
