@@ -21,6 +21,13 @@
 //     weights' gradients over all of its team's rows; teams and then CTAs are summed
 //     in a fixed order (no atomics: the same bits every time).
 // A team is a warp for narrow rows (no barrier but the warp's own), a CTA for wide.
+//
+// Measured on a B200 (6.55 TB/s copy): forward 103725 x 512 bf16, layer norms, channel gate 85 us (0.76 of HBM); both
+// directions 24490 x 512 fp16 with a sigmoid gate of every element 96 us (forward 29, backward 60, sums 5; floor 38), 4099 x
+// 5000 bf16 RMS 156 us (57, 100, 8; floor 50).  Backward is bound by instructions and the two dependent row sums: 1210
+// warp instructions a row at 512, issue slots half used at the 16 warps of an SM that its registers allow; wide rows
+// leave one row an SM.  Bounds of single values (rows that are no multiple of 8 wide) in the same loops took 1620 and
+// 131 us; five column sums instead of four and one thread asking for all copies 199 us.
 #include "common.cuh"
 
 #include <algorithm>

@@ -23,6 +23,14 @@
 // two GEMMs being 2 r (K + N) operations a token.  h is rounded to the model type
 // before the second product (its operand on the tensor cores), as it is where the
 // two products are separate operations; sums are fp32, out is rounded once.
+//
+// Measured on a B200: 64 tokens of their own adapters (512 to 1536, rank 16) 5.5 us,
+// a launch, a cluster barrier and three dependent reads; 103725 x 512 to 512, rank 16,
+// 82 us (0.60 of HBM: tiles take 17-21 us at the bandwidth, the few with over four
+// adapters 40 and end last); 4099 x 14336 to 512, rank 32, 47 us (H alone 28, at the
+// HBM rate of x; out alone about 17, most of it its start and the partial sums); 9001
+// x 1000 to 1544, rank 8, in runs of 7, 48 us (H 13, out 31 in its longest tile).
+// Ranks padded to 16 columns and four warps of rows took 83 us there.
 #include "common.cuh"
 
 #include <algorithm>
