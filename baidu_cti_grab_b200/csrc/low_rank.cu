@@ -246,6 +246,38 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   else return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
+// The tile's product adds the other adapters' columns times zeros, and a zero times an infinity or NaN in one of
+// THEIR B's is a NaN.  So where a row's 32 sums are not all finite they are taken again from its own adapter alone (h as
+// the H tile holds it): out = y + w * delta for `n` columns from B row `b`, added to column q by `at` (which holds copies: captured by reference, what the rows keep in registers went to memory for it, and
+// 103725 x 512 took 97 us for 83).
+template <typename T, typename At>
+__device__ __noinline__ void add_own(const T* b, int n, int rank, const uint8_t* h_tile, int r, int e0, float w, At at) {
+#pragma unroll 1
+  for (int q = 0; q < n; ++q) {
+    float s = 0.0f;
+#pragma unroll 1
+    for (int j = 0; j < rank / 8; ++j) {
+      const int e = e0 + j;
+      const uint4 h = *reinterpret_cast<const uint4*>(h_tile + (e >> 3) * kXBytes + r * 128 + (((e & 7) ^ (r & 7)) << 4));
+      s = dot8<T>(__ldg(reinterpret_cast<const uint4*>(b + (int64_t)q * rank + 8 * j)), h, s);
+    }
+    at(q, w, s);
+  }
+}
+// whether the first n of 32 are finite: their sum times zero is NaN where one is not (columns beyond N hold anything)
+__device__ __forceinline__ bool all_finite(const uint32_t* v, int n) {
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (n >= 32) {
+#pragma unroll
+    for (int q = 0; q < 32; ++q) s[q & 3] = fmaf(__uint_as_float(v[q]), 0.0f, s[q & 3]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 32; ++q) s[q & 3] = q < n ? fmaf(__uint_as_float(v[q]), 0.0f, s[q & 3]) : s[q & 3];
+  }
+  const float all = (s[0] + s[1]) + (s[2] + s[3]);
+  return all == all;
+}
+
 // sixteen values of a row from column c on (0 beyond N) as they lie in memory, and back
 template <typename T>
 __device__ __forceinline__ void load16(const T* row, int c, int N, int vec, uint32_t* w) {
@@ -660,7 +692,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       const int64_t row = (int64_t)tile * kRows + r;
       const bool live = row < p.T;
       const int count = s_count[lt.slot], groups = (count + group - 1) / group, slot = s_slot[lt.slot][r];
-      const float w = MODE != kHOnly && slot >= 0 && p.scale != nullptr ? __ldg(p.scale + s_list[lt.slot][slot]) : 1.0f;
+      const int adapter = slot >= 0 ? s_list[lt.slot][slot] : 0;
+      const float w = MODE != kHOnly && slot >= 0 && p.scale != nullptr ? __ldg(p.scale + adapter) : 1.0f;
       if (groups <= 1) mbar_arrive(smem_u32(&lempty[lt.slot]));
       const Turn<2> held = lt;
       lt.next();
@@ -748,7 +781,14 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + bt.slot * kChunk + half * 32), v);
             tc::tc_fence_before();
             mbar_arrive(smem_u32(&dempty[bt.slot]));
-            if (mine >= 0 && ok) {
+            const int n0 = ch * kChunk + half * 32;
+            if (mine >= 0 && ok && !all_finite(v, p.N - n0)) {
+              add_own<T>(static_cast<const T*>(p.b) + ((int64_t)adapter * p.N + n0) * p.rank, min(32, p.N - n0), p.rank, sH, r,
+                         mine * eights, w, [=](int q, float k, float d) {
+                           T* to = reinterpret_cast<T*>(mem + (((4 * half + (q >> 3)) ^ (r & 7)) << 4)) + (q & 7);
+                           *to = T(fmaf(k, d, to_f32(*to)));
+                         });
+            } else if (mine >= 0 && ok) {
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 uint4* at = reinterpret_cast<uint4*>(mem + (((4 * half + q) ^ (r & 7)) << 4));
@@ -799,7 +839,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + bt.slot * kChunk + half * 32), v);
             tc::tc_fence_before();
             mbar_arrive(smem_u32(&dempty[bt.slot]));
-            if (mine >= 0) {
+            if (mine >= 0 && !all_finite(v, p.N - c0)) {
+              add_own<T>(static_cast<const T*>(p.b) + ((int64_t)adapter * p.N + c0) * p.rank, min(32, p.N - c0), p.rank, sH, r,
+                         mine * eights, w, [=](int q, float k, float d) { out[c0 + q] = T(fmaf(k, d, to_f32(y[c0 + q]))); });
+            } else if (mine >= 0) {
               uint32_t o[16];
 #pragma unroll
               for (int q = 0; q < 16; ++q) {
@@ -812,6 +855,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             }
             bt.next();
           }
+          ok = rows_all(ok);  // a row's H is written by two threads: the next group's after both are done with this one's
         }
       }
       if (groups > 1) mbar_arrive(smem_u32(&lempty[held.slot]));

@@ -595,7 +595,7 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: Op
         counts = torch.empty((E,), dtype=torch.int32, device=dev)
         counts_ptr = counts.data_ptr()
     _call_on(dev, "rb_route_topk", logits.data_ptr(), _DT[dtype], ld, T, E, bias_ptr, k, kind, groups, topk_groups,
-             group_top, renormalize, scale, idx.data_ptr(), L.RB_I64 if idx_dtype is torch.int64 else L.RB_I32,
+             group_top, bool(renormalize), float(scale), idx.data_ptr(), L.RB_I64 if idx_dtype is torch.int64 else L.RB_I32,
              chosen.data_ptr(), _DT[score_dtype], probs_ptr, counts_ptr)
     return idx, chosen, probs, counts
 
@@ -632,7 +632,7 @@ def route_topk_backward(logits: torch.Tensor, idx: torch.Tensor, grad_score: Opt
     out = torch.empty((T, E), dtype=dtype, device=dev)
     _call_on(dev, "rb_route_topk_backward", logits.data_ptr(), _DT[dtype], ld, T, E, idx.data_ptr(),
              L.RB_I64 if idx.dtype is torch.int64 else L.RB_I32, idx.shape[1], gs_ptr, gs_type, gp_ptr, gp_type, kind,
-             renormalize, scale, out.data_ptr(), _DT[dtype])
+             bool(renormalize), float(scale), out.data_ptr(), _DT[dtype])
     return out
 
 
@@ -714,8 +714,8 @@ def sandwich_norm(x: torch.Tensor, h: torch.Tensor, *, post: Optional[str] = Non
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     z = torch.empty_like(y) if second[0] != L.RB_NORM_NONE else None
     stats = torch.empty((N, 4), dtype=torch.float32, device=dev) if want_stats else None
-    _call_on(dev, "rb_sandwich_norm", x2.data_ptr(), ldx, h2.data_ptr(), ldh, _DT[x.dtype], N, D, *first, post_eps, gk,
-             _ptr(g2), gt, ldg, act, scale, *second, pre_eps, y.data_ptr(), _ptr(z), _ptr(stats))
+    _call_on(dev, "rb_sandwich_norm", x2.data_ptr(), ldx, h2.data_ptr(), ldh, _DT[x.dtype], N, D, *first, float(post_eps), gk,
+             _ptr(g2), gt, ldg, act, float(scale), *second, float(pre_eps), y.data_ptr(), _ptr(z), _ptr(stats))
     return y, z, stats
 
 
@@ -753,7 +753,7 @@ def sandwich_norm_backward(grad_y: Optional[torch.Tensor], grad_z: Optional[torc
     ws_bytes = _plan_bytes(dev, "rb_sandwich_norm_workspace_size", N, D, _DT[x.dtype])
     ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
     _call_on(dev, "rb_sandwich_norm_backward", _ptr(dy), ldy, _ptr(dz), ldz, x2.data_ptr(), ldx, h2.data_ptr(), ldh,
-             stats.data_ptr(), _DT[x.dtype], N, D, *first, gk, _ptr(g2), gt, ldg, act, scale, *second, ws.data_ptr(),
+             stats.data_ptr(), _DT[x.dtype], N, D, *first, gk, _ptr(g2), gt, ldg, act, float(scale), *second, ws.data_ptr(),
              ws_bytes, dx.data_ptr(), dh.data_ptr(), *(_ptr(t) for t in outs))
     return (dx, dh, *outs)
 

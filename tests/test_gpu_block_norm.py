@@ -94,6 +94,11 @@ CASES = [
     (400, 4097, BF, FP, "rms", "layer", "channel", "sigmoid", 1.0),
     (310, 5000, BF, FP, "rms", "rms", "row", "none", 0.7),
     (20, 8191, HF, HF, "layer", "layer", "full", "none", 1.0),
+    (170, 5120, BF, BF, "layer", "layer", "full", "sigmoid", 1.0),   # the widest with constants in registers
+    (170, 5128, BF, BF, "layer", "layer", "channel", "none", 1.0),   # in shared memory
+    (33, 6144, BF, FP, "rms", "rms", None, "none", 1.0),
+    (33, 7200, FP, FP, "layer", "layer", "full", "none", 1.0),       # the widest fp32 of those
+    (33, 7208, FP, FP, "rms", "layer", "full", "none", 1.0),         # made for each row
     (160, 8192, FP, FP, "layer", "layer", "full", "sigmoid", 1.0),
 ]
 

@@ -136,6 +136,17 @@ def test_no_adapter_none_of_a_tile_and_nan(cuda_device):
         a2[4] = float("inf")  # an adapter that is not sound reaches its own tokens only
         adapter[3] = 0
         got = device_ops.low_rank_add(y, bad, a2, b, adapter, scale)
+        b2 = b.clone()
+        b2[4] = float("nan")
+        b2[4, ::3] = float("inf")
+        sick = device_ops.low_rank_add(y, x, a, b2, adapter, scale)
+        well = (adapter != 4) & (torch.arange(T, device=cuda_device) != 3)
+        # those of the others that shared a product with it are summed again, in another order: each within the
+        # rank's 16 rounded products of the other, then half a step of either
+        assert bool(sick[well].isfinite().all())
+        step = torch.finfo(HF).eps * clean[well].double().abs() + 16 * 2.0 ** -22
+        assert bool(((sick[well].double() - clean[well].double()).abs() <= step).all())
+        assert bool((~sick[adapter == 4].isfinite()).any(-1).all())
         rows = adapter != 4
         rows[3] = False
         assert torch.equal(got[rows], clean[rows])
