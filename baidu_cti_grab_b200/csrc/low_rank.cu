@@ -4,8 +4,8 @@
 //
 // Three kernels, by the sizes:
 //
-// * token kernel: a cluster of CTAs per token, CUDA cores.  Few tokens are bound by
-//   the latency of reading their adapters: the CTAs of a cluster split A's columns,
+// * token kernel: a cluster of CTAs per token, CUDA cores.  Few tokens (or few products
+//   in all) are bound by the latency of reading their adapters: the CTAs of a cluster split A's columns,
 //   share the partial h = A x through distributed shared memory and split B's rows.
 //   Also takes every shape that the tensor maps cannot.
 // * tile kernel: 128 tokens a CTA on tcgen05.  The tile's distinct adapters are
@@ -15,8 +15,8 @@
 //     out tile = H . [B_i | B_j | ...]^T               the zeros select the adapter
 //   so tokens need no sorting and a tile of mixed requests costs MMA work (of which
 //   there is plenty), not bytes.  A row is written in the group that has its adapter.
-// * the same split in two, H then out, when 128-token tiles are too few to fill the
-//   GPU: H is split along K (fp32 partials in the workspace, summed in a fixed
+// * the same split in two, H then out, when there is a 128-token tile an SM
+//   or fewer: H is split along K (fp32 partials in the workspace, summed in a fixed
 //   order), out along N.
 //
 // What bounds it: HBM from about 20k tokens (x and y read, out written once), the
@@ -26,10 +26,10 @@
 //
 // Measured on a B200: 64 tokens of their own adapters (512 to 1536, rank 16) 5.5 us,
 // a launch, a cluster barrier and three dependent reads; 103725 x 512 to 512, rank 16,
-// 82 us (0.60 of HBM: tiles take 17-21 us at the bandwidth, the few with over four
-// adapters 40 and end last); 4099 x 14336 to 512, rank 32, 47 us (H alone 28, at the
+// 83 us (0.59 of HBM: tiles take 17-21 us at the bandwidth, the few with over four
+// adapters 40 and end last); 4099 x 14336 to 512, rank 32, 49 us (H alone 28, at the
 // HBM rate of x; out alone about 17, most of it its start and the partial sums); 9001
-// x 1000 to 1544, rank 8, in runs of 7, 48 us (H 13, out 31 in its longest tile).
+// x 1000 to 1544, rank 8, in runs of 7, 49 us (H 13, out 31 in its longest tile).
 // Ranks padded to 16 columns and four warps of rows took 83 us there.
 #include "common.cuh"
 
@@ -877,18 +877,30 @@ struct Plan {
   int splits;  // 1: fused
   int chunks;  // 64-column chunks of a CTA of the out kernel
 };
-constexpr int kTokenMax = 96;
+// Tokens are taken one by one where there are few, or where all of their products are few (T rank (K + N) of 2^24):
+// the cost grows with the products, while tiles cost a start, and more for each group of adapters.  Token kernel / tiles
+// of one or two adapters / tiles of 8 and more, in us: 512 to 512, rank 8: 256 tokens 4.6 / 12.5 / 13.7, 1024 tokens 8.7 /
+// 12.8 / 13.8; 512 to 1536, rank 16: 256 tokens 7.4 / 13.5 / 42, 512 tokens 9.4 / 14.3 / 42; 512 to 512, rank 64: 256
+// tokens 13.4 / 18.7 / 47.  Above it: 14336 to 512, rank 32: 256 tokens 28 / 32-42 / 76, 512 tokens 48 / 34-44 / 75.
+constexpr int kTokenMax = 96, kTokenMaxOfFewProducts = 1024;
+constexpr int64_t kFewProducts = 1 << 24;
 
 static Plan plan_of(int64_t T, int K, int N, int rank) {
   Plan q{};
   if (T <= kTokenMax || rank % 8 != 0 || rank > 64 || K % 8 != 0) return q;
+  if (T <= kTokenMaxOfFewProducts && T * rank * ((int64_t)K + N) <= kFewProducts) return q;
   const int64_t tiles = (T + kRows - 1) / kRows;
   const int sms = sm_count();
   q.tiles = (int)tiles;
   q.splits = 1;
   const int kblocks = (K + 63) / 64, chunks = (N + kChunk - 1) / kChunk;
   q.chunks = chunks;
-  if (tiles * 2 <= sms) {  // two CTAs an SM are resident; below half of the SMs the two phases are spread
+  // Two CTAs an SM are resident: up to a tile an SM the two phases are spread over them.  Apart / fused, in us, in runs of
+  // 100 and of 1 token: 18000 x 14336 to 512, rank 32: 115 and 387 / 217 and 844; 18000 x 512 to 1536, rank 16: 40 and 121
+  // / 39 and 235; the other way 18000 x 512 to 512, rank 8: 20 and 22 / 18.6 and 19.6.  Above it fused: two parts a tile
+  // gained where most rows of a tile have their own adapter and lost where they share them (60000 x 2048 to 2048, rank 32,
+  // runs of 1, 100 and 3000: 361, 213 and 211 / 488, 212 and 156).
+  if (tiles <= sms) {
     const int64_t want = 2 * sms / tiles;
     q.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, (int64_t)(kblocks + 3) / 4, 16}));
     // every part sums H's partials again: two chunks at least for each

@@ -399,10 +399,11 @@ int rb_sandwich_norm_backward(const void* dy, int64_t ldy, const void* dz, int64
  *   scale      [R] fp32 or NULL (1)
  *   workspace  rb_low_rank_workspace_size(T, K, N, rank) bytes (may be 0; -1: bad
  *              shape), 16-byte aligned
- * Sums are fp32; from 97 tokens on, where rank and K are multiples of 8, rank <= 64
+ * Sums are fp32.  Above 96 tokens, where rank and K are multiples of 8, rank <= 64
  * and x, a and b are on 16-byte rows, the products run on the tensor cores and
- * A_i x is rounded to the model type between them; else it stays fp32.  out is
- * rounded once.  Forward only.
+ * A_i x is rounded to the model type between them; up to 1024 tokens only if
+ * T rank (K + N) is above 2^24.  Else A_i x stays fp32.  out is rounded once.
+ * Forward only.
  */
 int64_t rb_low_rank_workspace_size(int64_t T, int K, int N, int rank);
 int rb_low_rank_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int dtype, int64_t T, int K,

@@ -155,6 +155,57 @@ def test_no_adapter_none_of_a_tile_and_nan(cuda_device):
     assert y0.shape == (0, 80)
 
 
+@pytest.mark.parametrize("T,K,N,rank,R,dtype,run", [
+    (1024, 512, 512, 16, 5, BF, 30),        # the last that is taken token by token: 2^24 products
+    (1025, 512, 512, 16, 5, BF, 30),        # and tiles from there on
+    (1024, 512, 520, 16, 5, BF, 30),
+    (97, 14336, 512, 32, 3, BF, 1),         # few tokens, many products: tiles
+    (1025, 8, 16, 8, 2, HF, 10),
+    (1409, 72, 200, 8, 7, BF, 9),
+    (1100, 200, 100, 64, 3, BF, 50),
+    (1100, 200, 101, 24, 5, HF, 20),
+    (1026, 1000, 1544, 8, 24, HF, 7),
+    (1100, 512, 640, 40, 9, BF, 3),
+    (1152, 512, 512, 16, 300, BF, 1),       # every row of a tile its own adapter
+    (10000, 512, 1536, 16, 32, BF, 1),      # above half of the SMs in tiles: still H and out apart
+    (10001, 1000, 200, 32, 6, HF, 40),
+    (18900, 256, 192, 8, 11, BF, 60),
+])
+def test_tiles_above_the_token_kernels_share(cuda_device, T, K, N, rank, R, dtype, run):
+    test_against_float64(cuda_device, T, K, N, rank, R, dtype, run)
+
+
+@pytest.mark.parametrize("T,rank", [(1500, 16), (1500, 64), (12000, 8)])
+def test_tiles_apart_strides_none_and_what_is_not_finite(cuda_device, T, rank):
+    """H and out apart: rows at odd places, tokens without an adapter, adapters that are not sound."""
+    from baidu_cti_grab_b200 import _lib, device_ops
+
+    K, N = 640, 200
+    args = _inputs(T, K, N, rank, 6, BF, 12, T + rank)
+    y, x, a, b, adapter, scale = (t.to(cuda_device) for t in args)
+    assert _lib.load().rb_low_rank_workspace_size(T, K, N, rank) > 0
+    want = device_ops.low_rank_add(y, x, a, b, adapter, scale)
+    _check(want, *args)
+    for ldx, ld, off in ((K + 8, N + 8, 8), (K + 16, N + 3, 1)):
+        xv = torch.zeros(T, ldx, dtype=BF, device=cuda_device)[:, :K]
+        xv.copy_(x)
+        ry, ro = (torch.full((T * ld + off,), 7.0, dtype=BF, device=cuda_device) for _ in range(2))
+        yv, ov = ry[off:].view(T, ld)[:, :N], ro[off:].view(T, ld)
+        yv.copy_(y)
+        assert torch.equal(device_ops.low_rank_add(yv, xv, a, b, adapter, scale, out=ov[:, :N]), want)
+        assert bool((ov[:, N:] == 7.0).all()) and bool((ro[:off] == 7.0).all())
+    none = torch.full_like(adapter, -1)
+    none[::2] = 6  # past the bank
+    assert torch.equal(device_ops.low_rank_add(y, x, a, b, none, scale), y)
+    a2, b2 = a.clone(), b.clone()
+    a2[4] = float("inf")
+    b2[4] = float("nan")
+    rows = adapter != 4
+    assert torch.equal(device_ops.low_rank_add(y, x, a2, b, adapter, scale)[rows], want[rows])
+    sick = device_ops.low_rank_add(y, x, a, b2, adapter, scale)
+    assert bool(sick[rows].isfinite().all()) and bool((~sick[~rows].isfinite()).all())
+
+
 def test_bank_streams_and_graphs(cuda_device):
     from baidu_cti_grab_b200 import adapters, device_ops
 
