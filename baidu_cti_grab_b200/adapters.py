@@ -55,9 +55,12 @@ class AdapterBank(nn.Module):
     @staticmethod
     def per_token(request_adapter: torch.Tensor, offsets: torch.Tensor, n_tokens: int) -> torch.Tensor:
         """int32 [n_tokens]: each token's adapter, from its request's, request u being the tokens
-        offsets[u] .. offsets[u + 1] - 1 (the batch's ``user_offsets``); nothing is read back."""
-        lengths = offsets[1:] - offsets[:-1]
-        return torch.repeat_interleave(request_adapter.to(torch.int32), lengths, output_size=n_tokens)
+        offsets[u] .. offsets[u + 1] - 1 (the batch's ``user_offsets``); -1 for tokens before the first
+        and behind the last (a padded batch).  Nothing is read back."""
+        token = torch.arange(n_tokens, dtype=offsets.dtype, device=offsets.device)
+        request = torch.searchsorted(offsets[1:].contiguous(), token, right=True)
+        who = nn.functional.pad(request_adapter.to(torch.int32), (0, 1), value=-1)[request]
+        return who.masked_fill_(token < offsets[0], -1)
 
     @torch.no_grad()
     def forward(self, y: torch.Tensor, x: torch.Tensor, adapter: torch.Tensor, out: Optional[torch.Tensor] = None):

@@ -759,6 +759,18 @@ def sandwich_norm_backward(grad_y: Optional[torch.Tensor], grad_z: Optional[torc
 
 
 # -------------------------------------------------------- low-rank adapters
+def _rows_overlap(a: torch.Tensor, lda: int, b: torch.Tensor, ldb: int) -> bool:
+    """Whether two matrices of the same type and height, rows contiguous and lda / ldb apart, share elements (those of
+    different pitch in one range of memory are taken to)."""
+    (T, wa), wb, size = a.shape, b.shape[1], a.element_size()
+    if T == 0 or wa == 0 or wb == 0:
+        return False
+    d, odd = divmod(b.data_ptr() - a.data_ptr(), size)
+    if d >= (T - 1) * lda + wa or -d >= (T - 1) * ldb + wb:
+        return False
+    return lda != ldb or odd != 0 or not wa <= d % lda <= lda - wb
+
+
 def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.Tensor,
                  scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[t] + scale[i] * b[i] @ (a[i] @ x[t]) with i = adapter[t] (rb_low_rank_add): the adapters of many
@@ -766,7 +778,7 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
 
     y [T, N] and x [T, K] bf16/f16; a [R, rank, K] and b [R, N, rank] contiguous in the same type, rank <= 128;
     adapter int32/int64 [T], -1 (or anything outside [0, R)) for a token without one; scale fp32 [R].
-    ``out`` may be y.  Forward only: an input that asks for a gradient is refused."""
+    ``out`` may be y, and shares no other memory with y or x.  Forward only: an input that asks for a gradient is refused."""
     dev = _device_of("low_rank_add", y, x, a, b, adapter, scale, out)
     if y.dim() != 2 or x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
         raise ValueError("low_rank_add expects y [T, N], x [T, K], a [R, rank, K] and b [R, N, rank]")
@@ -788,18 +800,24 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad
                                     or (scale is not None and scale.requires_grad)):
         raise RuntimeError("low_rank_add has no backward: call it under torch.no_grad() or on detached tensors")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((T, N), dtype=dtype, device=dev)
     elif out.shape != (T, N) or out.dtype is not dtype or (N > 1 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N):
         raise ValueError(f"out must be a row-major [{T}, {N}] {dtype} tensor")
     y, ldy = _rows_of(y, T, N)
     x, ldx = _rows_of(x, T, K)
+    ldo = max(out.stride(0), N)
+    if given:
+        in_place = out.data_ptr() == y.data_ptr() and ldo == ldy
+        if (not in_place and _rows_overlap(out, ldo, y, ldy)) or _rows_overlap(out, ldo, x, ldx):
+            raise ValueError("out may be y itself, and must not overlap y or x elsewhere")
     adapter = adapter.contiguous()
     ws_bytes = _plan_bytes(dev, "rb_low_rank_workspace_size", T, K, N, rank)
     ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev) if ws_bytes else None
     _call_on(dev, "rb_low_rank_add", y.data_ptr(), ldy, x.data_ptr(), ldx, _DT[dtype], T, K, N, a.data_ptr(), b.data_ptr(), R,
              rank, adapter.data_ptr(), L.RB_I64 if adapter.dtype is torch.int64 else L.RB_I32, _ptr(scale), _ptr(ws), ws_bytes,
-             out.data_ptr(), max(out.stride(0), N))
+             out.data_ptr(), ldo)
     return out
 
 

@@ -206,6 +206,25 @@ def test_tiles_apart_strides_none_and_what_is_not_finite(cuda_device, T, rank):
     assert bool(sick[rows].isfinite().all()) and bool((~sick[~rows].isfinite()).all())
 
 
+@pytest.mark.parametrize("T", [30, 3000, 20000])
+def test_out_over_another_input_is_refused(cuda_device, T):
+    from baidu_cti_grab_b200 import device_ops
+
+    y, x, a, b, adapter, scale = (t.to(cuda_device) for t in _inputs(T, 64, 64, 8, 3, BF, 5, 1))
+    rows = torch.zeros(T + 1, 160, dtype=BF, device=cuda_device)
+    yv, xv, ov = rows[:T, :64], rows[:T, 64:128], rows[1:, :64]
+    yv.copy_(y)
+    xv.copy_(x)
+    before = rows.clone()
+    for bad in (ov, xv, rows[:T, 96:160], rows[:T, 8:72], rows.view(-1)[: T * 64].view(T, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            device_ops.low_rank_add(yv, xv, a, b, adapter, scale, out=bad)
+    assert torch.equal(rows, before)
+    want = device_ops.low_rank_add(y, x, a, b, adapter, scale)
+    assert torch.equal(device_ops.low_rank_add(yv, xv, a, b, adapter, scale, out=yv), want)  # beside x in one buffer
+    assert torch.equal(xv, x)
+
+
 def test_bank_streams_and_graphs(cuda_device):
     from baidu_cti_grab_b200 import adapters, device_ops
 

@@ -21,8 +21,8 @@ def _call(y=FAKE, ldy=512, x=FAKE, ldx=256, dtype=1, T=4, K=256, N=512, a=FAKE, 
     (dict(rank=129), "ranks"), (dict(dtype=0), "bf16"), (dict(it=1), "adapter ids"), (dict(T=1 << 29), "tokens"),
     (dict(R=1 << 24), "rows of all"), (dict(ldy=511), "leading"), (dict(ldo=1), "leading"), (dict(ldx=255), "leading"),
     (dict(y=None), "null"), (dict(x=None), "null"), (dict(a=None), "null"), (dict(b=None), "null"), (dict(idx=None), "null"),
-    (dict(out=None), "null"), (dict(T=1000), "workspace"), (dict(T=1000, ws=FAKE, size=16), "workspace"),
-    (dict(T=1000, ws=FAKE + 4, size=1 << 30), "workspace")])
+    (dict(out=None), "null"), (dict(T=2000), "workspace"), (dict(T=2000, ws=FAKE, size=16), "workspace"),
+    (dict(T=2000, ws=FAKE + 4, size=1 << 30), "workspace")])
 def test_refuses_on_the_host(bad, word):
     from baidu_cti_grab_b200 import _lib
 
@@ -54,3 +54,36 @@ def test_wrappers_refuse():
         adapters.AdapterBank(a, b[:1])
     with pytest.raises(ValueError):
         adapters.AdapterBank.stack([])
+
+
+def test_per_token_of_padded_and_empty_requests():
+    """Tokens outside every request have no adapter, whatever the batch's length."""
+    from baidu_cti_grab_b200.adapters import AdapterBank
+
+    who = torch.tensor([2, 0, -1, 1])
+    offsets = torch.tensor([1, 3, 3, 5, 6])
+    for dtype in (torch.int64, torch.int32):
+        got = AdapterBank.per_token(who, offsets.to(dtype), 9)
+        assert got.dtype == torch.int32 and got.tolist() == [-1, 2, 2, -1, -1, 1, -1, -1, -1]
+        assert AdapterBank.per_token(who, offsets.to(dtype), 4).tolist() == [-1, 2, 2, -1]
+        assert AdapterBank.per_token(who[:0], offsets[:1].to(dtype), 3).tolist() == [-1, -1, -1]
+        assert AdapterBank.per_token(who, offsets.to(dtype), 0).shape == (0,)
+
+
+def test_overlapping_rows_are_seen():
+    from baidu_cti_grab_b200.device_ops import _rows_overlap
+
+    g = torch.Generator().manual_seed(0)
+    both = [0, 0]
+    for _ in range(2000):
+        T, wa, wb, lda, same, off = (int(torch.randint(lo, hi, (1,), generator=g))
+                                     for lo, hi in ((1, 5), (1, 6), (1, 6), (6, 12), (0, 4), (-40, 41)))
+        ldb = lda if same else lda + 1
+        buf = torch.zeros(200, dtype=torch.bfloat16)
+        a, b = buf.as_strided((T, wa), (lda, 1), 80), buf.as_strided((T, wb), (ldb, 1), 80 + off)
+        a.fill_(1)
+        shared = bool((b == 1).any())
+        said = _rows_overlap(a, lda, b, ldb)
+        both[said] += 1
+        assert said == shared or (said and lda != ldb and T > 1)
+    assert min(both) > 100
