@@ -20,9 +20,12 @@
 //   order), out along N.
 //
 // What bounds it: HBM from about 20k tokens (x and y read, out written once), the
-// two GEMMs being 2 r (K + N) operations a token.  h is rounded to the model type
-// before the second product (its operand on the tensor cores), as it is where the
-// two products are separate operations; sums are fp32, out is rounded once.
+// two GEMMs being 2 r (K + N) operations a token.  Sums are fp32.  The second product
+// takes h in two values of the model type (16 or 22 bits; fp16 rows are brought into
+// the type's range first), the second of them from TMEM: the MMAs are twice as many
+// and cost nothing that was measured, splitting and storing h costs 3-6 % (103725 x
+// 512 83 -> 85.5 us, 4099 x 14336 48 -> 51, 9001 x 1000 50 -> 52.5).  With h rounded
+// to the type, out was 1.25 times as far from the exact sum.  out is rounded once.
 //
 // Measured on a B200: 64 tokens of their own adapters (512 to 1536, rank 16) 5.5 us,
 // a launch, a cluster barrier and three dependent reads; 103725 x 512 to 512, rank 16,
@@ -185,8 +188,10 @@ struct Tile {
   static constexpr int kHBytes = MODE == kHOnly ? 0 : (kCols + 63) / 64 * kXBytes;  // 64-column tiles of 16 KB
   static constexpr int kBBytes = MODE == kHOnly ? 0 : kChunk * kCols * 2;
   static constexpr int kSmem = 1024 + kStages * (kXBytes + kABytes) + kHBytes + 2 * kBBytes + kZeroBytes;
-  static constexpr int kHCols = MODE == kOutOnly ? 0 : kCols;  // TMEM: H, then two out chunks
-  static constexpr int kTmemCols = MODE == kFused ? 256 : 128;
+  // TMEM: H, then two out chunks, then the rest of what the H tile holds of h (two columns of H to a 32-bit word)
+  static constexpr int kHCols = MODE == kOutOnly ? 0 : kCols;
+  static constexpr int kRestAt = kHCols + 2 * kChunk;
+  static constexpr int kTmemCols = MODE == kHOnly ? 128 : 256;
 };
 
 // K-major operand without swizzle: eight rows of 16 bytes are 128 bytes in a row, groups of eight rows follow each
@@ -221,6 +226,28 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
 }
 
+// the same with A in TMEM: sixteen columns of a row are eight 32-bit words of its lane, the lower column in the lower half
+__device__ __forceinline__ void umma_f16_from_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* w) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(w[0]),
+               "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* w) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+      : "r"(taddr)
+      : "memory");
+}
+
 // whether all threads of the rows' warps say so; they meet here
 __device__ __forceinline__ bool rows_all(bool ok) {
   uint32_t every;
@@ -246,22 +273,56 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   else return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
+// h as the second product takes it: two values of the model type, top = h rounded and rest = what is left, rounded.  Their
+// sum is off by 2^-18 of h in bf16 and 2^-22 in fp16 (half a step of a half step), where top alone would be off by 2^-9 and
+// 2^-11: a token's result would then depend on whether its batch is taken by tokens or by tiles.
+template <typename T>
+__device__ __forceinline__ void split2(float a, float b, uint32_t& top, uint32_t& rest) {
+  top = pack2<T>(a, b);
+  const float2 u = unpack2<T>(top);
+  rest = pack2<T>(fabsf(u.x) < INFINITY ? a - u.x : 0.0f, fabsf(u.y) < INFINITY ? b - u.y : 0.0f);
+}
+// The power of two that brings a row of h, whose largest finite magnitude is `peak`, to [2^14, 2^15): in fp16 h itself may
+// be out of the type's range (65504), and its last bits are lost below 2^-14.  `down` takes it back.
+__device__ __forceinline__ float row_factor(float peak, float& down) {
+  const int up = min(14 - ((int)(__float_as_uint(peak) >> 23) - 127), 100);  // at least -113
+  down = __uint_as_float((uint32_t)(127 - up) << 23);
+  return __uint_as_float((uint32_t)(127 + up) << 23);
+}
+__device__ __forceinline__ float finite_max(float peak, float v) { return fabsf(v) < INFINITY ? fmaxf(peak, fabsf(v)) : peak; }
+
 // The tile's product adds the other adapters' columns times zeros, and a zero times an infinity or NaN in one of
-// THEIR B's is a NaN.  So where a row's 32 sums are not all finite they are taken again from its own adapter alone (h as
-// the H tile holds it): out = y + w * delta for `n` columns from B row `b`, added to column q by `at` (which holds copies: captured by reference, what the rows keep in registers went to memory for it, and
-// 103725 x 512 took 97 us for 83).
+// THEIR B's is a NaN.  So where a row's 32 sums are not all finite (`redo`) they are taken again from its own adapter alone (h as
+// the H tile and, its rest, TMEM hold it): out = y + w * delta for `n` columns from B row `b`, added to column q by `at`
+// (which holds copies: captured by reference, what the rows keep in registers went to memory for it, and 103725 x 512
+// took 97 us for 83).  Called by whole warps, whose lanes read their rows of TMEM together.
 template <typename T, typename At>
-__device__ __noinline__ void add_own(const T* b, int n, int rank, const uint8_t* h_tile, int r, int e0, float w, At at) {
+__device__ __noinline__ void add_own(bool redo, const T* b, int n, int rank, const uint8_t* h_tile, uint32_t rest_at, int sixteens,
+                                     int r, int e0, float w, At at) {
 #pragma unroll 1
   for (int q = 0; q < n; ++q) {
     float s = 0.0f;
 #pragma unroll 1
-    for (int j = 0; j < rank / 8; ++j) {
-      const int e = e0 + j;
-      const uint4 h = *reinterpret_cast<const uint4*>(h_tile + (e >> 3) * kXBytes + r * 128 + (((e & 7) ^ (r & 7)) << 4));
-      s = dot8<T>(__ldg(reinterpret_cast<const uint4*>(b + (int64_t)q * rank + 8 * j)), h, s);
+    for (int k = 0; k < sixteens; ++k) {
+      uint32_t rest[8];
+      __syncwarp();
+      tmem_ld8(rest_at + (uint32_t)(8 * k), rest);
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        const int e = 2 * k + d, j = e - e0;
+        if (!redo || j < 0 || j >= rank / 8) continue;
+        const uint4 h = *reinterpret_cast<const uint4*>(h_tile + (e >> 3) * kXBytes + r * 128 + (((e & 7) ^ (r & 7)) << 4));
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(b + (int64_t)q * rank + 8 * j));
+        const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 t = unpack2<T>(hw[i]), u = unpack2<T>(rest[4 * d + i]), f = unpack2<T>(vw[i]);
+          s = fmaf(f.x, t.x + u.x, s);
+          s = fmaf(f.y, t.y + u.y, s);
+        }
+      }
     }
-    at(q, w, s);
+    if (redo) at(q, w, s);
   }
 }
 // whether the first n of 32 are finite: their sum times zero is NaN where one is not (columns beyond N hold anything)
@@ -384,6 +445,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   __shared__ int s_tile[2], s_count[2], s_list[2][kRows], s_slot[2][kRows];  // of this tile and the next; tile -1: no more
+  __shared__ float s_peak[2][MODE == kOutOnly ? kRows : 1];  // of a row's h, by its two warps
   __shared__ __align__(16) uint4 s_told;
   __shared__ __align__(8) uint64_t told;
   volatile int* abort_flag = &abort_word;
@@ -391,9 +453,6 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
   constexpr uint32_t kIdesc = (1u << 4) | kType | ((uint32_t)(kRows >> 4) << 24);  // N is added where it is known
 
-  // The out kernel may start while this one's last CTAs run: it lists its tiles and asks for B and y meanwhile, none
-  // of which this kernel writes.
-  if constexpr (MODE == kHOnly) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
@@ -433,6 +492,9 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  // The out kernel may start while this one's last CTAs run: it lists its tiles and asks for B and y meanwhile, none
+  // of which this kernel writes.  Not before this CTA has its TMEM: the out kernel holds its own while it waits for this one.
+  if constexpr (MODE == kHOnly) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int group = C::kCols / p.rank;  // adapters of a group
   const int kblocks = (p.K + 63) / 64;
   const int split = MODE == kFused ? 0 : (int)blockIdx.y;
@@ -586,8 +648,9 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                   const int in_box = (e * 8) & (p.unit - 1);
                   bd = swizzled_desc(at_b + (uint32_t)((e * 8 - in_box) * kChunk * 2), p.unit * 2) + (uint64_t)(in_box >> 3);
                 }
-                umma_f16(tmem + C::kHCols + bt.slot * kChunk, hd + (uint64_t)((at >> 2) * (kXBytes >> 4) + 2 * (at & 3)), bd, idesc,
-                         e > 0 ? 1u : 0u);
+                const uint32_t to = tmem + C::kHCols + bt.slot * kChunk;
+                umma_f16(to, hd + (uint64_t)((at >> 2) * (kXBytes >> 4) + 2 * (at & 3)), bd, idesc, e > 0 ? 1u : 0u);
+                umma_f16_from_tmem(to, tmem + C::kRestAt + 8 * at, bd, idesc, 1u);
               }
               tc::umma_commit(smem_u32(&bempty[bt.slot]));
               tc::umma_commit(smem_u32(&dfull[bt.slot]));
@@ -717,55 +780,126 @@ __global__ void __launch_bounds__(kTileThreads, 2)
           ring.skip(kb1 - kb0);
         }
         hparity ^= 1;
-        // own adapter's h into this row of the H tile, zeros into the others' columns: sixteen columns at a time, whose
-        // eights may be of two adapters
-        if constexpr (MODE == kOutOnly) {
-          for (int c = half * 16; c < n * p.rank; c += 32) *piece_at(c / 8) = *piece_at(c / 8 + 1) = make_uint4(0u, 0u, 0u, 0u);
-          for (int q = 0; mine >= 0 && q < eights; ++q) {
-            const int e = mine * eights + q;
-            if (((e >> 1) & 1) != half) continue;  // the other warp's sixteen columns
-            const float4* from = reinterpret_cast<const float4*>(p.part + row * p.rank + 8 * q);
-            float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-            for (int k = 0; k < p.splits; ++k) {
-              const float4 f = __ldcg(from + k * (p.T * p.rank / 4)), h = __ldcg(from + k * (p.T * p.rank / 4) + 1);
-              s[0] += f.x;
-              s[1] += f.y;
-              s[2] += f.z;
-              s[3] += f.w;
-              s[4] += h.x;
-              s[5] += h.y;
-              s[6] += h.z;
-              s[7] += h.w;
-            }
-            *piece_at(e) = make_uint4(pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3]), pack2<T>(s[4], s[5]), pack2<T>(s[6], s[7]));
-          }
-        } else {
+        // own adapter's h into this row of the H tile (and its rest into TMEM), zeros into the others' columns: sixteen
+        // columns at a time, whose eights may be of two adapters
+        const int e0 = mine * eights;  // its first eight
+        float wh = w;  // times what the row's factor left to take back
+        if constexpr (MODE == kHOnly) {
           for (int c = half * 16; c < n * p.rank; c += 32) {
-            const int e = c / 8;
-            const bool in[2] = {mine >= 0 && e / eights == mine, mine >= 0 && (e + 1) / eights == mine};
             uint32_t v[16];
             __syncwarp();
             tc::swp::tmem_ld16(tmem + lanes + (uint32_t)c, v);
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
-              if constexpr (MODE == kHOnly) {
-                if (!in[d]) continue;
-                float* to = p.part + ((int64_t)split * p.T + row) * p.rank + (c + 8 * d - mine * p.rank);
+              const int j = c / 8 + d - e0;
+              if (mine < 0 || j < 0 || j >= eights) continue;
+              float* to = p.part + ((int64_t)split * p.T + row) * p.rank + 8 * j;
 #pragma unroll
-                for (int q = 0; q < 8; q += 4)
-                  *reinterpret_cast<float4*>(to + q) =
-                      make_float4(__uint_as_float(v[8 * d + q]), __uint_as_float(v[8 * d + q + 1]),
-                                  __uint_as_float(v[8 * d + q + 2]), __uint_as_float(v[8 * d + q + 3]));
-              } else {
-                uint32_t h[4];
+              for (int q = 0; q < 8; q += 4)
+                *reinterpret_cast<float4*>(to + q) =
+                    make_float4(__uint_as_float(v[8 * d + q]), __uint_as_float(v[8 * d + q + 1]),
+                                __uint_as_float(v[8 * d + q + 2]), __uint_as_float(v[8 * d + q + 3]));
+            }
+          }
+        } else {
+          float factor = 1.0f, down = 1.0f, own[2][16];
+          int k0 = 0;  // out alone: own[i] are the sums of the row's sixteen columns k0 + 2 i, where those are its own
+          if constexpr (MODE == kOutOnly) {
+            // its eights, eight at most and then from a multiple of eight on, lie in two of this warp's sixteens at most
+            k0 = e0 >> 1;
+            if ((k0 & 1) != half) ++k0;
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  h[q] = in[d] ? pack2<T>(__uint_as_float(v[8 * d + 2 * q]), __uint_as_float(v[8 * d + 2 * q + 1])) : 0u;
-                *piece_at(e + d) = make_uint4(h[0], h[1], h[2], h[3]);
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+              for (int d = 0; d < 2; ++d) {
+                float* s = own[i] + 8 * d;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) s[q] = 0.0f;
+                const int j = 2 * (k0 + 2 * i) + d - e0;
+                if (mine < 0 || j < 0 || j >= eights) continue;
+                const float4* from = reinterpret_cast<const float4*>(p.part + row * p.rank + 8 * j);
+#pragma unroll 4
+                for (int k = 0; k < p.splits; ++k) {
+                  const float4 f = __ldcg(from + k * (p.T * p.rank / 4)), h = __ldcg(from + k * (p.T * p.rank / 4) + 1);
+                  s[0] += f.x;
+                  s[1] += f.y;
+                  s[2] += f.z;
+                  s[3] += f.w;
+                  s[4] += h.x;
+                  s[5] += h.y;
+                  s[6] += h.z;
+                  s[7] += h.w;
+                }
               }
             }
           }
+          if constexpr (std::is_same<T, __half>::value) {
+            float peak = 0.0f;
+            if constexpr (MODE == kOutOnly) {
+#pragma unroll
+              for (int q = 0; q < 32; ++q) peak = finite_max(peak, own[q >> 4][q & 15]);
+              s_peak[half][r] = peak;  // the row's other columns are the other warp's
+              ok = rows_all(ok);
+              peak = fmaxf(peak, s_peak[half ^ 1][r]);
+            } else {
+              for (int c = 0; c < n * p.rank; c += 16) {
+                uint32_t v[16];
+                __syncwarp();
+                tc::swp::tmem_ld16(tmem + lanes + (uint32_t)c, v);
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                  const int j = c / 8 + d - e0;
+                  if (mine < 0 || j < 0 || j >= eights) continue;
+#pragma unroll
+                  for (int q = 0; q < 8; ++q) peak = finite_max(peak, __uint_as_float(v[8 * d + q]));
+                }
+              }
+            }
+            factor = row_factor(peak, down);
+            wh = w * down;
+          }
+          auto split16 = [&](const float* v, uint32_t* top, uint32_t* rest) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              if constexpr (std::is_same<T, __half>::value) split2<T>(v[2 * q] * factor, v[2 * q + 1] * factor, top[q], rest[q]);
+              else split2<T>(v[2 * q], v[2 * q + 1], top[q], rest[q]);
+            }
+          };
+          uint32_t tops[MODE == kOutOnly ? 2 : 1][8], rests[MODE == kOutOnly ? 2 : 1][8];
+          if constexpr (MODE == kOutOnly) {
+            split16(own[0], tops[0], rests[0]);
+            split16(own[1], tops[1], rests[1]);
+          }
+          for (int c = half * 16; c < n * p.rank; c += 32) {
+            const int k = c / 16;
+            uint32_t top[8], rest[8];
+            if constexpr (MODE == kOutOnly) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                top[q] = k == k0 ? tops[0][q] : k == k0 + 2 ? tops[1][q] : 0u;
+                rest[q] = k == k0 ? rests[0][q] : k == k0 + 2 ? rests[1][q] : 0u;
+              }
+            } else {
+              uint32_t t[16];
+              float v[16];
+              __syncwarp();
+              tc::swp::tmem_ld16(tmem + lanes + (uint32_t)c, t);
+#pragma unroll
+              for (int d = 0; d < 2; ++d) {
+                const int j = 2 * k + d - e0;
+                const bool in = mine >= 0 && j >= 0 && j < eights;
+#pragma unroll
+                for (int q = 8 * d; q < 8 * d + 8; ++q) v[q] = in ? __uint_as_float(t[q]) : 0.0f;
+              }
+              split16(v, top, rest);
+            }
+            *piece_at(2 * k) = make_uint4(top[0], top[1], top[2], top[3]);
+            *piece_at(2 * k + 1) = make_uint4(top[4], top[5], top[6], top[7]);
+            __syncwarp();
+            tmem_st8(tmem + lanes + (uint32_t)(C::kRestAt + 8 * k), rest);
+          }
+          __syncwarp();
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
         tc::tc_fence_before();
         if constexpr (MODE != kHOnly) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -776,19 +910,23 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                  mbar_wait_bounded(smem_u32(&dfull[bt.slot]), bt.parity, kWaitTimeoutEpilogue, abort_flag);
             tc::tc_fence_after();
             uint8_t* mem = sX + ring.slot * kXBytes + r * 128;
+            const uint32_t sums = tmem + lanes + (uint32_t)(C::kHCols + bt.slot * kChunk + half * 32);
             uint32_t v[32];
             __syncwarp();
-            tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + bt.slot * kChunk + half * 32), v);
-            tc::tc_fence_before();
-            mbar_arrive(smem_u32(&dempty[bt.slot]));
+            tc::tmem_ld32(sums, v);
             const int n0 = ch * kChunk + half * 32;
-            if (mine >= 0 && ok && !all_finite(v, p.N - n0)) {
-              add_own<T>(static_cast<const T*>(p.b) + ((int64_t)adapter * p.N + n0) * p.rank, min(32, p.N - n0), p.rank, sH, r,
-                         mine * eights, w, [=](int q, float k, float d) {
+            const bool redo = mine >= 0 && ok && !all_finite(v, p.N - n0);
+            if (__any_sync(kAll, redo)) {
+              add_own<T>(redo, static_cast<const T*>(p.b) + ((int64_t)adapter * p.N + n0) * p.rank, min(32, p.N - n0), p.rank, sH,
+                         tmem + lanes + C::kRestAt, (n * eights + 1) / 2, r, e0, wh, [=](int q, float k, float d) {
                            T* to = reinterpret_cast<T*>(mem + (((4 * half + (q >> 3)) ^ (r & 7)) << 4)) + (q & 7);
                            *to = T(fmaf(k, d, to_f32(*to)));
                          });
-            } else if (mine >= 0 && ok) {
+              tc::tmem_ld32(sums, v);  // of the other rows (kept over the call they would go to memory)
+            }
+            tc::tc_fence_before();
+            mbar_arrive(smem_u32(&dempty[bt.slot]));
+            if (mine >= 0 && ok && !redo) {
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 uint4* at = reinterpret_cast<uint4*>(mem + (((4 * half + q) ^ (r & 7)) << 4));
@@ -798,7 +936,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   const float2 u = unpack2<T>(fw[i]);
-                  o[i] = pack2<T>(fmaf(w, __uint_as_float(v[8 * q + 2 * i]), u.x), fmaf(w, __uint_as_float(v[8 * q + 2 * i + 1]), u.y));
+                  o[i] = pack2<T>(fmaf(wh, __uint_as_float(v[8 * q + 2 * i]), u.x), fmaf(wh, __uint_as_float(v[8 * q + 2 * i + 1]), u.y));
                 }
                 *at = make_uint4(o[0], o[1], o[2], o[3]);
               }
@@ -834,20 +972,25 @@ __global__ void __launch_bounds__(kTileThreads, 2)
               break;
             }
             tc::tc_fence_after();
+            const uint32_t sums = tmem + lanes + (uint32_t)(C::kHCols + bt.slot * kChunk + half * 32);
             uint32_t v[32];
             __syncwarp();
-            tc::tmem_ld32(tmem + lanes + (uint32_t)(C::kHCols + bt.slot * kChunk + half * 32), v);
+            tc::tmem_ld32(sums, v);
+            const bool redo = mine >= 0 && !all_finite(v, p.N - c0);
+            if (__any_sync(kAll, redo)) {
+              add_own<T>(redo, static_cast<const T*>(p.b) + ((int64_t)adapter * p.N + c0) * p.rank, min(32, p.N - c0), p.rank, sH,
+                         tmem + lanes + C::kRestAt, (n * eights + 1) / 2, r, e0, wh,
+                         [=](int q, float k, float d) { out[c0 + q] = T(fmaf(k, d, to_f32(y[c0 + q]))); });
+              tc::tmem_ld32(sums, v);
+            }
             tc::tc_fence_before();
             mbar_arrive(smem_u32(&dempty[bt.slot]));
-            if (mine >= 0 && !all_finite(v, p.N - c0)) {
-              add_own<T>(static_cast<const T*>(p.b) + ((int64_t)adapter * p.N + c0) * p.rank, min(32, p.N - c0), p.rank, sH, r,
-                         mine * eights, w, [=](int q, float k, float d) { out[c0 + q] = T(fmaf(k, d, to_f32(y[c0 + q]))); });
-            } else if (mine >= 0) {
+            if (mine >= 0 && !redo) {
               uint32_t o[16];
 #pragma unroll
               for (int q = 0; q < 16; ++q) {
                 const float2 f = unpack2<T>(base[q]);
-                o[q] = pack2<T>(fmaf(w, __uint_as_float(v[2 * q]), f.x), fmaf(w, __uint_as_float(v[2 * q + 1]), f.y));
+                o[q] = pack2<T>(fmaf(wh, __uint_as_float(v[2 * q]), f.x), fmaf(wh, __uint_as_float(v[2 * q + 1]), f.y));
               }
 #pragma unroll
               for (int c = 0; c < 32; c += 16)

@@ -400,9 +400,11 @@ int rb_sandwich_norm_backward(const void* dy, int64_t ldy, const void* dz, int64
  *   workspace  rb_low_rank_workspace_size(T, K, N, rank) bytes (may be 0; -1: bad
  *              shape), 16-byte aligned
  * Sums are fp32.  Above 96 tokens, where rank and K are multiples of 8, rank <= 64
- * and x, a and b are on 16-byte rows, the products run on the tensor cores and
- * A_i x is rounded to the model type between them; up to 1024 tokens only if
- * T rank (K + N) is above 2^24.  Else A_i x stays fp32.  out is rounded once.
+ * and x, a and b are on 16-byte rows, the products run on the tensor cores; up to
+ * 1024 tokens only if T rank (K + N) is above 2^24.  A_i x goes from one to the
+ * other as two values of the model type there (off by 2^-18 of it in bf16, 2^-22 in
+ * fp16, where it may also be outside the type's range), else in fp32.  out is
+ * rounded once.
  * Forward only.
  */
 int64_t rb_low_rank_workspace_size(int64_t T, int K, int N, int rank);

@@ -256,3 +256,116 @@ def test_bank_streams_and_graphs(cuda_device):
         g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(h, got) for h in held)
+
+
+# tiles: fused (19k and more; one tile of one chunk), H and out apart (with and without a split of K)
+H_SHAPES = [
+    # T, K, N, rank, R, run
+    (60, 64, 128, 16, 5, 3),        # token by token
+    (1100, 64, 64, 16, 5, 40),
+    (1100, 64, 256, 8, 5, 40),
+    (1101, 640, 200, 24, 9, 7),
+    (1500, 1024, 264, 40, 7, 5),
+    (1300, 128, 520, 64, 4, 30),
+    (1026, 1000, 1544, 8, 24, 7),
+    (19500, 64, 136, 8, 20, 9),
+    (19500, 128, 72, 24, 9, 2),
+    (19501, 64, 101, 48, 5, 30),
+    (20000, 192, 128, 64, 3, 50),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T,K,N,rank,R,run", H_SHAPES)
+def test_h_keeps_more_bits_than_the_type(cuda_device, T, K, N, rank, R, run, dtype):
+    """One nonzero in a row of x: h is a product of two values of the type (16 or 22 bits, exact in fp32).  B passes h on and y
+    takes h's leading bits off, so what is left is the second half of h: exact in the type, and in every sum on the way."""
+    from baidu_cti_grab_b200 import device_ops
+
+    gen = torch.Generator().manual_seed(T + rank)
+    _, _, a, _, adapter, _ = _inputs(T, K, N, rank, R, dtype, run, T)
+    x = torch.zeros(T, K, dtype=dtype)
+    at = torch.randint(0, K, (T,), generator=gen)
+    # magnitudes of 4 to 8: the products' last bits are far above fp16's subnormals
+    def some(*shape):
+        sign = torch.randint(0, 2, shape, generator=gen) * 2.0 - 1.0
+        return (sign * (4 + 4 * torch.rand(*shape, generator=gen))).to(dtype)
+
+    x[torch.arange(T), at] = some(T)
+    a = some(R, rank, K)
+    b = torch.zeros(R, N, rank, dtype=dtype)
+    b[:, torch.arange(N), torch.arange(N) % rank] = torch.where(torch.arange(N) // rank % 2 == 0, 1.0, -1.0).to(dtype)
+    own = adapter.clamp(min=0)
+    h = a[own, :, at].double() * x.double().gather(1, at[:, None])
+    passed = (b[own[0]].double() @ h.t()).t()  # B is the same in every adapter
+    y = (-passed).to(dtype)
+    want = torch.where((adapter >= 0)[:, None], y.double() + passed, y.double())
+    assert torch.equal(want.to(dtype).double(), want)
+    got = device_ops.low_rank_add(*(t.to(cuda_device) for t in (y, x, a, b, adapter)))
+    assert torch.equal(got.double().cpu(), want)
+    assert device_ops.device_error() == 0
+
+
+def _check_close(got, y, x, a, b, adapter, scale):
+    """The bound above with h not rounded to the type, but held as two of its values: off by 2^-22 of it and, its row brought
+    to 2^14 .. 2^15 before, by the subnormals' half step 2^-25, 2^-39 of the row's largest.  Sums on the tensor cores may
+    truncate: a whole step 2^-23 an addition."""
+    dev = got.device
+    y, x, a, b, adapter, scale = (t.to(dev) for t in (y, x, a, b, adapter, scale))
+    rank, K = a.shape[1:]
+    fi = torch.finfo(y.dtype)
+    tiny = fi.smallest_normal * fi.eps / 2
+    for i in range(a.shape[0]):
+        t = (adapter == i).nonzero()[:, 0]
+        xi, ai, bi, s = x[t].double(), a[i].double(), b[i].double(), scale[i].double()
+        h = xi @ ai.t()
+        want = y[t].double() + s * (h @ bi.t())
+        off = 2.0 ** -22 * h.abs() + 2.0 ** -39 * h.abs().amax(-1, keepdim=True) + (K + rank) * 2.0 ** -23 * (xi.abs() @ ai.abs().t())
+        limit = 1.01 * s.abs() * (off @ bi.abs().t()) + 2.0 ** -23 * y[t].double().abs() + fi.eps / 2 * want.abs() + tiny
+        over = (got[t].double() - want).abs() - limit
+        assert bool((over <= 0).all()), (i, float(over.max()), int((over > 0).sum()), int((~got[t].isfinite()).sum()))
+
+
+@pytest.mark.parametrize("grow,scale", [(4000.0, 1e-6), (2.0 ** -14, 1000.0)])
+@pytest.mark.parametrize("T,K,N,rank,R,run", H_SHAPES)
+def test_fp16_h_outside_the_type(cuda_device, T, K, N, rank, R, run, grow, scale):
+    """h above fp16's 65504 or among its subnormals, under an adapter scale that brings the sum back."""
+    from baidu_cti_grab_b200 import device_ops
+
+    y, x, a, b, adapter, _ = _inputs(T, K, N, rank, R, HF, run, T + 1)
+    x = (x.float().clamp(-4, 4) * grow).to(HF)
+    if grow > 1:
+        a = (a.float() * 100).to(HF)
+        assert float((x.float() @ a[0].float().t()).abs().max()) > 2e5
+    else:
+        a = (a.float() * 2.0 ** -7).to(HF)
+        y.zero_()
+        assert float((x.float() @ a[0].float().t()).abs().max()) < 2e-5
+    s = torch.full((R,), scale)
+    args = tuple(t.to(cuda_device) for t in (y, x, a, b, adapter, s))
+    got = device_ops.low_rank_add(*args)
+    _check_close(got, *args)
+    place = args[0].clone()
+    device_ops.low_rank_add(place, *args[1:], out=place)
+    assert torch.equal(place, got)
+
+
+@pytest.mark.parametrize("T", [1500, 20000])
+def test_infinite_own_b_under_an_exact_h(cuda_device, T):
+    """h without a second half (powers of two): an infinity in the token's own B times that zero is no NaN in the result."""
+    from baidu_cti_grab_b200 import device_ops
+
+    for dtype in (BF, HF):
+        y, x, a, b, adapter, scale = _inputs(T, 64, 200, 16, 6, dtype, 12, T)
+        x.zero_()
+        x[:, 5] = 2.0
+        a = torch.where(a < 0, -0.5, 0.5).to(dtype)
+        b[4, ::3, 2] = float("inf")
+        args = tuple(t.to(cuda_device) for t in (y, x, a, b, adapter, scale))
+        got = device_ops.low_rank_add(*args)
+        rows = args[4] == 4
+        sign = torch.sign(args[2][4, 2, 5].float())
+        assert bool((got[rows][:, ::3].float() == sign * float("inf")).all())
+        keep = torch.ones(200, dtype=torch.bool, device=cuda_device)
+        keep[::3] = False
+        assert bool(got[rows][:, keep].isfinite().all()) and bool(got[~rows].isfinite().all())
