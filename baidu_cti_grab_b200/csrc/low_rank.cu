@@ -775,7 +775,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         const int first = g * group, n = min(group, count - first);
         const int mine = slot >= first && slot < first + n ? slot - first : -1;
         if constexpr (MODE != kOutOnly) {
-          ok = ok && mbar_wait_bounded(smem_u32(&hfull), hparity, kWaitTimeoutEpilogue, abort_flag);
+          // a warp gives up on a wait as one, here and below: its lanes wait for each other before they load from TMEM
+          ok = __all_sync(kAll, ok && mbar_wait_bounded(smem_u32(&hfull), hparity, kWaitTimeoutEpilogue, abort_flag));
           tc::tc_fence_after();
           ring.skip(kb1 - kb0);
         }
@@ -967,10 +968,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
               for (int c = 0; c < 32; c += 16)
                 if (c0 + c < p.N) load16(y, c0 + c, p.N, p.vec_y, base + c / 2);
             }
-            if (!mbar_wait_bounded(smem_u32(&dfull[bt.slot]), bt.parity, kWaitTimeoutEpilogue, abort_flag)) {
-              ok = false;
-              break;
-            }
+            ok = __all_sync(kAll, ok && mbar_wait_bounded(smem_u32(&dfull[bt.slot]), bt.parity, kWaitTimeoutEpilogue, abort_flag));
+            if (!ok) break;
             tc::tc_fence_after();
             const uint32_t sums = tmem + lanes + (uint32_t)(C::kHCols + bt.slot * kChunk + half * 32);
             uint32_t v[32];
