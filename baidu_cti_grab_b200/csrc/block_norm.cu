@@ -104,11 +104,11 @@ __device__ __forceinline__ void narrow(const float* v, Eight<float>& e) {
                         __float_as_uint(v[4 * i + 3]));
 }
 
-// eight parameters from column c (0 beyond D), or `none` where there are none
+// eight parameters from column c, or `none` where there are none; 0 beyond D in either case
 __device__ __forceinline__ void param8(const void* p, int dtype, int c, int D, float none, float* v) {
   if (p == nullptr) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = none;
+    for (int i = 0; i < 8; ++i) v[i] = c + i < D ? none : 0.0f;
     return;
   }
   const int size = dtype == RB_F32 ? 4 : 2;

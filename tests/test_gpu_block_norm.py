@@ -307,3 +307,27 @@ def test_autograd_module_streams_and_graphs(cuda_device):
         for p, q, s, e in zip(want, other, held, held2):
             assert p is None or (torch.equal(p, q) and torch.equal(p, s) and torch.equal(p, e))
     assert device_ops.device_error() == 0
+
+
+AFFINE = ("post_weight", "post_bias", "pre_weight", "pre_bias")
+
+
+@pytest.mark.parametrize("absent", [AFFINE[:1], AFFINE[1:2], AFFINE[2:3], AFFINE[3:], (AFFINE[0], AFFINE[2]), AFFINE],
+                         ids="+".join)
+@pytest.mark.parametrize("D,dtype", [(7, HF), (100, BF), (512, HF), (520, BF), (768, FP), (1023, HF), (5000, BF), (5121, FP),
+                                     (5128, BF), (7208, FP)])
+@pytest.mark.parametrize("gate,act", [("row", "none"), ("channel", "sigmoid"), ("full", "sigmoid"), (None, "none")])
+def test_without_weights_or_biases(cuda_device, monkeypatch, D, dtype, gate, act, absent):
+    """Each of the norms' weights and biases left out, on widths that fill their team of threads and that do not."""
+    whole = _inputs
+
+    def fewer(*args):
+        t, gy, gz = whole(*args)
+        t.update(dict.fromkeys(absent))
+        return t, gy, gz
+
+    monkeypatch.setitem(globals(), "_inputs", fewer)
+    test_forward_and_gradients_against_float64(cuda_device, 37, D, dtype, dtype, "layer", "layer", gate, act, 0.7)
+    if gate is None:
+        test_forward_and_gradients_against_float64(cuda_device, 37, D, dtype, dtype, "rms", "layer", gate, act, 0.7)
+        test_forward_and_gradients_against_float64(cuda_device, 37, D, dtype, dtype, "layer", "rms", gate, act, 0.7)
