@@ -62,9 +62,9 @@ class AdapterBank(nn.Module):
         who = nn.functional.pad(request_adapter.to(torch.int32), (0, 1), value=-1)[request]
         return who.masked_fill_(token < offsets[0], -1)
 
-    @torch.no_grad()
     def forward(self, y: torch.Tensor, x: torch.Tensor, adapter: torch.Tensor, out: Optional[torch.Tensor] = None):
-        """y [..., N] plus each token's adapter of x [..., K]; adapter int32/int64 of the leading shape."""
+        """y [..., N] plus each token's adapter of x [..., K]; adapter int32/int64 of the leading shape.
+        No backward: with gradients enabled, tensors that ask for one are refused (call it under torch.no_grad())."""
         lead, N, K = y.shape[:-1], y.shape[-1], x.shape[-1]
         if out is not None and out.dim() != 2 and not out.is_contiguous():
             raise ValueError("out must be contiguous, or 2-D with contiguous rows")

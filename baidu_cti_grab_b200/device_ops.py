@@ -798,7 +798,8 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     if not a.is_contiguous() or not b.is_contiguous():
         raise ValueError("a and b must be contiguous")
     if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad
-                                    or (scale is not None and scale.requires_grad)):
+                                    or (scale is not None and scale.requires_grad)
+                                    or (out is not None and out.requires_grad)):
         raise RuntimeError("low_rank_add has no backward: call it under torch.no_grad() or on detached tensors")
     given = out is not None
     if not given:

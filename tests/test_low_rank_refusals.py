@@ -87,3 +87,27 @@ def test_overlapping_rows_are_seen():
         both[said] += 1
         assert said == shared or (said and lda != ldb and T > 1)
     assert min(both) > 100
+
+
+@pytest.mark.parametrize("which", ["y", "x", "out", "a"])
+def test_inputs_that_ask_for_a_gradient_are_refused(monkeypatch, which):
+    """The kernels have no backward: the module refuses what device_ops refuses, and neither drops a gradient."""
+    from baidu_cti_grab_b200 import adapters, device_ops
+
+    calls = []
+    monkeypatch.setattr(device_ops, "_device_of", lambda name, first, *others: first.device)
+    monkeypatch.setattr(device_ops, "_plan_bytes", lambda *args: 0)
+    monkeypatch.setattr(device_ops, "_call_on", lambda dev, name, *args: calls.append(name))
+    t = {k: torch.zeros(4, 8, dtype=torch.bfloat16) for k in ("y", "x", "out")}
+    bank = adapters.AdapterBank(*(torch.zeros(2, 8, 8, dtype=torch.bfloat16) for _ in range(2)))
+    who = torch.zeros(4, dtype=torch.int32)
+    bank(t["y"], t["x"], who, out=t["out"])
+    assert calls == ["rb_low_rank_add"]
+    (bank.a if which == "a" else t[which]).requires_grad_()
+    for call in (lambda: bank(t["y"], t["x"], who, out=t["out"]),
+                 lambda: device_ops.low_rank_add(t["y"], t["x"], bank.a, bank.b, who, bank.scale, out=t["out"])):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+    assert calls == ["rb_low_rank_add"]
+    with torch.no_grad():
+        assert bank(t["y"], t["x"], who, out=t["out"]) is t["out"]
