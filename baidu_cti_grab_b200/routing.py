@@ -98,7 +98,7 @@ class TopKRouter(nn.Module):
         """(idx [..., k], score [..., k], probs [..., E]) of x [..., d_model], as the reference's gate."""
         r = self.route(x)
         lead = x.shape[:-1]
-        return r.idx.view(*lead, -1), r.score.view(*lead, -1), r.probs.view(*lead, -1)
+        return r.idx.view(*lead, self.k), r.score.view(*lead, self.k), r.probs.view(*lead, r.probs.shape[-1])
 
     @torch.no_grad()
     def update_balance(self, counts: torch.Tensor, step: float = 1e-3) -> None:

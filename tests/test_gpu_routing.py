@@ -314,3 +314,15 @@ def test_streams_graphs_and_repeats(cuda_device):
     graph.replay()
     now = device_ops.route_topk(fresh, 4, bias=bias, want_counts=True)
     assert torch.equal(held[0], now[0]) and torch.equal(held[3], now[3])
+
+
+@pytest.mark.parametrize("lead", [(0,), (0, 5), (3, 0)])
+def test_empty_batch_through_the_router(cuda_device, lead):
+    from baidu_cti_grab_b200 import routing
+
+    gate = routing.TopKRouter(16, 8, 2, renormalize=True).to(cuda_device)
+    x = torch.zeros(*lead, 16, device=cuda_device, requires_grad=True)
+    idx, score, probs = gate(x)
+    assert idx.shape == score.shape == (*lead, 2) and probs.shape == (*lead, 8)
+    (score.sum() + probs.sum()).backward()
+    assert x.grad.shape == x.shape and bool((gate.w_g.weight.grad == 0).all())

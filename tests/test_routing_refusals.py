@@ -55,3 +55,17 @@ def test_cpu_tensors_are_refused():
         device_ops.route_topk_backward(torch.zeros(3, 8), torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2))
     with pytest.raises(ValueError):
         routing.TopKRouter(16, 8, 2).update_balance(torch.zeros(8))
+
+
+@pytest.mark.parametrize("lead", [(0,), (0, 5), (3, 0), (2, 4), ()])
+def test_router_keeps_the_leading_shape(monkeypatch, lead):
+    """An empty batch too: its shapes do not follow from the number of values."""
+    from baidu_cti_grab_b200 import routing
+
+    def choose(logits, k, **_):
+        T, E = logits.shape
+        return routing.Routing(torch.zeros(T, k, dtype=torch.int64), torch.zeros(T, k), torch.zeros(T, E), None)
+
+    monkeypatch.setattr(routing, "route_topk", choose)
+    idx, score, probs = routing.TopKRouter(16, 8, 2)(torch.zeros(*lead, 16))
+    assert idx.shape == score.shape == (*lead, 2) and probs.shape == (*lead, 8)
