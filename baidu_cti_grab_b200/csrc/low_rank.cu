@@ -1203,7 +1203,8 @@ extern "C" int rb_low_rank_add(const void* y, int64_t ldy, const void* x, int64_
   p.unit = rank % 64 == 0 ? 64 : rank % 32 == 0 ? 32 : rank % 16 == 0 ? 16 : 8;
   p.vec_y = vec_bytes(y, ldy);
   p.vec_out = vec_bytes(out, ldo);
-  p.chunk_io = p.vec_y >= 16 && p.vec_out >= 16;
+  // (a chunk's store goes by whole 16 bytes: with N off 8 it would write up to seven columns behind a row)
+  p.chunk_io = p.vec_y >= 16 && p.vec_out >= 16 && N % 8 == 0;
   cudaStream_t st = (cudaStream_t)stream;
   if (q.tiles == 0)
     return dtype == RB_BF16 ? run_tokens<__nv_bfloat16>(p, fit, st) : run_tokens<__half>(p, fit, st);

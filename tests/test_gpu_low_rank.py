@@ -369,3 +369,22 @@ def test_infinite_own_b_under_an_exact_h(cuda_device, T):
         keep = torch.ones(200, dtype=torch.bool, device=cuda_device)
         keep[::3] = False
         assert bool(got[rows][:, keep].isfinite().all()) and bool(got[~rows].isfinite().all())
+
+
+@pytest.mark.parametrize("T,K", [(60, 64), (1100, 64), (1500, 640), (20000, 64)])
+@pytest.mark.parametrize("N", [1, 7, 97, 101, 127])
+def test_odd_widths_in_padded_rows(cuda_device, T, K, N):
+    """Rows on 16 bytes whose last columns are no whole 16 bytes: what follows them is neither read into them nor written."""
+    from baidu_cti_grab_b200 import device_ops
+
+    args = _inputs(T, K, N, 16, 6, BF, 12, N)
+    y, x, a, b, adapter, scale = (t.to(cuda_device) for t in args)
+    ld = (N + 8) // 8 * 8
+    ry, ro = (torch.full((T, ld), v, dtype=BF, device=cuda_device) for v in (float("nan"), 7.0))
+    ry[:, :N].copy_(y)
+    device_ops.low_rank_add(ry[:, :N], x, a, b, adapter, scale, out=ro[:, :N])
+    _check(ro[:, :N], *args)
+    assert bool((ro[:, N:] == 7.0).all())
+    ry[:, N:] = 7.0
+    device_ops.low_rank_add(ry[:, :N], x, a, b, adapter, scale, out=ry[:, :N])
+    assert torch.equal(ry, ro)
