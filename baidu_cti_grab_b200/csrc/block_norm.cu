@@ -161,23 +161,24 @@ __device__ __forceinline__ float total(F2 v) {
 // thread's columns stay its own for all rows, so they are made once and held in registers; where a thread has too few
 // of those (backward, wider than 5120) in shared memory as fp32, and where that is full too they are made for each row.
 enum Where : int { kRegisters = 0, kTable = 1, kAgain = 2 };
+template <typename T>
 __device__ __forceinline__ float gate_act(float g, int act);
-template <int WHICH>
+template <int WHICH, typename T>
 __device__ __forceinline__ void make_column8(const Params& p, int c, float* v) {
   if constexpr (WHICH < 2) {
     param8(WHICH == 0 ? p.w1 : p.b1, p.w1_dtype, c, p.D, WHICH == 0 ? 1.0f : 0.0f, v);
     float g[8];
     if (p.gate_kind == kGateChannel) param8(p.gate, p.gate_dtype, c, p.D, 1.0f, g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= p.gate_kind == kGateChannel ? p.scale * gate_act(g[i], p.act) : p.scale;
+    for (int i = 0; i < 8; ++i) v[i] *= p.gate_kind == kGateChannel ? p.scale * gate_act<T>(g[i], p.act) : p.scale;
   } else {
     param8(WHICH == 2 ? p.w2 : p.b2, p.w2_dtype, c, p.D, WHICH == 2 ? 1.0f : 0.0f, v);
   }
 }
-template <int WHICH>
+template <int WHICH, typename T>
 __device__ __forceinline__ void column8(const Params& p, int c, F2* v) {
   float f[8];
-  make_column8<WHICH>(p, c, f);
+  make_column8<WHICH, T>(p, c, f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
 }
@@ -195,17 +196,28 @@ __device__ __forceinline__ void table8(uint32_t at, F2* v) {
   v[3] = f2(__uint_as_float(b.z), __uint_as_float(b.w));
 }
 // the table [3][pitch] of A, B and the pre norm's w, by all threads of the CTA
+template <typename T>
 __device__ __forceinline__ void fill_table(const Params& p, float* table, int pitch) {
   for (int c = threadIdx.x * 8; c < pitch; c += blockDim.x * 8) {
-    make_column8<0>(p, c, table + c);
-    make_column8<1>(p, c, table + pitch + c);
-    make_column8<2>(p, c, table + 2 * pitch + c);
+    make_column8<0, T>(p, c, table + c);
+    make_column8<1, T>(p, c, table + pitch + c);
+    make_column8<2, T>(p, c, table + 2 * pitch + c);
   }
 }
 
-// the sigmoid is off by a few units of 2^-24 (and |g| of them where it is small itself)
+// A sigmoid and its derivative, off by a few units of 2^-24 of themselves: from exp(-|g|), since 1 - a near a = 1 and
+// exp(-g) of a large -g would lose those bits.
+__device__ __forceinline__ float2 sigmoid_of(float g) {
+  const float e = expf(-fabsf(g)), r = __fdividef(1.0f, 1.0f + e), low = e * r;
+  return make_float2(g < 0.0f ? low : r, low * r);
+}
+// What a gate does to rows of type T.  16-bit rows: by the fast exponential and quotient, off by |g| units of 2^-23 where the
+// sigmoid is small, far below the rows' rounding to 2^-9 or 2^-11 (the exact form took 0.6 us more for a single row, most
+// of it instructions to fetch, and 2 of 96 us at 24490 x 512).
+template <typename T>
 __device__ __forceinline__ float gate_act(float g, int act) {
-  return act == kActSigmoid ? __fdividef(1.0f, 1.0f + __expf(-g)) : g;
+  if constexpr (sizeof(T) == 4) return act == kActSigmoid ? sigmoid_of(g).x : g;
+  else return act == kActSigmoid ? __fdividef(1.0f, 1.0f + __expf(-g)) : g;
 }
 
 // A team of G threads on a row of up to 8 V G values; thread r of the team holds the eights r, r + G, ...
@@ -474,10 +486,10 @@ __global__ void __launch_bounds__(Team<G>::kThreads, G == 320 ? 2 : 512 / Team<G
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     const int c = (k * G + r) * 8;
-    column8<0>(p, c, A + 4 * k);
-    column8<1>(p, c, B + 4 * k);
-    column8<2>(p, c, w2 + 4 * k);
-    column8<3>(p, c, b2 + 4 * k);
+    column8<0, T>(p, c, A + 4 * k);
+    column8<1, T>(p, c, B + 4 * k);
+    column8<2, T>(p, c, w2 + 4 * k);
+    column8<3, T>(p, c, b2 + 4 * k);
   }
 
   int stage = 0, turn = 0;
@@ -485,7 +497,7 @@ __global__ void __launch_bounds__(Team<G>::kThreads, G == 320 ? 2 : 512 / Team<G
   float next_gate = 1.0f;
   auto ahead = [&](int64_t row) {
     if (p.gate_kind == kGateRow && row < p.N)
-      next_gate = gate_act(load_as_f32(p.gate, p.gate_dtype, row * p.ldg), p.act);
+      next_gate = gate_act<T>(load_as_f32(p.gate, p.gate_dtype, row * p.ldg), p.act);
   };
   ahead(rows.first);
   for (int64_t row = rows.first; row < p.N; row += rows.step) {
@@ -509,7 +521,7 @@ __global__ void __launch_bounds__(Team<G>::kThreads, G == 320 ? 2 : 512 / Team<G
         float g[8];
         widen(e[2][k], g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = f2(gate_act(g[2 * i], p.act), gate_act(g[2 * i + 1], p.act));
+        for (int i = 0; i < 4; ++i) a[i] = f2(gate_act<T>(g[2 * i], p.act), gate_act<T>(g[2 * i + 1], p.act));
       }
 #pragma unroll
       for (int i = 4 * k; i < 4 * k + 4; ++i) y[i] = fma2(a[i & 3], fma2(n[i], A[i], B[i]), x[i & 3]);
@@ -558,7 +570,7 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
   F2 A[4], B[4], w2[4];
   uint32_t table = 0;
   if constexpr (WHERE == kTable) {
-    fill_table(p, reinterpret_cast<float*>(ring + p.table_at), pitch);
+    fill_table<T>(p, reinterpret_cast<float*>(ring + p.table_at), pitch);
     __syncthreads();
     table = smem_u32(ring + p.table_at) + (c < p.D ? 4 * c : 0);  // a thread beyond D: any columns, its x, h, dy and dz are 0
   }
@@ -572,9 +584,9 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
         for (int i = 0; i < 4; ++i) A[i] = B[i] = w2[i] = f2(0.0f, 0.0f);
       }
     } else {
-      column8<0>(p, c, A);
-      column8<1>(p, c, B);
-      if (pre) column8<2>(p, c, w2);
+      column8<0, T>(p, c, A);
+      column8<1, T>(p, c, B);
+      if (pre) column8<2, T>(p, c, w2);
     }
   };
   if constexpr (WHERE == kRegisters) columns(true);
@@ -595,7 +607,7 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
   auto ahead = [&](int64_t row) {  // the next row's scalars
     if (row < p.N) {
       st = __ldg(reinterpret_cast<const float4*>(p.stats) + row);
-      if (!FULL && p.gate_kind == kGateRow) g_row = gate_act(load_as_f32(p.gate, p.gate_dtype, row * p.ldg), p.act);
+      if (!FULL && p.gate_kind == kGateRow) g_row = gate_act<T>(load_as_f32(p.gate, p.gate_dtype, row * p.ldg), p.act);
     }
   };
   ahead(rows.first);
@@ -614,7 +626,7 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
       float g[8];
       widen(e[4][0], g);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = f2(gate_act(g[2 * i], p.act), gate_act(g[2 * i + 1], p.act));
+      for (int i = 0; i < 4; ++i) a[i] = f2(gate_act<T>(g[2 * i], p.act), gate_act<T>(g[2 * i + 1], p.act));
     } else {
       a[0] = f2(ar, ar);
     }
@@ -661,7 +673,17 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
       for (int i = 0; i < 4; ++i) {
         const F2 ai = a[FULL ? i : 0];
         F2 da = mul2(fma2(hh[i], A[i], B[i]), t[i]);
-        if (p.act == kActSigmoid) da = mul2(da, fma2(mul2(ai, f2(-1.0f, -1.0f)), ai, ai));
+        if constexpr (FULL) {
+          if (p.act == kActSigmoid) {
+            if constexpr (sizeof(T) == 4) {
+              float g[8];
+              widen(e[4][0], g);
+              da = mul2(da, f2(sigmoid_of(g[2 * i]).y, sigmoid_of(g[2 * i + 1]).y));
+            } else {
+              da = mul2(da, fma2(mul2(ai, f2(-1.0f, -1.0f)), ai, ai));
+            }
+          }
+        }
         yh[i] = da;  // of every element: its gradient
         s5 = add2(s5, da);
       }
@@ -683,7 +705,8 @@ __global__ void __launch_bounds__(Team<G>::kThreads, Team<G>::kThreads <= 512 ? 
       if constexpr (!FULL) s345[2] = total(s5);
       Tm::sum(s345, room, turn);
       if (!FULL && p.gate_kind == kGateRow && r == 0) {
-        const float d = s345[FULL ? 0 : 2];
+        float d = s345[FULL ? 0 : 2];
+        if (p.act == kActSigmoid) d *= sigmoid_of(load_as_f32(p.gate, p.gate_dtype, row * p.ldg)).y;
         if (p.gate_dtype == RB_F32) static_cast<float*>(p.out2)[row] = d;
         else if (p.gate_dtype == RB_BF16) static_cast<__nv_bfloat16*>(p.out2)[row] = __float2bfloat16_rn(d);
         else static_cast<__half*>(p.out2)[row] = __float2half_rn(d);
@@ -775,12 +798,12 @@ __global__ void __launch_bounds__(8 * kSumRuns) column_sums_kernel(const __grid_
   const float P = part[0][0][at], dw = part[1][0][at], Q = part[2][0][at], db = part[3][0][at];
   float k = p.scale;
   if (p.gate_kind == kGateChannel) {
-    const float g = load_as_f32(p.gate, p.gate_dtype, c), a = gate_act(g, p.act);
+    const float g = load_as_f32(p.gate, p.gate_dtype, c);
     const float w = p.w1 != nullptr ? load_as_f32(p.w1, p.w1_dtype, c) : 1.0f;
     const float b = p.b1 != nullptr ? load_as_f32(p.b1, p.w1_dtype, c) : 0.0f;
-    const float d = p.act == kActSigmoid ? a * (1.0f - a) : 1.0f;
-    store_param(o.dgate, p.gate_dtype, c, p.scale * d * fmaf(w, P, b * Q));
-    k *= a;
+    const float2 a = p.act == kActSigmoid ? sigmoid_of(g) : make_float2(g, 1.0f);
+    store_param(o.dgate, p.gate_dtype, c, p.scale * a.y * fmaf(w, P, b * Q));
+    k *= a.x;
   }
   store_param(o.dw1, p.w1_dtype, c, k * P);
   store_param(o.db1, p.w1_dtype, c, k * Q);

@@ -331,3 +331,38 @@ def test_without_weights_or_biases(cuda_device, monkeypatch, D, dtype, gate, act
     if gate is None:
         test_forward_and_gradients_against_float64(cuda_device, 37, D, dtype, dtype, "rms", "layer", gate, act, 0.7)
         test_forward_and_gradients_against_float64(cuda_device, 37, D, dtype, dtype, "layer", "rms", gate, act, 0.7)
+
+
+@pytest.mark.parametrize("gate,dtype", [("full", FP), ("row", FP), ("row", BF), ("channel", FP), ("channel", HF)])
+def test_saturated_sigmoid_gates(cuda_device, gate, dtype):
+    """Gates of -60 to 60 in fp32: the sigmoid and its derivative keep their own precision where they are small (y = a h without a
+    residual or norms; one element of h is not 0 in each sum).  exp's argument is exact, exp within 2 units of 2^-23, the sum,
+    quotient and up to four products half a unit each: under 2^-20 of the value.  16-bit rows are gated by the fast exponential,
+    off by 2 + 1.2 |g| units of 2^-23, 74 at 60: under 2^-16.  y and dh take half a step of the rows' type on top."""
+    from baidu_cti_grab_b200 import device_ops
+
+    N, D = (200, 40) if gate != "channel" else (40, 200)
+    gen = torch.Generator().manual_seed(5)
+    g = (torch.rand(N, D, generator=gen) - 0.5) * 120
+    one = torch.zeros(N, D)
+    one[torch.arange(N), torch.arange(N) % D] = 1.0
+    if gate == "channel":
+        one = torch.zeros(N, D)
+        one[torch.arange(D) % N, torch.arange(D)] = 1.0
+    g = {"full": g, "row": g[:, :1].contiguous(), "channel": g[0].contiguous()}[gate]
+    g.view(-1)[:5] = torch.tensor([0.0, -0.0, 20.0, -20.0, 60.0])
+    h = (torch.randn(N, D, generator=gen) * (1.0 if gate == "full" else one)).to(dtype)
+    gy = torch.randn(N, D, generator=gen).to(dtype)
+    x = torch.zeros(N, D, dtype=dtype)
+    a = 1.0 / (1.0 + torch.exp(-g.double()))
+    d = a * (1.0 / (1.0 + torch.exp(g.double())))
+    dev = {k: v.to(cuda_device) for k, v in dict(x=x, h=h, gate=g, gy=gy).items()}
+    y, _, stats = device_ops.sandwich_norm(dev["x"], dev["h"], gate=dev["gate"], gate_act="sigmoid", want_stats=True)
+    _, dh, dg, *_ = device_ops.sandwich_norm_backward(dev["gy"], None, dev["x"], dev["h"], stats, gate=dev["gate"],
+                                                      gate_act="sigmoid")
+    rows = 2.0 ** -20 if dtype == FP else 2.0 ** -16
+    _check(y, a * h.double(), dtype, rows * (a * h.double()).abs(), "y")
+    _check(dh, a * gy.double(), dtype, rows * (a * gy.double()).abs(), "dh")
+    want = d * h.double() * gy.double()
+    want = {"full": want, "row": want.sum(-1, keepdim=True), "channel": want.sum(0)}[gate]
+    _check(dg, want, FP, 2.0 ** -20 * want.abs(), "dgate")
