@@ -713,7 +713,10 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const __grid_c
   }
   if (p.kind == kSigmoid) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = ds[i] * s[i] * (1.0f - s[i]);
+    for (int i = 0; i < V; ++i) {
+      const float e = expf(-fabsf(l[i])), q = __fdividef(e, 1.0f + e);  // the smaller of s and 1 - s, to its own last bits
+      s[i] = ds[i] * q * (1.0f - q);
+    }
   } else {
     float dot = 0.0f;
 #pragma unroll

@@ -326,3 +326,20 @@ def test_empty_batch_through_the_router(cuda_device, lead):
     assert idx.shape == score.shape == (*lead, 2) and probs.shape == (*lead, 8)
     (score.sum() + probs.sum()).backward()
     assert x.grad.shape == x.shape and bool((gate.w_g.weight.grad == 0).all())
+
+
+@pytest.mark.parametrize("E", [8, 100, 300])
+def test_gradients_of_saturated_sigmoids(cuda_device, E):
+    """s (1 - s) of logits from -60 to 60: exp within 2 units of 2^-23, the sum, quotient, difference and products half a unit or
+    (the quotient) two each: under 2^-20 of the value, not of s."""
+    from baidu_cti_grab_b200 import device_ops
+
+    gen = torch.Generator().manual_seed(E)
+    logits = (torch.rand(70, E, generator=gen) - 0.5) * 120
+    logits[0, :4] = torch.tensor([0.0, 17.5, 40.0, -40.0])
+    gp = torch.randn(70, E, generator=gen)
+    idx = torch.zeros(70, 1, dtype=torch.int64)
+    grad = device_ops.route_topk_backward(logits.to(cuda_device), idx.to(cuda_device), None, gp.to(cuda_device), score="sigmoid")
+    l = logits.double()
+    want = gp.double() / (1.0 + torch.exp(-l)) / (1.0 + torch.exp(l))
+    assert bool(((grad.cpu().double() - want).abs() <= (2.0 ** -20 + 2.0 ** -24) * want.abs()).all())
