@@ -388,3 +388,44 @@ def test_odd_widths_in_padded_rows(cuda_device, T, K, N):
     ry[:, N:] = 7.0
     device_ops.low_rank_add(ry[:, :N], x, a, b, adapter, scale, out=ry[:, :N])
     assert torch.equal(ry, ro)
+
+
+@pytest.mark.parametrize("shapes", [((1500, 640), (12000, 512)), ((20000, 128), (1500, 640))])
+def test_tiles_on_two_streams_and_in_graphs(cuda_device, shapes):
+    """Two calls at once, each in one kernel or in two of which the second starts early, eager and replayed in any order."""
+    from baidu_cti_grab_b200 import device_ops
+
+    sets = [[t.to(cuda_device) for t in _inputs(T, K, 200, 16, 6, BF, 12, T)] for T, K in shapes]
+    want = [device_ops.low_rank_add(*s) for s in sets]
+    for s, w in zip(sets, want):
+        _check(w, *s)
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(device_ops.low_rank_add(*sets[i]))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in (0, 1) for g in got[i])
+    graphs, held = [torch.cuda.CUDAGraph() for _ in sets], []
+    for g, s in zip(graphs, sets):
+        with torch.cuda.graph(g):
+            # the second call reads what the first wrote
+            one = device_ops.low_rank_add(*s)
+            held.append((one, device_ops.low_rank_add(one, *s[1:])))
+    twice = [device_ops.low_rank_add(w, *s[1:]) for w, s in zip(want, sets)]
+    for order in ((0, 1), (1, 0), (0, 1)):
+        for t in held:
+            t[0].zero_(), t[1].zero_()
+        torch.cuda.synchronize()
+        for i in order:
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in order:
+            assert torch.equal(held[i][0], want[i]) and torch.equal(held[i][1], twice[i])
+    assert device_ops.device_error() == 0
