@@ -24,7 +24,7 @@
 //
 // Measured on a B200 (6.55 TB/s copy): forward 103725 x 512 bf16, layer norms, channel gate 85 us (0.76 of HBM); both
 // directions 24490 x 512 fp16 with a sigmoid gate of every element 96 us (forward 29, backward 60, sums 5; floor 38), 4099 x
-// 5000 bf16 RMS 156 us (57, 100, 8; floor 50).  Backward is bound by instructions and the two dependent row sums: 1210
+// 5000 bf16 RMS 154 us (57, 97, 8; floor 50).  Backward is bound by instructions and the two dependent row sums: 1210
 // warp instructions a row at 512, issue slots half used at the 16 warps of an SM that its registers allow; wide rows
 // leave one row an SM.  Bounds of single values (rows that are no multiple of 8 wide) in the same loops took 1620 and
 // 131 us; five column sums instead of four and one thread asking for all copies 199 us.
@@ -158,8 +158,10 @@ __device__ __forceinline__ float total(F2 v) {
 
 // What a column's constants come to: out of the post norm, y = x + a (A v^ + B) with A = scale a_c w, B = scale a_c b,
 // a_c the channel's gate (1 without one) and a the row's or element's; the pre norm's w and b; zeros beyond D.  A
-// thread's columns stay its own for all rows, so they are made once and held in registers; where a thread has too few
-// of those (backward, wider than 5120) in shared memory as fp32, and where that is full too they are made for each row.
+// thread's columns stay its own for all rows, so they are made once and kept as variables (registers up to 4096 columns of 16
+// bits; of the 320-thread forward and 640-thread backward forms above, and of fp32 rows, a part is spilled); where a thread
+// has too few registers for them (backward, wider than 5120) they lie in shared memory as fp32, and where that is full too
+// they are made for each row.
 enum Where : int { kRegisters = 0, kTable = 1, kAgain = 2 };
 template <typename T>
 __device__ __forceinline__ float gate_act(float g, int act);
@@ -833,7 +835,9 @@ static Shape shape_of(int team, int arrays, int D, int elt, int64_t budget, int 
   return s;
 }
 
-// eight values a thread
+// Eight values a thread.  640 threads from 4097 to 5120 columns: with 1024 the constants no longer fit the registers.
+// Backward, 20 M bf16 values, layer norms and RMS without biases, 640 / 1024 threads: 4104 wide 163 and 107 / 308 and 204 us,
+// 4608 148 and 101 / 288 and 192, 5120 139 and 95 / 263 and 175.
 static int team_of(int D) {
   for (int team : {32, 64, 128, 256, 512, 640})
     if (D <= 8 * team) return team;
@@ -877,8 +881,9 @@ static int forward(Params& p, cudaStream_t st) {
   // Sixteen values a thread: a row's fixed instructions (copies, waits, sums) fall to half the warps, and two rows
   // fit an SM where eight values leave room for one (50 M bf16 values on a B200, layer norms, sixteen against eight a
   // thread when it was chosen: 512 wide 94 / 146 us, 1024 119 / 151, 2048 119 / 174, 4096 133 / 185, 8192 145 / 195).
-  // Teams of 320 just above 4096: two rows an SM, where 512 threads would be used to two thirds (5000 wide: 146 us,
-  // 186 with 640 threads of eight, 229 with 512 of sixteen).
+  // Teams of 320 just above 4096: two rows an SM, where 512 threads of sixteen would be used to half or two thirds.  20 M
+  // bf16 values, layer norms and RMS, 320 / 512 threads: 4104 wide 78.9 and 62.5 / 93.9 and 70.8 us, 4608 71.1 and 57.6 /
+  // 84.8 and 64.1, 5120 65.8 and 54.4 / 78.0 and 58.8.
   const bool two = p.D > 256;
   const int team = !two ? 32 : p.D <= 4096 ? team_of((p.D + 1) / 2) : p.D <= 5120 ? 320 : 512;
   const Shape s = shape_of(team, 3, p.D, (int)sizeof(T), ring_budget(team, team == 320 ? 640 : kForwardThreads), 0);

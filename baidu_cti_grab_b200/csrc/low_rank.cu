@@ -23,17 +23,18 @@
 // two GEMMs being 2 r (K + N) operations a token.  Sums are fp32.  The second product
 // takes h in two values of the model type (16 or 22 bits; fp16 rows are brought into
 // the type's range first), the second of them from TMEM: the MMAs are twice as many
-// and cost nothing that was measured, splitting and storing h costs 3-6 % (103725 x
-// 512 83 -> 85.5 us, 4099 x 14336 48 -> 51, 9001 x 1000 50 -> 52.5).  With h rounded
+// and cost nothing that was measured, splitting and storing h costs 2-5 % (103725 x
+// 512 83 -> 85 us, 4099 x 14336 48.5 -> 51, 9001 x 1000 50 -> 52).  With h rounded
 // to the type, out was 1.25 times as far from the exact sum.  out is rounded once.
 //
 // Measured on a B200: 64 tokens of their own adapters (512 to 1536, rank 16) 5.5 us,
 // a launch, a cluster barrier and three dependent reads; 103725 x 512 to 512, rank 16,
-// 83 us (0.59 of HBM: tiles take 17-21 us at the bandwidth, the few with over four
-// adapters 40 and end last); 4099 x 14336 to 512, rank 32, 49 us (H alone 28, at the
-// HBM rate of x; out alone about 17, most of it its start and the partial sums); 9001
-// x 1000 to 1544, rank 8, in runs of 7, 49 us (H 13, out 31 in its longest tile).
-// Ranks padded to 16 columns and four warps of rows took 83 us there.
+// 85 us (0.57 of HBM: tiles take 17-21 us at the bandwidth, the few with over four
+// adapters 40 and end last); 4099 x 14336 to 512, rank 32, 51 us (H by itself 30, 0.6
+// of the copy rate in 264 CTAs of 28 K blocks each, of which the start is not hidden;
+// out by itself 24 for 8 MB, most of it its start and the partial sums); 9001 x 1000 to
+// 1544, rank 8, in runs of 7, 52 us (by themselves, caches cold, H 17 and out 49, in its
+// longest tile).  Ranks padded to 16 columns and four warps of rows took 83 us there.
 #include "common.cuh"
 
 #include <algorithm>
@@ -811,25 +812,24 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             if ((k0 & 1) != half) ++k0;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
+              float* s = own[i];
 #pragma unroll
-              for (int d = 0; d < 2; ++d) {
-                float* s = own[i] + 8 * d;
+              for (int q = 0; q < 16; ++q) s[q] = 0.0f;
+              const int j = 2 * (k0 + 2 * i) - e0;
+              const bool in[2] = {mine >= 0 && j >= 0 && j < eights, mine >= 0 && j + 1 >= 0 && j + 1 < eights};
+              if (!in[0] && !in[1]) continue;
+              const float4* from = reinterpret_cast<const float4*>(p.part + row * p.rank + 8 * j);
+              // (by 4 and 8, and one eight at a time by those, 0.1 to 2 us a call more: what they load ahead is spilled)
+#pragma unroll 2
+              for (int k = 0; k < p.splits; ++k, from += p.T * p.rank / 4) {
 #pragma unroll
-                for (int q = 0; q < 8; ++q) s[q] = 0.0f;
-                const int j = 2 * (k0 + 2 * i) + d - e0;
-                if (mine < 0 || j < 0 || j >= eights) continue;
-                const float4* from = reinterpret_cast<const float4*>(p.part + row * p.rank + 8 * j);
-#pragma unroll 4
-                for (int k = 0; k < p.splits; ++k) {
-                  const float4 f = __ldcg(from + k * (p.T * p.rank / 4)), h = __ldcg(from + k * (p.T * p.rank / 4) + 1);
-                  s[0] += f.x;
-                  s[1] += f.y;
-                  s[2] += f.z;
-                  s[3] += f.w;
-                  s[4] += h.x;
-                  s[5] += h.y;
-                  s[6] += h.z;
-                  s[7] += h.w;
+                for (int f = 0; f < 4; ++f) {
+                  if (!in[f >> 1]) continue;
+                  const float4 v = __ldcg(from + f);
+                  s[4 * f] += v.x;
+                  s[4 * f + 1] += v.y;
+                  s[4 * f + 2] += v.z;
+                  s[4 * f + 3] += v.w;
                 }
               }
             }
@@ -1021,9 +1021,9 @@ struct Plan {
 };
 // Tokens are taken one by one where there are few, or where all of their products are few (T rank (K + N) of 2^24):
 // the cost grows with the products, while tiles cost a start, and more for each group of adapters.  Token kernel / tiles
-// of one or two adapters / tiles of 8 and more, in us: 512 to 512, rank 8: 256 tokens 4.6 / 12.5 / 13.7, 1024 tokens 8.7 /
-// 12.8 / 13.8; 512 to 1536, rank 16: 256 tokens 7.4 / 13.5 / 42, 512 tokens 9.4 / 14.3 / 42; 512 to 512, rank 64: 256
-// tokens 13.4 / 18.7 / 47.  Above it: 14336 to 512, rank 32: 256 tokens 28 / 32-42 / 76, 512 tokens 48 / 34-44 / 75.
+// of one or two adapters / tiles of about 11, in us: 512 to 512, rank 8: 256 tokens 4.3 / 13.1 / 16.2, 1024 tokens 8.4 /
+// 13.8 / 16.5; 512 to 1536, rank 16: 256 tokens 7.5 / 14.1 / 22.6, 512 tokens 9.4 / 14.4 / 22.6; 512 to 512, rank 64: 256
+// tokens 13.2 / 19.6 / 54.  Above it: 14336 to 512, rank 32: 256 tokens 28 / 32 / 59, 512 tokens 48 / 34 / 60.
 constexpr int kTokenMax = 96, kTokenMaxOfFewProducts = 1024;
 constexpr int64_t kFewProducts = 1 << 24;
 
@@ -1038,10 +1038,10 @@ static Plan plan_of(int64_t T, int K, int N, int rank) {
   const int kblocks = (K + 63) / 64, chunks = (N + kChunk - 1) / kChunk;
   q.chunks = chunks;
   // Two CTAs an SM are resident: up to a tile an SM the two phases are spread over them.  Apart / fused, in us, in runs of
-  // 100 and of 1 token: 18000 x 14336 to 512, rank 32: 115 and 387 / 217 and 844; 18000 x 512 to 1536, rank 16: 40 and 121
-  // / 39 and 235; the other way 18000 x 512 to 512, rank 8: 20 and 22 / 18.6 and 19.6.  Above it fused: two parts a tile
+  // 100 and of 1 token of 32 adapters: 18000 x 14336 to 512, rank 32: 114 and 820 / 217 and 1780; 18000 x 512 to 1536, rank
+  // 16: 42 and 125 / 42 and 241; 18000 x 512 to 512, rank 8: 20.9 and 49 / 18.9 and 63.  Above it fused: two parts a tile
   // gained where most rows of a tile have their own adapter and lost where they share them (60000 x 2048 to 2048, rank 32,
-  // runs of 1, 100 and 3000: 361, 213 and 211 / 488, 212 and 156).
+  // runs of 1, 100 and 3000: 1170, 224 and 221 / 1700, 226 and 156).
   if (tiles <= sms) {
     const int64_t want = 2 * sms / tiles;
     q.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, (int64_t)(kblocks + 3) / 4, 16}));

@@ -21,10 +21,10 @@
 // Each lane sorts its V words once (a network of minima and maxima), so a round
 // is one maximum over the lanes' heads and a shift in the lane that had it.
 //
-// What bounds it: the launch for small calls (one token 2.5 us, 103725 x 8 4.2 us),
+// What bounds it: the launch for small calls (one token 2.1-2.5 us, 103725 x 8 4.2 us),
 // instructions for many experts (integer minima, maxima and selects run at half
 // rate), never bytes.  16411 x 256 fp32 in groups with a bias (17 MB, 2.8 us of HBM):
-// 18.8 M warp instructions, 29 us, of which about 11 are one or two tokens whose
+// 19.2 M warp instructions, 29 us, of which about 11 are one or two tokens whose
 // groups are decided again in fp64, late in the grid; rounds over unsorted lanes and
 // 64-bit words took 25.6 M and 40 us.  24490 x 64: 7.3 us forward, 6.2 backward.
 // Eight values a lane: with sixteen (half the lanes a token) 16411 x 256 took 22 us

@@ -327,7 +327,8 @@ int rb_smoe_experts(const void* x, int x_dtype, int64_t ldx, int64_t T, int D, c
  *              highest values stay
  *   idx        [T, k] RB_I64 or RB_I32, k <= 32: the experts of the k highest c among
  *              the groups that stay, c falling; ties (groups too) to the lowest
- *              index, decided on the exact values, whatever the fp32 scores round to.
+ *              index, decided on the values in fp64 (without biases and sums on the
+ *              logits themselves), whatever the fp32 scores round to.
  *              Where fewer than k are unmasked, masked ones follow with score 0.
  *   score      [T, k]: s of the chosen, divided by their sum when `renormalize` (0
  *              when the sum is 0), times `scale`
