@@ -30,10 +30,10 @@
 // Measured on a B200: 64 tokens of their own adapters (512 to 1536, rank 16) 5.5 us,
 // a launch, a cluster barrier and three dependent reads; 103725 x 512 to 512, rank 16,
 // 85 us (0.57 of HBM: tiles take 17-21 us at the bandwidth, the few with over four
-// adapters 40 and end last); 4099 x 14336 to 512, rank 32, 51 us (H by itself 30, 0.6
+// adapters 40 and end last); 4099 x 14336 to 512, rank 32, 51 us (H by itself 29, 0.6
 // of the copy rate in 264 CTAs of 28 K blocks each, of which the start is not hidden;
-// out by itself 24 for 8 MB, most of it its start and the partial sums); 9001 x 1000 to
-// 1544, rank 8, in runs of 7, 52 us (by themselves, caches cold, H 17 and out 49, in its
+// out by itself 25 for 8 MB, most of it its start and the partial sums); 9001 x 1000 to
+// 1544, rank 8, in runs of 7, 52 us (by themselves, caches cold, H 16 and out 49, in its
 // longest tile).  Ranks padded to 16 columns and four warps of rows took 83 us there.
 #include "common.cuh"
 
