@@ -718,8 +718,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       lt.next();
       tile = -1;
       if (MODE == kFused) {
-        // a tile of several groups takes long: its CTA takes over another one only when it is through
-        if (count > group && !__all_sync(kAll, mbar_wait_bounded(smem_u32(&lempty[mine.slot]), mine.parity, kWaitTimeoutProducer, abort_flag)))
+        // a tile of several groups takes long: its CTA takes over another one only when it is through.  All of its groups' time
+        // (N of millions: seconds), so a wait's usual budget for each; the others' waits are for one step of the work.
+        const uint64_t budget = kWaitBudgetNs * (uint64_t)((count + group - 1) / group);
+        if (count > group &&
+            !__all_sync(kAll, mbar_wait_bounded(smem_u32(&lempty[mine.slot]), mine.parity, kWaitTimeoutProducer, abort_flag, budget)))
           break;
         if (lane == 0) ask_tile(smem_u32(&s_told), smem_u32(&told));
         asked = true;
