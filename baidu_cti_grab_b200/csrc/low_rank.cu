@@ -926,6 +926,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                            T* to = reinterpret_cast<T*>(mem + (((4 * half + (q >> 3)) ^ (r & 7)) << 4)) + (q & 7);
                            *to = T(fmaf(k, d, to_f32(*to)));
                          });
+              __syncwarp();
               tc::tmem_ld32(sums, v);  // of the other rows (kept over the call they would go to memory)
             }
             tc::tc_fence_before();
@@ -983,6 +984,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
               add_own<T>(redo, static_cast<const T*>(p.b) + ((int64_t)adapter * p.N + c0) * p.rank, min(32, p.N - c0), p.rank, sH,
                          tmem + lanes + C::kRestAt, (n * eights + 1) / 2, r, e0, wh,
                          [=](int q, float k, float d) { out[c0 + q] = T(fmaf(k, d, to_f32(y[c0 + q]))); });
+              __syncwarp();
               tc::tmem_ld32(sums, v);
             }
             tc::tc_fence_before();
