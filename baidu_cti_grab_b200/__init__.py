@@ -14,6 +14,9 @@ and, around those kernels, what the reference leaves to separate torch ops or la
 * ``routing``             -- the gate: scores, balance bias, groups, top-k (with gradients)
 * ``block_norm``          -- norms, gate and residual scale between two blocks (with gradients)
 * ``adapters``            -- low-rank adapters of many requests beside a shared projection
+* ``attention``           -- attention within packed users (with gradients)
+* ``embedding``           -- embedding rows, and the table's gradient by sorted ids
+* ``grad_clip``           -- the norm of all gradients, and the clipping by it
 
 The CUDA library is loaded on first use (``baidu_cti_grab_b200._lib``); every
 device entry point raises if it cannot be loaded -- there is no CPU fallback.

@@ -74,6 +74,21 @@ SIGNATURES = {
     "rb_low_rank_workspace_size": [_i64, _i32, _i32, _i32],
     "rb_low_rank_add": [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp, _i64,
                         _vp, _i64, _vp],
+    "rb_segment_attention_workspace_size": [_i64, _i64, _i64, _i32, _i32, _i32],
+    "rb_segment_attention": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i64, _i64, _i32, _i32, _i32, _vp, _vp,
+                             _vp, _i32, _i64, _i32, _vp, _f32, _f32, _vp, _i64, _vp, _vp, _vp],
+    "rb_segment_attention_backward_workspace_size": [_i64, _i64, _i64, _i32, _i32, _i32],
+    "rb_segment_attention_backward": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i64,
+                                      _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _i64, _i32, _vp, _f32, _f32, _vp, _i64, _vp,
+                                      _vp, _vp, _vp],
+    "rb_embed_rows": [_vp, _i32, _i64, _i64, _i32, _vp, _i32, _i64, _f32, _vp, _i64, _vp],
+    "rb_embed_rows_backward_workspace_size": [_i64, _i32],
+    "rb_embed_rows_backward": [_vp, _i32, _i64, _i32, _vp, _i32, _i64, _i64, _vp, _i64, _i64, _f32, _i32, _vp, _i64, _vp, _i32,
+                               _i64, _vp],
+    "rb_embed_rows_backward_sparse": [_vp, _i32, _i64, _i32, _vp, _i32, _i64, _i64, _vp, _i64, _i64, _f32, _vp, _i64, _vp, _vp,
+                                      _i32, _i64, _vp, _vp],
+    "rb_grad_norm_workspace_size": [_i32],
+    "rb_clip_grads": [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _f32, _f32, _vp, _i64, _vp, _vp],
     "rb_rep_gather_pool_scatter": [_vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _i32, _i64,
                                    _i64, _vp],
     "rb_ipc_export": [_vp, _vp, _vp],
@@ -86,7 +101,9 @@ SIGNATURES = {
 }
 
 RETURNS_I64 = {"rb_w8a8_gemm_workspace_size", "rb_smoe_workspace_size", "rb_sandwich_norm_workspace_size",
-               "rb_low_rank_workspace_size"}
+               "rb_low_rank_workspace_size", "rb_segment_attention_workspace_size",
+               "rb_segment_attention_backward_workspace_size", "rb_embed_rows_backward_workspace_size",
+               "rb_grad_norm_workspace_size"}
 
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None

@@ -1,0 +1,1351 @@
+// attention.cu -- attention within packed segments (an encoder's users, documents): queries
+// [Tq, H, D] and keys/values [Tk, Hk, D] of S segments lie one behind the other, and a query
+// sees keys of its own segment only.  For query i (of n) and key j (of m) of a segment, head h:
+//
+//   x = scale q_i . k_j      s = cap tanh(x / cap)  (or x)  - slope_h |i + m - n - j|
+//   seen(i, j) = not causal, or j <= i + m - n, or j < prefix
+//   p_ij = exp(s_ij) / sum over seen exp(s)     out_i = sum_j p_ij v_j     (0 where nothing is seen)
+//
+// and, with dp_ij = dout_i . v_j, delta_i = dout_i . out_i, e_ij = p_ij (dp_ij - delta_i) (1 - tanh^2) scale:
+//
+//   dv_j = sum_i p_ij dout_i     dq_i = sum_j e_ij k_j     dk_j = sum_i e_ij q_i
+//
+// (dk, dv: summed over the query heads that share the key head).
+//
+// What every kernel uses: the mask of a row is ONE interval [lo, hi) of the packed keys, whatever mixes into it
+// (segments, causal order, prefix).  rows_kernel computes it once a call for all heads, so that tiles need not follow
+// segments: a tile is 128 rows of the packed order, its keys are the union of its rows' intervals, and a block of keys
+// that all rows see is not masked at all.
+#include "common.cuh"
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <mutex>
+#include <type_traits>
+
+namespace rb {
+namespace attn {
+
+constexpr unsigned kAll = 0xffffffffu;
+constexpr int kMaxWidth = 256;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Params {
+  const void *q, *k, *v, *o, *g;  // o, g: the forward call's output and the gradient it got
+  void *out, *dq, *dk, *dv;
+  float* lse;                     // [H, Tq] log of the sum of exp(s), -inf where nothing is seen
+  float* delta;                   // [H, Tq]
+  int4* rows;                     // [Tq]: lo, hi, place of the query among the packed keys, 0
+  const void *q_off, *k_off, *prefix;
+  const float* slopes;
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h, g_t, g_h;  // elements from token to token and from head to head
+  int Tq, Tk, S, H, Hk, G, D, off64, causal;
+  float scale, cap;
+  uint32_t* peaks;                // fp16 backward: the largest norms of a row of g and of v
+  int by_segment;                 // tiles follow segments (else: 128 rows of the packed order)
+};
+
+__device__ __forceinline__ int64_t entry(const void* a, int wide, int64_t i) {
+  return wide ? __ldg(static_cast<const int64_t*>(a) + i) : (int64_t)__ldg(static_cast<const int32_t*>(a) + i);
+}
+// an offset as it may be used: whatever the array holds, no row outside [0, total] is named
+__device__ __forceinline__ int offset_at(const void* a, int wide, int i, int total) {
+  return (int)min(max(entry(a, wide, i), (int64_t)0), (int64_t)total);
+}
+// the last segment that starts at or before row r, or -1
+__device__ __forceinline__ int segment_of(const void* off, int wide, int S, int total, int r) {
+  int a = 0, b = S;  // segments [0, a) start at or before r, [b, S) behind it
+  while (a < b) {
+    const int m = (a + b) >> 1;
+    if (offset_at(off, wide, m, total) <= r) a = m + 1;
+    else b = m;
+  }
+  return a - 1;
+}
+
+__device__ __forceinline__ int4 row_of(const Params& p, int r) {
+  const int s = segment_of(p.q_off, p.off64, p.S, p.Tq, r);
+  if (s < 0) return make_int4(0, 0, 0, 0);
+  const int q0 = offset_at(p.q_off, p.off64, s, p.Tq), q1 = offset_at(p.q_off, p.off64, s + 1, p.Tq);
+  if (r >= q1) return make_int4(0, 0, 0, 0);
+  const int k0 = offset_at(p.k_off, p.off64, s, p.Tk), k1 = max(k0, offset_at(p.k_off, p.off64, s + 1, p.Tk));
+  const int place = k0 + (r - q0) + (k1 - k0) - (q1 - q0);
+  int hi = k1;
+  if (p.causal) {
+    const int seen = p.prefix != nullptr ? (int)min(max(entry(p.prefix, p.off64, s), (int64_t)0), (int64_t)(k1 - k0)) : 0;
+    hi = min(k1, max(place + 1, k0 + seen));
+  }
+  return hi > k0 ? make_int4(k0, hi, place, 0) : make_int4(0, 0, place, 0);
+}
+
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r < p.Tq) p.rows[r] = row_of(p, r);
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) { return (float)v; }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// tanh from exp: 1 - 2 / (1 + e^2x).  Near 0 it is off by 2^-23 of 1, not of x: in the score that is 2^-23 cap, where
+// the hardware's own tanh is off by 2^-11 of x.
+__device__ __forceinline__ float tanh_of(float x) { return fmaf(-2.0f, rcp_fast(1.0f + exp2_fast(x * (2.0f * kLog2e))), 1.0f); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+
+// ------------------------------------------------------------ one row, one warp
+// The formulas as they stand, a warp for a row of one head, each lane D / 32 columns.  These take the shapes that the
+// tiles do not (D off 8 or above 128, rows off 16 bytes), and every row of a tile whose result is not finite: a tile
+// adds the keys that a row does not see times a zero weight, and a zero times an infinity or NaN there is a NaN.
+constexpr int kPerLane = kMaxWidth / 32;
+
+template <typename T>
+__device__ __forceinline__ void load_row(const void* base, int64_t at, int D, int lane, float* v) {
+  const T* t = static_cast<const T*>(base) + at;
+#pragma unroll
+  for (int c = 0; c < kPerLane; ++c) v[c] = lane + 32 * c < D ? to_f32(t[lane + 32 * c]) : 0.0f;
+}
+template <typename T>
+__device__ __forceinline__ void store_row(void* base, int64_t at, int D, int lane, const float* v, float w) {
+  T* t = static_cast<T*>(base) + at;
+#pragma unroll
+  for (int c = 0; c < kPerLane; ++c)
+    if (lane + 32 * c < D) t[lane + 32 * c] = T(v[c] * w);
+}
+__device__ __forceinline__ float dot_row(const float* a, const float* b) {
+  float s = 0.0f;
+#pragma unroll
+  for (int c = 0; c < kPerLane; ++c) s = fmaf(a[c], b[c], s);
+  return warp_sum(s);
+}
+// the score in units of log 2, and 1 - tanh^2
+__device__ __forceinline__ float score_of(const Params& p, float x, int place, int j, float slope, float& slant) {
+  x *= p.scale;
+  slant = 1.0f;
+  if (p.cap > 0.0f) {
+    const float t = tanh_of(x / p.cap);
+    slant = fmaf(-t, t, 1.0f);
+    x = p.cap * t;
+  }
+  return kLog2e * fmaf(-slope, (float)abs(place - j), x);
+}
+
+template <typename T>
+__device__ __noinline__ void row_forward(const Params& p, int r, int h) {
+  const int lane = threadIdx.x & 31, hk = h / p.G;
+  const int4 row = p.rows[r];
+  const float slope = p.slopes != nullptr ? __ldg(p.slopes + h) : 0.0f;
+  float q[kPerLane], o[kPerLane], x[kPerLane], top = -INFINITY, total = 0.0f, slant;
+  load_row<T>(p.q, r * p.q_t + h * p.q_h, p.D, lane, q);
+#pragma unroll
+  for (int c = 0; c < kPerLane; ++c) o[c] = 0.0f;
+#pragma unroll 1
+  for (int j = row.x; j < row.y; ++j) {
+    load_row<T>(p.k, j * p.k_t + hk * p.k_h, p.D, lane, x);
+    const float s = score_of(p, dot_row(q, x), row.z, j, slope, slant);
+    const float higher = fmaxf(top, s);
+    const float keep = higher == top ? 1.0f : exp2_fast(top - higher);
+    const float w = higher == -INFINITY ? s - s + 0.0f : exp2_fast(s - higher);  // (a score of -inf: nothing, or NaN)
+    top = higher;
+    const float e = s == -INFINITY ? 0.0f : w;
+    total = fmaf(total, keep, e);
+    load_row<T>(p.v, j * p.v_t + hk * p.v_h, p.D, lane, x);
+#pragma unroll
+    for (int c = 0; c < kPerLane; ++c) o[c] = fmaf(o[c], keep, e * x[c]);
+  }
+  store_row<T>(p.out, ((int64_t)r * p.H + h) * p.D, p.D, lane, o, total == 0.0f ? 0.0f : 1.0f / total);
+  if (p.lse != nullptr && lane == 0) p.lse[(int64_t)h * p.Tq + r] = total == 0.0f ? -INFINITY : kLn2 * (top + log2f(total));
+}
+
+// in units of log 2; +inf (all weights 0) for a row that sees nothing
+__device__ __forceinline__ float lse_of(const Params& p, int r, int h) {
+  const float l = __ldg(p.lse + (int64_t)h * p.Tq + r);
+  return l == -INFINITY ? INFINITY : kLog2e * l;
+}
+
+template <typename T>
+__device__ __noinline__ void row_dq(const Params& p, int r, int h) {
+  const int lane = threadIdx.x & 31, hk = h / p.G;
+  const int4 row = p.rows[r];
+  const float slope = p.slopes != nullptr ? __ldg(p.slopes + h) : 0.0f;
+  const float lse = lse_of(p, r, h), delta = p.delta[(int64_t)h * p.Tq + r];
+  float q[kPerLane], g[kPerLane], dq[kPerLane], k[kPerLane], v[kPerLane], slant;
+  load_row<T>(p.q, r * p.q_t + h * p.q_h, p.D, lane, q);
+  load_row<T>(p.g, r * p.g_t + h * p.g_h, p.D, lane, g);
+#pragma unroll
+  for (int c = 0; c < kPerLane; ++c) dq[c] = 0.0f;
+#pragma unroll 1
+  for (int j = row.x; j < row.y; ++j) {
+    load_row<T>(p.k, j * p.k_t + hk * p.k_h, p.D, lane, k);
+    load_row<T>(p.v, j * p.v_t + hk * p.v_h, p.D, lane, v);
+    const float s = score_of(p, dot_row(q, k), row.z, j, slope, slant);
+    const float e = exp2_fast(s - lse) * (dot_row(g, v) - delta) * slant;
+#pragma unroll
+    for (int c = 0; c < kPerLane; ++c) dq[c] = fmaf(e, k[c], dq[c]);
+  }
+  store_row<T>(p.dq, ((int64_t)r * p.H + h) * p.D, p.D, lane, dq, p.scale);
+}
+
+// the queries of the segment that key j belongs to: [x, y)
+__device__ __forceinline__ int2 queries_of(const Params& p, int j) {
+  const int s = segment_of(p.k_off, p.off64, p.S, p.Tk, j);
+  if (s < 0 || j >= offset_at(p.k_off, p.off64, s + 1, p.Tk)) return make_int2(0, 0);
+  return make_int2(offset_at(p.q_off, p.off64, s, p.Tq), offset_at(p.q_off, p.off64, s + 1, p.Tq));
+}
+
+template <typename T>
+__device__ __noinline__ void row_dkv(const Params& p, int j, int hk) {
+  const int lane = threadIdx.x & 31;
+  const int2 span = queries_of(p, j);
+  float k[kPerLane], v[kPerLane], dk[kPerLane], dv[kPerLane], q[kPerLane], g[kPerLane], slant;
+  load_row<T>(p.k, j * p.k_t + hk * p.k_h, p.D, lane, k);
+  load_row<T>(p.v, j * p.v_t + hk * p.v_h, p.D, lane, v);
+#pragma unroll
+  for (int c = 0; c < kPerLane; ++c) dk[c] = dv[c] = 0.0f;
+#pragma unroll 1
+  for (int h = hk * p.G; h < (hk + 1) * p.G; ++h) {
+    const float slope = p.slopes != nullptr ? __ldg(p.slopes + h) : 0.0f;
+#pragma unroll 1
+    for (int r = span.x; r < span.y; ++r) {
+      const int4 row = p.rows[r];
+      if (j < row.x || j >= row.y) continue;
+      load_row<T>(p.q, r * p.q_t + h * p.q_h, p.D, lane, q);
+      load_row<T>(p.g, r * p.g_t + h * p.g_h, p.D, lane, g);
+      const float s = score_of(p, dot_row(q, k), row.z, j, slope, slant);
+      const float w = exp2_fast(s - lse_of(p, r, h));
+      const float e = w * (dot_row(g, v) - p.delta[(int64_t)h * p.Tq + r]) * slant;
+#pragma unroll
+      for (int c = 0; c < kPerLane; ++c) {
+        dk[c] = fmaf(e, q[c], dk[c]);
+        dv[c] = fmaf(w, g[c], dv[c]);
+      }
+    }
+  }
+  const int64_t at = ((int64_t)j * p.Hk + hk) * p.D;
+  store_row<T>(p.dk, at, p.D, lane, dk, p.scale);
+  store_row<T>(p.dv, at, p.D, lane, dv, 1.0f);
+}
+
+enum RowPass : int { kRowForward, kRowDq, kRowDkv };
+template <typename T, int PASS>
+__global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int heads = PASS == kRowDkv ? p.Hk : p.H;
+  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= (int64_t)(PASS == kRowDkv ? p.Tk : p.Tq) * heads) return;
+  const int r = (int)(i / heads), h = (int)(i % heads);
+  if constexpr (PASS == kRowForward) row_forward<T>(p, r, h);
+  else if constexpr (PASS == kRowDq) row_dq<T>(p, r, h);
+  else row_dkv<T>(p, r, h);
+}
+
+// delta_i = dout_i . out_i, a warp a row of one head; in fp16 the largest norms of a row of dout and of v too (those that
+// are finite), as bits of positive floats, which order as numbers do.  Warps behind the queries' take v.
+template <typename T>
+__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr bool kPeaks = std::is_same<T, __half>::value;
+  const int lane = threadIdx.x & 31;
+  int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t queries = (int64_t)p.Tq * p.H;
+  float norm = 0.0f;
+  if (i < queries) {
+    const int r = (int)(i / p.H), h = (int)(i % p.H);
+    if (h == 0 && lane == 0) p.rows[r] = row_of(p, r);
+    const T* o = static_cast<const T*>(p.o) + i * p.D;
+    const T* g = static_cast<const T*>(p.g) + r * p.g_t + h * p.g_h;
+    float s = 0.0f;
+    for (int c = lane; c < p.D; c += 32) {
+      const float f = to_f32(g[c]);
+      s = fmaf(to_f32(o[c]), f, s);
+      norm = fmaf(f, f, norm);
+    }
+    s = warp_sum(s);
+    if (lane == 0) p.delta[(int64_t)h * p.Tq + r] = s;
+  } else if (kPeaks && i - queries < (int64_t)p.Tk * p.Hk) {
+    i -= queries;
+    const T* v = static_cast<const T*>(p.v) + i / p.Hk * p.v_t + i % p.Hk * p.v_h;
+    for (int c = lane; c < p.D; c += 32) norm = fmaf(to_f32(v[c]), to_f32(v[c]), norm);
+    i += queries;
+  }
+  if (kPeaks) {
+    norm = sqrtf(warp_sum(norm));
+    if (lane == 0 && norm > 0.0f && norm < INFINITY) atomicMax(p.peaks + (i < queries ? 0 : 1), __float_as_uint(norm));
+  }
+}
+
+// ------------------------------------------------------- tensor-core helpers
+constexpr int kTile = 128;    // rows of a tile: the lanes of TMEM
+constexpr int kBlock = 64;    // of the other side that a step takes
+constexpr int kThreads = 160; // a warp for the copies and the MMAs, four for the rows
+
+// K-major operand: 64 columns (128 bytes) a row, groups of eight rows 1024 bytes apart
+__device__ __forceinline__ uint64_t rows_desc(uint32_t saddr) { return tc::sw128_desc(saddr); }
+// the same bytes as an operand whose 64-column rows run along K: `next` bytes on lie the next 64 columns
+__device__ __forceinline__ uint64_t columns_desc(uint32_t saddr, uint32_t next) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
+}
+// A from TMEM: sixteen 16-bit values of a row are eight words of its lane
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 32 columns of this thread's lane, to be used after tmem_wait_ld
+__device__ __forceinline__ void tmem_get32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_put32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return pack_bf16x2(lo, hi);
+  else return pack_f16x2(lo, hi);
+}
+template <typename T>
+__host__ __device__ constexpr uint32_t type_bits() { return std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u; }
+// D fp32, M = 128, N columns; TURNED: B's rows run along K
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_of(int n, bool turned) {
+  return (1u << 4) | type_bits<T>() | (turned ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+
+// A row of fp32 sums of `n` columns times w, as the type, to 16-byte aligned memory
+template <typename T>
+__device__ __forceinline__ void store_sums(T* to, const uint32_t* v, int n, float w, bool wide) {
+#pragma unroll
+  for (int c = 0; c < 32; c += 16) {
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = pack2<T>(__uint_as_float(v[c + 2 * i]) * w, __uint_as_float(v[c + 2 * i + 1]) * w);
+    if (c + 16 <= n && wide) {
+      stg_v8(to + c, o);
+    } else {
+      if (c + 8 <= n) *reinterpret_cast<uint4*>(to + c) = make_uint4(o[0], o[1], o[2], o[3]);
+      if (c + 16 <= n) *reinterpret_cast<uint4*>(to + c + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+  }
+}
+__device__ __forceinline__ bool finite32(const uint32_t* v) {
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int q = 0; q < 32; ++q) s[q & 3] = fmaf(__uint_as_float(v[q]), 0.0f, s[q & 3]);
+  const float all = (s[0] + s[1]) + (s[2] + s[3]);
+  return all == all;
+}
+
+// whether all of the rows' N threads say so; they meet here
+template <int N>
+__device__ __forceinline__ bool rows_all(bool ok) {
+  uint32_t every;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(every)
+      : "r"((uint32_t)ok), "n"(N)
+      : "memory");
+  return every != 0;
+}
+
+// The rows [x, y) of tile b.  By the packed order, 128 rows a tile.  By segment, segment s has room for tiles from
+// floor(start / 128) + s on, which is as much as it needs and known without a sum over segments; the rows before the
+// first and behind the last count as segments too, and a tile that its segment does not need is empty.
+__device__ __forceinline__ int2 tile_rows(const void* off, int wide, int S, int total, int b, int by_segment) {
+  if (!by_segment) return make_int2(min(b * kTile, total), min((b + 1) * kTile, total));
+  // starts 0, off[0], ..., off[S]: the last i with floor(start_i / 128) + i <= b
+  int lo = 0, hi = S + 2;
+  const int lane = threadIdx.x & 31;
+  while (hi - lo > 1) {  // 32 probes at once
+    const int step = (hi - lo + 31) / 32;
+    const int i = lo + (lane + 1) * step;
+    const bool below = i < hi && offset_at(off, wide, i - 1, total) / kTile + i <= b;
+    const int n = __popc(__ballot_sync(kAll, below));
+    lo += n * step;
+    hi = min(hi, lo + step);
+  }
+  const int start = lo == 0 ? 0 : offset_at(off, wide, lo - 1, total);
+  const int end = lo == S + 1 ? total : offset_at(off, wide, lo, total);
+  const int first = start + (b - (start / kTile + lo)) * kTile;
+  return make_int2(min(first, end), min(first + kTile, end));
+}
+
+// scores in place of raw products, in units of log 2; `unit` is what is left to multiply by
+__device__ __forceinline__ void transform(const Params& p, uint32_t* raw, float slope2, int place, int j0) {
+  const float up = p.scale / p.cap, cap2 = p.cap * kLog2e;
+  if (p.cap > 0.0f) {
+#pragma unroll
+    for (int c = 0; c < kBlock; ++c) raw[c] = __float_as_uint(cap2 * tanh_of(__uint_as_float(raw[c]) * up));
+  }
+  if (slope2 != 0.0f) {
+    const float first = (float)(place - j0), unit = p.cap > 0.0f ? 1.0f : p.scale * kLog2e;
+#pragma unroll
+    for (int c = 0; c < kBlock; ++c)
+      raw[c] = __float_as_uint(fmaf(-slope2, fabsf(first - (float)c), __uint_as_float(raw[c]) * unit));
+  }
+}
+
+// ---------------------------------------------------------------- forward
+// One CTA a tile of 128 rows of one head.  A row's thread takes its 64 scores of a block out of TMEM, keeps the
+// running maximum and sum, and puts the weights back as 16-bit values, from where the second product takes them;
+// its accumulator is rescaled only when a maximum has grown by more than 2^8 over what it is scaled to (the weights
+// stay below 256, the sum is fp32).  Rounding a weight to the type is half a step of its own value (2^-9 bf16, 2^-12
+// fp16), independent from key to key.
+template <int DP>
+struct Forward {
+  static constexpr int kChunks = DP / 64;              // 64 columns, a swizzled row
+  static constexpr int kQBytes = kTile * 128 * kChunks;
+  static constexpr int kKvBytes = kBlock * 128 * kChunks;
+  static constexpr int kStages = DP == 64 ? 3 : 2;
+  static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kKvBytes;
+  // DP 64: the weights lie where the scores were, 128 columns in all and three CTAs an SM; DP 128: apart, two CTAs,
+  // and the next scores are computed meanwhile
+  static constexpr bool kApart = DP == 128;
+  static constexpr int kPAt = kApart ? 64 : 0, kOAt = kApart ? 128 : 64;
+  static constexpr int kTmemCols = kApart ? 256 : 128;
+  static constexpr int kCtas = kApart ? 2 : 3;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, Forward<DP>::kCtas)
+    forward_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
+  using C = Forward<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + C::kQBytes;
+  uint8_t* sV = sK + C::kStages * C::kKvBytes;
+  __shared__ __align__(8) uint64_t qfull, kfull[C::kStages], vfull[C::kStages];
+  __shared__ __align__(8) uint64_t sfull, sfree, pready, pvdone, drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word, s_lo[4], s_hi[4];
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // long rows come last in the packed order: their tiles start first
+  const int tile = gridDim.x - 1 - blockIdx.x, h = blockIdx.y, hk = h / p.G;
+
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&qfull), 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(smem_u32(&kfull[s]), 1);
+      mbar_init(smem_u32(&vfull[s]), 1);
+    }
+    mbar_init(smem_u32(&sfull), 1);
+    mbar_init(smem_u32(&sfree), kTile);
+    mbar_init(smem_u32(&pready), kTile);
+    mbar_init(smem_u32(&pvdone), 1);
+    mbar_init(smem_u32(&drained), 1);
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmQ)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmK)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmV)) : "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int2 span = tile_rows(p.q_off, p.off64, p.S, p.Tq, tile, p.by_segment);
+  const int quarter = warp & 3;  // of the lanes of TMEM, for the rows' warps
+  const int r = span.x + quarter * 32 + lane;
+  int4 row = make_int4(0, 0, 0, 0);
+  if (warp >= 1) {
+    if (r < span.y) row = __ldg(p.rows + r);
+    int lo = row.y > row.x ? row.x : INT_MAX, hi = row.y > row.x ? row.y : 0;
+    lo = __reduce_min_sync(kAll, lo);
+    hi = __reduce_max_sync(kAll, hi);
+    if (lane == 0) {
+      s_lo[quarter] = lo;
+      s_hi[quarter] = hi;
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int key0 = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
+  const int key1 = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+  const int blocks = key1 > key0 ? (key1 - key0 + kBlock - 1) / kBlock : 0;
+
+  if (warp == 0) {
+    if (lane == 0 && blocks > 0) {
+      // -------------------------------------------------- copies and MMAs
+      constexpr uint32_t idesc_s = idesc_of<T>(kBlock, false), idesc_o = idesc_of<T>(DP, true);
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(smem_u32(bar), parity, kWaitTimeoutMma, abort_flag); };
+      auto slot = [](int n) { return n % C::kStages; };
+      auto phase = [](int n) { return (uint32_t)(n / C::kStages) & 1u; };
+      int k_asked = 0, v_asked = 0;
+      auto ask = [&](uint64_t* full, uint8_t* to, const CUtensorMap* tm, int n) {
+        const uint32_t bar = smem_u32(&full[slot(n)]);
+        mbar_arrive_expect_tx(bar, C::kKvBytes);
+        for (int c = 0; c < C::kChunks; ++c)
+          tma_load_3d(smem_u32(to + slot(n) * C::kKvBytes + c * kBlock * 128), tm, 64 * c, hk, key0 + n * kBlock, bar);
+      };
+      auto ask_k = [&] { if (k_asked < blocks) ask(kfull, sK, &tmK, k_asked), ++k_asked; };
+      auto ask_v = [&] { if (v_asked < blocks) ask(vfull, sV, &tmV, v_asked), ++v_asked; };
+      const uint32_t qb = smem_u32(&qfull);
+      mbar_arrive_expect_tx(qb, C::kQBytes);
+      for (int c = 0; c < C::kChunks; ++c) tma_load_3d(smem_u32(sQ + c * kTile * 128), &tmQ, 64 * c, h, span.x, qb);
+      for (int s = 0; s < C::kStages; ++s) {
+        ask_k();
+        ask_v();
+      }
+      const int steps = (p.D + 15) / 16;  // of 16 columns (the rest of a row is zeros)
+      auto scores = [&](int n) {
+        if (!wait(&kfull[slot(n)], phase(n))) return false;
+        tc::tc_fence_after();
+        const uint64_t qd = rows_desc(smem_u32(sQ)), kd = rows_desc(smem_u32(sK + slot(n) * C::kKvBytes));
+        for (int i = 0; i < steps; ++i)
+          mma_ss(tmem, qd + (uint64_t)((i >> 2) * (kTile * 128 / 16) + (i & 3) * 2),
+                 kd + (uint64_t)((i >> 2) * (kBlock * 128 / 16) + (i & 3) * 2), idesc_s, i > 0);
+        tc::umma_commit(smem_u32(&sfull));
+        return true;
+      };
+      bool ok = wait(&qfull, 0) && scores(0);
+      for (int n = 0; n < blocks && ok; ++n) {
+        if (C::kApart) {  // the rows' threads have the scores: their columns and their keys' slot are free
+          ok = wait(&sfree, (uint32_t)n & 1u);
+          if (ok) {
+            tc::tc_fence_after();
+            ask_k();
+            if (n + 1 < blocks) ok = scores(n + 1);
+          }
+        }
+        ok = ok && wait(&pready, (uint32_t)n & 1u) && wait(&vfull[slot(n)], phase(n));
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (C::kApart && n > 0) ask_v();  // (the weights were written after the product before had ended)
+        const uint64_t vd = columns_desc(smem_u32(sV + slot(n) * C::kKvBytes), kBlock * 128);
+        for (int i = 0; i < kBlock / 16; ++i)
+          mma_ts(tmem + C::kOAt, tmem + C::kPAt + 8 * i, vd + (uint64_t)(i * 16 * 128 / 16), idesc_o, n > 0 || i > 0);
+        tc::umma_commit(smem_u32(&pvdone));
+        if (!C::kApart && n + 1 < blocks) {
+          ok = wait(&pvdone, (uint32_t)n & 1u);
+          if (ok) {
+            ask_k();
+            ask_v();
+            ok = scores(n + 1);
+          }
+        }
+      }
+      if (!ok) {  // given up: no MMA in flight behind this CTA
+        tc::umma_commit(smem_u32(&drained));
+        mbar_wait_bounded(smem_u32(&drained), 0, kWaitTimeoutMma, nullptr);
+      }
+      // nor a copy
+      mbar_wait_bounded(qb, 0, kWaitTimeoutProducer, nullptr);
+      for (int i = max(0, k_asked - C::kStages); i < k_asked; ++i) mbar_wait_bounded(smem_u32(&kfull[slot(i)]), phase(i), kWaitTimeoutProducer, nullptr);
+      for (int i = max(0, v_asked - C::kStages); i < v_asked; ++i) mbar_wait_bounded(smem_u32(&vfull[slot(i)]), phase(i), kWaitTimeoutProducer, nullptr);
+    }
+  } else {
+    // -------------------------------------------------------------- rows
+    const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
+    const float slope2 = p.slopes != nullptr ? kLog2e * __ldg(p.slopes + h) : 0.0f;
+    const float unit = p.cap > 0.0f || slope2 != 0.0f ? 1.0f : p.scale * kLog2e;
+    float top = -INFINITY, total = 0.0f;  // top: what the weights are scaled to, in the scores' units
+    bool ok = true;
+    for (int n = 0; n < blocks && ok; ++n) {
+      const int j0 = key0 + n * kBlock;
+      ok = mbar_wait_bounded(smem_u32(&sfull), (uint32_t)n & 1u, kWaitTimeoutEpilogue, abort_flag);
+      ok = __all_sync(kAll, ok);
+      if (!ok) break;
+      tc::tc_fence_after();
+      uint32_t x[kBlock];
+      tmem_get32(mine, x);
+      tmem_get32(mine + 32, x + 32);
+      tmem_wait_ld();
+      if (C::kApart) {
+        tc::tc_fence_before();
+        mbar_arrive(smem_u32(&sfree));
+      }
+      transform(p, x, slope2, row.z, j0);
+      if (!__all_sync(kAll, row.x <= j0 && row.y >= j0 + kBlock)) {
+        const int lo = row.x - j0, len = max(row.y - row.x, 0);
+#pragma unroll
+        for (int c = 0; c < kBlock; ++c)
+          if ((unsigned)(c - lo) >= (unsigned)len) x[c] = 0xff800000u;
+      }
+      float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < kBlock; ++c) m[c & 3] = fmaxf(m[c & 3], __uint_as_float(x[c]));
+      const float high = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      const bool grow = (high - top) * unit > 8.0f || (top == -INFINITY && high > -INFINITY);
+      if (C::kApart && n > 0) ok = mbar_wait_bounded(smem_u32(&pvdone), (uint32_t)(n - 1) & 1u, kWaitTimeoutEpilogue, abort_flag);
+      ok = __all_sync(kAll, ok);
+      if (!ok) break;
+      if (__any_sync(kAll, grow)) {
+        if (n > 0) {
+          const float keep = grow ? exp2_fast((top - high) * unit) : 1.0f;
+          total *= keep;
+          tc::tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            tmem_get32(mine + C::kOAt + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+            tmem_put32(mine + C::kOAt + c, o);
+          }
+        }
+        if (grow) top = high;
+      }
+      const float shift = top == -INFINITY ? 0.0f : -top * unit;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      uint32_t w[kBlock / 2];
+#pragma unroll
+      for (int c = 0; c < kBlock; c += 2) {
+        const float a = exp2_fast(fmaf(__uint_as_float(x[c]), unit, shift)), b = exp2_fast(fmaf(__uint_as_float(x[c + 1]), unit, shift));
+        sum[c & 2] += a;
+        sum[(c & 2) + 1] += b;
+        w[c / 2] = pack2<T>(a, b);
+      }
+      total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_put32(mine + C::kPAt, w);
+      tmem_wait_st();
+      tc::tc_fence_before();
+      mbar_arrive(smem_u32(&pready));
+    }
+    if (ok && blocks > 0) {
+      ok = mbar_wait_bounded(smem_u32(&pvdone), (uint32_t)(blocks - 1) & 1u, kWaitTimeoutEpilogue, abort_flag);
+      tc::tc_fence_after();
+    }
+    ok = __all_sync(kAll, ok);
+    if (ok) {
+      const bool sees = row.y > row.x;
+      const float w = total == 0.0f ? 0.0f : 1.0f / total;
+      T* out = static_cast<T*>(p.out) + ((int64_t)r * p.H + h) * p.D;
+      const bool wide = p.D % 16 == 0 && aligned(p.out, 32);
+      bool redo = sees && !(total < INFINITY);
+#pragma unroll 1
+      for (int c = 0; c < p.D; c += 32) {
+        uint32_t o[32];
+        if (blocks > 0) {
+          tmem_get32(mine + C::kOAt + c, o);
+          tmem_wait_ld();
+        }
+        if (!sees) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        } else {
+          redo = redo || !finite32(o);
+        }
+        if (r < span.y) store_sums<T>(out + c, o, p.D - c, sees ? w : 0.0f, wide);
+      }
+      if (r < span.y && p.lse != nullptr)
+        p.lse[(int64_t)h * p.Tq + r] = sees && total != 0.0f ? kLn2 * (fmaf(top, unit, log2f(total))) : -INFINITY;
+      uint32_t again = __ballot_sync(kAll, redo && r < span.y);
+      __syncwarp();
+      while (again != 0) {
+        const int i = __ffs(again) - 1;
+        again &= again - 1;
+        row_forward<T>(p, span.x + quarter * 32 + i, h);
+        __syncwarp();
+      }
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
+  }
+}
+
+// --------------------------------------------------------------- backward
+// Two kernels of one form, and no atomics: the same bits every time.  KEYS false: a CTA's 128 rows are queries of one
+// head, it goes over blocks of 64 keys and sums dq.  KEYS true: its rows are keys of one key head, it goes over blocks
+// of 64 queries of every head that shares it and sums dk and dv.  With (A1, A2) the resident tiles and (B1, B2) the
+// blocks, (Q, dO) and (K, V) or the other way round, a block is
+//
+//   S = A1 B1^T   dP = A2 B2^T   p = exp(s - lse)   e = p (dP - delta) (1 - tanh^2)   acc += e B1   [dv += p B2]
+//
+// seven products for both where one kernel that adds dq by atomics has five.  e and p go to the second products as
+// 16-bit values out of TMEM.  In fp16 they are brought into the type's range first: p by 2^15, e by that and the power
+// of two that keeps |dP - delta| under 1 (from the largest norms of a row of dO and of V).
+template <int DP, bool KEYS>
+struct Backward {
+  static constexpr int kChunks = DP / 64;
+  static constexpr int kABytes = kTile * 128 * kChunks;   // each of A1, A2
+  static constexpr int kBBytes = kBlock * 128 * kChunks;  // each of B1, B2
+  static constexpr int kStages = 3;
+  static constexpr int kSmem = 1024 + 2 * kABytes + 2 * kStages * kBBytes;
+  static constexpr int kSets = DP == 64 ? 1 : 2;          // warps that share 32 rows: each takes half of a block's columns
+  static constexpr int kRowThreads = 128 * kSets, kThreads = 32 + kRowThreads;
+  static constexpr int kCtas = DP == 64 ? 2 : 1;
+  // TMEM: S, dP, then the sums; the 16-bit values beside them (the next S and dP are then computed meanwhile) or in
+  // place of S and dP, where two CTAs of 256 columns leave no room
+  static constexpr int kAccAt = 128, kAcc2At = 128 + DP;
+  static constexpr bool kApart = !(DP == 64 && KEYS);
+  static constexpr int kEAt = !kApart ? 64 : KEYS ? kAcc2At + DP : kAcc2At;
+  static constexpr int kPAt = kApart ? kEAt + 32 : 0;     // (KEYS)
+  static constexpr int kTmemCols = DP == 64 ? 256 : 512;
+};
+
+template <typename T, int DP, bool KEYS>
+__global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEYS>::kCtas)
+    backward_kernel(const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmA2,
+                    const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmB2,
+                    const __grid_constant__ Params p) {
+  using C = Backward<DP, KEYS>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sA1 = smem;
+  uint8_t* sA2 = sA1 + C::kABytes;
+  uint8_t* sB1 = sA2 + C::kABytes;
+  uint8_t* sB2 = sB1 + C::kStages * C::kBBytes;
+  __shared__ __align__(8) uint64_t afull, bfull[C::kStages], sfull, sfree, ready, done, drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word, s_lo[4], s_hi[4], s_bad[kTile];
+  // of the block's queries (KEYS), for this block and the next: lse and delta, interval and place; whether all see all keys
+  __shared__ float2 s_lse[2][KEYS ? kBlock : 1];
+  __shared__ int4 s_row[2][KEYS ? kBlock : 1];
+  __shared__ int s_all[2][2];
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = blockIdx.y, tile = KEYS ? blockIdx.x : gridDim.x - 1 - blockIdx.x;
+
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&afull), 1);
+    for (int s = 0; s < C::kStages; ++s) mbar_init(smem_u32(&bfull[s]), 1);
+    mbar_init(smem_u32(&sfull), 1);
+    mbar_init(smem_u32(&sfree), C::kRowThreads);
+    mbar_init(smem_u32(&ready), C::kRowThreads);
+    mbar_init(smem_u32(&done), 1);
+    mbar_init(smem_u32(&drained), 1);
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (threadIdx.x < kTile) s_bad[threadIdx.x] = 0;
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int2 span = tile_rows(KEYS ? p.k_off : p.q_off, p.off64, p.S, KEYS ? p.Tk : p.Tq, tile, p.by_segment);
+  const int quarter = warp & 3, set = (warp - 1) >> 2;
+  const int r = span.x + quarter * 32 + lane;  // the thread's query or key
+  int4 row = make_int4(0, 0, 0, 0);
+  if (KEYS) {
+    if (threadIdx.x == 32) {
+      int lo = INT_MAX, hi = 0;
+      if (span.y > span.x) {
+        // queries of the segments from the first key's to the last key's
+        const int sa = max(segment_of(p.k_off, p.off64, p.S, p.Tk, span.x), 0), sb = segment_of(p.k_off, p.off64, p.S, p.Tk, span.y - 1);
+        if (sb >= 0) {
+          const int q0 = offset_at(p.q_off, p.off64, sa, p.Tq), k0 = offset_at(p.k_off, p.off64, sa, p.Tk);
+          const int n = max(0, offset_at(p.q_off, p.off64, sa + 1, p.Tq) - q0), m = max(0, offset_at(p.k_off, p.off64, sa + 1, p.Tk) - k0);
+          lo = q0;
+          hi = offset_at(p.q_off, p.off64, sb + 1, p.Tq);
+          if (p.causal) {
+            const int seen = p.prefix != nullptr ? (int)min(max(entry(p.prefix, p.off64, sa), (int64_t)0), (int64_t)m) : 0;
+            if (span.x - k0 >= seen) lo = q0 + min(max(span.x - k0 - m + n, 0), n);  // the first that sees the first key
+          }
+        }
+      }
+      s_lo[0] = s_lo[1] = s_lo[2] = s_lo[3] = lo;
+      s_hi[0] = s_hi[1] = s_hi[2] = s_hi[3] = hi;
+    }
+  } else if (warp >= 1 && warp < 5) {
+    if (r < span.y) row = __ldg(p.rows + r);
+    int lo = row.y > row.x ? row.x : INT_MAX, hi = row.y > row.x ? row.y : 0;
+    lo = __reduce_min_sync(kAll, lo);
+    hi = __reduce_max_sync(kAll, hi);
+    if (lane == 0) {
+      s_lo[quarter] = lo;
+      s_hi[quarter] = hi;
+    }
+  } else if (warp >= 5) {
+    if (r < span.y) row = __ldg(p.rows + r);
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int other0 = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), other1 = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+  const int each = other1 > other0 ? (other1 - other0 + kBlock - 1) / kBlock : 0;  // blocks of a head
+  const int blocks = KEYS ? each * p.G : each;
+  const int up = std::is_same<T, __half>::value ? 15 : 0;
+  float sigma = 1.0f;
+  if (up != 0) {
+    const float bound = 2.0f * __uint_as_float(p.peaks[0]) * __uint_as_float(p.peaks[1]);  // of |dP - delta|
+    const int e = (int)(__float_as_uint(bound) >> 23) - 126;                             // bound < 2^e
+    if (bound > 0.0f && bound < INFINITY) sigma = __uint_as_float((uint32_t)min(max(127 - e, 1), 254) << 23);
+  }
+
+  if (warp == 0) {
+    if (lane == 0 && blocks > 0) {
+      // -------------------------------------------------- copies and MMAs
+      constexpr uint32_t idesc_s = idesc_of<T>(kBlock, false), idesc_o = idesc_of<T>(DP, true);
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(smem_u32(bar), parity, kWaitTimeoutMma, abort_flag); };
+      auto slot = [](int n) { return n % C::kStages; };
+      auto phase = [](int n) { return (uint32_t)(n / C::kStages) & 1u; };
+      int asked = 0;
+      auto ask = [&] {
+        if (asked >= blocks) return;
+        const int n = asked++, at = other0 + (KEYS ? n % each : n) * kBlock, h = KEYS ? head * p.G + n / each : head / p.G;
+        const uint32_t bar = smem_u32(&bfull[slot(n)]);
+        mbar_arrive_expect_tx(bar, 2 * C::kBBytes);
+        for (int c = 0; c < C::kChunks; ++c) {
+          tma_load_3d(smem_u32(sB1 + slot(n) * C::kBBytes + c * kBlock * 128), &tmB1, 64 * c, h, at, bar);
+          tma_load_3d(smem_u32(sB2 + slot(n) * C::kBBytes + c * kBlock * 128), &tmB2, 64 * c, h, at, bar);
+        }
+      };
+      const uint32_t ab = smem_u32(&afull);
+      mbar_arrive_expect_tx(ab, 2 * C::kABytes);
+      for (int c = 0; c < C::kChunks; ++c) {
+        tma_load_3d(smem_u32(sA1 + c * kTile * 128), &tmA1, 64 * c, head, span.x, ab);
+        tma_load_3d(smem_u32(sA2 + c * kTile * 128), &tmA2, 64 * c, head, span.x, ab);
+      }
+      for (int s = 0; s < C::kStages; ++s) ask();
+      const int steps = (p.D + 15) / 16;
+      auto products = [&](int n) {  // S and dP
+        if (!wait(&bfull[slot(n)], phase(n))) return false;
+        tc::tc_fence_after();
+        const uint64_t a1 = rows_desc(smem_u32(sA1)), a2 = rows_desc(smem_u32(sA2));
+        const uint64_t b1 = rows_desc(smem_u32(sB1 + slot(n) * C::kBBytes)), b2 = rows_desc(smem_u32(sB2 + slot(n) * C::kBBytes));
+        for (int i = 0; i < steps; ++i) {
+          const uint64_t a = (uint64_t)((i >> 2) * (kTile * 128 / 16) + (i & 3) * 2), b = (uint64_t)((i >> 2) * (kBlock * 128 / 16) + (i & 3) * 2);
+          mma_ss(tmem, a1 + a, b1 + b, idesc_s, i > 0);
+          mma_ss(tmem + 64, a2 + a, b2 + b, idesc_s, i > 0);
+        }
+        tc::umma_commit(smem_u32(&sfull));
+        return true;
+      };
+      bool ok = wait(&afull, 0) && products(0);
+      for (int n = 0; n < blocks && ok; ++n) {
+        if (C::kApart && n + 1 < blocks) {
+          ok = wait(&sfree, (uint32_t)n & 1u);
+          if (ok) tc::tc_fence_after();
+          ok = ok && products(n + 1);
+        }
+        ok = ok && wait(&ready, (uint32_t)n & 1u);
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (C::kApart && n > 0) ask();  // (what is ready was written after the products before had ended)
+        const uint64_t b1 = columns_desc(smem_u32(sB1 + slot(n) * C::kBBytes), kBlock * 128);
+        const uint64_t b2 = columns_desc(smem_u32(sB2 + slot(n) * C::kBBytes), kBlock * 128);
+        for (int i = 0; i < kBlock / 16; ++i) {
+          if (KEYS) mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + 8 * i, b2 + (uint64_t)(i * 16 * 128 / 16), idesc_o, n > 0 || i > 0);
+          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + 8 * i, b1 + (uint64_t)(i * 16 * 128 / 16), idesc_o, n > 0 || i > 0);
+        }
+        tc::umma_commit(smem_u32(&done));
+        if (!C::kApart && n + 1 < blocks) {
+          ok = wait(&done, (uint32_t)n & 1u);
+          if (ok) {
+            ask();
+            ok = products(n + 1);
+          }
+        }
+      }
+      if (!ok) {  // given up: no MMA in flight behind this CTA
+        tc::umma_commit(smem_u32(&drained));
+        mbar_wait_bounded(smem_u32(&drained), 0, kWaitTimeoutMma, nullptr);
+      }
+      // nor a copy
+      mbar_wait_bounded(ab, 0, kWaitTimeoutProducer, nullptr);
+      for (int i = max(0, asked - C::kStages); i < asked; ++i) mbar_wait_bounded(smem_u32(&bfull[slot(i)]), phase(i), kWaitTimeoutProducer, nullptr);
+    }
+  } else {
+    // -------------------------------------------------------------- rows
+    const int t = threadIdx.x - 32;
+    const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
+    float unit = p.cap > 0.0f ? 1.0f : p.scale * kLog2e, slope2 = 0.0f, lse = 0.0f, delta = 0.0f;
+    if (!KEYS) {
+      slope2 = p.slopes != nullptr ? kLog2e * __ldg(p.slopes + head) : 0.0f;
+      lse = r < span.y ? lse_of(p, r, head) - up : INFINITY;
+      delta = r < span.y ? sigma * __ldg(p.delta + (int64_t)head * p.Tq + r) : 0.0f;
+    }
+    // a block's queries, by the first two warps of the rows: from memory, then to shared memory
+    float2 next_lse = make_float2(INFINITY, 0.0f);
+    int4 next_row = make_int4(0, 0, 0, 0);
+    auto fetch = [&](int n) {
+      if (t >= kBlock) return;
+      const int i = other0 + (n % each) * kBlock + t, h = head * p.G + n / each;
+      const bool there = i < other1;
+      next_row = there ? __ldg(p.rows + i) : make_int4(0, 0, 0, 0);
+      next_lse = there ? make_float2(lse_of(p, i, h) - up, sigma * __ldg(p.delta + (int64_t)h * p.Tq + i)) : make_float2(INFINITY, 0.0f);
+    };
+    auto deposit = [&](int n) {
+      if (t < kBlock) {
+        s_lse[n & 1][t] = next_lse;
+        s_row[n & 1][t] = next_row;
+        const bool all = __all_sync(kAll, next_row.x <= span.x && next_row.y >= span.y);
+        if (lane == 0) s_all[n & 1][t >> 5] = all;
+      }
+    };
+    auto meet = [](bool good) { return rows_all<C::kRowThreads>(good); };
+    bool ok = true;
+    if (KEYS && blocks > 0) {
+      fetch(0);
+      deposit(0);
+      meet(true);
+      if (blocks > 1) fetch(1);
+    }
+    for (int n = 0; n < blocks && ok; ++n) {
+      const int o0 = other0 + (KEYS ? n % each : n) * kBlock;
+      if (KEYS) slope2 = p.slopes != nullptr ? kLog2e * __ldg(p.slopes + head * p.G + n / each) : 0.0f;
+      ok = mbar_wait_bounded(smem_u32(&sfull), (uint32_t)n & 1u, kWaitTimeoutEpilogue, abort_flag);
+      ok = __all_sync(kAll, ok);
+      tc::tc_fence_after();
+      const bool all = KEYS ? s_all[n & 1][0] && s_all[n & 1][1] : __all_sync(kAll, row.x <= o0 && row.y >= o0 + kBlock);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (!ok || (C::kSets == 2 && half != set)) continue;
+        const int c0 = half * 32;
+        uint32_t x[32], y[32];
+        tmem_get32(mine + c0, x);
+        tmem_get32(mine + 64 + c0, y);
+        tmem_wait_ld();
+        if (C::kApart && (C::kSets == 2 || half == 1)) {
+          tc::tc_fence_before();
+          mbar_arrive(smem_u32(&sfree));
+        }
+        uint32_t w[16], e[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          float pw[2], ew[2];
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            float v = __uint_as_float(x[c + d]), slant = 1.0f;
+            float2 ld;
+            if (KEYS) ld = s_lse[n & 1][c0 + c + d];
+            else ld = make_float2(lse, delta);
+            if (p.cap > 0.0f) {
+              const float th = tanh_of(v * (p.scale / p.cap));
+              slant = fmaf(-th, th, 1.0f);
+              v = p.cap * kLog2e * th;
+            }
+            if (slope2 != 0.0f) {
+              const int far = KEYS ? s_row[n & 1][c0 + c + d].z - r : row.z - (o0 + c0 + c + d);
+              v = fmaf(-slope2, fabsf((float)far), v * unit) - ld.x;
+            } else {
+              v = fmaf(v, unit, -ld.x);
+            }
+            pw[d] = exp2_fast(v);
+            ew[d] = pw[d] * fmaf(__uint_as_float(y[c + d]), sigma, -ld.y) * slant;
+            if (!all) {
+              bool sees;
+              if (KEYS) {
+                const int4 q = s_row[n & 1][c0 + c + d];
+                sees = r >= q.x && r < q.y;
+              } else {
+                const int j = o0 + c0 + c + d;
+                sees = j >= row.x && j < row.y;
+              }
+              pw[d] = sees ? pw[d] : 0.0f;
+              ew[d] = sees ? ew[d] : 0.0f;
+            }
+          }
+          if (KEYS) w[c / 2] = pack2<T>(pw[0], pw[1]);
+          e[c / 2] = pack2<T>(ew[0], ew[1]);
+        }
+        if (C::kApart && n > 0 && (C::kSets == 2 || half == 0)) {  // the products before have read their values
+          ok = mbar_wait_bounded(smem_u32(&done), (uint32_t)(n - 1) & 1u, kWaitTimeoutEpilogue, abort_flag);
+          ok = __all_sync(kAll, ok);
+          tc::tc_fence_after();
+        }
+        if (ok) {
+          if (KEYS) tmem_put16(mine + C::kPAt + c0 / 2, w);
+          tmem_put16(mine + C::kEAt + c0 / 2, e);
+        }
+      }
+      if (ok) {
+        tmem_wait_st();
+        tc::tc_fence_before();
+        mbar_arrive(smem_u32(&ready));
+      }
+      if (KEYS && n + 1 < blocks) {  // (a give-up is everyone's: all meet here)
+        deposit(n + 1);
+        ok = meet(ok);
+        if (n + 2 < blocks) fetch(n + 2);
+      }
+    }
+    if (ok && blocks > 0) {
+      ok = mbar_wait_bounded(smem_u32(&done), (uint32_t)(blocks - 1) & 1u, kWaitTimeoutEpilogue, abort_flag);
+      tc::tc_fence_after();
+    }
+    ok = meet(ok);
+    // a row that is not finite is taken again by itself; the sums' columns are shared by the sets
+    const float down = up != 0 ? 0x1p-15f : 1.0f, w1 = p.scale * down / sigma;
+    const int heads = KEYS ? p.Hk : p.H;
+    const int64_t at = ((int64_t)r * heads + head) * p.D;
+    const bool mine_too = KEYS || row.y > row.x, there = r < span.y;
+    for (int pass = 0; pass < 2 && ok; ++pass) {
+      for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
+        T* out = static_cast<T*>(which ? p.dv : KEYS ? p.dk : p.dq);
+        const bool wide = p.D % 16 == 0 && aligned(out, 32);
+#pragma unroll 1
+        for (int c = 32 * set; c < p.D; c += 32 * C::kSets) {
+          uint32_t o[32];
+          __syncwarp();
+          if (blocks > 0) {
+            tmem_get32(mine + (which ? C::kAcc2At : C::kAccAt) + c, o);
+            tmem_wait_ld();
+          }
+          if (blocks == 0 || !mine_too) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+          if (pass == 0) {
+            if (there && !finite32(o)) s_bad[quarter * 32 + lane] = 1;
+          } else if (there && !s_bad[quarter * 32 + lane]) {
+            store_sums<T>(out + at + c, o, p.D - c, which ? down : w1, wide);
+          }
+        }
+      }
+      if (pass == 0) meet(true);
+    }
+    if (ok && set == 0) {
+      uint32_t again = __ballot_sync(kAll, there && s_bad[quarter * 32 + lane]);
+      while (again != 0) {
+        const int i = __ffs(again) - 1;
+        again &= again - 1;
+        if (KEYS) row_dkv<T>(p, span.x + quarter * 32 + i, head);
+        else row_dq<T>(p, span.x + quarter * 32 + i, head);
+        __syncwarp();
+      }
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------- host
+static int make_map(CUtensorMap* tm, const void* base, int D, int heads, int64_t T, int64_t t_stride, int64_t h_stride, int rows,
+                    CUtensorMapDataType dt) {
+  auto enc = tc::encode_fn();
+  if (enc == nullptr) return fail(RB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)T};
+  cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? h_stride : D) * 2, (cuuint64_t)(T > 1 ? t_stride : D) * 2};
+  cuuint32_t box[3] = {64, 1, (cuuint32_t)rows};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(tm, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(RB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return RB_OK;
+}
+
+// whether a tensor map can be made of it: 16-byte rows and strides (of the dimensions that have a second entry)
+static bool mappable(const void* base, int64_t T, int heads, int64_t t_stride, int64_t h_stride) {
+  auto fits = [](int64_t s) { return s > 0 && s % 8 == 0 && s < (int64_t)1 << 39; };
+  return aligned(base, 16) && (T <= 1 || fits(t_stride)) && (heads <= 1 || fits(h_stride));
+}
+
+template <typename K>
+static int launch(K kernel, dim3 grid, int threads, int smem, bool after, cudaStream_t st, const char* what, void** args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = after ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), args), what);
+}
+
+// Tiles by the packed order or by segment: which has fewer blocks of scores, were all segments alike.  By segment, every
+// segment has its own (partly empty) tiles; by the packed order a tile's rows see keys of several segments.
+static bool choose_by_segment(int64_t Tq, int64_t Tk, int64_t S) {
+  if (S <= 0) return false;
+  const double nq = (double)Tq / S, nk = (double)Tk / S;
+  const double own = S * std::ceil(nq / kTile) * std::ceil(nk / kBlock);
+  const double packed = std::ceil((double)Tq / kTile) * std::ceil(nk * (1.0 + kTile / std::max(nq, 1.0)) / kBlock);
+  return own < packed;
+}
+
+template <typename T, int DP>
+static int run_forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
+  using C = Forward<DP>;
+  static std::once_flag once[64];
+  int dev = 0, rc;
+  cudaGetDevice(&dev);
+  cudaError_t e = cudaSuccess;
+  std::call_once(once[dev & 63], [&] {
+    e = cudaFuncSetAttribute(forward_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  });
+  if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(attention forward_kernel)");
+  CUtensorMap tmQ, tmK, tmV;
+  if ((rc = make_map(&tmQ, p.q, p.D, p.H, p.Tq, p.q_t, p.q_h, kTile, dt))) return rc;
+  if ((rc = make_map(&tmK, p.k, p.D, p.Hk, p.Tk, p.k_t, p.k_h, kBlock, dt))) return rc;
+  if ((rc = make_map(&tmV, p.v, p.D, p.Hk, p.Tk, p.v_t, p.v_h, kBlock, dt))) return rc;
+  p.by_segment = choose_by_segment(p.Tq, p.Tk, p.S);
+  const int64_t tiles = p.by_segment ? p.Tq / kTile + p.S + 2 : ((int64_t)p.Tq + kTile - 1) / kTile;
+  void* args[] = {&tmQ, &tmK, &tmV, &p};
+  return launch(forward_kernel<T, DP>, dim3((unsigned)tiles, p.H), kThreads, C::kSmem, true, st, "attention forward_kernel launch", args);
+}
+
+static bool tiled(const Params& p) {
+  return p.D % 8 == 0 && p.D <= 128 && mappable(p.q, p.Tq, p.H, p.q_t, p.q_h) && mappable(p.k, p.Tk, p.Hk, p.k_t, p.k_h) &&
+         mappable(p.v, p.Tk, p.Hk, p.v_t, p.v_h);
+}
+
+template <typename T>
+static int forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
+  int rc;
+  rows_kernel<<<(p.Tq + 255) / 256, 256, 0, st>>>(p);
+  if ((rc = check_cuda(cudaGetLastError(), "attention rows_kernel launch"))) return rc;
+  if (tiled(p) && p.Tk > 0 && aligned(p.out, 16))
+    return p.D <= 64 ? run_forward<T, 64>(p, dt, st) : run_forward<T, 128>(p, dt, st);
+  void* args[] = {&p};
+  return launch(row_kernel<T, kRowForward>, dim3((unsigned)(((int64_t)p.Tq * p.H + 7) / 8)), 256, 0, true, st,
+                "attention row_kernel launch", args);
+}
+
+template <typename T, int DP, bool KEYS>
+static int run_backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
+  using C = Backward<DP, KEYS>;
+  static std::once_flag once[64];
+  int dev = 0, rc;
+  cudaGetDevice(&dev);
+  cudaError_t e = cudaSuccess;
+  std::call_once(once[dev & 63], [&] {
+    e = cudaFuncSetAttribute(backward_kernel<T, DP, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  });
+  if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(attention backward_kernel)");
+  const int q_rows = KEYS ? kBlock : kTile, k_rows = KEYS ? kTile : kBlock;
+  CUtensorMap q, g, k, v;
+  if ((rc = make_map(&q, p.q, p.D, p.H, p.Tq, p.q_t, p.q_h, q_rows, dt))) return rc;
+  if ((rc = make_map(&g, p.g, p.D, p.H, p.Tq, p.g_t, p.g_h, q_rows, dt))) return rc;
+  if ((rc = make_map(&k, p.k, p.D, p.Hk, p.Tk, p.k_t, p.k_h, k_rows, dt))) return rc;
+  if ((rc = make_map(&v, p.v, p.D, p.Hk, p.Tk, p.v_t, p.v_h, k_rows, dt))) return rc;
+  const int64_t total = KEYS ? p.Tk : p.Tq;
+  p.by_segment = KEYS ? choose_by_segment(p.Tk, p.Tq, p.S) : choose_by_segment(p.Tq, p.Tk, p.S);
+  const int64_t tiles = p.by_segment ? total / kTile + p.S + 2 : (total + kTile - 1) / kTile;
+  void* args[] = {KEYS ? &k : &q, KEYS ? &v : &g, KEYS ? &q : &k, KEYS ? &g : &v, &p};
+  return launch(backward_kernel<T, DP, KEYS>, dim3((unsigned)tiles, KEYS ? p.Hk : p.H), C::kThreads, C::kSmem, true, st,
+                "attention backward_kernel launch", args);
+}
+
+template <typename T>
+static int backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
+  int rc;
+  const bool peaks = std::is_same<T, __half>::value;
+  if (peaks && (rc = check_cuda(cudaMemsetAsync(p.peaks, 0, 8, st), "attention peaks"))) return rc;
+  const int64_t warps = (int64_t)p.Tq * p.H + (peaks ? (int64_t)p.Tk * p.Hk : 0);
+  if (warps > 0) {
+    delta_kernel<T><<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(p);
+    if ((rc = check_cuda(cudaGetLastError(), "attention delta_kernel launch"))) return rc;
+  }
+  const bool tiles = tiled(p) && p.Tq > 0 && p.Tk > 0 && mappable(p.g, p.Tq, p.H, p.g_t, p.g_h) && aligned(p.dq, 16) &&
+                     aligned(p.dk, 16) && aligned(p.dv, 16);
+  if (tiles) {
+    if ((rc = p.D <= 64 ? run_backward<T, 64, true>(p, dt, st) : run_backward<T, 128, true>(p, dt, st))) return rc;
+    return p.D <= 64 ? run_backward<T, 64, false>(p, dt, st) : run_backward<T, 128, false>(p, dt, st);
+  }
+  void* args[] = {&p};
+  if (p.Tk > 0 && (rc = launch(row_kernel<T, kRowDkv>, dim3((unsigned)(((int64_t)p.Tk * p.Hk + 7) / 8)), 256, 0, false, st,
+                               "attention row_kernel launch", args)))
+    return rc;
+  if (p.Tq == 0) return RB_OK;
+  return launch(row_kernel<T, kRowDq>, dim3((unsigned)(((int64_t)p.Tq * p.H + 7) / 8)), 256, 0, false, st,
+                "attention row_kernel launch", args);
+}
+
+static int check(const Params& p, int dtype, int64_t Tq, int64_t Tk, int64_t S, int idx_dtype) {
+  if (Tq < 0 || Tk < 0 || S < 0 || p.H <= 0 || p.Hk <= 0 || p.D <= 0) return fail(RB_ERR_VALUE, "negative or empty attention shape");
+  if (dtype != RB_BF16 && dtype != RB_F16) return fail(RB_ERR_UNSUPPORTED, "attention takes bf16 or f16");
+  if (idx_dtype != RB_I64 && idx_dtype != RB_I32) return fail(RB_ERR_VALUE, "offsets must be int64 or int32");
+  if (p.H % p.Hk != 0) return fail(RB_ERR_VALUE, "%d query heads cannot share %d key heads", p.H, p.Hk);
+  if (p.D > kMaxWidth) return fail(RB_ERR_UNSUPPORTED, "heads wider than %d", kMaxWidth);
+  if (Tq > 1 << 30 || Tk > 1 << 30 || S > 1 << 30 || p.H > 65535) return fail(RB_ERR_UNSUPPORTED, "more than 2^30 tokens or segments, or 65535 heads");
+  if (!(p.scale > 0.0f) || !(p.scale < INFINITY)) return fail(RB_ERR_VALUE, "scale must be positive");
+  if (!(p.cap >= 0.0f) || !(p.cap < INFINITY)) return fail(RB_ERR_VALUE, "cap must be positive, or 0 for none");
+  return RB_OK;
+}
+
+}  // namespace attn
+}  // namespace rb
+
+using namespace rb;
+
+extern "C" int64_t rb_segment_attention_workspace_size(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D) {
+  if (Tq < 0 || Tk < 0 || S < 0 || H <= 0 || Hk <= 0 || D <= 0 || Tq > 1 << 30) return -1;
+  return Tq * 16;
+}
+
+extern "C" int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h,
+                                    const void* v, int64_t v_t, int64_t v_h, int dtype, int64_t Tq, int64_t Tk, int H, int Hk,
+                                    int D, const void* q_offsets, const void* k_offsets, const void* prefix, int idx_dtype,
+                                    int64_t S, int causal, const float* slopes, float cap, float scale, void* workspace,
+                                    int64_t workspace_bytes, void* out, float* lse, void* stream) {
+  using namespace rb::attn;
+  Params p{};
+  p.H = H;
+  p.Hk = Hk;
+  p.D = D;
+  p.scale = scale;
+  p.cap = cap;
+  int rc;
+  if ((rc = check(p, dtype, Tq, Tk, S, idx_dtype))) return rc;
+  if (Tq > 0 && (q == nullptr || out == nullptr || (S > 0 && (q_offsets == nullptr || k_offsets == nullptr))))
+    return fail(RB_ERR_VALUE, "null operand");
+  if (Tk > 0 && (k == nullptr || v == nullptr)) return fail(RB_ERR_VALUE, "null operand");
+  const int64_t need = rb_segment_attention_workspace_size(Tq, Tk, S, H, Hk, D);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(RB_ERR_VALUE, "workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need,
+                (long long)workspace_bytes);
+  if (!device_is_sm100()) return fail(RB_ERR_DEVICE, "rb_segment_attention needs an sm_100 (B200) device");
+  if (Tq == 0) return RB_OK;
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.out = out;
+  p.lse = lse;
+  p.rows = static_cast<int4*>(workspace);
+  p.q_off = q_offsets;
+  p.k_off = k_offsets;
+  p.prefix = prefix;
+  p.slopes = slopes;
+  p.q_t = q_t;
+  p.q_h = q_h;
+  p.k_t = k_t;
+  p.k_h = k_h;
+  p.v_t = v_t;
+  p.v_h = v_h;
+  p.Tq = (int)Tq;
+  p.Tk = (int)Tk;
+  p.S = (int)S;
+  p.G = H / Hk;
+  p.off64 = idx_dtype == RB_I64;
+  p.causal = causal != 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  return dtype == RB_BF16 ? forward<__nv_bfloat16>(p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, st)
+                          : forward<__half>(p, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, st);
+}
+
+extern "C" int64_t rb_segment_attention_backward_workspace_size(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D) {
+  if (Tq < 0 || Tk < 0 || S < 0 || H <= 0 || Hk <= 0 || D <= 0 || Tq > 1 << 30) return -1;
+  return 16 + Tq * 16 + (int64_t)H * Tq * 4;
+}
+
+extern "C" int rb_segment_attention_backward(const void* grad, int64_t g_t, int64_t g_h, const void* q, int64_t q_t, int64_t q_h,
+                                             const void* k, int64_t k_t, int64_t k_h, const void* v, int64_t v_t, int64_t v_h,
+                                             const void* out, const float* lse, int dtype, int64_t Tq, int64_t Tk, int H, int Hk,
+                                             int D, const void* q_offsets, const void* k_offsets, const void* prefix,
+                                             int idx_dtype, int64_t S, int causal, const float* slopes, float cap, float scale,
+                                             void* workspace, int64_t workspace_bytes, void* dq, void* dk, void* dv, void* stream) {
+  using namespace rb::attn;
+  Params p{};
+  p.H = H;
+  p.Hk = Hk;
+  p.D = D;
+  p.scale = scale;
+  p.cap = cap;
+  int rc;
+  if ((rc = check(p, dtype, Tq, Tk, S, idx_dtype))) return rc;
+  if (S > 0 && (q_offsets == nullptr || k_offsets == nullptr)) return fail(RB_ERR_VALUE, "null offsets");
+  if (Tq > 0 && (grad == nullptr || q == nullptr || out == nullptr || lse == nullptr || dq == nullptr)) return fail(RB_ERR_VALUE, "null operand");
+  if (Tk > 0 && (k == nullptr || v == nullptr || dk == nullptr || dv == nullptr)) return fail(RB_ERR_VALUE, "null operand");
+  const int64_t need = rb_segment_attention_backward_workspace_size(Tq, Tk, S, H, Hk, D);
+  if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16))
+    return fail(RB_ERR_VALUE, "workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need,
+                (long long)workspace_bytes);
+  if (!device_is_sm100()) return fail(RB_ERR_DEVICE, "rb_segment_attention_backward needs an sm_100 (B200) device");
+  p.g = grad;
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.o = out;
+  p.lse = const_cast<float*>(lse);
+  p.dq = dq;
+  p.dk = dk;
+  p.dv = dv;
+  p.peaks = static_cast<uint32_t*>(workspace);
+  p.rows = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + 16);
+  p.delta = reinterpret_cast<float*>(p.rows + Tq);
+  p.q_off = q_offsets;
+  p.k_off = k_offsets;
+  p.prefix = prefix;
+  p.slopes = slopes;
+  p.g_t = g_t;
+  p.g_h = g_h;
+  p.q_t = q_t;
+  p.q_h = q_h;
+  p.k_t = k_t;
+  p.k_h = k_h;
+  p.v_t = v_t;
+  p.v_h = v_h;
+  p.Tq = (int)Tq;
+  p.Tk = (int)Tk;
+  p.S = (int)S;
+  p.G = H / Hk;
+  p.off64 = idx_dtype == RB_I64;
+  p.causal = causal != 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  return dtype == RB_BF16 ? backward<__nv_bfloat16>(p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, st)
+                          : backward<__half>(p, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, st);
+}

@@ -8,4 +8,7 @@
 #include "route.cu"
 #include "block_norm.cu"
 #include "low_rank.cu"
+#include "attention.cu"
+#include "embedding.cu"
+#include "clip.cu"
 #include "peer.cu"

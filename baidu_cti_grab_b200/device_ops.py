@@ -500,6 +500,7 @@ def smoe_experts(x: torch.Tensor, topk_idx: torch.Tensor, topk_score: torch.Tens
 
 # ------------------------------------------------------- routing to experts
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_INDEX = {torch.int32: L.RB_I32, torch.int64: L.RB_I64}
 _SCORES = {"softmax": L.RB_SCORE_SOFTMAX, "sigmoid": L.RB_SCORE_SIGMOID}
 
 
@@ -820,6 +821,319 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
              rank, adapter.data_ptr(), L.RB_I64 if adapter.dtype is torch.int64 else L.RB_I32, _ptr(scale), _ptr(ws), ws_bytes,
              out.data_ptr(), ldo)
     return out
+
+
+# ------------------------------------------------- attention within segments
+_HALVES = (torch.bfloat16, torch.float16)
+
+
+def _heads_of(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """t [T, heads, D] with contiguous columns on 16-byte rows (a copy only where it has none), and its strides."""
+    T, heads, D = t.shape
+    st, sh, sd = t.stride()
+    if (sd != 1 and D > 1) or (D % 8 == 0 and (t.data_ptr() % 16 or (T > 1 and (st % 8 or st <= 0))
+                                               or (heads > 1 and (sh % 8 or sh <= 0)))):
+        t = t.clone(memory_format=torch.contiguous_format)  # (a contiguous one may start off 16 bytes)
+        st, sh = heads * D, D
+    return t, st, sh
+
+
+def _attention_args(name, q, k, v, offsets, k_offsets, causal, prefix, slopes, cap, scale):
+    """What both directions check: (device, strided q, k and v, sizes and mask arguments of the entry points)."""
+    dev = _device_of(name, q, k, v, offsets, k_offsets, prefix, slopes)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
+        raise ValueError(f"{name} expects q [Tq, H, D] and k, v [Tk, Hk, D]")
+    (Tq, H, D), (Tk, Hk, _) = q.shape, k.shape
+    dtype = q.dtype
+    if dtype not in _HALVES or k.dtype is not dtype or v.dtype is not dtype:
+        raise ValueError("q, k and v must all be bf16 or all f16")
+    if k.shape[2] != D or Hk == 0 or H % Hk:
+        raise ValueError(f"k and v must be [Tk, Hk, {D}] with Hk a divisor of {H}")
+    if k_offsets is None:
+        if Tq != Tk:
+            raise ValueError("without k_offsets there must be as many keys as queries")
+        k_offsets = offsets
+    idx = _INDEX.get(offsets.dtype)
+    if idx is None or offsets.dim() != 1 or offsets.numel() < 1 or k_offsets.shape != offsets.shape \
+            or k_offsets.dtype is not offsets.dtype:
+        raise ValueError("offsets (and k_offsets, alike) must be int32 or int64 [segments + 1]")
+    S = offsets.numel() - 1
+    if prefix is not None:
+        if prefix.shape != (S,) or prefix.dtype not in _INDEX:
+            raise ValueError(f"prefix must be int32 or int64 [{S}]")
+        prefix = prefix.to(offsets.dtype).contiguous()
+    if slopes is not None:
+        if slopes.shape != (H,) or slopes.dtype is not torch.float32:
+            raise ValueError(f"slopes must be fp32 [{H}]")
+        slopes = slopes.contiguous()
+    scale = D ** -0.5 if scale is None else float(scale)
+    q, k, v = _heads_of(q), _heads_of(k), _heads_of(v)
+    offsets, k_offsets = offsets.contiguous(), k_offsets.contiguous()
+    sizes = (_DT[dtype], Tq, Tk, H, Hk, D)
+    mask = (offsets, k_offsets, prefix, idx, S, bool(causal), slopes, float(cap), scale)
+    return dev, q, k, v, sizes, mask
+
+
+def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
+                      k_offsets: Optional[torch.Tensor] = None, *, causal: bool = True,
+                      prefix: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None, cap: float = 0.0,
+                      scale: Optional[float] = None, want_lse: bool = False):
+    """Attention within packed segments (rb_segment_attention): softmax over the keys of a query's own segment.
+
+    q [Tq, H, D], k and v [Tk, Hk, D] bf16/f16 (views of one projection do; Hk divides H), D <= 256; segment s has
+    queries offsets[s] .. offsets[s + 1] and keys k_offsets[s] .. (default: the same rows).  Query i of n sees key j of m
+    if not `causal`, if j <= i + m - n, or if j < prefix[s].  Scores are scale q.k (default D ** -0.5), with `cap` > 0
+    cap tanh(. / cap), with fp32 slopes [H] less slopes[h] |i + m - n - j|.  A query that sees nothing (rows outside
+    every segment among them) gets zeros.  Returns (out [Tq, H, D], lse fp32 [H, Tq] or None)."""
+    dev, (q, qt, qh), (k, kt, kh), (v, vt, vh), sizes, mask = _attention_args(
+        "segment_attention", q, k, v, offsets, k_offsets, causal, prefix, slopes, cap, scale)
+    _, Tq, Tk, H, Hk, D = sizes
+    off, k_off, prefix, idx, S, causal, slopes, cap, scale = mask
+    out = torch.empty((Tq, H, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((H, Tq), dtype=torch.float32, device=dev) if want_lse else None
+    ws_bytes = _plan_bytes(dev, "rb_segment_attention_workspace_size", Tq, Tk, S, H, Hk, D)
+    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+    _call_on(dev, "rb_segment_attention", q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, *sizes,
+             off.data_ptr(), k_off.data_ptr(), _ptr(prefix), idx, S, causal, _ptr(slopes), cap, scale, ws.data_ptr(), ws_bytes,
+             out.data_ptr(), _ptr(lse))
+    return out, lse
+
+
+def segment_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                               lse: torch.Tensor, offsets: torch.Tensor, k_offsets: Optional[torch.Tensor] = None, *,
+                               causal: bool = True, prefix: Optional[torch.Tensor] = None,
+                               slopes: Optional[torch.Tensor] = None, cap: float = 0.0, scale: Optional[float] = None):
+    """Gradients (q [Tq, H, D], k, v [Tk, Hk, D]) of segment_attention (rb_segment_attention_backward) from that of its
+    output and the forward call's inputs, output and lse.  The same bits every time; slopes get no gradient."""
+    dev, (q, qt, qh), (k, kt, kh), (v, vt, vh), sizes, mask = _attention_args(
+        "segment_attention_backward", q, k, v, offsets, k_offsets, causal, prefix, slopes, cap, scale)
+    _device_of("segment_attention_backward", q, grad, out, lse)
+    dtype, Tq, Tk, H, Hk, D = sizes
+    off, k_off, prefix, idx, S, causal, slopes, cap, scale = mask
+    for t in (grad, out):
+        if t.shape != (Tq, H, D) or t.dtype is not q.dtype:
+            raise ValueError(f"grad and out must be [{Tq}, {H}, {D}] in q's type")
+    if lse.shape != (H, Tq) or lse.dtype is not torch.float32 or not lse.is_contiguous():
+        raise ValueError(f"lse must be the forward call's fp32 [{H}, {Tq}]")
+    grad, gt, gh = _heads_of(grad)
+    out = out.contiguous()
+    dq = torch.empty((Tq, H, D), dtype=q.dtype, device=dev)
+    dk = torch.empty((Tk, Hk, D), dtype=q.dtype, device=dev)
+    dv = torch.empty_like(dk)
+    ws_bytes = _plan_bytes(dev, "rb_segment_attention_backward_workspace_size", Tq, Tk, S, H, Hk, D)
+    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+    _call_on(dev, "rb_segment_attention_backward", grad.data_ptr(), gt, gh, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh,
+             v.data_ptr(), vt, vh, out.data_ptr(), lse.data_ptr(), *sizes, off.data_ptr(), k_off.data_ptr(), _ptr(prefix), idx, S,
+             causal, _ptr(slopes), cap, scale, ws.data_ptr(), ws_bytes, dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+    return dq, dk, dv
+
+
+# ------------------------------------------- embedding rows and their gradient
+def embed_rows(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[ids] (rb_embed_rows): table [V, D] fp32/bf16/f16 with contiguous rows, ids int32/int64 of any
+    shape, clamped to [0, V - 1].  Returns [*ids.shape, D] in the table's type."""
+    dev = _device_of("embed_rows", table, ids)
+    if table.dim() != 2 or table.dtype not in _FLOATS or table.shape[1] == 0:
+        raise ValueError("embed_rows expects a table [V, D] in fp32, bf16 or f16")
+    if ids.dtype not in _INDEX:
+        raise ValueError("ids must be int32 or int64")
+    V, D = table.shape
+    table, ld = _rows_of(table, V, D)
+    out = torch.empty((*ids.shape, D), dtype=table.dtype, device=dev)
+    ids = ids.contiguous()
+    _call_on(dev, "rb_embed_rows", table.data_ptr(), _DT[table.dtype], ld, V, D, ids.data_ptr(), _INDEX[ids.dtype], ids.numel(),
+             float(scale), out.data_ptr(), D)
+    return out
+
+
+def _embed_grad_args(name, grad, ids, rows, bags, padding_idx):
+    """What both forms of the gradient check: (device, grad rows, their pitch, width, ids, bags, number of bags, padding)."""
+    dev = _device_of(name, grad, ids, bags)
+    if grad.dim() < 1 or grad.dtype not in _FLOATS or grad.shape[-1] == 0:
+        raise ValueError(f"{name} expects grad [..., D] in fp32, bf16 or f16")
+    if ids.dtype not in _INDEX:
+        raise ValueError("ids must be int32 or int64")
+    if rows < 0:
+        raise ValueError("the table cannot have a negative number of rows")
+    D = grad.shape[-1]
+    n_bags = 0
+    if bags is None:
+        if grad.shape[:-1] != ids.shape:
+            raise ValueError(f"grad must be [{', '.join(map(str, ids.shape))}, D]")
+    else:
+        if ids.dim() != 1 or bags.dim() != 1 or bags.numel() < 1 or bags.dtype not in _INDEX:
+            raise ValueError("with bags, ids are [n] and bags int32 or int64 [bags + 1]")
+        n_bags = bags.numel() - 1
+        if grad.shape != (n_bags, D):
+            raise ValueError(f"grad must be [{n_bags}, D], a row a bag")
+        bags = bags.to(ids.dtype).contiguous()
+    grad, ld = _rows2d(grad, D)
+    padding = -1
+    if padding_idx is not None:
+        if not 0 <= padding_idx < max(rows, 1):
+            raise ValueError(f"padding_idx must be in [0, {rows})")
+        padding = padding_idx
+    return dev, grad, ld, D, ids.contiguous(), bags, n_bags, padding
+
+
+def embed_rows_backward(grad: torch.Tensor, ids: torch.Tensor, rows: int, *, bags: Optional[torch.Tensor] = None,
+                        scale: float = 1.0, padding_idx: Optional[int] = None,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient [rows, D] of embed_rows' table (rb_embed_rows_backward): for each row scale times the sum of grad over the
+    ids that name it (clamped as the lookup clamps them), zeros where none does; the same bits every time.
+
+    grad [*ids.shape, D]; with `bags` (offsets [bags + 1] into ids [n]) grad [bags, D], every id taking its bag's row: the
+    gradient of sum-pooled bags, ids in no bag taking none.  Ids of padding_idx add nothing.  With `out` [rows, D] (any
+    float type) the sums are added to what it holds, rows that no id names being left as they were."""
+    dev, grad, ld, D, ids, bags, n_bags, padding = _embed_grad_args("embed_rows_backward", grad, ids, rows, bags, padding_idx)
+    given = out is not None
+    if not given:
+        out = torch.empty((rows, D), dtype=grad.dtype, device=dev)
+    else:
+        _device_of("embed_rows_backward", grad, out)
+        if out.shape != (rows, D) or out.dtype not in _FLOATS or (D > 1 and out.stride(1) != 1) \
+                or (rows > 1 and out.stride(0) < D):
+            raise ValueError(f"out must be a row-major [{rows}, {D}] tensor in fp32, bf16 or f16")
+    n = ids.numel()
+    ws_bytes = _plan_bytes(dev, "rb_embed_rows_backward_workspace_size", n, D)
+    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+    _call_on(dev, "rb_embed_rows_backward", grad.data_ptr(), _DT[grad.dtype], ld, D, ids.data_ptr(), _INDEX[ids.dtype], n, rows,
+             _ptr(bags), n_bags, padding, float(scale), given, ws.data_ptr(), ws_bytes, out.data_ptr(), _DT[out.dtype],
+             max(out.stride(0), D))
+    return out
+
+
+def embed_rows_backward_sparse(grad: torch.Tensor, ids: torch.Tensor, rows: int, *, bags: Optional[torch.Tensor] = None,
+                               scale: float = 1.0, padding_idx: Optional[int] = None,
+                               out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
+    """embed_rows_backward of the touched rows alone (rb_embed_rows_backward_sparse).
+
+    Returns (row ids int64 [n], ascending; their gradients [n, D]; count int32 [1] on the device): the first `count`
+    entries hold, those behind are left as they were (of fresh tensors: any values).  n is ids.numel(); `out` gives
+    both buffers, the gradients' in any float type."""
+    name = "embed_rows_backward_sparse"
+    dev, grad, ld, D, ids, bags, n_bags, padding = _embed_grad_args(name, grad, ids, rows, bags, padding_idx)
+    n = ids.numel()
+    if out is None:
+        out = torch.empty((n,), dtype=torch.int64, device=dev), torch.empty((n, D), dtype=grad.dtype, device=dev)
+    out_ids, out_rows = out
+    _device_of(name, grad, out_ids, out_rows)
+    if out_ids.shape != (n,) or out_ids.dtype is not torch.int64 or not out_ids.is_contiguous():
+        raise ValueError(f"out's ids must be contiguous int64 [{n}]")
+    if out_rows.shape != (n, D) or out_rows.dtype not in _FLOATS or (D > 1 and out_rows.stride(1) != 1) \
+            or (n > 1 and out_rows.stride(0) < D):
+        raise ValueError(f"out's rows must be a row-major [{n}, {D}] tensor in fp32, bf16 or f16")
+    count = torch.empty((1,), dtype=torch.int32, device=dev)
+    ws_bytes = _plan_bytes(dev, "rb_embed_rows_backward_workspace_size", n, D)
+    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+    _call_on(dev, "rb_embed_rows_backward_sparse", grad.data_ptr(), _DT[grad.dtype], ld, D, ids.data_ptr(), _INDEX[ids.dtype], n,
+             rows, _ptr(bags), n_bags, padding, float(scale), ws.data_ptr(), ws_bytes, out_ids.data_ptr(), out_rows.data_ptr(),
+             _DT[out_rows.dtype], max(out_rows.stride(0), D), count.data_ptr())
+    return out_ids, out_rows, count
+
+
+# ----------------------------------------------- the norm of all gradients
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t's values fill one run of memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    at = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != at:
+            return False
+        at *= size
+    return True
+
+
+def _gradients(name: str, grads):
+    """(tensors, row counts or None) of a list of gradients, pairs (rows, count) among them."""
+    tensors, counts = [], None
+    for i, g in enumerate(grads):
+        if isinstance(g, torch.Tensor):
+            tensors.append(g)
+            continue
+        rows, count = g
+        if rows.dim() != 2 or not rows.is_contiguous() or count.numel() != 1 or count.dtype is not torch.int32:
+            raise ValueError(f"{name}: counted rows are a contiguous [n, D] and an int32 [1]")
+        if counts is None:
+            counts = {}
+        counts[i] = count
+        tensors.append(rows)
+    return tensors, counts
+
+
+def _clip(name: str, grads, most: float, out, scale: float) -> torch.Tensor:
+    tensors, counts = _gradients(name, grads)
+    n = len(tensors)
+    if n == 0:
+        raise ValueError(f"{name} expects at least one gradient")
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise RuntimeError(f"{name} expects CUDA tensors")
+    index = dev.index
+    if {t.get_device() for t in tensors} != {index} or (counts and any(c.device != dev for c in counts.values())):
+        raise RuntimeError(f"{name}: tensors on different devices")
+    try:
+        types = [_GRAD_TYPES[t.dtype] for t in tensors]
+    except KeyError:
+        raise ValueError("gradients must be fp32, bf16 or f16") from None
+    clip = most >= 0.0
+    back = []  # (a copy, where it goes): gradients whose values lie apart
+    for i, t in enumerate(tensors):
+        if not t.is_contiguous() and not _dense(t):
+            tensors[i] = t.contiguous()
+            if clip and out is None:
+                back.append((tensors[i], t))
+    sizes = [t.numel() for t in tensors]
+    ptrs = [t.data_ptr() for t in tensors]
+    to = ptrs
+    if not clip:
+        to = None
+    elif out is not None:
+        if len(out) != n:
+            raise ValueError(f"out must have {n} tensors")
+        for o, t in zip(out, tensors):
+            if o.shape != t.shape or o.dtype is not t.dtype or o.get_device() != index or \
+                    not (o.is_contiguous() and t.is_contiguous() or (o.stride() == t.stride() and _dense(o))):
+                raise ValueError("out's tensors must be as the gradients, their values in one run of memory")
+        to = [o.data_ptr() for o in out]
+    if clip and len(set(to)) < n and len({a for a, m in zip(to, sizes) if m}) < sum(1 for m in sizes if m):
+        raise ValueError(f"{name}: a tensor to be clipped was given twice")
+    pointers, longs = ctypes.c_void_p * n, ctypes.c_int64 * n
+    counted = widths = None
+    if counts:
+        counted, widths = pointers(), longs()
+        for i, c in counts.items():
+            counted[i], widths[i] = c.data_ptr(), max(tensors[i].shape[1], 1)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws_bytes = _plan_bytes(dev, "rb_grad_norm_workspace_size", n)
+    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+    _call_on(dev, "rb_clip_grads", pointers(*ptrs), None if to is None else pointers(*to), longs(*sizes), (ctypes.c_int * n)(*types),
+             counted, widths, n, float(scale), float(most), ws.data_ptr(), ws_bytes, norm.data_ptr())
+    for copy, t in back:
+        t.copy_(copy)
+    return norm
+
+
+_GRAD_TYPES = {t: _DT[t] for t in _FLOATS}
+
+
+def grad_norm(grads, *, scale: float = 1.0) -> torch.Tensor:
+    """scale times the 2-norm of all values of `grads` together, fp32 [] on the device (rb_clip_grads without clipping).
+
+    Each gradient is a tensor (fp32, bf16, f16; any shape), or a pair (rows [n, D], count int32 [1]) of which the first
+    `count` rows count (what embed_rows_backward_sparse returns)."""
+    return _clip("grad_norm", list(grads), -1.0, None, scale)
+
+
+def clip_grads(grads, max_norm: float, *, out=None, scale: float = 1.0) -> torch.Tensor:
+    """Clip gradients by their norm together (rb_clip_grads): with norm = grad_norm(grads, scale=scale), each gradient
+    becomes scale * g * min(1, max_norm / (norm + 1e-6)), in place or in the tensors `out` (laid out as the gradients).
+    Returns the norm, which nothing waits for.  A norm of NaN makes all of them NaN, an infinite one zeros (and NaN where
+    they are infinite).  Tensors must not share memory."""
+    if not max_norm >= 0.0:
+        raise ValueError("max_norm must not be negative")
+    return _clip("clip_grads", list(grads), max_norm, None if out is None else list(out), scale)
 
 
 def device_error(reset: bool = False) -> int:

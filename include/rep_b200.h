@@ -414,6 +414,95 @@ int rb_low_rank_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int 
                     const float* scale, void* workspace, int64_t workspace_bytes, void* out, int64_t ldo,
                     void* stream);
 
+/*
+ * Attention within packed segments (an encoder's users, documents), with gradients:
+ *   x = scale q_i . k_j;  s = cap tanh(x / cap) if cap > 0, else x;  s -= slopes[h] |i + m - n - j|
+ *   seen(i, j) = not causal, or j <= i + m - n, or j < prefix[segment]
+ *   out_i = sum over seen j of softmax(s)_j v_j        (zeros where nothing is seen)
+ * for query i of n and key j of m of one segment; other segments are not seen.
+ *   q          [Tq, H, D] RB_BF16 or RB_F16, q_t and q_h elements from token to token
+ *              and from head to head, columns contiguous; D <= 256
+ *   k, v       [Tk, Hk, D] likewise; query head h takes key head h / (H / Hk)
+ *   q_offsets, k_offsets   [S + 1] RB_I32 or RB_I64, non-decreasing: segment s has the
+ *              rows offsets[s] .. offsets[s + 1] - 1.  Entries outside the rows are
+ *              taken as the nearest row; rows in no segment see nothing
+ *   prefix     [S] in the offsets' type, or NULL: a segment's first keys that all of
+ *              its queries see
+ *   slopes     [H] fp32 or NULL; cap 0: none; scale > 0
+ *   workspace  rb_segment_attention_workspace_size bytes (-1: bad shape), 16-byte
+ *              aligned; likewise for the backward call
+ *   out        [Tq, H, D] contiguous;  lse [H, Tq] fp32 or NULL: log of the sum of
+ *              exp(s), -inf where nothing is seen (the backward call takes it)
+ * The backward call takes the output's gradient (strided as q), the forward call's
+ * inputs, output and lse, and writes dq [Tq, H, D], dk and dv [Tk, Hk, D] contiguous
+ * (sums over the heads that share a key head), in a fixed order: the same bits every time.
+ * Scores, softmax and sums are fp32; on the tensor cores (D <= 128 a multiple of 8, 16-byte
+ * rows) weights and their gradients enter the second products as values of the model
+ * type.  What a row does not see does not reach it, infinities and NaN included.
+ */
+int64_t rb_segment_attention_workspace_size(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D);
+int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h,
+                         const void* v, int64_t v_t, int64_t v_h, int dtype, int64_t Tq, int64_t Tk, int H,
+                         int Hk, int D, const void* q_offsets, const void* k_offsets, const void* prefix,
+                         int idx_dtype, int64_t S, int causal, const float* slopes, float cap, float scale,
+                         void* workspace, int64_t workspace_bytes, void* out, float* lse, void* stream);
+int64_t rb_segment_attention_backward_workspace_size(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D);
+int rb_segment_attention_backward(const void* grad, int64_t g_t, int64_t g_h, const void* q, int64_t q_t,
+                                  int64_t q_h, const void* k, int64_t k_t, int64_t k_h, const void* v,
+                                  int64_t v_t, int64_t v_h, const void* out, const float* lse, int dtype,
+                                  int64_t Tq, int64_t Tk, int H, int Hk, int D, const void* q_offsets,
+                                  const void* k_offsets, const void* prefix, int idx_dtype, int64_t S,
+                                  int causal, const float* slopes, float cap, float scale, void* workspace,
+                                  int64_t workspace_bytes, void* dq, void* dk, void* dv, void* stream);
+
+/*
+ * Rows of an embedding table by id, and the table's gradient:
+ *   out[i] = scale table[id_i]          dtable[r] = scale sum over id_i = r of grad[row(i)]
+ *   table      [V, ld] fp32, bf16 or fp16, D values a row; out [n, ldo] of that type
+ *   ids        [n] RB_I32 or RB_I64, clamped to [0, V - 1] in both directions
+ *   grad       [n, ld_grad] (any float type), row(i) = i; with bags [n_bags + 1] (the
+ *              ids' type, non-decreasing) [n_bags, ld_grad], row(i) = the bag with
+ *              bags[b] <= i < bags[b + 1]: the gradient of sum-pooled bags.  An id in no
+ *              bag, or equal to padding (-1: none), adds nothing
+ *   workspace  rb_embed_rows_backward_workspace_size bytes (-1: bad shape), 16-byte aligned
+ * rb_embed_rows_backward writes out [V, ld_out] (any float type), zeros where no id
+ * points; with accumulate it adds to what out holds and leaves the other rows alone.
+ * rb_embed_rows_backward_sparse writes the touched rows alone: their numbers, ascending,
+ * to out_ids [n], the gradients to out_rows [n, ld_out], and how many to count; entries
+ * behind are left as they were.  Sums are fp32, in the ids' order within runs of 16 to
+ * 256 equal or neighbouring ids: the same bits every time.
+ */
+int rb_embed_rows(const void* table, int dtype, int64_t ld, int64_t V, int D, const void* ids, int idx_dtype,
+                  int64_t n, float scale, void* out, int64_t ldo, void* stream);
+int64_t rb_embed_rows_backward_workspace_size(int64_t n, int D);
+int rb_embed_rows_backward(const void* grad, int dtype, int64_t ld_grad, int D, const void* ids, int idx_dtype,
+                           int64_t n, int64_t V, const void* bags, int64_t n_bags, int64_t padding, float scale,
+                           int accumulate, void* workspace, int64_t workspace_bytes, void* out, int out_dtype,
+                           int64_t ld_out, void* stream);
+int rb_embed_rows_backward_sparse(const void* grad, int dtype, int64_t ld_grad, int D, const void* ids,
+                                  int idx_dtype, int64_t n, int64_t V, const void* bags, int64_t n_bags,
+                                  int64_t padding, float scale, void* workspace, int64_t workspace_bytes,
+                                  int64_t* out_ids, void* out_rows, int out_dtype, int64_t ld_out, int32_t* count,
+                                  void* stream);
+
+/*
+ * The norm of many gradients together, and the clipping by it:
+ *   norm = scale sqrt(sum g^2);  to = scale g min(1, most / (norm + 1e-6))
+ *   from, to   `tensors` device pointers each (host arrays); to may be from, tensors share no
+ *              memory otherwise.  most < 0: the norm alone (to may be NULL)
+ *   values, dtypes   each tensor's number of values, and type (fp32, bf16, fp16)
+ *   counts, widths   NULL, or for some tensors an int32 on the device and a row's width:
+ *              only the first *count rows are read and written
+ *   norm       fp32 on the device
+ *   workspace  rb_grad_norm_workspace_size(tensors) bytes (-1: bad shape), 8-byte aligned
+ * Squares are summed in fp32 up to 32 values and in fp64 above (fp64 at once where a
+ * square is outside fp32's range), in a fixed order: the same bits every time.
+ */
+int64_t rb_grad_norm_workspace_size(int tensors);
+int rb_clip_grads(const void* const* from, void* const* to, const int64_t* values, const int* dtypes,
+                  const void* const* counts, const int64_t* widths, int tensors, float scale, float most,
+                  void* workspace, int64_t workspace_bytes, float* norm, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
