@@ -37,13 +37,15 @@ struct Params {
   float* lse;                     // [H, Tq] log of the sum of exp(s), -inf where nothing is seen
   float* delta;                   // [H, Tq]
   int4* rows;                     // [Tq]: lo, hi, place of the query among the packed keys, 0
+  int4* tiles;                    // of the queries: rows [x, y), the keys that they see [z, w)
+  uint32_t* next;                 // tickets for work
   const void *q_off, *k_off, *prefix;
   const float* slopes;
   int64_t q_t, q_h, k_t, k_h, v_t, v_h, g_t, g_h;  // elements from token to token and from head to head
   int Tq, Tk, S, H, Hk, G, D, off64, causal;
   float scale, cap;
   uint32_t* peaks;                // fp16 backward: the largest norms of a row of g and of v
-  int by_segment;                 // tiles follow segments (else: 128 rows of the packed order)
+  int by_segment, n_tiles;        // tiles follow segments (else: 128 rows of the packed order)
 };
 
 __device__ __forceinline__ int64_t entry(const void* a, int wide, int64_t i) {
@@ -79,12 +81,6 @@ __device__ __forceinline__ int4 row_of(const Params& p, int r) {
   return hi > k0 ? make_int4(k0, hi, place, 0) : make_int4(0, 0, place, 0);
 }
 
-__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Params p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int r = blockIdx.x * 256 + threadIdx.x;
-  if (r < p.Tq) p.rows[r] = row_of(p, r);
-}
-
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 
@@ -106,6 +102,60 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
   return v;
+}
+
+constexpr int kTile = 128;  // rows of a tile: the lanes of TMEM
+
+// The rows [x, y) of tile b.  By the packed order, 128 rows a tile.  By segment, segment s has room for tiles from
+// floor(start / 128) + s on, which is as much as it needs and known without a sum over segments; the rows before the
+// first and behind the last count as segments too, and a tile that its segment does not need is empty.
+__device__ __forceinline__ int2 tile_rows(const void* off, int wide, int S, int total, int b, int by_segment) {
+  if (!by_segment) return make_int2(min(b * kTile, total), min((b + 1) * kTile, total));
+  // starts 0, off[0], ..., off[S]: the last i with floor(start_i / 128) + i <= b
+  int lo = 0, hi = S + 2;
+  const int lane = threadIdx.x & 31;
+  while (hi - lo > 1) {  // 32 probes at once
+    const int step = (hi - lo + 31) / 32;
+    const int i = lo + (lane + 1) * step;
+    const bool below = i < hi && offset_at(off, wide, i - 1, total) / kTile + i <= b;
+    const int n = __popc(__ballot_sync(kAll, below));
+    lo += n * step;
+    hi = min(hi, lo + step);
+  }
+  const int start = lo == 0 ? 0 : offset_at(off, wide, lo - 1, total);
+  const int end = lo == S + 1 ? total : offset_at(off, wide, lo, total);
+  const int first = start + (b - (start / kTile + lo)) * kTile;
+  return make_int2(min(first, end), min(first + kTile, end));
+}
+
+// The rows' intervals, once a call for all heads, a CTA a tile; and what its rows see together.  A tile that sees nothing
+// is finished here (zeros).
+template <typename T>
+__global__ void __launch_bounds__(kTile) plan_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ int s_lo[4], s_hi[4];
+  if (blockIdx.x == 0 && threadIdx.x == 0 && p.next != nullptr) *p.next = 0;
+  const int2 span = tile_rows(p.q_off, p.off64, p.S, p.Tq, blockIdx.x, p.by_segment);
+  const int r = span.x + threadIdx.x, warp = threadIdx.x >> 5;
+  int4 row = make_int4(0, 0, 0, 0);
+  if (r < span.y) {
+    row = row_of(p, r);
+    p.rows[r] = row;
+  }
+  const int lo = __reduce_min_sync(kAll, row.y > row.x ? row.x : INT_MAX), hi = __reduce_max_sync(kAll, row.y > row.x ? row.y : 0);
+  if ((threadIdx.x & 31) == 0) {
+    s_lo[warp] = lo;
+    s_hi[warp] = hi;
+  }
+  __syncthreads();
+  const int first = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), last = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+  if (threadIdx.x == 0 && p.tiles != nullptr) p.tiles[blockIdx.x] = make_int4(span.x, span.y, first, last);
+  if (first >= last && p.tiles != nullptr) {
+    T* out = static_cast<T*>(p.out) + (int64_t)span.x * p.H * p.D;
+    for (int64_t i = threadIdx.x; i < (int64_t)max(span.y - span.x, 0) * p.H * p.D; i += kTile) out[i] = T(0.0f);
+    if (p.lse != nullptr && r < span.y)
+      for (int h = 0; h < p.H; ++h) p.lse[(int64_t)h * p.Tq + r] = -INFINITY;
+  }
 }
 
 // ------------------------------------------------------------ one row, one warp
@@ -254,45 +304,102 @@ __global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ Params
   else row_dkv<T>(p, r, h);
 }
 
-// delta_i = dout_i . out_i, a warp a row of one head; in fp16 the largest norms of a row of dout and of v too (those that
-// are finite), as bits of positive floats, which order as numbers do.  Warps behind the queries' take v.
+// What the gradients need of each query: its interval (the first CTAs, a thread a query), delta_i = dout_i . out_i, and in
+// fp16 the largest norms of a row of dout and of v (those that are finite), as bits of positive floats, which order as
+// numbers do.  LANES lanes take a row of one head by 16 bytes each (32, value by value, where rows do not allow that).
+constexpr int kDeltaCtas = 8;  // an SM, at most: every CTA ends with an atomic maximum to the same two words
 template <typename T>
+__device__ __forceinline__ float2 widen2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(bf16_lo(w), bf16_hi(w));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+// (a . b, b . b) of a row, summed over its lanes
+template <typename T, int LANES, bool VEC>
+__device__ __forceinline__ float2 row_sums(const T* a, const T* b, int D) {
+  const int lane = threadIdx.x % LANES;
+  float s = 0.0f, n = 0.0f;
+  if constexpr (VEC) {
+    for (int c = lane * 8; c < D; c += LANES * 8) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(b + c));
+      const uint4 u = a != nullptr ? __ldg(reinterpret_cast<const uint4*>(a + c)) : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = widen2<T>(uw[i]), y = widen2<T>(vw[i]);
+        s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
+        n = fmaf(y.x, y.x, fmaf(y.y, y.y, n));
+      }
+    }
+  } else {
+    for (int c = lane; c < D; c += LANES) {
+      const float y = to_f32(b[c]);
+      if (a != nullptr) s = fmaf(to_f32(a[c]), y, s);
+      n = fmaf(y, y, n);
+    }
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(kAll, s, o);
+    n += __shfl_xor_sync(kAll, n, o);
+  }
+  return make_float2(s, n);
+}
+template <typename T, int LANES, bool VEC>
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Params p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr bool kPeaks = std::is_same<T, __half>::value;
-  const int lane = threadIdx.x & 31;
-  int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int64_t queries = (int64_t)p.Tq * p.H;
-  float norm = 0.0f;
-  if (i < queries) {
-    const int r = (int)(i / p.H), h = (int)(i % p.H);
-    if (h == 0 && lane == 0) p.rows[r] = row_of(p, r);
-    const T* o = static_cast<const T*>(p.o) + i * p.D;
-    const T* g = static_cast<const T*>(p.g) + r * p.g_t + h * p.g_h;
-    float s = 0.0f;
-    for (int c = lane; c < p.D; c += 32) {
-      const float f = to_f32(g[c]);
-      s = fmaf(to_f32(o[c]), f, s);
-      norm = fmaf(f, f, norm);
+  __shared__ uint32_t s_peak[2];
+  const int row_ctas = (p.Tq + 255) / 256;
+  if ((int)blockIdx.x < row_ctas) {
+    const int r = blockIdx.x * 256 + threadIdx.x;
+    if (r < p.Tq) p.rows[r] = row_of(p, r);
+    return;
+  }
+  if (kPeaks && threadIdx.x < 2) s_peak[threadIdx.x] = 0;
+  __syncthreads();
+  constexpr int kRows = 256 / LANES;
+  const int64_t queries = (int64_t)p.Tq * p.H, all = queries + (kPeaks ? (int64_t)p.Tk * p.Hk : 0);
+  const int64_t step = (int64_t)(gridDim.x - row_ctas) * kRows;
+  for (int64_t i0 = (int64_t)(blockIdx.x - row_ctas) * kRows; i0 < all; i0 += step) {
+    const int64_t i = i0 + threadIdx.x / LANES;
+    const bool query = i < queries;
+    float2 s = make_float2(0.0f, 0.0f);
+    if (query) {
+      const int64_t r = i / p.H;
+      const int h = (int)(i - r * p.H);
+      s = row_sums<T, LANES, VEC>(static_cast<const T*>(p.o) + i * p.D, static_cast<const T*>(p.g) + r * p.g_t + h * p.g_h, p.D);
+      if (threadIdx.x % LANES == 0) p.delta[(int64_t)h * p.Tq + r] = s.x;
+    } else if (kPeaks) {
+      const int64_t j = min(i, all - 1) - queries, r = j / p.Hk;
+      s = row_sums<T, LANES, VEC>(nullptr, static_cast<const T*>(p.v) + r * p.v_t + (j - r * p.Hk) * p.v_h, p.D);
     }
-    s = warp_sum(s);
-    if (lane == 0) p.delta[(int64_t)h * p.Tq + r] = s;
-  } else if (kPeaks && i - queries < (int64_t)p.Tk * p.Hk) {
-    i -= queries;
-    const T* v = static_cast<const T*>(p.v) + i / p.Hk * p.v_t + i % p.Hk * p.v_h;
-    for (int c = lane; c < p.D; c += 32) norm = fmaf(to_f32(v[c]), to_f32(v[c]), norm);
-    i += queries;
+    if (kPeaks && i < all && s.y > 0.0f && s.y < INFINITY && threadIdx.x % LANES == 0) atomicMax(&s_peak[query ? 0 : 1], __float_as_uint(sqrtf(s.y)));
   }
   if (kPeaks) {
-    norm = sqrtf(warp_sum(norm));
-    if (lane == 0 && norm > 0.0f && norm < INFINITY) atomicMax(p.peaks + (i < queries ? 0 : 1), __float_as_uint(norm));
+    __syncthreads();
+    if (threadIdx.x < 2) atomicMax(p.peaks + threadIdx.x, s_peak[threadIdx.x]);
   }
 }
 
 // ------------------------------------------------------- tensor-core helpers
-constexpr int kTile = 128;    // rows of a tile: the lanes of TMEM
 constexpr int kBlock = 64;    // of the other side that a step takes
-constexpr int kThreads = 160; // a warp for the copies and the MMAs, four for the rows
+
+// A wait for others of the CTA, for at most 2^27 tries (seconds).  Short code on purpose: a wait stands between any two
+// pieces of work here, and fetching instructions is among what these kernels lose most to.
+__device__ __noinline__ bool given_up(uint32_t tries, int code, volatile int* abort_flag) {
+  if (abort_flag != nullptr && *abort_flag) return true;
+  if (tries < 1u << 27) return false;
+  raise_device_error(code);
+  if (abort_flag != nullptr) *abort_flag = 1;
+  return true;
+}
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, int code, volatile int* abort_flag) {
+  const uint32_t at = smem_u32(bar);
+  uint32_t tries = 0;
+  while (!mbar_try_wait(at, parity & 1u))
+    if ((++tries & 0xfffu) == 0 && given_up(tries, code, abort_flag)) return false;
+  return true;
+}
 
 // K-major operand: 64 columns (128 bytes) a row, groups of eight rows 1024 bytes apart
 __device__ __forceinline__ uint64_t rows_desc(uint32_t saddr) { return tc::sw128_desc(saddr); }
@@ -408,66 +515,86 @@ __device__ __forceinline__ bool rows_all(bool ok) {
   return every != 0;
 }
 
-// The rows [x, y) of tile b.  By the packed order, 128 rows a tile.  By segment, segment s has room for tiles from
-// floor(start / 128) + s on, which is as much as it needs and known without a sum over segments; the rows before the
-// first and behind the last count as segments too, and a tile that its segment does not need is empty.
-__device__ __forceinline__ int2 tile_rows(const void* off, int wide, int S, int total, int b, int by_segment) {
-  if (!by_segment) return make_int2(min(b * kTile, total), min((b + 1) * kTile, total));
-  // starts 0, off[0], ..., off[S]: the last i with floor(start_i / 128) + i <= b
-  int lo = 0, hi = S + 2;
-  const int lane = threadIdx.x & 31;
-  while (hi - lo > 1) {  // 32 probes at once
-    const int step = (hi - lo + 31) / 32;
-    const int i = lo + (lane + 1) * step;
-    const bool below = i < hi && offset_at(off, wide, i - 1, total) / kTile + i <= b;
-    const int n = __popc(__ballot_sync(kAll, below));
-    lo += n * step;
-    hi = min(hi, lo + step);
+// Half a block of neighbouring keys and the rows of a warp: seen by none of them, by all, or by some.
+enum Seen : int { kNone = 0, kSome = 1, kEvery = 2 };
+constexpr int kHalf = 32;
+struct Span {  // of a warp's rows' intervals
+  int lo_min, lo_max, hi_min, hi_max;
+  __device__ Seen of(int j) const {
+    return j + kHalf <= lo_min || j >= hi_max ? kNone : j >= lo_max && j + kHalf <= hi_min ? kEvery : kSome;
   }
-  const int start = lo == 0 ? 0 : offset_at(off, wide, lo - 1, total);
-  const int end = lo == S + 1 ? total : offset_at(off, wide, lo, total);
-  const int first = start + (b - (start / kTile + lo)) * kTile;
-  return make_int2(min(first, end), min(first + kTile, end));
+};
+__device__ __forceinline__ Span span_of(int4 row) {
+  const bool sees = row.y > row.x;
+  Span s;
+  s.lo_min = __reduce_min_sync(kAll, sees ? row.x : INT_MAX);
+  s.hi_max = __reduce_max_sync(kAll, sees ? row.y : 0);
+  s.lo_max = __reduce_max_sync(kAll, row.x);
+  s.hi_min = __reduce_min_sync(kAll, row.y);  // 0 with a row that sees nothing: kEvery never
+  return s;
 }
 
-// scores in place of raw products, in units of log 2; `unit` is what is left to multiply by
-__device__ __forceinline__ void transform(const Params& p, uint32_t* raw, float slope2, int place, int j0) {
-  const float up = p.scale / p.cap, cap2 = p.cap * kLog2e;
-  if (p.cap > 0.0f) {
+__device__ __forceinline__ F2 pair(const uint32_t* x) { return f2(__uint_as_float(x[0]), __uint_as_float(x[1])); }
+__device__ __forceinline__ void put(uint32_t* x, F2 v) {
+  const float2 f = un(v);
+  x[0] = __float_as_uint(f.x);
+  x[1] = __float_as_uint(f.y);
+}
+// scores in place of raw products, in units of log 2, of the 32 keys from j on
+__device__ __forceinline__ void transform(const Params& p, uint32_t* raw, float slope2, int place, int j) {
+  if (p.cap > 0.0f) {  // cap tanh(y) = cap - 2 cap / (1 + e^2y), as tanh_of has it
+    const float in = p.scale / p.cap * (2.0f * kLog2e), cap2 = p.cap * kLog2e;
+    const F2 in2 = f2(in, in), one = f2(1.0f, 1.0f), base = f2(cap2, cap2), minus = f2(-2.0f * cap2, -2.0f * cap2);
 #pragma unroll
-    for (int c = 0; c < kBlock; ++c) raw[c] = __float_as_uint(cap2 * tanh_of(__uint_as_float(raw[c]) * up));
+    for (int c = 0; c < kHalf; c += 2) {
+      const float2 y = un(mul2(pair(raw + c), in2));
+      const float2 d = un(add2(f2(exp2_fast(y.x), exp2_fast(y.y)), one));
+      put(raw + c, fma2(f2(rcp_fast(d.x), rcp_fast(d.y)), minus, base));
+    }
   }
   if (slope2 != 0.0f) {
-    const float first = (float)(place - j0), unit = p.cap > 0.0f ? 1.0f : p.scale * kLog2e;
+    const float first = (float)(place - j), unit = p.cap > 0.0f ? 1.0f : p.scale * kLog2e;
 #pragma unroll
-    for (int c = 0; c < kBlock; ++c)
+    for (int c = 0; c < kHalf; ++c)
       raw[c] = __float_as_uint(fmaf(-slope2, fabsf(first - (float)c), __uint_as_float(raw[c]) * unit));
   }
 }
 
 // ---------------------------------------------------------------- forward
-// One CTA a tile of 128 rows of one head.  A row's thread takes its 64 scores of a block out of TMEM, keeps the
-// running maximum and sum, and puts the weights back as 16-bit values, from where the second product takes them;
-// its accumulator is rescaled only when a maximum has grown by more than 2^8 over what it is scaled to (the weights
-// stay below 256, the sum is fp32).  Rounding a weight to the type is half a step of its own value (2^-9 bf16, 2^-12
-// fp16), independent from key to key.
+// A persistent CTA takes tiles of 128 rows of one head, the next by a ticket (long ones first), and treats their blocks
+// of 64 keys as one stream: the thread that issues copies and MMAs asks for a block's keys and values kStages blocks
+// ahead, in the next tile where this one ends, so that no tile waits for memory at its start.  With a CTA a tile, 1024
+// users took 265 us: three quarters of a CTA's life went to its start and end.
+//
+// A row's thread goes over the block's scores in TMEM twice, 32 at a time: the maximum (scores that are masked or capped
+// or fall with distance are put back in their place), then the weights, which go back as 16-bit values for the second
+// product.  The running sum is fp32; the accumulator is rescaled only when a maximum has grown by more than 2^8 over
+// what it is scaled to.  Rounding a weight to the type is half a step of its own value (2^-9 bf16, 2^-12 fp16),
+// independent from key to key.
 template <int DP>
 struct Forward {
   static constexpr int kChunks = DP / 64;              // 64 columns, a swizzled row
   static constexpr int kQBytes = kTile * 128 * kChunks;
   static constexpr int kKvBytes = kBlock * 128 * kChunks;
-  static constexpr int kStages = DP == 64 ? 3 : 2;
+  static constexpr int kStages = 2;
   static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kKvBytes;
-  // DP 64: the weights lie where the scores were, 128 columns in all and three CTAs an SM; DP 128: apart, two CTAs,
-  // and the next scores are computed meanwhile
+  // DP 64: the weights lie where the scores were, 128 columns in all, and four CTAs an SM fill each other's waits; DP
+  // 128: apart, two CTAs, and the next block's scores are computed meanwhile
   static constexpr bool kApart = DP == 128;
   static constexpr int kPAt = kApart ? 64 : 0, kOAt = kApart ? 128 : 64;
   static constexpr int kTmemCols = kApart ? 256 : 128;
-  static constexpr int kCtas = kApart ? 2 : 3;
+  static constexpr int kCtas = kApart ? 2 : 4;
+  // warps that share 32 rows, each with half of a block's keys: sixteen warps of rows an SM either way
+  static constexpr int kSets = kApart ? 2 : 1;
+  static constexpr int kRowThreads = 128 * kSets, kThreads = 32 + kRowThreads;
+};
+constexpr int kItems = 4;  // tiles that are posted to the rows: theirs, up to two ahead, and one more
+struct Item {
+  int r0, r1, head, key0, blocks;  // blocks 0: no more
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, Forward<DP>::kCtas)
+__global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
     forward_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
   using C = Forward<DP>;
@@ -476,14 +603,18 @@ __global__ void __launch_bounds__(kThreads, Forward<DP>::kCtas)
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + C::kQBytes;
   uint8_t* sV = sK + C::kStages * C::kKvBytes;
-  __shared__ __align__(8) uint64_t qfull, kfull[C::kStages], vfull[C::kStages];
+  __shared__ __align__(8) uint64_t qfull, kfull[C::kStages], vfull[C::kStages], ifull[kItems];
   __shared__ __align__(8) uint64_t sfull, sfree, pready, pvdone, drained;
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word, s_lo[4], s_hi[4];
+  __shared__ int abort_word;
+  __shared__ Item s_item[kItems];
+  // what the two warps of 32 rows tell each other: a row's maximum of either half (of this block and the next), its sums,
+  // whether they are finite
+  __shared__ __align__(8) uint64_t pairs[4];
+  __shared__ float s_max[2][2][C::kSets == 2 ? kTile : 1], s_total[2][C::kSets == 2 ? kTile : 1];
+  __shared__ int s_redo[C::kSets == 2 ? kTile : 1];
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // long rows come last in the packed order: their tiles start first
-  const int tile = gridDim.x - 1 - blockIdx.x, h = blockIdx.y, hk = h / p.G;
 
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&qfull), 1);
@@ -491,11 +622,13 @@ __global__ void __launch_bounds__(kThreads, Forward<DP>::kCtas)
       mbar_init(smem_u32(&kfull[s]), 1);
       mbar_init(smem_u32(&vfull[s]), 1);
     }
+    for (int s = 0; s < kItems; ++s) mbar_init(smem_u32(&ifull[s]), 1);
     mbar_init(smem_u32(&sfull), 1);
-    mbar_init(smem_u32(&sfree), kTile);
-    mbar_init(smem_u32(&pready), kTile);
+    mbar_init(smem_u32(&sfree), C::kRowThreads);
+    mbar_init(smem_u32(&pready), C::kRowThreads);
     mbar_init(smem_u32(&pvdone), 1);
     mbar_init(smem_u32(&drained), 1);
+    for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&pairs[q]), 64);
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -508,204 +641,313 @@ __global__ void __launch_bounds__(kThreads, Forward<DP>::kCtas)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int2 span = tile_rows(p.q_off, p.off64, p.S, p.Tq, tile, p.by_segment);
-  const int quarter = warp & 3;  // of the lanes of TMEM, for the rows' warps
-  const int r = span.x + quarter * 32 + lane;
-  int4 row = make_int4(0, 0, 0, 0);
-  if (warp >= 1) {
-    if (r < span.y) row = __ldg(p.rows + r);
-    int lo = row.y > row.x ? row.x : INT_MAX, hi = row.y > row.x ? row.y : 0;
-    lo = __reduce_min_sync(kAll, lo);
-    hi = __reduce_max_sync(kAll, hi);
-    if (lane == 0) {
-      s_lo[quarter] = lo;
-      s_hi[quarter] = hi;
-    }
-  }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int key0 = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
-  const int key1 = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
-  const int blocks = key1 > key0 ? (key1 - key0 + kBlock - 1) / kBlock : 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (warp == 0) {
-    if (lane == 0 && blocks > 0) {
+    if (lane == 0) {
       // -------------------------------------------------- copies and MMAs
       constexpr uint32_t idesc_s = idesc_of<T>(kBlock, false), idesc_o = idesc_of<T>(DP, true);
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(smem_u32(bar), parity, kWaitTimeoutMma, abort_flag); };
-      auto slot = [](int n) { return n % C::kStages; };
-      auto phase = [](int n) { return (uint32_t)(n / C::kStages) & 1u; };
-      int k_asked = 0, v_asked = 0;
-      auto ask = [&](uint64_t* full, uint8_t* to, const CUtensorMap* tm, int n) {
-        const uint32_t bar = smem_u32(&full[slot(n)]);
+      auto wait = [&](uint64_t* bar, int n) { return wait_on(bar, (uint32_t)n, kWaitTimeoutMma, abort_flag); };
+      auto slot = [](int t) { return t % C::kStages; };
+      auto phase = [](int t) { return t / C::kStages; };
+      const uint32_t items = (uint32_t)p.n_tiles * p.H;
+      // `ahead`: the tile whose keys are asked for, the `posted`th, from block a_block on; the values follow, block v_block
+      // of tile v_tile.  Posting overwrites what was posted four tiles ago: its blocks lie three tiles back at least and
+      // the rows are past them.
+      Item ahead{};
+      int posted = 0, a_block = 0, k_asked = 0, v_tile = 0, v_block = 0, v_asked = 0;
+      uint32_t ticket = atomicAdd(p.next, 1u);
+      auto take = [&] {
+        ahead.blocks = 0;
+        a_block = 0;
+        while (ticket < items && ahead.blocks == 0) {
+          const int4 t = __ldg(p.tiles + (p.n_tiles - 1 - ticket / p.H));
+          ahead = Item{t.x, t.y, (int)(ticket % p.H), t.z, t.w > t.z ? (t.w - t.z + kBlock - 1) / kBlock : 0};
+          ticket = atomicAdd(p.next, 1u);  // (needed a tile later)
+        }
+        s_item[posted % kItems] = ahead;
+        mbar_arrive(smem_u32(&ifull[posted % kItems]));
+        ++posted;
+      };
+      auto copy = [&](uint64_t* full, uint8_t* to, const CUtensorMap* tm, int i, int head, int key) {
+        const uint32_t bar = smem_u32(&full[slot(i)]);
         mbar_arrive_expect_tx(bar, C::kKvBytes);
         for (int c = 0; c < C::kChunks; ++c)
-          tma_load_3d(smem_u32(to + slot(n) * C::kKvBytes + c * kBlock * 128), tm, 64 * c, hk, key0 + n * kBlock, bar);
+          tma_load_3d(smem_u32(to + slot(i) * C::kKvBytes + c * kBlock * 128), tm, 64 * c, head / p.G, key, bar);
       };
-      auto ask_k = [&] { if (k_asked < blocks) ask(kfull, sK, &tmK, k_asked), ++k_asked; };
-      auto ask_v = [&] { if (v_asked < blocks) ask(vfull, sV, &tmV, v_asked), ++v_asked; };
-      const uint32_t qb = smem_u32(&qfull);
-      mbar_arrive_expect_tx(qb, C::kQBytes);
-      for (int c = 0; c < C::kChunks; ++c) tma_load_3d(smem_u32(sQ + c * kTile * 128), &tmQ, 64 * c, h, span.x, qb);
-      for (int s = 0; s < C::kStages; ++s) {
-        ask_k();
-        ask_v();
-      }
+      auto ask_k = [&] {  // for the next block's keys, whose slot is free
+        if (ahead.blocks == 0) return;
+        copy(kfull, sK, &tmK, k_asked++, ahead.head, ahead.key0 + a_block * kBlock);
+        if (++a_block == ahead.blocks) take();
+      };
+      auto ask_v = [&] {  // for its values
+        if (v_asked == k_asked) return;
+        const Item& it = s_item[v_tile % kItems];
+        copy(vfull, sV, &tmV, v_asked++, it.head, it.key0 + v_block * kBlock);
+        if (++v_block == it.blocks) {
+          v_block = 0;
+          ++v_tile;
+        }
+      };
+      int queried = 0;
+      auto ask_queries = [&](const Item& it) {
+        const uint32_t bar = smem_u32(&qfull);
+        mbar_arrive_expect_tx(bar, C::kQBytes);
+        for (int c = 0; c < C::kChunks; ++c) tma_load_3d(smem_u32(sQ + c * kTile * 128), &tmQ, 64 * c, it.head, it.r0, bar);
+        ++queried;
+      };
       const int steps = (p.D + 15) / 16;  // of 16 columns (the rest of a row is zeros)
-      auto scores = [&](int n) {
-        if (!wait(&kfull[slot(n)], phase(n))) return false;
+      auto scores = [&](int t, bool first) {
+        if (first && !wait(&qfull, queried - 1)) return false;
+        if (!wait(&kfull[slot(t)], phase(t))) return false;
         tc::tc_fence_after();
-        const uint64_t qd = rows_desc(smem_u32(sQ)), kd = rows_desc(smem_u32(sK + slot(n) * C::kKvBytes));
+        const uint64_t qd = rows_desc(smem_u32(sQ)), kd = rows_desc(smem_u32(sK + slot(t) * C::kKvBytes));
         for (int i = 0; i < steps; ++i)
           mma_ss(tmem, qd + (uint64_t)((i >> 2) * (kTile * 128 / 16) + (i & 3) * 2),
                  kd + (uint64_t)((i >> 2) * (kBlock * 128 / 16) + (i & 3) * 2), idesc_s, i > 0);
         tc::umma_commit(smem_u32(&sfull));
         return true;
       };
-      bool ok = wait(&qfull, 0) && scores(0);
-      for (int n = 0; n < blocks && ok; ++n) {
-        if (C::kApart) {  // the rows' threads have the scores: their columns and their keys' slot are free
-          ok = wait(&sfree, (uint32_t)n & 1u);
-          if (ok) {
-            tc::tc_fence_after();
-            ask_k();
-            if (n + 1 < blocks) ok = scores(n + 1);
-          }
+      take();
+      Item now = ahead;
+      bool ok = true;
+      if (now.blocks > 0) {
+        ask_queries(now);
+        for (int s = 0; s < C::kStages; ++s) {
+          ask_k();
+          ask_v();
         }
-        ok = ok && wait(&pready, (uint32_t)n & 1u) && wait(&vfull[slot(n)], phase(n));
-        if (!ok) break;
-        tc::tc_fence_after();
-        if (C::kApart && n > 0) ask_v();  // (the weights were written after the product before had ended)
-        const uint64_t vd = columns_desc(smem_u32(sV + slot(n) * C::kKvBytes), kBlock * 128);
-        for (int i = 0; i < kBlock / 16; ++i)
-          mma_ts(tmem + C::kOAt, tmem + C::kPAt + 8 * i, vd + (uint64_t)(i * 16 * 128 / 16), idesc_o, n > 0 || i > 0);
-        tc::umma_commit(smem_u32(&pvdone));
-        if (!C::kApart && n + 1 < blocks) {
-          ok = wait(&pvdone, (uint32_t)n & 1u);
-          if (ok) {
+        ok = scores(0, true);
+      }
+      int t = 0;  // block of all tiles
+      for (int tile = 0; now.blocks > 0 && ok; ++tile) {
+        Item next{};
+        for (int n = 0; n < now.blocks && ok; ++n, ++t) {
+          const bool last = n + 1 == now.blocks;
+          // (a tile is posted when the last block before it is asked for, kStages before this one is done)
+          if (C::kApart) {  // the rows' threads have the scores: their columns are free, and their keys' slot
+            ok = wait(&sfree, t);
+            if (ok) {
+              tc::tc_fence_after();
+              ask_k();
+              if (!last) ok = scores(t + 1, false);
+            }
+          }
+          ok = ok && wait(&pready, t);
+          if (!ok) break;
+          if (last) {
+            next = s_item[(tile + 1) % kItems];
+            if (next.blocks > 0) ask_queries(next);
+          }
+          ok = wait(&vfull[slot(t)], phase(t));
+          if (!ok) break;
+          tc::tc_fence_after();
+          const uint64_t vd = columns_desc(smem_u32(sV + slot(t) * C::kKvBytes), kBlock * 128);
+          for (int i = 0; i < kBlock / 16; ++i)
+            mma_ts(tmem + C::kOAt, tmem + C::kPAt + 8 * i, vd + (uint64_t)(i * 16 * 128 / 16), idesc_o, n > 0 || i > 0);
+          tc::umma_commit(smem_u32(&pvdone));
+          const bool more = !last || next.blocks > 0;
+          if (C::kApart) {
+            if (t > 0) ask_v();  // (into the slot of the block before: its product had ended before these weights were written)
+            if (last && more) ok = scores(t + 1, true);
+          } else if (more) {
+            ok = wait(&pvdone, t);
+            if (ok) ok = scores(t + 1, last);
             ask_k();
             ask_v();
-            ok = scores(n + 1);
           }
         }
+        now = next;
       }
       if (!ok) {  // given up: no MMA in flight behind this CTA
         tc::umma_commit(smem_u32(&drained));
-        mbar_wait_bounded(smem_u32(&drained), 0, kWaitTimeoutMma, nullptr);
+        wait_on(&drained, 0, kWaitTimeoutMma, nullptr);
       }
       // nor a copy
-      mbar_wait_bounded(qb, 0, kWaitTimeoutProducer, nullptr);
-      for (int i = max(0, k_asked - C::kStages); i < k_asked; ++i) mbar_wait_bounded(smem_u32(&kfull[slot(i)]), phase(i), kWaitTimeoutProducer, nullptr);
-      for (int i = max(0, v_asked - C::kStages); i < v_asked; ++i) mbar_wait_bounded(smem_u32(&vfull[slot(i)]), phase(i), kWaitTimeoutProducer, nullptr);
+      if (queried > 0) wait_on(&qfull, (uint32_t)(queried - 1), kWaitTimeoutProducer, nullptr);
+      for (int i = max(0, k_asked - C::kStages); i < k_asked; ++i) wait_on(&kfull[slot(i)], (uint32_t)phase(i), kWaitTimeoutProducer, nullptr);
+      for (int i = max(0, v_asked - C::kStages); i < v_asked; ++i) wait_on(&vfull[slot(i)], (uint32_t)phase(i), kWaitTimeoutProducer, nullptr);
     }
   } else {
     // -------------------------------------------------------------- rows
+    const int quarter = warp & 3, set = (warp - 1) >> 2;  // of the lanes of TMEM; of the columns
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
-    const float slope2 = p.slopes != nullptr ? kLog2e * __ldg(p.slopes + h) : 0.0f;
-    const float unit = p.cap > 0.0f || slope2 != 0.0f ? 1.0f : p.scale * kLog2e;
-    float top = -INFINITY, total = 0.0f;  // top: what the weights are scaled to, in the scores' units
-    bool ok = true;
-    for (int n = 0; n < blocks && ok; ++n) {
-      const int j0 = key0 + n * kBlock;
-      ok = mbar_wait_bounded(smem_u32(&sfull), (uint32_t)n & 1u, kWaitTimeoutEpilogue, abort_flag);
-      ok = __all_sync(kAll, ok);
-      if (!ok) break;
-      tc::tc_fence_after();
-      uint32_t x[kBlock];
-      tmem_get32(mine, x);
-      tmem_get32(mine + 32, x + 32);
-      tmem_wait_ld();
-      if (C::kApart) {
-        tc::tc_fence_before();
-        mbar_arrive(smem_u32(&sfree));
-      }
-      transform(p, x, slope2, row.z, j0);
-      if (!__all_sync(kAll, row.x <= j0 && row.y >= j0 + kBlock)) {
-        const int lo = row.x - j0, len = max(row.y - row.x, 0);
+    auto wait = [&](uint64_t* bar, int n) {
+      return __all_sync(kAll, wait_on(bar, (uint32_t)n, kWaitTimeoutEpilogue, abort_flag)) != 0;
+    };
+    int met = 0;
+    auto meet = [&] {  // the two warps of a quarter
+      mbar_arrive(smem_u32(&pairs[quarter]));
+      return wait(&pairs[quarter], met++);
+    };
+    bool ok = wait(&ifull[0], 0);
+    Item it = s_item[0];
+    int4 row = make_int4(0, 0, 0, 0);
+    if (ok && it.blocks > 0 && it.r0 + quarter * 32 + lane < it.r1) row = __ldg(p.rows + it.r0 + quarter * 32 + lane);
+    int t = 0;  // block of all tiles
+    for (int tile = 0; ok && it.blocks > 0; ++tile) {
+      const int r = it.r0 + quarter * 32 + lane, h = it.head;
+      const float slope2 = p.slopes != nullptr ? kLog2e * __ldg(p.slopes + h) : 0.0f;
+      const bool plain = p.cap == 0.0f && slope2 == 0.0f;
+      const float unit = plain ? p.scale * kLog2e : 1.0f;
+      const Span reach = span_of(row);
+      float top = -INFINITY, total = 0.0f;  // top: what the weights are scaled to, in the scores' units
+      for (int n = 0; n < it.blocks && ok; ++n, ++t) {
+        const int j0 = it.key0 + n * kBlock;
+        ok = wait(&sfull, t);
+        if (!ok) break;
+        tc::tc_fence_after();
+        float high = -INFINITY;
+        auto prepare = [&](uint32_t* x, int j, Seen seen) {  // scores of 32 keys, and their maximum
+          if (!plain) transform(p, x, slope2, row.z, j);
+          if (seen == kSome) {
+            const int lo = row.x - j, len = max(row.y - row.x, 0);
 #pragma unroll
-        for (int c = 0; c < kBlock; ++c)
-          if ((unsigned)(c - lo) >= (unsigned)len) x[c] = 0xff800000u;
-      }
-      float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < kBlock; ++c) m[c & 3] = fmaxf(m[c & 3], __uint_as_float(x[c]));
-      const float high = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-      const bool grow = (high - top) * unit > 8.0f || (top == -INFINITY && high > -INFINITY);
-      if (C::kApart && n > 0) ok = mbar_wait_bounded(smem_u32(&pvdone), (uint32_t)(n - 1) & 1u, kWaitTimeoutEpilogue, abort_flag);
-      ok = __all_sync(kAll, ok);
-      if (!ok) break;
-      if (__any_sync(kAll, grow)) {
-        if (n > 0) {
-          const float keep = grow ? exp2_fast((top - high) * unit) : 1.0f;
-          total *= keep;
-          tc::tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < DP; c += 32) {
-            uint32_t o[32];
-            tmem_get32(mine + C::kOAt + c, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-            tmem_put32(mine + C::kOAt + c, o);
+            for (int c = 0; c < kHalf; ++c)
+              if ((unsigned)(c - lo) >= (unsigned)len) x[c] = 0xff800000u;
           }
-        }
-        if (grow) top = high;
-      }
-      const float shift = top == -INFINITY ? 0.0f : -top * unit;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      uint32_t w[kBlock / 2];
+          float m[4] = {high, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < kBlock; c += 2) {
-        const float a = exp2_fast(fmaf(__uint_as_float(x[c]), unit, shift)), b = exp2_fast(fmaf(__uint_as_float(x[c + 1]), unit, shift));
-        sum[c & 2] += a;
-        sum[(c & 2) + 1] += b;
-        w[c / 2] = pack2<T>(a, b);
+          for (int c = 0; c < kHalf; c += 2) m[(c >> 1) & 3] = fmaxf(fmaxf(m[(c >> 1) & 3], __uint_as_float(x[c])), __uint_as_float(x[c + 1]));
+          high = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        };
+        uint32_t held[C::kSets == 2 ? kHalf : 1];
+        if constexpr (C::kSets == 2) {
+          tmem_get32(mine + set * kHalf, held);
+          tmem_wait_ld();
+          tc::tc_fence_before();
+          mbar_arrive(smem_u32(&sfree));
+          const Seen seen = reach.of(j0 + set * kHalf);
+          if (seen != kNone) prepare(held, j0 + set * kHalf, seen);
+          s_max[t & 1][set][quarter * 32 + lane] = high;
+          ok = meet();
+          high = fmaxf(high, s_max[t & 1][set ^ 1][quarter * 32 + lane]);
+        } else {
+          bool kept = false;
+#pragma unroll 1
+          for (int c0 = 0; c0 < kBlock; c0 += kHalf) {
+            const Seen seen = reach.of(j0 + c0);
+            if (seen == kNone) continue;
+            uint32_t x[kHalf];
+            tmem_get32(mine + c0, x);
+            tmem_wait_ld();
+            prepare(x, j0 + c0, seen);
+            if (!plain || seen == kSome) {
+              tmem_put32(mine + c0, x);
+              kept = true;
+            }
+          }
+          if (kept) tmem_wait_st();
+        }
+        const bool grow = (high - top) * unit > 8.0f || (top == -INFINITY && high > -INFINITY);
+        if (C::kApart && n > 0) ok = ok && wait(&pvdone, t - 1);  // the product before has read its weights
+        if (!ok) break;
+        if (__any_sync(kAll, grow)) {
+          if (n > 0) {
+            const float keep = grow ? exp2_fast((top - high) * unit) : 1.0f;
+            total *= keep;
+            tc::tc_fence_after();
+#pragma unroll 1
+            for (int c = 32 * set; c < DP; c += 32 * C::kSets) {
+              uint32_t o[32];
+              tmem_get32(mine + C::kOAt + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+              tmem_put32(mine + C::kOAt + c, o);
+            }
+          }
+          if (grow) top = high;
+        }
+        const float shift = top == -INFINITY ? 0.0f : -top * unit;
+        const F2 unit2 = f2(unit, unit), shift2 = f2(shift, shift);
+        F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+        auto weigh = [&](const uint32_t* x, uint32_t* w) {
+#pragma unroll
+          for (int c = 0; c < kHalf; c += 2) {
+            const float2 e = un(fma2(f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), unit2, shift2));
+            const float a = exp2_fast(e.x), b = exp2_fast(e.y);
+            sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], f2(a, b));
+            w[c / 2] = pack2<T>(a, b);
+          }
+        };
+#pragma unroll 1
+        for (int c0 = C::kSets == 2 ? set * kHalf : 0; c0 < (C::kSets == 2 ? (set + 1) * kHalf : kBlock); c0 += kHalf) {
+          uint32_t w[kHalf / 2];
+          if (reach.of(j0 + c0) == kNone) {
+#pragma unroll
+            for (int c = 0; c < kHalf / 2; ++c) w[c] = 0u;
+          } else if constexpr (C::kSets == 2) {
+            weigh(held, w);
+          } else {
+            uint32_t x[kHalf];
+            tmem_get32(mine + c0, x);
+            tmem_wait_ld();
+            weigh(x, w);
+          }
+          tmem_put16(mine + C::kPAt + c0 / 2, w);
+        }
+        const float2 s2 = un(add2(sum[0], sum[1]));
+        total += s2.x + s2.y;
+        tmem_wait_st();
+        tc::tc_fence_before();
+        mbar_arrive(smem_u32(&pready));
       }
-      total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_put32(mine + C::kPAt, w);
-      tmem_wait_st();
-      tc::tc_fence_before();
-      mbar_arrive(smem_u32(&pready));
-    }
-    if (ok && blocks > 0) {
-      ok = mbar_wait_bounded(smem_u32(&pvdone), (uint32_t)(blocks - 1) & 1u, kWaitTimeoutEpilogue, abort_flag);
+      // the next tile's intervals come while the last product runs
+      ok = ok && wait(&ifull[(tile + 1) % kItems], (tile + 1) / kItems);
+      if (!ok) break;
+      const Item next = s_item[(tile + 1) % kItems];
+      int4 next_row = make_int4(0, 0, 0, 0);
+      if (next.blocks > 0 && next.r0 + quarter * 32 + lane < next.r1) next_row = __ldg(p.rows + next.r0 + quarter * 32 + lane);
+      ok = wait(&pvdone, t - 1);
+      if (!ok) break;
       tc::tc_fence_after();
-    }
-    ok = __all_sync(kAll, ok);
-    if (ok) {
-      const bool sees = row.y > row.x;
+      const bool sees = row.y > row.x, there = r < it.r1;
+      if constexpr (C::kSets == 2) {
+        s_total[set][quarter * 32 + lane] = total;
+        ok = meet();
+        if (!ok) break;
+        total += s_total[set ^ 1][quarter * 32 + lane];
+      }
       const float w = total == 0.0f ? 0.0f : 1.0f / total;
       T* out = static_cast<T*>(p.out) + ((int64_t)r * p.H + h) * p.D;
       const bool wide = p.D % 16 == 0 && aligned(p.out, 32);
       bool redo = sees && !(total < INFINITY);
 #pragma unroll 1
-      for (int c = 0; c < p.D; c += 32) {
+      for (int c = 32 * set; c < p.D; c += 32 * C::kSets) {
         uint32_t o[32];
-        if (blocks > 0) {
-          tmem_get32(mine + C::kOAt + c, o);
-          tmem_wait_ld();
-        }
+        tmem_get32(mine + C::kOAt + c, o);
+        tmem_wait_ld();
         if (!sees) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         } else {
           redo = redo || !finite32(o);
         }
-        if (r < span.y) store_sums<T>(out + c, o, p.D - c, sees ? w : 0.0f, wide);
+        if (there) store_sums<T>(out + c, o, p.D - c, sees ? w : 0.0f, wide);
       }
-      if (r < span.y && p.lse != nullptr)
-        p.lse[(int64_t)h * p.Tq + r] = sees && total != 0.0f ? kLn2 * (fmaf(top, unit, log2f(total))) : -INFINITY;
-      uint32_t again = __ballot_sync(kAll, redo && r < span.y);
+      if (there && p.lse != nullptr && set == 0)
+        p.lse[(int64_t)h * p.Tq + r] = sees && total != 0.0f ? kLn2 * fmaf(top, unit, log2f(total)) : -INFINITY;
+      if constexpr (C::kSets == 2) {  // what either finds not finite in its columns the first takes again, once both have stored
+        if (set == 1) s_redo[quarter * 32 + lane] = redo;
+        ok = meet();
+        if (!ok) break;
+        redo = set == 0 && (redo || s_redo[quarter * 32 + lane] != 0);
+      }
+      uint32_t again = __ballot_sync(kAll, redo && there);
       __syncwarp();
       while (again != 0) {
         const int i = __ffs(again) - 1;
         again &= again - 1;
-        row_forward<T>(p, span.x + quarter * 32 + i, h);
+        row_forward<T>(p, it.r0 + quarter * 32 + i, h);
         __syncwarp();
       }
+      it = next;
+      row = next_row;
     }
   }
   tc::tc_fence_before();
@@ -761,10 +1003,11 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   __shared__ __align__(8) uint64_t afull, bfull[C::kStages], sfull, sfree, ready, done, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word, s_lo[4], s_hi[4], s_bad[kTile];
-  // of the block's queries (KEYS), for this block and the next: lse and delta, interval and place; whether all see all keys
-  __shared__ float2 s_lse[2][KEYS ? kBlock : 1];
+  // of the block's queries (KEYS), for this block and the next: lse and delta (negative), interval and place; and, of its
+  // halves, what all of them see together
+  __shared__ __align__(16) float s_lse[2][KEYS ? kBlock : 4], s_delta[2][KEYS ? kBlock : 4];
   __shared__ int4 s_row[2][KEYS ? kBlock : 1];
-  __shared__ int s_all[2][2];
+  __shared__ Span s_span[2][2];
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.y, tile = KEYS ? blockIdx.x : gridDim.x - 1 - blockIdx.x;
@@ -843,7 +1086,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
     if (lane == 0 && blocks > 0) {
       // -------------------------------------------------- copies and MMAs
       constexpr uint32_t idesc_s = idesc_of<T>(kBlock, false), idesc_o = idesc_of<T>(DP, true);
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(smem_u32(bar), parity, kWaitTimeoutMma, abort_flag); };
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_on(bar, parity, kWaitTimeoutMma, abort_flag); };
       auto slot = [](int n) { return n % C::kStages; };
       auto phase = [](int n) { return (uint32_t)(n / C::kStages) & 1u; };
       int asked = 0;
@@ -906,38 +1149,43 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
       }
       if (!ok) {  // given up: no MMA in flight behind this CTA
         tc::umma_commit(smem_u32(&drained));
-        mbar_wait_bounded(smem_u32(&drained), 0, kWaitTimeoutMma, nullptr);
+        wait_on(&drained, 0, kWaitTimeoutMma, nullptr);
       }
       // nor a copy
-      mbar_wait_bounded(ab, 0, kWaitTimeoutProducer, nullptr);
-      for (int i = max(0, asked - C::kStages); i < asked; ++i) mbar_wait_bounded(smem_u32(&bfull[slot(i)]), phase(i), kWaitTimeoutProducer, nullptr);
+      wait_on(&afull, 0, kWaitTimeoutProducer, nullptr);
+      for (int i = max(0, asked - C::kStages); i < asked; ++i) wait_on(&bfull[slot(i)], phase(i), kWaitTimeoutProducer, nullptr);
     }
   } else {
     // -------------------------------------------------------------- rows
     const int t = threadIdx.x - 32;
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
-    float unit = p.cap > 0.0f ? 1.0f : p.scale * kLog2e, slope2 = 0.0f, lse = 0.0f, delta = 0.0f;
+    const float unit = p.cap > 0.0f ? p.cap * kLog2e : p.scale * kLog2e;
+    float slope2 = 0.0f, lse = 0.0f, delta = 0.0f;
+    Span reach{};
+    if (!KEYS) reach = span_of(row);
     if (!KEYS) {
       slope2 = p.slopes != nullptr ? kLog2e * __ldg(p.slopes + head) : 0.0f;
       lse = r < span.y ? lse_of(p, r, head) - up : INFINITY;
       delta = r < span.y ? sigma * __ldg(p.delta + (int64_t)head * p.Tq + r) : 0.0f;
     }
     // a block's queries, by the first two warps of the rows: from memory, then to shared memory
-    float2 next_lse = make_float2(INFINITY, 0.0f);
+    float next_lse = INFINITY, next_delta = 0.0f;
     int4 next_row = make_int4(0, 0, 0, 0);
     auto fetch = [&](int n) {
       if (t >= kBlock) return;
       const int i = other0 + (n % each) * kBlock + t, h = head * p.G + n / each;
       const bool there = i < other1;
       next_row = there ? __ldg(p.rows + i) : make_int4(0, 0, 0, 0);
-      next_lse = there ? make_float2(lse_of(p, i, h) - up, sigma * __ldg(p.delta + (int64_t)h * p.Tq + i)) : make_float2(INFINITY, 0.0f);
+      next_lse = there ? lse_of(p, i, h) - up : INFINITY;
+      next_delta = there ? sigma * __ldg(p.delta + (int64_t)h * p.Tq + i) : 0.0f;
     };
     auto deposit = [&](int n) {
       if (t < kBlock) {
-        s_lse[n & 1][t] = next_lse;
+        s_lse[n & 1][t] = -next_lse;
+        s_delta[n & 1][t] = -next_delta;
         s_row[n & 1][t] = next_row;
-        const bool all = __all_sync(kAll, next_row.x <= span.x && next_row.y >= span.y);
-        if (lane == 0) s_all[n & 1][t >> 5] = all;
+        const Span span = span_of(next_row);
+        if (lane == 0) s_span[n & 1][t >> 5] = span;
       }
     };
     auto meet = [](bool good) { return rows_all<C::kRowThreads>(good); };
@@ -951,64 +1199,80 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
     for (int n = 0; n < blocks && ok; ++n) {
       const int o0 = other0 + (KEYS ? n % each : n) * kBlock;
       if (KEYS) slope2 = p.slopes != nullptr ? kLog2e * __ldg(p.slopes + head * p.G + n / each) : 0.0f;
-      ok = mbar_wait_bounded(smem_u32(&sfull), (uint32_t)n & 1u, kWaitTimeoutEpilogue, abort_flag);
-      ok = __all_sync(kAll, ok);
+      ok = __all_sync(kAll, wait_on(&sfull, (uint32_t)n, kWaitTimeoutEpilogue, abort_flag));
       tc::tc_fence_after();
-      const bool all = KEYS ? s_all[n & 1][0] && s_all[n & 1][1] : __all_sync(kAll, row.x <= o0 && row.y >= o0 + kBlock);
+#pragma unroll 1
+      for (int half = C::kSets == 2 ? set : 0; half < (C::kSets == 2 ? set + 1 : 2) && ok; ++half) {
+        const int c0 = half * kHalf;
+        // of the half's keys (queries) and the warp's rows: is there one that sees, do all
+        const Seen seen = KEYS ? s_span[n & 1][half].of(span.x + quarter * 32) : reach.of(o0 + c0);
+        uint32_t w[16], e[16];
+        if (seen != kNone) {
+          uint32_t x[kHalf], y[kHalf];
+          tmem_get32(mine + c0, x);
+          tmem_get32(mine + 64 + c0, y);
+          tmem_wait_ld();
+          // y: (dP - delta) times the slant; x: the score in units of log 2 (over `unit`)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (!ok || (C::kSets == 2 && half != set)) continue;
-        const int c0 = half * 32;
-        uint32_t x[32], y[32];
-        tmem_get32(mine + c0, x);
-        tmem_get32(mine + 64 + c0, y);
-        tmem_wait_ld();
+          for (int c = 0; c < kHalf; c += 2) {
+            const F2 d = KEYS ? *reinterpret_cast<const F2*>(&s_delta[n & 1][c0 + c]) : f2(-delta, -delta);
+            const float2 v = un(fma2(f2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), f2(sigma, sigma), d));
+            y[c] = __float_as_uint(v.x);
+            y[c + 1] = __float_as_uint(v.y);
+          }
+          float left = unit;
+          if (p.cap > 0.0f) {
+            const float in = p.scale / p.cap * (2.0f * kLog2e);
+            const F2 in2 = f2(in, in), one = f2(1.0f, 1.0f), minus = f2(-2.0f, -2.0f);
+#pragma unroll
+            for (int c = 0; c < kHalf; c += 2) {
+              const float2 v = un(mul2(pair(x + c), in2));
+              const float2 d = un(add2(f2(exp2_fast(v.x), exp2_fast(v.y)), one));
+              const F2 th = fma2(f2(rcp_fast(d.x), rcp_fast(d.y)), minus, one);
+              const float2 t = un(th);
+              put(x + c, th);
+              put(y + c, mul2(pair(y + c), fma2(f2(-t.x, -t.y), th, one)));
+            }
+          }
+          if (slope2 != 0.0f) {
+#pragma unroll
+            for (int c = 0; c < kHalf; ++c) {
+              const int far = KEYS ? s_row[n & 1][c0 + c].z - r : row.z - (o0 + c0 + c);
+              x[c] = __float_as_uint(fmaf(-slope2, fabsf((float)far), __uint_as_float(x[c]) * left));
+            }
+            left = 1.0f;
+          }
+          if (seen == kSome) {
+#pragma unroll
+            for (int c = 0; c < kHalf; ++c) {
+              int4 q = row;
+              if (KEYS) q = s_row[n & 1][c0 + c];
+              const int j = KEYS ? r : o0 + c0 + c;
+              if (!(j >= q.x && j < q.y)) {
+                x[c] = 0xff800000u;
+                y[c] = 0u;
+              }
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < kHalf; c += 2) {
+            const F2 l = KEYS ? *reinterpret_cast<const F2*>(&s_lse[n & 1][c0 + c]) : f2(-lse, -lse);
+            const float2 v = un(fma2(f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), f2(left, left), l));
+            const float a = exp2_fast(v.x), b = exp2_fast(v.y);
+            if (KEYS) w[c / 2] = pack2<T>(a, b);
+            const float2 g = un(mul2(f2(a, b), pair(y + c)));
+            e[c / 2] = pack2<T>(g.x, g.y);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) w[c] = e[c] = 0u;
+        }
         if (C::kApart && (C::kSets == 2 || half == 1)) {
           tc::tc_fence_before();
           mbar_arrive(smem_u32(&sfree));
         }
-        uint32_t w[16], e[16];
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          float pw[2], ew[2];
-#pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            float v = __uint_as_float(x[c + d]), slant = 1.0f;
-            float2 ld;
-            if (KEYS) ld = s_lse[n & 1][c0 + c + d];
-            else ld = make_float2(lse, delta);
-            if (p.cap > 0.0f) {
-              const float th = tanh_of(v * (p.scale / p.cap));
-              slant = fmaf(-th, th, 1.0f);
-              v = p.cap * kLog2e * th;
-            }
-            if (slope2 != 0.0f) {
-              const int far = KEYS ? s_row[n & 1][c0 + c + d].z - r : row.z - (o0 + c0 + c + d);
-              v = fmaf(-slope2, fabsf((float)far), v * unit) - ld.x;
-            } else {
-              v = fmaf(v, unit, -ld.x);
-            }
-            pw[d] = exp2_fast(v);
-            ew[d] = pw[d] * fmaf(__uint_as_float(y[c + d]), sigma, -ld.y) * slant;
-            if (!all) {
-              bool sees;
-              if (KEYS) {
-                const int4 q = s_row[n & 1][c0 + c + d];
-                sees = r >= q.x && r < q.y;
-              } else {
-                const int j = o0 + c0 + c + d;
-                sees = j >= row.x && j < row.y;
-              }
-              pw[d] = sees ? pw[d] : 0.0f;
-              ew[d] = sees ? ew[d] : 0.0f;
-            }
-          }
-          if (KEYS) w[c / 2] = pack2<T>(pw[0], pw[1]);
-          e[c / 2] = pack2<T>(ew[0], ew[1]);
-        }
         if (C::kApart && n > 0 && (C::kSets == 2 || half == 0)) {  // the products before have read their values
-          ok = mbar_wait_bounded(smem_u32(&done), (uint32_t)(n - 1) & 1u, kWaitTimeoutEpilogue, abort_flag);
-          ok = __all_sync(kAll, ok);
+          ok = __all_sync(kAll, wait_on(&done, (uint32_t)(n - 1), kWaitTimeoutEpilogue, abort_flag));
           tc::tc_fence_after();
         }
         if (ok) {
@@ -1028,7 +1292,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
       }
     }
     if (ok && blocks > 0) {
-      ok = mbar_wait_bounded(smem_u32(&done), (uint32_t)(blocks - 1) & 1u, kWaitTimeoutEpilogue, abort_flag);
+      ok = wait_on(&done, (uint32_t)(blocks - 1) & 1u, kWaitTimeoutEpilogue, abort_flag);
       tc::tc_fence_after();
     }
     ok = meet(ok);
@@ -1122,10 +1386,12 @@ static int launch(K kernel, dim3 grid, int threads, int smem, bool after, cudaSt
 static bool choose_by_segment(int64_t Tq, int64_t Tk, int64_t S) {
   if (S <= 0) return false;
   const double nq = (double)Tq / S, nk = (double)Tk / S;
-  const double own = S * std::ceil(nq / kTile) * std::ceil(nk / kBlock);
-  const double packed = std::ceil((double)Tq / kTile) * std::ceil(nk * (1.0 + kTile / std::max(nq, 1.0)) / kBlock);
+  const double own = S * (nq / kTile + 0.5) * (nk / kBlock + 0.5 + 2.0);  // a tile costs about two blocks besides its own
+  const double packed = ((double)Tq / kTile + 0.5) * (nk * (1.0 + kTile / std::max(nq, 1.0)) / kBlock + 0.5 + 2.0);
   return own < packed;
 }
+
+static int tiles_of(int64_t T, int64_t S, bool by_segment) { return (int)(by_segment ? T / kTile + S + 2 : (T + kTile - 1) / kTile); }
 
 template <typename T, int DP>
 static int run_forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
@@ -1142,10 +1408,9 @@ static int run_forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   if ((rc = make_map(&tmQ, p.q, p.D, p.H, p.Tq, p.q_t, p.q_h, kTile, dt))) return rc;
   if ((rc = make_map(&tmK, p.k, p.D, p.Hk, p.Tk, p.k_t, p.k_h, kBlock, dt))) return rc;
   if ((rc = make_map(&tmV, p.v, p.D, p.Hk, p.Tk, p.v_t, p.v_h, kBlock, dt))) return rc;
-  p.by_segment = choose_by_segment(p.Tq, p.Tk, p.S);
-  const int64_t tiles = p.by_segment ? p.Tq / kTile + p.S + 2 : ((int64_t)p.Tq + kTile - 1) / kTile;
+  const int64_t ctas = std::min<int64_t>((int64_t)p.n_tiles * p.H, (int64_t)sm_count() * C::kCtas);
   void* args[] = {&tmQ, &tmK, &tmV, &p};
-  return launch(forward_kernel<T, DP>, dim3((unsigned)tiles, p.H), kThreads, C::kSmem, true, st, "attention forward_kernel launch", args);
+  return launch(forward_kernel<T, DP>, dim3((unsigned)ctas), C::kThreads, C::kSmem, true, st, "attention forward_kernel launch", args);
 }
 
 static bool tiled(const Params& p) {
@@ -1156,10 +1421,13 @@ static bool tiled(const Params& p) {
 template <typename T>
 static int forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   int rc;
-  rows_kernel<<<(p.Tq + 255) / 256, 256, 0, st>>>(p);
-  if ((rc = check_cuda(cudaGetLastError(), "attention rows_kernel launch"))) return rc;
-  if (tiled(p) && p.Tk > 0 && aligned(p.out, 16))
-    return p.D <= 64 ? run_forward<T, 64>(p, dt, st) : run_forward<T, 128>(p, dt, st);
+  const bool tiles = tiled(p) && p.Tk > 0 && aligned(p.out, 16);
+  p.by_segment = choose_by_segment(p.Tq, p.Tk, p.S);
+  p.n_tiles = tiles_of(p.Tq, p.S, p.by_segment);
+  if (!tiles) p.tiles = nullptr;
+  plan_kernel<T><<<p.n_tiles, kTile, 0, st>>>(p);
+  if ((rc = check_cuda(cudaGetLastError(), "attention plan_kernel launch"))) return rc;
+  if (tiles) return p.D <= 64 ? run_forward<T, 64>(p, dt, st) : run_forward<T, 128>(p, dt, st);
   void* args[] = {&p};
   return launch(row_kernel<T, kRowForward>, dim3((unsigned)(((int64_t)p.Tq * p.H + 7) / 8)), 256, 0, true, st,
                 "attention row_kernel launch", args);
@@ -1195,9 +1463,15 @@ static int backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   int rc;
   const bool peaks = std::is_same<T, __half>::value;
   if (peaks && (rc = check_cuda(cudaMemsetAsync(p.peaks, 0, 8, st), "attention peaks"))) return rc;
-  const int64_t warps = (int64_t)p.Tq * p.H + (peaks ? (int64_t)p.Tk * p.Hk : 0);
-  if (warps > 0) {
-    delta_kernel<T><<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(p);
+  const int64_t heads = (int64_t)p.Tq * p.H + (peaks ? (int64_t)p.Tk * p.Hk : 0);
+  if (heads > 0) {
+    const bool vec = p.D % 8 == 0 && aligned(p.o, 16) && mappable(p.g, p.Tq, p.H, p.g_t, p.g_h) && mappable(p.v, p.Tk, p.Hk, p.v_t, p.v_h);
+    const int lanes = !vec || p.D > 128 ? 32 : p.D > 64 ? 16 : 8;
+    const unsigned grid = (unsigned)((p.Tq + 255) / 256 + std::min<int64_t>((heads * lanes + 255) / 256, (int64_t)sm_count() * kDeltaCtas));
+    if (!vec) delta_kernel<T, 32, false><<<grid, 256, 0, st>>>(p);
+    else if (lanes == 32) delta_kernel<T, 32, true><<<grid, 256, 0, st>>>(p);
+    else if (lanes == 16) delta_kernel<T, 16, true><<<grid, 256, 0, st>>>(p);
+    else delta_kernel<T, 8, true><<<grid, 256, 0, st>>>(p);
     if ((rc = check_cuda(cudaGetLastError(), "attention delta_kernel launch"))) return rc;
   }
   const bool tiles = tiled(p) && p.Tq > 0 && p.Tk > 0 && mappable(p.g, p.Tq, p.H, p.g_t, p.g_h) && aligned(p.dq, 16) &&
@@ -1222,6 +1496,7 @@ static int check(const Params& p, int dtype, int64_t Tq, int64_t Tk, int64_t S, 
   if (p.H % p.Hk != 0) return fail(RB_ERR_VALUE, "%d query heads cannot share %d key heads", p.H, p.Hk);
   if (p.D > kMaxWidth) return fail(RB_ERR_UNSUPPORTED, "heads wider than %d", kMaxWidth);
   if (Tq > 1 << 30 || Tk > 1 << 30 || S > 1 << 30 || p.H > 65535) return fail(RB_ERR_UNSUPPORTED, "more than 2^30 tokens or segments, or 65535 heads");
+  if ((Tq / kTile + Tk / kTile + S + 2) * p.H > 0x7fffffffLL) return fail(RB_ERR_UNSUPPORTED, "more than 2^31 tiles of all heads");
   if (!(p.scale > 0.0f) || !(p.scale < INFINITY)) return fail(RB_ERR_VALUE, "scale must be positive");
   if (!(p.cap >= 0.0f) || !(p.cap < INFINITY)) return fail(RB_ERR_VALUE, "cap must be positive, or 0 for none");
   return RB_OK;
@@ -1234,7 +1509,7 @@ using namespace rb;
 
 extern "C" int64_t rb_segment_attention_workspace_size(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D) {
   if (Tq < 0 || Tk < 0 || S < 0 || H <= 0 || Hk <= 0 || D <= 0 || Tq > 1 << 30) return -1;
-  return Tq * 16;
+  return 16 + Tq * 16 + (Tq / attn::kTile + S + 2) * 16;
 }
 
 extern "C" int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h,
@@ -1265,7 +1540,9 @@ extern "C" int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, con
   p.v = v;
   p.out = out;
   p.lse = lse;
-  p.rows = static_cast<int4*>(workspace);
+  p.next = static_cast<uint32_t*>(workspace);
+  p.rows = static_cast<int4*>(workspace) + 1;
+  p.tiles = p.rows + Tq;
   p.q_off = q_offsets;
   p.k_off = k_offsets;
   p.prefix = prefix;
