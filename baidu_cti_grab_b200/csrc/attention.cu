@@ -39,6 +39,8 @@ struct Params {
   int4* rows;                     // [Tq]: lo, hi, place of the query among the packed keys, 0
   int4* tiles;                    // of the queries: rows [x, y), the keys that they see [z, w)
   uint32_t* next;                 // tickets for work
+  float* part;                    // few queries: of every row and split, the sums [D], their maximum and their weights' sum
+  int splits;
   const void *q_off, *k_off, *prefix;
   const float* slopes;
   int64_t q_t, q_h, k_t, k_h, v_t, v_h, g_t, g_h;  // elements from token to token and from head to head
@@ -106,26 +108,27 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 constexpr int kTile = 128;  // rows of a tile: the lanes of TMEM
 
-// The rows [x, y) of tile b.  By the packed order, 128 rows a tile.  By segment, segment s has room for tiles from
-// floor(start / 128) + s on, which is as much as it needs and known without a sum over segments; the rows before the
-// first and behind the last count as segments too, and a tile that its segment does not need is empty.
-__device__ __forceinline__ int2 tile_rows(const void* off, int wide, int S, int total, int b, int by_segment) {
-  if (!by_segment) return make_int2(min(b * kTile, total), min((b + 1) * kTile, total));
-  // starts 0, off[0], ..., off[S]: the last i with floor(start_i / 128) + i <= b
+// The rows [x, y) of tile b of `size` rows.  By the packed order, 128 rows a tile.  By segment, segment s has room for
+// tiles from floor(start / size) + s on, which is as much as it needs and known without a sum over segments; the rows
+// before the first and behind the last count as segments too, and a tile that its segment does not need is empty.
+// A token may be `factor` rows.
+__device__ __forceinline__ int2 tile_rows(const void* off, int wide, int S, int total, int b, int by_segment, int size = kTile, int factor = 1) {
+  if (!by_segment) return make_int2(min(b * size, total * factor), min((b + 1) * size, total * factor));
+  // starts 0, off[0], ..., off[S]: the last i with floor(start_i / size) + i <= b
   int lo = 0, hi = S + 2;
   const int lane = threadIdx.x & 31;
   while (hi - lo > 1) {  // 32 probes at once
     const int step = (hi - lo + 31) / 32;
     const int i = lo + (lane + 1) * step;
-    const bool below = i < hi && offset_at(off, wide, i - 1, total) / kTile + i <= b;
+    const bool below = i < hi && offset_at(off, wide, i - 1, total) * factor / size + i <= b;
     const int n = __popc(__ballot_sync(kAll, below));
     lo += n * step;
     hi = min(hi, lo + step);
   }
-  const int start = lo == 0 ? 0 : offset_at(off, wide, lo - 1, total);
-  const int end = lo == S + 1 ? total : offset_at(off, wide, lo, total);
-  const int first = start + (b - (start / kTile + lo)) * kTile;
-  return make_int2(min(first, end), min(first + kTile, end));
+  const int start = lo == 0 ? 0 : offset_at(off, wide, lo - 1, total) * factor;
+  const int end = lo == S + 1 ? total * factor : offset_at(off, wide, lo, total) * factor;
+  const int first = start + (b - (start / size + lo)) * size;
+  return make_int2(min(first, end), min(first + size, end));
 }
 
 // The rows' intervals, once a call for all heads, a CTA a tile; and what its rows see together.  A tile that sees nothing
@@ -958,6 +961,292 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
   }
 }
 
+// ------------------------------------------------- few queries, long histories
+// Some queries of a segment over many keys (a user's new items over a cached history): bound by reading the keys and
+// values once.  A CTA takes 16 rows (a key head's query heads, for one token or several) and one of `splits` parts of
+// the segment's keys, so that a single query still fills the GPU; a producer warp keeps kStages blocks of 64 keys
+// coming, and each of four warps takes 16 keys of a block with products of 16 x 8 x 16 (most of the 128 rows of the
+// larger tensor-core products would be empty here).  Warps, then parts, are added up in their order.
+template <int DP>
+struct Few {
+  static constexpr int kRows = 16, kWarps = 4, kThreads = 32 * (kWarps + 1);
+  static constexpr int kChunks = DP / 64;
+  static constexpr int kBytes = kBlock * 128 * kChunks;  // of a block's keys, and of its values
+  static constexpr int kStages = DP == 64 ? 4 : 3;
+  static constexpr int kSmem = 1024 + kStages * 2 * kBytes;
+  static constexpr int kCtas = DP == 64 ? 3 : 2;
+  static_assert(kWarps * kRows * (DP + 4) * 4 <= kStages * 2 * kBytes, "the warps' sums lie where the blocks did");
+};
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_turned(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(Few<DP>::kThreads, Few<DP>::kCtas)
+    few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
+  using C = Few<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile = blockIdx.x / p.splits, split = blockIdx.x % p.splits, hk = blockIdx.y;
+  const int2 span = tile_rows(p.q_off, p.off64, p.S, p.Tq, tile, 1, C::kRows, p.G);
+  if (span.x >= span.y) return;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), C::kWarps);
+    }
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // rows g and g + 8 of the tile are this thread's; a row is (token, head of the group)
+  const int g = lane >> 2, q4 = lane & 3;
+  int4 mine[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = span.x + g + 8 * i;
+    mine[i] = row < span.y ? __ldg(p.rows + row / p.G) : make_int4(0, 0, 0, 0);
+  }
+  const Span a = span_of(mine[0]), b = span_of(mine[1]);
+  const int lo = min(a.lo_min, b.lo_min), hi = max(a.hi_max, b.hi_max);  // of all rows
+  const int all_lo = max(a.lo_max, b.lo_max), all_hi = min(a.hi_min, b.hi_min);
+  // this part of the keys: whole blocks
+  const int blocks_all = hi > lo ? (hi - lo + kBlock - 1) / kBlock : 0;
+  const int first = (int)((int64_t)blocks_all * split / p.splits), blocks = (int)((int64_t)blocks_all * (split + 1) / p.splits) - first;
+  const int key0 = lo + first * kBlock;
+
+  if (warp == C::kWarps) {
+    if (lane == 0) {
+      int n = 0;
+      for (; n < blocks; ++n) {
+        const int s = n % C::kStages;
+        if (!wait_on(&empty[s], (uint32_t)(n / C::kStages) ^ 1u, kWaitTimeoutProducer, abort_flag)) break;
+        const uint32_t bar = smem_u32(&full[s]), to = smem_u32(smem + s * 2 * C::kBytes);
+        mbar_arrive_expect_tx(bar, 2 * C::kBytes);
+        for (int c = 0; c < C::kChunks; ++c) {
+          tma_load_3d(to + c * kBlock * 128, &tmK, 64 * c, hk, key0 + n * kBlock, bar);
+          tma_load_3d(to + C::kBytes + c * kBlock * 128, &tmV, 64 * c, hk, key0 + n * kBlock, bar);
+        }
+      }
+      for (int i = max(0, n - C::kStages); i < n; ++i) wait_on(&full[i % C::kStages], (uint32_t)(i / C::kStages), kWaitTimeoutProducer, nullptr);
+    }
+  }
+  float top[2] = {-INFINITY, -INFINITY}, total[2] = {0.0f, 0.0f}, o[DP / 8][4];
+#pragma unroll
+  for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[i][c] = 0.0f;
+  bool ok = true;
+  if (warp < C::kWarps && blocks > 0) {
+    uint32_t q[DP / 16][4];
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int row = span.x + g + 8 * (c & 1), col = 16 * k + 8 * (c >> 1) + 2 * q4;
+        const T* from = static_cast<const T*>(p.q) + (int64_t)(row / p.G) * p.q_t + (int64_t)(hk * p.G + row % p.G) * p.q_h + col;
+        q[k][c] = row < span.y && col < p.D ? __ldg(reinterpret_cast<const uint32_t*>(from)) : 0u;
+      }
+    float slope2[2] = {0.0f, 0.0f};
+    if (p.slopes != nullptr)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) slope2[i] = kLog2e * __ldg(p.slopes + hk * p.G + (span.x + g + 8 * i) % p.G);
+    const float unit = p.cap > 0.0f ? 1.0f : p.scale * kLog2e;
+    const int key = 16 * warp + (lane & 7) + 8 * ((lane >> 3) & 1);  // the row of a block that this lane points ldmatrix at
+    const int half = lane >> 4;                                      // and which eight of sixteen columns
+    for (int n = 0; n < blocks; ++n) {
+      const int s = n % C::kStages, j0 = key0 + n * kBlock + 16 * warp;
+      ok = __all_sync(kAll, wait_on(&full[s], (uint32_t)(n / C::kStages), kWaitTimeoutEpilogue, abort_flag));
+      if (!ok) break;
+      if (j0 < hi) {
+        const uint32_t at = smem_u32(smem + s * 2 * C::kBytes) + key * 128;
+        float x[2][4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[0][c] = x[1][c] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          uint32_t r[4];  // keys 0-7 and 8-15 of the first eight columns, then of the second
+          ldsm4(at + (k >> 2) * kBlock * 128 + ((((k & 3) * 2 + half) ^ (key & 7)) << 4), r);
+          mma16<T>(x[0], q[k], r[0], r[2]);
+          mma16<T>(x[1], q[k], r[1], r[3]);
+        }
+        // x[e][2 i + d]: row g + 8 i, key j0 + 8 e + 2 q4 + d
+        const bool every = j0 >= all_lo && j0 + 16 <= all_hi;
+        float high[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int i = c >> 1, j = j0 + 8 * e + 2 * q4 + (c & 1);
+            float v = x[e][c];
+            if (p.cap > 0.0f) v = p.cap * kLog2e * tanh_of(v * (p.scale / p.cap));
+            else v *= unit;
+            v = fmaf(-slope2[i], (float)abs(mine[i].z - j), v);
+            if (!every && !(j >= mine[i].x && j < mine[i].y)) v = -INFINITY;
+            x[e][c] = v;
+            high[i] = fmaxf(high[i], v);
+          }
+        float keep[2], shift[2];
+        bool grow = false;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          high[i] = fmaxf(high[i], __shfl_xor_sync(kAll, high[i], 1));
+          high[i] = fmaxf(high[i], __shfl_xor_sync(kAll, high[i], 2));
+          keep[i] = 1.0f;
+          if (high[i] > top[i] + 8.0f || (top[i] == -INFINITY && high[i] > -INFINITY)) {
+            keep[i] = exp2_fast(top[i] - high[i]);
+            top[i] = high[i];
+            grow = true;
+          }
+          shift[i] = top[i] == -INFINITY ? 0.0f : top[i];
+        }
+        if (__any_sync(kAll, grow)) {
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i) {
+            o[i][0] *= keep[0];
+            o[i][1] *= keep[0];
+            o[i][2] *= keep[1];
+            o[i][3] *= keep[1];
+          }
+          total[0] *= keep[0];
+          total[1] *= keep[1];
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float u = exp2_fast(x[e][2 * i] - shift[i]), v = exp2_fast(x[e][2 * i + 1] - shift[i]);
+            total[i] += u + v;
+            w[2 * e + i] = pack2<T>(u, v);
+          }
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          uint32_t r[4];  // keys 0-7 and 8-15 of eight columns, then of the next eight
+          ldsm4_turned(at + C::kBytes + (k >> 2) * kBlock * 128 + ((((k & 3) * 2 + half) ^ (key & 7)) << 4), r);
+          mma16<T>(o[2 * k], w, r[0], r[1]);
+          mma16<T>(o[2 * k + 1], w, r[2], r[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
+    }
+  }
+  ok = __syncthreads_and(ok);
+  if (!ok) return;
+  // the warps' sums, on one maximum: [warp][row][D], then maximum and sum
+  float* sums = reinterpret_cast<float*>(smem);
+  float* tops = sums + C::kWarps * C::kRows * DP;
+  float* totals = tops + C::kWarps * C::kRows;
+  if (warp < C::kWarps) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      total[i] += __shfl_xor_sync(kAll, total[i], 1);
+      total[i] += __shfl_xor_sync(kAll, total[i], 2);
+      if (q4 == 0) {
+        tops[warp * C::kRows + g + 8 * i] = top[i];
+        totals[warp * C::kRows + g + 8 * i] = total[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) {
+      float* to = sums + (warp * C::kRows + g) * DP + 8 * i + 2 * q4;
+      *reinterpret_cast<float2*>(to) = make_float2(o[i][0], o[i][1]);
+      *reinterpret_cast<float2*>(to + 8 * DP) = make_float2(o[i][2], o[i][3]);
+    }
+  }
+  __syncthreads();
+  const int rows = span.y - span.x;
+  for (int r = warp; r < rows; r += C::kWarps + 1) {  // a warp a row
+    float high = -INFINITY, sum = 0.0f, scale[C::kWarps];
+#pragma unroll
+    for (int w = 0; w < C::kWarps; ++w) high = fmaxf(high, tops[w * C::kRows + r]);
+#pragma unroll
+    for (int w = 0; w < C::kWarps; ++w) {
+      scale[w] = high == -INFINITY ? 1.0f : exp2_fast(tops[w * C::kRows + r] - high);
+      sum = fmaf(scale[w], totals[w * C::kRows + r], sum);
+    }
+    const int token = (span.x + r) / p.G, h = hk * p.G + (span.x + r) % p.G;
+    const int64_t at = (int64_t)token * p.H + h;
+    bool finite = sum < INFINITY;
+    for (int c = lane; c < p.D; c += 32) {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < C::kWarps; ++w) v = fmaf(scale[w], sums[(w * C::kRows + r) * DP + c], v);
+      if (p.splits > 1) {
+        p.part[(at * p.splits + split) * (p.D + 2) + c] = v;
+      } else {
+        finite = finite && fabsf(v) < INFINITY;
+        static_cast<T*>(p.out)[at * p.D + c] = T(sum == 0.0f ? 0.0f : v / sum);
+      }
+    }
+    if (p.splits > 1) {
+      if (lane < 2) p.part[(at * p.splits + split) * (p.D + 2) + p.D + lane] = lane ? sum : high;
+    } else {
+      if (lane == 0 && p.lse != nullptr) p.lse[(int64_t)h * p.Tq + token] = sum == 0.0f ? -INFINITY : kLn2 * (high + log2f(sum));
+      if (!__all_sync(kAll, finite)) {
+        __syncwarp();
+        row_forward<T>(p, token, h);
+      }
+    }
+  }
+}
+
+// the parts of a row, a warp a row of one head
+template <typename T>
+__global__ void __launch_bounds__(256) few_join_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (at >= (int64_t)p.Tq * p.H) return;
+  const float* part = p.part + at * p.splits * (p.D + 2);
+  float high = -INFINITY, sum = 0.0f;
+  for (int s = lane; s < p.splits; s += 32) high = fmaxf(high, part[s * (p.D + 2) + p.D]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) high = fmaxf(high, __shfl_xor_sync(kAll, high, o));
+  for (int s = 0; s < p.splits; ++s) {
+    const float w = high == -INFINITY ? 1.0f : exp2_fast(part[s * (p.D + 2) + p.D] - high);
+    sum = fmaf(w, part[s * (p.D + 2) + p.D + 1], sum);
+  }
+  bool finite = sum < INFINITY;
+  for (int c = lane; c < p.D; c += 32) {
+    float v = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+      const float w = high == -INFINITY ? 1.0f : exp2_fast(part[s * (p.D + 2) + p.D] - high);
+      v = fmaf(w, part[s * (p.D + 2) + c], v);
+    }
+    finite = finite && fabsf(v) < INFINITY;
+    static_cast<T*>(p.out)[at * p.D + c] = T(sum == 0.0f ? 0.0f : v / sum);
+  }
+  const int token = (int)(at / p.H), h = (int)(at % p.H);
+  if (lane == 0 && p.lse != nullptr) p.lse[(int64_t)h * p.Tq + token] = sum == 0.0f ? -INFINITY : kLn2 * (high + log2f(sum));
+  if (!__all_sync(kAll, finite)) {
+    __syncwarp();
+    row_forward<T>(p, token, h);
+  }
+}
+
+
 // --------------------------------------------------------------- backward
 // Two kernels of one form, and no atomics: the same bits every time.  KEYS false: a CTA's 128 rows are queries of one
 // head, it goes over blocks of 64 keys and sums dq.  KEYS true: its rows are keys of one key head, it goes over blocks
@@ -1413,6 +1702,38 @@ static int run_forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   return launch(forward_kernel<T, DP>, dim3((unsigned)ctas), C::kThreads, C::kSmem, true, st, "attention forward_kernel launch", args);
 }
 
+// How many parts the keys of a segment are split into where there are few queries, 0: not that kernel.  It reads a key
+// head's keys once for 16 rows; the tiles read them once for 128, but fill 128 rows with what there is.
+static int splits_of(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D) {
+  const int64_t G = H / Hk;
+  if (S <= 0 || D % 8 != 0 || D > 128 || Tk < 4 * Tq || Tq * G > 32 * S || Tq * G > 1 << 30) return 0;
+  const int64_t ctas = std::max<int64_t>(1, S * ((Tq * G / S + 15) / 16) * Hk), want = (int64_t)sm_count() * 16;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(want + ctas - 1) / ctas, Tk / S / 256, 64}));
+}
+
+template <typename T, int DP>
+static int run_few(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
+  using C = Few<DP>;
+  static std::once_flag once[64];
+  int dev = 0, rc;
+  cudaGetDevice(&dev);
+  cudaError_t e = cudaSuccess;
+  std::call_once(once[dev & 63], [&] {
+    e = cudaFuncSetAttribute(few_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  });
+  if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(attention few_kernel)");
+  CUtensorMap tmK, tmV;
+  if ((rc = make_map(&tmK, p.k, p.D, p.Hk, p.Tk, p.k_t, p.k_h, kBlock, dt))) return rc;
+  if ((rc = make_map(&tmV, p.v, p.D, p.Hk, p.Tk, p.v_t, p.v_h, kBlock, dt))) return rc;
+  const int64_t tiles = (int64_t)p.Tq * p.G / C::kRows + p.S + 2;
+  void* args[] = {&tmK, &tmV, &p};
+  if ((rc = launch(few_kernel<T, DP>, dim3((unsigned)(tiles * p.splits), p.Hk), C::kThreads, C::kSmem, true, st, "attention few_kernel launch", args)))
+    return rc;
+  if (p.splits == 1) return RB_OK;
+  void* join[] = {&p};
+  return launch(few_join_kernel<T>, dim3((unsigned)(((int64_t)p.Tq * p.H + 7) / 8)), 256, 0, true, st, "attention few_join_kernel launch", join);
+}
+
 static bool tiled(const Params& p) {
   return p.D % 8 == 0 && p.D <= 128 && mappable(p.q, p.Tq, p.H, p.q_t, p.q_h) && mappable(p.k, p.Tk, p.Hk, p.k_t, p.k_h) &&
          mappable(p.v, p.Tk, p.Hk, p.v_t, p.v_h);
@@ -1423,10 +1744,12 @@ static int forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   int rc;
   const bool tiles = tiled(p) && p.Tk > 0 && aligned(p.out, 16);
   p.by_segment = choose_by_segment(p.Tq, p.Tk, p.S);
+  p.splits = tiles ? splits_of(p.Tq, p.Tk, p.S, p.H, p.Hk, p.D) : 0;
   p.n_tiles = tiles_of(p.Tq, p.S, p.by_segment);
-  if (!tiles) p.tiles = nullptr;
+  if (!tiles || p.splits > 0) p.tiles = nullptr;
   plan_kernel<T><<<p.n_tiles, kTile, 0, st>>>(p);
   if ((rc = check_cuda(cudaGetLastError(), "attention plan_kernel launch"))) return rc;
+  if (p.splits > 0) return p.D <= 64 ? run_few<T, 64>(p, dt, st) : run_few<T, 128>(p, dt, st);
   if (tiles) return p.D <= 64 ? run_forward<T, 64>(p, dt, st) : run_forward<T, 128>(p, dt, st);
   void* args[] = {&p};
   return launch(row_kernel<T, kRowForward>, dim3((unsigned)(((int64_t)p.Tq * p.H + 7) / 8)), 256, 0, true, st,
@@ -1509,7 +1832,9 @@ using namespace rb;
 
 extern "C" int64_t rb_segment_attention_workspace_size(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D) {
   if (Tq < 0 || Tk < 0 || S < 0 || H <= 0 || Hk <= 0 || D <= 0 || Tq > 1 << 30) return -1;
-  return 16 + Tq * 16 + (Tq / attn::kTile + S + 2) * 16;
+  const int64_t splits = H % Hk == 0 ? attn::splits_of(Tq, Tk, S, H, Hk, D) : 0;
+  const int64_t lists = 16 + Tq * 16 + (Tq / attn::kTile + S + 2) * 16;
+  return lists + (splits > 1 ? Tq * H * splits * (D + 2) * 4 : 0);
 }
 
 extern "C" int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h,
@@ -1543,6 +1868,7 @@ extern "C" int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, con
   p.next = static_cast<uint32_t*>(workspace);
   p.rows = static_cast<int4*>(workspace) + 1;
   p.tiles = p.rows + Tq;
+  p.part = reinterpret_cast<float*>(p.tiles + (Tq / kTile + S + 2));
   p.q_off = q_offsets;
   p.k_off = k_offsets;
   p.prefix = prefix;
