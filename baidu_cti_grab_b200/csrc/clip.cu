@@ -20,7 +20,7 @@ namespace rb {
 namespace clip {
 
 constexpr int kMaxTensors = 448, kFewTensors = 24;  // (parameters are copied at every launch: few tensors, few bytes)
-constexpr int kThreads = 256, kPer = 32, kPiece = kThreads * kPer;
+constexpr int kThreads = 256, kPer = 32, kPiece = kThreads * kPer, kCtas = 4;  // CTAs an SM holds: the grid is one wave
 
 struct Tensor {
   const void* from;
@@ -167,12 +167,25 @@ __device__ __forceinline__ double block_sum(double v) {
   return s;
 }
 
+// A CTA takes neighbouring pieces: the tensor is searched for once, then stepped to.  The second kernel takes them in the
+// opposite order, so that what the first read last, which L2 still holds, is read first.
+struct Range {
+  int first, last;
+};
 template <int N>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Params<N> p) {
+__device__ __forceinline__ Range pieces_of(const Params<N>& p) {
+  return Range{(int)((int64_t)p.pieces * blockIdx.x / gridDim.x), (int)((int64_t)p.pieces * (blockIdx.x + 1) / gridDim.x)};
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads, kCtas) norm_kernel(const __grid_constant__ Params<N> p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   double sum = 0.0;
-  for (int i = blockIdx.x; i < p.pieces; i += gridDim.x) {
-    const Tensor& t = p.t[tensor_of(p, i)];
+  const Range q = pieces_of(p);
+  int at_tensor = q.first < q.last ? tensor_of(p, q.first) : 0;
+  for (int i = q.first; i < q.last; ++i) {
+    while (at_tensor + 1 < p.tensors && p.t[at_tensor + 1].first <= i) ++at_tensor;
+    const Tensor& t = p.t[at_tensor];
     const int64_t at = (int64_t)(i - t.first) * kPiece, n = values_of(t);
     if (at >= n) continue;
     if (t.dtype == RB_BF16) sum += squares<RB_BF16>(t.from, at, n, t.vec);
@@ -189,25 +202,29 @@ __device__ __forceinline__ void scaled(const void* from, void* to, int64_t at, i
   const typename Y::T* x = static_cast<const typename Y::T*>(from);
   typename Y::T* y = static_cast<typename Y::T*>(to);
   if (vec) {
-    uint4 w[kPer / Y::kVec];
+    constexpr int kBatch = 4;  // loads in flight (more did not fit the registers of four CTAs)
+#pragma unroll 1
+    for (int k0 = 0; k0 < kPer / Y::kVec; k0 += kBatch) {
+      uint4 w[kBatch];
+      const int64_t i0 = at + (int64_t)(k0 * kThreads + threadIdx.x) * Y::kVec;
 #pragma unroll
-    for (int k = 0; k < kPer / Y::kVec; ++k) {
-      const int64_t i = at + (int64_t)(k * kThreads + threadIdx.x) * Y::kVec;
-      if (i + Y::kVec <= n) w[k] = *reinterpret_cast<const uint4*>(x + i);
-    }
+      for (int k = 0; k < kBatch; ++k)
+        if (i0 + (k * kThreads + 1) * Y::kVec <= n) w[k] = *reinterpret_cast<const uint4*>(x + i0 + k * kThreads * Y::kVec);
 #pragma unroll
-    for (int k = 0; k < kPer / Y::kVec; ++k) {
-      const int64_t i = at + (int64_t)(k * kThreads + threadIdx.x) * Y::kVec;
-      if (i + Y::kVec <= n) {
-        float v[Y::kVec];
-        Y::widen(w[k], v);
+      for (int k = 0; k < kBatch; ++k) {
+        const int64_t i = i0 + k * kThreads * Y::kVec;
+        if (i + Y::kVec <= n) {
+          float v[Y::kVec];
+          Y::widen(w[k], v);
 #pragma unroll
-        for (int c = 0; c < Y::kVec; ++c) v[c] *= f;
-        *reinterpret_cast<uint4*>(y + i) = Y::narrow(v);
-      } else {
-        for (int64_t c = i; c < n; ++c) y[c] = typename Y::T((float)x[c] * f);
+          for (int c = 0; c < Y::kVec; ++c) v[c] *= f;
+          *reinterpret_cast<uint4*>(y + i) = Y::narrow(v);
+        }
       }
     }
+    // the last values, off the vectors: by the first threads of the CTA that has them
+    const int64_t tail = n / Y::kVec * Y::kVec;
+    if (tail >= at && tail < at + kPiece && tail + threadIdx.x < n && threadIdx.x < Y::kVec) y[tail + threadIdx.x] = typename Y::T((float)x[tail + threadIdx.x] * f);
   } else {
 #pragma unroll 4
     for (int k = 0; k < kPer; ++k) {
@@ -219,7 +236,7 @@ __device__ __forceinline__ void scaled(const void* from, void* to, int64_t at, i
 
 // most < 0: the norm alone
 template <int N>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Params<N> p) {
+__global__ void __launch_bounds__(kThreads, kCtas) scale_kernel(const __grid_constant__ Params<N> p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   double sum = 0.0;
   for (int i = threadIdx.x; i < p.slots; i += kThreads) sum += p.sums[i];
@@ -228,8 +245,11 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
   if (p.most < 0.0f) return;
   float f = p.most / (norm + 1e-6f);
   f = p.scale * (f < 1.0f || f != f ? f : 1.0f);
-  for (int i = blockIdx.x; i < p.pieces; i += gridDim.x) {
-    const Tensor& t = p.t[tensor_of(p, i)];
+  const Range q = pieces_of(p);
+  int at_tensor = q.first < q.last ? tensor_of(p, q.last - 1) : 0;
+  for (int i = q.last - 1; i >= q.first; --i) {
+    while (at_tensor > 0 && p.t[at_tensor].first > i) --at_tensor;
+    const Tensor& t = p.t[at_tensor];
     if (f == 1.0f && t.from == t.to) continue;
     const int64_t at = (int64_t)(i - t.first) * kPiece, n = values_of(t);
     if (at >= n) continue;
@@ -240,7 +260,7 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
 }
 
 // CTAs of a launch, at most
-static int grid_of(int64_t pieces) { return (int)std::min<int64_t>(std::max<int64_t>(pieces, 1), (int64_t)sm_count() * 8); }
+static int grid_of(int64_t pieces) { return (int)std::min<int64_t>(std::max<int64_t>(pieces, 1), (int64_t)sm_count() * kCtas); }
 
 struct List {
   const void* const* from;
@@ -316,7 +336,7 @@ using namespace rb;
 extern "C" int64_t rb_grad_norm_workspace_size(int tensors) {
   if (tensors < 0) return -1;
   const int64_t launches = std::max<int64_t>(1, (tensors + clip::kMaxTensors - 1) / clip::kMaxTensors);
-  return launches * sm_count() * 8 * 8;
+  return launches * sm_count() * clip::kCtas * 8;
 }
 
 extern "C" int rb_clip_grads(const void* const* from, void* const* to, const int64_t* values, const int* dtypes,

@@ -44,29 +44,37 @@ struct Params {
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 
-// VEC values from memory as fp32
 template <typename T, int VEC>
-__device__ __forceinline__ void load_values(const T* p, float* v) {
-  if constexpr (VEC == 1) {
-    v[0] = to_f32(__ldg(p));
-  } else {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+struct Raw {  // VEC values as they lie in memory
+  typename std::conditional<VEC == 1, T, uint4>::type v;
+  __device__ void load(const T* from) { v = __ldg(reinterpret_cast<const decltype(v)*>(from)); }
+  __device__ void widen(float* f) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, float>::value) {
-        v[i] = __uint_as_float(u[i]);
-      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        v[2 * i] = bf16_lo(u[i]);
-        v[2 * i + 1] = bf16_hi(u[i]);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+    for (int i = 0; i < VEC; ++i) f[i] = 0.0f;
+    add_to(f);
+  }
+  __device__ void add_to(float* acc) const {
+    if constexpr (VEC == 1) {
+      acc[0] += to_f32(v);
+    } else {
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, float>::value) {
+          acc[i] += __uint_as_float(u[i]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          acc[2 * i] += bf16_lo(u[i]);
+          acc[2 * i + 1] += bf16_hi(u[i]);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+          acc[2 * i] += f.x;
+          acc[2 * i + 1] += f.y;
+        }
       }
     }
   }
-}
+};
+
 // VEC values to memory as T2, whole words where there are several (from an aligned address)
 template <typename T2, int VEC>
 __device__ __forceinline__ void store_as(T2* p, const float* v) {
@@ -115,67 +123,65 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int wide, int64_t i) {
 }
 
 // ----------------------------------------------------------------- lookup
-constexpr int kRowsAThread = 4;  // loads in flight
+constexpr int kLookupRows = 4, kLookupWide = 2;  // rows, and loads of a row, that a thread has in flight
 
+// teams of p.team lanes, a row each
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) lookup_kernel(const __grid_constant__ Params p) {
-  const int chunks = (p.D + VEC - 1) / VEC;
-  const int64_t total = p.n * chunks, step = (int64_t)gridDim.x * 256;
+  const int lane = threadIdx.x % p.team, teams = 256 / p.team;
   const T* table = static_cast<const T*>(p.table);
   T* out = static_cast<T*>(p.out);
-  for (int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x; i0 < total; i0 += step * kRowsAThread) {
-    float v[kRowsAThread][VEC];
-    int64_t to[kRowsAThread];
+  const int64_t step = (int64_t)gridDim.x * teams * kLookupRows;
+  for (int64_t r0 = ((int64_t)blockIdx.x * teams + threadIdx.x / p.team) * kLookupRows; r0 < p.n; r0 += step) {
+    const T* from[kLookupRows];
 #pragma unroll
-    for (int k = 0; k < kRowsAThread; ++k) {
-      const int64_t i = i0 + k * step;
-      to[k] = -1;
-      if (i < total) {
-        const int64_t r = i / chunks;
-        const int c = (int)(i - r * chunks) * VEC;
-        const int64_t id = min(max(id_at(p.ids, p.wide_ids, r), (int64_t)0), p.V - 1);
-        load_values<T, VEC>(table + id * p.ld_table + c, v[k]);
-        to[k] = r * p.ld_out + c;
-      }
-    }
+    for (int k = 0; k < kLookupRows; ++k)
+      from[k] = table + (r0 + k < p.n ? min(max(id_at(p.ids, p.wide_ids, r0 + k), (int64_t)0), p.V - 1) : 0) * p.ld_table;
+    for (int c0 = lane * VEC; c0 < p.D; c0 += p.team * VEC * kLookupWide) {
+      Raw<T, VEC> v[kLookupRows][kLookupWide];
 #pragma unroll
-    for (int k = 0; k < kRowsAThread; ++k) {
-      if (to[k] < 0) continue;
+      for (int k = 0; k < kLookupRows; ++k)
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) v[k][c] *= p.scale;
-      store_as<T, VEC>(out + to[k], v[k]);
+        for (int u = 0; u < kLookupWide; ++u)
+          if (r0 + k < p.n && c0 + u * p.team * VEC < p.D) v[k][u].load(from[k] + c0 + u * p.team * VEC);
+#pragma unroll
+      for (int k = 0; k < kLookupRows; ++k)
+#pragma unroll
+        for (int u = 0; u < kLookupWide; ++u) {
+          if (r0 + k >= p.n || c0 + u * p.team * VEC >= p.D) continue;
+          float f[VEC];
+          v[k][u].widen(f);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) f[i] *= p.scale;
+          store_as<T, VEC>(out + (r0 + k) * p.ld_out + c0 + u * p.team * VEC, f);
+        }
     }
   }
 }
 
 // ------------------------------------------------------------------- sort
-// A stable radix sort, 8 bits a pass.  A CTA ranks a tile of kTile keys: each warp counts its own 512 in their order
+// A stable radix sort, 8 bits a pass.  A CTA ranks a tile of kTile keys: each warp counts its own 128 in their order
 // (lanes with equal digits find each other by eight ballots), then warps and tiles are added up before it.
-constexpr int kSortThreads = 256, kPerThread = 16, kTile = kSortThreads * kPerThread;
+constexpr int kSortThreads = 512, kPerThread = 4, kTile = kSortThreads * kPerThread, kSortWarps = kSortThreads / 32;
 constexpr int kDigits = 256;
 constexpr int kDirect = 64;  // up to so many tiles a CTA adds up the counts of those before it by itself
 
-// the row of grad of id i, or -1: i itself, or its bag, searched in [lo, hi]
-__device__ __forceinline__ int bag_of(const Params& p, int64_t i, int64_t lo, int64_t hi) {
-  // the last b in [lo, hi] with bags[b] <= i
-  while (lo < hi) {
-    const int64_t m = (lo + hi + 1) >> 1;
-    if (id_at(p.bags, p.wide_ids, m) <= i) lo = m;
-    else hi = m - 1;
+// the last b in [0, n_bags] with bags[b] <= i, 0 where there is none: a warp, 32 probes at once
+__device__ __forceinline__ int64_t bag_of(const Params& p, int64_t i) {
+  int64_t lo = 0, hi = p.n_bags + 1;
+  const int lane = threadIdx.x & 31;
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 31) / 32, b = lo + (lane + 1) * step;
+    const int n = __popc(__ballot_sync(kAll, b < hi && id_at(p.bags, p.wide_ids, b) <= i));
+    lo += n * step;
+    hi = min(hi, lo + step);
   }
-  return (int)lo;
+  return lo;
 }
-// key (the table row, V for an id that gets nothing) and row of grad of id i
-__device__ __forceinline__ void source_of(const Params& p, int64_t i, int64_t lo, int64_t hi, int& key, int& row) {
-  const int64_t id = id_at(p.ids, p.wide_ids, i);
-  key = (int)min(max(id, (int64_t)0), p.V - 1);
-  row = (int)i;
-  if (p.bags != nullptr) {
-    row = bag_of(p, i, lo, hi);
-    if (row >= p.n_bags || i < id_at(p.bags, p.wide_ids, row) || i >= id_at(p.bags, p.wide_ids, row + 1)) key = (int)p.V;
-    row = min(row, (int)max(p.n_bags - 1, (int64_t)0));
-  }
-  if (p.padding >= 0 && key == p.padding) key = (int)p.V;
+// key of id i: the table row, or V for an id that gets nothing
+__device__ __forceinline__ int key_of(const Params& p, int64_t i) {
+  const int key = (int)min(max(id_at(p.ids, p.wide_ids, i), (int64_t)0), p.V - 1);
+  return p.padding >= 0 && key == p.padding ? (int)p.V : key;
 }
 
 __device__ __forceinline__ uint32_t peers_of(int digit, bool there) {
@@ -193,52 +199,102 @@ __device__ __forceinline__ int64_t item_at(int tile, int k) {
   return (int64_t)tile * kTile + (threadIdx.x >> 5) * (32 * kPerThread) + k * 32 + (threadIdx.x & 31);
 }
 
+// zeros over the gradient, by CTAs beside those that sort (few of which there are)
 __device__ __forceinline__ void zero_fill(const Params& p, int64_t block, int64_t blocks) {
   uint4* to = static_cast<uint4*>(p.out);
   const int64_t n = p.zero_bytes / 16;
-  for (int64_t i = block * kSortThreads + threadIdx.x; i < n; i += blocks * kSortThreads) to[i] = make_uint4(0u, 0u, 0u, 0u);
+  for (int64_t i = block * blockDim.x + threadIdx.x; i < n; i += blocks * blockDim.x) to[i] = make_uint4(0u, 0u, 0u, 0u);
   uint8_t* rest = static_cast<uint8_t*>(p.out);
   if (block == 0 && threadIdx.x < p.zero_bytes % 16) rest[n * 16 + threadIdx.x] = 0;
+}
+
+// The rows of grad of the ids [i0, i0 + count) that lie in bags: every bag that starts among them marks its first id (the
+// last of several, the others being empty), and a running maximum carries it on.  -1: in no bag.
+__device__ __forceinline__ void mark_bags(const Params& p, int64_t i0, int count, int* s_mark, int* s_warp) {
+  __shared__ int64_t s_edge[2];
+  if (threadIdx.x < 64) {
+    const int which = threadIdx.x >> 5;
+    const int64_t b = bag_of(p, which ? i0 + count - 1 : i0);
+    if ((threadIdx.x & 31) == 0) s_edge[which] = b;
+  }
+  for (int k = threadIdx.x; k < count; k += blockDim.x) s_mark[k] = -1;
+  __syncthreads();
+  for (int64_t b = s_edge[0] + threadIdx.x; b <= s_edge[1]; b += blockDim.x) {
+    const int64_t at = id_at(p.bags, p.wide_ids, b) - i0;
+    if (at < count) atomicMax(&s_mark[max(at, (int64_t)0)], (int)b);
+  }
+  __syncthreads();
+  // a thread's own run of marks, then the runs before it
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = (count + (int)blockDim.x - 1) / (int)blockDim.x;
+  const int k0 = min((int)threadIdx.x * per, count), k1 = min(k0 + per, count);
+  int high = -1;
+  for (int k = k0; k < k1; ++k) high = max(high, s_mark[k]);
+  int x = high;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(kAll, x, o);
+    if (lane >= o) x = max(x, y);
+  }
+  if (lane == 31) s_warp[warp] = x;
+  __syncthreads();
+  int before = __shfl_up_sync(kAll, x, 1);
+  if (lane == 0) before = -1;
+  for (int w = 0; w < warp; ++w) before = max(before, s_warp[w]);
+  for (int k = k0; k < k1; ++k) {
+    before = max(before, s_mark[k]);
+    s_mark[k] = before < p.n_bags ? before : -1;
+  }
+  __syncthreads();
 }
 
 // Counts of a pass's digits in each tile.  FIRST: keys come from the ids and are written in their order with their rows;
 // CTAs behind the tiles' fill the gradient with zeros, which few tiles leave most of the GPU free for.
 template <bool FIRST>
 __global__ void __launch_bounds__(kSortThreads) count_kernel(const __grid_constant__ Params p) {
+  __shared__ int s_count[kDigits], s_mark[FIRST ? kTile : 1], s_warp[kSortWarps];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (FIRST && (int)blockIdx.x >= p.tiles) {
     zero_fill(p, blockIdx.x - p.tiles, gridDim.x - p.tiles);
     return;
   }
-  __shared__ int s_count[kDigits];
-  __shared__ int64_t s_bag[2];
-  s_count[threadIdx.x] = 0;
   const int tile = blockIdx.x;
-  if (FIRST && p.bags != nullptr && threadIdx.x < 2) {
-    const int64_t i = threadIdx.x ? min(p.n - 1, (int64_t)(tile + 1) * kTile - 1) : (int64_t)tile * kTile;
-    s_bag[threadIdx.x] = bag_of(p, i, 0, p.n_bags);
-  }
-  __syncthreads();
-#pragma unroll 4
+  const int64_t i0 = (int64_t)tile * kTile;
+  const int count = (int)min((int64_t)kTile, p.n - i0);
+  if (threadIdx.x < kDigits) s_count[threadIdx.x] = 0;
+  if (FIRST && p.bags != nullptr) mark_bags(p, i0, count, s_mark, s_warp);
+  else __syncthreads();
+  int key[kPerThread];
+#pragma unroll
   for (int k = 0; k < kPerThread; ++k) {
     const int64_t i = item_at(tile, k);
-    if (i >= p.n) continue;
-    int key;
+    key[k] = i >= p.n ? -1 : FIRST ? key_of(p, i) : __ldg(p.key[0] + i);
+  }
+#pragma unroll
+  for (int k = 0; k < kPerThread; ++k) {
+    if (key[k] < 0) continue;
     if (FIRST) {
-      int row;
-      source_of(p, i, s_bag[0], s_bag[1], key, row);
-      p.key[0][i] = key;
+      const int64_t i = item_at(tile, k);
+      int row = (int)i;
+      if (p.bags != nullptr) {
+        row = s_mark[i - i0];
+        if (row < 0) {
+          row = 0;
+          key[k] = (int)p.V;
+        }
+      }
+      p.key[0][i] = key[k];
       p.row[0][i] = row;
-    } else {
-      key = __ldg(p.key[0] + i);
     }
-    atomicAdd(&s_count[(key >> p.shift) & (kDigits - 1)], 1);
+    atomicAdd(&s_count[(key[k] >> p.shift) & (kDigits - 1)], 1);
   }
   __syncthreads();
+  if (threadIdx.x >= kDigits) return;
   if (p.scanned) p.counts[(int64_t)threadIdx.x * p.tiles + tile] = s_count[threadIdx.x];
   else p.counts[tile * kDigits + threadIdx.x] = s_count[threadIdx.x];
 }
 
-// sums before each of a CTA's values (256 threads), and their total
+// sums before each of a CTA's values, and their total
 __device__ __forceinline__ int block_before(int v, int* s_warp, int& total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int x = v;
@@ -250,11 +306,9 @@ __device__ __forceinline__ int block_before(int v, int* s_warp, int& total) {
   __syncthreads();
   if (lane == 31) s_warp[warp] = x;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < (int)blockDim.x / 32; ++w) {
-    if (w < warp) before += s_warp[w];
-    all += s_warp[w];
-  }
+  int w = lane < (int)blockDim.x / 32 ? s_warp[lane] : 0;
+  const int all = __reduce_add_sync(kAll, w);
+  const int before = __reduce_add_sync(kAll, lane < warp ? w : 0);
   total = all;
   return before + x - v;
 }
@@ -262,6 +316,8 @@ __device__ __forceinline__ int block_before(int v, int* s_warp, int& total) {
 // one CTA a digit: its counts become the sums before them
 __global__ void __launch_bounds__(256) scan_kernel(const __grid_constant__ Params p) {
   __shared__ int s_warp[8];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   int32_t* mine = p.counts + (int64_t)blockIdx.x * p.tiles;
   int carry = 0;
   for (int t0 = 0; t0 < p.tiles; t0 += 256) {
@@ -274,10 +330,14 @@ __global__ void __launch_bounds__(256) scan_kernel(const __grid_constant__ Param
   if (threadIdx.x == 0) p.totals[blockIdx.x] = carry;
 }
 
-__global__ void __launch_bounds__(kSortThreads) scatter_kernel(const __grid_constant__ Params p) {
-  __shared__ int s_hist[kSortThreads / 32][kDigits];
-  __shared__ int s_warp[8];
+__global__ void __launch_bounds__(kSortThreads, 3) scatter_kernel(const __grid_constant__ Params p) {
+  __shared__ int s_hist[kSortWarps][kDigits];  // 16 KB
+  __shared__ int s_warp[kSortWarps], s_mine[kSortThreads / kDigits][kDigits], s_all[kSortThreads / kDigits][kDigits];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) s_hist[0][i] = 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tile = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int digit_of = threadIdx.x % kDigits, part = threadIdx.x / kDigits;
   int key[kPerThread], row[kPerThread], rank[kPerThread];
 #pragma unroll
   for (int k = 0; k < kPerThread; ++k) {
@@ -285,25 +345,36 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(const __grid_cons
     key[k] = i < p.n ? __ldg(p.key[0] + i) : -1;
     row[k] = i < p.n ? __ldg(p.row[0] + i) : 0;
   }
-  for (int w = 0; w < kSortThreads / 32; ++w) s_hist[w][threadIdx.x] = 0;
-  // where each digit's keys of this tile go
-  int total, mine = 0, all = 0;
+  // where each digit's keys of this tile go: two threads a digit add up the tiles
+  int mine = 0, all = 0, total;
   if (p.scanned) {
-    mine = p.counts[(int64_t)threadIdx.x * p.tiles + tile];
-    all = p.totals[threadIdx.x];
+    if (part == 0) {
+      mine = p.counts[(int64_t)digit_of * p.tiles + tile];
+      all = p.totals[digit_of];
+    }
   } else {
-#pragma unroll 8
-    for (int t = 0; t < p.tiles; ++t) {
-      const int c = p.counts[t * kDigits + threadIdx.x];
+#pragma unroll 16
+    for (int t = part; t < p.tiles; t += kSortThreads / kDigits) {
+      const int c = p.counts[t * kDigits + digit_of];
       if (t < tile) mine += c;
       all += c;
     }
   }
-  mine += block_before(all, s_warp, total);
+  s_mine[part][digit_of] = mine;
+  s_all[part][digit_of] = all;
   __syncthreads();
+  mine = all = 0;
+  if (threadIdx.x < kDigits) {
+#pragma unroll
+    for (int q = 0; q < kSortThreads / kDigits; ++q) {
+      mine += s_mine[q][threadIdx.x];
+      all += s_all[q][threadIdx.x];
+    }
+  }
+  mine += block_before(all, s_warp, total);
 #pragma unroll
   for (int k = 0; k < kPerThread; ++k) {
-    const bool there = item_at(tile, k) < p.n;
+    const bool there = key[k] >= 0;
     const int digit = (key[k] >> p.shift) & (kDigits - 1);
     const uint32_t same = peers_of(digit, there);
     const int before = there ? s_hist[warp][digit] : 0;
@@ -313,15 +384,26 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(const __grid_cons
     __syncwarp();
   }
   __syncthreads();
-  for (int w = 0; w < kSortThreads / 32; ++w) {
-    const int c = s_hist[w][threadIdx.x];
-    s_hist[w][threadIdx.x] = mine;
-    mine += c;
+  // the warps before: two threads a digit, eight warps each
+  constexpr int kEach = kSortWarps / (kSortThreads / kDigits);
+  int sum = 0;
+#pragma unroll
+  for (int w = 0; w < kEach; ++w) sum += s_hist[part * kEach + w][digit_of];
+  s_all[part][digit_of] = sum;
+  if (part == 0) s_mine[0][digit_of] = mine;
+  __syncthreads();
+  int base = s_mine[0][digit_of];
+  for (int q = 0; q < part; ++q) base += s_all[q][digit_of];
+#pragma unroll
+  for (int w = 0; w < kEach; ++w) {
+    const int c = s_hist[part * kEach + w][digit_of];
+    s_hist[part * kEach + w][digit_of] = base;
+    base += c;
   }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kPerThread; ++k) {
-    if (item_at(tile, k) >= p.n) continue;
+    if (key[k] < 0) continue;
     const int to = s_hist[warp][(key[k] >> p.shift) & (kDigits - 1)] + rank[k];
     p.key[1][to] = key[k];
     p.row[1][to] = row[k];
@@ -338,16 +420,25 @@ struct Small {
 __global__ void __launch_bounds__(kSmallThreads) small_sort_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) uint8_t raw[];
   Small& s = *reinterpret_cast<Small*>(raw);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x > 0) {
-    uint4* to = static_cast<uint4*>(p.out);
-    const int64_t n = p.zero_bytes / 16;
-    for (int64_t i = (int64_t)(blockIdx.x - 1) * kSmallThreads + threadIdx.x; i < n; i += (int64_t)(gridDim.x - 1) * kSmallThreads)
-      to[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (blockIdx.x == 1 && threadIdx.x < p.zero_bytes % 16) static_cast<uint8_t*>(p.out)[n * 16 + threadIdx.x] = 0;
+    zero_fill(p, blockIdx.x - 1, gridDim.x - 1);
     return;
   }
   const int n = (int)p.n, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < n; i += kSmallThreads) source_of(p, i, 0, p.n_bags, s.key[0][i], s.row[0][i]);
+  if (p.bags != nullptr) mark_bags(p, 0, n, s.row[0], s.warp);
+  for (int i = threadIdx.x; i < n; i += kSmallThreads) {
+    int key = key_of(p, i), row = i;
+    if (p.bags != nullptr) {
+      row = s.row[0][i];
+      if (row < 0) {
+        row = 0;
+        key = (int)p.V;
+      }
+    }
+    s.key[0][i] = key;
+    s.row[0][i] = row;
+  }
   int from = 0;
   for (int shift = 0; shift < p.bits; shift += 8, from ^= 1) {
     for (int d = lane; d < kDigits; d += 32) s.hist[warp][d] = 0;
@@ -396,6 +487,8 @@ __global__ void __launch_bounds__(kSmallThreads) small_sort_kernel(const __grid_
 // -------------------------------------------------------------------- sums
 // (sparse) how many rows start in each run of sorted ids, a warp a run
 __global__ void __launch_bounds__(256) heads_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int run = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (run >= p.runs) return;
   int n = 0;
@@ -412,6 +505,8 @@ __global__ void __launch_bounds__(256) heads_kernel(const __grid_constant__ Para
 // ... and how many before it, by one CTA
 __global__ void __launch_bounds__(1024) heads_scan_kernel(const __grid_constant__ Params p) {
   __shared__ int s_warp[32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   int carry = 0;
   for (int t0 = 0; t0 < p.runs; t0 += 4096) {
     int v[4], sum = 0, total;
@@ -434,112 +529,163 @@ __global__ void __launch_bounds__(1024) heads_scan_kernel(const __grid_constant_
 }
 
 constexpr int kSumThreads = 256, kAhead = 4;  // rows of grad that a thread has in flight
+constexpr int kMaxRun = 256;
 
+// A team of p.team threads takes a run of sorted ids: ids and rows go to shared memory at once, so that the loop waits for
+// rows of grad alone, and those are asked for kAhead ahead.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kSumThreads) sums_kernel(const __grid_constant__ Params p) {
-  const int team = threadIdx.x / p.team, run = blockIdx.x * (kSumThreads / p.team) + team;
-  const int c = (blockIdx.y * p.team + threadIdx.x % p.team) * VEC;
-  if (run >= p.runs || c >= p.D) return;
+  extern __shared__ int2 s_runs[];  // [teams][run]: key, row
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int team = threadIdx.x / p.team, lane = threadIdx.x % p.team, run = blockIdx.x * (kSumThreads / p.team) + team;
+  const int c = (blockIdx.y * p.team + lane) * VEC;
   const int64_t i0 = (int64_t)run * p.run, i1 = min(p.n, i0 + p.run);
-  const T* grad = static_cast<const T*>(p.grad) + c;
+  const int count = run < p.runs ? (int)(i1 - i0) : 0;
   const int32_t* keys = p.key[0];
-  int cur = __ldg(keys + i0);
-  bool before = i0 > 0 && __ldg(keys + i0 - 1) == cur;
-  int64_t rank = p.sparse ? (int64_t)p.heads[run] - (before ? 1 : 0) : 0;  // of the current row among the touched
+  int2* mine = s_runs + team * p.run;
+  for (int k = lane; k < count; k += p.team) mine[k] = make_int2(__ldg(keys + i0 + k), __ldg(p.row[0] + i0 + k));
+  int prev = -1, next = -1, rank = 0;
+  if (count > 0) {
+    if (i0 > 0) prev = __ldg(keys + i0 - 1);
+    if (i1 < p.n) next = __ldg(keys + i1);
+    if (p.sparse) rank = p.heads[run];
+  }
+  __syncthreads();
+  if (count == 0 || c >= p.D) return;
+  const T* grad = static_cast<const T*>(p.grad) + c;
+  int cur = mine[0].x;
+  bool before = prev == cur;
+  if (before) --rank;  // of the current row among the touched
   float acc[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
   auto part = [&](int which) {
     float* to = p.part + ((int64_t)run * 2 + which) * p.D + c;
+    if constexpr (VEC == 1) {
+      to[0] = acc[0];
+    } else {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) to[v] = acc[v];
+      for (int v = 0; v < VEC; v += 4) *reinterpret_cast<float4*>(to + v) = make_float4(acc[v], acc[v + 1], acc[v + 2], acc[v + 3]);
+    }
   };
   auto finish = [&] {
-    if (cur >= p.V) return;
     if (before) return part(0);
     if (p.sparse && c == 0) p.out_ids[rank] = cur;
-    store_sums<VEC>(p, p.sparse ? rank : (int64_t)cur, c, acc);
+    store_sums<VEC>(p, p.sparse ? (int64_t)rank : (int64_t)cur, c, acc);
   };
-  for (int64_t i = i0; i < i1; i += kAhead) {
-    float g[kAhead][VEC];
-    int key[kAhead];
+  Raw<T, VEC> g[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (k < count) g[k].load(grad + (int64_t)mine[k].y * p.ld_grad);
+  for (int i = 0; i < count; i += kAhead) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      key[k] = i + k < i1 ? __ldg(keys + i + k) : -1;
-      if (key[k] >= 0 && key[k] < p.V) load_values<T, VEC>(grad + (int64_t)__ldg(p.row[0] + i + k) * p.ld_grad, g[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (key[k] < 0 || key[k] >= p.V) {
-        if (key[k] >= 0 && key[k] != cur) {
-          finish();
-          cur = key[k];
-        }
-        continue;
-      }
-      if (key[k] != cur) {
+      if (i + k >= count) break;
+      const int key = mine[i + k].x;
+      if (key != cur) {
         finish();
-        cur = key[k];
+        cur = key;
+        if (cur >= p.V) return;  // (the ids that get nothing are the last)
         before = false;
         ++rank;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
       }
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) acc[v] += g[k][v];
+      if (cur >= p.V) return;
+      g[k].add_to(acc);
+      if (i + k + kAhead < count) g[k].load(grad + (int64_t)mine[i + k + kAhead].y * p.ld_grad);
     }
   }
-  if (cur >= p.V) return;
-  const bool on = i1 < p.n && __ldg(keys + i1) == cur;
-  if (!on) return finish();
+  if (next != cur) return finish();
   part(before ? 0 : 1);
 }
 
-// A CTA for each run whose last row starts in it and goes on: the partial sums of that row, in teams that take every so
-// manyth of them, then the teams in their order.
+// A warp for each run whose last row starts in it and goes on: the partial sums of that row, in their order.  Rows over
+// more than kNear runs are left to the CTA: teams take every so manyth partial sum, then the teams are added up.
+constexpr int kFar = 32, kNear = 12;
 template <int VEC>
 __global__ void __launch_bounds__(kSumThreads) combine_kernel(const __grid_constant__ Params p) {
   __shared__ float s_sum[kSumThreads * VEC];
-  const int run = blockIdx.x;
-  const int64_t i0 = (int64_t)run * p.run, i1 = i0 + p.run;
-  if (i1 >= p.n) return;
+  __shared__ int s_last[kSumThreads / 32];  // of a row that is left to the CTA, else -1
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, run0 = blockIdx.x * (kSumThreads / 32);
   const int32_t* keys = p.key[0];
-  const int key = __ldg(keys + i1 - 1);
-  if (key >= p.V || __ldg(keys + i1) != key) return;
-  if (__ldg(keys + i0) == key && i0 > 0 && __ldg(keys + i0 - 1) == key) return;  // (it came from before)
-  int64_t lo = i1, hi = p.n;  // the first id behind the row
-  while (lo < hi) {
-    const int64_t m = (lo + hi) >> 1;
-    if (__ldg(keys + m) <= key) lo = m + 1;
-    else hi = m;
-  }
-  const int last = (int)((lo - 1) >> p.run_log);
-  const int teams = kSumThreads / p.team, team = threadIdx.x / p.team;
-  const int c = (blockIdx.y * p.team + threadIdx.x % p.team) * VEC;
-  float acc[VEC];
+  // the key of the row that starts in run r and goes on, or -1
+  auto starts = [&](int r) {
+    const int64_t i0 = (int64_t)r * p.run, i1 = i0 + p.run;
+    if (i1 >= p.n) return -1;
+    const int key = __ldg(keys + i1 - 1), next = __ldg(keys + i1), first = __ldg(keys + i0), prev = i0 > 0 ? __ldg(keys + i0 - 1) : -1;
+    return key < p.V && next == key && !(first == key && prev == key) ? key : -1;  // (else it came from before)
+  };
+  auto add = [&](int j, int from_run, int c, float* acc) {
+    const float* from = p.part + ((int64_t)j * 2 + (j == from_run ? 1 : 0)) * p.D + c;
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
-  if (c < p.D) {
-#pragma unroll 4
-    for (int j = run + team; j <= last; j += teams) {
-      const float* from = p.part + ((int64_t)j * 2 + (j == run ? 1 : 0)) * p.D + c;
+    for (int v = 0; v < VEC; ++v) acc[v] += from[v];
+  };
+  auto store = [&](int r, int key, int c, float* acc) {
+    int64_t at = key;
+    if (p.sparse) {
+      at = (int64_t)p.heads[r + 1] - 1;
+      if (c == 0) p.out_ids[at] = key;
+    }
+    store_sums<VEC>(p, at, c, acc);
+  };
+  const int run = run0 + warp, key = starts(run);
+  int last = -1;
+  if (key >= 0) {  // the runs behind: how many of them end with the row still going on
+    const int64_t end = ((int64_t)run + 2 + lane) * p.run - 1;  // of run + 1 + lane
+    const bool on = end + 1 < p.n && __ldg(keys + end) == key && __ldg(keys + end + 1) == key;
+    const uint32_t off = __ballot_sync(kAll, !on);
+    last = run + __ffs(off);
+    if (off == 0) {  // the last id of the row, 32 probes at once
+      int64_t lo = ((int64_t)run + kFar) * p.run, hi = p.n;
+      while (hi - lo > 1) {
+        const int64_t step = (hi - lo + 31) / 32, m = lo + (lane + 1) * step;
+        const int n = __popc(__ballot_sync(kAll, m < hi && __ldg(keys + m) == key));
+        lo += n * step;
+        hi = min(hi, lo + step);
+      }
+      last = (int)(lo >> p.run_log);
+    } else if (last <= run + kNear) {
+      for (int c = lane * VEC; c < p.D; c += 32 * VEC) {
+        float acc[VEC];
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) acc[v] += from[v];
+        for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+#pragma unroll 6
+        for (int j = run; j <= last; ++j) add(j, run, c, acc);
+        store(run, key, c, acc);
+      }
+      last = -1;
     }
   }
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) s_sum[threadIdx.x * VEC + v] = acc[v];
+  if (lane == 0) s_last[warp] = last;
   __syncthreads();
-  if (team > 0 || c >= p.D) return;
-  for (int t = 1; t < teams; ++t)
+  const int teams = kSumThreads / p.team, team = threadIdx.x / p.team, slab = p.team * VEC;
+  for (int w = 0; w < kSumThreads / 32; ++w) {
+    if (s_last[w] < 0) continue;
+    const int from = run0 + w, k = starts(from);
+    for (int c0 = 0; c0 < p.D; c0 += slab) {
+      const int c = c0 + threadIdx.x % p.team * VEC;
+      float acc[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) acc[v] += s_sum[(t * p.team + threadIdx.x) * VEC + v];
-  int64_t at = key;
-  if (p.sparse) {
-    at = (int64_t)p.heads[run + 1] - 1;
-    if (c == 0) p.out_ids[at] = key;
+      for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+      if (c < p.D) {
+#pragma unroll 8
+        for (int j = from + team; j <= s_last[w]; j += teams) add(j, from, c, acc);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) s_sum[threadIdx.x * VEC + v] = acc[v];
+      __syncthreads();
+      if (team == 0 && c < p.D) {
+        for (int t = 1; t < teams; ++t)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) acc[v] += s_sum[(t * p.team + threadIdx.x) * VEC + v];
+        store(from, k, c, acc);
+      }
+    }
   }
-  store_sums<VEC>(p, at, c, acc);
 }
 
 // ------------------------------------------------------------------- host
@@ -552,7 +698,7 @@ static int bits_of(int64_t values) {
 // every run costs up to two partial sums.
 static int run_log_of(int64_t n) {
   int log = 4;
-  while (log < 8 && (n >> log) > (int64_t)sm_count() * 32) ++log;
+  while (log < 8 && (n >> log) > (int64_t)sm_count() * 64) ++log;
   return log;
 }
 struct Sizes {
@@ -577,11 +723,30 @@ static int vec_of(const void* a, int64_t lda, const void* b, int64_t ldb, int b_
 }
 
 template <typename T, int VEC>
-static int run_lookup(const Params& p, cudaStream_t st) {
-  const int64_t total = p.n * ((p.D + VEC - 1) / VEC);
-  const int64_t blocks = std::min<int64_t>((total + 255) / 256, (int64_t)sm_count() * 32);
+static int run_lookup(Params p, cudaStream_t st) {
+  const int chunks = (p.D + VEC - 1) / VEC;
+  p.team = 1;
+  while (p.team < chunks && p.team < 32) p.team *= 2;
+  const int64_t rows = (int64_t)(256 / p.team) * kLookupRows;  // of a CTA at a time
+  const int64_t blocks = std::min<int64_t>((p.n + rows - 1) / rows, (int64_t)sm_count() * 64);
   lookup_kernel<T, VEC><<<(unsigned)blocks, 256, 0, st>>>(p);
   return check_cuda(cudaGetLastError(), "embedding lookup_kernel launch");
+}
+
+// a launch that may start under the one before it (whose results it waits for by itself)
+static int chain(const void* kernel, dim3 grid, int threads, int smem, cudaStream_t st, Params& p, const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  void* args[] = {&p};
+  return check_cuda(cudaLaunchKernelExC(&cfg, kernel, args), what);
 }
 
 static int sort_ids(Params& p, cudaStream_t st) {
@@ -602,15 +767,15 @@ static int sort_ids(Params& p, cudaStream_t st) {
   p.tiles = (int)((p.n + kTile - 1) / kTile);
   p.scanned = p.tiles > kDirect;
   for (p.shift = 0; p.shift < p.bits; p.shift += 8) {
-    if (p.shift == 0) count_kernel<true><<<p.tiles + fill, kSortThreads, 0, st>>>(p);
-    else count_kernel<false><<<p.tiles, kSortThreads, 0, st>>>(p);
-    if ((rc = check_cuda(cudaGetLastError(), "embedding count_kernel launch"))) return rc;
-    if (p.scanned) {
-      scan_kernel<<<kDigits, 256, 0, st>>>(p);
-      if ((rc = check_cuda(cudaGetLastError(), "embedding scan_kernel launch"))) return rc;
+    if (p.shift == 0) {
+      count_kernel<true><<<p.tiles + fill, kSortThreads, 0, st>>>(p);
+      rc = check_cuda(cudaGetLastError(), "embedding count_kernel launch");
+    } else {
+      rc = chain((const void*)count_kernel<false>, dim3(p.tiles), kSortThreads, 0, st, p, "embedding count_kernel launch");
     }
-    scatter_kernel<<<p.tiles, kSortThreads, 0, st>>>(p);
-    if ((rc = check_cuda(cudaGetLastError(), "embedding scatter_kernel launch"))) return rc;
+    if (rc) return rc;
+    if (p.scanned && (rc = chain((const void*)scan_kernel, dim3(kDigits), 256, 0, st, p, "embedding scan_kernel launch"))) return rc;
+    if ((rc = chain((const void*)scatter_kernel, dim3(p.tiles), kSortThreads, 0, st, p, "embedding scatter_kernel launch"))) return rc;
     std::swap(p.key[0], p.key[1]);
     std::swap(p.row[0], p.row[1]);
   }
@@ -626,18 +791,14 @@ static int run_sums(Params& p, cudaStream_t st) {
   const unsigned slabs = (unsigned)((chunks + p.team - 1) / p.team);
   const int teams = kSumThreads / p.team;
   if (p.sparse) {
-    heads_kernel<<<(p.runs + 7) / 8, 256, 0, st>>>(p);
-    if ((rc = check_cuda(cudaGetLastError(), "embedding heads_kernel launch"))) return rc;
-    heads_scan_kernel<<<1, 1024, 0, st>>>(p);
-    if ((rc = check_cuda(cudaGetLastError(), "embedding heads_scan_kernel launch"))) return rc;
+    if ((rc = chain((const void*)heads_kernel, dim3((p.runs + 7) / 8), 256, 0, st, p, "embedding heads_kernel launch"))) return rc;
+    if ((rc = chain((const void*)heads_scan_kernel, dim3(1), 1024, 0, st, p, "embedding heads_scan_kernel launch"))) return rc;
   }
-  sums_kernel<T, VEC><<<dim3((p.runs + teams - 1) / teams, slabs), kSumThreads, 0, st>>>(p);
-  if ((rc = check_cuda(cudaGetLastError(), "embedding sums_kernel launch"))) return rc;
-  if (p.runs > 1) {
-    combine_kernel<VEC><<<dim3(p.runs - 1, slabs), kSumThreads, 0, st>>>(p);
-    rc = check_cuda(cudaGetLastError(), "embedding combine_kernel launch");
-  }
-  return rc;
+  if ((rc = chain((const void*)sums_kernel<T, VEC>, dim3((p.runs + teams - 1) / teams, slabs), kSumThreads, teams * p.run * 8, st, p,
+                  "embedding sums_kernel launch")))
+    return rc;
+  if (p.runs == 1) return RB_OK;
+  return chain((const void*)combine_kernel<VEC>, dim3((p.runs + 7) / 8), kSumThreads, 0, st, p, "embedding combine_kernel launch");
 }
 
 template <typename T>

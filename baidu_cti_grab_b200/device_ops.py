@@ -9,7 +9,9 @@ rep_encoder_fusion, rep_encoder) are built on them.
 from __future__ import annotations
 
 import ctypes
+import operator
 import weakref
+from array import array
 from typing import Dict, Optional, Sequence, Tuple
 
 import torch
@@ -1047,7 +1049,9 @@ def _dense(t: torch.Tensor) -> bool:
 
 def _gradients(name: str, grads):
     """(tensors, row counts or None) of a list of gradients, pairs (rows, count) among them."""
-    tensors, counts = [], None
+    if set(map(type, grads)) <= _PLAIN:
+        return grads, None
+    tensors, counts = [], {}
     for i, g in enumerate(grads):
         if isinstance(g, torch.Tensor):
             tensors.append(g)
@@ -1055,14 +1059,16 @@ def _gradients(name: str, grads):
         rows, count = g
         if rows.dim() != 2 or not rows.is_contiguous() or count.numel() != 1 or count.dtype is not torch.int32:
             raise ValueError(f"{name}: counted rows are a contiguous [n, D] and an int32 [1]")
-        if counts is None:
-            counts = {}
         counts[i] = count
         tensors.append(rows)
     return tensors, counts
 
 
+_dtype_of, _T, _PLAIN = operator.attrgetter("dtype"), torch.Tensor, {torch.Tensor, torch.nn.Parameter}
+
+
 def _clip(name: str, grads, most: float, out, scale: float) -> torch.Tensor:
+    # (a call has hundreds of tensors: what is asked of each is asked by map, without Python code per tensor)
     tensors, counts = _gradients(name, grads)
     n = len(tensors)
     if n == 0:
@@ -1071,45 +1077,44 @@ def _clip(name: str, grads, most: float, out, scale: float) -> torch.Tensor:
     if dev.type != "cuda":
         raise RuntimeError(f"{name} expects CUDA tensors")
     index = dev.index
-    if {t.get_device() for t in tensors} != {index} or (counts and any(c.device != dev for c in counts.values())):
+    if set(map(_T.get_device, tensors)) != {index} or (counts and any(c.device != dev for c in counts.values())):
         raise RuntimeError(f"{name}: tensors on different devices")
-    try:
-        types = [_GRAD_TYPES[t.dtype] for t in tensors]
-    except KeyError:
-        raise ValueError("gradients must be fp32, bf16 or f16") from None
+    dtypes = list(map(_dtype_of, tensors))
+    if not set(dtypes) <= _GRAD_TYPES.keys():
+        raise ValueError("gradients must be fp32, bf16 or f16")
     clip = most >= 0.0
     back = []  # (a copy, where it goes): gradients whose values lie apart
-    for i, t in enumerate(tensors):
-        if not t.is_contiguous() and not _dense(t):
-            tensors[i] = t.contiguous()
-            if clip and out is None:
-                back.append((tensors[i], t))
-    sizes = [t.numel() for t in tensors]
-    ptrs = [t.data_ptr() for t in tensors]
-    to = ptrs
+    whole = all(map(_T.is_contiguous, tensors))
+    if not whole:
+        for i, t in enumerate(tensors):
+            if not _dense(t):
+                tensors[i] = t.contiguous()
+                if clip and out is None:
+                    back.append((tensors[i], t))
+    sizes = array("q", map(_T.numel, tensors))
+    ptrs = to = array("q", map(_T.data_ptr, tensors))
     if not clip:
         to = None
     elif out is not None:
-        if len(out) != n:
-            raise ValueError(f"out must have {n} tensors")
-        for o, t in zip(out, tensors):
-            if o.shape != t.shape or o.dtype is not t.dtype or o.get_device() != index or \
-                    not (o.is_contiguous() and t.is_contiguous() or (o.stride() == t.stride() and _dense(o))):
-                raise ValueError("out's tensors must be as the gradients, their values in one run of memory")
-        to = [o.data_ptr() for o in out]
+        if len(out) != n or set(map(_T.get_device, out)) != {index} or list(map(_dtype_of, out)) != dtypes or \
+                array("q", map(_T.numel, out)) != sizes or \
+                not (whole and all(map(_T.is_contiguous, out)) or
+                     all(o.stride() == t.stride() and _dense(o) for o, t in zip(out, tensors))):
+            raise ValueError("out's tensors must be as the gradients, their values in one run of memory")
+        to = array("q", map(_T.data_ptr, out))
     if clip and len(set(to)) < n and len({a for a, m in zip(to, sizes) if m}) < sum(1 for m in sizes if m):
         raise ValueError(f"{name}: a tensor to be clipped was given twice")
-    pointers, longs = ctypes.c_void_p * n, ctypes.c_int64 * n
+    types = array("i", map(_GRAD_TYPES.__getitem__, dtypes))
     counted = widths = None
     if counts:
-        counted, widths = pointers(), longs()
+        counted, widths = array("q", bytes(8 * n)), array("q", bytes(8 * n))
         for i, c in counts.items():
             counted[i], widths[i] = c.data_ptr(), max(tensors[i].shape[1], 1)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     ws_bytes = _plan_bytes(dev, "rb_grad_norm_workspace_size", n)
     ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
-    _call_on(dev, "rb_clip_grads", pointers(*ptrs), None if to is None else pointers(*to), longs(*sizes), (ctypes.c_int * n)(*types),
-             counted, widths, n, float(scale), float(most), ws.data_ptr(), ws_bytes, norm.data_ptr())
+    lists = [None if a is None else a.buffer_info()[0] for a in (ptrs, to, sizes, types, counted, widths)]
+    _call_on(dev, "rb_clip_grads", *lists, n, float(scale), float(most), ws.data_ptr(), ws_bytes, norm.data_ptr())
     for copy, t in back:
         t.copy_(copy)
     return norm
