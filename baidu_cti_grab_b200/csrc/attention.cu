@@ -398,34 +398,64 @@ __device__ __noinline__ bool given_up(uint32_t tries, int code, volatile int* ab
 }
 __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, int code, volatile int* abort_flag) {
   const uint32_t at = smem_u32(bar);
-  uint32_t tries = 0;
-  while (!mbar_try_wait(at, parity & 1u))
+  uint32_t tries = 0, done;
+  while (true) {  // a try may sleep for up to a millisecond
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(at), "r"(parity & 1u), "r"(1000000u)
+        : "memory");
+    if (done) return true;
     if ((++tries & 0xfffu) == 0 && given_up(tries, code, abort_flag)) return false;
-  return true;
+  }
+}
+// one arrival for a warp, whose lanes have all come here
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(bar));
 }
 
-// K-major operand: 64 columns (128 bytes) a row, groups of eight rows 1024 bytes apart
-__device__ __forceinline__ uint64_t rows_desc(uint32_t saddr) { return tc::sw128_desc(saddr); }
-// the same bytes as an operand whose 64-column rows run along K: `next` bytes on lie the next 64 columns
-__device__ __forceinline__ uint64_t columns_desc(uint32_t saddr, uint32_t next) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Operands under the 128-byte swizzle: 64 columns (128 bytes) a row, groups of eight rows 1024 bytes apart.  Their
+// descriptors differ in the low word alone: the address, and how far on the next 64 columns lie where rows run along K.
+// One thread issues all products, and what it computes between two of them holds the tensor cores up: so low words,
+// loops unrolled, no division.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t rows_desc(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t columns_desc(uint32_t saddr, uint32_t next) { return (saddr >> 4) | ((next >> 4) << 16); }
+// (without the operand that switches lanes of D off: with it one thread issued a product in 95 cycles, without in 50)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "r"(kDescHigh));
 }
 // A from TMEM: sixteen 16-bit values of a row are eight words of its lane
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "r"(kDescHigh));
 }
+// where in operands of `rows` rows the i-th sixteen columns lie, in 16-byte units
+__host__ __device__ constexpr uint32_t sixteenth(int i, int rows) { return (uint32_t)((i >> 2) * rows * 8 + (i & 3) * 2); }
+// a position in a ring of S slots, and the parity of its use
+template <int S>
+struct Turn {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == S) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+};
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
@@ -456,6 +486,18 @@ __device__ __forceinline__ void tmem_put32(uint32_t taddr, const uint32_t* r) {
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+__device__ __forceinline__ void tmem_get16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_put8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -523,8 +565,8 @@ enum Seen : int { kNone = 0, kSome = 1, kEvery = 2 };
 constexpr int kHalf = 32;
 struct Span {  // of a warp's rows' intervals
   int lo_min, lo_max, hi_min, hi_max;
-  __device__ Seen of(int j) const {
-    return j + kHalf <= lo_min || j >= hi_max ? kNone : j >= lo_max && j + kHalf <= hi_min ? kEvery : kSome;
+  __device__ Seen of(int j, int width = kHalf) const {  // of keys [j, j + width)
+    return j + width <= lo_min || j >= hi_max ? kNone : j >= lo_max && j + width <= hi_min ? kEvery : kSome;
   }
 };
 __device__ __forceinline__ Span span_of(int4 row) {
@@ -627,11 +669,11 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
     }
     for (int s = 0; s < kItems; ++s) mbar_init(smem_u32(&ifull[s]), 1);
     mbar_init(smem_u32(&sfull), 1);
-    mbar_init(smem_u32(&sfree), C::kRowThreads);
-    mbar_init(smem_u32(&pready), C::kRowThreads);
+    mbar_init(smem_u32(&sfree), C::kRowThreads / 32);
+    mbar_init(smem_u32(&pready), C::kRowThreads / 32);
     mbar_init(smem_u32(&pvdone), 1);
     mbar_init(smem_u32(&drained), 1);
-    for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&pairs[q]), 64);
+    for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&pairs[q]), 2);
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -655,14 +697,14 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
       // -------------------------------------------------- copies and MMAs
       constexpr uint32_t idesc_s = idesc_of<T>(kBlock, false), idesc_o = idesc_of<T>(DP, true);
       auto wait = [&](uint64_t* bar, int n) { return wait_on(bar, (uint32_t)n, kWaitTimeoutMma, abort_flag); };
-      auto slot = [](int t) { return t % C::kStages; };
-      auto phase = [](int t) { return t / C::kStages; };
       const uint32_t items = (uint32_t)p.n_tiles * p.H;
+      const uint32_t q_at = smem_u32(sQ), k_at = smem_u32(sK), v_at = smem_u32(sV);
       // `ahead`: the tile whose keys are asked for, the `posted`th, from block a_block on; the values follow, block v_block
       // of tile v_tile.  Posting overwrites what was posted four tiles ago: its blocks lie three tiles back at least and
       // the rows are past them.
       Item ahead{};
-      int posted = 0, a_block = 0, k_asked = 0, v_tile = 0, v_block = 0, v_asked = 0;
+      int posted = 0, a_block = 0, k_asked = 0, v_tile = 0, v_block = 0, v_asked = 0, queried = 0;
+      Turn<C::kStages> k_ask, v_ask, k_use, v_use;
       uint32_t ticket = atomicAdd(p.next, 1u);
       auto take = [&] {
         ahead.blocks = 0;
@@ -676,43 +718,48 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
         mbar_arrive(smem_u32(&ifull[posted % kItems]));
         ++posted;
       };
-      auto copy = [&](uint64_t* full, uint8_t* to, const CUtensorMap* tm, int i, int head, int key) {
-        const uint32_t bar = smem_u32(&full[slot(i)]);
+      auto copy = [&](uint64_t* full, uint32_t to, const CUtensorMap* tm, int slot, int head, int key) {
+        const uint32_t bar = smem_u32(&full[slot]);
         mbar_arrive_expect_tx(bar, C::kKvBytes);
-        for (int c = 0; c < C::kChunks; ++c)
-          tma_load_3d(smem_u32(to + slot(i) * C::kKvBytes + c * kBlock * 128), tm, 64 * c, head / p.G, key, bar);
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c) tma_load_3d(to + slot * C::kKvBytes + c * kBlock * 128, tm, 64 * c, head / p.G, key, bar);
       };
       auto ask_k = [&] {  // for the next block's keys, whose slot is free
         if (ahead.blocks == 0) return;
-        copy(kfull, sK, &tmK, k_asked++, ahead.head, ahead.key0 + a_block * kBlock);
+        copy(kfull, k_at, &tmK, k_ask.slot, ahead.head, ahead.key0 + a_block * kBlock);
+        k_ask.next();
+        ++k_asked;
         if (++a_block == ahead.blocks) take();
       };
       auto ask_v = [&] {  // for its values
         if (v_asked == k_asked) return;
         const Item& it = s_item[v_tile % kItems];
-        copy(vfull, sV, &tmV, v_asked++, it.head, it.key0 + v_block * kBlock);
+        copy(vfull, v_at, &tmV, v_ask.slot, it.head, it.key0 + v_block * kBlock);
+        v_ask.next();
+        ++v_asked;
         if (++v_block == it.blocks) {
           v_block = 0;
           ++v_tile;
         }
       };
-      int queried = 0;
       auto ask_queries = [&](const Item& it) {
         const uint32_t bar = smem_u32(&qfull);
         mbar_arrive_expect_tx(bar, C::kQBytes);
-        for (int c = 0; c < C::kChunks; ++c) tma_load_3d(smem_u32(sQ + c * kTile * 128), &tmQ, 64 * c, it.head, it.r0, bar);
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c) tma_load_3d(q_at + c * kTile * 128, &tmQ, 64 * c, it.head, it.r0, bar);
         ++queried;
       };
       const int steps = (p.D + 15) / 16;  // of 16 columns (the rest of a row is zeros)
-      auto scores = [&](int t, bool first) {
+      auto scores = [&](bool first) {  // of the next block
         if (first && !wait(&qfull, queried - 1)) return false;
-        if (!wait(&kfull[slot(t)], phase(t))) return false;
+        if (!wait(&kfull[k_use.slot], k_use.parity)) return false;
         tc::tc_fence_after();
-        const uint64_t qd = rows_desc(smem_u32(sQ)), kd = rows_desc(smem_u32(sK + slot(t) * C::kKvBytes));
-        for (int i = 0; i < steps; ++i)
-          mma_ss(tmem, qd + (uint64_t)((i >> 2) * (kTile * 128 / 16) + (i & 3) * 2),
-                 kd + (uint64_t)((i >> 2) * (kBlock * 128 / 16) + (i & 3) * 2), idesc_s, i > 0);
+        const uint32_t qd = rows_desc(q_at), kd = rows_desc(k_at + k_use.slot * C::kKvBytes);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i)
+          if (i < steps) mma_ss(tmem, qd + sixteenth(i, kTile), kd + sixteenth(i, kBlock), idesc_s, i > 0);
         tc::umma_commit(smem_u32(&sfull));
+        k_use.next();
         return true;
       };
       take();
@@ -724,7 +771,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
           ask_k();
           ask_v();
         }
-        ok = scores(0, true);
+        ok = scores(true);
       }
       int t = 0;  // block of all tiles
       for (int tile = 0; now.blocks > 0 && ok; ++tile) {
@@ -736,30 +783,29 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
             ok = wait(&sfree, t);
             if (ok) {
               tc::tc_fence_after();
+              if (!last) ok = scores(false);
               ask_k();
-              if (!last) ok = scores(t + 1, false);
             }
           }
-          ok = ok && wait(&pready, t);
+          ok = ok && wait(&vfull[v_use.slot], v_use.parity) && wait(&pready, t);
           if (!ok) break;
+          tc::tc_fence_after();
+          const uint32_t vd = columns_desc(v_at + v_use.slot * C::kKvBytes, kBlock * 128);
+#pragma unroll
+          for (int i = 0; i < kBlock / 16; ++i) mma_ts(tmem + C::kOAt, tmem + C::kPAt + 8 * i, vd + i * (16 * 128 / 16), idesc_o, n > 0 || i > 0);
+          tc::umma_commit(smem_u32(&pvdone));
+          v_use.next();
           if (last) {
             next = s_item[(tile + 1) % kItems];
             if (next.blocks > 0) ask_queries(next);
           }
-          ok = wait(&vfull[slot(t)], phase(t));
-          if (!ok) break;
-          tc::tc_fence_after();
-          const uint64_t vd = columns_desc(smem_u32(sV + slot(t) * C::kKvBytes), kBlock * 128);
-          for (int i = 0; i < kBlock / 16; ++i)
-            mma_ts(tmem + C::kOAt, tmem + C::kPAt + 8 * i, vd + (uint64_t)(i * 16 * 128 / 16), idesc_o, n > 0 || i > 0);
-          tc::umma_commit(smem_u32(&pvdone));
           const bool more = !last || next.blocks > 0;
           if (C::kApart) {
             if (t > 0) ask_v();  // (into the slot of the block before: its product had ended before these weights were written)
-            if (last && more) ok = scores(t + 1, true);
+            if (last && more) ok = scores(true);
           } else if (more) {
             ok = wait(&pvdone, t);
-            if (ok) ok = scores(t + 1, last);
+            if (ok) ok = scores(last);
             ask_k();
             ask_v();
           }
@@ -772,8 +818,8 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
       }
       // nor a copy
       if (queried > 0) wait_on(&qfull, (uint32_t)(queried - 1), kWaitTimeoutProducer, nullptr);
-      for (int i = max(0, k_asked - C::kStages); i < k_asked; ++i) wait_on(&kfull[slot(i)], (uint32_t)phase(i), kWaitTimeoutProducer, nullptr);
-      for (int i = max(0, v_asked - C::kStages); i < v_asked; ++i) wait_on(&vfull[slot(i)], (uint32_t)phase(i), kWaitTimeoutProducer, nullptr);
+      for (int i = max(0, k_asked - C::kStages); i < k_asked; ++i) wait_on(&kfull[i % C::kStages], (uint32_t)(i / C::kStages), kWaitTimeoutProducer, nullptr);
+      for (int i = max(0, v_asked - C::kStages); i < v_asked; ++i) wait_on(&vfull[i % C::kStages], (uint32_t)(i / C::kStages), kWaitTimeoutProducer, nullptr);
     }
   } else {
     // -------------------------------------------------------------- rows
@@ -784,7 +830,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
     };
     int met = 0;
     auto meet = [&] {  // the two warps of a quarter
-      mbar_arrive(smem_u32(&pairs[quarter]));
+      warp_arrive(&pairs[quarter]);
       return wait(&pairs[quarter], met++);
     };
     bool ok = wait(&ifull[0], 0);
@@ -823,7 +869,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
           tmem_get32(mine + set * kHalf, held);
           tmem_wait_ld();
           tc::tc_fence_before();
-          mbar_arrive(smem_u32(&sfree));
+          warp_arrive(&sfree);
           const Seen seen = reach.of(j0 + set * kHalf);
           if (seen != kNone) prepare(held, j0 + set * kHalf, seen);
           s_max[t & 1][set][quarter * 32 + lane] = high;
@@ -898,7 +944,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
         total += s2.x + s2.y;
         tmem_wait_st();
         tc::tc_fence_before();
-        mbar_arrive(smem_u32(&pready));
+        warp_arrive(&pready);
       }
       // the next tile's intervals come while the last product runs
       ok = ok && wait(&ifull[(tile + 1) % kItems], (tile + 1) / kItems);
@@ -1263,9 +1309,11 @@ struct Backward {
   static constexpr int kChunks = DP / 64;
   static constexpr int kABytes = kTile * 128 * kChunks;   // each of A1, A2
   static constexpr int kBBytes = kBlock * 128 * kChunks;  // each of B1, B2
-  static constexpr int kStages = 3;
+  static constexpr int kStages = 4;
   static constexpr int kSmem = 1024 + 2 * kABytes + 2 * kStages * kBBytes;
-  static constexpr int kSets = DP == 64 ? 1 : 2;          // warps that share 32 rows: each takes half of a block's columns
+  // Warps that share 32 rows, each with its part of a block's columns, kPart at a time: sixteen warps of rows an SM.  (With
+  // eight, issue slots were used to 25 % and two long documents' gradients took 1.69 ms.)
+  static constexpr int kSets = DP == 64 ? 2 : 4, kPart = 16, kSteps = kBlock / kPart / kSets;
   static constexpr int kRowThreads = 128 * kSets, kThreads = 32 + kRowThreads;
   static constexpr int kCtas = DP == 64 ? 2 : 1;
   // TMEM: S, dP, then the sums; the 16-bit values beside them (the next S and dP are then computed meanwhile) or in
@@ -1274,6 +1322,7 @@ struct Backward {
   static constexpr bool kApart = !(DP == 64 && KEYS);
   static constexpr int kEAt = !kApart ? 64 : KEYS ? kAcc2At + DP : kAcc2At;
   static constexpr int kPAt = kApart ? kEAt + 32 : 0;     // (KEYS)
+  static constexpr int kStride = kApart ? 8 : 16;         // from sixteen values to the next: in place, at their own columns
   static constexpr int kTmemCols = DP == 64 ? 256 : 512;
 };
 
@@ -1305,8 +1354,8 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
     mbar_init(smem_u32(&afull), 1);
     for (int s = 0; s < C::kStages; ++s) mbar_init(smem_u32(&bfull[s]), 1);
     mbar_init(smem_u32(&sfull), 1);
-    mbar_init(smem_u32(&sfree), C::kRowThreads);
-    mbar_init(smem_u32(&ready), C::kRowThreads);
+    mbar_init(smem_u32(&sfree), C::kRowThreads / 32);
+    mbar_init(smem_u32(&ready), C::kRowThreads / 32);
     mbar_init(smem_u32(&done), 1);
     mbar_init(smem_u32(&drained), 1);
     abort_word = 0;
@@ -1376,64 +1425,78 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
       // -------------------------------------------------- copies and MMAs
       constexpr uint32_t idesc_s = idesc_of<T>(kBlock, false), idesc_o = idesc_of<T>(DP, true);
       auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_on(bar, parity, kWaitTimeoutMma, abort_flag); };
-      auto slot = [](int n) { return n % C::kStages; };
-      auto phase = [](int n) { return (uint32_t)(n / C::kStages) & 1u; };
-      int asked = 0;
+      const uint32_t a1_at = smem_u32(sA1), a2_at = smem_u32(sA2), b1_at = smem_u32(sB1), b2_at = smem_u32(sB2);
+      int asked = 0, a_block = 0, a_head = KEYS ? head * p.G : head / p.G;
+      Turn<C::kStages> ring, used, held;  // what is asked for next, what S and dP take next, what the sums take next
       auto ask = [&] {
         if (asked >= blocks) return;
-        const int n = asked++, at = other0 + (KEYS ? n % each : n) * kBlock, h = KEYS ? head * p.G + n / each : head / p.G;
-        const uint32_t bar = smem_u32(&bfull[slot(n)]);
+        ++asked;
+        const int at = other0 + a_block * kBlock;
+        const uint32_t bar = smem_u32(&bfull[ring.slot]), to = ring.slot * C::kBBytes;
         mbar_arrive_expect_tx(bar, 2 * C::kBBytes);
+#pragma unroll
         for (int c = 0; c < C::kChunks; ++c) {
-          tma_load_3d(smem_u32(sB1 + slot(n) * C::kBBytes + c * kBlock * 128), &tmB1, 64 * c, h, at, bar);
-          tma_load_3d(smem_u32(sB2 + slot(n) * C::kBBytes + c * kBlock * 128), &tmB2, 64 * c, h, at, bar);
+          tma_load_3d(b1_at + to + c * kBlock * 128, &tmB1, 64 * c, a_head, at, bar);
+          tma_load_3d(b2_at + to + c * kBlock * 128, &tmB2, 64 * c, a_head, at, bar);
+        }
+        ring.next();
+        if (++a_block == each) {
+          a_block = 0;
+          ++a_head;
         }
       };
       const uint32_t ab = smem_u32(&afull);
       mbar_arrive_expect_tx(ab, 2 * C::kABytes);
+#pragma unroll
       for (int c = 0; c < C::kChunks; ++c) {
-        tma_load_3d(smem_u32(sA1 + c * kTile * 128), &tmA1, 64 * c, head, span.x, ab);
-        tma_load_3d(smem_u32(sA2 + c * kTile * 128), &tmA2, 64 * c, head, span.x, ab);
+        tma_load_3d(a1_at + c * kTile * 128, &tmA1, 64 * c, head, span.x, ab);
+        tma_load_3d(a2_at + c * kTile * 128, &tmA2, 64 * c, head, span.x, ab);
       }
       for (int s = 0; s < C::kStages; ++s) ask();
       const int steps = (p.D + 15) / 16;
-      auto products = [&](int n) {  // S and dP
-        if (!wait(&bfull[slot(n)], phase(n))) return false;
+      auto products = [&] {  // S and dP of the next block
+        if (!wait(&bfull[used.slot], used.parity)) return false;
         tc::tc_fence_after();
-        const uint64_t a1 = rows_desc(smem_u32(sA1)), a2 = rows_desc(smem_u32(sA2));
-        const uint64_t b1 = rows_desc(smem_u32(sB1 + slot(n) * C::kBBytes)), b2 = rows_desc(smem_u32(sB2 + slot(n) * C::kBBytes));
-        for (int i = 0; i < steps; ++i) {
-          const uint64_t a = (uint64_t)((i >> 2) * (kTile * 128 / 16) + (i & 3) * 2), b = (uint64_t)((i >> 2) * (kBlock * 128 / 16) + (i & 3) * 2);
-          mma_ss(tmem, a1 + a, b1 + b, idesc_s, i > 0);
-          mma_ss(tmem + 64, a2 + a, b2 + b, idesc_s, i > 0);
+        const uint32_t a1 = rows_desc(a1_at), a2 = rows_desc(a2_at);
+        const uint32_t b1 = rows_desc(b1_at + used.slot * C::kBBytes), b2 = rows_desc(b2_at + used.slot * C::kBBytes);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          if (i >= steps) continue;
+          mma_ss(tmem, a1 + sixteenth(i, kTile), b1 + sixteenth(i, kBlock), idesc_s, i > 0);
+          mma_ss(tmem + 64, a2 + sixteenth(i, kTile), b2 + sixteenth(i, kBlock), idesc_s, i > 0);
         }
         tc::umma_commit(smem_u32(&sfull));
+        used.next();
         return true;
       };
-      bool ok = wait(&afull, 0) && products(0);
+      bool ok = wait(&afull, 0) && products();
       for (int n = 0; n < blocks && ok; ++n) {
-        if (C::kApart && n + 1 < blocks) {
-          ok = wait(&sfree, (uint32_t)n & 1u);
-          if (ok) tc::tc_fence_after();
-          ok = ok && products(n + 1);
+        if (C::kApart) {
+          if (n + 1 < blocks) {
+            ok = wait(&sfree, (uint32_t)n);
+            if (ok) tc::tc_fence_after();
+            ok = ok && products();
+          }
+          if (n > 0) {  // into the slot of the block before
+            ok = ok && wait(&done, (uint32_t)(n - 1));
+            if (ok) ask();
+          }
         }
-        ok = ok && wait(&ready, (uint32_t)n & 1u);
+        ok = ok && wait(&ready, (uint32_t)n);
         if (!ok) break;
         tc::tc_fence_after();
-        if (C::kApart && n > 0) ask();  // (what is ready was written after the products before had ended)
-        const uint64_t b1 = columns_desc(smem_u32(sB1 + slot(n) * C::kBBytes), kBlock * 128);
-        const uint64_t b2 = columns_desc(smem_u32(sB2 + slot(n) * C::kBBytes), kBlock * 128);
+        const uint32_t b1 = columns_desc(b1_at + held.slot * C::kBBytes, kBlock * 128), b2 = columns_desc(b2_at + held.slot * C::kBBytes, kBlock * 128);
+#pragma unroll
         for (int i = 0; i < kBlock / 16; ++i) {
-          if (KEYS) mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + 8 * i, b2 + (uint64_t)(i * 16 * 128 / 16), idesc_o, n > 0 || i > 0);
-          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + 8 * i, b1 + (uint64_t)(i * 16 * 128 / 16), idesc_o, n > 0 || i > 0);
+          if (KEYS) mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + C::kStride * i, b2 + i * (16 * 128 / 16), idesc_o, n > 0 || i > 0);
+          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kStride * i, b1 + i * (16 * 128 / 16), idesc_o, n > 0 || i > 0);
         }
         tc::umma_commit(smem_u32(&done));
+        held.next();
         if (!C::kApart && n + 1 < blocks) {
-          ok = wait(&done, (uint32_t)n & 1u);
-          if (ok) {
-            ask();
-            ok = products(n + 1);
-          }
+          ok = wait(&done, (uint32_t)n);
+          if (ok) ok = products();
+          ask();
         }
       }
       if (!ok) {  // given up: no MMA in flight behind this CTA
@@ -1442,7 +1505,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
       }
       // nor a copy
       wait_on(&afull, 0, kWaitTimeoutProducer, nullptr);
-      for (int i = max(0, asked - C::kStages); i < asked; ++i) wait_on(&bfull[slot(i)], phase(i), kWaitTimeoutProducer, nullptr);
+      for (int i = max(0, asked - C::kStages); i < asked; ++i) wait_on(&bfull[i % C::kStages], (uint32_t)(i / C::kStages), kWaitTimeoutProducer, nullptr);
     }
   } else {
     // -------------------------------------------------------------- rows
@@ -1491,19 +1554,23 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
       ok = __all_sync(kAll, wait_on(&sfull, (uint32_t)n, kWaitTimeoutEpilogue, abort_flag));
       tc::tc_fence_after();
 #pragma unroll 1
-      for (int half = C::kSets == 2 ? set : 0; half < (C::kSets == 2 ? set + 1 : 2) && ok; ++half) {
-        const int c0 = half * kHalf;
-        // of the half's keys (queries) and the warp's rows: is there one that sees, do all
-        const Seen seen = KEYS ? s_span[n & 1][half].of(span.x + quarter * 32) : reach.of(o0 + c0);
-        uint32_t w[16], e[16];
+      for (int step = 0; step < C::kSteps && ok; ++step) {
+        const int c0 = (set * C::kSteps + step) * C::kPart;
+        // of these keys (queries) and the warp's rows: is there one that sees, do all
+        const Seen seen = KEYS ? s_span[n & 1][c0 / kHalf].of(span.x + quarter * 32) : reach.of(o0 + c0, C::kPart);
+        uint32_t w[C::kPart / 2], e[C::kPart / 2];
         if (seen != kNone) {
-          uint32_t x[kHalf], y[kHalf];
-          tmem_get32(mine + c0, x);
-          tmem_get32(mine + 64 + c0, y);
+          uint32_t x[C::kPart], y[C::kPart];
+          tmem_get16(mine + c0, x);
+          tmem_get16(mine + 64 + c0, y);
           tmem_wait_ld();
+          if (C::kApart && step == C::kSteps - 1) {  // the next block's products may begin
+            tc::tc_fence_before();
+            warp_arrive(&sfree);
+          }
           // y: (dP - delta) times the slant; x: the score in units of log 2 (over `unit`)
 #pragma unroll
-          for (int c = 0; c < kHalf; c += 2) {
+          for (int c = 0; c < C::kPart; c += 2) {
             const F2 d = KEYS ? *reinterpret_cast<const F2*>(&s_delta[n & 1][c0 + c]) : f2(-delta, -delta);
             const float2 v = un(fma2(f2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), f2(sigma, sigma), d));
             y[c] = __float_as_uint(v.x);
@@ -1514,7 +1581,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
             const float in = p.scale / p.cap * (2.0f * kLog2e);
             const F2 in2 = f2(in, in), one = f2(1.0f, 1.0f), minus = f2(-2.0f, -2.0f);
 #pragma unroll
-            for (int c = 0; c < kHalf; c += 2) {
+            for (int c = 0; c < C::kPart; c += 2) {
               const float2 v = un(mul2(pair(x + c), in2));
               const float2 d = un(add2(f2(exp2_fast(v.x), exp2_fast(v.y)), one));
               const F2 th = fma2(f2(rcp_fast(d.x), rcp_fast(d.y)), minus, one);
@@ -1525,7 +1592,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
           }
           if (slope2 != 0.0f) {
 #pragma unroll
-            for (int c = 0; c < kHalf; ++c) {
+            for (int c = 0; c < C::kPart; ++c) {
               const int far = KEYS ? s_row[n & 1][c0 + c].z - r : row.z - (o0 + c0 + c);
               x[c] = __float_as_uint(fmaf(-slope2, fabsf((float)far), __uint_as_float(x[c]) * left));
             }
@@ -1533,7 +1600,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
           }
           if (seen == kSome) {
 #pragma unroll
-            for (int c = 0; c < kHalf; ++c) {
+            for (int c = 0; c < C::kPart; ++c) {
               int4 q = row;
               if (KEYS) q = s_row[n & 1][c0 + c];
               const int j = KEYS ? r : o0 + c0 + c;
@@ -1544,7 +1611,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
             }
           }
 #pragma unroll
-          for (int c = 0; c < kHalf; c += 2) {
+          for (int c = 0; c < C::kPart; c += 2) {
             const F2 l = KEYS ? *reinterpret_cast<const F2*>(&s_lse[n & 1][c0 + c]) : f2(-lse, -lse);
             const float2 v = un(fma2(f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), f2(left, left), l));
             const float a = exp2_fast(v.x), b = exp2_fast(v.y);
@@ -1554,25 +1621,25 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) w[c] = e[c] = 0u;
+          for (int c = 0; c < C::kPart / 2; ++c) w[c] = e[c] = 0u;
+          if (C::kApart && step == C::kSteps - 1) {
+            tc::tc_fence_before();
+            warp_arrive(&sfree);
+          }
         }
-        if (C::kApart && (C::kSets == 2 || half == 1)) {
-          tc::tc_fence_before();
-          mbar_arrive(smem_u32(&sfree));
-        }
-        if (C::kApart && n > 0 && (C::kSets == 2 || half == 0)) {  // the products before have read their values
+        if (C::kApart && n > 0 && step == 0) {  // the products before have read their values
           ok = __all_sync(kAll, wait_on(&done, (uint32_t)(n - 1), kWaitTimeoutEpilogue, abort_flag));
           tc::tc_fence_after();
         }
         if (ok) {
-          if (KEYS) tmem_put16(mine + C::kPAt + c0 / 2, w);
-          tmem_put16(mine + C::kEAt + c0 / 2, e);
+          if (KEYS) tmem_put8(mine + C::kPAt + c0 / C::kPart * C::kStride, w);
+          tmem_put8(mine + C::kEAt + c0 / C::kPart * C::kStride, e);
         }
       }
       if (ok) {
         tmem_wait_st();
         tc::tc_fence_before();
-        mbar_arrive(smem_u32(&ready));
+        warp_arrive(&ready);
       }
       if (KEYS && n + 1 < blocks) {  // (a give-up is everyone's: all meet here)
         deposit(n + 1);
