@@ -40,7 +40,7 @@ struct Params {
   int4* tiles;                    // of the queries: rows [x, y), the keys that they see [z, w)
   uint32_t* next;                 // tickets for work
   float* part;                    // few queries: of every row and split, the sums [D], their maximum and their weights' sum
-  int splits;
+  int splits, parts;
   const void *q_off, *k_off, *prefix;
   const float* slopes;
   int64_t q_t, q_h, k_t, k_h, v_t, v_h, g_t, g_h;  // elements from token to token and from head to head
@@ -316,36 +316,15 @@ __device__ __forceinline__ float2 widen2(uint32_t w) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(bf16_lo(w), bf16_hi(w));
   else return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
-// (a . b, b . b) of a row, summed over its lanes
-template <typename T, int LANES, bool VEC>
-__device__ __forceinline__ float2 row_sums(const T* a, const T* b, int D) {
-  const int lane = threadIdx.x % LANES;
-  float s = 0.0f, n = 0.0f;
-  if constexpr (VEC) {
-    for (int c = lane * 8; c < D; c += LANES * 8) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(b + c));
-      const uint4 u = a != nullptr ? __ldg(reinterpret_cast<const uint4*>(a + c)) : make_uint4(0u, 0u, 0u, 0u);
-      const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 x = widen2<T>(uw[i]), y = widen2<T>(vw[i]);
-        s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
-        n = fmaf(y.x, y.x, fmaf(y.y, y.y, n));
-      }
-    }
-  } else {
-    for (int c = lane; c < D; c += LANES) {
-      const float y = to_f32(b[c]);
-      if (a != nullptr) s = fmaf(to_f32(a[c]), y, s);
-      n = fmaf(y, y, n);
-    }
-  }
+// sums over the lanes of a row
+template <int LANES>
+__device__ __forceinline__ float2 lanes_sum(float2 s) {
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(kAll, s, o);
-    n += __shfl_xor_sync(kAll, n, o);
+    s.x += __shfl_xor_sync(kAll, s.x, o);
+    s.y += __shfl_xor_sync(kAll, s.y, o);
   }
-  return make_float2(s, n);
+  return s;
 }
 template <typename T, int LANES, bool VEC>
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Params p) {
@@ -360,27 +339,89 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Para
   }
   if (kPeaks && threadIdx.x < 2) s_peak[threadIdx.x] = 0;
   __syncthreads();
-  constexpr int kRows = 256 / LANES;
-  const int64_t queries = (int64_t)p.Tq * p.H, all = queries + (kPeaks ? (int64_t)p.Tk * p.Hk : 0);
-  const int64_t step = (int64_t)(gridDim.x - row_ctas) * kRows;
-  for (int64_t i0 = (int64_t)(blockIdx.x - row_ctas) * kRows; i0 < all; i0 += step) {
-    const int64_t i = i0 + threadIdx.x / LANES;
-    const bool query = i < queries;
-    float2 s = make_float2(0.0f, 0.0f);
-    if (query) {
-      const int64_t r = i / p.H;
-      const int h = (int)(i - r * p.H);
-      s = row_sums<T, LANES, VEC>(static_cast<const T*>(p.o) + i * p.D, static_cast<const T*>(p.g) + r * p.g_t + h * p.g_h, p.D);
-      if (threadIdx.x % LANES == 0) p.delta[(int64_t)h * p.Tq + r] = s.x;
-    } else if (kPeaks) {
-      const int64_t j = min(i, all - 1) - queries, r = j / p.Hk;
-      s = row_sums<T, LANES, VEC>(nullptr, static_cast<const T*>(p.v) + r * p.v_t + (j - r * p.Hk) * p.v_h, p.D);
+  float peak[2] = {0.0f, 0.0f};  // squares
+  constexpr int kRows = 256 / LANES, kTwo = 2;  // rows of a CTA at a time, twice
+  const int lane = threadIdx.x % LANES, c = lane * 8;
+  // rows (token, head) [0, tokens * heads), the CTAs in turn; from one to this thread's next without a quotient
+  auto scan = [&](int tokens, int heads, auto source, auto use) {
+    const int64_t step = (int64_t)(gridDim.x - row_ctas) * kRows, first = (int64_t)(blockIdx.x - row_ctas) * kRows + threadIdx.x / LANES;
+    const int d_token = (int)(step / heads), d_head = (int)(step - (int64_t)d_token * heads);
+    int64_t token = first / heads;
+    int head = (int)(first - token * heads);
+    while (__any_sync(kAll, token < tokens)) {
+      int64_t at[kTwo];
+      int h[kTwo];
+      const T *x[kTwo], *y[kTwo];
+      float2 s[kTwo];
+#pragma unroll
+      for (int u = 0; u < kTwo; ++u) {
+        at[u] = token;
+        h[u] = head;
+        x[u] = y[u] = nullptr;
+        if (token < tokens) source(token, head, x[u], y[u]);
+        s[u] = make_float2(0.0f, 0.0f);
+        token += d_token;
+        head += d_head;
+        if (head >= heads) {
+          head -= heads;
+          ++token;
+        }
+      }
+      if constexpr (VEC) {  // (a lane's sixteen bytes are its part of a row)
+        uint4 xv[kTwo], yv[kTwo];
+#pragma unroll
+        for (int u = 0; u < kTwo; ++u) {
+          xv[u] = x[u] != nullptr && c < p.D ? __ldg(reinterpret_cast<const uint4*>(x[u] + c)) : make_uint4(0u, 0u, 0u, 0u);
+          yv[u] = y[u] != nullptr && c < p.D ? __ldg(reinterpret_cast<const uint4*>(y[u] + c)) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int u = 0; u < kTwo; ++u) {
+          const uint32_t xw[4] = {xv[u].x, xv[u].y, xv[u].z, xv[u].w}, yw[4] = {yv[u].x, yv[u].y, yv[u].z, yv[u].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = widen2<T>(xw[k]), g = widen2<T>(yw[k]);
+            s[u].x = fmaf(f.x, g.x, fmaf(f.y, g.y, s[u].x));
+            if (kPeaks) s[u].y = fmaf(g.x, g.x, fmaf(g.y, g.y, s[u].y));
+          }
+        }
+      } else {
+        for (int u = 0; u < kTwo; ++u)
+          for (int k = lane; y[u] != nullptr && k < p.D; k += LANES) {
+            const float g = to_f32(y[u][k]);
+            if (x[u] != nullptr) s[u].x = fmaf(to_f32(x[u][k]), g, s[u].x);
+            s[u].y = fmaf(g, g, s[u].y);
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < kTwo; ++u) {
+        s[u] = lanes_sum<LANES>(s[u]);
+        if (lane == 0 && y[u] != nullptr) use(at[u], h[u], s[u]);
+      }
     }
-    if (kPeaks && i < all && s.y > 0.0f && s.y < INFINITY && threadIdx.x % LANES == 0) atomicMax(&s_peak[query ? 0 : 1], __float_as_uint(sqrtf(s.y)));
-  }
+  };
+  scan(p.Tq, p.H,
+       [&](int64_t r, int h, const T*& x, const T*& y) {
+         x = static_cast<const T*>(p.o) + (r * p.H + h) * p.D;
+         y = static_cast<const T*>(p.g) + r * p.g_t + h * p.g_h;
+       },
+       [&](int64_t r, int h, float2 s) {
+         p.delta[(int64_t)h * p.Tq + r] = s.x;
+         if (kPeaks && s.y < INFINITY) peak[0] = fmaxf(peak[0], s.y);
+       });
+  if constexpr (kPeaks)
+    scan(p.Tk, p.Hk, [&](int64_t r, int h, const T*&, const T*& y) { y = static_cast<const T*>(p.v) + r * p.v_t + h * p.v_h; },
+         [&](int64_t, int, float2 s) {
+           if (s.y < INFINITY) peak[1] = fmaxf(peak[1], s.y);
+         });
   if (kPeaks) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t high = __reduce_max_sync(kAll, __float_as_uint(sqrtf(peak[i])));
+      if ((threadIdx.x & 31) == 0) atomicMax(&s_peak[i], high);
+    }
     __syncthreads();
-    if (threadIdx.x < 2) atomicMax(p.peaks + threadIdx.x, s_peak[threadIdx.x]);
+    if (threadIdx.x < 2 && s_peak[threadIdx.x] > *reinterpret_cast<volatile uint32_t*>(p.peaks + threadIdx.x))
+      atomicMax(p.peaks + threadIdx.x, s_peak[threadIdx.x]);
   }
 }
 
@@ -1314,7 +1355,7 @@ struct Backward {
   // Warps that share 32 rows, each with its part of a block's columns, kPart at a time: sixteen warps of rows an SM.  (With
   // eight, issue slots were used to 25 % and two long documents' gradients took 1.69 ms.)
   static constexpr int kSets = DP == 64 ? 2 : 4, kPart = 16, kSteps = kBlock / kPart / kSets;
-  static constexpr int kRowThreads = 128 * kSets, kThreads = 32 + kRowThreads;
+  static constexpr int kRowThreads = 128 * kSets, kThreads = 64 + kRowThreads;
   static constexpr int kCtas = DP == 64 ? 2 : 1;
   // TMEM: S, dP, then the sums; the 16-bit values beside them (the next S and dP are then computed meanwhile) or in
   // place of S and dP, where two CTAs of 256 columns leave no room
@@ -1325,6 +1366,13 @@ struct Backward {
   static constexpr int kStride = kApart ? 8 : 16;         // from sixteen values to the next: in place, at their own columns
   static constexpr int kTmemCols = DP == 64 ? 256 : 512;
 };
+
+// (fp16) the power of two that keeps |dP - delta| times it under 1
+__device__ __forceinline__ float range_of(const Params& p) {
+  const float bound = 2.0f * __uint_as_float(p.peaks[0]) * __uint_as_float(p.peaks[1]);  // of |dP - delta|
+  const int e = (int)(__float_as_uint(bound) >> 23) - 126;                             // bound < 2^e
+  return bound > 0.0f && bound < INFINITY ? __uint_as_float((uint32_t)min(max(127 - e, 1), 254) << 23) : 1.0f;
+}
 
 template <typename T, int DP, bool KEYS>
 __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEYS>::kCtas)
@@ -1338,7 +1386,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   uint8_t* sA2 = sA1 + C::kABytes;
   uint8_t* sB1 = sA2 + C::kABytes;
   uint8_t* sB2 = sB1 + C::kStages * C::kBBytes;
-  __shared__ __align__(8) uint64_t afull, bfull[C::kStages], sfull, sfree, ready, done, drained;
+  __shared__ __align__(8) uint64_t afull, bfull[C::kStages], sfull, sfree, ready, done, drained[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word, s_lo[4], s_hi[4], s_bad[kTile];
   // of the block's queries (KEYS), for this block and the next: lse and delta (negative), interval and place; and, of its
@@ -1348,7 +1396,9 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   __shared__ Span s_span[2][2];
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int head = blockIdx.y, tile = KEYS ? blockIdx.x : gridDim.x - 1 - blockIdx.x;
+  // (KEYS) blockIdx.z: one of the heads that share the key head, where there are parts; else all of them
+  const int head = blockIdx.y, heads = KEYS && p.parts ? 1 : p.G, first_head = head * p.G + (KEYS ? (int)blockIdx.z : 0);
+  const int tile = KEYS ? blockIdx.x : gridDim.x - 1 - blockIdx.x;
 
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&afull), 1);
@@ -1357,7 +1407,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
     mbar_init(smem_u32(&sfree), C::kRowThreads / 32);
     mbar_init(smem_u32(&ready), C::kRowThreads / 32);
     mbar_init(smem_u32(&done), 1);
-    mbar_init(smem_u32(&drained), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&drained[i]), 1);
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1370,11 +1420,11 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 span = tile_rows(KEYS ? p.k_off : p.q_off, p.off64, p.S, KEYS ? p.Tk : p.Tq, tile, p.by_segment);
-  const int quarter = warp & 3, set = (warp - 1) >> 2;
+  const int quarter = warp & 3, set = (warp - 2) >> 2;
   const int r = span.x + quarter * 32 + lane;  // the thread's query or key
   int4 row = make_int4(0, 0, 0, 0);
   if (KEYS) {
-    if (threadIdx.x == 32) {
+    if (threadIdx.x == 64) {
       int lo = INT_MAX, hi = 0;
       if (span.y > span.x) {
         // queries of the segments from the first key's to the last key's
@@ -1393,7 +1443,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
       s_lo[0] = s_lo[1] = s_lo[2] = s_lo[3] = lo;
       s_hi[0] = s_hi[1] = s_hi[2] = s_hi[3] = hi;
     }
-  } else if (warp >= 1 && warp < 5) {
+  } else if (warp >= 2 && warp < 6) {
     if (r < span.y) row = __ldg(p.rows + r);
     int lo = row.y > row.x ? row.x : INT_MAX, hi = row.y > row.x ? row.y : 0;
     lo = __reduce_min_sync(kAll, lo);
@@ -1402,7 +1452,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
       s_lo[quarter] = lo;
       s_hi[quarter] = hi;
     }
-  } else if (warp >= 5) {
+  } else if (warp >= 6) {
     if (r < span.y) row = __ldg(p.rows + r);
   }
   tc::tc_fence_before();
@@ -1411,23 +1461,55 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   const uint32_t tmem = tmem_slot;
   const int other0 = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), other1 = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
   const int each = other1 > other0 ? (other1 - other0 + kBlock - 1) / kBlock : 0;  // blocks of a head
-  const int blocks = KEYS ? each * p.G : each;
+  const int blocks = KEYS ? each * heads : each;
   const int up = std::is_same<T, __half>::value ? 15 : 0;
-  float sigma = 1.0f;
-  if (up != 0) {
-    const float bound = 2.0f * __uint_as_float(p.peaks[0]) * __uint_as_float(p.peaks[1]);  // of |dP - delta|
-    const int e = (int)(__float_as_uint(bound) >> 23) - 126;                             // bound < 2^e
-    if (bound > 0.0f && bound < INFINITY) sigma = __uint_as_float((uint32_t)min(max(127 - e, 1), 254) << 23);
-  }
+  const float sigma = up != 0 ? range_of(p) : 1.0f;
 
   if (warp == 0) {
     if (lane == 0 && blocks > 0) {
-      // -------------------------------------------------- copies and MMAs
-      constexpr uint32_t idesc_s = idesc_of<T>(kBlock, false), idesc_o = idesc_of<T>(DP, true);
+      // ----------------------------------------- the resident tiles, S and dP
+      constexpr uint32_t idesc = idesc_of<T>(kBlock, false);
       auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_on(bar, parity, kWaitTimeoutMma, abort_flag); };
-      const uint32_t a1_at = smem_u32(sA1), a2_at = smem_u32(sA2), b1_at = smem_u32(sB1), b2_at = smem_u32(sB2);
-      int asked = 0, a_block = 0, a_head = KEYS ? head * p.G : head / p.G;
-      Turn<C::kStages> ring, used, held;  // what is asked for next, what S and dP take next, what the sums take next
+      const uint32_t a1_at = smem_u32(sA1), a2_at = smem_u32(sA2), b1_at = smem_u32(sB1), b2_at = smem_u32(sB2), ab = smem_u32(&afull);
+      mbar_arrive_expect_tx(ab, 2 * C::kABytes);
+#pragma unroll
+      for (int c = 0; c < C::kChunks; ++c) {
+        tma_load_3d(a1_at + c * kTile * 128, &tmA1, 64 * c, head, span.x, ab);
+        tma_load_3d(a2_at + c * kTile * 128, &tmA2, 64 * c, head, span.x, ab);
+      }
+      Turn<C::kStages> used;
+      const int steps = (p.D + 15) / 16;
+      const uint32_t a1 = rows_desc(a1_at), a2 = rows_desc(a2_at);
+      bool ok = wait(&afull, 0);
+      for (int n = 0; n < blocks && ok; ++n) {
+        ok = wait(&bfull[used.slot], used.parity);
+        if (n > 0) ok = ok && wait(C::kApart ? &sfree : &done, (uint32_t)(n - 1));  // S's and dP's columns
+        if (!ok) break;
+        tc::tc_fence_after();
+        const uint32_t b1 = rows_desc(b1_at + used.slot * C::kBBytes), b2 = rows_desc(b2_at + used.slot * C::kBBytes);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          if (i >= steps) continue;
+          mma_ss(tmem, a1 + sixteenth(i, kTile), b1 + sixteenth(i, kBlock), idesc, i > 0);
+          mma_ss(tmem + 64, a2 + sixteenth(i, kTile), b2 + sixteenth(i, kBlock), idesc, i > 0);
+        }
+        tc::umma_commit(smem_u32(&sfull));
+        used.next();
+      }
+      if (!ok) {  // given up: no MMA in flight behind this CTA
+        tc::umma_commit(smem_u32(&drained[0]));
+        wait_on(&drained[0], 0, kWaitTimeoutMma, nullptr);
+      }
+      wait_on(&afull, 0, kWaitTimeoutProducer, nullptr);  // nor a copy
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && blocks > 0) {
+      // ---------------------------------------------- the blocks, the sums
+      constexpr uint32_t idesc = idesc_of<T>(DP, true);
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_on(bar, parity, kWaitTimeoutMma, abort_flag); };
+      const uint32_t b1_at = smem_u32(sB1), b2_at = smem_u32(sB2);
+      int asked = 0, a_block = 0, a_head = KEYS ? first_head : head / p.G;
+      Turn<C::kStages> ring, held;  // what is asked for next, what the sums take next
       auto ask = [&] {
         if (asked >= blocks) return;
         ++asked;
@@ -1445,71 +1527,31 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
           ++a_head;
         }
       };
-      const uint32_t ab = smem_u32(&afull);
-      mbar_arrive_expect_tx(ab, 2 * C::kABytes);
-#pragma unroll
-      for (int c = 0; c < C::kChunks; ++c) {
-        tma_load_3d(a1_at + c * kTile * 128, &tmA1, 64 * c, head, span.x, ab);
-        tma_load_3d(a2_at + c * kTile * 128, &tmA2, 64 * c, head, span.x, ab);
-      }
       for (int s = 0; s < C::kStages; ++s) ask();
-      const int steps = (p.D + 15) / 16;
-      auto products = [&] {  // S and dP of the next block
-        if (!wait(&bfull[used.slot], used.parity)) return false;
-        tc::tc_fence_after();
-        const uint32_t a1 = rows_desc(a1_at), a2 = rows_desc(a2_at);
-        const uint32_t b1 = rows_desc(b1_at + used.slot * C::kBBytes), b2 = rows_desc(b2_at + used.slot * C::kBBytes);
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          if (i >= steps) continue;
-          mma_ss(tmem, a1 + sixteenth(i, kTile), b1 + sixteenth(i, kBlock), idesc_s, i > 0);
-          mma_ss(tmem + 64, a2 + sixteenth(i, kTile), b2 + sixteenth(i, kBlock), idesc_s, i > 0);
-        }
-        tc::umma_commit(smem_u32(&sfull));
-        used.next();
-        return true;
-      };
-      bool ok = wait(&afull, 0) && products();
-      for (int n = 0; n < blocks && ok; ++n) {
-        if (C::kApart) {
-          if (n + 1 < blocks) {
-            ok = wait(&sfree, (uint32_t)n);
-            if (ok) tc::tc_fence_after();
-            ok = ok && products();
-          }
-          if (n > 0) {  // into the slot of the block before
-            ok = ok && wait(&done, (uint32_t)(n - 1));
-            if (ok) ask();
-          }
-        }
-        ok = ok && wait(&ready, (uint32_t)n);
+      bool ok = true;
+      for (int n = 0; n < blocks; ++n) {
+        ok = wait(&bfull[held.slot], held.parity) && wait(&ready, (uint32_t)n);
         if (!ok) break;
         tc::tc_fence_after();
         const uint32_t b1 = columns_desc(b1_at + held.slot * C::kBBytes, kBlock * 128), b2 = columns_desc(b2_at + held.slot * C::kBBytes, kBlock * 128);
 #pragma unroll
         for (int i = 0; i < kBlock / 16; ++i) {
-          if (KEYS) mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + C::kStride * i, b2 + i * (16 * 128 / 16), idesc_o, n > 0 || i > 0);
-          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kStride * i, b1 + i * (16 * 128 / 16), idesc_o, n > 0 || i > 0);
+          if (KEYS) mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + C::kStride * i, b2 + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
+          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kStride * i, b1 + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
         }
         tc::umma_commit(smem_u32(&done));
         held.next();
-        if (!C::kApart && n + 1 < blocks) {
-          ok = wait(&done, (uint32_t)n);
-          if (ok) ok = products();
-          ask();
-        }
+        if (n > 0) ask();  // (into the slot of the block before: its sums had ended before these values were written)
       }
-      if (!ok) {  // given up: no MMA in flight behind this CTA
-        tc::umma_commit(smem_u32(&drained));
-        wait_on(&drained, 0, kWaitTimeoutMma, nullptr);
+      if (!ok) {
+        tc::umma_commit(smem_u32(&drained[1]));
+        wait_on(&drained[1], 0, kWaitTimeoutMma, nullptr);
       }
-      // nor a copy
-      wait_on(&afull, 0, kWaitTimeoutProducer, nullptr);
       for (int i = max(0, asked - C::kStages); i < asked; ++i) wait_on(&bfull[i % C::kStages], (uint32_t)(i / C::kStages), kWaitTimeoutProducer, nullptr);
     }
   } else {
     // -------------------------------------------------------------- rows
-    const int t = threadIdx.x - 32;
+    const int t = threadIdx.x - 64;
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
     const float unit = p.cap > 0.0f ? p.cap * kLog2e : p.scale * kLog2e;
     float slope2 = 0.0f, lse = 0.0f, delta = 0.0f;
@@ -1525,7 +1567,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
     int4 next_row = make_int4(0, 0, 0, 0);
     auto fetch = [&](int n) {
       if (t >= kBlock) return;
-      const int i = other0 + (n % each) * kBlock + t, h = head * p.G + n / each;
+      const int i = other0 + (n % each) * kBlock + t, h = first_head + n / each;
       const bool there = i < other1;
       next_row = there ? __ldg(p.rows + i) : make_int4(0, 0, 0, 0);
       next_lse = there ? lse_of(p, i, h) - up : INFINITY;
@@ -1550,7 +1592,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
     }
     for (int n = 0; n < blocks && ok; ++n) {
       const int o0 = other0 + (KEYS ? n % each : n) * kBlock;
-      if (KEYS) slope2 = p.slopes != nullptr ? kLog2e * __ldg(p.slopes + head * p.G + n / each) : 0.0f;
+      if (KEYS) slope2 = p.slopes != nullptr ? kLog2e * __ldg(p.slopes + first_head + n / each) : 0.0f;
       ok = __all_sync(kAll, wait_on(&sfull, (uint32_t)n, kWaitTimeoutEpilogue, abort_flag));
       tc::tc_fence_after();
 #pragma unroll 1
@@ -1654,8 +1696,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
     ok = meet(ok);
     // a row that is not finite is taken again by itself; the sums' columns are shared by the sets
     const float down = up != 0 ? 0x1p-15f : 1.0f, w1 = p.scale * down / sigma;
-    const int heads = KEYS ? p.Hk : p.H;
-    const int64_t at = ((int64_t)r * heads + head) * p.D;
+    const int64_t at = ((int64_t)r * (KEYS ? p.Hk : p.H) + head) * p.D;
     const bool mine_too = KEYS || row.y > row.x, there = r < span.y;
     for (int pass = 0; pass < 2 && ok; ++pass) {
       for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
@@ -1675,6 +1716,13 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
           }
           if (pass == 0) {
             if (there && !finite32(o)) s_bad[quarter * 32 + lane] = 1;
+          } else if (KEYS && p.parts) {  // (whatever they are: their sum is looked at)
+            float* to = p.part + ((int64_t)(which * p.G + blockIdx.z) * p.Tk * p.Hk * p.D) + at + c;
+            if (there)
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                if (c + i < p.D)
+                  *reinterpret_cast<float4*>(to + i) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
           } else if (there && !s_bad[quarter * 32 + lane]) {
             store_sums<T>(out + at + c, o, p.D - c, which ? down : w1, wide);
           }
@@ -1683,7 +1731,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
       if (pass == 0) meet(true);
     }
     if (ok && set == 0) {
-      uint32_t again = __ballot_sync(kAll, there && s_bad[quarter * 32 + lane]);
+      uint32_t again = __ballot_sync(kAll, there && s_bad[quarter * 32 + lane] && !(KEYS && p.parts));
       while (again != 0) {
         const int i = __ffs(again) - 1;
         again &= again - 1;
@@ -1698,6 +1746,40 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   if (warp == 0) {
     tc::tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
+  }
+}
+
+// dk and dv of a key head from its query heads' parts, a warp a row
+template <typename T>
+__global__ void __launch_bounds__(256) keys_join_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (int64_t)p.Tk * p.Hk;
+  if (row >= rows) return;
+  constexpr bool kHalfType = std::is_same<T, __half>::value;
+  const float down = kHalfType ? 0x1p-15f : 1.0f, w1 = p.scale * down / (kHalfType ? range_of(p) : 1.0f);
+  bool finite = true;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    T* out = static_cast<T*>(which ? p.dv : p.dk) + row * p.D;
+    for (int c = lane * 4; c < p.D; c += 128) {
+      float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+      for (int g = 0; g < p.G; ++g) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p.part + (int64_t)(which * p.G + g) * rows * p.D + row * p.D + c));
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+      }
+      const float w = which ? down : w1, any = s.x * 0.0f + s.y * 0.0f + s.z * 0.0f + s.w * 0.0f;
+      finite = finite && any == any;
+      *reinterpret_cast<uint2*>(out + c) = make_uint2(pack2<T>(s.x * w, s.y * w), pack2<T>(s.z * w, s.w * w));
+    }
+  }
+  if (!__all_sync(kAll, finite)) {
+    __syncwarp();
+    row_dkv<T>(p, (int)(row / p.Hk), (int)(row % p.Hk));
   }
 }
 
@@ -1823,6 +1905,11 @@ static int forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
                 "attention row_kernel launch", args);
 }
 
+// Whether the query heads that share a key head go to CTAs of their own, whose sums are added up after: with fewer than
+// four tiles of keys an SM the last ones take too long by themselves (two documents of 6100 keys, two key heads for eight:
+// 194 tiles of up to 384 blocks, 749 us; 776 of 96).  Each part is written and read once, in 32 bits.
+static bool key_parts(int64_t Tk, int H, int Hk) { return H > Hk && H / Hk <= 64 && Tk >= kTile && Tk / kTile * Hk < 4 * (int64_t)sm_count(); }
+
 template <typename T, int DP, bool KEYS>
 static int run_backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   using C = Backward<DP, KEYS>;
@@ -1844,8 +1931,12 @@ static int run_backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   p.by_segment = KEYS ? choose_by_segment(p.Tk, p.Tq, p.S) : choose_by_segment(p.Tq, p.Tk, p.S);
   const int64_t tiles = p.by_segment ? total / kTile + p.S + 2 : (total + kTile - 1) / kTile;
   void* args[] = {KEYS ? &k : &q, KEYS ? &v : &g, KEYS ? &q : &k, KEYS ? &g : &v, &p};
-  return launch(backward_kernel<T, DP, KEYS>, dim3((unsigned)tiles, KEYS ? p.Hk : p.H), C::kThreads, C::kSmem, true, st,
-                "attention backward_kernel launch", args);
+  if ((rc = launch(backward_kernel<T, DP, KEYS>, dim3((unsigned)tiles, KEYS ? p.Hk : p.H, KEYS && p.parts ? p.G : 1), C::kThreads, C::kSmem,
+                   true, st, "attention backward_kernel launch", args)))
+    return rc;
+  if (!KEYS || !p.parts) return RB_OK;
+  void* join[] = {&p};
+  return launch(keys_join_kernel<T>, dim3((unsigned)(((int64_t)p.Tk * p.Hk + 7) / 8)), 256, 0, true, st, "attention keys_join_kernel launch", join);
 }
 
 template <typename T>
@@ -1867,6 +1958,7 @@ static int backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   const bool tiles = tiled(p) && p.Tq > 0 && p.Tk > 0 && mappable(p.g, p.Tq, p.H, p.g_t, p.g_h) && aligned(p.dq, 16) &&
                      aligned(p.dk, 16) && aligned(p.dv, 16);
   if (tiles) {
+    p.parts = key_parts(p.Tk, p.H, p.Hk);
     if ((rc = p.D <= 64 ? run_backward<T, 64, true>(p, dt, st) : run_backward<T, 128, true>(p, dt, st))) return rc;
     return p.D <= 64 ? run_backward<T, 64, false>(p, dt, st) : run_backward<T, 128, false>(p, dt, st);
   }
@@ -1959,7 +2051,8 @@ extern "C" int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, con
 
 extern "C" int64_t rb_segment_attention_backward_workspace_size(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D) {
   if (Tq < 0 || Tk < 0 || S < 0 || H <= 0 || Hk <= 0 || D <= 0 || Tq > 1 << 30) return -1;
-  return 16 + Tq * 16 + (int64_t)H * Tq * 4;
+  const int64_t parts = H % Hk == 0 && D % 8 == 0 && D <= 128 && attn::key_parts(Tk, H, Hk) ? (int64_t)2 * H * Tk * D * 4 : 0;
+  return 16 + Tq * 16 + ((int64_t)H * Tq * 4 + 15) / 16 * 16 + parts;
 }
 
 extern "C" int rb_segment_attention_backward(const void* grad, int64_t g_t, int64_t g_h, const void* q, int64_t q_t, int64_t q_h,
@@ -1997,6 +2090,7 @@ extern "C" int rb_segment_attention_backward(const void* grad, int64_t g_t, int6
   p.peaks = static_cast<uint32_t*>(workspace);
   p.rows = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + 16);
   p.delta = reinterpret_cast<float*>(p.rows + Tq);
+  p.part = p.delta + ((int64_t)H * Tq + 3) / 4 * 4;
   p.q_off = q_offsets;
   p.k_off = k_offsets;
   p.prefix = prefix;
