@@ -38,6 +38,7 @@ struct Params {
   float* delta;                   // [H, Tq]
   int4* rows;                     // [Tq]: lo, hi, place of the query among the packed keys, 0
   int4* tiles;                    // of the queries: rows [x, y), the keys that they see [z, w)
+  int4* key_tiles;                // (backward) of the keys: rows [x, y), queries that may see them [z, w)
   uint32_t* next;                 // tickets for work
   float* part;                    // few queries: of every row and split, the sums [D], their maximum and their weights' sum
   int splits, parts;
@@ -48,6 +49,7 @@ struct Params {
   float scale, cap;
   uint32_t* peaks;                // fp16 backward: the largest norms of a row of g and of v
   int by_segment, n_tiles;        // tiles follow segments (else: 128 rows of the packed order)
+  int keys_by_segment, n_key_tiles;
 };
 
 __device__ __forceinline__ int64_t entry(const void* a, int wide, int64_t i) {
@@ -127,7 +129,7 @@ __device__ __forceinline__ int2 tile_rows(const void* off, int wide, int S, int 
   }
   const int start = lo == 0 ? 0 : offset_at(off, wide, lo - 1, total) * factor;
   const int end = lo == S + 1 ? total * factor : offset_at(off, wide, lo, total) * factor;
-  const int first = start + (b - (start / size + lo)) * size;
+  const int first = start + max(b - (start / size + lo), 0) * size;
   return make_int2(min(first, end), min(first + size, end));
 }
 
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ Params
   else row_dkv<T>(p, r, h);
 }
 
-// What the gradients need of each query: its interval (the first CTAs, a thread a query), delta_i = dout_i . out_i, and in
+// What the gradients need: each query's interval and the lists of tiles (the first CTAs), delta_i = dout_i . out_i, and in
 // fp16 the largest norms of a row of dout and of v (those that are finite), as bits of positive floats, which order as
 // numbers do.  LANES lanes take a row of one head by 16 bytes each (32, value by value, where rows do not allow that).
 constexpr int kDeltaCtas = 8;  // an SM, at most: every CTA ends with an atomic maximum to the same two words
@@ -326,15 +328,59 @@ __device__ __forceinline__ float2 lanes_sum(float2 s) {
   }
   return s;
 }
+// a warp a tile: the rows of tile b of the queries and the keys that any of them sees
+__device__ __forceinline__ void list_queries(const Params& p, int b) {
+  const int lane = threadIdx.x & 31;
+  const int2 span = tile_rows(p.q_off, p.off64, p.S, p.Tq, b, p.by_segment);
+  int lo = INT_MAX, hi = 0;
+  for (int r = span.x + lane; r < span.y; r += 32) {
+    const int4 row = row_of(p, r);
+    if (row.y > row.x) {
+      lo = min(lo, row.x);
+      hi = max(hi, row.y);
+    }
+  }
+  lo = __reduce_min_sync(kAll, lo);
+  hi = __reduce_max_sync(kAll, hi);
+  if (lane == 0) p.tiles[b] = make_int4(span.x, span.y, lo, hi);
+}
+// and of tile b of the keys, with the queries of the segments from the first key's to the last key's (in causal order,
+// from the first that sees the first key)
+__device__ __forceinline__ void list_keys(const Params& p, int b) {
+  const int2 span = tile_rows(p.k_off, p.off64, p.S, p.Tk, b, p.keys_by_segment);
+  if ((threadIdx.x & 31) != 0) return;
+  int lo = INT_MAX, hi = 0;
+  if (span.y > span.x) {
+    const int sa = max(segment_of(p.k_off, p.off64, p.S, p.Tk, span.x), 0), sb = segment_of(p.k_off, p.off64, p.S, p.Tk, span.y - 1);
+    if (sb >= 0) {
+      const int q0 = offset_at(p.q_off, p.off64, sa, p.Tq), k0 = offset_at(p.k_off, p.off64, sa, p.Tk);
+      const int n = max(0, offset_at(p.q_off, p.off64, sa + 1, p.Tq) - q0), m = max(0, offset_at(p.k_off, p.off64, sa + 1, p.Tk) - k0);
+      lo = q0;
+      hi = offset_at(p.q_off, p.off64, sb + 1, p.Tq);
+      if (p.causal) {
+        const int seen = p.prefix != nullptr ? (int)min(max(entry(p.prefix, p.off64, sa), (int64_t)0), (int64_t)m) : 0;
+        if (span.x - k0 >= seen) lo = q0 + min(max(span.x - k0 - m + n, 0), n);
+      }
+    }
+  }
+  p.key_tiles[b] = make_int4(span.x, span.y, lo, hi);
+}
+
 template <typename T, int LANES, bool VEC>
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Params p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr bool kPeaks = std::is_same<T, __half>::value;
   __shared__ uint32_t s_peak[2];
-  const int row_ctas = (p.Tq + 255) / 256;
-  if ((int)blockIdx.x < row_ctas) {
+  const int list_ctas = (p.Tq + 255) / 256, row_ctas = list_ctas + (p.n_tiles + p.n_key_tiles + 7) / 8;
+  if ((int)blockIdx.x < list_ctas) {
     const int r = blockIdx.x * 256 + threadIdx.x;
     if (r < p.Tq) p.rows[r] = row_of(p, r);
+    return;
+  }
+  if ((int)blockIdx.x < row_ctas) {
+    const int b = (blockIdx.x - list_ctas) * 8 + (threadIdx.x >> 5);
+    if (b < p.n_tiles) list_queries(p, b);
+    else if (b < p.n_tiles + p.n_key_tiles) list_keys(p, b - p.n_tiles);
     return;
   }
   if (kPeaks && threadIdx.x < 2) s_peak[threadIdx.x] = 0;
@@ -428,19 +474,23 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Para
 // ------------------------------------------------------- tensor-core helpers
 constexpr int kBlock = 64;    // of the other side that a step takes
 
-// A wait for others of the CTA, for at most 2^27 tries (seconds).  Short code on purpose: a wait stands between any two
-// pieces of work here, and fetching instructions is among what these kernels lose most to.
-__device__ __noinline__ bool given_up(uint32_t tries, int code, volatile int* abort_flag) {
-  if (abort_flag != nullptr && *abort_flag) return true;
-  if (tries < 1u << 27) return false;
+// A wait for others of the CTA, with mbar_wait_bounded's budget, in as little code as will do: a wait stands between any
+// two pieces of work here.  A try may sleep for up to a millisecond; the clock is read once in 64.
+constexpr uint64_t kGivenUp = ~0ull;
+__device__ __noinline__ uint64_t later(uint64_t since, int code, volatile int* abort_flag) {
+  if (abort_flag != nullptr && *abort_flag) return kGivenUp;
+  const uint64_t now = global_ns();
+  if (since == 0) return now;
+  if (now - since < kWaitBudgetNs) return since;
   raise_device_error(code);
   if (abort_flag != nullptr) *abort_flag = 1;
-  return true;
+  return kGivenUp;
 }
 __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, int code, volatile int* abort_flag) {
   const uint32_t at = smem_u32(bar);
   uint32_t tries = 0, done;
-  while (true) {  // a try may sleep for up to a millisecond
+  uint64_t since = 0;
+  while (true) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
@@ -449,9 +499,10 @@ __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, int code
         : "r"(at), "r"(parity & 1u), "r"(1000000u)
         : "memory");
     if (done) return true;
-    if ((++tries & 0xfffu) == 0 && given_up(tries, code, abort_flag)) return false;
+    if ((++tries & 63u) == 0 && (since = later(since, code, abort_flag)) == kGivenUp) return false;
   }
 }
+
 // one arrival for a warp, whose lanes have all come here
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   __syncwarp();
@@ -1388,7 +1439,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   uint8_t* sB2 = sB1 + C::kStages * C::kBBytes;
   __shared__ __align__(8) uint64_t afull, bfull[C::kStages], sfull, sfree, ready, done, drained[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word, s_lo[4], s_hi[4], s_bad[kTile];
+  __shared__ int abort_word, s_bad[kTile];
   // of the block's queries (KEYS), for this block and the next: lse and delta (negative), interval and place; and, of its
   // halves, what all of them see together
   __shared__ __align__(16) float s_lse[2][KEYS ? kBlock : 4], s_delta[2][KEYS ? kBlock : 4];
@@ -1398,7 +1449,9 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // (KEYS) blockIdx.z: one of the heads that share the key head, where there are parts; else all of them
   const int head = blockIdx.y, heads = KEYS && p.parts ? 1 : p.G, first_head = head * p.G + (KEYS ? (int)blockIdx.z : 0);
-  const int tile = KEYS ? blockIdx.x : gridDim.x - 1 - blockIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 span = __ldg(KEYS ? p.key_tiles + blockIdx.x : p.tiles + (gridDim.x - 1 - blockIdx.x));  // (long ones first)
+  if (span.x >= span.y) return;
 
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&afull), 1);
@@ -1418,48 +1471,15 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int2 span = tile_rows(KEYS ? p.k_off : p.q_off, p.off64, p.S, KEYS ? p.Tk : p.Tq, tile, p.by_segment);
   const int quarter = warp & 3, set = (warp - 2) >> 2;
   const int r = span.x + quarter * 32 + lane;  // the thread's query or key
   int4 row = make_int4(0, 0, 0, 0);
-  if (KEYS) {
-    if (threadIdx.x == 64) {
-      int lo = INT_MAX, hi = 0;
-      if (span.y > span.x) {
-        // queries of the segments from the first key's to the last key's
-        const int sa = max(segment_of(p.k_off, p.off64, p.S, p.Tk, span.x), 0), sb = segment_of(p.k_off, p.off64, p.S, p.Tk, span.y - 1);
-        if (sb >= 0) {
-          const int q0 = offset_at(p.q_off, p.off64, sa, p.Tq), k0 = offset_at(p.k_off, p.off64, sa, p.Tk);
-          const int n = max(0, offset_at(p.q_off, p.off64, sa + 1, p.Tq) - q0), m = max(0, offset_at(p.k_off, p.off64, sa + 1, p.Tk) - k0);
-          lo = q0;
-          hi = offset_at(p.q_off, p.off64, sb + 1, p.Tq);
-          if (p.causal) {
-            const int seen = p.prefix != nullptr ? (int)min(max(entry(p.prefix, p.off64, sa), (int64_t)0), (int64_t)m) : 0;
-            if (span.x - k0 >= seen) lo = q0 + min(max(span.x - k0 - m + n, 0), n);  // the first that sees the first key
-          }
-        }
-      }
-      s_lo[0] = s_lo[1] = s_lo[2] = s_lo[3] = lo;
-      s_hi[0] = s_hi[1] = s_hi[2] = s_hi[3] = hi;
-    }
-  } else if (warp >= 2 && warp < 6) {
-    if (r < span.y) row = __ldg(p.rows + r);
-    int lo = row.y > row.x ? row.x : INT_MAX, hi = row.y > row.x ? row.y : 0;
-    lo = __reduce_min_sync(kAll, lo);
-    hi = __reduce_max_sync(kAll, hi);
-    if (lane == 0) {
-      s_lo[quarter] = lo;
-      s_hi[quarter] = hi;
-    }
-  } else if (warp >= 6) {
-    if (r < span.y) row = __ldg(p.rows + r);
-  }
+  if (!KEYS && warp >= 2 && r < span.y) row = __ldg(p.rows + r);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int other0 = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), other1 = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+  const int other0 = span.z, other1 = span.w;
   const int each = other1 > other0 ? (other1 - other0 + kBlock - 1) / kBlock : 0;  // blocks of a head
   const int blocks = KEYS ? each * heads : each;
   const int up = std::is_same<T, __half>::value ? 15 : 0;
@@ -1698,7 +1718,8 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
     const float down = up != 0 ? 0x1p-15f : 1.0f, w1 = p.scale * down / sigma;
     const int64_t at = ((int64_t)r * (KEYS ? p.Hk : p.H) + head) * p.D;
     const bool mine_too = KEYS || row.y > row.x, there = r < span.y;
-    for (int pass = 0; pass < 2 && ok; ++pass) {
+    if (ok) {
+      bool bad = false;
       for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
         T* out = static_cast<T*>(which ? p.dv : KEYS ? p.dk : p.dq);
         const bool wide = p.D % 16 == 0 && aligned(out, 32);
@@ -1714,24 +1735,24 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0u;
           }
-          if (pass == 0) {
-            if (there && !finite32(o)) s_bad[quarter * 32 + lane] = 1;
-          } else if (KEYS && p.parts) {  // (whatever they are: their sum is looked at)
+          if (KEYS && p.parts) {  // (whatever they are: their sum is looked at)
             float* to = p.part + ((int64_t)(which * p.G + blockIdx.z) * p.Tk * p.Hk * p.D) + at + c;
             if (there)
 #pragma unroll
               for (int i = 0; i < 32; i += 4)
                 if (c + i < p.D)
                   *reinterpret_cast<float4*>(to + i) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-          } else if (there && !s_bad[quarter * 32 + lane]) {
+          } else if (there) {
+            bad = bad || !finite32(o);
             store_sums<T>(out + at + c, o, p.D - c, which ? down : w1, wide);
           }
         }
       }
-      if (pass == 0) meet(true);
+      if (bad) s_bad[quarter * 32 + lane] = 1;
+      meet(true);  // (all have stored)
     }
     if (ok && set == 0) {
-      uint32_t again = __ballot_sync(kAll, there && s_bad[quarter * 32 + lane] && !(KEYS && p.parts));
+      uint32_t again = __ballot_sync(kAll, there && s_bad[quarter * 32 + lane]);
       while (again != 0) {
         const int i = __ffs(again) - 1;
         again &= again - 1;
@@ -1927,9 +1948,7 @@ static int run_backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   if ((rc = make_map(&g, p.g, p.D, p.H, p.Tq, p.g_t, p.g_h, q_rows, dt))) return rc;
   if ((rc = make_map(&k, p.k, p.D, p.Hk, p.Tk, p.k_t, p.k_h, k_rows, dt))) return rc;
   if ((rc = make_map(&v, p.v, p.D, p.Hk, p.Tk, p.v_t, p.v_h, k_rows, dt))) return rc;
-  const int64_t total = KEYS ? p.Tk : p.Tq;
-  p.by_segment = KEYS ? choose_by_segment(p.Tk, p.Tq, p.S) : choose_by_segment(p.Tq, p.Tk, p.S);
-  const int64_t tiles = p.by_segment ? total / kTile + p.S + 2 : (total + kTile - 1) / kTile;
+  const int tiles = KEYS ? p.n_key_tiles : p.n_tiles;
   void* args[] = {KEYS ? &k : &q, KEYS ? &v : &g, KEYS ? &q : &k, KEYS ? &g : &v, &p};
   if ((rc = launch(backward_kernel<T, DP, KEYS>, dim3((unsigned)tiles, KEYS ? p.Hk : p.H, KEYS && p.parts ? p.G : 1), C::kThreads, C::kSmem,
                    true, st, "attention backward_kernel launch", args)))
@@ -1944,19 +1963,26 @@ static int backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   int rc;
   const bool peaks = std::is_same<T, __half>::value;
   if (peaks && (rc = check_cuda(cudaMemsetAsync(p.peaks, 0, 8, st), "attention peaks"))) return rc;
+  const bool tiles = tiled(p) && p.Tq > 0 && p.Tk > 0 && mappable(p.g, p.Tq, p.H, p.g_t, p.g_h) && aligned(p.dq, 16) &&
+                     aligned(p.dk, 16) && aligned(p.dv, 16);
+  if (tiles) {
+    p.by_segment = choose_by_segment(p.Tq, p.Tk, p.S);
+    p.keys_by_segment = choose_by_segment(p.Tk, p.Tq, p.S);
+    p.n_tiles = tiles_of(p.Tq, p.S, p.by_segment);
+    p.n_key_tiles = tiles_of(p.Tk, p.S, p.keys_by_segment);
+    p.key_tiles = p.tiles + p.n_tiles;
+  }
   const int64_t heads = (int64_t)p.Tq * p.H + (peaks ? (int64_t)p.Tk * p.Hk : 0);
   if (heads > 0) {
     const bool vec = p.D % 8 == 0 && aligned(p.o, 16) && mappable(p.g, p.Tq, p.H, p.g_t, p.g_h) && mappable(p.v, p.Tk, p.Hk, p.v_t, p.v_h);
     const int lanes = !vec || p.D > 128 ? 32 : p.D > 64 ? 16 : 8;
-    const unsigned grid = (unsigned)((p.Tq + 255) / 256 + std::min<int64_t>((heads * lanes + 255) / 256, (int64_t)sm_count() * kDeltaCtas));
+    const unsigned grid = (unsigned)((p.Tq + 255) / 256 + (p.n_tiles + p.n_key_tiles + 7) / 8 + std::min<int64_t>((heads * lanes + 255) / 256, (int64_t)sm_count() * kDeltaCtas));
     if (!vec) delta_kernel<T, 32, false><<<grid, 256, 0, st>>>(p);
     else if (lanes == 32) delta_kernel<T, 32, true><<<grid, 256, 0, st>>>(p);
     else if (lanes == 16) delta_kernel<T, 16, true><<<grid, 256, 0, st>>>(p);
     else delta_kernel<T, 8, true><<<grid, 256, 0, st>>>(p);
     if ((rc = check_cuda(cudaGetLastError(), "attention delta_kernel launch"))) return rc;
   }
-  const bool tiles = tiled(p) && p.Tq > 0 && p.Tk > 0 && mappable(p.g, p.Tq, p.H, p.g_t, p.g_h) && aligned(p.dq, 16) &&
-                     aligned(p.dk, 16) && aligned(p.dv, 16);
   if (tiles) {
     p.parts = key_parts(p.Tk, p.H, p.Hk);
     if ((rc = p.D <= 64 ? run_backward<T, 64, true>(p, dt, st) : run_backward<T, 128, true>(p, dt, st))) return rc;
@@ -2052,7 +2078,8 @@ extern "C" int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, con
 extern "C" int64_t rb_segment_attention_backward_workspace_size(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D) {
   if (Tq < 0 || Tk < 0 || S < 0 || H <= 0 || Hk <= 0 || D <= 0 || Tq > 1 << 30) return -1;
   const int64_t parts = H % Hk == 0 && D % 8 == 0 && D <= 128 && attn::key_parts(Tk, H, Hk) ? (int64_t)2 * H * Tk * D * 4 : 0;
-  return 16 + Tq * 16 + ((int64_t)H * Tq * 4 + 15) / 16 * 16 + parts;
+  const int64_t lists = (Tq + Tq / attn::kTile + Tk / attn::kTile + 2 * S + 4) * 16;
+  return 16 + lists + ((int64_t)H * Tq * 4 + 15) / 16 * 16 + parts;
 }
 
 extern "C" int rb_segment_attention_backward(const void* grad, int64_t g_t, int64_t g_h, const void* q, int64_t q_t, int64_t q_h,
@@ -2089,7 +2116,8 @@ extern "C" int rb_segment_attention_backward(const void* grad, int64_t g_t, int6
   p.dv = dv;
   p.peaks = static_cast<uint32_t*>(workspace);
   p.rows = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + 16);
-  p.delta = reinterpret_cast<float*>(p.rows + Tq);
+  p.tiles = p.rows + Tq;
+  p.delta = reinterpret_cast<float*>(p.tiles + (Tq / kTile + Tk / kTile + 2 * S + 4));
   p.part = p.delta + ((int64_t)H * Tq + 3) / 4 * 4;
   p.q_off = q_offsets;
   p.k_off = k_offsets;

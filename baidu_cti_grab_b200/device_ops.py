@@ -849,8 +849,8 @@ def _attention_args(name, q, k, v, offsets, k_offsets, causal, prefix, slopes, c
     dtype = q.dtype
     if dtype not in _HALVES or k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError("q, k and v must all be bf16 or all f16")
-    if k.shape[2] != D or Hk == 0 or H % Hk:
-        raise ValueError(f"k and v must be [Tk, Hk, {D}] with Hk a divisor of {H}")
+    if k.shape[2] != D or D == 0 or H == 0 or Hk == 0 or H % Hk:
+        raise ValueError(f"k and v must be [Tk, Hk, {D}] with Hk a divisor of {H}, and no dimension of a head empty")
     if k_offsets is None:
         if Tq != Tk:
             raise ValueError("without k_offsets there must be as many keys as queries")

@@ -163,6 +163,8 @@ CASES = [
     ([4] * 70, None, 8, 2, 32, BF, {}),
     ([1] * 300, [3] * 300, 2, 2, 40, HF, {}),
     ([2] * 9, [700, 1, 64, 65, 900, 0, 128, 63, 300], 8, 2, 128, BF, {}),
+    ([60, 40], None, 4, 2, 64, BF, {}),                             # fewer keys than a tile: heads that share them in one CTA
+    ([60, 40], None, 6, 2, 128, HF, dict(prefix=[50, 0])),
     ([17, 16, 1], [1500, 40, 2000], 16, 1, 64, HF, dict(causal=False, slopes=True)),
     ([1, 1, 1], [5000, 1, 3001], 6, 2, 128, BF, dict(cap=15.0, slopes=True)),
     ([1000, 37], None, 1, 1, 16, BF, dict(scale=0.9)),
@@ -246,6 +248,48 @@ def test_what_is_not_seen_stays_out(cuda_device, D, bad):
     assert all(bool(t.isfinite().all()) for t in grads)
     torch.cuda.synchronize()
     assert device_ops.device_error() == 0
+
+
+@pytest.mark.parametrize("splits", [1, 4])
+def test_what_few_queries_do_not_see_stays_out(cuda_device, splits):
+    """The same where few queries meet many keys: another segment's NaN, and the keys behind a query's own."""
+    from baidu_cti_grab_b200 import device_ops
+
+    nq, nk = [2, 1, 2], [300 * splits, 70, 299 * splits]
+    q, k, v, _ = _inputs(nq, nk, 4, 2, 128, BF, 13, cuda_device, 5)
+    off, k_off = _offsets(nq, torch.int32, cuda_device, 5), _offsets(nk, torch.int32, cuda_device, 5)
+    val, tol = oracle(q, k, v, nq, nk, 5, 5, half=2.0 ** -8)
+    out, lse = device_ops.segment_attention(q, k, v, off, k_off, want_lse=True)
+    _close(out, val["out"], tol["out"], BF)
+    _close(lse, val["lse"], tol["lse"], torch.float32)
+    for t in (k, v):
+        t[:5] = math.nan
+        t[5 + nk[0]:5 + nk[0] + nk[1]] = math.inf
+        t[5 + sum(nk) - 1:] = math.nan  # the last key of the third segment: only its last query sees it
+    q[:5] = math.nan
+    out, _ = device_ops.segment_attention(q, k, v, off, k_off)
+    clean = torch.tensor([5, 6, 8], device=cuda_device)
+    _close(out[clean], val["out"][clean], tol["out"][clean], BF)
+    assert torch.equal(out[:5], torch.zeros_like(out[:5])) and torch.equal(out[10:], torch.zeros_like(out[10:]))
+
+
+def test_no_segments_and_no_keys(cuda_device):
+    """No segment at all, segments without keys, no query: zeros, and shapes."""
+    from baidu_cti_grab_b200 import device_ops
+
+    q, k, v, g = _inputs([40], [70], 2, 1, 64, BF, 3, cuda_device)
+    none = torch.zeros(1, dtype=torch.int64, device=cuda_device)
+    for off, k_off, keys in ((none, none, 70), (torch.tensor([0, 40], device=cuda_device), torch.tensor([0, 0], device=cuda_device), 70),
+                             (torch.tensor([0, 40], device=cuda_device), torch.tensor([0, 0], device=cuda_device), 0)):
+        out, lse = device_ops.segment_attention(q, k[:keys], v[:keys], off, k_off, want_lse=True)
+        assert not out.any() and bool(torch.isneginf(lse).all())
+        grads = device_ops.segment_attention_backward(g, q, k[:keys], v[:keys], out, lse, off, k_off)
+        assert not any(bool(t.any()) for t in grads)
+    off = torch.zeros(2, dtype=torch.int64, device=cuda_device)
+    out, lse = device_ops.segment_attention(q[:0], k, v, off, torch.tensor([0, 70], device=cuda_device), want_lse=True)
+    assert out.shape == (0, 2, 64) and lse.shape == (2, 0)
+    dq, dk, dv = device_ops.segment_attention_backward(g[:0], q[:0], k, v, out, lse, off, torch.tensor([0, 70], device=cuda_device))
+    assert dq.shape == (0, 2, 64) and not dk.any() and not dv.any()
 
 
 def test_gradients_of_any_size_in_fp16(cuda_device):
