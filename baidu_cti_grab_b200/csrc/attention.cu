@@ -1393,9 +1393,12 @@ __global__ void __launch_bounds__(256) few_join_kernel(const __grid_constant__ P
 //
 //   S = A1 B1^T   dP = A2 B2^T   p = exp(s - lse)   e = p (dP - delta) (1 - tanh^2)   acc += e B1   [dv += p B2]
 //
-// seven products for both where one kernel that adds dq by atomics has five.  e and p go to the second products as
-// 16-bit values out of TMEM.  In fp16 they are brought into the type's range first: p by 2^15, e by that and the power
-// of two that keeps |dP - delta| under 1 (from the largest norms of a row of dO and of V).
+// seven products for both where one kernel that adds dq by atomics has five.  p goes to the second products as 16-bit
+// values out of TMEM, e as two of them: what it is rounded to, and what is left, rounded.  (With the first alone dq and dk
+// are 1.3 to 1.4 times as far from the exact sums, 2.4e-3 for 1.7e-3 in bf16; the products of the second are hidden behind
+// the rows' arithmetic: 1501 and 1564 us with and without for two long documents.)  In fp16 they are brought into the
+// type's range first: p by 2^15, e by that and the power of two that keeps |dP - delta| under 1 (from the largest norms of
+// a row of dO and of V).
 template <int DP, bool KEYS>
 struct Backward {
   static constexpr int kChunks = DP / 64;
@@ -1413,8 +1416,9 @@ struct Backward {
   static constexpr int kAccAt = 128, kAcc2At = 128 + DP;
   static constexpr bool kApart = !(DP == 64 && KEYS);
   static constexpr int kEAt = !kApart ? 64 : KEYS ? kAcc2At + DP : kAcc2At;
-  static constexpr int kPAt = kApart ? kEAt + 32 : 0;     // (KEYS)
-  static constexpr int kStride = kApart ? 8 : 16;         // from sixteen values to the next: in place, at their own columns
+  static constexpr int kPAt = kApart ? kEAt + 64 : 0;     // (KEYS)
+  static constexpr int kStride = kApart ? 8 : 16;         // from sixteen of p to the next: in place, at their own columns
+  static constexpr int kEStride = 16;                     // sixteen of e as they are rounded, then what is left of them
   static constexpr int kTmemCols = DP == 64 ? 256 : 512;
 };
 
@@ -1557,7 +1561,8 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
 #pragma unroll
         for (int i = 0; i < kBlock / 16; ++i) {
           if (KEYS) mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + C::kStride * i, b2 + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
-          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kStride * i, b1 + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
+          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kEStride * i, b1 + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
+          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kEStride * i + 8, b1 + i * (16 * 128 / 16), idesc, true);
         }
         tc::umma_commit(smem_u32(&done));
         held.next();
@@ -1620,7 +1625,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
         const int c0 = (set * C::kSteps + step) * C::kPart;
         // of these keys (queries) and the warp's rows: is there one that sees, do all
         const Seen seen = KEYS ? s_span[n & 1][c0 / kHalf].of(span.x + quarter * 32) : reach.of(o0 + c0, C::kPart);
-        uint32_t w[C::kPart / 2], e[C::kPart / 2];
+        uint32_t w[C::kPart / 2], e[C::kPart];
         if (seen != kNone) {
           uint32_t x[C::kPart], y[C::kPart];
           tmem_get16(mine + c0, x);
@@ -1678,12 +1683,15 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
             const float2 v = un(fma2(f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), f2(left, left), l));
             const float a = exp2_fast(v.x), b = exp2_fast(v.y);
             if (KEYS) w[c / 2] = pack2<T>(a, b);
-            const float2 g = un(mul2(f2(a, b), pair(y + c)));
-            e[c / 2] = pack2<T>(g.x, g.y);
+            const F2 g = mul2(f2(a, b), pair(y + c));
+            const float2 whole = un(g);
+            e[c / 2] = pack2<T>(whole.x, whole.y);
+            const float2 top = widen2<T>(e[c / 2]), rest = un(sub2(g, f2(top.x, top.y)));
+            e[C::kPart / 2 + c / 2] = pack2<T>(rest.x, rest.y);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < C::kPart / 2; ++c) w[c] = e[c] = 0u;
+          for (int c = 0; c < C::kPart / 2; ++c) w[c] = e[c] = e[C::kPart / 2 + c] = 0u;
           if (C::kApart && step == C::kSteps - 1) {
             tc::tc_fence_before();
             warp_arrive(&sfree);
@@ -1695,7 +1703,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
         }
         if (ok) {
           if (KEYS) tmem_put8(mine + C::kPAt + c0 / C::kPart * C::kStride, w);
-          tmem_put8(mine + C::kEAt + c0 / C::kPart * C::kStride, e);
+          tmem_put16(mine + C::kEAt + c0 / C::kPart * C::kEStride, e);
         }
       }
       if (ok) {
