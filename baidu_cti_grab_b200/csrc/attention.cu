@@ -13,7 +13,7 @@
 // (dk, dv: summed over the query heads that share the key head).
 //
 // What every kernel uses: the mask of a row is ONE interval [lo, hi) of the packed keys, whatever mixes into it
-// (segments, causal order, prefix).  rows_kernel computes it once a call for all heads, so that tiles need not follow
+// (segments, causal order, prefix).  plan_kernel (delta_kernel for the gradients) computes it once a call for all heads, so that tiles need not follow
 // segments: a tile is 128 rows of the packed order, its keys are the union of its rows' intervals, and a block of keys
 // that all rows see is not masked at all.
 #include "common.cuh"
@@ -706,7 +706,7 @@ __device__ __forceinline__ void transform(const Params& p, uint32_t* raw, float 
 // A row's thread goes over the block's scores in TMEM twice, 32 at a time: the maximum (scores that are masked or capped
 // or fall with distance are put back in their place), then the weights, which go back as 16-bit values for the second
 // product.  The running sum is fp32; the accumulator is rescaled only when a maximum has grown by more than 2^8 over
-// what it is scaled to.  Rounding a weight to the type is half a step of its own value (2^-9 bf16, 2^-12 fp16),
+// what it is scaled to.  Rounding a weight to the type is half a step of its own value (2^-8 bf16, 2^-11 fp16),
 // independent from key to key.
 template <int DP>
 struct Forward {
@@ -1848,14 +1848,16 @@ static int launch(K kernel, dim3 grid, int threads, int smem, bool after, cudaSt
   return check_cuda(cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), args), what);
 }
 
-// Tiles by the packed order or by segment: which has fewer blocks of scores, were all segments alike.  By segment, every
-// segment has its own (partly empty) tiles; by the packed order a tile's rows see keys of several segments.
-static bool choose_by_segment(int64_t Tq, int64_t Tk, int64_t S) {
+// Tiles by the packed order or by segment: which takes less time, were all segments alike.  By segment, every segment has
+// its own (partly empty) tiles; by the packed order a tile's rows see keys of several segments.  A tile costs about two
+// blocks besides its own, fewer tiles than the GPU holds at once take as long as those, and the last are half alone.  Eight heads of 64, us packed |
+// by segment: 2048 users of 40: 81 | 105 (gradients 396 | 788), 700 of 128: 71 | 77, 512 of mean 200, uneven: 140 | 134,
+// 128 of mean 700, uneven: 248 | 243, 512 single queries over 16 keys each: 64 | 30, 512 times 30 over 256: 116 | 77.
+static bool choose_by_segment(int64_t Tq, int64_t Tk, int64_t S, int heads) {
   if (S <= 0) return false;
-  const double nq = (double)Tq / S, nk = (double)Tk / S;
-  const double own = S * (nq / kTile + 0.5) * (nk / kBlock + 0.5 + 2.0);  // a tile costs about two blocks besides its own
-  const double packed = ((double)Tq / kTile + 0.5) * (nk * (1.0 + kTile / std::max(nq, 1.0)) / kBlock + 0.5 + 2.0);
-  return own < packed;
+  const double nq = (double)Tq / S, nk = (double)Tk / S, wave = 4.0 * sm_count();
+  auto time = [&](double tiles, double keys) { return (std::max(tiles * heads, wave) + wave / 2) * (keys / kBlock + 0.5 + 2.0); };
+  return time(S * std::max(nq / kTile + 0.5, 1.0), nk) < time((double)Tq / kTile + 0.5, nk * (1.0 + kTile / std::max(nq, 1.0)));
 }
 
 static int tiles_of(int64_t T, int64_t S, bool by_segment) { return (int)(by_segment ? T / kTile + S + 2 : (T + kTile - 1) / kTile); }
@@ -1881,12 +1883,22 @@ static int run_forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
 }
 
 // How many parts the keys of a segment are split into where there are few queries, 0: not that kernel.  It reads a key
-// head's keys once for 16 rows; the tiles read them once for 128, but fill 128 rows with what there is.
+// head's keys for 16 rows, each query's heads among them; the tiles read them for 128 rows of one head, most of them empty.
+// So 16 rows cost 0.7 of a tile and half a tile for each segment, while fewer tiles than five an SM take as long as those
+// (64 segments of 4000 keys, tiles | this, us: 1 query of 8 heads over 8, 244 | 126; over 1, 240 | 38; 16 over 1, 239 |
+// 110; 64 over 8, 234 | 332; 512 segments of 1000 keys: 1 over 8, 225 | 250, 8 over 1, 225 | 101).
+// Parts fill the GPU once (of 256 keys or more); where it holds fewer than three of each, segments of different lengths
+// are evened out by up to eight CTAs an SM, of 1024 keys or more (64 histories of 1000 to 16000 keys, 16 heads over 4: one
+// wave 236, eight CTAs an SM 208, sixteen 208; 64 times 4 queries over 4000 keys, 8 heads over 2: 66, 68 and 105).
 static int splits_of(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D) {
-  const int64_t G = H / Hk;
-  if (S <= 0 || D % 8 != 0 || D > 128 || Tk < 4 * Tq || Tq * G > 32 * S || Tq * G > 1 << 30) return 0;
-  const int64_t ctas = std::max<int64_t>(1, S * ((Tq * G / S + 15) / 16) * Hk), want = (int64_t)sm_count() * 16;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(want + ctas - 1) / ctas, Tk / S / 256, 64}));
+  const int64_t G = H / Hk, sm = sm_count();
+  if (S <= 0 || D % 8 != 0 || D > 128 || Tk < 4 * Tq || Tq * G > 1 << 30) return 0;
+  if (7 * Hk * (Tq * G / 16 + S) + 5 * Hk * S >= 10 * std::max<int64_t>(H * (Tq / kTile + S), 5 * sm)) return 0;
+  const int64_t ctas = S * ((Tq * G / S + 15) / 16) * Hk, keys = Tk / S;
+  if (ctas == 0) return 1;
+  const int64_t once = sm * (D > 64 ? Few<128>::kCtas : Few<64>::kCtas) / ctas;
+  const int64_t parts = once > 2 ? std::min(once, keys / 256) : std::max(std::min(once, keys / 256), std::min((8 * sm + ctas - 1) / ctas, keys / 1024));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(parts, 64));
 }
 
 template <typename T, int DP>
@@ -1921,7 +1933,7 @@ template <typename T>
 static int forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   int rc;
   const bool tiles = tiled(p) && p.Tk > 0 && aligned(p.out, 16);
-  p.by_segment = choose_by_segment(p.Tq, p.Tk, p.S);
+  p.by_segment = choose_by_segment(p.Tq, p.Tk, p.S, p.H);
   p.splits = tiles ? splits_of(p.Tq, p.Tk, p.S, p.H, p.Hk, p.D) : 0;
   p.n_tiles = tiles_of(p.Tq, p.S, p.by_segment);
   if (!tiles || p.splits > 0) p.tiles = nullptr;
@@ -1934,10 +1946,15 @@ static int forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
                 "attention row_kernel launch", args);
 }
 
-// Whether the query heads that share a key head go to CTAs of their own, whose sums are added up after: with fewer than
-// four tiles of keys an SM the last ones take too long by themselves (two documents of 6100 keys, two key heads for eight:
-// 194 tiles of up to 384 blocks, 749 us; 776 of 96).  Each part is written and read once, in 32 bits.
-static bool key_parts(int64_t Tk, int H, int Hk) { return H > Hk && H / Hk <= 64 && Tk >= kTile && Tk / kTile * Hk < 4 * (int64_t)sm_count(); }
+// Whether the query heads that share a key head go to CTAs of their own, whose sums are added up after (each part is
+// written and read once, in 32 bits): with few tiles of keys an SM the longest take too long by themselves.  Eight heads
+// over two, both gradients, together | apart, us: 1 document of 6100 keys (0.6 tiles an SM) 703 | 479; 2 of them 855 | 832,
+// in heads of 64 values 1061 | 729; 8 of 3000 (2.5 tiles) 863 | 904; 64 users of 150 (1.0) 80 | 95; 16 of 300 (0.5) 72 | 70.
+static bool key_parts(int64_t Tk, int64_t S, int H, int Hk) {
+  if (H <= Hk || H / Hk > 64 || Tk < kTile) return false;
+  const int64_t tiles = Tk / kTile * Hk, sm = sm_count();
+  return 2 * tiles < sm || (tiles < 2 * sm && Tk >= 1024 * S);
+}
 
 template <typename T, int DP, bool KEYS>
 static int run_backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
@@ -1974,8 +1991,8 @@ static int backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   const bool tiles = tiled(p) && p.Tq > 0 && p.Tk > 0 && mappable(p.g, p.Tq, p.H, p.g_t, p.g_h) && aligned(p.dq, 16) &&
                      aligned(p.dk, 16) && aligned(p.dv, 16);
   if (tiles) {
-    p.by_segment = choose_by_segment(p.Tq, p.Tk, p.S);
-    p.keys_by_segment = choose_by_segment(p.Tk, p.Tq, p.S);
+    p.by_segment = choose_by_segment(p.Tq, p.Tk, p.S, p.H);
+    p.keys_by_segment = choose_by_segment(p.Tk, p.Tq, p.S, p.Hk);
     p.n_tiles = tiles_of(p.Tq, p.S, p.by_segment);
     p.n_key_tiles = tiles_of(p.Tk, p.S, p.keys_by_segment);
     p.key_tiles = p.tiles + p.n_tiles;
@@ -1992,7 +2009,7 @@ static int backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
     if ((rc = check_cuda(cudaGetLastError(), "attention delta_kernel launch"))) return rc;
   }
   if (tiles) {
-    p.parts = key_parts(p.Tk, p.H, p.Hk);
+    p.parts = key_parts(p.Tk, p.S, p.H, p.Hk);
     if ((rc = p.D <= 64 ? run_backward<T, 64, true>(p, dt, st) : run_backward<T, 128, true>(p, dt, st))) return rc;
     return p.D <= 64 ? run_backward<T, 64, false>(p, dt, st) : run_backward<T, 128, false>(p, dt, st);
   }
@@ -2085,7 +2102,7 @@ extern "C" int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, con
 
 extern "C" int64_t rb_segment_attention_backward_workspace_size(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D) {
   if (Tq < 0 || Tk < 0 || S < 0 || H <= 0 || Hk <= 0 || D <= 0 || Tq > 1 << 30) return -1;
-  const int64_t parts = H % Hk == 0 && D % 8 == 0 && D <= 128 && attn::key_parts(Tk, H, Hk) ? (int64_t)2 * H * Tk * D * 4 : 0;
+  const int64_t parts = H % Hk == 0 && D % 8 == 0 && D <= 128 && attn::key_parts(Tk, S, H, Hk) ? (int64_t)2 * H * Tk * D * 4 : 0;
   const int64_t lists = (Tq + Tq / attn::kTile + Tk / attn::kTile + 2 * S + 4) * 16;
   return 16 + lists + ((int64_t)H * Tq * 4 + 15) / 16 * 16 + parts;
 }

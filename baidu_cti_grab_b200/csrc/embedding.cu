@@ -30,7 +30,6 @@ struct Params {
   int64_t ld_table, ld_grad, ld_out, V, n, n_bags, padding;
   float scale;
   int D, wide_ids, out_dtype, accumulate, sparse;
-  int vec;                       // values of a thread's load (16 bytes), or 1
   // workspace
   int32_t *key[2], *row[2];      // ids and their rows of grad, before and after a pass
   int32_t* counts;               // of a pass: [tiles][256], or [256][tiles] scanned
@@ -46,7 +45,9 @@ __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 
 template <typename T, int VEC>
 struct Raw {  // VEC values as they lie in memory
-  typename std::conditional<VEC == 1, T, uint4>::type v;
+  static constexpr int kWords = VEC * (int)sizeof(T) / 4;
+  using Word = typename std::conditional<kWords <= 1, uint32_t, typename std::conditional<kWords == 2, uint2, uint4>::type>::type;
+  typename std::conditional<VEC == 1, T, Word>::type v;
   __device__ void load(const T* from) { v = __ldg(reinterpret_cast<const decltype(v)*>(from)); }
   __device__ void widen(float* f) const {
 #pragma unroll
@@ -57,9 +58,12 @@ struct Raw {  // VEC values as they lie in memory
     if constexpr (VEC == 1) {
       acc[0] += to_f32(v);
     } else {
-      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+      uint32_t u[kWords];
+      if constexpr (kWords == 1) u[0] = v;
+      else u[0] = v.x, u[1] = v.y;
+      if constexpr (kWords == 4) u[2] = v.z, u[3] = v.w;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kWords; ++i) {
         if constexpr (std::is_same<T, float>::value) {
           acc[i] += __uint_as_float(u[i]);
         } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
@@ -80,6 +84,8 @@ template <typename T2, int VEC>
 __device__ __forceinline__ void store_as(T2* p, const float* v) {
   if constexpr (VEC == 1) {
     p[0] = T2(v[0]);
+  } else if constexpr (std::is_same<T2, float>::value && VEC == 2) {
+    *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
   } else if constexpr (std::is_same<T2, float>::value) {
 #pragma unroll
     for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
@@ -90,7 +96,8 @@ __device__ __forceinline__ void store_as(T2* p, const float* v) {
       if constexpr (std::is_same<T2, __nv_bfloat16>::value) u[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
       else u[i] = pack_f16x2(v[2 * i], v[2 * i + 1]);
     }
-    if constexpr (VEC == 4) *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+    if constexpr (VEC == 2) *reinterpret_cast<uint32_t*>(p) = u[0];
+    else if constexpr (VEC == 4) *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
     else *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
   }
 }
@@ -164,7 +171,9 @@ __global__ void __launch_bounds__(256) lookup_kernel(const __grid_constant__ Par
 // (lanes with equal digits find each other by eight ballots), then warps and tiles are added up before it.
 constexpr int kSortThreads = 512, kPerThread = 4, kTile = kSortThreads * kPerThread, kSortWarps = kSortThreads / 32;
 constexpr int kDigits = 256;
-constexpr int kDirect = 64;  // up to so many tiles a CTA adds up the counts of those before it by itself
+// Up to so many tiles a CTA adds up the counts of those before it by itself, above that a kernel does it for all: 20,000
+// ids (10 tiles) 30 us and 35, 60,000 36 and 36, 100,000 40 and 38, 400,000 69 and 63.
+constexpr int kDirect = 32;
 
 // the last b in [0, n_bags] with bags[b] <= i, 0 where there is none: a warp, 32 probes at once
 __device__ __forceinline__ int64_t bag_of(const Params& p, int64_t i) {
@@ -410,7 +419,7 @@ __global__ void __launch_bounds__(kSortThreads, 3) scatter_kernel(const __grid_c
   }
 }
 
-// All passes of up to kSmall ids in one CTA, in shared memory.
+// All passes of up to kSmall ids in one CTA, in shared memory: a gradient takes 22 us, with a kernel a pass 30.
 constexpr int kSmallThreads = 1024, kSmallPer = 4, kSmall = kSmallThreads * kSmallPer;
 struct Small {
   int key[2][kSmall], row[2][kSmall];
@@ -562,12 +571,7 @@ __global__ void __launch_bounds__(kSumThreads) sums_kernel(const __grid_constant
   for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
   auto part = [&](int which) {
     float* to = p.part + ((int64_t)run * 2 + which) * p.D + c;
-    if constexpr (VEC == 1) {
-      to[0] = acc[0];
-    } else {
-#pragma unroll
-      for (int v = 0; v < VEC; v += 4) *reinterpret_cast<float4*>(to + v) = make_float4(acc[v], acc[v + 1], acc[v + 2], acc[v + 3]);
-    }
+    store_as<float, VEC>(to, acc);
   };
   auto finish = [&] {
     if (before) return part(0);
@@ -603,7 +607,7 @@ __global__ void __launch_bounds__(kSumThreads) sums_kernel(const __grid_constant
 
 // A warp for each run whose last row starts in it and goes on: the partial sums of that row, in their order.  Rows over
 // more than kNear runs are left to the CTA: teams take every so manyth partial sum, then the teams are added up.
-constexpr int kFar = 32, kNear = 12;
+constexpr int kFar = 32, kNear = 12;  // (3 to 31: the same within 6 %)
 template <int VEC>
 __global__ void __launch_bounds__(kSumThreads) combine_kernel(const __grid_constant__ Params p) {
   __shared__ float s_sum[kSumThreads * VEC];
@@ -694,11 +698,12 @@ static int bits_of(int64_t values) {
   while (b < 31 && ((int64_t)1 << b) < values) ++b;
   return b;
 }
-// Sorted ids of a team: enough teams to fill the GPU (32 of 64 threads an SM), runs as long as that leaves them, since
-// every run costs up to two partial sums.
+// Sorted ids of a team, 16 to 128: enough teams to fill the GPU (32 of 64 threads an SM), runs as long as that leaves
+// them, since every run costs up to two partial sums.  512 values a row, us for 16 | 32 | 64 | 128 | 256 ids: 20,000 ids 58 |
+// 63 | 71 | 92 | 134, 400,000 ids 194 | 172 | 163 | 178 | 171, 1.4 million 519 | 429 | 392 | 373 | 395.
 static int run_log_of(int64_t n) {
   int log = 4;
-  while (log < 8 && (n >> log) > (int64_t)sm_count() * 64) ++log;
+  while (log < 7 && (n >> log) > (int64_t)sm_count() * 64) ++log;
   return log;
 }
 struct Sizes {
@@ -716,10 +721,18 @@ static Sizes sizes_of(int64_t n, int D) {
   return z;
 }
 
-template <typename T>
-static int vec_of(const void* a, int64_t lda, const void* b, int64_t ldb, int b_size, int D) {
-  const int v = 16 / (int)sizeof(T);
-  return D % v == 0 && aligned(a, 16) && lda % v == 0 && aligned(b, 16) && ldb * b_size % 16 == 0 ? v : 1;
+// Values of a thread's load: 16 bytes, or 8 or 4 or one value where the width, the strides or the addresses are not whole
+// multiples of that; calls f with their number as a type.  60,000 rows of 1022 bf16 values, two a load: gradient 188 us,
+// lookup 56 (one a load 302 and 85); of 513, one a load, 171 and 42; of 512, eight a load, 77 and 21.
+template <typename T, typename F>
+static int with_vec(const void* a, int64_t lda, const void* b, int64_t ldb, int b_size, int D, const F& f) {
+  auto whole = [&](int v) {
+    return D % v == 0 && lda % v == 0 && ldb % v == 0 && aligned(a, v * (int)sizeof(T)) && aligned(b, std::min(v * b_size, 16));
+  };
+  if (whole(16 / (int)sizeof(T))) return f(std::integral_constant<int, 16 / (int)sizeof(T)>());
+  if (sizeof(T) == 2 && whole(4)) return f(std::integral_constant<int, 4>());
+  if (whole(2)) return f(std::integral_constant<int, 2>());
+  return f(std::integral_constant<int, 1>());
 }
 
 template <typename T, int VEC>
@@ -805,8 +818,8 @@ template <typename T>
 static int run_backward(Params& p, cudaStream_t st) {
   int rc;
   if ((rc = sort_ids(p, st))) return rc;
-  if (vec_of<T>(p.grad, p.ld_grad, p.out, p.ld_out, dtype_size(p.out_dtype), p.D) > 1) return run_sums<T, 16 / sizeof(T)>(p, st);
-  return run_sums<T, 1>(p, st);
+  return with_vec<T>(p.grad, p.ld_grad, p.out, p.ld_out, dtype_size(p.out_dtype), p.D,
+                     [&](auto v) { return run_sums<T, decltype(v)::value>(p, st); });
 }
 
 static int check_shape(int64_t V, int D, int64_t n, int idx_dtype, int dtype) {
@@ -889,8 +902,8 @@ static int backward(const void* grad, int dtype, int64_t ld_grad, int D, const v
 
 template <typename T>
 static int lookup(const Params& p, cudaStream_t st) {
-  if (vec_of<T>(p.table, p.ld_table, p.out, p.ld_out, sizeof(T), p.D) > 1) return run_lookup<T, 16 / sizeof(T)>(p, st);
-  return run_lookup<T, 1>(p, st);
+  return with_vec<T>(p.table, p.ld_table, p.out, p.ld_out, sizeof(T), p.D,
+                     [&](auto v) { return run_lookup<T, decltype(v)::value>(p, st); });
 }
 
 }  // namespace embed

@@ -471,7 +471,7 @@ int rb_segment_attention_backward(const void* grad, int64_t g_t, int64_t g_h, co
  * rb_embed_rows_backward_sparse writes the touched rows alone: their numbers, ascending,
  * to out_ids [n], the gradients to out_rows [n, ld_out], and how many to count; entries
  * behind are left as they were.  Sums are fp32, in the ids' order within runs of 16 to
- * 256 equal or neighbouring ids: the same bits every time.
+ * 128 equal or neighbouring ids: the same bits every time.
  */
 int rb_embed_rows(const void* table, int dtype, int64_t ld, int64_t V, int D, const void* ids, int idx_dtype,
                   int64_t n, float scale, void* out, int64_t ldo, void* stream);

@@ -180,6 +180,19 @@ def test_against_float64(cuda_device, nq, nk, H, Hk, D, dtype, mask):
     run(nq, nk, H, Hk, D, dtype, cuda_device, seed=len(nq) + D, **mask)
 
 
+@pytest.mark.parametrize("nq,nk,H,Hk,D,dtype", [
+    ([300], [3000], 1, 1, 64, BF),                  # many queries of few heads: 16 rows a CTA, keys in parts
+    ([33, 1, 20], [900, 2600, 4000], 8, 1, 64, HF),
+    ([31] * 12, [700, 3, 129, 400] * 3, 8, 2, 128, BF),
+    ([1] * 200, [16] * 200, 8, 8, 64, BF),          # tiles of single queries by segment
+    ([30] * 100, [130] * 100, 8, 8, 64, HF),        # tiles rather than 16 rows a CTA
+    ([700, 900], None, 8, 2, 64, HF),               # few tiles of keys: heads that share them apart
+    ([70] * 40, None, 8, 2, 64, BF),                # and together
+])
+def test_either_side_of_the_choices(cuda_device, nq, nk, H, Hk, D, dtype):
+    run(nq, nk, H, Hk, D, dtype, cuda_device, seed=len(nq) + H)
+
+
 @pytest.mark.parametrize("idx", [torch.int32, torch.int64])
 @pytest.mark.parametrize("D", [64, 128, 20])
 def test_rows_outside_every_segment(cuda_device, idx, D):

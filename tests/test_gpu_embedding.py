@@ -94,6 +94,29 @@ def test_against_float64(cuda_device, n, V, D, dtype):
     assert torch.equal(total[~touched], base[~touched])
 
 
+@pytest.mark.parametrize("D,step", [(46, 46), (100, 100), (100, 101), (48, 50), (770, 772), (1022, 1022)])
+@pytest.mark.parametrize("dtype", [F32, BF, HF])
+def test_widths_and_strides_of_fewer_bytes(cuda_device, D, step, dtype):
+    """Rows that are whole multiples of 8, 4 or 2 bytes only, by their width or their stride."""
+    from baidu_cti_grab_b200 import device_ops
+
+    gen = torch.Generator(device=cuda_device).manual_seed(D)
+    n, V = 3000, 500
+    table = torch.randn(V, step, device=cuda_device, generator=gen).to(dtype)[:, :D]
+    grad = torch.randn(n, step, device=cuda_device, generator=gen).to(dtype)[:, :D]
+    ids = _ids(n, V, D).to(cuda_device)
+    assert torch.equal(device_ops.embed_rows(table, ids), table[ids])
+    want, bound, touched = _oracle(grad, ids, V)
+    got = device_ops.embed_rows_backward(grad, ids, V)
+    _close(got, want, bound)
+    where, rows, count = device_ops.embed_rows_backward_sparse(grad, ids, V)
+    m = int(count)
+    assert torch.equal(rows[:m], got[where[:m]])
+    total = torch.ones(V, step, device=cuda_device)[:, :D]
+    device_ops.embed_rows_backward(grad, ids, V, out=total)
+    _close(total, want + 1.0, bound + U)
+
+
 def test_ids_outside_the_table_and_padding(cuda_device):
     """Ids are clamped in both directions; those of the padding row add nothing (clamped ones among them)."""
     from baidu_cti_grab_b200 import device_ops
