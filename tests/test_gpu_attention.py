@@ -14,6 +14,8 @@ Tolerance.  u = 2^-24, half = eps / 2 of the model type.
   of itself and p slant times these two (the slant 1 - tanh^2 by 8 u).  In fp16 an e below the type's normal range loses
   2^-25 of 2^15 / (2 max |g| max |v|), and p likewise 2^-25 of 2^15.
   dq, dk and dv are those errors times |k|, |q| and |g|, summed, plus n u for a sum of n terms, and half of themselves.
+* `near`: rows of few keys have delta as the sum of p dp, off by (eta + n u) of sum p |dp| and 2 D u of sum p |g| |v|; and e
+  is carried as two values of the type, off by half of half of itself, in fp16 by twice 2^-25.
 """
 
 import math
@@ -29,7 +31,7 @@ U = 2.0 ** -24
 
 
 def oracle(q, k, v, nq, nk, first=0, k_first=0, g=None, causal=True, prefix=None, slopes=None, cap=0.0, scale=None, half=0.0,
-           fp16=False):
+           fp16=False, near=False):
     """(values, bounds) by name in float64, from inputs of any type."""
     (Tq, H, D), (Tk, Hk, _) = q.shape, k.shape
     scale = D ** -0.5 if scale is None else scale
@@ -85,8 +87,10 @@ def oracle(q, k, v, nq, nk, first=0, k_first=0, g=None, causal=True, prefix=None
                 dp, delta = g1 @ V.t(), (g1 * o).sum(-1, keepdim=True)
                 e = p * (dp - delta) * slant
                 d_delta = (g1.abs() * tol["out"][a:a + n, h]).sum(-1, keepdim=True) + 2 * D * U * (g1 * o).abs().sum(-1, keepdim=True)
-                d_e = e.abs() * (half + eta + 16 * U) + p * (slant + 8 * U) * (d_delta + 2 * D * U * (g1.abs() @ V.abs().t()))
-                d_e = d_e + p * (dp - delta).abs() * 8 * U + (tiny * 2.0 ** -15 * peak + flushed * (dp - delta).abs()) * seen
+                if near:
+                    d_delta = (p * dp.abs()).sum(-1, keepdim=True) * (eta + m * U) + 2 * D * U * (p * (g1.abs() @ V.abs().t())).sum(-1, keepdim=True)
+                d_e = e.abs() * ((half * half if near else half) + eta + 16 * U) + p * (slant + 8 * U) * (d_delta + 2 * D * U * (g1.abs() @ V.abs().t()))
+                d_e = d_e + p * (dp - delta).abs() * 8 * U + ((2.0 if near else 1.0) * tiny * 2.0 ** -15 * peak + flushed * (dp - delta).abs()) * seen
                 d_p = p * (half + eta) + (tiny * 2.0 ** -15 + flushed) * seen
                 val["dq"][a:a + n, h] = scale * (e @ K)
                 tol["dq"][a:a + n, h] = scale * ((d_e + m * U * e.abs()) @ K.abs())
@@ -178,6 +182,28 @@ CASES = [
 @pytest.mark.parametrize("nq,nk,H,Hk,D,dtype,mask", CASES)
 def test_against_float64(cuda_device, nq, nk, H, Hk, D, dtype, mask):
     run(nq, nk, H, Hk, D, dtype, cuda_device, seed=len(nq) + D, **mask)
+
+
+@pytest.mark.parametrize("H,Hk,D,mask", [(2, 2, 64, {}), (4, 1, 128, dict(slopes=True)), (2, 1, 96, dict(cap=8.0)),
+                                         (1, 1, 20, {}), (2, 2, 200, dict(prefix=[3] * 72)), (3, 3, 32, dict(causal=False))])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_gradients_of_few_keys(cuda_device, dtype, H, Hk, D, mask):
+    """Where dp - delta is a small difference: dq and dk as near as their own rounding."""
+    from baidu_cti_grab_b200 import device_ops
+
+    nq = [4, 5, 0, 7, 8, 1, 2, 3] * 9
+    q, k, v, g = _inputs(nq, nq, H, Hk, D, dtype, D, cuda_device)
+    off = _offsets(nq, torch.int64, cuda_device)
+    how = dict(mask, slopes=torch.full((H,), 0.25, device=cuda_device) if mask.get("slopes") else None)
+    if "prefix" in mask:
+        how["prefix"] = torch.tensor(mask["prefix"], device=cuda_device)
+    out, lse = device_ops.segment_attention(q, k, v, off, want_lse=True, **how)
+    grads = device_ops.segment_attention_backward(g, q, k, v, out, lse, off, **how)
+    if "prefix" in mask:
+        how["prefix"] = mask["prefix"]
+    val, tol = oracle(q, k, v, nq, nq, g=g, half=torch.finfo(dtype).eps / 2, fp16=dtype is HF, near=True, **how)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        _close(got, val[name], tol[name], dtype)
 
 
 @pytest.mark.parametrize("nq,nk,H,Hk,D,dtype", [
