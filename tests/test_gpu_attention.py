@@ -210,6 +210,7 @@ def test_gradients_of_few_keys(cuda_device, dtype, H, Hk, D, mask):
     ([300], [3000], 1, 1, 64, BF),                  # many queries of few heads: 16 rows a CTA, keys in parts
     ([33, 1, 20], [900, 2600, 4000], 8, 1, 64, HF),
     ([31] * 12, [700, 3, 129, 400] * 3, 8, 2, 128, BF),
+    ([0, 0, 1, 0, 3] * 8, [900, 30, 700, 5, 2000] * 8, 8, 2, 64, HF),  # segments without queries among them
     ([1] * 200, [16] * 200, 8, 8, 64, BF),          # tiles of single queries by segment
     ([30] * 100, [130] * 100, 8, 8, 64, HF),        # tiles rather than 16 rows a CTA
     ([700, 900], None, 8, 2, 64, HF),               # few tiles of keys: heads that share them apart
