@@ -11,6 +11,8 @@
 // CTA of the second kernel adds all of them up in the same order.  A piece's squares are summed in fp32, each thread's
 // of at most 32 values; where such a sum is outside [2^-90, 2^120] (a square of a bf16 or fp32 value may be outside
 // fp32's range) it is taken again in fp64, and everything above it is fp64.
+//
+// 290 bf16 tensors of 166 MB together: norm 35 us (4.7 TB/s, what L2 held among it), scaling 56 (5.9 TB/s read and written).
 #include "common.cuh"
 
 #include <algorithm>
