@@ -628,8 +628,22 @@ __global__ void __launch_bounds__(kSumThreads) combine_kernel(const __grid_const
   };
   auto add = [&](int j, int from_run, int c, float* acc) {
     const float* from = p.part + ((int64_t)j * 2 + (j == from_run ? 1 : 0)) * p.D + c;
+    if constexpr (VEC == 1) {
+      acc[0] += from[0];
+    } else if constexpr (VEC == 2) {
+      const float2 f = *reinterpret_cast<const float2*>(from);
+      acc[0] += f.x;
+      acc[1] += f.y;
+    } else {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) acc[v] += from[v];
+      for (int v = 0; v < VEC; v += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(from + v);
+        acc[v] += f.x;
+        acc[v + 1] += f.y;
+        acc[v + 2] += f.z;
+        acc[v + 3] += f.w;
+      }
+    }
   };
   auto store = [&](int r, int key, int c, float* acc) {
     int64_t at = key;
