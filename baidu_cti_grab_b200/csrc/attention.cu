@@ -16,6 +16,9 @@
 // (segments, causal order, prefix).  plan_kernel (delta_kernel for the gradients) computes it once a call for all heads, so
 // that tiles need not follow segments: a tile is 128 rows of the packed order, its keys are the union of its rows'
 // intervals, and a block of keys that all rows see is not masked at all.
+//
+// The kernels of a call start under one another's tails.  What one of them writes (the workspace) the next reads by plain
+// loads behind its griddepcontrol.wait, never by __ldg, which asks for memory that nobody writes while the kernel lives.
 #include "common.cuh"
 
 #include <algorithm>
@@ -903,7 +906,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
         ahead.blocks = 0;
         a_block = 0;
         while (ticket < items && ahead.blocks == 0) {
-          const int4 t = __ldg(p.tiles + (p.n_tiles - 1 - ticket / p.H));
+          const int4 t = p.tiles[p.n_tiles - 1 - ticket / p.H];
           ahead = Item{t.x, t.y, (int)(ticket % p.H), t.z, t.w > t.z ? (t.w - t.z + kBlock - 1) / kBlock : 0};
           ticket = atomicAdd(p.next, 1u);  // (needed a tile later)
         }
@@ -1029,7 +1032,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
     bool ok = wait(&ifull[0], 0);
     Item it = s_item[0];
     int4 row = make_int4(0, 0, 0, 0);
-    if (ok && it.blocks > 0 && it.r0 + quarter * 32 + lane < it.r1) row = __ldg(p.rows + it.r0 + quarter * 32 + lane);
+    if (ok && it.blocks > 0 && it.r0 + quarter * 32 + lane < it.r1) row = p.rows[it.r0 + quarter * 32 + lane];
     int t = 0;  // block of all tiles
     for (int tile = 0; ok && it.blocks > 0; ++tile) {
       const int r = it.r0 + quarter * 32 + lane, h = it.head;
@@ -1144,7 +1147,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
       if (!ok) break;
       const Item next = s_item[(tile + 1) % kItems];
       int4 next_row = make_int4(0, 0, 0, 0);
-      if (next.blocks > 0 && next.r0 + quarter * 32 + lane < next.r1) next_row = __ldg(p.rows + next.r0 + quarter * 32 + lane);
+      if (next.blocks > 0 && next.r0 + quarter * 32 + lane < next.r1) next_row = p.rows[next.r0 + quarter * 32 + lane];
       ok = wait(&pvdone, t - 1);
       if (!ok) break;
       tc::tc_fence_after();
@@ -1264,7 +1267,7 @@ __global__ void __launch_bounds__(Few<DP>::kThreads, Few<DP>::kCtas)
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = span.x + g + 8 * i;
-    mine[i] = row < span.y ? __ldg(p.rows + row / p.G) : make_int4(0, 0, 0, 0);
+    mine[i] = row < span.y ? p.rows[row / p.G] : make_int4(0, 0, 0, 0);
   }
   const Span a = span_of(mine[0]), b = span_of(mine[1]);
   const int lo = min(a.lo_min, b.lo_min), hi = max(a.hi_max, b.hi_max);  // of all rows
@@ -1559,7 +1562,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   // (KEYS) blockIdx.z: one of the heads that share the key head, where there are parts; else all of them
   const int head = blockIdx.y, heads = KEYS && p.parts ? 1 : p.G, first_head = head * p.G + (KEYS ? (int)blockIdx.z : 0);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 span = __ldg(KEYS ? p.key_tiles + blockIdx.x : p.tiles + (gridDim.x - 1 - blockIdx.x));  // (long ones first)
+  const int4 span = *(KEYS ? p.key_tiles + blockIdx.x : p.tiles + (gridDim.x - 1 - blockIdx.x));  // (long ones first)
   if (span.x >= span.y) return;
 
   if (threadIdx.x == 0) {
@@ -1583,7 +1586,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   const int quarter = warp & 3, set = (warp - 2) >> 2;
   const int r = span.x + quarter * 32 + lane;  // the thread's query or key
   int4 row = make_int4(0, 0, 0, 0);
-  if (!KEYS && warp >= 2 && r < span.y) row = __ldg(p.rows + r);
+  if (!KEYS && warp >= 2 && r < span.y) row = p.rows[r];
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -1690,7 +1693,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
     if (!KEYS) {
       slope2 = p.slopes != nullptr ? kLog2e * __ldg(p.slopes + head) : 0.0f;
       lse = r < span.y ? lse_of(p, r, head) - up : INFINITY;
-      delta = r < span.y ? sigma * __ldg(p.delta + (int64_t)head * p.Tq + r) : 0.0f;
+      delta = r < span.y ? sigma * p.delta[(int64_t)head * p.Tq + r] : 0.0f;
     }
     // a block's queries, by the first two warps of the rows: from memory, then to shared memory
     float next_lse = INFINITY, next_delta = 0.0f;
@@ -1699,9 +1702,9 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
       if (t >= kBlock) return;
       const int i = other0 + (n % each) * kBlock + t, h = first_head + n / each;
       const bool there = i < other1;
-      next_row = there ? __ldg(p.rows + i) : make_int4(0, 0, 0, 0);
+      next_row = there ? p.rows[i] : make_int4(0, 0, 0, 0);
       next_lse = there ? lse_of(p, i, h) - up : INFINITY;
-      next_delta = there ? sigma * __ldg(p.delta + (int64_t)h * p.Tq + i) : 0.0f;
+      next_delta = there ? sigma * p.delta[(int64_t)h * p.Tq + i] : 0.0f;
     };
     auto deposit = [&](int n) {
       if (t < kBlock) {
@@ -1900,7 +1903,7 @@ __global__ void __launch_bounds__(256) keys_join_kernel(const __grid_constant__ 
       float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
       for (int g = 0; g < p.G; ++g) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(p.part + (int64_t)(which * p.G + g) * rows * p.D + row * p.D + c));
+        const float4 v = *reinterpret_cast<const float4*>(p.part + (int64_t)(which * p.G + g) * rows * p.D + row * p.D + c);
         s.x += v.x;
         s.y += v.y;
         s.z += v.z;

@@ -34,7 +34,8 @@ struct Params {
   int64_t ld_table, ld_grad, ld_out, V, n, n_bags, padding;
   float scale;
   int D, wide_ids, out_dtype, accumulate, sparse;
-  // workspace
+  // workspace: written by one kernel of a call and read by the next, which starts under its tail, so by plain loads behind
+  // griddepcontrol.wait and never by __ldg, which asks for memory that nobody writes while the kernel lives
   int32_t *key[2], *row[2];      // ids and their rows of grad, before and after a pass
   int32_t* counts;               // of a pass: [tiles][256], or [256][tiles] scanned
   int32_t* totals;               // [256]
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const __grid_consta
 #pragma unroll
   for (int k = 0; k < kPerThread; ++k) {
     const int64_t i = item_at(tile, k);
-    key[k] = i >= p.n ? -1 : FIRST ? key_of(p, i) : __ldg(p.key[0] + i);
+    key[k] = i >= p.n ? -1 : FIRST ? key_of(p, i) : p.key[0][i];
   }
 #pragma unroll
   for (int k = 0; k < kPerThread; ++k) {
@@ -355,8 +356,8 @@ __global__ void __launch_bounds__(kSortThreads, 3) scatter_kernel(const __grid_c
 #pragma unroll
   for (int k = 0; k < kPerThread; ++k) {
     const int64_t i = item_at(tile, k);
-    key[k] = i < p.n ? __ldg(p.key[0] + i) : -1;
-    row[k] = i < p.n ? __ldg(p.row[0] + i) : 0;
+    key[k] = i < p.n ? p.key[0][i] : -1;
+    row[k] = i < p.n ? p.row[0][i] : 0;
   }
   // where each digit's keys of this tile go: two threads a digit add up the tiles
   int mine = 0, all = 0, total;
@@ -508,8 +509,8 @@ __global__ void __launch_bounds__(256) heads_kernel(const __grid_constant__ Para
   for (int k = lane; k < p.run; k += 32) {
     const int64_t i = (int64_t)run * p.run + k;
     if (i < p.n) {
-      const int key = __ldg(p.key[0] + i);
-      n += key < p.V && (i == 0 || __ldg(p.key[0] + i - 1) != key);
+      const int key = p.key[0][i];
+      n += key < p.V && (i == 0 || p.key[0][i - 1] != key);
     }
   }
   n = __reduce_add_sync(kAll, n);
@@ -557,11 +558,11 @@ __global__ void __launch_bounds__(kSumThreads) sums_kernel(const __grid_constant
   const int count = run < p.runs ? (int)(i1 - i0) : 0;
   const int32_t* keys = p.key[0];
   int2* mine = s_runs + team * p.run;
-  for (int k = lane; k < count; k += p.team) mine[k] = make_int2(__ldg(keys + i0 + k), __ldg(p.row[0] + i0 + k));
+  for (int k = lane; k < count; k += p.team) mine[k] = make_int2(keys[i0 + k], p.row[0][i0 + k]);
   int prev = -1, next = -1, rank = 0;
   if (count > 0) {
-    if (i0 > 0) prev = __ldg(keys + i0 - 1);
-    if (i1 < p.n) next = __ldg(keys + i1);
+    if (i0 > 0) prev = keys[i0 - 1];
+    if (i1 < p.n) next = keys[i1];
     if (p.sparse) rank = p.heads[run];
   }
   __syncthreads();
@@ -623,7 +624,7 @@ __global__ void __launch_bounds__(kSumThreads) combine_kernel(const __grid_const
   auto starts = [&](int r) {
     const int64_t i0 = (int64_t)r * p.run, i1 = i0 + p.run;
     if (i1 >= p.n) return -1;
-    const int key = __ldg(keys + i1 - 1), next = __ldg(keys + i1), first = __ldg(keys + i0), prev = i0 > 0 ? __ldg(keys + i0 - 1) : -1;
+    const int key = keys[i1 - 1], next = keys[i1], first = keys[i0], prev = i0 > 0 ? keys[i0 - 1] : -1;
     return key < p.V && next == key && !(first == key && prev == key) ? key : -1;  // (else it came from before)
   };
   auto add = [&](int j, int from_run, int c, float* acc) {
@@ -657,14 +658,14 @@ __global__ void __launch_bounds__(kSumThreads) combine_kernel(const __grid_const
   int last = -1;
   if (key >= 0) {  // the runs behind: how many of them end with the row still going on
     const int64_t end = ((int64_t)run + 2 + lane) * p.run - 1;  // of run + 1 + lane
-    const bool on = end + 1 < p.n && __ldg(keys + end) == key && __ldg(keys + end + 1) == key;
+    const bool on = end + 1 < p.n && keys[end] == key && keys[end + 1] == key;
     const uint32_t off = __ballot_sync(kAll, !on);
     last = run + __ffs(off);
     if (off == 0) {  // the last id of the row, 32 probes at once
       int64_t lo = ((int64_t)run + kFar) * p.run, hi = p.n;
       while (hi - lo > 1) {
         const int64_t step = (hi - lo + 31) / 32, m = lo + (lane + 1) * step;
-        const int n = __popc(__ballot_sync(kAll, m < hi && __ldg(keys + m) == key));
+        const int n = __popc(__ballot_sync(kAll, m < hi && keys[m] == key));
         lo += n * step;
         hi = min(hi, lo + step);
       }
