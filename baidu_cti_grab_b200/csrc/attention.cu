@@ -43,6 +43,7 @@ struct Params {
   int4* tiles;                    // of the queries: rows [x, y), the keys that they see [z, w)
   int4* key_tiles;                // (backward) of the keys: rows [x, y), queries that may see them [z, w)
   uint32_t* next;                 // tickets for work
+  int2* redo;                     // (forward tiles) [tiles x heads][4]: rows of 32 to be taken again, the entry before it
   float* part;                    // few queries: of every row and split, the sums [D], their maximum and their weights' sum
   int splits, parts;
   const void *q_off, *k_off, *prefix;
@@ -808,7 +809,7 @@ __device__ __forceinline__ void transform(const Params& p, uint32_t* raw, float 
 // or fall with distance are put back in their place), then the weights, which go back as 16-bit values for the second
 // product.  The running sum is fp32; the accumulator is rescaled only when a maximum has grown by more than 2^8 over
 // what it is scaled to.  Rounding a weight to the type is half a step of its own value (2^-8 bf16, 2^-11 fp16),
-// independent from key to key.
+// independent from key to key.  Rows whose sums are not finite are noted and taken again at the CTA's end.
 //
 // Bound by the row warps' issue slots: 1024 users of 1 to 200 items in 8 heads of 64 take 115 us (their bytes 65);
 // two causal documents of 4100 to 7001 rows, 8 heads of 128, capped scores, 427 us.
@@ -831,7 +832,7 @@ struct Forward {
 };
 constexpr int kItems = 4;  // tiles that are posted to the rows: theirs, up to two ahead, and one more
 struct Item {
-  int r0, r1, head, key0, blocks;  // blocks 0: no more
+  int r0, r1, head, key0, blocks, unit;  // blocks 0: no more; unit: the ticket
 };
 
 template <typename T, int DP>
@@ -854,6 +855,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
   __shared__ __align__(8) uint64_t pairs[4];
   __shared__ float s_max[2][2][C::kSets == 2 ? kTile : 1], s_total[2][C::kSets == 2 ? kTile : 1];
   __shared__ int s_redo[C::kSets == 2 ? kTile : 1];
+  __shared__ int s_redo_last[4];  // of 32 rows: the last unit with rows that are taken again, or -1
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -869,7 +871,10 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
     mbar_init(smem_u32(&pready), C::kRowThreads / 32);
     mbar_init(smem_u32(&pvdone), 1);
     mbar_init(smem_u32(&drained), 1);
-    for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&pairs[q]), 2);
+    for (int q = 0; q < 4; ++q) {
+      mbar_init(smem_u32(&pairs[q]), 2);
+      s_redo_last[q] = -1;
+    }
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -907,7 +912,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
         a_block = 0;
         while (ticket < items && ahead.blocks == 0) {
           const int4 t = p.tiles[p.n_tiles - 1 - ticket / p.H];
-          ahead = Item{t.x, t.y, (int)(ticket % p.H), t.z, t.w > t.z ? (t.w - t.z + kBlock - 1) / kBlock : 0};
+          ahead = Item{t.x, t.y, (int)(ticket % p.H), t.z, t.w > t.z ? (t.w - t.z + kBlock - 1) / kBlock : 0, (int)ticket};
           ticket = atomicAdd(p.next, 1u);  // (needed a tile later)
         }
         s_item[posted % kItems] = ahead;
@@ -1183,16 +1188,25 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
         if (!ok) break;
         redo = set == 0 && (redo || s_redo[quarter * 32 + lane] != 0);
       }
-      uint32_t again = __ballot_sync(kAll, redo && there);
-      __syncwarp();
-      while (again != 0) {
-        const int i = __ffs(again) - 1;
-        again &= again - 1;
-        row_forward<T>(p, it.r0 + quarter * 32 + i, h);
-        __syncwarp();
+      // (not here: others of this CTA wait for the next tile's rows, and a row over long keys takes longer than they do)
+      const uint32_t again = __ballot_sync(kAll, redo && there);
+      if (again != 0 && lane == 0) {
+        p.redo[(int64_t)it.unit * 4 + quarter] = make_int2((int)again, s_redo_last[quarter]);
+        s_redo_last[quarter] = it.unit;
       }
       it = next;
       row = next_row;
+    }
+    // the rows that were not finite, one by one, when nothing waits for this warp but the CTA's end
+    __syncwarp();
+    for (int unit = set == 0 ? s_redo_last[quarter] : -1; unit >= 0;) {
+      const int2 entry = p.redo[(int64_t)unit * 4 + quarter];
+      const int r0 = p.tiles[p.n_tiles - 1 - unit / p.H].x + quarter * 32, h = unit % p.H;
+      for (uint32_t again = (uint32_t)entry.x; again != 0; again &= again - 1) {
+        row_forward<T>(p, r0 + __ffs(again) - 1, h);
+        __syncwarp();
+      }
+      unit = entry.y;
     }
   }
   tc::tc_fence_before();
@@ -2161,8 +2175,9 @@ using namespace rb;
 extern "C" int64_t rb_segment_attention_workspace_size(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D) {
   if (Tq < 0 || Tk < 0 || S < 0 || H <= 0 || Hk <= 0 || D <= 0 || Tq > 1 << 30) return -1;
   const int64_t splits = H % Hk == 0 ? attn::splits_of(Tq, Tk, S, H, Hk, D) : 0;
-  const int64_t lists = 16 + Tq * 16 + (Tq / attn::kTile + S + 2) * 16;
-  return lists + (splits > 1 ? Tq * H * splits * (D + 2) * 4 : 0);
+  const int64_t tiles = Tq / attn::kTile + S + 2, lists = 16 + Tq * 16 + tiles * 16;
+  if (splits > 0) return lists + (splits > 1 ? Tq * H * splits * (D + 2) * 4 : 0);
+  return lists + (D % 8 == 0 && D <= 128 ? tiles * H * 32 : 0);
 }
 
 extern "C" int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h,
@@ -2197,6 +2212,7 @@ extern "C" int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, con
   p.rows = static_cast<int4*>(workspace) + 1;
   p.tiles = p.rows + Tq;
   p.part = reinterpret_cast<float*>(p.tiles + (Tq / kTile + S + 2));
+  p.redo = reinterpret_cast<int2*>(p.part);  // (no kernel uses both)
   p.q_off = q_offsets;
   p.k_off = k_offsets;
   p.prefix = prefix;

@@ -449,3 +449,29 @@ def test_module_trains_and_reads_a_cache(cuda_device):
         assert rel(new, y[last].double()) < 2.0 ** -6
     with pytest.raises(RuntimeError):
         attention.segment_attention(q.bfloat16(), k, v, off, slopes=layer.slopes.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_that_are_taken_again_hold_nobody_up(cuda_device, D):
+    """A NaN among a long segment's values: a tile that meets it takes its rows again one by one, seconds of work for 32
+    rows of 120,000 keys, and the tiles behind it in the same CTA have waits of bounded time.  All rows are written, other
+    users' and those before the last tile with the same bits as without the NaN.
+
+    The last tile's rows: either result is within half + eta + n u of sum p |v| and half of itself, with
+    eta < 2^-10 (scale sum |q| |k| is under 2^5 here, so ds under 2 D u 2^5 = 2^-11)."""
+    from baidu_cti_grab_b200 import device_ops
+
+    n = [120_000, 300]
+    q, k, v, _ = _inputs(n, n, 1, 1, D, BF, D, cuda_device)
+    off = _offsets(n, torch.int32, cuda_device)
+    want, _ = device_ops.segment_attention(q, k, v, off)
+    spread, _ = device_ops.segment_attention(q, k, v.abs(), off)
+    v[n[0] - 1] = math.nan  # which the segment's last query alone sees
+    got, _ = device_ops.segment_attention(q, k, v, off)
+    assert device_ops.device_error() == 0
+    assert torch.equal(got[:n[0] - 128], want[:n[0] - 128]) and torch.equal(got[n[0] + 128:], want[n[0] + 128:])
+    rest = [i for i in range(n[0] - 128, n[0] + 128) if i != n[0] - 1]
+    off_by = (got[rest].double() - want[rest].double()).abs()
+    half = torch.finfo(BF).eps / 2
+    assert bool((off_by <= 2 * ((half + 2.0 ** -10 + n[0] * U) * spread[rest].double() * (1 + half) + half * want[rest].double().abs() * (1 + half))).all())
+    assert bool(got[n[0] - 1].isnan().all())
