@@ -715,6 +715,18 @@ __host__ __device__ constexpr uint32_t idesc_of(int n, bool turned) {
   return (1u << 4) | type_bits<T>() | (turned ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
 
+// Weights meet the values as two values of the type: what a weight is rounded to, and what is left, rounded (2^-18 of it
+// bf16, 2^-22 fp16).  In fp16 they are 2^7 times as large, so that those of 2^-25 of a row's largest are still there.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+template <typename T>
+__device__ __forceinline__ void two_values(F2 v, uint32_t& whole, uint32_t& rest) {
+  const float2 f = un(v);
+  whole = pack2<T>(f.x, f.y);
+  const float2 top = widen2<T>(whole), left = un(sub2(v, f2(top.x, top.y)));
+  rest = pack2<T>(left.x, left.y);
+}
+
 // A row of fp32 sums of `n` columns times w, as the type, to 16-byte aligned memory
 template <typename T>
 __device__ __forceinline__ void store_sums(T* to, const uint32_t* v, int n, float w, bool wide) {
@@ -808,8 +820,8 @@ __device__ __forceinline__ void transform(const Params& p, uint32_t* raw, float 
 // A row's thread goes over the block's scores in TMEM twice, 32 at a time: the maximum (scores that are masked or capped
 // or fall with distance are put back in their place), then the weights, which go back as 16-bit values for the second
 // product.  The running sum is fp32; the accumulator is rescaled only when a maximum has grown by more than 2^8 over
-// what it is scaled to.  Rounding a weight to the type is half a step of its own value (2^-8 bf16, 2^-11 fp16),
-// independent from key to key.  Rows whose sums are not finite are noted and taken again at the CTA's end.
+// what it is scaled to.  A weight goes into the second product as two values of the type (with the first alone `out` was
+// 1.4 times as far from the exact sums as its own rounding makes it).  Rows whose sums are not finite are noted and taken again at the CTA's end.
 //
 // Bound by the row warps' issue slots: 1024 users of 1 to 200 items in 8 heads of 64 take 115 us (their bytes 65);
 // two causal documents of 4100 to 7001 rows, 8 heads of 128, capped scores, 427 us.
@@ -820,8 +832,8 @@ struct Forward {
   static constexpr int kKvBytes = kBlock * 128 * kChunks;
   static constexpr int kStages = 2;
   static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kKvBytes;
-  // DP 64: the weights lie where the scores were, 128 columns in all, and four CTAs an SM fill each other's waits; DP
-  // 128: apart, two CTAs, and the next block's scores are computed meanwhile
+  // DP 64: the weights (both of their values) lie where the scores were, 128 columns in all, and four CTAs an SM fill each
+  // other's waits; DP 128: apart, two CTAs, and the next block's scores are computed meanwhile
   static constexpr bool kApart = DP == 128;
   static constexpr int kPAt = kApart ? 64 : 0, kOAt = kApart ? 128 : 64;
   static constexpr int kTmemCols = kApart ? 256 : 128;
@@ -993,7 +1005,11 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
           tc::tc_fence_after();
           const uint32_t vd = columns_desc(v_at + v_use.slot * C::kKvBytes, kBlock * 128);
 #pragma unroll
-          for (int i = 0; i < kBlock / 16; ++i) mma_ts(tmem + C::kOAt, tmem + C::kPAt + 8 * i, vd + i * (16 * 128 / 16), idesc_o, n > 0 || i > 0);
+          for (int i = 0; i < kBlock / 16; ++i) {
+            const uint32_t w = tmem + C::kPAt + (i >> 1) * kHalf + (i & 1) * 8;
+            mma_ts(tmem + C::kOAt, w, vd + i * (16 * 128 / 16), idesc_o, n > 0 || i > 0);
+            mma_ts(tmem + C::kOAt, w + kHalf / 2, vd + i * (16 * 128 / 16), idesc_o, true);
+          }
           tc::umma_commit(smem_u32(&pvdone));
           v_use.next();
           if (last) {
@@ -1113,7 +1129,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
           }
           if (grow) top = high;
         }
-        const float shift = top == -INFINITY ? 0.0f : -top * unit;
+        const float shift = top == -INFINITY ? 0.0f : fmaf(-top, unit, kLift<T>);
         const F2 unit2 = f2(unit, unit), shift2 = f2(shift, shift);
         F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
         auto weigh = [&](const uint32_t* x, uint32_t* w) {
@@ -1122,15 +1138,15 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
             const float2 e = un(fma2(f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), unit2, shift2));
             const float a = exp2_fast(e.x), b = exp2_fast(e.y);
             sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], f2(a, b));
-            w[c / 2] = pack2<T>(a, b);
+            two_values<T>(f2(a, b), w[c / 2], w[kHalf / 2 + c / 2]);
           }
         };
 #pragma unroll 1
         for (int c0 = C::kSets == 2 ? set * kHalf : 0; c0 < (C::kSets == 2 ? (set + 1) * kHalf : kBlock); c0 += kHalf) {
-          uint32_t w[kHalf / 2];
+          uint32_t w[kHalf];  // of 32 keys: what the weights are rounded to, and what is left, in the scores' columns
           if (reach.of(j0 + c0) == kNone) {
 #pragma unroll
-            for (int c = 0; c < kHalf / 2; ++c) w[c] = 0u;
+            for (int c = 0; c < kHalf; ++c) w[c] = 0u;
           } else if constexpr (C::kSets == 2) {
             weigh(held, w);
           } else {
@@ -1139,7 +1155,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
             tmem_wait_ld();
             weigh(x, w);
           }
-          tmem_put16(mine + C::kPAt + c0 / 2, w);
+          tmem_put32(mine + C::kPAt + c0, w);
         }
         const float2 s2 = un(add2(sum[0], sum[1]));
         total += s2.x + s2.y;
@@ -1181,7 +1197,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
         if (there) store_sums<T>(out + c, o, p.D - c, sees ? w : 0.0f, wide);
       }
       if (there && p.lse != nullptr && set == 0)
-        p.lse[(int64_t)h * p.Tq + r] = sees && total != 0.0f ? kLn2 * fmaf(top, unit, log2f(total)) : -INFINITY;
+        p.lse[(int64_t)h * p.Tq + r] = sees && total != 0.0f ? kLn2 * fmaf(top, unit, log2f(total) - kLift<T>) : -INFINITY;
       if constexpr (C::kSets == 2) {  // what either finds not finite in its columns the first takes again, once both have stored
         if (set == 1) s_redo[quarter * 32 + lane] = redo;
         ok = meet();
@@ -1374,7 +1390,7 @@ __global__ void __launch_bounds__(Few<DP>::kThreads, Few<DP>::kCtas)
             top[i] = high[i];
             grow = true;
           }
-          shift[i] = top[i] == -INFINITY ? 0.0f : top[i];
+          shift[i] = top[i] == -INFINITY ? 0.0f : top[i] - kLift<T>;
         }
         if (__any_sync(kAll, grow)) {
 #pragma unroll
@@ -1387,14 +1403,14 @@ __global__ void __launch_bounds__(Few<DP>::kThreads, Few<DP>::kCtas)
           total[0] *= keep[0];
           total[1] *= keep[1];
         }
-        uint32_t w[4];
+        uint32_t w[4], rest[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float u = exp2_fast(x[e][2 * i] - shift[i]), v = exp2_fast(x[e][2 * i + 1] - shift[i]);
             total[i] += u + v;
-            w[2 * e + i] = pack2<T>(u, v);
+            two_values<T>(f2(u, v), w[2 * e + i], rest[2 * e + i]);
           }
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
@@ -1402,6 +1418,8 @@ __global__ void __launch_bounds__(Few<DP>::kThreads, Few<DP>::kCtas)
           ldsm4_turned(at + C::kBytes + (k >> 2) * kBlock * 128 + ((((k & 3) * 2 + half) ^ (key & 7)) << 4), r);
           mma16<T>(o[2 * k], w, r[0], r[1]);
           mma16<T>(o[2 * k + 1], w, r[2], r[3]);
+          mma16<T>(o[2 * k], rest, r[0], r[1]);
+          mma16<T>(o[2 * k + 1], rest, r[2], r[3]);
         }
       }
       __syncwarp();
@@ -1459,7 +1477,7 @@ __global__ void __launch_bounds__(Few<DP>::kThreads, Few<DP>::kCtas)
     if (p.splits > 1) {
       if (lane < 2) p.part[(at * p.splits + split) * (p.D + 2) + p.D + lane] = lane ? sum : high;
     } else {
-      if (lane == 0 && p.lse != nullptr) p.lse[(int64_t)h * p.Tq + token] = sum == 0.0f ? -INFINITY : kLn2 * (high + log2f(sum));
+      if (lane == 0 && p.lse != nullptr) p.lse[(int64_t)h * p.Tq + token] = sum == 0.0f ? -INFINITY : kLn2 * (high + (log2f(sum) - kLift<T>));
       if (!__all_sync(kAll, finite)) {
         __syncwarp();
         row_forward<T>(p, token, h);
@@ -1496,7 +1514,7 @@ __global__ void __launch_bounds__(256) few_join_kernel(const __grid_constant__ P
     static_cast<T*>(p.out)[at * p.D + c] = T(sum == 0.0f ? 0.0f : v / sum);
   }
   const int token = (int)(at / p.H), h = (int)(at % p.H);
-  if (lane == 0 && p.lse != nullptr) p.lse[(int64_t)h * p.Tq + token] = sum == 0.0f ? -INFINITY : kLn2 * (high + log2f(sum));
+  if (lane == 0 && p.lse != nullptr) p.lse[(int64_t)h * p.Tq + token] = sum == 0.0f ? -INFINITY : kLn2 * (high + (log2f(sum) - kLift<T>));
   if (!__all_sync(kAll, finite)) {
     __syncwarp();
     row_forward<T>(p, token, h);

@@ -475,3 +475,44 @@ def test_rows_that_are_taken_again_hold_nobody_up(cuda_device, D):
     half = torch.finfo(BF).eps / 2
     assert bool((off_by <= 2 * ((half + 2.0 ** -10 + n[0] * U) * spread[rest].double() * (1 + half) + half * want[rest].double().abs() * (1 + half))).all())
     assert bool(got[n[0] - 1].isnan().all())
+
+
+def _few_bits(dtype, exact, spread, loose):
+    """A value rounded once: half of itself, and sums of weights as two values (half of half of them, in fp16 2^-32 of the
+    largest of up to 3000) beside `loose`, the bound without any of these."""
+    half = torch.finfo(dtype).eps / 2
+    return half * exact.abs() + (half * half + (3000 * 2.0 ** -32 if dtype is HF else 0.0)) * spread + loose * (1 + half)
+
+
+@pytest.mark.parametrize("nq,nk,H,Hk,D,mask", [
+    ([300, 41], None, 2, 2, 64, {}), ([257, 130], None, 4, 1, 128, dict(cap=20.0)), ([90] * 8, None, 2, 2, 40, dict(causal=False)),
+    ([2, 1, 3], [1500, 40, 2700], 8, 2, 64, {}), ([5], [2900], 4, 1, 128, dict(causal=False)),
+])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_weights_keep_their_bits(cuda_device, dtype, nq, nk, H, Hk, D, mask):
+    """`out` is as near as its own rounding: the weights meet the values with twice the type's bits."""
+    from baidu_cti_grab_b200 import device_ops
+
+    nk = nq if nk is None else nk
+    q, k, v, _ = _inputs(nq, nk, H, Hk, D, dtype, D, cuda_device)
+    off, k_off = _offsets(nq, torch.int32, cuda_device), _offsets(nk, torch.int32, cuda_device)
+    out, _ = device_ops.segment_attention(q, k, v, off, k_off, **mask)
+    val, loose = oracle(q, k, v, nq, nk, **mask)
+    spread, _ = oracle(q, k, v.abs(), nq, nk, **mask)
+    _close(out, val["out"], _few_bits(dtype, val["out"], spread["out"], loose["out"]), dtype)
+
+
+def test_many_small_weights_in_fp16(cuda_device):
+    """One key of a score 17 above 20,000 others, whose weights of 2^-24.5 fp16 by itself rounds to 2^-24: what a weight is
+    rounded to is 2^-32 of the largest, and each sum is off by m u.  Either form of the kernels."""
+    from baidu_cti_grab_b200 import device_ops
+
+    m = 20_000
+    for Tq in (1, 6000):
+        q, k, v = (torch.zeros(n, 1, 64, device=cuda_device, dtype=HF) for n in (Tq, m, m))
+        q[..., 0], k[0, :, 0], v[1:] = 8.0, 17.0, 1.0
+        off, k_off = _offsets([Tq], torch.int32, cuda_device), _offsets([m], torch.int32, cuda_device)
+        out, lse = device_ops.segment_attention(q, k, v, off, k_off, causal=False, want_lse=True)
+        w = (m - 1) * math.exp(-17.0)
+        assert bool((out.double() - w / (1 + w)).abs().max() <= w / (1 + w) * (2.0 ** -11 + 2.0 ** -17 + 2 * m * U) + m * 2.0 ** -32)
+        assert bool((lse.double() - 17.0 - math.log1p(w)).abs().max() <= 2.0 ** -17 + m * U)
