@@ -689,10 +689,6 @@ __device__ __forceinline__ void tmem_get16(uint32_t taddr, uint32_t* r) {
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_put8(uint32_t taddr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
 __device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -1530,10 +1526,9 @@ __global__ void __launch_bounds__(256) few_join_kernel(const __grid_constant__ P
 //
 //   S = A1 B1^T   dP = A2 B2^T   p = exp(s - lse)   e = p (dP - delta) (1 - tanh^2)   acc += e B1   [dv += p B2]
 //
-// seven products for both where one kernel that adds dq by atomics has five.  p goes to the second products as 16-bit
-// values out of TMEM, e as two of them: what it is rounded to, and what is left, rounded.  (With the first alone dq and dk
-// are 1.3 to 1.4 times as far from the exact sums, 2.4e-3 for 1.7e-3 in bf16; the products of the second are hidden behind
-// the rows' arithmetic: 1501 and 1564 us with and without for two long documents.)  In fp16 they are brought into the
+// seven products for both where one kernel that adds dq by atomics has five.  p and e go to the second products as two
+// values of the type each, out of TMEM: what they are rounded to, and what is left, rounded.  (With the first alone dq, dk
+// and dv are 1.3 to 1.4 times as far from the exact sums, 2.4e-3 for 1.7e-3 in bf16.)  In fp16 they are brought into the
 // type's range first: p by 2^15, e by that and the power of two that keeps |dP - delta| under 1 (from the largest norms of
 // a row of dO and of V).
 //
@@ -1557,8 +1552,7 @@ struct Backward {
   static constexpr bool kApart = !(DP == 64 && KEYS);
   static constexpr int kEAt = !kApart ? 64 : KEYS ? kAcc2At + DP : kAcc2At;
   static constexpr int kPAt = kApart ? kEAt + 64 : 0;     // (KEYS)
-  static constexpr int kStride = kApart ? 8 : 16;         // from sixteen of p to the next: in place, at their own columns
-  static constexpr int kEStride = 16;                     // sixteen of e as they are rounded, then what is left of them
+  static constexpr int kStride = 16;                      // sixteen of p or e as they are rounded, then what is left of them
   static constexpr int kTmemCols = DP == 64 ? 256 : 512;
 };
 
@@ -1700,9 +1694,12 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
         const uint32_t b1 = columns_desc(b1_at + held.slot * C::kBBytes, kBlock * 128), b2 = columns_desc(b2_at + held.slot * C::kBBytes, kBlock * 128);
 #pragma unroll
         for (int i = 0; i < kBlock / 16; ++i) {
-          if (KEYS) mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + C::kStride * i, b2 + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
-          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kEStride * i, b1 + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
-          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kEStride * i + 8, b1 + i * (16 * 128 / 16), idesc, true);
+          if (KEYS) {
+            mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + C::kStride * i, b2 + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
+            mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + C::kStride * i + 8, b2 + i * (16 * 128 / 16), idesc, true);
+          }
+          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kStride * i, b1 + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
+          mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kStride * i + 8, b1 + i * (16 * 128 / 16), idesc, true);
         }
         tc::umma_commit(smem_u32(&done));
         held.next();
@@ -1765,7 +1762,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
         const int c0 = (set * C::kSteps + step) * C::kPart;
         // of these keys (queries) and the warp's rows: is there one that sees, do all
         const Seen seen = KEYS ? s_span[n & 1][c0 / kHalf].of(span.x + quarter * 32) : reach.of(o0 + c0, C::kPart);
-        uint32_t w[C::kPart / 2], e[C::kPart];
+        uint32_t w[C::kPart], e[C::kPart];
         if (seen != kNone) {
           uint32_t x[C::kPart], y[C::kPart];
           tmem_get16(mine + c0, x);
@@ -1822,16 +1819,12 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
             const F2 l = KEYS ? *reinterpret_cast<const F2*>(&s_lse[n & 1][c0 + c]) : f2(-lse, -lse);
             const float2 v = un(fma2(f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), f2(left, left), l));
             const float a = exp2_fast(v.x), b = exp2_fast(v.y);
-            if (KEYS) w[c / 2] = pack2<T>(a, b);
-            const F2 g = mul2(f2(a, b), pair(y + c));
-            const float2 whole = un(g);
-            e[c / 2] = pack2<T>(whole.x, whole.y);
-            const float2 top = widen2<T>(e[c / 2]), rest = un(sub2(g, f2(top.x, top.y)));
-            e[C::kPart / 2 + c / 2] = pack2<T>(rest.x, rest.y);
+            if (KEYS) two_values<T>(f2(a, b), w[c / 2], w[C::kPart / 2 + c / 2]);
+            two_values<T>(mul2(f2(a, b), pair(y + c)), e[c / 2], e[C::kPart / 2 + c / 2]);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < C::kPart / 2; ++c) w[c] = e[c] = e[C::kPart / 2 + c] = 0u;
+          for (int c = 0; c < C::kPart; ++c) w[c] = e[c] = 0u;
           if (C::kApart && step == C::kSteps - 1) {
             tc::tc_fence_before();
             warp_arrive(&sfree);
@@ -1842,8 +1835,8 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
           tc::tc_fence_after();
         }
         if (ok) {
-          if (KEYS) tmem_put8(mine + C::kPAt + c0 / C::kPart * C::kStride, w);
-          tmem_put16(mine + C::kEAt + c0 / C::kPart * C::kEStride, e);
+          if (KEYS) tmem_put16(mine + C::kPAt + c0 / C::kPart * C::kStride, w);
+          tmem_put16(mine + C::kEAt + c0 / C::kPart * C::kStride, e);
         }
       }
       if (ok) {

@@ -516,3 +516,23 @@ def test_many_small_weights_in_fp16(cuda_device):
         w = (m - 1) * math.exp(-17.0)
         assert bool((out.double() - w / (1 + w)).abs().max() <= w / (1 + w) * (2.0 ** -11 + 2.0 ** -17 + 2 * m * U) + m * 2.0 ** -32)
         assert bool((lse.double() - 17.0 - math.log1p(w)).abs().max() <= 2.0 ** -17 + m * U)
+
+
+@pytest.mark.parametrize("nq,nk,H,Hk,D,mask", [
+    ([300, 41], None, 2, 2, 64, {}), ([700], None, 4, 1, 64, dict(causal=False)), ([257, 130], None, 4, 2, 128, dict(cap=20.0)),
+    ([90] * 8, [200] * 8, 2, 2, 40, {}),
+])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_value_gradients_keep_their_bits(cuda_device, dtype, nq, nk, H, Hk, D, mask):
+    """dv is as near as its own rounding: p meets the output's gradient with twice the type's bits (in fp16 p is brought
+    up by 2^15 and loses 2^-40 of at most 3000 rows)."""
+    from baidu_cti_grab_b200 import device_ops
+
+    nk = nq if nk is None else nk
+    q, k, v, g = _inputs(nq, nk, H, Hk, D, dtype, D, cuda_device)
+    off, k_off = _offsets(nq, torch.int32, cuda_device), _offsets(nk, torch.int32, cuda_device)
+    out, lse = device_ops.segment_attention(q, k, v, off, k_off, want_lse=True, **mask)
+    dv = device_ops.segment_attention_backward(g, q, k, v, out, lse, off, k_off, **mask)[2]
+    val, loose = oracle(q, k, v, nq, nk, g=g, **mask)
+    spread, _ = oracle(q, k, v, nq, nk, g=g.abs(), **mask)
+    _close(dv, val["dv"], _few_bits(dtype, val["dv"], spread["dv"], loose["dv"]), dtype)
