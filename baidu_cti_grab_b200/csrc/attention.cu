@@ -38,7 +38,7 @@ struct Params {
   const void *q, *k, *v, *o, *g;  // o, g: the forward call's output and the gradient it got
   void *out, *dq, *dk, *dv;
   float* lse;                     // [H, Tq] log of the sum of exp(s), -inf where nothing is seen
-  float* delta;                   // [H, Tq]
+  float* delta;                   // [H, Tq] dout . out, then (behind the queries' gradients) the sum of p dp
   int4* rows;                     // [Tq]: lo, hi, place of the query among the packed keys, 0
   int4* tiles;                    // of the queries: rows [x, y), the keys that they see [z, w)
   int4* key_tiles;                // (backward) of the keys: rows [x, y), queries that may see them [z, w)
@@ -237,26 +237,34 @@ __device__ __forceinline__ float lse_of(const Params& p, int r, int h) {
   return l == -INFINITY ? INFINITY : kLog2e * l;
 }
 
+// (delta and what it is off by: at backward_kernel)
 template <typename T>
 __device__ __noinline__ void row_dq(const Params& p, int r, int h) {
   const int lane = threadIdx.x & 31, hk = h / p.G;
   const int4 row = p.rows[r];
   const float slope = p.slopes != nullptr ? __ldg(p.slopes + h) : 0.0f;
   const float lse = lse_of(p, r, h), delta = p.delta[(int64_t)h * p.Tq + r];
-  float q[kPerLane], g[kPerLane], dq[kPerLane], k[kPerLane], v[kPerLane], slant;
+  float q[kPerLane], g[kPerLane], dq[kPerLane], mean[kPerLane], k[kPerLane], v[kPerLane], slant, off = 0.0f;
   load_row<T>(p.q, r * p.q_t + h * p.q_h, p.D, lane, q);
   load_row<T>(p.g, r * p.g_t + h * p.g_h, p.D, lane, g);
 #pragma unroll
-  for (int c = 0; c < kPerLane; ++c) dq[c] = 0.0f;
+  for (int c = 0; c < kPerLane; ++c) dq[c] = mean[c] = 0.0f;
 #pragma unroll 1
   for (int j = row.x; j < row.y; ++j) {
     load_row<T>(p.k, j * p.k_t + hk * p.k_h, p.D, lane, k);
     load_row<T>(p.v, j * p.v_t + hk * p.v_h, p.D, lane, v);
     const float s = score_of(p, dot_row(q, k), row.z, j, slope, slant);
-    const float e = exp2_fast(s - lse) * (dot_row(g, v) - delta) * slant;
+    const float w = exp2_fast(s - lse), d = w * (dot_row(g, v) - delta);
+    off += d;
 #pragma unroll
-    for (int c = 0; c < kPerLane; ++c) dq[c] = fmaf(e, k[c], dq[c]);
+    for (int c = 0; c < kPerLane; ++c) {
+      dq[c] = fmaf(d * slant, k[c], dq[c]);
+      mean[c] = fmaf(w * slant, k[c], mean[c]);
+    }
   }
+#pragma unroll
+  for (int c = 0; c < kPerLane; ++c) dq[c] = fmaf(-off, mean[c], dq[c]);
+  if (lane == 0) p.delta[(int64_t)h * p.Tq + r] = delta + off;
   store_row<T>(p.dq, ((int64_t)r * p.H + h) * p.D, p.D, lane, dq, p.scale);
 }
 
@@ -475,104 +483,6 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Para
   }
 }
 
-// delta again, as sum_j p_ij dp_ij, for the rows that see at most kNear keys.  There dp_ij - delta_i is a small difference,
-// and the output's rounding in dout . out is no longer small beside it: dq and dk of segments of 4 to 7 rows were 1.6 times
-// as far from the exact ones (fp16) as their own rounding makes them.  The error of row i falls with its weights, so longer
-// rows keep the product with the output.  A CTA lists those of its rows, and LANES threads take one of a head.  Bound by the
-// latency of its reads: 11 us of 464 for 60 users of 10 to 1000 items in both directions, 49 of 445 for 2048 users of 40
-// (backward); with rows of up to 16 keys 26 us and more.
-constexpr int kNear = 8;
-template <typename T, int LANES, bool VEC>
-__global__ void __launch_bounds__(256) near_kernel(const __grid_constant__ Params p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int kPer = VEC ? 8 : (kMaxWidth + LANES - 1) / LANES, kTeams = 32 / LANES;  // of a warp
-  __shared__ int s_row[32], s_count;
-  const int lane = threadIdx.x % LANES;
-  if (threadIdx.x < 32) {  // those of this CTA's rows (32 at most) that see few keys
-    const int each = (p.Tq + (int)gridDim.x - 1) / (int)gridDim.x;
-    const int64_t r = (int64_t)blockIdx.x * each + threadIdx.x;
-    const int4 row = (int)threadIdx.x < each && r < p.Tq ? p.rows[r] : make_int4(0, 0, 0, 0);
-    const bool few = row.y > row.x && row.y - row.x <= kNear;
-    const uint32_t all = __ballot_sync(kAll, few);
-    if (few) s_row[__popc(all & ((1u << threadIdx.x) - 1u))] = (int)r;
-    if (threadIdx.x == 0) s_count = __popc(all);
-  }
-  __syncthreads();
-  const int64_t units = (int64_t)s_count * p.H;
-  auto raw = [&](const void* from, int64_t at, bool there) {
-    return there && lane * 8 < p.D ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(from) + at + lane * 8)) : make_uint4(0u, 0u, 0u, 0u);
-  };
-  auto widen = [](const uint4& v, float* f) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = widen2<T>(w[i]);
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
-    }
-  };
-  auto load = [&](const void* from, int64_t at, bool there, float* f) {
-    if constexpr (VEC) {
-      widen(raw(from, at, there), f);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) f[i] = there && lane + i * LANES < p.D ? to_f32(static_cast<const T*>(from)[at + lane + i * LANES]) : 0.0f;
-    }
-  };
-  for (int64_t first = threadIdx.x / 32 * kTeams; first < units; first += 256 / LANES) {
-    const int64_t unit = min(first + threadIdx.x % 32 / LANES, units - 1);  // (the last of them twice, to the same place)
-    const int64_t r = s_row[unit / p.H];
-    const int h = (int)(unit % p.H), hk = h / p.G;
-    const int4 row = p.rows[r];
-    const int n = row.y - row.x, most = __reduce_max_sync(kAll, n);
-    float q[kPer], g[kPer], total = 0.0f, slant;
-    load(p.q, r * p.q_t + h * p.q_h, true, q);
-    load(p.g, r * p.g_t + h * p.g_h, true, g);
-    const float lse = lse_of(p, (int)r, h), slope = p.slopes != nullptr ? __ldg(p.slopes + h) : 0.0f;
-    constexpr int kTogether = VEC ? 4 : 1;  // keys whose rows are in flight
-    for (int i0 = 0; i0 < most; i0 += kTogether) {
-      uint4 k[kTogether], v[kTogether];
-      float2 s[kTogether];
-#pragma unroll
-      for (int u = 0; u < kTogether; ++u) {
-        const int64_t j = row.x + i0 + u;
-        const bool there = i0 + u < n;
-        s[u] = make_float2(0.0f, 0.0f);
-        if constexpr (VEC) {
-          k[u] = raw(p.k, j * p.k_t + hk * p.k_h, there);
-          v[u] = raw(p.v, j * p.v_t + hk * p.v_h, there);
-        } else if (there) {
-          const T *kj = static_cast<const T*>(p.k) + j * p.k_t + hk * p.k_h, *vj = static_cast<const T*>(p.v) + j * p.v_t + hk * p.v_h;
-#pragma unroll
-          for (int c = 0; c < kPer; ++c)
-            if (lane + c * LANES < p.D) {
-              s[u].x = fmaf(q[c], to_f32(kj[lane + c * LANES]), s[u].x);
-              s[u].y = fmaf(g[c], to_f32(vj[lane + c * LANES]), s[u].y);
-            }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kTogether; ++u) {
-        if constexpr (VEC) {
-          float x[8], y[8];
-          widen(k[u], x);
-          widen(v[u], y);
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            s[u].x = fmaf(q[c], x[c], s[u].x);
-            s[u].y = fmaf(g[c], y[c], s[u].y);
-          }
-        }
-        s[u] = lanes_sum<LANES>(s[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < kTogether; ++u)
-        if (i0 + u < n) total = fmaf(exp2_fast(score_of(p, s[u].x, row.z, row.x + i0 + u, slope, slant) - lse), s[u].y, total);
-    }
-    if (lane == 0) p.delta[(int64_t)h * p.Tq + r] = total;
-  }
-}
-
 // ------------------------------------------------------- tensor-core helpers
 constexpr int kBlock = 64;    // of the other side that a step takes
 
@@ -688,6 +598,10 @@ __device__ __forceinline__ void tmem_get16(uint32_t taddr, uint32_t* r) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_put8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -1526,6 +1440,12 @@ __global__ void __launch_bounds__(256) few_join_kernel(const __grid_constant__ P
 //
 //   S = A1 B1^T   dP = A2 B2^T   p = exp(s - lse)   e = p (dP - delta) (1 - tanh^2)   acc += e B1   [dv += p B2]
 //
+// delta_i = sum_j p_ij dP_ij.  As dO_i . out_i, which delta_kernel has, it is off by what rounding `out` left off, and where
+// few keys hold a row's weight dP - delta is a small difference beside that (dq and dk of such rows had no right digit).
+// The queries' kernel comes first and sums what it is off by: d_i = sum_j p_ij (dP_ij - delta_i), and with it
+// dq_i = acc_i - d_i sum_j p_ij (1 - tanh^2)_ij k_j, whose last sum is its second accumulator (of p rounded once: d is
+// small).  delta_i + d_i is what the keys' kernel gets.
+//
 // seven products for both where one kernel that adds dq by atomics has five.  p and e go to the second products as two
 // values of the type each, out of TMEM: what they are rounded to, and what is left, rounded.  (With the first alone dq, dk
 // and dv are 1.3 to 1.4 times as far from the exact sums, 2.4e-3 for 1.7e-3 in bf16.)  In fp16 they are brought into the
@@ -1549,9 +1469,9 @@ struct Backward {
   // TMEM: S, dP, then the sums; the 16-bit values beside them (the next S and dP are then computed meanwhile) or in
   // place of S and dP, where two CTAs of 256 columns leave no room
   static constexpr int kAccAt = 128, kAcc2At = 128 + DP;
-  static constexpr bool kApart = !(DP == 64 && KEYS);
-  static constexpr int kEAt = !kApart ? 64 : KEYS ? kAcc2At + DP : kAcc2At;
-  static constexpr int kPAt = kApart ? kEAt + 64 : 0;     // (KEYS)
+  static constexpr bool kApart = DP != 64;
+  static constexpr int kEAt = kApart ? kAcc2At + DP : 64;
+  static constexpr int kPAt = kApart ? kEAt + 64 : 0;
   static constexpr int kStride = 16;                      // sixteen of p or e as they are rounded, then what is left of them
   static constexpr int kTmemCols = DP == 64 ? 256 : 512;
 };
@@ -1583,6 +1503,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   __shared__ __align__(16) float s_lse[2][KEYS ? kBlock : 4], s_delta[2][KEYS ? kBlock : 4];
   __shared__ int4 s_row[2][KEYS ? kBlock : 1];
   __shared__ Span s_span[2][2];
+  __shared__ float s_off[KEYS ? 1 : C::kSets][KEYS ? 1 : kTile];  // (queries) what delta is off by, of a set's columns
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // (KEYS) blockIdx.z: one of the heads that share the key head, where there are parts; else all of them
@@ -1694,10 +1615,8 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
         const uint32_t b1 = columns_desc(b1_at + held.slot * C::kBBytes, kBlock * 128), b2 = columns_desc(b2_at + held.slot * C::kBBytes, kBlock * 128);
 #pragma unroll
         for (int i = 0; i < kBlock / 16; ++i) {
-          if (KEYS) {
-            mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + C::kStride * i, b2 + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
-            mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + C::kStride * i + 8, b2 + i * (16 * 128 / 16), idesc, true);
-          }
+          mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + C::kStride * i, (KEYS ? b2 : b1) + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
+          if (KEYS) mma_ts(tmem + C::kAcc2At, tmem + C::kPAt + C::kStride * i + 8, b2 + i * (16 * 128 / 16), idesc, true);
           mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kStride * i, b1 + i * (16 * 128 / 16), idesc, n > 0 || i > 0);
           mma_ts(tmem + C::kAccAt, tmem + C::kEAt + C::kStride * i + 8, b1 + i * (16 * 128 / 16), idesc, true);
         }
@@ -1717,6 +1636,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
     const float unit = p.cap > 0.0f ? p.cap * kLog2e : p.scale * kLog2e;
     float slope2 = 0.0f, lse = 0.0f, delta = 0.0f;
+    F2 off = f2(0.0f, 0.0f);
     Span reach{};
     if (!KEYS) reach = span_of(row);
     if (!KEYS) {
@@ -1764,7 +1684,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
         const Seen seen = KEYS ? s_span[n & 1][c0 / kHalf].of(span.x + quarter * 32) : reach.of(o0 + c0, C::kPart);
         uint32_t w[C::kPart], e[C::kPart];
         if (seen != kNone) {
-          uint32_t x[C::kPart], y[C::kPart];
+          uint32_t x[C::kPart], y[C::kPart], slant[KEYS ? 1 : C::kPart];
           tmem_get16(mine + c0, x);
           tmem_get16(mine + 64 + c0, y);
           tmem_wait_ld();
@@ -1772,7 +1692,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
             tc::tc_fence_before();
             warp_arrive(&sfree);
           }
-          // y: (dP - delta) times the slant; x: the score in units of log 2 (over `unit`)
+          // y: dP - delta (KEYS: times the slant 1 - tanh^2); x: the score in units of log 2 (over `unit`)
 #pragma unroll
           for (int c = 0; c < C::kPart; c += 2) {
             const F2 d = KEYS ? *reinterpret_cast<const F2*>(&s_delta[n & 1][c0 + c]) : f2(-delta, -delta);
@@ -1791,7 +1711,9 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
               const F2 th = fma2(f2(rcp_fast(d.x), rcp_fast(d.y)), minus, one);
               const float2 t = un(th);
               put(x + c, th);
-              put(y + c, mul2(pair(y + c), fma2(f2(-t.x, -t.y), th, one)));
+              const F2 sl = fma2(f2(-t.x, -t.y), th, one);
+              if (KEYS) put(y + c, mul2(pair(y + c), sl));
+              else put(slant + c, sl);
             }
           }
           if (slope2 != 0.0f) {
@@ -1814,14 +1736,28 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
               }
             }
           }
+          auto weigh = [&](auto capped) {
 #pragma unroll
-          for (int c = 0; c < C::kPart; c += 2) {
-            const F2 l = KEYS ? *reinterpret_cast<const F2*>(&s_lse[n & 1][c0 + c]) : f2(-lse, -lse);
-            const float2 v = un(fma2(f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), f2(left, left), l));
-            const float a = exp2_fast(v.x), b = exp2_fast(v.y);
-            if (KEYS) two_values<T>(f2(a, b), w[c / 2], w[C::kPart / 2 + c / 2]);
-            two_values<T>(mul2(f2(a, b), pair(y + c)), e[c / 2], e[C::kPart / 2 + c / 2]);
-          }
+            for (int c = 0; c < C::kPart; c += 2) {
+              const F2 l = KEYS ? *reinterpret_cast<const F2*>(&s_lse[n & 1][c0 + c]) : f2(-lse, -lse);
+              const float2 v = un(fma2(f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), f2(left, left), l));
+              F2 a = f2(exp2_fast(v.x), exp2_fast(v.y)), g = mul2(a, pair(y + c));
+              if constexpr (KEYS) {
+                two_values<T>(a, w[c / 2], w[C::kPart / 2 + c / 2]);
+              } else {
+                off = add2(off, g);
+                if constexpr (decltype(capped)::value) {
+                  a = mul2(a, pair(slant + c));
+                  g = mul2(g, pair(slant + c));
+                }
+                const float2 f = un(a);
+                w[c / 2] = pack2<T>(f.x, f.y);
+              }
+              two_values<T>(g, e[c / 2], e[C::kPart / 2 + c / 2]);
+            }
+          };
+          if (!KEYS && p.cap > 0.0f) weigh(std::true_type());
+          else weigh(std::false_type());
         } else {
 #pragma unroll
           for (int c = 0; c < C::kPart; ++c) w[c] = e[c] = 0u;
@@ -1836,6 +1772,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
         }
         if (ok) {
           if (KEYS) tmem_put16(mine + C::kPAt + c0 / C::kPart * C::kStride, w);
+          else tmem_put8(mine + C::kPAt + c0 / C::kPart * C::kStride, w);
           tmem_put16(mine + C::kEAt + c0 / C::kPart * C::kStride, e);
         }
       }
@@ -1854,11 +1791,21 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
       ok = wait_on(&done, (uint32_t)(blocks - 1) & 1u, kWaitTimeoutEpilogue, abort_flag);
       tc::tc_fence_after();
     }
+    if constexpr (!KEYS) {
+      const float2 both = un(off);
+      s_off[set][quarter * 32 + lane] = both.x + both.y;
+    }
     ok = meet(ok);
     // a row that is not finite is taken again by itself; the sums' columns are shared by the sets
     const float down = up != 0 ? 0x1p-15f : 1.0f, w1 = p.scale * down / sigma;
     const int64_t at = ((int64_t)r * (KEYS ? p.Hk : p.H) + head) * p.D;
     const bool mine_too = KEYS || row.y > row.x, there = r < span.y;
+    float d = 0.0f;  // what delta is off by, as p and dP are scaled
+    if constexpr (!KEYS) {
+      for (int i = 0; i < C::kSets; ++i) d += s_off[i][quarter * 32 + lane];
+      d *= down;
+      if (ok && set == 0 && there && mine_too) p.delta[(int64_t)head * p.Tq + r] = (delta + d) / sigma;
+    }
     if (ok) {
       bool bad = false;
       for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
@@ -1871,6 +1818,13 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
           if (blocks > 0) {
             tmem_get32(mine + (which ? C::kAcc2At : C::kAccAt) + c, o);
             tmem_wait_ld();
+          }
+          if (!KEYS && blocks > 0) {
+            uint32_t k[32];
+            tmem_get32(mine + C::kAcc2At + c, k);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(-d, __uint_as_float(k[i]), __uint_as_float(o[i])));
           }
           if (blocks == 0 || !mine_too) {
 #pragma unroll
@@ -2140,28 +2094,19 @@ static int backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
     else if (lanes == 16) delta_kernel<T, 16, true><<<grid, 256, 0, st>>>(p);
     else delta_kernel<T, 8, true><<<grid, 256, 0, st>>>(p);
     if ((rc = check_cuda(cudaGetLastError(), "attention delta_kernel launch"))) return rc;
-    if (p.Tq > 0 && p.Tk > 0) {
-      const bool whole = vec && mappable(p.q, p.Tq, p.H, p.q_t, p.q_h) && mappable(p.k, p.Tk, p.Hk, p.k_t, p.k_h);
-      const dim3 near((unsigned)std::max(((int64_t)p.Tq + 31) / 32, std::min<int64_t>(p.Tq, (int64_t)sm_count() * 4)));
-      void* args[] = {&p};
-      rc = !whole        ? launch(near_kernel<T, 32, false>, near, 256, 0, true, st, "attention near_kernel launch", args)
-           : lanes == 32 ? launch(near_kernel<T, 32, true>, near, 256, 0, true, st, "attention near_kernel launch", args)
-           : lanes == 16 ? launch(near_kernel<T, 16, true>, near, 256, 0, true, st, "attention near_kernel launch", args)
-                         : launch(near_kernel<T, 8, true>, near, 256, 0, true, st, "attention near_kernel launch", args);
-      if (rc) return rc;
-    }
   }
   if (tiles) {
+    // the queries first: they give the keys their delta
     p.parts = key_parts(p.Tk, p.S, p.H, p.Hk);
-    if ((rc = p.D <= 64 ? run_backward<T, 64, true>(p, dt, st) : run_backward<T, 128, true>(p, dt, st))) return rc;
-    return p.D <= 64 ? run_backward<T, 64, false>(p, dt, st) : run_backward<T, 128, false>(p, dt, st);
+    if ((rc = p.D <= 64 ? run_backward<T, 64, false>(p, dt, st) : run_backward<T, 128, false>(p, dt, st))) return rc;
+    return p.D <= 64 ? run_backward<T, 64, true>(p, dt, st) : run_backward<T, 128, true>(p, dt, st);
   }
   void* args[] = {&p};
-  if (p.Tk > 0 && (rc = launch(row_kernel<T, kRowDkv>, dim3((unsigned)(((int64_t)p.Tk * p.Hk + 7) / 8)), 256, 0, false, st,
+  if (p.Tq > 0 && (rc = launch(row_kernel<T, kRowDq>, dim3((unsigned)(((int64_t)p.Tq * p.H + 7) / 8)), 256, 0, false, st,
                                "attention row_kernel launch", args)))
     return rc;
-  if (p.Tq == 0) return RB_OK;
-  return launch(row_kernel<T, kRowDq>, dim3((unsigned)(((int64_t)p.Tq * p.H + 7) / 8)), 256, 0, false, st,
+  if (p.Tk == 0) return RB_OK;
+  return launch(row_kernel<T, kRowDkv>, dim3((unsigned)(((int64_t)p.Tk * p.Hk + 7) / 8)), 256, 0, false, st,
                 "attention row_kernel launch", args);
 }
 

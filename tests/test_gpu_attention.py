@@ -536,3 +536,26 @@ def test_value_gradients_keep_their_bits(cuda_device, dtype, nq, nk, H, Hk, D, m
     val, loose = oracle(q, k, v, nq, nk, g=g, **mask)
     spread, _ = oracle(q, k, v, nq, nk, g=g.abs(), **mask)
     _close(dv, val["dv"], _few_bits(dtype, val["dv"], spread["dv"], loose["dv"]), dtype)
+
+
+@pytest.mark.parametrize("D,mask", [(64, {}), (64, dict(cap=50.0)), (128, {}), (128, dict(cap=40.0, causal=False)), (24, {}), (20, {}), (200, {})])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_gradients_where_one_key_has_the_weight(cuda_device, dtype, D, mask):
+    """Long rows whose weight lies on one key: dp - delta is a small difference there as in short rows, and dq and dk are as
+    near as their own rounding.  Beside `near`'s bound: the first delta is off by half of out at most, and that times
+    sum p |k|, whose p is rounded once, is what the correction of dq is off by."""
+    from baidu_cti_grab_b200 import device_ops
+
+    nq, H = [300, 41, 700], 2
+    q, k, v, g = _inputs(nq, nq, H, H, D, dtype, D, cuda_device)
+    q = (1.5 * (64 / D) ** 0.25 * k.float()).to(dtype)
+    off = _offsets(nq, torch.int32, cuda_device)
+    out, lse = device_ops.segment_attention(q, k, v, off, want_lse=True, **mask)
+    grads = device_ops.segment_attention_backward(g, q, k, v, out, lse, off, **mask)
+    half = torch.finfo(dtype).eps / 2
+    val, tol = oracle(q, k, v, nq, nq, g=g, half=half, fp16=dtype is HF, near=True, **mask)
+    reach, _ = oracle(q, k, k.abs(), nq, nq, **mask)
+    first = (g.double().abs() * val["out"].abs()).sum(-1, keepdim=True) * half * (1 + 2.0 ** -6)
+    tol["dq"] += D ** -0.5 * half * first * reach["out"]
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        _close(got, val[name], tol[name], dtype)
