@@ -26,6 +26,15 @@ class SparseRows(NamedTuple):
     count: torch.Tensor   # int32 [1], on the device
 
 
+def _padding_row(padding_idx: Optional[int], rows: int) -> Optional[int]:
+    """padding_idx as a row of the table: one below 0 counts from its end, as torch's does."""
+    if padding_idx is None:
+        return None
+    if not -rows <= padding_idx < max(rows, 1):
+        raise ValueError(f"padding_idx must be a row of the table's {rows}, or count from its end")
+    return padding_idx + rows if padding_idx < 0 else padding_idx
+
+
 class _Embed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale, padding_idx):
@@ -42,7 +51,8 @@ class _Embed(torch.autograd.Function):
 
 def embed(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """scale * table[ids] [*ids.shape, D], with the table's gradient; the row of padding_idx is looked up as it is and gets
-    no gradient.  Ids are clamped to the table, as the RepEncoder clamps them."""
+    no gradient.  Ids are clamped to the table, as the RepEncoder clamps them; a padding_idx below 0 counts from its end."""
+    padding_idx = _padding_row(padding_idx, table.shape[0])
     if torch.is_grad_enabled() and table.requires_grad:
         return _Embed.apply(table, ids, scale, padding_idx)
     return device_ops.embed_rows(table, ids, scale=scale)
@@ -54,7 +64,7 @@ def bag_gradient(grad: torch.Tensor, ids: torch.Tensor, bags: torch.Tensor, rows
 
     Ids of padding_idx (row 0, as the RepEncoder has it) add nothing.  A tensor [rows, D], added to `out` where that is
     given, or SparseRows."""
-    how = dict(bags=bags, scale=scale, padding_idx=padding_idx)
+    how = dict(bags=bags, scale=scale, padding_idx=_padding_row(padding_idx, rows))
     if not sparse:
         return device_ops.embed_rows_backward(grad, ids, rows, out=out, **how)
     if out is not None:
@@ -67,10 +77,10 @@ class RowEmbedding(nn.Module):
 
     def __init__(self, rows: int, width: int, *, scale: float = 1.0, padding_idx: Optional[int] = None, std: float = 0.02):
         super().__init__()
-        self.scale, self.padding_idx = scale, padding_idx
+        self.scale, self.padding_idx = scale, _padding_row(padding_idx, rows)
         weight = torch.randn(rows, width) * std
         if padding_idx is not None:
-            weight[padding_idx] = 0.0
+            weight[self.padding_idx] = 0.0
         self.weight = nn.Parameter(weight)
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
