@@ -931,6 +931,10 @@ def segment_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Ten
 
 
 # ------------------------------------------- embedding rows and their gradient
+# A kernel wrote into a caller's tensors: autograd's check that what it saved is unchanged has to know.
+_written = torch.autograd.graph.increment_version
+
+
 def embed_rows(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
     """scale * table[ids] (rb_embed_rows): table [V, D] fp32/bf16/f16 with contiguous rows, ids int32/int64 of any
     shape, clamped to [0, V - 1].  Returns [*ids.shape, D] in the table's type."""
@@ -1002,6 +1006,8 @@ def embed_rows_backward(grad: torch.Tensor, ids: torch.Tensor, rows: int, *, bag
     _call_on(dev, "rb_embed_rows_backward", grad.data_ptr(), _DT[grad.dtype], ld, D, ids.data_ptr(), _INDEX[ids.dtype], n, rows,
              _ptr(bags), n_bags, padding, float(scale), given, ws.data_ptr(), ws_bytes, out.data_ptr(), _DT[out.dtype],
              max(out.stride(0), D))
+    if given:
+        _written(out)
     return out
 
 
@@ -1016,7 +1022,8 @@ def embed_rows_backward_sparse(grad: torch.Tensor, ids: torch.Tensor, rows: int,
     name = "embed_rows_backward_sparse"
     dev, grad, ld, D, ids, bags, n_bags, padding = _embed_grad_args(name, grad, ids, rows, bags, padding_idx)
     n = ids.numel()
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((n,), dtype=torch.int64, device=dev), torch.empty((n, D), dtype=grad.dtype, device=dev)
     out_ids, out_rows = out
     _device_of(name, grad, out_ids, out_rows)
@@ -1031,6 +1038,8 @@ def embed_rows_backward_sparse(grad: torch.Tensor, ids: torch.Tensor, rows: int,
     _call_on(dev, "rb_embed_rows_backward_sparse", grad.data_ptr(), _DT[grad.dtype], ld, D, ids.data_ptr(), _INDEX[ids.dtype], n,
              rows, _ptr(bags), n_bags, padding, float(scale), ws.data_ptr(), ws_bytes, out_ids.data_ptr(), out_rows.data_ptr(),
              _DT[out_rows.dtype], max(out_rows.stride(0), D), count.data_ptr())
+    if given:
+        _written((out_ids, out_rows))
     return out_ids, out_rows, count
 
 
@@ -1115,6 +1124,8 @@ def _clip(name: str, grads, most: float, out, scale: float) -> torch.Tensor:
     ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
     lists = [None if a is None else a.buffer_info()[0] for a in (ptrs, to, sizes, types, counted, widths)]
     _call_on(dev, "rb_clip_grads", *lists, n, float(scale), float(most), ws.data_ptr(), ws_bytes, norm.data_ptr())
+    if clip:
+        _written(tensors if out is None else out)
     for copy, t in back:
         t.copy_(copy)
     return norm

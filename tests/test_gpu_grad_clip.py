@@ -167,3 +167,23 @@ def test_streams_graphs_and_training(cuda_device):
     assert abs(float(n) - norm) <= 7 * U * norm
     _check([layer.weight.grad, layer.bias.grad, sparse.rows[:m]], before, norm, 0.1 * norm)
     assert float(grad_clip.clip_grad_norm([unused], 1.0)) == 0.0
+
+
+def test_clipped_tensors_count_as_modified(cuda_device):
+    """Autograd refuses a backward pass over a saved tensor that was clipped since; the norm alone modifies nothing."""
+    from baidu_cti_grab_b200 import device_ops
+
+    w = torch.ones(40, device=cuda_device, requires_grad=True)
+    saved = torch.ones(40, device=cuda_device)
+    y = (w * saved).sum()
+    device_ops.grad_norm([saved])
+    assert saved._version == 0
+    device_ops.clip_grads([saved], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    out = [torch.empty_like(saved)]
+    device_ops.clip_grads([saved], 1.0, out=out)
+    assert out[0]._version == 1 and saved._version == 1
+    rows, count = torch.ones(6, 4, device=cuda_device), torch.tensor([3], dtype=torch.int32, device=cuda_device)
+    device_ops.clip_grads([(rows, count)], 1.0)
+    assert rows._version == 1

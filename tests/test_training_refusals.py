@@ -113,3 +113,15 @@ def test_c_entries_refuse():
     assert lib.rb_embed_rows_backward_workspace_size(-1, 8) == -1
     assert lib.rb_embed_rows_backward_workspace_size(0, 8) == 0
     assert lib.rb_grad_norm_workspace_size(-1) == -1
+
+
+def test_what_a_kernel_writes_counts_as_modified(calls):
+    """Autograd refuses a backward pass over a saved tensor that was written since: by torch, or by these calls."""
+    from baidu_cti_grab_b200 import device_ops as d
+
+    out, grad = torch.zeros(5, 8, dtype=torch.bfloat16), torch.zeros(3, 8)
+    d.embed_rows_backward(grad, IDS, 5, out=out)
+    assert out._version == 1
+    pair = torch.zeros(3, dtype=torch.int64), torch.zeros(3, 8)
+    d.embed_rows_backward_sparse(grad, IDS, 5, out=pair)
+    assert [t._version for t in pair] == [1, 1]
