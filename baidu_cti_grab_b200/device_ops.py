@@ -863,7 +863,9 @@ def _attention_args(name, q, k, v, offsets, k_offsets, causal, prefix, slopes, c
     if prefix is not None:
         if prefix.shape != (S,) or prefix.dtype not in _INDEX:
             raise ValueError(f"prefix must be int32 or int64 [{S}]")
-        prefix = prefix.to(offsets.dtype).contiguous()
+        if prefix.dtype is not offsets.dtype:  # (what int32 cannot hold is more than any segment has)
+            prefix = prefix.clamp(0, 2 ** 31 - 1).to(offsets.dtype)
+        prefix = prefix.contiguous()
     if slopes is not None:
         if slopes.shape != (H,) or slopes.dtype is not torch.float32:
             raise ValueError(f"slopes must be fp32 [{H}]")

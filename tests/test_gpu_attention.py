@@ -559,3 +559,18 @@ def test_gradients_where_one_key_has_the_weight(cuda_device, dtype, D, mask):
     tol["dq"] += D ** -0.5 * half * first * reach["out"]
     for name, got in zip(("dq", "dk", "dv"), grads):
         _close(got, val[name], tol[name], dtype)
+
+
+def test_prefix_of_another_type_than_the_offsets(cuda_device):
+    """A prefix beyond int32 is all of a segment's keys, whatever the offsets' type; one below 0 is none."""
+    from baidu_cti_grab_b200 import device_ops
+
+    nq = [40, 30, 50]
+    q, k, v, _ = _inputs(nq, nq, 2, 2, 64, BF, 3, cuda_device)
+    all_of = torch.tensor([1 << 32, (1 << 40) + 1, -(1 << 33) + 5], device=cuda_device)
+    want, _ = device_ops.segment_attention(q, k, v, _offsets(nq, torch.int64, cuda_device), prefix=all_of)
+    got, _ = device_ops.segment_attention(q, k, v, _offsets(nq, torch.int32, cuda_device), prefix=all_of)
+    small, _ = device_ops.segment_attention(q, k, v, _offsets(nq, torch.int32, cuda_device), prefix=torch.tensor([40, 30, 0], device=cuda_device))
+    assert torch.equal(got, want) and torch.equal(got, small)
+    val, tol = oracle(q, k, v, nq, nq, prefix=[40, 30, 0], half=2.0 ** -8)
+    _close(got, val["out"], tol["out"], BF)
