@@ -105,6 +105,12 @@ __device__ __forceinline__ float rcp_fast(float x) {
 // tanh from exp: 1 - 2 / (1 + e^2x).  Near 0 it is off by 2^-23 of 1, not of x: in the score that is 2^-23 cap, where
 // the hardware's own tanh is off by 2^-11 of x.
 __device__ __forceinline__ float tanh_of(float x) { return fmaf(-2.0f, rcp_fast(1.0f + exp2_fast(x * (2.0f * kLog2e))), 1.0f); }
+// 1 - tanh^2: with w = e^-2|x| and m = 2 w / (1 + w) = 1 - |tanh| it is m (2 - m), right to a few 2^-24 of itself however
+// near to 1 the tanh is (1 - t t is off by 2^-23 of 1)
+__device__ __forceinline__ float slant_of(float x) {
+  const float w = exp2_fast(-fabsf(x) * (2.0f * kLog2e)), m = 2.0f * w * rcp_fast(1.0f + w);
+  return m * (2.0f - m);
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -197,9 +203,8 @@ __device__ __forceinline__ float score_of(const Params& p, float x, int place, i
   x *= p.scale;
   slant = 1.0f;
   if (p.cap > 0.0f) {
-    const float t = tanh_of(x / p.cap);
-    slant = fmaf(-t, t, 1.0f);
-    x = p.cap * t;
+    slant = slant_of(x / p.cap);
+    x = p.cap * tanh_of(x / p.cap);
   }
   return kLog2e * fmaf(-slope, (float)abs(place - j), x);
 }
@@ -1703,15 +1708,17 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
           float left = unit;
           if (p.cap > 0.0f) {
             const float in = p.scale / p.cap * (2.0f * kLog2e);
-            const F2 in2 = f2(in, in), one = f2(1.0f, 1.0f), minus = f2(-2.0f, -2.0f);
+            const F2 in2 = f2(in, in), one = f2(1.0f, 1.0f);
 #pragma unroll
-            for (int c = 0; c < C::kPart; c += 2) {
+            for (int c = 0; c < C::kPart; c += 2) {  // as slant_of has it, and the tanh 1 - m with x's sign
               const float2 v = un(mul2(pair(x + c), in2));
-              const float2 d = un(add2(f2(exp2_fast(v.x), exp2_fast(v.y)), one));
-              const F2 th = fma2(f2(rcp_fast(d.x), rcp_fast(d.y)), minus, one);
+              const F2 w = f2(exp2_fast(-fabsf(v.x)), exp2_fast(-fabsf(v.y)));
+              const float2 d = un(add2(w, one));
+              const F2 m = mul2(add2(w, w), f2(rcp_fast(d.x), rcp_fast(d.y))), th = sub2(one, m);
               const float2 t = un(th);
-              put(x + c, th);
-              const F2 sl = fma2(f2(-t.x, -t.y), th, one);
+              x[c] = __float_as_uint(copysignf(t.x, v.x));
+              x[c + 1] = __float_as_uint(copysignf(t.y, v.y));
+              const F2 sl = mul2(m, add2(th, one));
               if (KEYS) put(y + c, mul2(pair(y + c), sl));
               else put(slant + c, sl);
             }

@@ -574,3 +574,43 @@ def test_prefix_of_another_type_than_the_offsets(cuda_device):
     assert torch.equal(got, want) and torch.equal(got, small)
     val, tol = oracle(q, k, v, nq, nq, prefix=[40, 30, 0], half=2.0 ** -8)
     _close(got, val["out"], tol["out"], BF)
+
+
+@pytest.mark.parametrize("D", [16, 20, 72])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_gradients_of_saturated_scores(cuda_device, dtype, D):
+    """Scores of 4.5 to 8 caps: dk and dq follow 1 - tanh^2, 5e-4 to 5e-7, which has to keep its own precision.
+
+    1 - tanh(y)^2 changes by 2 of what y is off by; the rest as at the head of this file, delta as in `near`."""
+    from baidu_cti_grab_b200 import device_ops
+
+    n, m, cap = 96, 130, 0.5
+    gen = torch.Generator().manual_seed(D)
+    q, k, v, g = (torch.randn(r, 1, D, generator=gen) for r in (n, m, m, n))
+    q, k = 0.01 * q, 0.01 * k
+    q[..., 0] = 1.0
+    k[:, 0, 0] = torch.linspace(4.5, 8.0, m) * cap * (1 - 2 * (torch.arange(m) % 2))
+    q, k, v, g = (t.to(dtype).to(cuda_device) for t in (q, k, v, g))
+    off, k_off = _offsets([n], torch.int32, cuda_device), _offsets([m], torch.int32, cuda_device)
+    how = dict(causal=False, cap=cap, scale=1.0)
+    out, lse = device_ops.segment_attention(q, k, v, off, k_off, want_lse=True, **how)
+    dq, dk, _ = device_ops.segment_attention_backward(g, q, k, v, out, lse, off, k_off, **how)
+    Q, K, V, G = (t[:, 0].double() for t in (q, k, v, g))
+    x = Q @ K.t()
+    ds = 2 * D * U * (Q.abs() @ K.abs().t())
+    slant = 1 / torch.cosh(x / cap) ** 2
+    p = torch.softmax(cap * torch.tanh(x / cap), -1)
+    dp = G @ V.t()
+    delta = (p * dp).sum(-1, keepdim=True)
+    e = p * (dp - delta) * slant
+    half = torch.finfo(dtype).eps / 2
+    eta = torch.expm1(2 * (ds.amax(-1, keepdim=True) + 8 * U * cap)) + 8 * U
+    d_dp = 2 * D * U * (G.abs() @ V.abs().t())
+    first = half * (G.abs() * (p @ V).abs()).sum(-1, keepdim=True)  # the delta that dq is corrected from, p rounded once
+    d_delta = (p * dp.abs()).sum(-1, keepdim=True) * (eta + m * U) + (p * d_dp).sum(-1, keepdim=True)
+    d_e = e.abs() * (half * half + eta + 2 * (ds / cap + 4 * U * (x / cap).abs()) + 16 * U) + p * slant * (d_delta + d_dp)
+    if dtype is HF:
+        d_e = d_e + 2 * 2.0 ** -40 * 2 * G.norm(dim=-1).max() * V.norm(dim=-1).max()
+    for got, want, tol in ((dq, e @ K, (d_e + half * first * p * slant) @ K.abs() + m * U * (e.abs() @ K.abs())),
+                           (dk, e.t() @ Q, (d_e + n * U * e.abs()).t() @ Q.abs())):
+        _close(got[:, 0], want, tol + half * want.abs(), dtype)
