@@ -102,9 +102,19 @@ __device__ __forceinline__ float rcp_fast(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// tanh from exp: 1 - 2 / (1 + e^2x).  Near 0 it is off by 2^-23 of 1, not of x: in the score that is 2^-23 cap, where
-// the hardware's own tanh is off by 2^-11 of x.
+// tanh from exp: 1 - 2 / (1 + e^2x).  Near 0 it is off by 2^-22 of 1, not of x: in the score that is 2^-22 cap, where
+// the hardware's own tanh is off by 2^-11 of x.  Caps above kWideCap, for which that would be 2^-14 and more, take the
+// series below 1/4 (its next term is 2^-26 of x there), in tile kernels of their own (WIDE, of 128 columns for all widths):
+// as a branch of the others it cost those 2 to 5 % by its registers.
+constexpr float kWideCap = 256.0f;
 __device__ __forceinline__ float tanh_of(float x) { return fmaf(-2.0f, rcp_fast(1.0f + exp2_fast(x * (2.0f * kLog2e))), 1.0f); }
+__device__ __forceinline__ float tanh_wide(float x) {
+  const float z = x * x;
+  float s = fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f);
+  s = fmaf(z, s, 2.0f / 15.0f);
+  s = fmaf(z, s, -1.0f / 3.0f);
+  return z < 0.0625f ? fmaf(x * z, s, x) : tanh_of(x);
+}
 // 1 - tanh^2: with w = e^-2|x| and m = 2 w / (1 + w) = 1 - |tanh| it is m (2 - m), right to a few 2^-24 of itself however
 // near to 1 the tanh is (1 - t t is off by 2^-23 of 1)
 __device__ __forceinline__ float slant_of(float x) {
@@ -204,7 +214,7 @@ __device__ __forceinline__ float score_of(const Params& p, float x, int place, i
   slant = 1.0f;
   if (p.cap > 0.0f) {
     slant = slant_of(x / p.cap);
-    x = p.cap * tanh_of(x / p.cap);
+    x = p.cap * (p.cap > kWideCap ? tanh_wide(x / p.cap) : tanh_of(x / p.cap));
   }
   return kLog2e * fmaf(-slope, (float)abs(place - j), x);
 }
@@ -707,8 +717,13 @@ __device__ __forceinline__ void put(uint32_t* x, F2 v) {
   x[1] = __float_as_uint(f.y);
 }
 // scores in place of raw products, in units of log 2, of the 32 keys from j on
+template <bool WIDE>
 __device__ __forceinline__ void transform(const Params& p, uint32_t* raw, float slope2, int place, int j) {
-  if (p.cap > 0.0f) {  // cap tanh(y) = cap - 2 cap / (1 + e^2y), as tanh_of has it
+  if constexpr (WIDE) {
+    const float in = p.scale / p.cap, cap2 = p.cap * kLog2e;
+#pragma unroll
+    for (int c = 0; c < kHalf; ++c) raw[c] = __float_as_uint(cap2 * tanh_wide(__uint_as_float(raw[c]) * in));
+  } else if (p.cap > 0.0f) {  // cap tanh(y) = cap - 2 cap / (1 + e^2y), as tanh_of has it
     const float in = p.scale / p.cap * (2.0f * kLog2e), cap2 = p.cap * kLog2e;
     const F2 in2 = f2(in, in), one = f2(1.0f, 1.0f), base = f2(cap2, cap2), minus = f2(-2.0f * cap2, -2.0f * cap2);
 #pragma unroll
@@ -762,7 +777,7 @@ struct Item {
   int r0, r1, head, key0, blocks, unit;  // blocks 0: no more; unit: the ticket
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool WIDE>
 __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
     forward_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
@@ -984,7 +999,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
         tc::tc_fence_after();
         float high = -INFINITY;
         auto prepare = [&](uint32_t* x, int j, Seen seen) {  // scores of 32 keys, and their maximum
-          if (!plain) transform(p, x, slope2, row.z, j);
+          if (!plain) transform<WIDE>(p, x, slope2, row.z, j);
           if (seen == kSome) {
             const int lo = row.x - j, len = max(row.y - row.x, 0);
 #pragma unroll
@@ -1286,7 +1301,8 @@ __global__ void __launch_bounds__(Few<DP>::kThreads, Few<DP>::kCtas)
           for (int c = 0; c < 4; ++c) {
             const int i = c >> 1, j = j0 + 8 * e + 2 * q4 + (c & 1);
             float v = x[e][c];
-            if (p.cap > 0.0f) v = p.cap * kLog2e * tanh_of(v * (p.scale / p.cap));
+            if (p.cap > kWideCap) v = p.cap * kLog2e * tanh_wide(v * (p.scale / p.cap));
+            else if (p.cap > 0.0f) v = p.cap * kLog2e * tanh_of(v * (p.scale / p.cap));
             else v *= unit;
             v = fmaf(-slope2[i], (float)abs(mine[i].z - j), v);
             if (!every && !(j >= mine[i].x && j < mine[i].y)) v = -INFINITY;
@@ -1488,7 +1504,7 @@ __device__ __forceinline__ float range_of(const Params& p) {
   return bound > 0.0f && bound < INFINITY ? __uint_as_float((uint32_t)min(max(127 - e, 1), 254) << 23) : 1.0f;
 }
 
-template <typename T, int DP, bool KEYS>
+template <typename T, int DP, bool KEYS, bool WIDE>
 __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEYS>::kCtas)
     backward_kernel(const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmA2,
                     const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmB2,
@@ -1706,7 +1722,16 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
             y[c + 1] = __float_as_uint(v.y);
           }
           float left = unit;
-          if (p.cap > 0.0f) {
+          if constexpr (WIDE) {
+            const float in = p.scale / p.cap;
+#pragma unroll
+            for (int c = 0; c < C::kPart; ++c) {
+              const float v = __uint_as_float(x[c]) * in, sl = slant_of(v);
+              x[c] = __float_as_uint(tanh_wide(v));
+              if (KEYS) y[c] = __float_as_uint(__uint_as_float(y[c]) * sl);
+              else slant[c] = __float_as_uint(sl);
+            }
+          } else if (p.cap > 0.0f) {
             const float in = p.scale / p.cap * (2.0f * kLog2e);
             const F2 in2 = f2(in, in), one = f2(1.0f, 1.0f);
 #pragma unroll
@@ -1956,7 +1981,7 @@ static bool choose_by_segment(int64_t Tq, int64_t Tk, int64_t S, int heads) {
 
 static int tiles_of(int64_t T, int64_t S, bool by_segment) { return (int)(by_segment ? T / kTile + S + 2 : (T + kTile - 1) / kTile); }
 
-template <typename T, int DP>
+template <typename T, int DP, bool WIDE>
 static int run_forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   using C = Forward<DP>;
   static std::once_flag once[64];
@@ -1964,7 +1989,7 @@ static int run_forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   cudaGetDevice(&dev);
   cudaError_t e = cudaSuccess;
   std::call_once(once[dev & 63], [&] {
-    e = cudaFuncSetAttribute(forward_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    e = cudaFuncSetAttribute(forward_kernel<T, DP, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
   if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(attention forward_kernel)");
   CUtensorMap tmQ, tmK, tmV;
@@ -1973,7 +1998,7 @@ static int run_forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   if ((rc = make_map(&tmV, p.v, p.D, p.Hk, p.Tk, p.v_t, p.v_h, kBlock, dt))) return rc;
   const int64_t ctas = std::min<int64_t>((int64_t)p.n_tiles * p.H, (int64_t)sm_count() * C::kCtas);
   void* args[] = {&tmQ, &tmK, &tmV, &p};
-  return launch(forward_kernel<T, DP>, dim3((unsigned)ctas), C::kThreads, C::kSmem, true, st, "attention forward_kernel launch", args);
+  return launch(forward_kernel<T, DP, WIDE>, dim3((unsigned)ctas), C::kThreads, C::kSmem, true, st, "attention forward_kernel launch", args);
 }
 
 // How many parts the keys of a segment are split into where there are few queries, 0: not that kernel.  It reads a key
@@ -2034,7 +2059,8 @@ static int forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   plan_kernel<T><<<p.n_tiles, kTile, 0, st>>>(p);
   if ((rc = check_cuda(cudaGetLastError(), "attention plan_kernel launch"))) return rc;
   if (p.splits > 0) return p.D <= 64 ? run_few<T, 64>(p, dt, st) : run_few<T, 128>(p, dt, st);
-  if (tiles) return p.D <= 64 ? run_forward<T, 64>(p, dt, st) : run_forward<T, 128>(p, dt, st);
+  if (tiles && p.cap > kWideCap) return run_forward<T, 128, true>(p, dt, st);
+  if (tiles) return p.D <= 64 ? run_forward<T, 64, false>(p, dt, st) : run_forward<T, 128, false>(p, dt, st);
   void* args[] = {&p};
   return launch(row_kernel<T, kRowForward>, dim3((unsigned)(((int64_t)p.Tq * p.H + 7) / 8)), 256, 0, true, st,
                 "attention row_kernel launch", args);
@@ -2050,7 +2076,7 @@ static bool key_parts(int64_t Tk, int64_t S, int H, int Hk) {
   return 2 * tiles < sm || (tiles < 2 * sm && Tk >= 1024 * S);
 }
 
-template <typename T, int DP, bool KEYS>
+template <typename T, int DP, bool KEYS, bool WIDE>
 static int run_backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   using C = Backward<DP, KEYS>;
   static std::once_flag once[64];
@@ -2058,7 +2084,7 @@ static int run_backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   cudaGetDevice(&dev);
   cudaError_t e = cudaSuccess;
   std::call_once(once[dev & 63], [&] {
-    e = cudaFuncSetAttribute(backward_kernel<T, DP, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    e = cudaFuncSetAttribute(backward_kernel<T, DP, KEYS, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
   if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(attention backward_kernel)");
   const int q_rows = KEYS ? kBlock : kTile, k_rows = KEYS ? kTile : kBlock;
@@ -2069,7 +2095,7 @@ static int run_backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   if ((rc = make_map(&v, p.v, p.D, p.Hk, p.Tk, p.v_t, p.v_h, k_rows, dt))) return rc;
   const int tiles = KEYS ? p.n_key_tiles : p.n_tiles;
   void* args[] = {KEYS ? &k : &q, KEYS ? &v : &g, KEYS ? &q : &k, KEYS ? &g : &v, &p};
-  if ((rc = launch(backward_kernel<T, DP, KEYS>, dim3((unsigned)tiles, KEYS ? p.Hk : p.H, KEYS && p.parts ? p.G : 1), C::kThreads, C::kSmem,
+  if ((rc = launch(backward_kernel<T, DP, KEYS, WIDE>, dim3((unsigned)tiles, KEYS ? p.Hk : p.H, KEYS && p.parts ? p.G : 1), C::kThreads, C::kSmem,
                    true, st, "attention backward_kernel launch", args)))
     return rc;
   if (!KEYS || !p.parts) return RB_OK;
@@ -2105,8 +2131,12 @@ static int backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   if (tiles) {
     // the queries first: they give the keys their delta
     p.parts = key_parts(p.Tk, p.S, p.H, p.Hk);
-    if ((rc = p.D <= 64 ? run_backward<T, 64, false>(p, dt, st) : run_backward<T, 128, false>(p, dt, st))) return rc;
-    return p.D <= 64 ? run_backward<T, 64, true>(p, dt, st) : run_backward<T, 128, true>(p, dt, st);
+    if (p.cap > kWideCap) {
+      if ((rc = run_backward<T, 128, false, true>(p, dt, st))) return rc;
+      return run_backward<T, 128, true, true>(p, dt, st);
+    }
+    if ((rc = p.D <= 64 ? run_backward<T, 64, false, false>(p, dt, st) : run_backward<T, 128, false, false>(p, dt, st))) return rc;
+    return p.D <= 64 ? run_backward<T, 64, true, false>(p, dt, st) : run_backward<T, 128, true, false>(p, dt, st);
   }
   void* args[] = {&p};
   if (p.Tq > 0 && (rc = launch(row_kernel<T, kRowDq>, dim3((unsigned)(((int64_t)p.Tq * p.H + 7) / 8)), 256, 0, false, st,

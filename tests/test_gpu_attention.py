@@ -614,3 +614,28 @@ def test_gradients_of_saturated_scores(cuda_device, dtype, D):
     for got, want, tol in ((dq, e @ K, (d_e + half * first * p * slant) @ K.abs() + m * U * (e.abs() @ K.abs())),
                            (dk, e.t() @ Q, (d_e + n * U * e.abs()).t() @ Q.abs())):
         _close(got[:, 0], want, tol + half * want.abs(), dtype)
+
+
+@pytest.mark.parametrize("nq,nk,H,Hk,D", [([200, 65], None, 2, 1, 64), ([130], None, 2, 2, 128), ([2, 1], [900, 1500], 4, 1, 64),
+                                          ([60], None, 1, 1, 20)])
+@pytest.mark.parametrize("cap", [300.0, 1e5, 1e30])
+def test_caps_far_above_the_scores(cuda_device, cap, nq, nk, H, Hk, D):
+    """A cap that no score comes near changes nothing: a score is off by 16 u of itself, however large the cap is (and by
+    x^3 / 3 cap^2 from x, which the definition has too)."""
+    from baidu_cti_grab_b200 import device_ops
+
+    nk = nq if nk is None else nk
+    q, k, v, g = _inputs(nq, nk, H, Hk, D, HF, D, cuda_device)
+    off, k_off = _offsets(nq, torch.int32, cuda_device), _offsets(nk, torch.int32, cuda_device)
+    out, lse = device_ops.segment_attention(q, k, v, off, k_off, want_lse=True, cap=cap)
+    grads = device_ops.segment_attention_backward(g, q, k, v, out, lse, off, k_off, cap=cap)
+    val, _ = oracle(q, k, v, nq, nk, g=g, cap=cap)
+    spread, _ = oracle(q, k, v.abs(), nq, nk, cap=cap)
+    _, loose = oracle(q, k, v, nq, nk, g=g, half=2.0 ** -11, fp16=True)
+    _, bare = oracle(q, k, v, nq, nk)
+    more = 2.0 ** -18  # 2 (16 u) |x|, of scores under 8: exp's argument and the sum's
+    assert float(val["lse"].abs().max()) < 16
+    _close(out, val["out"], _few_bits(HF, val["out"], spread["out"], bare["out"] + more * spread["out"]), HF)
+    _close(lse, val["lse"], bare["lse"] + more, torch.float32)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        _close(got, val[name], loose[name], HF)
