@@ -38,10 +38,12 @@ struct Params {
   const void *q, *k, *v, *o, *g;  // o, g: the forward call's output and the gradient it got
   void *out, *dq, *dk, *dv;
   float* lse;                     // [H, Tq] log of the sum of exp(s), -inf where nothing is seen
-  float* delta;                   // [H, Tq] dout . out, then (behind the queries' gradients) the sum of p dp
-  int4* rows;                     // [Tq]: lo, hi, place of the query among the packed keys, 0
+  float* delta;                   // [H, Tq] dout . out, then (behind the queries' gradients) the sum of p dp; in fp16, from
+                                  // the tiles, times range_of
+  int4* rows;                     // [Tq]: lo, hi, place of the query among the packed keys, segment (-1: in none)
   int4* tiles;                    // of the queries: rows [x, y), the keys that they see [z, w)
   int4* key_tiles;                // (backward) of the keys: rows [x, y), queries that may see them [z, w)
+  int32_t* key_segments;          // (fp16 backward) [Tk]: of the keys, -1: in none
   uint32_t* next;                 // tickets for work
   int2* redo;                     // (forward tiles) [tiles x heads][4]: rows of 32 to be taken again, the entry before it
   float* part;                    // few queries: of every row and split, the sums [D], their maximum and their weights' sum
@@ -51,7 +53,7 @@ struct Params {
   int64_t q_t, q_h, k_t, k_h, v_t, v_h, g_t, g_h;  // elements from token to token and from head to head
   int Tq, Tk, S, H, Hk, G, D, off64, causal;
   float scale, cap;
-  uint32_t* peaks;                // fp16 backward: the largest norms of a row of g and of v
+  uint32_t* peaks;                // fp16 backward: [S, Hk] the largest squared norms of a row of g and of v
   int by_segment, n_tiles;        // tiles follow segments (else: 128 rows of the packed order)
   int keys_by_segment, n_key_tiles;
 };
@@ -76,9 +78,9 @@ __device__ __forceinline__ int segment_of(const void* off, int wide, int S, int 
 
 __device__ __forceinline__ int4 row_of(const Params& p, int r) {
   const int s = segment_of(p.q_off, p.off64, p.S, p.Tq, r);
-  if (s < 0) return make_int4(0, 0, 0, 0);
+  if (s < 0) return make_int4(0, 0, 0, -1);
   const int q0 = offset_at(p.q_off, p.off64, s, p.Tq), q1 = offset_at(p.q_off, p.off64, s + 1, p.Tq);
-  if (r >= q1) return make_int4(0, 0, 0, 0);
+  if (r >= q1) return make_int4(0, 0, 0, -1);
   const int k0 = offset_at(p.k_off, p.off64, s, p.Tk), k1 = max(k0, offset_at(p.k_off, p.off64, s + 1, p.Tk));
   const int place = k0 + (r - q0) + (k1 - k0) - (q1 - q0);
   int hi = k1;
@@ -86,7 +88,7 @@ __device__ __forceinline__ int4 row_of(const Params& p, int r) {
     const int seen = p.prefix != nullptr ? (int)min(max(entry(p.prefix, p.off64, s), (int64_t)0), (int64_t)(k1 - k0)) : 0;
     hi = min(k1, max(place + 1, k0 + seen));
   }
-  return hi > k0 ? make_int4(k0, hi, place, 0) : make_int4(0, 0, place, 0);
+  return hi > k0 ? make_int4(k0, hi, place, s) : make_int4(0, 0, place, s);
 }
 
 template <typename T>
@@ -252,13 +254,27 @@ __device__ __forceinline__ float lse_of(const Params& p, int r, int h) {
   return l == -INFINITY ? INFINITY : kLog2e * l;
 }
 
+// (fp16) the power of two that keeps |dP - delta| of a segment's rows times it under 1
+__device__ __forceinline__ float range_of(const Params& p, int segment, int hk) {
+  if (segment < 0) return 1.0f;
+  const uint32_t* peak = p.peaks + ((int64_t)segment * p.Hk + hk) * 2;
+  const float bound = 2.0f * sqrtf(__uint_as_float(peak[0])) * sqrtf(__uint_as_float(peak[1]));  // of |dP - delta|
+  const int e = (int)(__float_as_uint(bound) >> 23) - 126;                                       // bound < 2^e
+  return bound > 0.0f && bound < INFINITY ? __uint_as_float((uint32_t)min(max(127 - e, 1), 254) << 23) : 1.0f;
+}
+
+// delta of a row, which the tiles of fp16 queries leave times its range
+template <typename T>
+__device__ __forceinline__ float delta_unit(const Params& p, int r, int h) {
+  return std::is_same<T, __half>::value && p.key_tiles != nullptr ? range_of(p, p.rows[r].w, h / p.G) : 1.0f;
+}
 // (delta and what it is off by: at backward_kernel)
 template <typename T>
 __device__ __noinline__ void row_dq(const Params& p, int r, int h) {
   const int lane = threadIdx.x & 31, hk = h / p.G;
   const int4 row = p.rows[r];
   const float slope = p.slopes != nullptr ? __ldg(p.slopes + h) : 0.0f;
-  const float lse = lse_of(p, r, h), delta = p.delta[(int64_t)h * p.Tq + r];
+  const float lse = lse_of(p, r, h), range = delta_unit<T>(p, r, h), delta = p.delta[(int64_t)h * p.Tq + r] / range;
   float q[kPerLane], g[kPerLane], dq[kPerLane], mean[kPerLane], k[kPerLane], v[kPerLane], slant, off = 0.0f;
   load_row<T>(p.q, r * p.q_t + h * p.q_h, p.D, lane, q);
   load_row<T>(p.g, r * p.g_t + h * p.g_h, p.D, lane, g);
@@ -279,14 +295,19 @@ __device__ __noinline__ void row_dq(const Params& p, int r, int h) {
   }
 #pragma unroll
   for (int c = 0; c < kPerLane; ++c) dq[c] = fmaf(-off, mean[c], dq[c]);
-  if (lane == 0) p.delta[(int64_t)h * p.Tq + r] = delta + off;
+  if (lane == 0) p.delta[(int64_t)h * p.Tq + r] = (delta + off) * range;
   store_row<T>(p.dq, ((int64_t)r * p.H + h) * p.D, p.D, lane, dq, p.scale);
 }
 
+// the segment that a row is in, or -1
+__device__ __forceinline__ int segment_with(const Params& p, const void* off, int total, int r) {
+  const int s = segment_of(off, p.off64, p.S, total, r);
+  return s >= 0 && r < offset_at(off, p.off64, s + 1, total) ? s : -1;
+}
 // the queries of the segment that key j belongs to: [x, y)
 __device__ __forceinline__ int2 queries_of(const Params& p, int j) {
-  const int s = segment_of(p.k_off, p.off64, p.S, p.Tk, j);
-  if (s < 0 || j >= offset_at(p.k_off, p.off64, s + 1, p.Tk)) return make_int2(0, 0);
+  const int s = segment_with(p, p.k_off, p.Tk, j);
+  if (s < 0) return make_int2(0, 0);
   return make_int2(offset_at(p.q_off, p.off64, s, p.Tq), offset_at(p.q_off, p.off64, s + 1, p.Tq));
 }
 
@@ -310,7 +331,7 @@ __device__ __noinline__ void row_dkv(const Params& p, int j, int hk) {
       load_row<T>(p.g, r * p.g_t + h * p.g_h, p.D, lane, g);
       const float s = score_of(p, dot_row(q, k), row.z, j, slope, slant);
       const float w = exp2_fast(s - lse_of(p, r, h));
-      const float e = w * (dot_row(g, v) - p.delta[(int64_t)h * p.Tq + r]) * slant;
+      const float e = w * (dot_row(g, v) - p.delta[(int64_t)h * p.Tq + r] / delta_unit<T>(p, r, h)) * slant;
 #pragma unroll
       for (int c = 0; c < kPerLane; ++c) {
         dk[c] = fmaf(e, q[c], dk[c]);
@@ -337,9 +358,9 @@ __global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ Params
 }
 
 // What the gradients need: each query's interval and the lists of tiles (the first CTAs), delta_i = dout_i . out_i, and in
-// fp16 the largest norms of a row of dout and of v (those that are finite), as bits of positive floats, which order as
-// numbers do.  LANES lanes take a row of one head by 16 bytes each (32, value by value, where rows do not allow that).
-constexpr int kDeltaCtas = 8;  // an SM, at most: every CTA ends with an atomic maximum to the same two words
+// fp16, for each segment and key head, the largest squared norms of a row of dout and of v (those that are finite), as bits
+// of positive floats, which order as numbers do.  LANES lanes take a row of one head by 16 bytes each (32, value by value, where rows do not allow that).
+constexpr int kDeltaCtas = 6;  // an SM, at most (fp16, 60 users of 10 to 1000 items: 35.4 us, with 8 and fewer registers 37.7)
 template <typename T>
 __device__ __forceinline__ float2 widen2(uint32_t w) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(bf16_lo(w), bf16_hi(w));
@@ -394,14 +415,19 @@ __device__ __forceinline__ void list_keys(const Params& p, int b) {
 }
 
 template <typename T, int LANES, bool VEC>
-__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(256, kDeltaCtas) delta_kernel(const __grid_constant__ Params p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr bool kPeaks = std::is_same<T, __half>::value;
-  __shared__ uint32_t s_peak[2];
-  const int list_ctas = (p.Tq + 255) / 256, row_ctas = list_ctas + (p.n_tiles + p.n_key_tiles + 7) / 8;
-  if ((int)blockIdx.x < list_ctas) {
+  const int query_ctas = (p.Tq + 255) / 256, list_ctas = query_ctas + (kPeaks ? (p.Tk + 255) / 256 : 0);
+  const int row_ctas = list_ctas + (p.n_tiles + p.n_key_tiles + 7) / 8;
+  if ((int)blockIdx.x < query_ctas) {
     const int r = blockIdx.x * 256 + threadIdx.x;
     if (r < p.Tq) p.rows[r] = row_of(p, r);
+    return;
+  }
+  if (kPeaks && (int)blockIdx.x < list_ctas) {
+    const int j = (blockIdx.x - query_ctas) * 256 + threadIdx.x;
+    if (j < p.Tk) p.key_segments[j] = segment_with(p, p.k_off, p.Tk, j);
     return;
   }
   if ((int)blockIdx.x < row_ctas) {
@@ -410,17 +436,53 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Para
     else if (b < p.n_tiles + p.n_key_tiles) list_keys(p, b - p.n_tiles);
     return;
   }
-  if (kPeaks && threadIdx.x < 2) s_peak[threadIdx.x] = 0;
-  __syncthreads();
-  float peak[2] = {0.0f, 0.0f};  // squares
+  // (fp16) the largest square of the rows of one segment and key head that this thread meets one behind the other
+  uint32_t* peak = nullptr;
+  float high = 0.0f;
+  // of the last row, and the first row behind it: at first those of the CTA's first row, found by a warp with 32 probes
+  int segment = -1, until = 0;
+  __shared__ int2 s_first[2];
+  const int64_t ctas = gridDim.x - row_ctas, cta = blockIdx.x - row_ctas;
+  if (kPeaks) {
+    if (threadIdx.x < 64) {
+      const void* off = threadIdx.x < 32 ? p.q_off : p.k_off;
+      const int total = threadIdx.x < 32 ? p.Tq : p.Tk, r = (int)(total * cta / ctas);
+      int a = 0, b = p.S;  // segments [0, a) start at or before r, [b, S) behind it
+      while (a < b) {
+        const int step = (b - a + 31) / 32, m = a + (int)(threadIdx.x % 32) * step;
+        const int n = __popc(__ballot_sync(kAll, m < b && offset_at(off, p.off64, m, total) <= r));
+        b = min(b, a + n * step);
+        if (n > 0) a += (n - 1) * step + 1;
+      }
+      const int end = a > 0 ? offset_at(off, p.off64, a, total) : 0;
+      if (threadIdx.x % 32 == 0) s_first[threadIdx.x / 32] = end > r ? make_int2(a - 1, end) : make_int2(-1, r);
+    }
+    __syncthreads();
+    segment = s_first[0].x;
+    until = s_first[0].y;
+  }
+  auto raise = [&](uint32_t* next) {
+    if (peak != nullptr) atomicMax(peak, __float_as_uint(high));
+    peak = next;
+    high = 0.0f;
+  };
+  auto meet = [&](const void* off, int total, int r, int hk, int which, float square) {
+    if (r >= until) {
+      segment = segment_with(p, off, total, r);
+      until = segment < 0 ? r + 1 : offset_at(off, p.off64, segment + 1, total);
+    }
+    uint32_t* mine = segment < 0 ? nullptr : p.peaks + ((int64_t)segment * p.Hk + hk) * 2 + which;
+    if (mine != peak) raise(mine);
+    if (square < INFINITY) high = fmaxf(high, square);
+  };
   constexpr int kRows = 256 / LANES, kTwo = 2;  // rows of a CTA at a time, twice
   const int lane = threadIdx.x % LANES, c = lane * 8;
-  // rows (token, head) [0, tokens * heads), the CTAs in turn; from one to this thread's next without a quotient
-  auto scan = [&](int tokens, int heads, auto source, auto use) {
-    const int64_t step = (int64_t)(gridDim.x - row_ctas) * kRows, first = (int64_t)(blockIdx.x - row_ctas) * kRows + threadIdx.x / LANES;
-    const int d_token = (int)(step / heads), d_head = (int)(step - (int64_t)d_token * heads);
-    int64_t token = first / heads;
-    int head = (int)(first - token * heads);
+  // rows (token, head) [0, tokens * heads), a run of tokens a CTA; from one to this thread's next without a quotient
+  auto scan = [&](int all_tokens, int heads, auto source, auto use) {
+    const int d_token = kRows / heads, d_head = kRows % heads, first = threadIdx.x / LANES;
+    const int64_t tokens = all_tokens * (cta + 1) / ctas;
+    int64_t token = all_tokens * cta / ctas + first / heads;
+    int head = first % heads;
     while (__any_sync(kAll, token < tokens)) {
       int64_t at[kTwo];
       int h[kTwo];
@@ -479,22 +541,15 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Para
        },
        [&](int64_t r, int h, float2 s) {
          p.delta[(int64_t)h * p.Tq + r] = s.x;
-         if (kPeaks && s.y < INFINITY) peak[0] = fmaxf(peak[0], s.y);
+         if (kPeaks) meet(p.q_off, p.Tq, (int)r, h / p.G, 0, s.y);
        });
-  if constexpr (kPeaks)
+  if constexpr (kPeaks) {
+    raise(nullptr);
+    segment = s_first[1].x;
+    until = s_first[1].y;
     scan(p.Tk, p.Hk, [&](int64_t r, int h, const T*&, const T*& y) { y = static_cast<const T*>(p.v) + r * p.v_t + h * p.v_h; },
-         [&](int64_t, int, float2 s) {
-           if (s.y < INFINITY) peak[1] = fmaxf(peak[1], s.y);
-         });
-  if (kPeaks) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t high = __reduce_max_sync(kAll, __float_as_uint(sqrtf(peak[i])));
-      if ((threadIdx.x & 31) == 0) atomicMax(&s_peak[i], high);
-    }
-    __syncthreads();
-    if (threadIdx.x < 2 && s_peak[threadIdx.x] > *reinterpret_cast<volatile uint32_t*>(p.peaks + threadIdx.x))
-      atomicMax(p.peaks + threadIdx.x, s_peak[threadIdx.x]);
+         [&](int64_t r, int h, float2 s) { meet(p.k_off, p.Tk, (int)r, h, 1, s.y); });
+    raise(nullptr);
   }
 }
 
@@ -1470,8 +1525,8 @@ __global__ void __launch_bounds__(256) few_join_kernel(const __grid_constant__ P
 // seven products for both where one kernel that adds dq by atomics has five.  p and e go to the second products as two
 // values of the type each, out of TMEM: what they are rounded to, and what is left, rounded.  (With the first alone dq, dk
 // and dv are 1.3 to 1.4 times as far from the exact sums, 2.4e-3 for 1.7e-3 in bf16.)  In fp16 they are brought into the
-// type's range first: p by 2^15, e by that and the power of two that keeps |dP - delta| under 1 (from the largest norms of
-// a row of dO and of V).
+// type's range first: p by 2^15, e by that and the power of two that keeps |dP - delta| of the row's own segment and key head
+// under 1 (from the largest norms of a row of dO and of V there): what other users hold does not take bits from a row.
 //
 // Bound by the row warps' issue slots (half of them used, the tensor pipe 35 % busy): two causal documents of 4100 to 7001
 // rows, 8 heads over 2 of 128: dk and dv 587 us, dq 427; 60 users of 10 to 1000 items, 8 heads of 64, fp16: 188 and 138.
@@ -1496,13 +1551,6 @@ struct Backward {
   static constexpr int kStride = 16;                      // sixteen of p or e as they are rounded, then what is left of them
   static constexpr int kTmemCols = DP == 64 ? 256 : 512;
 };
-
-// (fp16) the power of two that keeps |dP - delta| times it under 1
-__device__ __forceinline__ float range_of(const Params& p) {
-  const float bound = 2.0f * __uint_as_float(p.peaks[0]) * __uint_as_float(p.peaks[1]);  // of |dP - delta|
-  const int e = (int)(__float_as_uint(bound) >> 23) - 126;                             // bound < 2^e
-  return bound > 0.0f && bound < INFINITY ? __uint_as_float((uint32_t)min(max(127 - e, 1), 254) << 23) : 1.0f;
-}
 
 template <typename T, int DP, bool KEYS, bool WIDE>
 __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEYS>::kCtas)
@@ -1563,7 +1611,8 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
   const int each = other1 > other0 ? (other1 - other0 + kBlock - 1) / kBlock : 0;  // blocks of a head
   const int blocks = KEYS ? each * heads : each;
   const int up = std::is_same<T, __half>::value ? 15 : 0;
-  const float sigma = up != 0 ? range_of(p) : 1.0f;
+  float sigma = 1.0f;  // of the thread's row
+  if (up != 0 && warp >= 2 && r < span.y) sigma = range_of(p, KEYS ? p.key_segments[r] : row.w, KEYS ? head : head / p.G);
 
   if (warp == 0) {
     if (lane == 0 && blocks > 0) {
@@ -1674,7 +1723,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
       const bool there = i < other1;
       next_row = there ? p.rows[i] : make_int4(0, 0, 0, 0);
       next_lse = there ? lse_of(p, i, h) - up : INFINITY;
-      next_delta = there ? sigma * p.delta[(int64_t)h * p.Tq + i] : 0.0f;
+      next_delta = there ? p.delta[(int64_t)h * p.Tq + i] : 0.0f;  // (times the range, which a query and its keys share)
     };
     auto deposit = [&](int n) {
       if (t < kBlock) {
@@ -1836,7 +1885,7 @@ __global__ void __launch_bounds__(Backward<DP, KEYS>::kThreads, Backward<DP, KEY
     if constexpr (!KEYS) {
       for (int i = 0; i < C::kSets; ++i) d += s_off[i][quarter * 32 + lane];
       d *= down;
-      if (ok && set == 0 && there && mine_too) p.delta[(int64_t)head * p.Tq + r] = (delta + d) / sigma;
+      if (ok && set == 0 && there && mine_too) p.delta[(int64_t)head * p.Tq + r] = delta + d;  // (fp16: times the range)
     }
     if (ok) {
       bool bad = false;
@@ -1905,7 +1954,7 @@ __global__ void __launch_bounds__(256) keys_join_kernel(const __grid_constant__ 
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (int64_t)p.Tk * p.Hk;
   if (row >= rows) return;
   constexpr bool kHalfType = std::is_same<T, __half>::value;
-  const float down = kHalfType ? 0x1p-15f : 1.0f, w1 = p.scale * down / (kHalfType ? range_of(p) : 1.0f);
+  const float down = kHalfType ? 0x1p-15f : 1.0f, w1 = p.scale * down / (kHalfType ? range_of(p, p.key_segments[row / p.Hk], (int)(row % p.Hk)) : 1.0f);
   bool finite = true;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
@@ -2107,7 +2156,7 @@ template <typename T>
 static int backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   int rc;
   const bool peaks = std::is_same<T, __half>::value;
-  if (peaks && (rc = check_cuda(cudaMemsetAsync(p.peaks, 0, 8, st), "attention peaks"))) return rc;
+  if (peaks && p.S > 0 && (rc = check_cuda(cudaMemsetAsync(p.peaks, 0, (size_t)p.S * p.Hk * 8, st), "attention peaks"))) return rc;
   const bool tiles = tiled(p) && p.Tq > 0 && p.Tk > 0 && mappable(p.g, p.Tq, p.H, p.g_t, p.g_h) && aligned(p.dq, 16) &&
                      aligned(p.dk, 16) && aligned(p.dv, 16);
   if (tiles) {
@@ -2121,7 +2170,7 @@ static int backward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
   if (heads > 0) {
     const bool vec = p.D % 8 == 0 && aligned(p.o, 16) && mappable(p.g, p.Tq, p.H, p.g_t, p.g_h) && mappable(p.v, p.Tk, p.Hk, p.v_t, p.v_h);
     const int lanes = !vec || p.D > 128 ? 32 : p.D > 64 ? 16 : 8;
-    const unsigned grid = (unsigned)((p.Tq + 255) / 256 + (p.n_tiles + p.n_key_tiles + 7) / 8 + std::min<int64_t>((heads * lanes + 255) / 256, (int64_t)sm_count() * kDeltaCtas));
+    const unsigned grid = (unsigned)((p.Tq + 255) / 256 + (peaks ? (p.Tk + 255) / 256 : 0) + (p.n_tiles + p.n_key_tiles + 7) / 8 + std::min<int64_t>((heads * lanes + 255) / 256, (int64_t)sm_count() * kDeltaCtas));
     if (!vec) delta_kernel<T, 32, false><<<grid, 256, 0, st>>>(p);
     else if (lanes == 32) delta_kernel<T, 32, true><<<grid, 256, 0, st>>>(p);
     else if (lanes == 16) delta_kernel<T, 16, true><<<grid, 256, 0, st>>>(p);
@@ -2231,7 +2280,7 @@ extern "C" int64_t rb_segment_attention_backward_workspace_size(int64_t Tq, int6
   if (Tq < 0 || Tk < 0 || S < 0 || H <= 0 || Hk <= 0 || D <= 0 || Tq > 1 << 30) return -1;
   const int64_t parts = H % Hk == 0 && D % 8 == 0 && D <= 128 && attn::key_parts(Tk, S, H, Hk) ? (int64_t)2 * H * Tk * D * 4 : 0;
   const int64_t lists = (Tq + Tq / attn::kTile + Tk / attn::kTile + 2 * S + 4) * 16;
-  return 16 + lists + ((int64_t)H * Tq * 4 + 15) / 16 * 16 + parts;
+  return (S * Hk * 8 + 15) / 16 * 16 + lists + ((int64_t)H * Tq * 4 + 15) / 16 * 16 + (Tk * 4 + 15) / 16 * 16 + parts;
 }
 
 extern "C" int rb_segment_attention_backward(const void* grad, int64_t g_t, int64_t g_h, const void* q, int64_t q_t, int64_t q_h,
@@ -2267,10 +2316,11 @@ extern "C" int rb_segment_attention_backward(const void* grad, int64_t g_t, int6
   p.dk = dk;
   p.dv = dv;
   p.peaks = static_cast<uint32_t*>(workspace);
-  p.rows = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + 16);
+  p.rows = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + (S * Hk * 8 + 15) / 16 * 16);
   p.tiles = p.rows + Tq;
   p.delta = reinterpret_cast<float*>(p.tiles + (Tq / kTile + Tk / kTile + 2 * S + 4));
-  p.part = p.delta + ((int64_t)H * Tq + 3) / 4 * 4;
+  p.key_segments = reinterpret_cast<int32_t*>(p.delta + ((int64_t)H * Tq + 3) / 4 * 4);
+  p.part = reinterpret_cast<float*>(p.key_segments + (Tk + 3) / 4 * 4);
   p.q_off = q_offsets;
   p.k_off = k_offsets;
   p.prefix = prefix;

@@ -10,7 +10,7 @@ import pytest
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "baidu_cti_grab_b200", "csrc")
 # the workspaces' fields, which kernels of the same call write
 WRITTEN = {
-    "attention.cu": ("rows", "tiles", "key_tiles", "delta", "part", "next", "peaks", "redo"),
+    "attention.cu": ("rows", "tiles", "key_tiles", "delta", "part", "next", "peaks", "redo", "key_segments"),
     "embedding.cu": ("key", "row", "counts", "totals", "heads", "part"),
     "clip.cu": ("sums",),
 }

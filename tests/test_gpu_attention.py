@@ -639,3 +639,34 @@ def test_caps_far_above_the_scores(cuda_device, cap, nq, nk, H, Hk, D):
     _close(lse, val["lse"], bare["lse"] + more, torch.float32)
     for name, got in zip(("dq", "dk", "dv"), grads):
         _close(got, val[name], loose[name], HF)
+
+
+@pytest.mark.parametrize("H,Hk,D", [(2, 2, 64), (4, 2, 128), (6, 1, 32), (2, 1, 20)])
+def test_other_users_take_no_bits_in_fp16(cuda_device, H, Hk, D):
+    """The gradients of one segment in fp16 are the same bits whatever the size of another segment's rows and of the rows
+    behind the last, and as near as their own rounding (e is scaled by the segment's own largest rows)."""
+    from baidu_cti_grab_b200 import device_ops
+
+    nq = [100, 90, 170]
+    q, k, v, g = _inputs(nq, nq, H, Hk, D, HF, D, cuda_device, 40)
+    off = _offsets(nq, torch.int32, cuda_device, 40)
+    g = (g.float() * 2.0 ** -6).to(HF)
+    grads = {}
+    for up in (1.0, 2.0 ** 9):
+        g2, v2 = g.clone(), v.clone()
+        for t in (g2, v2):
+            for rows in (slice(0, 40), slice(140, 230), slice(400, None)):
+                t[rows] = (t[rows].float() * up).to(HF)
+        g2[140:230] = (g2[140:230].float() * up ** 0.5).to(HF)
+        out, lse = device_ops.segment_attention(q, k, v2, off, want_lse=True)
+        grads[up] = device_ops.segment_attention_backward(g2, q, k, v2, out, lse, off)
+    for a, b in zip(*grads.values()):
+        assert torch.equal(a[40:140], b[40:140]) and torch.equal(a[230:400], b[230:400])
+    for first, n in ((40, 100), (230, 170)):
+        mine = slice(first, first + n)
+        val, tol = oracle(q[mine], k[mine], v[mine], [n], [n], g=g[mine], half=2.0 ** -11, fp16=True, near=True)
+        reach, _ = oracle(q[mine], k[mine], k[mine].abs(), [n], [n])
+        near = (g[mine].double().abs() * val["out"].abs()).sum(-1, keepdim=True) * 2.0 ** -11 * (1 + 2.0 ** -6)
+        tol["dq"] += D ** -0.5 * 2.0 ** -11 * near * reach["out"]
+        for name, got in zip(("dq", "dk", "dv"), grads[2.0 ** 9]):
+            _close(got[mine], val[name], tol[name], HF)
