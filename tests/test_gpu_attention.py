@@ -670,3 +670,72 @@ def test_other_users_take_no_bits_in_fp16(cuda_device, H, Hk, D):
         tol["dq"] += D ** -0.5 * 2.0 ** -11 * near * reach["out"]
         for name, got in zip(("dq", "dk", "dv"), grads[2.0 ** 9]):
             _close(got[mine], val[name], tol[name], HF)
+
+
+@pytest.mark.parametrize("nq,H,Hk,D,dtype,mask", [
+    ([300] * 60, 4, 2, 128, BF, {}), ([260, 700, 130, 1, 515] * 12, 4, 4, 96, HF, dict(cap=15.0)),
+    ([2500, 2300], 16, 4, 128, BF, dict(causal=False)), ([400] * 150, 6, 6, 64, HF, {}),
+])
+def test_tiles_behind_one_another(cuda_device, nq, H, Hk, D, dtype, mask):
+    """More tiles of several blocks than the GPU holds CTAs: each takes several of them in turn, the next tile's copies and
+    scores begun before the last one's rows are done."""
+    run(nq, None, H, Hk, D, dtype, cuda_device, seed=D, **mask)
+
+
+@pytest.mark.parametrize("D", [64, 128, 20])
+def test_columns_apart(cuda_device, D):
+    """Heads whose columns lie two elements apart, in any of the operands: the same bits as contiguous ones."""
+    from baidu_cti_grab_b200 import device_ops
+
+    nq = [40, 300, 1, 90]
+    operands = _inputs(nq, nq, 4, 2, D, BF, 22, cuda_device)
+    q, k, v, g = operands
+    off = _offsets(nq, torch.int64, cuda_device)
+    out, lse = device_ops.segment_attention(q, k, v, off, want_lse=True)
+    grads = device_ops.segment_attention_backward(g, q, k, v, out, lse, off)
+    apart = [torch.stack([t, -t], -1)[..., 0] for t in operands]
+    assert all(t.stride(-1) == 2 and torch.equal(t, o) for t, o in zip(apart, operands))
+    for which in ((0,), (1,), (2,), (3,), (0, 1, 2, 3)):
+        a, b, c, d = (apart[i] if i in which else operands[i] for i in range(4))
+        o2, l2 = device_ops.segment_attention(a, b, c, off, want_lse=True)
+        assert torch.equal(o2, out) and torch.equal(l2, lse)
+        for x, y in zip(device_ops.segment_attention_backward(d, a, b, c, o2, l2, off), grads):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("D", [64, 128, 24])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_what_is_not_seen_stays_out_in_fp16(cuda_device, D, bad):
+    """In fp16 too, whose gradients are scaled by the largest finite rows: another segment's NaN and infinities, and those
+    of the rows outside, change no bit of the first and third segment's."""
+    from baidu_cti_grab_b200 import device_ops
+
+    nq = [70, 90, 50]
+    clean = _inputs(nq, nq, 2, 1, D, HF, 11, cuda_device, 9)
+    off = _offsets(nq, torch.int32, cuda_device, 9)
+    half = 2.0 ** -11
+    val, tol = oracle(*clean[:3], nq, nq, 9, 9, clean[3], half=half, fp16=True)
+    q, k, v, g = (t.clone() for t in clean)
+    for t in (q, k, v, g):
+        t[:9] = bad
+        t[79:169] = bad
+        t[219:] = bad
+    out, lse = device_ops.segment_attention(q, k, v, off, want_lse=True)
+    grads = device_ops.segment_attention_backward(g, q, k, v, out, lse, off)
+    mine = torch.cat([torch.arange(9, 79), torch.arange(169, 219)]).to(cuda_device)
+    for name, got in (("out", out), *zip(("dq", "dk", "dv"), grads)):
+        _close(got[mine], val[name][mine], tol[name][mine], HF)
+        assert not got[:9].any() and not got[219:].any()
+    _close(lse[:, mine], val["lse"][:, mine], tol["lse"][:, mine], torch.float32)
+    # a NaN of its own makes a row of the gradients NaN, and the keys that it sees, and nothing else
+    q, k, v, g = (t.clone() for t in clean)
+    g[9 + 40] = bad
+    out, lse = device_ops.segment_attention(q, k, v, off, want_lse=True)
+    dq, dk, dv = device_ops.segment_attention_backward(g, q, k, v, out, lse, off)
+    assert bool((~dq[49].isfinite()).any(-1).all()) and bool((~dv[9:50].isfinite()).any(-1).all())
+    rest = torch.tensor([i for i in range(9, 79) if i != 49] + list(range(79, 219)), device=cuda_device)
+    _close(dq[rest], val["dq"][rest], tol["dq"][rest], HF)
+    for name, got in (("dk", dk), ("dv", dv)):
+        _close(got[50:], val[name][50:], tol[name][50:], HF)
+    torch.cuda.synchronize()
+    assert device_ops.device_error() == 0

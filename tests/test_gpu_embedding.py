@@ -267,3 +267,53 @@ def test_module_gradients(cuda_device):
     _close(m.weight.grad, want, bound)
     with torch.no_grad():
         assert not m(ids).requires_grad
+
+
+@pytest.mark.parametrize("out_dtype", [BF, HF])
+@pytest.mark.parametrize("dtype,D", [(F32, 100), (BF, 512), (HF, 46), (BF, 7)])
+def test_results_of_another_type(cuda_device, dtype, D, out_dtype):
+    """Sums added to a bf16 or fp16 tensor (rounded once, from fp32), and touched rows in another type than grad's."""
+    from baidu_cti_grab_b200 import device_ops
+
+    n, V = 3000, 700
+    gen = torch.Generator(device=cuda_device).manual_seed(D)
+    grad = torch.randn(n, D, device=cuda_device, generator=gen).to(dtype)
+    ids = _ids(n, V, D).to(cuda_device)
+    want, bound, touched = _oracle(grad, ids, V)
+    base = torch.randn(V, D, device=cuda_device, generator=gen).to(out_dtype)
+    total = base.clone()
+    device_ops.embed_rows_backward(grad, ids, V, out=total)
+    exact = want + base.double()
+    _close(total, exact, bound + U * exact.abs())
+    assert torch.equal(total[~touched], base[~touched])
+    out = torch.full((n,), -7, dtype=torch.int64, device=cuda_device), torch.full((n, D), 9.0, dtype=out_dtype, device=cuda_device)
+    where, rows, count = device_ops.embed_rows_backward_sparse(grad, ids, V, out=out)
+    m = int(count)
+    assert where is out[0] and rows is out[1] and torch.equal(where[:m], touched.nonzero()[:, 0])
+    _close(rows[:m], want[where[:m]], bound[where[:m]])
+    assert bool((where[m:] == -7).all()) and bool((rows[m:] == 9.0).all())
+
+
+@pytest.mark.parametrize("n", [3000, 50_000])
+def test_tables_above_2_to_the_24_rows(cuda_device, n):
+    """Four passes of the sort: ids that differ in their highest byte alone, and the last rows of the table."""
+    from baidu_cti_grab_b200 import device_ops
+
+    V, D = (1 << 24) + 70_000, 8
+    gen = torch.Generator().manual_seed(n)
+    ids = torch.randint(0, V, (n,), generator=gen)
+    ids[::5] = torch.randint(0, 4, (len(ids[::5]),), generator=gen)
+    ids[1::5] = (1 << 24) + torch.randint(0, 4, (len(ids[1::5]),), generator=gen)
+    ids[2] = V - 1
+    ids = ids.to(cuda_device)
+    grad = torch.randn(n, D, generator=gen).to(cuda_device)
+    distinct, place = torch.unique(ids, return_inverse=True)
+    want, bound, _ = _oracle(grad, place, len(distinct))
+    where, rows, count = device_ops.embed_rows_backward_sparse(grad, ids, V)
+    m = int(count)
+    assert torch.equal(where[:m], distinct)
+    _close(rows[:m], want, bound)
+    dense = device_ops.embed_rows_backward(grad, ids, V)
+    assert torch.equal(dense[distinct], rows[:m])
+    dense[distinct] = 0.0
+    assert not dense.any()
