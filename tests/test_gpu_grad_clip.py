@@ -187,3 +187,17 @@ def test_clipped_tensors_count_as_modified(cuda_device):
     rows, count = torch.ones(6, 4, device=cuda_device), torch.tensor([3], dtype=torch.int32, device=cuda_device)
     device_ops.clip_grads([(rows, count)], 1.0)
     assert rows._version == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("at", [0, 777, 9000])
+def test_zeros_and_what_hides_among_them(cuda_device, dtype, at):
+    """Zeros alone are a norm of 0; one value among them is the norm, however small its square, and a NaN is NaN."""
+    from baidu_cti_grab_b200 import device_ops
+
+    x = torch.zeros(10_001, dtype=dtype, device=cuda_device)
+    assert float(device_ops.grad_norm([x])) == 0.0
+    for value in (1e-38, 3e-23, 2.0, -5e30, math.nan):
+        x[at] = value
+        got, want = float(device_ops.grad_norm([x])), abs(float(x[at]))
+        assert (math.isnan(got) and math.isnan(want)) or abs(got - want) <= 2.0 ** -22 * want
