@@ -543,7 +543,6 @@ __global__ void __launch_bounds__(1024) heads_scan_kernel(const __grid_constant_
 }
 
 constexpr int kSumThreads = 256, kAhead = 4;  // rows of grad that a thread has in flight
-constexpr int kMaxRun = 256;
 
 // A team of p.team threads takes a run of sorted ids: ids and rows go to shared memory at once, so that the loop waits for
 // rows of grad alone, and those are asked for kAhead ahead.
