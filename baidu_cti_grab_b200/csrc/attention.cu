@@ -808,8 +808,9 @@ __device__ __forceinline__ void transform(const Params& p, uint32_t* raw, float 
 // what it is scaled to.  A weight goes into the second product as two values of the type (with the first alone `out` was
 // 1.4 times as far from the exact sums as its own rounding makes it).  Rows whose sums are not finite are noted and taken again at the CTA's end.
 //
-// Bound by the row warps' issue slots: 1024 users of 1 to 200 items in 8 heads of 64 take 115 us (their bytes 65);
-// two causal documents of 4100 to 7001 rows, 8 heads of 128, capped scores, 427 us.
+// Bound by the row warps' issue slots (45 to 52 % used): 1024 users of 1 to 200 items in 8 heads of 64 take 132 us (their
+// bytes 65; with weights of one value 117); two causal documents of 4100 to 7001 rows, 8 heads of 128, capped scores, 446 us
+// (412).
 template <int DP>
 struct Forward {
   static constexpr int kChunks = DP / 64;              // 64 columns, a swizzled row
@@ -1224,7 +1225,7 @@ __global__ void __launch_bounds__(Forward<DP>::kThreads, Forward<DP>::kCtas)
 // the segment's keys, so that a single query still fills the GPU; a producer warp keeps kStages blocks of 64 keys
 // coming, and each of four warps takes 16 keys of a block with products of 16 x 8 x 16 (most of the 128 rows of the
 // larger tensor-core products would be empty here).  Warps, then parts, are added up in their order.  64 queries of 16 heads
-// (4 key heads of 128) over 1000 to 16000 keys each: 205 us, 0.9 of the copy rate.
+// (4 key heads of 128) over 1000 to 16000 keys each: 204 us, 0.9 of the copy rate.
 template <int DP>
 struct Few {
   static constexpr int kRows = 16, kWarps = 4, kThreads = 32 * (kWarps + 1);
@@ -1522,14 +1523,16 @@ __global__ void __launch_bounds__(256) few_join_kernel(const __grid_constant__ P
 // dq_i = acc_i - d_i sum_j p_ij (1 - tanh^2)_ij k_j, whose last sum is its second accumulator (of p rounded once: d is
 // small).  delta_i + d_i is what the keys' kernel gets.
 //
-// seven products for both where one kernel that adds dq by atomics has five.  p and e go to the second products as two
+// seven products for both where one kernel that adds dq by atomics has five, the queries' second sum apart.  p and e go to the second products as two
 // values of the type each, out of TMEM: what they are rounded to, and what is left, rounded.  (With the first alone dq, dk
 // and dv are 1.3 to 1.4 times as far from the exact sums, 2.4e-3 for 1.7e-3 in bf16.)  In fp16 they are brought into the
 // type's range first: p by 2^15, e by that and the power of two that keeps |dP - delta| of the row's own segment and key head
 // under 1 (from the largest norms of a row of dO and of V there): what other users hold does not take bits from a row.
 //
-// Bound by the row warps' issue slots (half of them used, the tensor pipe 35 % busy): two causal documents of 4100 to 7001
-// rows, 8 heads over 2 of 128: dk and dv 587 us, dq 427; 60 users of 10 to 1000 items, 8 heads of 64, fp16: 188 and 138.
+// Bound by the row warps' issue slots (44 to 55 % used, the tensor pipe 36 to 39 % busy at 128 columns): two causal documents
+// of 4100 to 7001 rows, 8 heads over 2 of 128: dk and dv 604 us, dq 486; 60 users of 10 to 1000 items, 8 heads of 64, fp16:
+// 209 and 182, the latter (38 % of the slots) waiting for products, since its second accumulator leaves S and dP no columns
+// beside p and e (138 with one accumulator and p and e apart).
 template <int DP, bool KEYS>
 struct Backward {
   static constexpr int kChunks = DP / 64;
@@ -2019,8 +2022,9 @@ static int launch(K kernel, dim3 grid, int threads, int smem, bool after, cudaSt
 // Tiles by the packed order or by segment: which takes less time, were all segments alike.  By segment, every segment has
 // its own (partly empty) tiles; by the packed order a tile's rows see keys of several segments.  A tile costs about two
 // blocks besides its own, fewer tiles than the GPU holds at once take as long as those, and the last are half alone.  Eight heads of 64, us packed |
-// by segment: 2048 users of 40: 81 | 105 (gradients 396 | 788), 700 of 128: 71 | 77, 512 of mean 200, uneven: 140 | 134,
-// 128 of mean 700, uneven: 248 | 243, 512 single queries over 16 keys each: 64 | 30, 512 times 30 over 256: 116 | 77.
+// by segment: 2048 users of 40: 88 | 111 (gradients 419 | 784), 700 of 128: 76 | 82 (393 | 517), 512 of mean 200, uneven:
+// 158 | 151 (723 | 770), 128 of mean 700, uneven: 290 | 285, 512 single queries over 16 keys each: 73 | 32, 512 times 30 over
+// 256: 132 | 85.
 static bool choose_by_segment(int64_t Tq, int64_t Tk, int64_t S, int heads) {
   if (S <= 0) return false;
   const double nq = (double)Tq / S, nk = (double)Tk / S, wave = 4.0 * sm_count();
@@ -2053,11 +2057,12 @@ static int run_forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
 // How many parts the keys of a segment are split into where there are few queries, 0: not that kernel.  It reads a key
 // head's keys for 16 rows, each query's heads among them; the tiles read them for 128 rows of one head, most of them empty.
 // So 16 rows cost 0.7 of a tile and half a tile for each segment, while fewer tiles than five an SM take as long as those
-// (64 segments of 4000 keys, tiles | this, us: 1 query of 8 heads over 8, 244 | 126; over 1, 240 | 38; 16 over 1, 239 |
-// 110; 64 over 8, 234 | 332; 512 segments of 1000 keys: 1 over 8, 225 | 250, 8 over 1, 225 | 101).
+// (64 segments of 4000 keys, tiles | this, us: 1 query of 8 heads over 8, 282 | 122; over 1, 278 | 28; 16 over 1, 281 |
+// 110; 64 over 8, 277 | 309; 512 segments of 1000 keys: 1 over 8, 260 | 256, 8 over 1, 265 | 114).
 // Parts fill the GPU once (of 256 keys or more); where it holds fewer than three of each, segments of different lengths
-// are evened out by up to eight CTAs an SM, of 1024 keys or more (64 histories of 1000 to 16000 keys, 16 heads over 4: one
-// wave 236, eight CTAs an SM 208, sixteen 208; 64 times 4 queries over 4000 keys, 8 heads over 2: 66, 68 and 105).
+// are evened out by up to eight CTAs an SM, of 1024 keys or more (64 histories of 1000 to 16000 keys, 16 heads over 4: whole
+// 283, in two 240, in five, which are eight CTAs an SM, 204, in nine 199; 64 times 4 queries over 4000 keys, 8 heads over 2:
+// whole 69, in three, which fill the GPU once, 55, in eight 54).
 static int splits_of(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D) {
   const int64_t G = H / Hk, sm = sm_count(), used = std::min(S, Tq);  // segments with queries, at most
   if (used <= 0 || D % 8 != 0 || D > 128 || Tk < 4 * Tq || Tq * G > 1 << 30) return 0;
@@ -2117,8 +2122,8 @@ static int forward(Params& p, CUtensorMapDataType dt, cudaStream_t st) {
 
 // Whether the query heads that share a key head go to CTAs of their own, whose sums are added up after (each part is
 // written and read once, in 32 bits): with few tiles of keys an SM the longest take too long by themselves.  Eight heads
-// over two, both gradients, together | apart, us: 1 document of 6100 keys (0.6 tiles an SM) 703 | 479; 2 of them 855 | 832,
-// in heads of 64 values 1061 | 729; 8 of 3000 (2.5 tiles) 863 | 904; 64 users of 150 (1.0) 80 | 95; 16 of 300 (0.5) 72 | 70.
+// over two, both gradients, together | apart, us: 1 document of 6100 keys (0.6 tiles an SM) 744 | 511; 2 of them 913 | 891,
+// in heads of 64 values 1306 | 906; 8 of 3000 (2.5 tiles) 921 | 966; 64 users of 150 (1.0) 120 | 183; 16 of 300 (0.5) 76 | 95.
 static bool key_parts(int64_t Tk, int64_t S, int H, int Hk) {
   if (H <= Hk || H / Hk > 64 || Tk < kTile) return false;
   const int64_t tiles = Tk / kTile * Hk, sm = sm_count();

@@ -10,9 +10,10 @@
 //   sums_kernel     a team of threads takes a run of sorted ids, sums in fp32 and writes every row whose ids lie in its
 //                   run; what goes on in the next run, or came from the one before, goes to a partial sum
 //   combine_kernel  adds the partial sums of a row that crosses runs, in their order
-// so a row that a tenth of all ids ask for costs no more than its bytes.
+// The partial sums of one row are added up by one CTA: a row that many ids ask for waits for it (150,000 ids of 512 bf16
+// values: 84 us over 50,000 rows, 440 over two, 650 over one).
 //
-// 103,725 ids of 50,000 rows of 512 bf16 values: lookup 30 us, gradient 83 (the sort about half).  1.45 million ids in bags
+// 103,725 ids of 50,000 rows of 512 bf16 values: lookup 30 us, gradient 80 (the sort about a third).  1.45 million ids in bags
 // over 2.8 million rows of 512, the touched rows: 483 us, 366 of them sums that wait for rows of grad in the ids' order
 // (each row of grad and of the result once: 252 us at the copy rate).
 #include "common.cuh"

@@ -437,9 +437,11 @@ int rb_low_rank_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int 
  * inputs, output and lse, and writes dq [Tq, H, D], dk and dv [Tk, Hk, D] contiguous
  * (sums over the heads that share a key head), in a fixed order: the same bits every time.
  * Scores, softmax and sums are fp32; on the tensor cores (D <= 128 a multiple of 8, 16-byte
- * rows) weights enter the second products as values of the model type, the scores'
- * gradients as the sum of two of them.  What a row does not see does not reach it,
- * infinities and NaN included.
+ * rows) weights and the scores' gradients enter the second products as the sum of two
+ * values of the model type, in fp16 scaled by the largest rows of grad and v of their own
+ * segment and key head (what is 2^-40 of these is lost).  What a row does not see does not
+ * reach it, infinities and NaN included; a row that is not finite, or lies in a tile that
+ * such values meet, is taken again by itself and costs many times the others.
  */
 int64_t rb_segment_attention_workspace_size(int64_t Tq, int64_t Tk, int64_t S, int H, int Hk, int D);
 int rb_segment_attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h,
